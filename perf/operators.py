@@ -26,33 +26,33 @@ DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 def listed():
     return [
         # one short window of the small model: what a first training step or a test runs; launches and latency
-        {"name": "head, one window", "op": "head", "rows": 32, "time": 32, "d": 256, "vocab": 8192, "packed": True,
+        {"name": "head one window", "op": "head", "rows": 32, "time": 32, "d": 256, "vocab": 8192, "packed": True,
          "dtype": "f16", "ignored": 0.0},
         # the training batch of the default model: 8 contexts
-        {"name": "head, default batch", "op": "head", "rows": 16384, "time": 2048, "d": 512, "vocab": 8192, "packed": True,
+        {"name": "head default batch", "op": "head", "rows": 16384, "time": 2048, "d": 512, "vocab": 8192, "packed": True,
          "dtype": "f16", "ignored": 0.0},
         # conversations cut to an odd length, the user's half of the tokens unsupervised, a vocabulary of no round size
-        {"name": "head, ragged chat", "op": "head", "rows": 7655, "time": 1531, "d": 256, "vocab": 10007, "packed": True,
+        {"name": "head ragged chat", "op": "head", "rows": 7655, "time": 1531, "d": 256, "vocab": 10007, "packed": True,
          "dtype": "bf16", "ignored": 0.5},
         # a dense 16-bit head over a large vocabulary: the largest call
-        {"name": "head, large vocabulary", "op": "head", "rows": 4096, "time": 2048, "d": 512, "vocab": 131072, "packed": False,
+        {"name": "head large vocabulary", "op": "head", "rows": 4096, "time": 2048, "d": 512, "vocab": 131072, "packed": False,
          "dtype": "bf16", "ignored": 0.0},
         # LayerNorm of one window, forward with the tape and backward from it
-        {"name": "norm, one window", "op": "norm", "rows": 512, "channels": 256, "dtype": "f32"},
+        {"name": "norm one window", "op": "norm", "rows": 512, "channels": 256, "dtype": "f32"},
         # the residual stream of the default model's training batch
-        {"name": "norm, default batch", "op": "norm", "rows": 16384, "channels": 512, "dtype": "f32"},
+        {"name": "norm default batch", "op": "norm", "rows": 16384, "channels": 512, "dtype": "f32"},
         # the headline workload's 64 contexts in 16 bits
-        {"name": "norm, 64 contexts", "op": "norm", "rows": 131072, "channels": 512, "dtype": "bf16"},
+        {"name": "norm 64 contexts", "op": "norm", "rows": 131072, "channels": 512, "dtype": "bf16"},
         # weight gradient of the feed-forward key for one context
-        {"name": "weight gradient, one context", "op": "weight", "rows": 2048, "in": 512, "out": 2048, "dtype": "f16"},
+        {"name": "weight gradient one context", "op": "weight", "rows": 2048, "in": 512, "out": 2048, "dtype": "f16"},
         # ... for the default batch
-        {"name": "weight gradient, batch", "op": "weight", "rows": 16384, "in": 512, "out": 2048, "dtype": "bf16"},
+        {"name": "weight gradient batch", "op": "weight", "rows": 16384, "in": 512, "out": 2048, "dtype": "bf16"},
         # weight gradient of the feed-forward value, ragged contexts
-        {"name": "weight gradient, ragged", "op": "weight", "rows": 7655, "in": 2048, "out": 512, "dtype": "f16"},
+        {"name": "weight gradient ragged", "op": "weight", "rows": 7655, "in": 2048, "out": 512, "dtype": "f16"},
         # activations to 8 bits and back: the default batch
-        {"name": "tape, default batch", "op": "tape", "rows": 16384, "channels": 512, "dtype": "f32"},
+        {"name": "tape default batch", "op": "tape", "rows": 16384, "channels": 512, "dtype": "f32"},
         # ... and a width that ends inside a block
-        {"name": "tape, ragged", "op": "tape", "rows": 7655, "channels": 1000, "dtype": "bf16"},
+        {"name": "tape ragged", "op": "tape", "rows": 7655, "channels": 1000, "dtype": "bf16"},
     ]
 
 
