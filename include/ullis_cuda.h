@@ -82,6 +82,9 @@ enum {
     ULLIS_CUDA_TAP_HIDDEN = 8      /* f32 ln_out output (layer argument ignored) */
 };
 
+/* Element types of device arrays. */
+enum { ULLIS_CUDA_F32 = 0, ULLIS_CUDA_F16 = 1, ULLIS_CUDA_BF16 = 2 };
+
 /* ---------------------------------------------------------------- lifecycle
  * Replaces MetalRuntime::new (src/metal.rs:466) and the `--backend` runtime
  * construction in train() (src/main.rs:650-678). */
@@ -407,6 +410,62 @@ ULLIS_CUDA_API int32_t ullis_cuda_streamed_ce(ullis_cuda_runtime* rt, const floa
 ULLIS_CUDA_API int32_t ullis_cuda_rosa_sam_static(int32_t device, void* cuda_stream, const uint32_t* q_sw,
                                                   const uint32_t* k_sw, const uint32_t* v_sw, uint32_t* idx_sw,
                                                   size_t streams, size_t time);
+
+/* ------------------------------------------------------- operators on device memory
+ * For callers whose activations are on the runtime's device.  None of these has a
+ * counterpart of its own in the reference; the layers they serve are cited.
+ *  - Every array is a DEVICE pointer, aligned to its elements; none may overlap an
+ *    output.  Matrices are row-major; a stride is the distance of two rows in
+ *    elements, and arrays without one have no gaps.  Any alignment, stride and size
+ *    is taken; rows that start on 16 bytes with a multiple of 8 columns go faster.
+ *  - Kernels are enqueued on `cuda_stream` (a cudaStream_t, NULL = default stream)
+ *    and the call returns without waiting, so it may be captured into a graph.  It
+ *    allocates nothing: a workspace of at least the bytes that the function with
+ *    `_workspace` in its name gives for the same sizes, aligned to 256 bytes, is the
+ *    caller's and free again when the stream has passed the call (two graphs that
+ *    may run at once need one each).  The current device is left as it was.
+ *  - A refused call (ULLIS_CUDA_ERR_ARG, ULLIS_CUDA_ERR_SHAPE) has enqueued nothing.
+ *    Should a kernel give up waiting, which none does in working order, the next
+ *    call on the runtime or ullis_cuda_runtime_synchronize returns
+ *    ULLIS_CUDA_ERR_TIMEOUT, and the outputs of the call that it belonged to are void.
+ *  - Zero rows are no error: nothing but sums over rows, which are zero, is written.
+ *
+ * The 8-bit tape of x [rows, channels]: blocks of 32 consecutive channels of a row
+ * (the last one may be shorter) have one exponent e, the smallest integer of
+ * -126 .. 121 with 127 * 2^e >= max |x|; codes [rows, channels] are round(x * 2^-e),
+ * ties to even, as two's complement bytes, exponents [rows, ceil(channels / 32)] hold
+ * e + 127.  A code stands for code * 2^e, off by at most half a step of 2^e, that is
+ * max |x| / 127.  (No exponent holds |x| above 127 * 2^121, 3.376e38: codes stay
+ * within +/-127 there.)  A block with a value that is not finite has the exponent byte 255
+ * and stands for NaN throughout. */
+
+/* x (dtype, stride) -> its tape, and what a tape stands for -> x, rounded once. */
+ULLIS_CUDA_API int32_t ullis_cuda_tape_pack(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const void* x,
+                                            size_t x_stride, size_t rows, size_t channels, uint8_t* codes,
+                                            uint8_t* exponents);
+ULLIS_CUDA_API int32_t ullis_cuda_tape_unpack(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype,
+                                              const uint8_t* codes, const uint8_t* exponents, size_t rows,
+                                              size_t channels, void* x, size_t x_stride);
+
+/* LayerNorm (src/model.rs:259-276, eps 1e-5) that leaves its input on the tape:
+ * y [rows, channels] (dtype) = LayerNorm(x), weight and bias FP16 [channels], sums
+ * in f32.  At most 8192 channels. */
+ULLIS_CUDA_API int32_t ullis_cuda_tape_layer_norm(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const void* x,
+                                                  size_t x_stride, const uint16_t* weight, const uint16_t* bias,
+                                                  size_t rows, size_t channels, void* y, uint8_t* codes,
+                                                  uint8_t* exponents);
+/* Its backward pass (src/model.rs:270-315) at what the tape stands for: gx [rows,
+ * channels] = residual + d/dx (residual: the gradient that comes past the norm,
+ * dtype, nullable), g_weight and g_bias [channels] f32.  The sums over rows have a
+ * fixed order.  gx may be residual (the same pointer, residual_stride = channels). */
+ULLIS_CUDA_API int32_t ullis_cuda_tape_layer_norm_backward_workspace(const ullis_cuda_runtime* rt, size_t rows,
+                                                                     size_t channels, size_t* bytes);
+ULLIS_CUDA_API int32_t ullis_cuda_tape_layer_norm_backward(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype,
+                                                           const uint8_t* codes, const uint8_t* exponents, const void* gy,
+                                                           size_t gy_stride, const uint16_t* weight,
+                                                           const void* residual, size_t residual_stride, size_t rows,
+                                                           size_t channels, void* gx, float* g_weight, float* g_bias,
+                                                           void* workspace, size_t workspace_bytes);
 
 /* ------------------------------------------------------------ data parallel
  * Sequences are independent; ranks own disjoint blocks of sequences and only

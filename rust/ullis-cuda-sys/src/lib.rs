@@ -83,6 +83,9 @@ pub const ULLIS_CUDA_TAP_IDX: i32 = 5;
 pub const ULLIS_CUDA_TAP_AFTER_ROSA: i32 = 6;
 pub const ULLIS_CUDA_TAP_BLOCK_OUT: i32 = 7;
 pub const ULLIS_CUDA_TAP_HIDDEN: i32 = 8;
+pub const ULLIS_CUDA_F32: i32 = 0;
+pub const ULLIS_CUDA_F16: i32 = 1;
+pub const ULLIS_CUDA_BF16: i32 = 2;
 pub const ULLIS_CUDA_SAM_STATIC_BYTES: usize = 64 << 20;
 
 unsafe extern "C" {
@@ -431,6 +434,67 @@ unsafe extern "C" {
         idx_sw: *mut u32,
         streams: usize,
         time: usize,
+    ) -> i32;
+    pub fn ullis_cuda_tape_pack(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        dtype: i32,
+        x: *const c_void,
+        x_stride: usize,
+        rows: usize,
+        channels: usize,
+        codes: *mut u8,
+        exponents: *mut u8,
+    ) -> i32;
+    pub fn ullis_cuda_tape_unpack(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        dtype: i32,
+        codes: *const u8,
+        exponents: *const u8,
+        rows: usize,
+        channels: usize,
+        x: *mut c_void,
+        x_stride: usize,
+    ) -> i32;
+    pub fn ullis_cuda_tape_layer_norm(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        dtype: i32,
+        x: *const c_void,
+        x_stride: usize,
+        weight: *const u16,
+        bias: *const u16,
+        rows: usize,
+        channels: usize,
+        y: *mut c_void,
+        codes: *mut u8,
+        exponents: *mut u8,
+    ) -> i32;
+    pub fn ullis_cuda_tape_layer_norm_backward_workspace(
+        rt: *const ullis_cuda_runtime,
+        rows: usize,
+        channels: usize,
+        bytes: *mut usize,
+    ) -> i32;
+    pub fn ullis_cuda_tape_layer_norm_backward(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        dtype: i32,
+        codes: *const u8,
+        exponents: *const u8,
+        gy: *const c_void,
+        gy_stride: usize,
+        weight: *const u16,
+        residual: *const c_void,
+        residual_stride: usize,
+        rows: usize,
+        channels: usize,
+        gx: *mut c_void,
+        g_weight: *mut f32,
+        g_bias: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
     ) -> i32;
     pub fn ullis_cuda_dp_unique_id(id: *mut u8) -> i32;
     pub fn ullis_cuda_dp_rendezvous(

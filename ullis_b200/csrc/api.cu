@@ -366,6 +366,14 @@ void ullis_cuda_runtime::check_status() {
     throw_on_status();
 }
 
+void ullis_cuda_runtime::throw_on_async_status() {
+    volatile uint32_t* words = async_status;
+    const uint32_t code = words[0], site = words[1];
+    if (code == ULLIS_DEV_OK) return;
+    words[0] = ULLIS_DEV_OK;
+    fail(ULLIS_CUDA_ERR_TIMEOUT, "a kernel of an earlier call gave up waiting (site " + std::to_string(site) + ")");
+}
+
 void ullis_cuda_runtime::throw_on_status() {
     const uint32_t code = host_status[0];
     if (code == ULLIS_DEV_OK) return;
@@ -417,6 +425,8 @@ int32_t ullis_cuda_runtime_create(int32_t device, ullis_cuda_runtime** out) {
         ULLIS_CUDA_CHECK(cudaStreamCreateWithFlags(&rt->stream, cudaStreamNonBlocking));
         ULLIS_CUDA_CHECK(cudaMalloc(&rt->dev_status, 16));
         ULLIS_CUDA_CHECK(cudaMallocHost(&rt->host_status, 16));
+        ULLIS_CUDA_CHECK(cudaMallocHost(&rt->async_status, 8));
+        rt->async_status[0] = rt->async_status[1] = 0;
         {   // mapped pinned memory: the kernels store into it, the host reads it without a copy or a wait
             void* hints = nullptr;
             ULLIS_CUDA_CHECK(cudaHostAlloc(&hints, ullis_cuda_runtime::SAM_HINT_SLOTS * sizeof(uint32_t), cudaHostAllocMapped));
@@ -512,6 +522,7 @@ void ullis_cuda_runtime_destroy(ullis_cuda_runtime* rt) {
     if (rt->side_join) cudaEventDestroy(rt->side_join);
     if (rt->dev_status) cudaFree(rt->dev_status);
     if (rt->host_status) cudaFreeHost(rt->host_status);
+    if (rt->async_status) cudaFreeHost(rt->async_status);
     if (rt->sam_hints) cudaFreeHost(rt->sam_hints);
     for (auto& m : rt->marks) {
         cudaEventDestroy(m.done);
@@ -541,7 +552,10 @@ int32_t ullis_cuda_runtime_set_sam(ullis_cuda_runtime* rt, int32_t sam_algo) {
 }
 
 int32_t ullis_cuda_runtime_synchronize(ullis_cuda_runtime* rt) {
-    return guard(rt, [&] { rt->sync(); });
+    return guard(rt, [&] {
+        rt->sync();
+        rt->throw_on_async_status();
+    });
 }
 
 void* ullis_cuda_runtime_stream(ullis_cuda_runtime* rt) { return rt ? (void*)rt->stream : nullptr; }

@@ -138,6 +138,7 @@ struct ullis_cuda_runtime {
     std::string last_error;
     uint32_t* dev_status = nullptr;     // 4 words, device
     uint32_t* host_status = nullptr;    // 4 words, pinned
+    uint32_t* async_status = nullptr;   // 2 words, pinned: written by a kernel of a call on a caller's stream that gives up
     ullis::DeviceBuffer pool[24];       // op-level scratch slots
     // Small inputs of one op-level call, side by side in page-locked memory and copied to the device together.
     static constexpr size_t INPUTS_BYTES = 1 << 20, SMALL_INPUT = 64 << 10;
@@ -213,6 +214,8 @@ struct ullis_cuda_runtime {
     void check_status();
     // Throws when host_status (already copied back and synchronised) holds a kernel's report.
     void throw_on_status();
+    // The same, once, for kernels of calls on a caller's stream; no synchronisation.
+    void throw_on_async_status();
     void launched(const char* what);  // counts a launch and checks the launch error
     // Launches a kernel whose first statement is chain_entry(): it may be set up while the kernel before it on `stream`
     // still runs, 2 to 3 us less between two kernels that follow on each other.
@@ -230,6 +233,10 @@ struct ullis_cuda_runtime {
     }
     template <typename... P>
     void launch(bool chained, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, P... args) {
+        launch_on(stream, chained, kernel, grid, block, smem, args...);
+    }
+    template <typename... P>
+    static void launch_on(cudaStream_t stream, bool chained, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, P... args) {
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -1,0 +1,49 @@
+// Operators on device memory: what the entry points with a `cuda_stream` argument launch, and what the training step launches on
+// its own stream.  Nothing here allocates, synchronises or keeps anything between calls: outputs and workspaces are the caller's.
+#pragma once
+#include "common.hpp"
+
+namespace ullis {
+namespace dev {
+
+enum { F32 = ULLIS_CUDA_F32, F16 = ULLIS_CUDA_F16, BF16 = ULLIS_CUDA_BF16 };
+inline size_t size_of(int dtype) { return dtype == F32 ? 4 : 2; }
+
+struct Stream {   // where a call's kernels go
+    ullis_cuda_runtime* rt;
+    cudaStream_t stream;
+    uint32_t* status;   // two words for a kernel that gives up waiting
+
+    // A kernel whose first statement is chain_entry() (common.hpp), set up while the one before it runs.
+    template <typename... P, typename... A>
+    void chain(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, A... args) const {
+        rt->launch_on(stream, true, kernel, grid, block, smem, P(args)...);
+        launched(what);
+    }
+    void launched(const char* what) const {
+        if (stream == rt->stream) { rt->launched(what); return; }   // (timing marks are events on that stream)
+        ++rt->launches;
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) fail(ULLIS_CUDA_ERR_CUDA, std::string("launch of ") + what + ": " + cudaGetErrorString(e));
+    }
+};
+
+// A matrix of rows of `channels` elements, `stride` elements apart.
+struct Rows {
+    const void* data;
+    size_t stride;
+};
+
+// ---- the 8-bit tape (tape.cuh); codes [rows, channels] and exponents [rows, ceil(channels / 32)] without gaps
+void tape_pack(const Stream& s, int dtype, Rows x, size_t rows, size_t channels, uint8_t* codes, uint8_t* exponents);
+void tape_unpack(const Stream& s, int dtype, const uint8_t* codes, const uint8_t* exponents, size_t rows, size_t channels, void* x,
+                 size_t x_stride);
+constexpr size_t TAPE_NORM_CHANNELS = 8192;   // the widest row that the two kernels below keep in registers
+void tape_layer_norm(const Stream& s, int dtype, Rows x, const uint16_t* weight, const uint16_t* bias, size_t rows, size_t channels,
+                     void* y, uint8_t* codes, uint8_t* exponents);
+size_t tape_layer_norm_backward_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels);
+void tape_layer_norm_backward(const Stream& s, int dtype, const uint8_t* codes, const uint8_t* exponents, Rows gy, const uint16_t* weight,
+                              Rows residual, size_t rows, size_t channels, void* gx, float* g_weight, float* g_bias, void* workspace);
+
+}  // namespace dev
+}  // namespace ullis

@@ -22,10 +22,13 @@ import threading
 
 import numpy as np
 
+from .device import DeviceOps, Tape  # noqa: F401
+from .errors import (ERR_ARG, ERR_CHECKPOINT, ERR_CUDA, ERR_DEVICE_CHECK, ERR_NCCL, ERR_NOMEM, ERR_SHAPE,  # noqa: F401
+                     ERR_TIMEOUT, ERR_TOKEN, OK, UllisCudaError)
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libullis_cuda.so")
 
-OK, ERR_SHAPE, ERR_CHECKPOINT, ERR_CUDA, ERR_DEVICE_CHECK, ERR_NCCL, ERR_TIMEOUT, ERR_ARG, ERR_TOKEN, ERR_NOMEM = range(10)
 MODE_FAST, MODE_EXACT = 0, 1
 SAM_EULER, SAM_EAGER = 0, 1
 CE_NO_IGNORE = 0xFFFFFFFF  # reference src/model.rs:24
@@ -59,14 +62,9 @@ ABI_SYMBOLS = (
     "ullis_cuda_host_free", "ullis_cuda_model_read_loss_global", "ullis_cuda_dp_rendezvous",
     "ullis_cuda_dp_unique_id", "ullis_cuda_dp_init",
     "ullis_cuda_dp_allreduce_loss", "ullis_cuda_dp_finalize",
+    "ullis_cuda_tape_pack", "ullis_cuda_tape_unpack", "ullis_cuda_tape_layer_norm",
+    "ullis_cuda_tape_layer_norm_backward_workspace", "ullis_cuda_tape_layer_norm_backward",
 )
-
-
-class UllisCudaError(RuntimeError):
-    def __init__(self, code: int, message: str):
-        super().__init__(f"[ullis-cuda {code}] {message}")
-        self.code = code
-        self.message = message
 
 
 _LIB = None
@@ -275,8 +273,9 @@ def release_result_memory() -> None:
     _RESULTS.release()
 
 
-class CudaRuntime:
-    """One per device per process, used from one thread (like MetalRuntime)."""
+class CudaRuntime(DeviceOps):
+    """One per device per process, used from one thread (like MetalRuntime).  The methods of `DeviceOps` take torch tensors on
+    the device, all others host arrays."""
 
     def __init__(self, device: int = 0):
         self._lib = load_library()
