@@ -467,6 +467,43 @@ ULLIS_CUDA_API int32_t ullis_cuda_tape_layer_norm_backward(ullis_cuda_runtime* r
                                                            size_t channels, void* gx, float* g_weight, float* g_bias,
                                                            void* workspace, size_t workspace_bytes);
 
+/* Gradient of a linear's weights from the tape of its input (backward_ste's G,
+ * src/model.rs:759-790; Fp16Linear's g_W, src/model.rs:1138-1140): g
+ * [out_features, in_features] f32 = gy^T . x, gy [rows, out_features] F16 or BF16, x
+ * what the tape [rows, in_features] stands for.  Products are exact, sums in f32. */
+ULLIS_CUDA_API int32_t ullis_cuda_tape_weight_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t in_features,
+                                                             size_t out_features, size_t* bytes);
+ULLIS_CUDA_API int32_t ullis_cuda_tape_weight_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype,
+                                                   const uint8_t* codes, const uint8_t* exponents, const void* gy,
+                                                   size_t gy_stride, size_t rows, size_t in_features, size_t out_features,
+                                                   float* g, void* workspace, size_t workspace_bytes);
+
+/* Next-token cross-entropy of a head with its gradient and without logits
+ * (apply_head_ce, src/model.rs:3132-3275; row rule src/model.rs:27-39): row m counts
+ * unless it is the last of its `time` rows or labels[m + 1] == ignore_id.
+ *   z = scale * (hidden . weight^T) + bias, row_loss = log sum exp z - z[target],
+ *   g = loss_scale * (softmax(z) - onehot(target)), 0 on rows that do not count.
+ * hidden [rows, channels] is F16 or BF16 (dtype).  The head is either packed +/-1
+ * (`bits` words in checkpoint order and FP16 `scale` [vocab]; `weight` NULL) or dense
+ * (`weight` [vocab, channels] of hidden's type; `bits` and `scale` NULL); bias FP16
+ * [vocab], nullable.  Outputs: row_loss [rows] f32 (0 where a row does not count),
+ * g_hidden [rows, channels] and g_weight [vocab, channels] (with bits: of the +/-1
+ * weights, that is with the row's scale in it) in hidden's type, g_scale (packed
+ * only) and g_bias [vocab] f32, both nullable.  log sum exp, losses and the sums
+ * behind g_scale and g_bias are f32; g * scale is rounded to hidden's type for the
+ * two gradient products, which accumulate in f32.  What rows hold that do not count
+ * (infinities, NaN) has no effect.  A label outside the vocabulary makes its row's
+ * loss NaN and gives no gradient.  Rows must be a multiple of `time`. */
+ULLIS_CUDA_API int32_t ullis_cuda_head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels,
+                                                         size_t vocab, size_t* bytes);
+ULLIS_CUDA_API int32_t ullis_cuda_head_ce_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype,
+                                               const void* hidden, size_t hidden_stride, const uint32_t* bits,
+                                               const void* weight, const uint16_t* scale, const uint16_t* bias,
+                                               const uint32_t* labels, uint32_t ignore_id, size_t rows, size_t time,
+                                               size_t channels, size_t vocab, float loss_scale, float* row_loss,
+                                               void* g_hidden, void* g_weight, float* g_scale, float* g_bias,
+                                               void* workspace, size_t workspace_bytes);
+
 /* ------------------------------------------------------------ data parallel
  * Sequences are independent; ranks own disjoint blocks of sequences and only
  * {loss_sum, n_valid} is summed across ranks (NCCL all-reduce, 16 bytes).

@@ -496,6 +496,60 @@ unsafe extern "C" {
         workspace: *mut c_void,
         workspace_bytes: usize,
     ) -> i32;
+    pub fn ullis_cuda_tape_weight_grad_workspace(
+        rt: *const ullis_cuda_runtime,
+        rows: usize,
+        in_features: usize,
+        out_features: usize,
+        bytes: *mut usize,
+    ) -> i32;
+    pub fn ullis_cuda_tape_weight_grad(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        dtype: i32,
+        codes: *const u8,
+        exponents: *const u8,
+        gy: *const c_void,
+        gy_stride: usize,
+        rows: usize,
+        in_features: usize,
+        out_features: usize,
+        g: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+    ) -> i32;
+    pub fn ullis_cuda_head_ce_grad_workspace(
+        rt: *const ullis_cuda_runtime,
+        rows: usize,
+        channels: usize,
+        vocab: usize,
+        bytes: *mut usize,
+    ) -> i32;
+    pub fn ullis_cuda_head_ce_grad(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        dtype: i32,
+        hidden: *const c_void,
+        hidden_stride: usize,
+        bits: *const u32,
+        weight: *const c_void,
+        scale: *const u16,
+        bias: *const u16,
+        labels: *const u32,
+        ignore_id: u32,
+        rows: usize,
+        time: usize,
+        channels: usize,
+        vocab: usize,
+        loss_scale: f32,
+        row_loss: *mut f32,
+        g_hidden: *mut c_void,
+        g_weight: *mut c_void,
+        g_scale: *mut f32,
+        g_bias: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+    ) -> i32;
     pub fn ullis_cuda_dp_unique_id(id: *mut u8) -> i32;
     pub fn ullis_cuda_dp_rendezvous(
         dir: *const c_char,

@@ -65,6 +65,18 @@ def codes(rows=4, channels=64):
     return torch.zeros(rows, channels, dtype=I8), torch.zeros(rows, -(-channels // 32), dtype=U8)
 
 
+def hidden(rows=4, channels=64):
+    return torch.zeros(rows, channels, dtype=H)
+
+
+def dense(vocab=9, channels=64):
+    return torch.zeros(vocab, channels, dtype=H)
+
+
+def labels(rows):
+    return torch.zeros(rows, dtype=torch.int32)
+
+
 REFUSED = {
     "pack: an array": (lambda rt: rt.tape_pack(np.zeros((4, 64), np.float32)), cuda.ERR_ARG),
     "pack: another device": (lambda rt: rt.tape_pack(torch.zeros(4, 64, device="meta")), cuda.ERR_ARG),
@@ -85,6 +97,22 @@ REFUSED = {
                             cuda.ERR_SHAPE),
     "norm backward: residual's type": (lambda rt: rt.tape_layer_norm_backward(
         codes(), torch.zeros(4, 64), torch.zeros(64, dtype=H), residual=torch.zeros(4, 64, dtype=H)), cuda.ERR_ARG),
+    "weight gradient: f32": (lambda rt: rt.tape_weight_grad(codes(), torch.zeros(4, 8)), cuda.ERR_ARG),
+    "weight gradient: rows": (lambda rt: rt.tape_weight_grad(codes(), torch.zeros(3, 8, dtype=H)), cuda.ERR_SHAPE),
+    "head: f32": (lambda rt: rt.head_ce_grad(torch.zeros(4, 64), torch.zeros(9, 64), labels(4)), cuda.ERR_ARG),
+    "head: labels": (lambda rt: rt.head_ce_grad(hidden(), dense(), labels(5)), cuda.ERR_SHAPE),
+    "head: 64-bit labels": (lambda rt: rt.head_ce_grad(hidden(), dense(), labels(4).long()), cuda.ERR_ARG),
+    "head: time": (lambda rt: rt.head_ce_grad(hidden(), dense(), labels(4), time=3), cuda.ERR_SHAPE),
+    "head: no time": (lambda rt: rt.head_ce_grad(hidden(), dense(), labels(4), time=0), cuda.ERR_SHAPE),
+    "head: channels": (lambda rt: rt.head_ce_grad(hidden(), dense(9, 32), labels(4)), cuda.ERR_SHAPE),
+    "head: transposed weights": (lambda rt: rt.head_ce_grad(hidden(), dense(64, 9).t(), labels(4)), cuda.ERR_SHAPE),
+    "head: weight's type": (lambda rt: rt.head_ce_grad(hidden(), dense().bfloat16(), labels(4)), cuda.ERR_ARG),
+    "head: packed without scales": (lambda rt: rt.head_ce_grad(hidden(), torch.zeros(18, dtype=torch.int32), labels(4)), cuda.ERR_ARG),
+    "head: too few words": (lambda rt: rt.head_ce_grad(hidden(), torch.zeros(17, dtype=torch.int32), labels(4),
+                                                       scale=torch.zeros(9, dtype=H)), cuda.ERR_SHAPE),
+    "head: bias": (lambda rt: rt.head_ce_grad(hidden(), dense(), labels(4), bias=torch.zeros(8, dtype=H)), cuda.ERR_SHAPE),
+    "head: bias's type": (lambda rt: rt.head_ce_grad(hidden(), dense(), labels(4), bias=torch.zeros(9)), cuda.ERR_ARG),
+    "head: ignore_id": (lambda rt: rt.head_ce_grad(hidden(), dense(), labels(4), ignore_id=1 << 32), cuda.ERR_ARG),
     "norm backward: residual's rows": (lambda rt: rt.tape_layer_norm_backward(
         codes(), torch.zeros(4, 64), torch.zeros(64, dtype=H), residual=torch.zeros(3, 64)), cuda.ERR_SHAPE),
 }

@@ -1,0 +1,136 @@
+"""CudaRuntime.tape_weight_grad against the product in 64 bits.  Products of 16-bit numbers and codes are exact in f32; within 1024
+rows the tensor cores cut off each addition (2^-23 per term), everything else is added with rounding (2^-24)."""
+import pytest
+import torch
+
+from ullis_b200 import cuda
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def tape_of(rows, c, seed=0, spread=1.0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    size = torch.exp(spread * torch.randn(rows, -(-c // 32), generator=g, device="cuda"))
+    codes = torch.randint(-127, 128, (rows, c), generator=g, device="cuda").to(torch.int8)
+    exponents = (torch.floor(torch.log2(size)) + 120).to(torch.uint8)
+    return codes, exponents
+
+
+def values(codes, exponents):
+    e = torch.exp2(exponents.double() - 127.0)
+    e = torch.where(exponents == 255, torch.nan, e)
+    return codes.double() * e.repeat_interleave(32, 1)[:, : codes.shape[1]]
+
+
+def check(got, gy, tape):
+    x, g = values(*tape), gy.double()
+    want, sizes = g.t() @ x, g.abs().t() @ x.abs()
+    rows = gy.shape[0]
+    off = U * (2 * min(rows, 1024) + 32 + rows / 1024) * sizes
+    assert got.dtype == torch.float32 and ((got.double() - want).abs() <= off).all()
+
+
+CASES = [(1, 1, 1), (1, 64, 200), (3, 33, 7), (63, 64, 64), (64, 256, 256), (65, 250, 1000), (333, 512, 96), (1024, 100, 300),
+         (1025, 520, 264), (3000, 2048, 64), (5000, 129, 2050), (16384, 64, 8), (20000, 512, 512)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_the_product(cuda_rt, case, dtype):
+    rows, i, o = case
+    tape = tape_of(rows, i, rows)
+    gy = (1e-2 * torch.randn(rows, o, device="cuda")).to(TYPES[dtype])
+    check(cuda_rt.tape_weight_grad(tape, gy), gy, tape)
+
+
+def test_terms_of_one_sign(cuda_rt):
+    """What the tensor cores cut off adds up where all terms have one sign."""
+    codes, exponents = tape_of(16384, 128, 3)
+    tape = codes.abs(), exponents
+    gy = torch.rand(16384, 64, device="cuda").half()
+    got = cuda_rt.tape_weight_grad(tape, gy)
+    want = gy.double().t() @ values(*tape)
+    assert (got.double() - want).norm() <= 1.5e-5 * want.norm()      # 64 accumulations of 16 terms: 64 * 2^-23 at most, and roundings
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_blocks_of_every_exponent(cuda_rt, dtype):
+    """A block's exponents 30 binades apart lose nothing in FP16; blocks of very different size do not meet."""
+    codes, _ = tape_of(512, 160, 1)
+    g = torch.Generator("cuda").manual_seed(2)
+    exponents = torch.empty(512, 5, dtype=torch.uint8, device="cuda")
+    for b, base in enumerate((1, 40, 127, 180, 215)):
+        exponents[:, b] = (base + torch.randint(0, 31, (512,), generator=g, device="cuda")).to(torch.uint8)
+    gy = (1e-2 * torch.randn(512, 72, device="cuda")).to(TYPES[dtype])
+    tape = codes, exponents
+    x = values(*tape)
+    got = cuda_rt.tape_weight_grad(tape, gy).double()
+    want, sizes = gy.double().t() @ x, gy.double().abs().t() @ x.abs()
+    assert ((got - want).abs() <= U * 1100 * sizes + 2.0 ** -149 * 512).all()
+
+
+def test_a_block_that_is_not_finite(cuda_rt):
+    codes, exponents = tape_of(100, 96, 5)
+    exponents[17, 1] = 255
+    for dtype in TYPES.values():
+        gy = torch.randn(100, 40, device="cuda").to(dtype)
+        got = cuda_rt.tape_weight_grad((codes, exponents), gy)
+        assert torch.isnan(got[:, 32:64]).all() and torch.isfinite(got[:, :32]).all() and torch.isfinite(got[:, 64:]).all()
+
+
+@pytest.mark.parametrize("offset,stride", [(0, 104), (1, 97), (8, 96), (3, 96)])
+def test_rows_with_gaps_and_odd_starts(cuda_rt, offset, stride):
+    tape = tape_of(300, 64)
+    base = torch.full((300 * stride + offset + 96,), float("nan"), device="cuda").half()
+    gy = base.as_strided((300, 96), (stride, 1), offset)
+    gy.copy_(torch.randn(300, 96, device="cuda"))
+    got = cuda_rt.tape_weight_grad(tape, gy)
+    assert torch.equal(got, cuda_rt.tape_weight_grad(tape, gy.contiguous()))
+    check(got, gy, tape)
+
+
+def test_zero_rows_and_leading_dimensions(cuda_rt):
+    empty = torch.zeros(0, 64, dtype=torch.int8, device="cuda"), torch.zeros(0, 2, dtype=torch.uint8, device="cuda")
+    got = cuda_rt.tape_weight_grad(empty, torch.zeros(0, 24, device="cuda").half())
+    assert got.shape == (24, 64) and not got.any()
+    x = torch.randn(3, 50, 64, device="cuda").half()
+    gy = torch.randn(3, 50, 24, device="cuda").half()
+    tape = cuda_rt.tape_pack(x)
+    assert tape.codes.shape == (3, 50, 64)
+    flat = tape.codes.reshape(150, 64), tape.exponents
+    assert torch.equal(cuda_rt.tape_weight_grad(tape, gy), cuda_rt.tape_weight_grad(flat, gy.reshape(150, 24)))
+
+
+def test_norm_linear_and_head_together(cuda_rt):
+    """Norm, linear and head of a small model from the 8-bit tape: every gradient as autograd gives it in 64 bits at the values that
+    the tape keeps."""
+    rows, time, d, vocab = 256, 64, 96, 500
+    t = torch.bfloat16
+    x = torch.randn(rows, d, device="cuda").to(t)
+    nw = (1 + 0.1 * torch.randn(d, device="cuda")).half()
+    nb = (0.1 * torch.randn(d, device="cuda")).half()
+    lin = (torch.randn(d, d, device="cuda") / d ** 0.5).to(t)
+    head = (0.05 * torch.randn(vocab, d, device="cuda")).to(t)
+    labels = torch.randint(0, vocab, (rows,), device="cuda").to(torch.int32)
+    y, tape_x = cuda_rt.tape_layer_norm(x, nw, nb)
+    tape_y = cuda_rt.tape_pack(y)
+    h = y @ lin.t()
+    r = cuda_rt.head_ce_grad(h, head, labels, time=time)
+    g_lin = cuda_rt.tape_weight_grad(tape_y, r.hidden)
+    gy = (r.hidden.float() @ lin.float()).to(t)
+    gx, gw, gb = cuda_rt.tape_layer_norm_backward(tape_x, gy, nw)
+
+    kept = cuda_rt.tape_unpack(tape_x, torch.float32).double().requires_grad_()
+    wd, bd = nw.double().requires_grad_(), nb.double().requires_grad_()
+    ld = lin.double().requires_grad_()
+    yd = torch.nn.functional.layer_norm(kept, (d,), wd, bd, 1e-5)
+    hd = yd @ ld.t()
+    z = hd @ head.double().t()
+    loss = (torch.logsumexp(z, 1) - z.gather(1, torch.roll(labels, -1).long()[:, None])[:, 0])
+    loss[torch.arange(rows, device="cuda") % time < time - 1].sum().backward()
+    # 8-bit inputs, and four 16-bit roundings on the way: half a step of 2^-7 is the largest of them
+    for name, got, want in (("x", gx, kept.grad), ("norm weight", gw, wd.grad), ("norm bias", gb, bd.grad), ("linear", g_lin, ld.grad)):
+        assert (got.double() - want).norm() <= 4 * 2.0 ** -7 * want.norm(), name

@@ -1,5 +1,6 @@
 // extern "C" entry points of the operators on device memory (include/ullis_cuda.h): checks of the arguments, the caller's stream
 // and device.  No C++ exception leaves this file.
+#include <cmath>
 #include <exception>
 #include <new>
 
@@ -44,6 +45,26 @@ int32_t on_stream(ullis_cuda_runtime* rt, void* cuda_stream, F&& body) {
     }
 }
 
+// Bytes of a workspace; the text of a refusal is ullis_cuda_last_error(NULL)'s.
+template <typename F>
+int32_t workspace_of(const ullis_cuda_runtime* rt, size_t* bytes, F&& body) {
+    if (!rt || !bytes) {
+        set_global_error(rt ? "bytes is null" : "runtime handle is null");
+        return ULLIS_CUDA_ERR_ARG;
+    }
+    *bytes = 0;
+    try {
+        *bytes = body();
+        return ULLIS_CUDA_OK;
+    } catch (const Error& e) {
+        set_global_error(e.msg.c_str());
+        return e.code;
+    } catch (const std::exception& e) {
+        set_global_error(e.what());
+        return ULLIS_CUDA_ERR_ARG;
+    }
+}
+
 void need_array(const void* p, const char* name, size_t align) {
     if (!p) fail(ULLIS_CUDA_ERR_ARG, std::string(name) + " is null");
     if (reinterpret_cast<uintptr_t>(p) % align) fail(ULLIS_CUDA_ERR_ARG, std::string(name) + " is not aligned to its elements");
@@ -70,9 +91,31 @@ void need_norm(size_t rows, size_t channels) {
     need_sizes(rows, channels, "tape LayerNorm");
     if (channels > dev::TAPE_NORM_CHANNELS) fail(ULLIS_CUDA_ERR_SHAPE, "tape LayerNorm takes at most 8192 channels");
 }
+void need_sm100(const ullis_cuda_runtime* rt) {
+    if (rt->cc_major != 10) fail(ULLIS_CUDA_ERR_CUDA, "this operator needs the tensor cores of an sm_100 device");
+}
 void need_codes(const uint8_t* codes, const uint8_t* exponents) {
     need_array(codes, "codes", 1);
     need_array(exponents, "exponents", 1);
+}
+
+// The tiles of a product are counted in 32 bits (up to 16 ranges of K each).
+void need_tiles(size_t m, size_t n, const char* what) {
+    if ((m + 255) / 256 * ((n + 255) / 256) >= ((size_t)1 << 27)) fail(ULLIS_CUDA_ERR_SHAPE, std::string(what) + " shape overflow");
+}
+void need_product(size_t rows, size_t in_features, size_t out_features) {
+    const char* what = "tape weight gradient";
+    need_sizes(rows, in_features, what);
+    need_sizes(rows, out_features, what);
+    need_tiles(out_features, in_features, what);
+}
+void need_head(size_t rows, size_t channels, size_t vocab) {
+    const char* what = "head cross-entropy";
+    need_sizes(rows, channels, what);
+    need_sizes(rows, vocab, what);
+    need_tiles(rows, vocab, what);
+    need_tiles(rows, channels, what);
+    need_tiles(vocab, channels, what);
 }
 
 }  // namespace
@@ -123,19 +166,10 @@ int32_t ullis_cuda_tape_layer_norm(ullis_cuda_runtime* rt, void* cuda_stream, in
 }
 
 int32_t ullis_cuda_tape_layer_norm_backward_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t* bytes) {
-    if (!rt || !bytes) {
-        set_global_error(rt ? "bytes is null" : "runtime handle is null");
-        return ULLIS_CUDA_ERR_ARG;
-    }
-    *bytes = 0;
-    try {
+    return workspace_of(rt, bytes, [&] {
         need_norm(rows, channels);
-    } catch (const Error& e) {
-        set_global_error(e.msg.c_str());
-        return e.code;
-    }
-    *bytes = dev::tape_layer_norm_backward_workspace(rt, rows, channels);
-    return ULLIS_CUDA_OK;
+        return dev::tape_layer_norm_backward_workspace(rt, rows, channels);
+    });
 }
 
 int32_t ullis_cuda_tape_layer_norm_backward(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const uint8_t* codes,
@@ -163,6 +197,100 @@ int32_t ullis_cuda_tape_layer_norm_backward(ullis_cuda_runtime* rt, void* cuda_s
         need_workspace(workspace, workspace_bytes, dev::tape_layer_norm_backward_workspace(rt, rows, channels));
         dev::tape_layer_norm_backward(s, dtype, codes, exponents, dev::Rows{gy, gy_stride}, weight, dev::Rows{residual, residual_stride},
                                       rows, channels, gx, g_weight, g_bias, workspace);
+    });
+}
+
+int32_t ullis_cuda_tape_weight_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t in_features, size_t out_features,
+                                              size_t* bytes) {
+    return workspace_of(rt, bytes, [&] {
+        need_product(rows, in_features, out_features);
+        return dev::tape_weight_grad_workspace(rt, rows, in_features, out_features);
+    });
+}
+
+int32_t ullis_cuda_tape_weight_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const uint8_t* codes,
+                                    const uint8_t* exponents, const void* gy, size_t gy_stride, size_t rows, size_t in_features,
+                                    size_t out_features, float* g, void* workspace, size_t workspace_bytes) {
+    return on_stream(rt, cuda_stream, [&](const dev::Stream& s) {
+        need_dtype(dtype, false);
+        need_product(rows, in_features, out_features);
+        need_stride(gy_stride, out_features, "gy");
+        need_array(g, "g", 4);
+        if (rows == 0) {
+            ULLIS_CUDA_CHECK(cudaMemsetAsync(g, 0, in_features * out_features * 4, s.stream));
+            return;
+        }
+        need_codes(codes, exponents);
+        need_array(gy, "gy", 2);
+        need_workspace(workspace, workspace_bytes, dev::tape_weight_grad_workspace(rt, rows, in_features, out_features));
+        need_sm100(rt);
+        dev::tape_weight_grad(s, dtype, codes, exponents, dev::Rows{gy, gy_stride}, rows, in_features, out_features, g, workspace);
+    });
+}
+
+int32_t ullis_cuda_head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, size_t* bytes) {
+    return workspace_of(rt, bytes, [&] {
+        need_head(rows, channels, vocab);
+        return dev::head_ce_grad_workspace(rt, rows, channels, vocab);
+    });
+}
+
+int32_t ullis_cuda_head_ce_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const void* hidden, size_t hidden_stride,
+                                const uint32_t* bits, const void* weight, const uint16_t* scale, const uint16_t* bias,
+                                const uint32_t* labels, uint32_t ignore_id, size_t rows, size_t time, size_t channels, size_t vocab,
+                                float loss_scale, float* row_loss, void* g_hidden, void* g_weight, float* g_scale, float* g_bias,
+                                void* workspace, size_t workspace_bytes) {
+    return on_stream(rt, cuda_stream, [&](const dev::Stream& s) {
+        need_dtype(dtype, false);
+        need_head(rows, channels, vocab);
+        if (time == 0 || time >= ((size_t)1 << 31) || rows % time) fail(ULLIS_CUDA_ERR_SHAPE, "rows must be a multiple of time");
+        need_stride(hidden_stride, channels, "hidden");
+        if (!std::isfinite(loss_scale)) fail(ULLIS_CUDA_ERR_ARG, "loss_scale is not finite");
+        if ((bits != nullptr) == (weight != nullptr)) fail(ULLIS_CUDA_ERR_ARG, "a head is either packed (bits) or dense (weight)");
+        if ((bits != nullptr) != (scale != nullptr)) fail(ULLIS_CUDA_ERR_ARG, "a packed head has row scales, a dense one none");
+        if (g_scale && !scale) fail(ULLIS_CUDA_ERR_ARG, "g_scale without row scales");
+        if (bits) {
+            need_array(bits, "bits", 4);
+            need_array(scale, "scale", 2);
+        } else {
+            need_array(weight, "weight", 2);
+        }
+        if (bias) need_array(bias, "bias", 2);
+        need_array(g_weight, "g_weight", 2);
+        if (g_scale) need_array(g_scale, "g_scale", 4);
+        if (g_bias) need_array(g_bias, "g_bias", 4);
+        if (rows == 0) {
+            ULLIS_CUDA_CHECK(cudaMemsetAsync(g_weight, 0, vocab * channels * 2, s.stream));
+            if (g_scale) ULLIS_CUDA_CHECK(cudaMemsetAsync(g_scale, 0, vocab * 4, s.stream));
+            if (g_bias) ULLIS_CUDA_CHECK(cudaMemsetAsync(g_bias, 0, vocab * 4, s.stream));
+            return;
+        }
+        need_array(hidden, "hidden", 2);
+        need_array(labels, "labels", 4);
+        need_array(row_loss, "row_loss", 4);
+        need_array(g_hidden, "g_hidden", 2);
+        need_workspace(workspace, workspace_bytes, dev::head_ce_grad_workspace(rt, rows, channels, vocab));
+        need_sm100(rt);
+        dev::HeadGrad h{};
+        h.dtype = dtype;
+        h.hidden = dev::Rows{hidden, hidden_stride};
+        h.bits = bits;
+        h.weight = weight;
+        h.scale = scale;
+        h.bias = bias;
+        h.labels = labels;
+        h.ignore_id = ignore_id;
+        h.rows = rows;
+        h.time = time;
+        h.channels = channels;
+        h.vocab = vocab;
+        h.loss_scale = loss_scale;
+        h.row_loss = row_loss;
+        h.g_hidden = g_hidden;
+        h.g_weight = g_weight;
+        h.g_scale = g_scale;
+        h.g_bias = g_bias;
+        dev::head_ce_grad(s, h, workspace);
     });
 }
 

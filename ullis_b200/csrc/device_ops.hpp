@@ -45,5 +45,31 @@ size_t tape_layer_norm_backward_workspace(const ullis_cuda_runtime* rt, size_t r
 void tape_layer_norm_backward(const Stream& s, int dtype, const uint8_t* codes, const uint8_t* exponents, Rows gy, const uint16_t* weight,
                               Rows residual, size_t rows, size_t channels, void* gx, float* g_weight, float* g_bias, void* workspace);
 
+// ---- gradient of a linear's weights from the tape of its input: g [out, in] f32 = gy^T . x^ (gy F16 or BF16)
+size_t tape_weight_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t in_features, size_t out_features);
+void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const uint8_t* exponents, Rows gy, size_t rows,
+                      size_t in_features, size_t out_features, float* g, void* workspace);
+
+// ---- cross-entropy of a head with its gradient
+struct HeadGrad {
+    int dtype;                 // of hidden and of the 16-bit outputs: F16 or BF16; hidden F32 (hidden_f32) is rounded to F16
+    bool hidden_f32;
+    Rows hidden;               // [rows, channels]
+    const uint32_t* bits;      // packed signs, or null and
+    const void* weight;        // dense [vocab, channels] of `dtype`
+    const uint16_t* scale;     // FP16 [vocab], with bits
+    const uint16_t* bias;      // FP16 [vocab], nullable
+    const uint32_t* labels;    // [rows]
+    uint32_t ignore_id;
+    size_t rows, time, channels, vocab;
+    float loss_scale;
+    float* row_loss;           // [rows]
+    void* g_hidden;            // [rows, channels]
+    void* g_weight;            // [vocab, channels]
+    float *g_scale, *g_bias;   // [vocab], nullable
+};
+size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab);
+void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace);
+
 }  // namespace dev
 }  // namespace ullis

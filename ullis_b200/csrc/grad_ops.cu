@@ -1,0 +1,646 @@
+// Cross-entropy of the head with its gradient, and weight gradients from the 8-bit tape, on the products of pair_gemm.cuh.
+//
+// Head (reference src/model.rs:3132-3275): a = h . s^T, z = scale * a + bias, loss = log sum exp z - z[target], and with
+// g = loss_scale * (softmax(z) - onehot), 0 on the rows that do not count (src/model.rs:27-39),
+//   g_hidden = (g * scale) . s,  g_weight = (g * scale)^T . h,  g_scale = sum over rows of g * a,  g_bias = sum of g.
+// The logits are never kept: one product gives log sum exp of every row, and piece by piece of the vocabulary a second one gives
+// g * scale in 16 bits, which the two gradient products read where it lies, by rows and by columns.  8 R V D operations instead of
+// the 6 R V D of a step that keeps R x V logits in 32 bits; a logit costs 2 D operations (0.7 ns at D = 512 and 1.5 PFLOP/s per
+// 1000) and would cost 8 bytes to write and read (1.2 ns).
+//
+// g is at most 1, the row scales are FP16 of any size: 2^k with max |scale| * 2^k in [2^14, 2^15) brings g * scale where 16 bits
+// hold most of it (FP16 from 2^-24 to 65504), and the products are multiplied by 2^-k * loss_scale at the end.  The rounding of
+// g * scale to 16 bits is the same that the training step's operands have (half a step: 2^-11 in FP16, 2^-8 in bf16, independent
+// from term to term); g_scale and g_bias are sums of what was not rounded.
+#include <algorithm>
+
+#include <cudaTypedefs.h>
+
+#include "device_ops.hpp"
+#include "pair_gemm.cuh"
+#include "tape.cuh"
+
+namespace ullis {
+namespace dev {
+namespace {
+
+constexpr int THREADS = 256;
+constexpr float LN2 = 0.6931471805599453f;
+
+size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
+size_t ceil_div(size_t n, size_t by) { return (n + by - 1) / by; }
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// The parts of a workspace, one behind the other on 256 bytes.
+struct Parts {
+    size_t bytes = 0;
+    size_t add(size_t n) {
+        const size_t at = bytes;
+        bytes += up(n, 256);
+        return at;
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ products
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        ULLIS_CUDA_CHECK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
+        if (!p || q != cudaDriverEntryPointSuccess) fail(ULLIS_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+// A 16-bit row-major matrix as an operand: boxes of 64 columns and 128 rows, or (mn: the columns are the operand's M or N) 64 rows.
+// The first column is 16-byte aligned and the stride a multiple of 8 elements.
+struct Operand {
+    const void* data;
+    size_t rows, columns, stride;
+    bool mn;
+};
+CUtensorMap operand_map(const Operand& o, bool bf16) {
+    CUtensorMap m;
+    const cuuint64_t dims[2] = {o.columns, o.rows}, strides[1] = {o.stride * 2};
+    const cuuint32_t box[2] = {64, o.mn ? 64u : 128u}, steps[2] = {1, 1};
+    const CUresult r = encode_fn()(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(o.data),
+                                   dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fail(ULLIS_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+    return m;
+}
+
+uint32_t pairs_of(const ullis_cuda_runtime* rt) { return std::max(1, rt->sm_count / 2); }
+
+template <int EPI, int ACCS>
+void launch(const Stream& s, const char* what, const Operand& a, const Operand& b, bool bf16, pg::Params p, uint32_t pairs) {
+    const auto kernel = pg::pair_gemm_kernel<EPI, ACCS>;
+    const size_t smem = pg::smem_bytes(EPI, ACCS);
+    ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    p.a_mn = a.mn;
+    p.b_mn = b.mn;
+    p.bf16 = bf16;
+    p.stages = pg::stages_for(EPI, ACCS);
+    p.status = s.status;
+    const pg::Maps maps{operand_map(a, bf16), operand_map(b, bf16)};
+    s.chain(what, kernel, 2 * pairs, pg::THREADS, smem, maps, p);
+}
+
+// How a product [M, N] over K is cut for `pairs` pairs: accumulators of 256 columns per pair (one or two) and ranges of K.
+// Estimated in k-blocks (256 x 256 x 64 on a pair, 0.3 us): rounds * (k-blocks + an epilogue nothing overlaps) and, with several
+// ranges, their sums written and read once more at 4 TB/s.
+struct Cut {
+    uint32_t accs, splits;
+};
+Cut cut_of(size_t M, size_t N, size_t K, uint32_t pairs, bool two) {
+    const size_t blocks = std::max<size_t>(1, ceil_div(K, pg::BK));
+    Cut best{1, 1};
+    double least = 1e300;
+    for (uint32_t accs = 1; accs <= (two && N > 256 ? 2u : 1u); ++accs) {
+        const size_t tiles = ceil_div(M, 256) * ceil_div(N, 256 * accs);
+        for (uint32_t splits = 1; splits <= std::min<size_t>(16, std::max<size_t>(1, blocks / 4)); ++splits) {
+            const double rounds = (double)ceil_div(tiles * splits, pairs);
+            const double epilogue = accs == 2 ? 10.0 : 1.0;
+            double cost = rounds * (ceil_div(blocks, splits) * accs + epilogue) + 4.0;
+            if (splits > 1) cost += (2.0 * splits + 1.0) * M * N * 4.0 / 4e6 / 0.3 + 8.0;
+            if (cost < least) {
+                least = cost;
+                best = Cut{accs, splits};
+            }
+        }
+    }
+    return best;
+}
+size_t partial_bytes(size_t M, size_t N, const Cut& c) { return c.splits > 1 ? c.splits * M * N * 4 : 0; }
+
+// The sum of `splits` arrays of n elements, in their order, times alpha (the columns' factors) as 16 bits or f32; with `accum`
+// added to it, or left there where `out` is null.
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+combine_kernel(const float* __restrict__ partial, uint32_t splits, size_t n, const float* __restrict__ factor, float* __restrict__ accum,
+               uint32_t accum_read, T* __restrict__ out) {
+    chain_entry();
+    const size_t i = ((size_t)blockIdx.x * THREADS + threadIdx.x) * 4;
+    if (i >= n) return;
+    const float alpha = factor ? *factor : 1.0f;
+    const bool whole = i + 4 <= n && n % 4 == 0;   // (each of the arrays on 16 bytes)
+    float v[4] = {};
+    const auto add = [&](const float* from) {
+        if (whole) {
+            const float4 t = *reinterpret_cast<const float4*>(from + i);
+            v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+        } else {
+            for (int e = 0; e < 4; ++e) if (i + e < n) v[e] += from[i + e];
+        }
+    };
+    for (uint32_t k = 0; k < splits; ++k) add(partial + k * n);
+    if (accum && accum_read) add(accum);
+    for (int e = 0; e < 4; ++e) {
+        if (i + e >= n) break;
+        if (out) out[i + e] = tape::from_float<T>(v[e] * alpha);
+        else accum[i + e] = v[e];
+    }
+}
+
+struct Output {
+    void* out;             // 16 bits, or null: `accum` is left
+    float* accum;
+    bool accum_read;
+    const float* factor;
+    float* partial;
+};
+// A 16-bit product out of `cut`
+void product(const Stream& s, const char* what, const Operand& a, const Operand& b, bool bf16, size_t M, size_t N, size_t K, const Cut& cut,
+             const Output& o) {
+    pg::Params p{};
+    p.M = (uint32_t)M;
+    p.N = (uint32_t)N;
+    p.K = (uint32_t)K;
+    p.splits = cut.splits;
+    p.out = o.out;
+    p.accum = o.accum;
+    p.accum_read = o.accum_read;
+    p.factor = o.factor;
+    p.partial = o.partial;
+    const uint32_t pairs = (uint32_t)std::min<size_t>(pairs_of(s.rt), ceil_div(M, 256) * ceil_div(N, 256 * cut.accs) * cut.splits);
+    if (cut.accs == 2) launch<pg::STORE, 2>(s, what, a, b, bf16, p, pairs);
+    else launch<pg::STORE, 1>(s, what, a, b, bf16, p, pairs);
+    if (cut.splits == 1) return;
+    const size_t n = M * N;
+    const unsigned grid = (unsigned)ceil_div(n, 4 * THREADS);
+    if (bf16) s.chain("combine", combine_kernel<__nv_bfloat16>, grid, THREADS, 0, o.partial, cut.splits, n, o.factor, o.accum, (uint32_t)o.accum_read,
+                      static_cast<__nv_bfloat16*>(o.out));
+    else s.chain("combine", combine_kernel<__half>, grid, THREADS, 0, o.partial, cut.splits, n, o.factor, o.accum, (uint32_t)o.accum_read,
+                 static_cast<__half*>(o.out));
+}
+
+// ------------------------------------------------------------------------------------------------ operands of the head
+// Rows of hidden as the operand [rows, Dp] (columns from D on and rows that do not count are 0: what a masked row holds, an
+// infinity say, stays out of the products), the rows' targets (-1: does not count, -2: a label outside the vocabulary), the weights
+// [vocab, Dp] (+/-1, or a copy of dense rows that no tensor map takes) and the largest |scale| per CTA of that part.
+struct HeadOperands {
+    const void* hidden;
+    size_t stride;
+    uint32_t rows, time, D, Dp, vocab;
+    const uint32_t* labels;
+    uint32_t ignore_id;
+    uint16_t* h16;
+    int32_t* target;
+    const uint32_t* bits;
+    const uint16_t *dense, *scale;
+    uint16_t* w16;              // null: the dense weights are taken as they are
+    float* scale_max;
+    uint32_t hidden_ctas;
+    uint32_t bf16;
+};
+constexpr uint32_t WEIGHT_CTAS = 1024;
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+head_operands_kernel(const HeadOperands o) {
+    chain_entry();
+    const uint32_t chunks = o.Dp / 8;
+    if (blockIdx.x < o.hidden_ctas) {
+        const size_t item = (size_t)blockIdx.x * THREADS + threadIdx.x;
+        const size_t row = item >> 32 ? item / chunks : (uint32_t)item / chunks;
+        if (row >= o.rows) return;
+        const uint32_t c = (uint32_t)(item - row * chunks) * 8;
+        int32_t target = -1;
+        if ((uint32_t)row % o.time + 1u < o.time) {   // then row + 1 is a row of the same sequence
+            const uint32_t label = o.labels[row + 1];
+            if (label != o.ignore_id) target = label < o.vocab ? (int32_t)label : -2;
+        }
+        if (c == 0) o.target[row] = target;
+        uint32_t w[4] = {};
+        if (target >= 0) {
+            const T* from = static_cast<const T*>(o.hidden) + row * o.stride + c;
+            if (sizeof(T) == 2 && c + 8 <= o.D && reinterpret_cast<uintptr_t>(from) % 16 == 0) {
+                const uint4 t = *reinterpret_cast<const uint4*>(from);
+                w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < o.D) {
+                        uint16_t h;
+                        if constexpr (sizeof(T) == 4) h = __half_as_ushort(__float2half_rn(from[e]));
+                        else h = *reinterpret_cast<const uint16_t*>(from + e);
+                        w[e >> 1] |= (uint32_t)h << (16 * (e & 1));
+                    }
+            }
+        }
+        *reinterpret_cast<uint4*>(o.h16 + row * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        return;
+    }
+    const uint32_t cta = blockIdx.x - o.hidden_ctas;
+    const uint32_t plus = o.bf16 ? 0x3F80u : 0x3C00u;
+    const size_t items = (size_t)o.vocab * chunks, words = ((size_t)o.vocab * o.D + 31) / 32;
+    float top = 0.0f;
+    for (size_t item = (size_t)cta * THREADS + threadIdx.x; item < items; item += (size_t)WEIGHT_CTAS * THREADS) {
+        const size_t v = item >> 32 ? item / chunks : (uint32_t)item / chunks;
+        const uint32_t c = (uint32_t)(item - v * chunks) * 8;
+        uint32_t w[4] = {};
+        if (o.bits) {
+            const size_t bit = v * o.D + c;
+            uint32_t signs = o.bits[bit >> 5] >> (bit & 31);
+            if ((bit & 31) > 24 && (bit >> 5) + 1 < words) signs |= o.bits[(bit >> 5) + 1] << (32 - (bit & 31));
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < o.D) w[e >> 1] |= (plus | ((signs >> e) & 1u ? 0u : 0x8000u)) << (16 * (e & 1));
+            if (c == 0) top = fmaxf(top, fabsf(__half2float(__ushort_as_half(o.scale[v]))));
+        } else {
+            const uint16_t* from = o.dense + v * o.D + c;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < o.D) w[e >> 1] |= (uint32_t)from[e] << (16 * (e & 1));
+        }
+        *reinterpret_cast<uint4*>(o.w16 + v * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (!o.bits) return;
+    __shared__ float tops[THREADS / 32];
+    for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+        o.scale_max[cta] = top;
+    }
+}
+
+// log2 sum exp of every row out of its parts, the row's loss, and (first CTA) the powers of two of g * scale.
+struct HeadRows {
+    const float2* part;
+    uint32_t rows, whole_rows, m_tiles, n_tiles, piece_tiles, slots, pairs;
+    const int32_t* target;
+    const float* target_logit;
+    float *lse2, *row_loss;
+    const float* scale_max;   // null: dense weights
+    float* factors;           // 2^k, 2^-k * loss_scale
+    float loss_scale;
+};
+__global__ void __launch_bounds__(128)
+head_rows_kernel(const HeadRows o) {
+    chain_entry();
+    if (blockIdx.x == 0) {
+        __shared__ float tops[4];
+        float top = o.scale_max ? 0.0f : 1.0f;
+        if (o.scale_max)
+            for (uint32_t i = threadIdx.x; i < WEIGHT_CTAS; i += 128) top = fmaxf(top, o.scale_max[i]);
+        for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            const int exponent = (int)(__float_as_uint(top) >> 23) - 127;
+            const int k = top > 0.0f && exponent < 128 ? 14 - exponent : 0;
+            o.factors[0] = exp2f((float)k);
+            o.factors[1] = exp2f((float)-k) * o.loss_scale;
+        }
+    }
+    const uint32_t row = blockIdx.x * 128 + threadIdx.x;
+    if (row >= o.rows) return;
+    const int32_t target = o.target[row];
+    if (target < 0) {
+        o.lse2[row] = INFINITY;
+        o.row_loss[row] = target == -1 ? 0.0f : NAN;
+        return;
+    }
+    const uint32_t m = row / pg::BM;
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t first = 0, piece = 0; first < o.n_tiles; first += o.piece_tiles, ++piece) {
+        const uint32_t width = min(o.piece_tiles, o.n_tiles - first);
+        const pg::Share share = pg::share_of(o.m_tiles * width, o.pairs);
+        const uint32_t slots = share.owner(m * width + width - 1) - share.owner(m * width) + 1;
+        for (uint32_t i = 0; i < slots * 4; ++i) {
+            const float2 t = o.part[((size_t)piece * o.slots * 4 + i) * o.whole_rows + row];
+            if (t.x > top) {
+                sum = sum * exp2f(top - t.x) + t.y;
+                top = t.x;
+            } else if (t.y != 0.0f) {   // (NaN too)
+                sum += t.y * exp2f(t.x - top);
+            }
+        }
+    }
+    const float lse2 = top + log2f(sum);
+    o.lse2[row] = lse2;
+    o.row_loss[row] = (lse2 - o.target_logit[row]) * LN2;
+}
+
+// The columns' sums of a piece out of their parts, times loss_scale.
+__global__ void __launch_bounds__(256)
+head_columns_kernel(const float* __restrict__ part, uint32_t pitch, uint32_t m_tiles, uint32_t n_tiles, uint32_t pairs, uint32_t columns,
+                    float loss_scale, float* __restrict__ g_scale, float* __restrict__ g_bias) {
+    chain_entry();
+    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= columns) return;
+    const pg::Share share = pg::share_of(m_tiles * n_tiles, pairs);
+    const uint32_t n = c / pg::BN, slots = share.owner(n * m_tiles + m_tiles - 1) - share.owner(n * m_tiles) + 1;
+    float g = 0.0f, ga = 0.0f;
+    for (uint32_t i = 0; i < slots * 8; ++i) {
+        g += part[(size_t)i * 2 * pitch + c];
+        ga += part[((size_t)i * 2 + 1) * pitch + c];
+    }
+    if (g_bias) g_bias[c] = g * loss_scale;
+    if (g_scale) g_scale[c] = ga * loss_scale;
+}
+
+// ------------------------------------------------------------------------------------------------ the head's plan
+struct HeadPlan {
+    size_t Dp, m_tiles, n_tiles;
+    uint32_t pairs;
+    uint32_t lse_tiles, lse_pieces, lse_slots;   // column tiles of a piece, pieces, parts per row in one
+    size_t piece, pieces;                        // columns of a piece of g (a multiple of 256), pieces
+    uint32_t col_slots;
+    Cut hidden, weight;
+    size_t h16, w16, target, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, partial, bytes;
+};
+constexpr size_t GRAD_ELEMENTS = (size_t)1 << 27;   // of a piece of g: 256 MiB
+
+uint32_t most_slots(uint32_t outer, uint32_t inner, uint32_t pairs) {
+    const pg::Share s = pg::share_of(outer * inner, pairs);
+    uint32_t most = 1;
+    for (uint32_t o = 0; o < outer; ++o) most = std::max(most, s.owner(o * inner + inner - 1) - s.owner(o * inner) + 1);
+    return most;
+}
+
+HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V) {
+    HeadPlan p{};
+    p.pairs = pairs_of(rt);
+    p.Dp = up(D, 8);
+    p.m_tiles = ceil_div(rows, pg::BM);
+    p.n_tiles = ceil_div(V, pg::BN);
+    // weights of a piece: up to 32 MiB, a quarter of L2
+    p.lse_tiles = (uint32_t)std::min(p.n_tiles, std::max<size_t>(8, ((size_t)32 << 20) / (pg::BN * p.Dp * 2)));
+    p.lse_pieces = (uint32_t)ceil_div(p.n_tiles, p.lse_tiles);
+    p.lse_slots = most_slots((uint32_t)p.m_tiles, p.lse_tiles, p.pairs);
+    const uint32_t rest = (uint32_t)(p.n_tiles - (p.lse_pieces - 1) * (size_t)p.lse_tiles);
+    p.lse_slots = std::max(p.lse_slots, most_slots((uint32_t)p.m_tiles, rest, p.pairs));
+    const size_t most = std::max<size_t>(1, GRAD_ELEMENTS / (p.m_tiles * pg::BM) / pg::BN);   // column tiles of a piece
+    p.pieces = ceil_div(p.n_tiles, most);
+    const size_t tiles = ceil_div(p.n_tiles, p.pieces);
+    p.pieces = ceil_div(p.n_tiles, tiles);
+    p.piece = tiles * pg::BN;
+    const size_t last = p.n_tiles - (p.pieces - 1) * tiles;
+    p.col_slots = std::max(most_slots((uint32_t)tiles, (uint32_t)p.m_tiles, p.pairs), most_slots((uint32_t)last, (uint32_t)p.m_tiles, p.pairs));
+    const size_t width = std::min(p.piece, V);
+    p.hidden = cut_of(rows, D, width, p.pairs, true);
+    p.weight = cut_of(width, D, rows, p.pairs, true);
+    Parts at;
+    p.h16 = at.add(rows * p.Dp * 2);
+    p.w16 = at.add(V * p.Dp * 2);
+    p.target = at.add(rows * 4);
+    p.lse2 = at.add(rows * 4);
+    p.logit = at.add(rows * 4);
+    p.factors = at.add(8);
+    p.scale_max = at.add(WEIGHT_CTAS * 4);
+    p.row_part = at.add((size_t)p.lse_pieces * p.lse_slots * 4 * p.m_tiles * pg::BM * 8);
+    p.grad = at.add(rows * p.piece * 2);
+    p.col_part = at.add((size_t)p.col_slots * 16 * p.piece * 4);
+    p.accum = at.add(p.pieces > 1 ? rows * D * 4 : 0);
+    p.partial = at.add(std::max(partial_bytes(rows, D, p.hidden), partial_bytes(width, D, p.weight)));
+    p.bytes = at.bytes;
+    return p;
+}
+
+}  // namespace
+
+size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab) {
+    return rows ? head_plan(rt, rows, channels, vocab).bytes : 0;
+}
+
+void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
+    const HeadPlan p = head_plan(s.rt, h.rows, h.channels, h.vocab);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const bool bf16 = h.dtype == BF16;
+    const size_t rows = h.rows, D = h.channels, V = h.vocab;
+    // dense weights that a tensor map takes are read where they are
+    const bool as_is = !h.bits && D % 8 == 0 && aligned(h.weight, 16);
+    const void* w16 = as_is ? h.weight : static_cast<const void*>(ws + p.w16);
+
+    HeadOperands o{};
+    o.hidden = h.hidden.data;
+    o.stride = h.hidden.stride;
+    o.rows = (uint32_t)rows;
+    o.time = (uint32_t)h.time;
+    o.D = (uint32_t)D;
+    o.Dp = (uint32_t)p.Dp;
+    o.vocab = (uint32_t)V;
+    o.labels = h.labels;
+    o.ignore_id = h.ignore_id;
+    o.h16 = reinterpret_cast<uint16_t*>(ws + p.h16);
+    o.target = reinterpret_cast<int32_t*>(ws + p.target);
+    o.bits = h.bits;
+    o.dense = static_cast<const uint16_t*>(h.weight);
+    o.scale = h.scale;
+    o.w16 = as_is ? nullptr : reinterpret_cast<uint16_t*>(ws + p.w16);
+    o.scale_max = reinterpret_cast<float*>(ws + p.scale_max);
+    o.hidden_ctas = (uint32_t)ceil_div(rows * (p.Dp / 8), THREADS);
+    o.bf16 = bf16;
+    const unsigned grid = o.hidden_ctas + (as_is ? 0 : WEIGHT_CTAS);
+    if (h.hidden_f32) s.chain("head_operands", head_operands_kernel<float>, grid, THREADS, 0, o);
+    else s.chain("head_operands", head_operands_kernel<__half>, grid, THREADS, 0, o);   // (moved, not read: bf16 too)
+
+    const Operand hidden{o.h16, rows, D, p.Dp, false}, weight{w16, V, D, as_is ? D : p.Dp, false};
+    pg::Params q{};
+    q.M = (uint32_t)rows;
+    q.N = (uint32_t)V;
+    q.K = (uint32_t)D;
+    q.scale = h.bits ? h.scale : nullptr;
+    q.bias = h.bias;
+    q.target = o.target;
+    q.piece_tiles = p.lse_tiles;
+    q.slots = p.lse_slots;
+    q.row_part = reinterpret_cast<float2*>(ws + p.row_part);
+    q.target_logit = reinterpret_cast<float*>(ws + p.logit);
+    q.lse2 = reinterpret_cast<float*>(ws + p.lse2);
+    float* factors = reinterpret_cast<float*>(ws + p.factors);
+    launch<pg::LSE, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+
+    HeadRows r{};
+    r.part = q.row_part;
+    r.rows = (uint32_t)rows;
+    r.whole_rows = (uint32_t)(p.m_tiles * pg::BM);
+    r.m_tiles = (uint32_t)p.m_tiles;
+    r.n_tiles = (uint32_t)p.n_tiles;
+    r.piece_tiles = p.lse_tiles;
+    r.slots = p.lse_slots;
+    r.pairs = p.pairs;
+    r.target = o.target;
+    r.target_logit = q.target_logit;
+    r.lse2 = reinterpret_cast<float*>(ws + p.lse2);
+    r.row_loss = h.row_loss;
+    r.scale_max = h.bits ? o.scale_max : nullptr;
+    r.factors = factors;
+    r.loss_scale = h.loss_scale;
+    s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 128), 128, 0, r);
+
+    uint16_t* grad = reinterpret_cast<uint16_t*>(ws + p.grad);
+    for (size_t piece = 0; piece < p.pieces; ++piece) {
+        const size_t v0 = piece * p.piece, width = std::min(p.piece, V - v0);
+        const uint32_t n_tiles = (uint32_t)ceil_div(width, pg::BN);
+        pg::Params g = q;
+        g.N = (uint32_t)width;
+        g.n_first = (uint32_t)v0;
+        g.scale = q.scale ? q.scale + v0 : nullptr;
+        g.bias = q.bias ? q.bias + v0 : nullptr;
+        g.factor = factors;
+        g.grad = grad;
+        g.pitch = (uint32_t)p.piece;
+        g.col_part = reinterpret_cast<float*>(ws + p.col_part);
+        Operand wp = weight;
+        wp.data = static_cast<const uint16_t*>(w16) + v0 * weight.stride;
+        wp.rows = width;
+        launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs);
+        if (h.g_bias || h.g_scale)
+            s.chain("head_columns", head_columns_kernel, (unsigned)ceil_div(width, 256), 256, 0, static_cast<const float*>(g.col_part), g.pitch,
+                    (uint32_t)p.m_tiles, n_tiles, p.pairs, (uint32_t)width, h.loss_scale, h.g_scale ? h.g_scale + v0 : nullptr,
+                    h.g_bias ? h.g_bias + v0 : nullptr);
+        // g_hidden: over the pieces in f32
+        const Operand by_rows{grad, rows, width, p.piece, false};
+        wp.mn = true;
+        const bool last = piece + 1 == p.pieces;
+        product(s, "head_g_hidden", by_rows, wp, bf16, rows, D, width, p.hidden,
+                Output{last ? h.g_hidden : nullptr, p.pieces > 1 ? reinterpret_cast<float*>(ws + p.accum) : nullptr, piece > 0, factors + 1,
+                       reinterpret_cast<float*>(ws + p.partial)});
+        const Operand by_columns{grad, rows, width, p.piece, true};
+        Operand hc = hidden;
+        hc.mn = true;
+        product(s, "head_g_weight", by_columns, hc, bf16, width, D, rows, p.weight,
+                Output{static_cast<uint16_t*>(h.g_weight) + v0 * D, nullptr, false, factors + 1, reinterpret_cast<float*>(ws + p.partial)});
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ weight gradient from the tape
+namespace {
+
+// The largest exponent byte of each block of 32 channels over the rows.  A thread has a block and every `slices`-th row.
+__global__ void __launch_bounds__(THREADS)
+tape_exponent_max_kernel(const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t blocks, uint32_t slices, uint32_t* __restrict__ top) {
+    chain_entry();
+    const uint32_t item = blockIdx.x * THREADS + threadIdx.x, slice = item / blocks, b = item - slice * blocks;
+    if (slice >= slices) return;
+    uint32_t most = 0;
+    for (uint32_t r = slice; r < rows; r += slices) most = max(most, (uint32_t)exponents[(size_t)r * blocks + b]);
+    atomicMax(top + b, most);
+}
+
+// What the codes stand for as a 16-bit operand [rows, Cp].  bf16 holds every value (8 significant bits, the range of f32).  FP16
+// does not: there each block of 32 channels is shifted by a power of two common to all rows, so that its largest exponent comes to 8
+// (127 * 2^8 = 32 512), and the column's sums are shifted back.  What is lost lies 2^32 below the block's largest value.
+template <bool BF>
+__global__ void __launch_bounds__(THREADS)
+tape_operand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t C, uint32_t Cp,
+                    const uint32_t* __restrict__ top, uint16_t* __restrict__ out, float* __restrict__ col_factor) {
+    chain_entry();
+    const uint32_t chunks = Cp / 8, blocks = (C + 31) / 32;
+    const size_t item = (size_t)blockIdx.x * THREADS + threadIdx.x;
+    if (!BF && item < blocks) {
+        const uint32_t byte = top[item];
+        col_factor[item] = byte == tape::NOT_FINITE ? 1.0f : exp2f((float)((int)byte - 127 - 8));
+    }
+    const size_t row = item >> 32 ? item / chunks : (uint32_t)item / chunks;
+    if (row >= rows) return;
+    const uint32_t c = (uint32_t)(item - row * chunks) * 8, byte = exponents[row * blocks + c / 32];
+    float step = tape::power(byte);
+    if (!BF && byte != tape::NOT_FINITE) {
+        const uint32_t most = top[c / 32];
+        step = exp2f((float)((int)byte - (int)(most == tape::NOT_FINITE ? byte : most) + 8));
+    }
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (c + e < C) {
+            const float v = (float)(int8_t)codes[row * C + c + e] * step;
+            const uint32_t h = BF ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+            w[e >> 1] |= h << (16 * (e & 1));
+        }
+    *reinterpret_cast<uint4*>(out + row * Cp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 16-bit rows that no tensor map takes, with a stride of whole 16 bytes
+__global__ void __launch_bounds__(THREADS)
+rows16_kernel(const uint16_t* __restrict__ x, size_t stride, uint32_t rows, uint32_t C, uint32_t Cp, uint16_t* __restrict__ out) {
+    chain_entry();
+    const uint32_t chunks = Cp / 8;
+    const size_t item = (size_t)blockIdx.x * THREADS + threadIdx.x;
+    const size_t row = item >> 32 ? item / chunks : (uint32_t)item / chunks;
+    if (row >= rows) return;
+    const uint32_t c = (uint32_t)(item - row * chunks) * 8;
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (c + e < C) w[e >> 1] |= (uint32_t)x[row * stride + c + e] << (16 * (e & 1));
+    *reinterpret_cast<uint4*>(out + row * Cp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct WeightPlan {
+    size_t ip, op;
+    Cut cut;
+    size_t x16, gy16, top, col_factor, partial, bytes;
+};
+WeightPlan weight_plan(const ullis_cuda_runtime* rt, size_t rows, size_t in, size_t out) {
+    WeightPlan p{};
+    p.ip = up(in, 8);
+    p.op = up(out, 8);
+    p.cut = cut_of(out, in, rows, pairs_of(rt), false);
+    Parts at;
+    p.x16 = at.add(rows * p.ip * 2);
+    p.gy16 = at.add(rows * p.op * 2);
+    p.top = at.add(tape::blocks_of(in) * 4);
+    p.col_factor = at.add(tape::blocks_of(in) * 4);
+    p.partial = at.add(partial_bytes(out, in, p.cut));
+    p.bytes = at.bytes;
+    return p;
+}
+
+}  // namespace
+
+size_t tape_weight_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t in_features, size_t out_features) {
+    return rows ? weight_plan(rt, rows, in_features, out_features).bytes : 0;
+}
+
+void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const uint8_t* exponents, Rows gy, size_t rows, size_t in,
+                      size_t out, float* g, void* workspace) {
+    const WeightPlan p = weight_plan(s.rt, rows, in, out);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const bool bf16 = dtype == BF16;
+    uint16_t* x16 = reinterpret_cast<uint16_t*>(ws + p.x16);
+    uint32_t* top = reinterpret_cast<uint32_t*>(ws + p.top);
+    float* col_factor = reinterpret_cast<float*>(ws + p.col_factor);
+    const uint32_t blocks = (uint32_t)tape::blocks_of(in);
+    const unsigned grid = (unsigned)ceil_div(rows * (p.ip / 8), THREADS);
+    if (bf16) {
+        s.chain("tape_operand", tape_operand_kernel<true>, grid, THREADS, 0, codes, exponents, (uint32_t)rows, (uint32_t)in, (uint32_t)p.ip,
+                static_cast<const uint32_t*>(top), x16, col_factor);
+    } else {
+        ULLIS_CUDA_CHECK(cudaMemsetAsync(top, 0, blocks * 4, s.stream));
+        const uint32_t slices = (uint32_t)std::min<size_t>(ceil_div(rows, 16), 4096);
+        s.chain("tape_exponent_max", tape_exponent_max_kernel, (unsigned)ceil_div((size_t)slices * blocks, THREADS), THREADS, 0, exponents,
+                (uint32_t)rows, blocks, slices, top);
+        s.chain("tape_operand", tape_operand_kernel<false>, grid, THREADS, 0, codes, exponents, (uint32_t)rows, (uint32_t)in, (uint32_t)p.ip,
+                static_cast<const uint32_t*>(top), x16, col_factor);
+    }
+    Operand a{gy.data, rows, out, gy.stride, true};
+    if (!aligned(gy.data, 16) || gy.stride % 8) {
+        uint16_t* gy16 = reinterpret_cast<uint16_t*>(ws + p.gy16);
+        s.chain("rows16", rows16_kernel, (unsigned)ceil_div(rows * (p.op / 8), THREADS), THREADS, 0, static_cast<const uint16_t*>(gy.data),
+                gy.stride, (uint32_t)rows, (uint32_t)out, (uint32_t)p.op, gy16);
+        a = Operand{gy16, rows, out, p.op, true};
+    }
+    const Operand b{x16, rows, in, p.ip, true};
+    pg::Params q{};
+    q.M = (uint32_t)out;
+    q.N = (uint32_t)in;
+    q.K = (uint32_t)rows;
+    q.splits = p.cut.splits;
+    q.out = g;
+    q.partial = reinterpret_cast<float*>(ws + p.partial);
+    q.col_factor = bf16 ? nullptr : col_factor;
+    const uint32_t pairs = (uint32_t)std::min<size_t>(pairs_of(s.rt), ceil_div(out, 256) * ceil_div(in, 256) * p.cut.splits);
+    launch<pg::SUM, 1>(s, "tape_weight_grad", a, b, bf16, q, pairs);
+    if (p.cut.splits > 1)
+        s.chain("combine", combine_kernel<float>, (unsigned)ceil_div(out * in, 4 * THREADS), THREADS, 0, static_cast<const float*>(q.partial), p.cut.splits,
+                out * in, static_cast<const float*>(nullptr), static_cast<float*>(nullptr), 0u, g);
+}
+
+}  // namespace dev
+}  // namespace ullis

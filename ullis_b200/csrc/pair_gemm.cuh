@@ -1,0 +1,680 @@
+// Matrix products D[M,N] = A . B^T on CTA pairs (tcgen05.mma.cta_group::2, M = 256), 16-bit operands, f32 accumulators in TMEM,
+// for the gradient of the head and of linears.  Either operand may lie in memory with its K elements side by side (row-major [M,K])
+// or with its M (N) elements side by side ([K,M] row-major): the tensor cores read both from 128-byte-swizzled tiles, so a
+// gradient product takes an activation as the forward pass left it and nothing is transposed in memory.
+//
+//  * A pair has 256 rows and 256 * ACCS columns of the output.  CTA r of it brings rows 128 r .. of A and of each 256 columns'
+//    B into its own ring of shared memory; the even CTA issues the products, each CTA finds its 128 rows in its own TMEM.
+//    ACCS = 1: two accumulators take turns, the epilogue drains one while the other fills.  ACCS = 2: one of 512 columns, every
+//    element of A is fetched once for 512 columns; for products whose K is long beside the epilogue.
+//  * Warp 0 fetches, warp 1 multiplies, 16 warps are the epilogue: four to a TMEM lane quarter, 64 columns each.
+//  * The grid is persistent; which tiles a pair has follows from its number alone (Work below), so all sums have a fixed order.
+//
+// Epilogues:
+//   LSE    z = scale * acc + bias: running maximum and sum of exp over the columns, per row and quarter of the columns
+//   GRAD   g = softmax(z) - onehot, by rows as the 16-bit operand g * scale * 2^k of the products that follow, and by columns the
+//          f32 sums of g and g * acc
+//   STORE  alpha * acc in 16 bits, or into an f32 accumulator, or as one of several partial sums
+//   SUM    acc in f32: the tensor cores cut off what falls below the accumulator's last bit (measured: K = 16384 1.9e-5 off in
+//          norm, 1.1e-4 where all terms have one sign; K = 1024 1e-6), so every 1024 terms the accumulator moves to registers
+//          and is added there with rounding
+// Every wait is bounded and reports through the status words, as in tc_gemm_ws2.cuh.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.hpp"
+#include "tc_ptx.cuh"
+
+namespace ullis {
+namespace pg {
+
+enum { LSE = 0, GRAD = 1, STORE = 2, SUM = 3 };
+
+constexpr uint32_t BM = 256, BN = 256, BK = 64;         // of a pair, per accumulator
+constexpr uint32_t OPERAND_BYTES = 128 * BK * 2;        // one CTA's 128 rows of A, or of one accumulator's B
+constexpr uint32_t EPI_WARPS = 16;
+constexpr int THREADS = 64 + 32 * (int)EPI_WARPS;
+constexpr uint32_t MAX_STAGES = 6, SMEM_LIMIT = 227 * 1024;
+constexpr uint32_t STAGING_BYTES = 16 * 128;            // per epilogue warp: 16 rows of 64 16-bit outputs
+constexpr uint32_t COLUMN_BYTES = 3 * 64 * 4;           // per epilogue warp: its columns' constants
+constexpr uint32_t SUM_BLOCKS = 16;                     // k-blocks between two rounded additions
+
+struct Maps {
+    CUtensorMap a, b;
+};
+
+struct Params {
+    uint32_t M, N, K;
+    uint32_t a_mn, b_mn;       // operand with M (N) side by side
+    uint32_t bf16;
+    uint32_t stages;
+    uint32_t* status;
+    // LSE, GRAD: columns [n_first, n_first + N) of the vocabulary
+    const uint16_t *scale, *bias;   // FP16 or null, of the first column
+    const int32_t* target;          // [M] column of the vocabulary, or negative
+    uint32_t n_first;
+    uint32_t piece_tiles;      // LSE: column tiles that all pairs go through before the next ones
+    uint32_t slots;            // LSE: partial sums per piece and row
+    float2* row_part;          // LSE: [piece][slot][4][rows, whole tiles]
+    float* target_logit;       // LSE: [M] in units of log2 e
+    const float* lse2;         // GRAD: [M] log2 of the sum of exp, +inf for a row that does not count
+    const float* factor;       // GRAD: 2^k ; STORE: alpha
+    uint16_t* grad;            // GRAD: [M][pitch]
+    uint32_t pitch;
+    float* col_part;           // GRAD: [slot][8][2][pitch]
+    // STORE, SUM
+    uint32_t splits;           // of K
+    void* out;                 // 16 bits [M][N] (STORE) or f32 [M][N] (SUM), where nothing follows
+    float* accum;              // f32 [M][N]; STORE: read first if `accum_read`, written unless `out` is
+    uint32_t accum_read;
+    float* partial;            // splits > 1: [split][M][N]
+    const float* col_factor;   // SUM: [ceil(N / 32)] or null
+};
+
+inline uint32_t stage_bytes(int accs) { return OPERAND_BYTES * (1 + accs); }
+inline uint32_t fixed_bytes(int epi) {
+    return 1024 /*alignment*/ + 256 /*barriers*/ + EPI_WARPS * ((epi == GRAD || epi == STORE ? STAGING_BYTES : 0u) +
+                                                               (epi == LSE || epi == GRAD ? COLUMN_BYTES : 0u));
+}
+inline uint32_t stages_for(int epi, int accs) {
+    const uint32_t fit = (SMEM_LIMIT - fixed_bytes(epi)) / stage_bytes(accs);
+    return fit < MAX_STAGES ? fit : MAX_STAGES;
+}
+inline uint32_t smem_bytes(int epi, int accs) { return fixed_bytes(epi) + stages_for(epi, accs) * stage_bytes(accs); }
+
+// `total` tiles in a row are shared out to `pairs` (at most `total`) pairs without gaps: pair c has [first(c), first(c + 1)).
+struct Share {
+    uint32_t total, pairs;
+    __host__ __device__ uint32_t first(uint32_t c) const { return (uint32_t)((uint64_t)c * total / pairs); }
+    __host__ __device__ uint32_t owner(uint32_t tile) const { return (uint32_t)((((uint64_t)tile + 1) * pairs - 1) / total); }
+};
+__host__ __device__ inline Share share_of(uint32_t total, uint32_t pairs) { return Share{total, total < pairs ? total : pairs}; }
+
+// What a pair computes, tile by tile; every warp of the pair goes through the same list.
+//  LSE   piece after piece of the columns (whose B stays in L2); in a piece the tiles of 256 rows follow one another
+//  GRAD  tiles of 256 columns follow one another
+//  STORE, SUM  jobs of one tile and one range of K, dealt out in turn
+template <int EPI, int ACCS>
+struct Work {
+    const Params& p;
+    uint32_t pair, pairs, m_tiles, n_tiles, blocks;
+    uint32_t piece = 0, at = 0, end = 0, width = 0;   // LSE, GRAD
+    uint32_t job = 0;                                 // STORE, SUM
+    // the tile
+    uint32_t m = 0, n = 0, k0 = 0, k1 = 0, split = 0;
+
+    __device__ Work(const Params& p_, uint32_t pair_, uint32_t pairs_) : p(p_), pair(pair_), pairs(pairs_) {
+        m_tiles = (p.M + BM - 1) / BM;
+        n_tiles = (p.N + BN * ACCS - 1) / (BN * ACCS);
+        blocks = (p.K + BK - 1) / BK;
+        k1 = blocks;
+        job = pair;
+        if (EPI == LSE) open_piece();
+        if (EPI == GRAD) open(m_tiles * n_tiles);
+    }
+    __device__ void open(uint32_t total) {
+        const Share s = share_of(total, pairs);
+        at = end = 0;
+        if (pair < s.pairs) { at = s.first(pair); end = s.first(pair + 1); }
+    }
+    __device__ void open_piece() {
+        width = min(p.piece_tiles, n_tiles - piece * p.piece_tiles);
+        open(m_tiles * width);
+    }
+    __device__ bool next() {
+        if (EPI == LSE) {
+            while (at == end) {
+                if (++piece * p.piece_tiles >= n_tiles) return false;
+                open_piece();
+            }
+            m = at / width;
+            n = piece * p.piece_tiles + at % width;
+            ++at;
+            return true;
+        }
+        if (EPI == GRAD) {
+            if (at == end) return false;
+            n = at / m_tiles;
+            m = at % m_tiles;
+            ++at;
+            return true;
+        }
+        if (job >= m_tiles * n_tiles * p.splits) return false;
+        const uint32_t tile = job / p.splits;
+        split = job % p.splits;
+        m = tile / n_tiles;
+        n = tile % n_tiles;
+        k0 = (uint32_t)((uint64_t)split * blocks / p.splits);
+        k1 = (uint32_t)((uint64_t)(split + 1) * blocks / p.splits);
+        job += pairs;
+        return true;
+    }
+};
+
+// 16 lanes x 64 columns: register 4 j + i of thread t has row t / 4 + 8 (i / 2), column 8 j + 2 (t % 4) + i % 2
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+// Descriptor of a tile with the M (N) elements side by side: atoms of 64 of them (128 bytes, swizzled) x 8 k, 1024 bytes apart
+// along k; the next 64 elements 64 k-rows, 8192 bytes, on.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16) {
+    if (bf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float half_at(const uint16_t* p, uint32_t i, float missing) {
+    return p ? __half2float(__ushort_as_half(p[i])) : missing;
+}
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* s_error) {
+    for (uint32_t spin = 0; spin < ptx::WAIT_POLLS; ++spin) {
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+        if (spin > 64) {
+            __nanosleep(spin > 4096 ? 256 : 32);
+            if ((spin & 1023u) == 0 && *s_error) return false;
+        }
+    }
+    return false;
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// The constants of this warp's 64 columns of the tile at n0: scale and bias times log2 e, scale * 2^k.  Columns past N have a
+// probability of 0.
+template <int EPI>
+__device__ __forceinline__ void load_columns(const Params& p, uint32_t n0, int lane, float* columns, float power) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t c = i * 32 + lane, n = n0 + c;
+        const bool in = n < p.N;
+        const float s = in ? half_at(p.scale, n, 1.0f) : 0.0f;
+        columns[c] = s * LOG2E;
+        columns[64 + c] = in ? half_at(p.bias, n, 0.0f) * LOG2E : -INFINITY;
+        if (EPI == GRAD) columns[128 + c] = s * power;
+    }
+}
+
+template <int EPI, int ACCS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr uint32_t STAGE = OPERAND_BYTES * (1 + ACCS);
+    const uint32_t STAGES = p.stages;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);   // [STAGES] even CTA: both CTAs' bytes have landed
+    uint64_t* empty = full + MAX_STAGES;                                   // [STAGES] the products that read the stage are done
+    uint64_t* tmem_full = empty + MAX_STAGES;                              // [2] accumulator complete
+    uint64_t* tmem_empty = tmem_full + 2;                                  // [2] even CTA: drained in both CTAs
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+    uint32_t* s_error = tmem_slot + 1;
+    uint8_t* epi_smem = reinterpret_cast<uint8_t*>(full) + 256;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_ctarank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], 1);
+        }
+        for (uint32_t b = 0; b < 2; ++b) {
+            ptx::mbar_init(&tmem_full[b], 1);
+            ptx::mbar_init(&tmem_empty[b], 2 * EPI_WARPS);
+        }
+        *s_error = 0;
+        ptx::fence_mbar_init();
+        ptx::tma_prefetch_desc(&maps.a);
+        ptx::tma_prefetch_desc(&maps.b);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(tmem_slot, 512);
+        ptx::tmem_relinquish_pair();
+    }
+    chain_entry();
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync_all();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    constexpr uint32_t BUFFERS = ACCS == 1 ? 2 : 1;
+    Work<EPI, ACCS> work(p, pair, pairs);
+
+    if (warp == 0) {
+        // ------------------------------------------------------ fetching (both CTAs, own rows)
+        if (ptx::elect_one()) {
+            const uint32_t full_even = ptx::cluster_map(full, 0);
+            uint32_t it = 0;
+            bool ok = true;
+            while (ok && work.next()) {
+                const int32_t m0 = (int32_t)(work.m * BM + rank * 128), n0 = (int32_t)(work.n * BN * ACCS + rank * 128);
+                for (uint32_t kb = work.k0; kb < work.k1; ++kb, ++it) {
+                    const uint32_t s = it % STAGES;
+                    if (it >= STAGES && !wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, s_error)) {
+                        atomicCAS(s_error, 0u, 1u);
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* st = smem + s * STAGE;
+                    const int32_t k = (int32_t)(kb * BK);
+                    const uint32_t bar = full_even + 8 * s;
+                    if (rank == 0) ptx::mbar_arrive_expect_tx(&full[s], 2 * STAGE);
+                    if (p.a_mn) {
+                        ptx::tma_load_2d_pair(st, &maps.a, bar, m0, k);
+                        ptx::tma_load_2d_pair(st + 8192, &maps.a, bar, m0 + 64, k);
+                    } else {
+                        ptx::tma_load_2d_pair(st, &maps.a, bar, k, m0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < ACCS; ++i) {
+                        uint8_t* bt = st + (1 + i) * OPERAND_BYTES;
+                        const int32_t nb = n0 + i * (int32_t)BN;
+                        if (p.b_mn) {
+                            ptx::tma_load_2d_pair(bt, &maps.b, bar, nb, k);
+                            ptx::tma_load_2d_pair(bt + 8192, &maps.b, bar, nb + 64, k);
+                        } else {
+                            ptx::tma_load_2d_pair(bt, &maps.b, bar, k, nb);
+                        }
+                    }
+                }
+            }
+            // On the way out after a failed wait, leave no copy in flight (as in tc_gemm_ws2.cuh: the even CTA waits for every
+            // stage filled last, the odd one, which cannot poll those barriers, far longer than a copy takes).
+            if (!ok && rank == 0) {
+                const uint32_t first = it > STAGES ? it - STAGES : 0;
+                for (uint32_t k = first; k < it; ++k) ptx::mbar_wait(&full[k % STAGES], (k / STAGES) & 1u, 1u << 12);
+            }
+            if (!ok && rank == 1)
+                for (int i = 0; i < 64; ++i) __nanosleep(1000);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------ products (even CTA)
+        if (rank == 0 && ptx::elect_one()) {
+            const uint32_t idesc = ptx::idesc_f16(p.bf16, p.bf16, BM, BN) | p.a_mn << 15 | p.b_mn << 16;
+            const uint32_t a_step = p.a_mn ? 2048u : 32u, b_step = p.b_mn ? 2048u : 32u;   // 16 k
+            const uint32_t ring = ptx::smem_u32(smem);
+            uint32_t it = 0, done = 0;   // k-blocks, accumulators
+            bool ok = true;
+            while (ok && work.next()) {
+                for (uint32_t kb = work.k0; kb < work.k1 && ok;) {
+                    const uint32_t last = EPI == SUM ? min(work.k1, kb + SUM_BLOCKS) : work.k1;
+                    const uint32_t buf = done % BUFFERS;
+                    if (done >= BUFFERS && !wait(&tmem_empty[buf], ((done / BUFFERS) & 1u) ^ 1u, s_error)) {
+                        atomicCAS(s_error, 0u, 2u);
+                        ok = false;
+                        break;
+                    }
+                    ptx::tc_fence_after_sync();
+                    bool add = false;
+                    for (; kb < last; ++kb, ++it) {
+                        const uint32_t s = it % STAGES;
+                        if (!wait(&full[s], (it / STAGES) & 1u, s_error)) {
+                            atomicCAS(s_error, 0u, 3u);
+                            ok = false;
+                            break;
+                        }
+                        ptx::tc_fence_after_sync();
+                        const uint32_t a = ring + s * STAGE, b = a + OPERAND_BYTES;
+#pragma unroll
+                        for (uint32_t k4 = 0; k4 < BK / 16; ++k4) {
+                            const uint64_t da = p.a_mn ? smem_desc_mn(a + k4 * a_step) : ptx::smem_desc_sw128(a + k4 * a_step);
+#pragma unroll
+                            for (int i = 0; i < ACCS; ++i) {
+                                const uint32_t bi = b + i * OPERAND_BYTES + k4 * b_step;
+                                const uint64_t db = p.b_mn ? smem_desc_mn(bi) : ptx::smem_desc_sw128(bi);
+                                ptx::mma_f16_ss_pair(tmem_base + (ACCS == 1 ? buf : i) * BN, da, db, idesc, add || k4);
+                            }
+                        }
+                        add = true;
+                        ptx::mma_commit_pair(&empty[s]);
+                    }
+                    ptx::mma_commit_pair(&tmem_full[buf]);   // on the way out too: the epilogues do not wait in vain
+                    ++done;
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------ epilogue (both CTAs, own rows)
+        const uint32_t quarter = warp & 3, group = (uint32_t)(warp - 2) >> 2, mine = warp - 2;
+        const uint32_t empty_even = ptx::cluster_map(tmem_empty, 0);
+        uint8_t* staging = epi_smem + mine * STAGING_BYTES;
+        float* columns = reinterpret_cast<float*>(epi_smem + (EPI == GRAD ? EPI_WARPS * STAGING_BYTES : 0u) + mine * COLUMN_BYTES);
+        uint32_t done = 0;
+        // Waits for the next accumulator; false: leave.  The loads are warp-collective: the whole warp decides.
+        const auto filled = [&](uint32_t* taddr) {
+            const uint32_t buf = done % BUFFERS;
+            if (!__all_sync(0xffffffffu, wait(&tmem_full[buf], (done / BUFFERS) & 1u, s_error))) {
+                atomicCAS(s_error, 0u, 4u);
+                return false;
+            }
+            ptx::tc_fence_after_sync();
+            if (__any_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(s_error) != 0u)) return false;
+            *taddr = tmem_base + buf * BN + ((quarter * 32) << 16);
+            return true;
+        };
+        const auto drained = [&]() {
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster(empty_even + 8 * (done % BUFFERS));
+            ++done;
+        };
+        const uint32_t q2 = (lane & 3) * 2, r0 = lane >> 2;   // of the 16 x 64 form: first column of a pair, first row
+
+        if constexpr (EPI == LSE) {
+            const uint32_t rows = work.m_tiles * BM;
+            uint32_t m_now = 0xFFFFFFFFu, piece_now = 0;
+            float top = -INFINITY, sum = 0.0f;
+            int32_t target = -1;
+            const auto leave = [&]() {
+                if (m_now == 0xFFFFFFFFu) return;
+                const uint32_t width = min(p.piece_tiles, work.n_tiles - piece_now * p.piece_tiles);
+                const uint32_t slot = pair - share_of(work.m_tiles * width, pairs).owner(m_now * width);
+                const size_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
+                p.row_part[(((size_t)piece_now * p.slots + slot) * 4 + group) * rows + row] = make_float2(top, sum);
+            };
+            while (work.next()) {
+                const uint32_t n0 = work.n * BN + group * 64;
+                if (work.m != m_now || work.piece != piece_now) {
+                    leave();
+                    m_now = work.m;
+                    piece_now = work.piece;
+                    top = -INFINITY;
+                    sum = 0.0f;
+                    const uint32_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
+                    target = row < p.M ? p.target[row] : -1;
+                }
+                __syncwarp();
+                load_columns<EPI>(p, n0, lane, columns, 0.0f);
+                __syncwarp();
+                uint32_t taddr;
+                if (!filled(&taddr)) break;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t r[32];
+                    ptx::tmem_ld_32x32(taddr + group * 64 + c * 32, r);
+                    ptx::tmem_ld_wait();
+                    if (c == 1) drained();
+                    const int32_t hit = target - (int32_t)(n0 + c * 32);
+                    float z[32], best = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 s = *reinterpret_cast<const float4*>(columns + c * 32 + i);
+                        const float4 b = *reinterpret_cast<const float4*>(columns + 64 + c * 32 + i);
+                        z[i] = fmaf(__uint_as_float(r[i]), s.x, b.x);
+                        z[i + 1] = fmaf(__uint_as_float(r[i + 1]), s.y, b.y);
+                        z[i + 2] = fmaf(__uint_as_float(r[i + 2]), s.z, b.z);
+                        z[i + 3] = fmaf(__uint_as_float(r[i + 3]), s.w, b.w);
+                    }
+                    if (hit >= 0 && hit < 32) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (hit == i) p.target_logit[m_now * BM + rank * 128 + quarter * 32 + lane] = z[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) best = fmaxf(best, z[i]);
+                    if (best > top) {
+                        sum *= exp2_fast(top - best);   // top = -inf: 0 * 0
+                        top = best;
+                    }
+                    const float base = top == -INFINITY ? 0.0f : top;   // (a NaN among z makes the sum one)
+                    float here[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) here[i & 3] += exp2_fast(z[i] - base);
+                    sum += (here[0] + here[1]) + (here[2] + here[3]);
+                }
+            }
+            leave();
+        } else if constexpr (EPI == GRAD) {
+            const float power = *p.factor;
+            const Share all = share_of(work.m_tiles * work.n_tiles, pairs);
+            uint32_t n_now = 0xFFFFFFFFu;
+            float g_sum[16], ga_sum[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) g_sum[i] = ga_sum[i] = 0.0f;
+            const auto leave = [&]() {   // the sums of 32 rows: over the lanes that share columns, then out
+                if (n_now == 0xFFFFFFFFu) return;
+                const uint32_t slot = pair - all.owner(n_now * work.m_tiles);
+                float* to = p.col_part + (((size_t)slot * 8 + rank * 4 + quarter) * 2) * p.pitch + n_now * BN + group * 64 + q2;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float a = g_sum[i], b = ga_sum[i];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        a += __shfl_xor_sync(0xffffffffu, a, o);
+                        b += __shfl_xor_sync(0xffffffffu, b, o);
+                    }
+                    if (lane < 4) {
+                        to[(i >> 1) * 8 + (i & 1)] = a;
+                        to[p.pitch + (i >> 1) * 8 + (i & 1)] = b;
+                    }
+                    g_sum[i] = ga_sum[i] = 0.0f;
+                }
+            };
+            while (work.next()) {
+                const uint32_t n0 = work.n * BN + group * 64, m0 = work.m * BM + rank * 128 + quarter * 32;
+                if (work.n != n_now) {
+                    leave();
+                    n_now = work.n;
+                    __syncwarp();
+                    load_columns<EPI>(p, n0, lane, columns, power);
+                    __syncwarp();
+                }
+                float lse[4];
+                int32_t hit[4];
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t row = m0 + r0 + i * 8;
+                    lse[i] = row < p.M ? p.lse2[row] : INFINITY;
+                    hit[i] = (row < p.M ? p.target[row] : -1) - (int32_t)(p.n_first + n0);
+                    any |= hit[i] >= 0 && hit[i] < 64;
+                }
+                any = __any_sync(0xffffffffu, any);
+                uint32_t taddr;
+                if (!filled(&taddr)) break;
+                const auto half = [&](int h, auto targets) {
+                    uint32_t r[32];
+                    tmem_ld_16x64(taddr + group * 64 + ((h * 16) << 16), r);
+                    ptx::tmem_ld_wait();
+                    if (h == 1) drained();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 s = *reinterpret_cast<const float2*>(columns + j * 8 + q2);
+                        const float2 b = *reinterpret_cast<const float2*>(columns + 64 + j * 8 + q2);
+                        const float2 k = *reinterpret_cast<const float2*>(columns + 128 + j * 8 + q2);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float a0 = __uint_as_float(r[j * 4 + i * 2]), a1 = __uint_as_float(r[j * 4 + i * 2 + 1]);
+                            float g0 = exp2_fast(fmaf(a0, s.x, b.x) - lse[h * 2 + i]), g1 = exp2_fast(fmaf(a1, s.y, b.y) - lse[h * 2 + i]);
+                            if (decltype(targets)::value) {
+                                if (hit[h * 2 + i] == j * 8 + (int)q2) g0 -= 1.0f;
+                                if (hit[h * 2 + i] == j * 8 + (int)q2 + 1) g1 -= 1.0f;
+                            }
+                            g_sum[j * 2] += g0;
+                            g_sum[j * 2 + 1] += g1;
+                            ga_sum[j * 2] = fmaf(g0, a0, ga_sum[j * 2]);
+                            ga_sum[j * 2 + 1] = fmaf(g1, a1, ga_sum[j * 2 + 1]);
+                            // 16-byte piece j of the row at j ^ (row % 8): neither side meets a bank conflict
+                            *reinterpret_cast<uint32_t*>(staging + (r0 + i * 8) * 128 + ((j ^ r0) << 4) + (lane & 3) * 4) =
+                                pack16(g0 * k.x, g1 * k.y, p.bf16);
+                        }
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t row = i * 4 + (lane >> 3), piece = lane & 7;
+                        const uint4 v = *reinterpret_cast<const uint4*>(staging + row * 128 + ((piece ^ (row & 7)) << 4));
+                        const uint32_t gm = m0 + h * 16 + row;
+                        if (gm < p.M) *reinterpret_cast<uint4*>(p.grad + (size_t)gm * p.pitch + n0 + piece * 8) = v;
+                    }
+                    __syncwarp();
+                };
+                if (any) {
+                    half(0, std::true_type{});
+                    half(1, std::true_type{});
+                } else {
+                    half(0, std::false_type{});
+                    half(1, std::false_type{});
+                }
+            }
+            leave();
+        } else if constexpr (EPI == STORE) {
+            const float alpha = p.factor ? *p.factor : 1.0f;
+            const bool pairs_ok = (p.N & 1) == 0;   // two columns of an f32 row lie on 8 bytes
+            const bool wide = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+            uint16_t* out = static_cast<uint16_t*>(p.out);
+            while (work.next()) {
+                uint32_t taddr;
+                if (!filled(&taddr)) break;
+                const uint32_t m0 = work.m * BM + rank * 128 + quarter * 32;
+                float* partial = p.splits > 1 ? p.partial + (size_t)work.split * p.M * p.N : nullptr;
+                const bool to16 = !partial && p.out;
+#pragma unroll 1
+                for (uint32_t part = 0; part < 2 * ACCS; ++part) {
+                    const uint32_t h = part & 1, c0 = (group * ACCS + (part >> 1)) * 64, n0 = work.n * BN * ACCS + c0;
+                    uint32_t r[32];
+                    tmem_ld_16x64(taddr + c0 + ((h * 16) << 16), r);
+                    ptx::tmem_ld_wait();
+                    if (part == 2 * ACCS - 1) drained();
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                    const auto f32_rows = [&](float* at, bool read, bool write) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t row = m0 + h * 16 + r0 + i * 8;
+                            if (row >= p.M) continue;
+                            float* line = at + (size_t)row * p.N;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const uint32_t c = n0 + j * 8 + q2;
+                                float &x = v[j * 4 + i * 2], &y = v[j * 4 + i * 2 + 1];
+                                if (pairs_ok) {
+                                    if (c < p.N) {
+                                        float2* both = reinterpret_cast<float2*>(line + c);
+                                        if (read) { const float2 old = *both; x += old.x; y += old.y; }
+                                        if (write) *both = make_float2(x, y);
+                                    }
+                                } else {
+                                    if (c < p.N) { if (read) x += line[c]; if (write) line[c] = x; }
+                                    if (c + 1 < p.N) { if (read) y += line[c + 1]; if (write) line[c + 1] = y; }
+                                }
+                            }
+                        }
+                    };
+                    if (partial) { f32_rows(partial, false, true); continue; }
+                    if (p.accum) f32_rows(p.accum, p.accum_read, !to16);
+                    if (!to16) continue;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            *reinterpret_cast<uint32_t*>(staging + (r0 + i * 8) * 128 + ((j ^ r0) << 4) + (lane & 3) * 4) =
+                                pack16(v[j * 4 + i * 2] * alpha, v[j * 4 + i * 2 + 1] * alpha, p.bf16);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t row = i * 4 + (lane >> 3), piece = lane & 7, gm = m0 + h * 16 + row, c = n0 + piece * 8;
+                        const uint4 w = *reinterpret_cast<const uint4*>(staging + row * 128 + ((piece ^ (row & 7)) << 4));
+                        if (gm >= p.M || c >= p.N) continue;
+                        uint16_t* to = out + (size_t)gm * p.N + c;
+                        if (wide) {
+                            *reinterpret_cast<uint4*>(to) = w;
+                        } else {
+                            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (c + e < p.N) to[e] = (uint16_t)(words[e >> 1] >> (16 * (e & 1)));
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        } else {
+            static_assert(EPI != SUM || ACCS == 1, "");
+            const bool pairs_ok = (p.N & 1) == 0;
+            bool ok = true;
+            while (ok && work.next()) {
+                float v[64];
+#pragma unroll
+                for (int i = 0; i < 64; ++i) v[i] = 0.0f;
+                for (uint32_t kb = work.k0; kb < work.k1; kb += SUM_BLOCKS) {
+                    uint32_t taddr;
+                    ok = filled(&taddr);
+                    if (!ok) break;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t r[32];
+                        tmem_ld_16x64(taddr + group * 64 + ((h * 16) << 16), r);
+                        ptx::tmem_ld_wait();
+                        if (h == 1) drained();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[h * 32 + i] += __uint_as_float(r[i]);
+                    }
+                }
+                if (!ok) break;
+                const uint32_t m0 = work.m * BM + rank * 128 + quarter * 32, n0 = work.n * BN + group * 64;
+                float f[2] = {1.0f, 1.0f};
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (p.col_factor && n0 + i * 32 < p.N) f[i] = p.col_factor[n0 / 32 + i];
+                float* out = p.splits > 1 ? p.partial + (size_t)work.split * p.M * p.N : static_cast<float*>(p.out);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t row = m0 + r0 + i * 8;
+                    if (row >= p.M) continue;
+                    float* line = out + (size_t)row * p.N;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t c = n0 + j * 8 + q2;
+                        const int at = (i >> 1) * 32 + j * 4 + (i & 1) * 2;
+                        const float x = v[at] * f[j >> 2], y = v[at + 1] * f[j >> 2];
+                        if (pairs_ok) {
+                            if (c < p.N) *reinterpret_cast<float2*>(line + c) = make_float2(x, y);
+                        } else {
+                            if (c < p.N) line[c] = x;
+                            if (c + 1 < p.N) line[c + 1] = y;
+                        }
+                    }
+                }
+            }
+        }
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync_all();   // neither CTA leaves while the other may still read its tiles or ring its barriers
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc_pair(tmem_base, 512);
+    }
+    if (threadIdx.x == 0 && *s_error) {
+        volatile uint32_t* status = p.status;   // a caller's stream: pinned host memory
+        status[1] = 64u + *s_error;
+        __threadfence_system();
+        status[0] = ULLIS_DEV_WAIT_TIMEOUT;
+    }
+}
+
+}  // namespace pg
+}  // namespace ullis

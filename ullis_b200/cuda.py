@@ -22,7 +22,7 @@ import threading
 
 import numpy as np
 
-from .device import DeviceOps, Tape  # noqa: F401
+from .device import DeviceOps, HeadGrad, Tape  # noqa: F401
 from .errors import (ERR_ARG, ERR_CHECKPOINT, ERR_CUDA, ERR_DEVICE_CHECK, ERR_NCCL, ERR_NOMEM, ERR_SHAPE,  # noqa: F401
                      ERR_TIMEOUT, ERR_TOKEN, OK, UllisCudaError)
 
@@ -64,6 +64,8 @@ ABI_SYMBOLS = (
     "ullis_cuda_dp_allreduce_loss", "ullis_cuda_dp_finalize",
     "ullis_cuda_tape_pack", "ullis_cuda_tape_unpack", "ullis_cuda_tape_layer_norm",
     "ullis_cuda_tape_layer_norm_backward_workspace", "ullis_cuda_tape_layer_norm_backward",
+    "ullis_cuda_tape_weight_grad_workspace", "ullis_cuda_tape_weight_grad", "ullis_cuda_head_ce_grad_workspace",
+    "ullis_cuda_head_ce_grad",
 )
 
 

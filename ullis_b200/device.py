@@ -21,6 +21,17 @@ class Tape(NamedTuple):
     exponents: object
 
 
+class HeadGrad(NamedTuple):
+    """row_loss float32 [rows]; hidden, weight: gradients in hidden's type; scale (None for a dense head), bias (None without
+    one): gradients in float32 [vocab]."""
+
+    row_loss: object
+    hidden: object
+    weight: object
+    scale: object
+    bias: object
+
+
 _DTYPES = None
 
 
@@ -175,3 +186,64 @@ class DeviceOps:
             _p(residual), _z(r_stride), _z(rows), _z(channels), _p(gx), C.c_void_p(g.data_ptr()),
             C.c_void_p(g.data_ptr() + 4 * channels), _p(work), size))
         return gx, g[0], g[1]
+
+    def tape_weight_grad(self, tape, gy):
+        """Gradient of a linear's weights, float32 [out, in]: gy [..., out] (float16, bfloat16) transposed times what the tape
+        of the linear's input stands for."""
+        torch = _torch()
+        codes, exponents, rows, channels = self._tape(tape)
+        gy, g_rows, out, stride = self._matrix(gy, "gy", (torch.float16, torch.bfloat16))
+        if g_rows != rows:
+            _shape_error("gy", gy.shape, (rows, out))
+        g = self._new((out, channels), torch.float32)
+        work, size = self._workspace(self._lib.ullis_cuda_tape_weight_grad_workspace, _z(rows), _z(channels), _z(out))
+        self._check(self._lib.ullis_cuda_tape_weight_grad(
+            self._h, self._stream_of(), C.c_int32(_DTYPES[gy.dtype]), _p(codes), _p(exponents), _p(gy), _z(stride), _z(rows),
+            _z(channels), _z(out), _p(g), _p(work), size))
+        return g
+
+    # ------------------------------------------------------------------------------------------ head
+    def head_ce_grad(self, hidden, weight, labels, *, scale=None, bias=None, ignore_id: int = 0xFFFFFFFF, time=None,
+                     loss_scale: float = 1.0) -> HeadGrad:
+        """Next-token cross-entropy of a head with its gradient; logits are never kept.
+
+        hidden [..., channels] float16 or bfloat16; labels int32, one per row (a negative id and `ignore_id` are taken as the
+        unsigned 32-bit number they are); `time` rows to a sequence (default: all, or with three dimensions the second).  A
+        packed head is `weight` int32 words of sign bits in checkpoint order with `scale` float16 [vocab]; a dense one is
+        `weight` [vocab, channels] in hidden's type and no scale.  bias float16 [vocab] or None.  Gradients are of
+        loss_scale * sum of row_loss; that of a packed weight is of the +/-1 values."""
+        torch = _torch()
+        hidden, rows, channels, stride = self._matrix(hidden, "hidden", (torch.float16, torch.bfloat16))
+        labels = self._vector(labels, "labels", (torch.int32,), rows)
+        if time is None:
+            time = hidden.shape[-2] if hidden.dim() == 3 else max(rows, 1)
+        if scale is not None:
+            scale = self._tensor(scale, "scale", (torch.float16,))
+            vocab = scale.numel()
+            scale = self._vector(scale, "scale", (torch.float16,), vocab)
+            weight = self._vector(weight, "weight", (torch.int32,), (vocab * channels + 31) // 32)
+        else:
+            weight = self._tensor(weight, "weight", (hidden.dtype,))
+            if weight.dim() != 2 or weight.shape[1] != channels or not weight.is_contiguous():
+                _shape_error("weight", weight.shape, ("vocab", channels))
+            vocab = weight.shape[0]
+        if bias is not None:
+            bias = self._vector(bias, "bias", (torch.float16,), vocab)
+        ignore = int(ignore_id)
+        if not -(1 << 31) <= ignore < 1 << 32:
+            raise UllisCudaError(ERR_ARG, "ignore_id is not a 32-bit number")
+        if not 0 < int(time) < 1 << 31 or rows % int(time):
+            raise UllisCudaError(ERR_SHAPE, "rows must be a multiple of time")
+        row_loss = self._new((rows,), torch.float32)
+        g_hidden = self._new(hidden.shape, hidden.dtype)
+        g_weight = self._new((vocab, channels), hidden.dtype)
+        g_scale = None if scale is None else self._new((vocab,), torch.float32)
+        g_bias = None if bias is None else self._new((vocab,), torch.float32)
+        work, size = self._workspace(self._lib.ullis_cuda_head_ce_grad_workspace, _z(rows), _z(channels), _z(vocab))
+        packed = scale is not None
+        self._check(self._lib.ullis_cuda_head_ce_grad(
+            self._h, self._stream_of(), C.c_int32(_DTYPES[hidden.dtype]), _p(hidden), _z(stride), _p(weight if packed else None),
+            _p(None if packed else weight), _p(scale), _p(bias), _p(labels), C.c_uint32(ignore & 0xFFFFFFFF), _z(rows),
+            _z(int(time)), _z(channels), _z(vocab), C.c_float(loss_scale), _p(row_loss), _p(g_hidden), _p(g_weight), _p(g_scale),
+            _p(g_bias), _p(work), size))
+        return HeadGrad(row_loss, g_hidden, g_weight, g_scale, g_bias)
