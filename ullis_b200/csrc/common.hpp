@@ -167,6 +167,7 @@ struct ullis_cuda_runtime {
     int tc_ws2_clusters[5] = {0, 0, 0, 0, 0};   // CTA pairs of that kernel the device holds at once, per epilogue
     bool tc_fuse_ln = true;             // LayerNorm folded into the kernel that writes the 16-bit operands of the next GEMM
     bool tc_fix_blocks = true;          // exact sign recomputation by blocks of 32 steps with their rows in shared memory; false: the window form
+    uint32_t pair_gemms_ready = 0;      // forms of pair_gemm_kernel that have been allowed their dynamic shared memory
     int tc_ready = 0;                   // 0 = not probed, 1 = usable, -1 = unusable on this device
     ullis::NcclState* nccl = nullptr;
 

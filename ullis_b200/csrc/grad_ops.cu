@@ -59,31 +59,41 @@ struct Operand {
     size_t rows, columns, stride;
     bool mn;
 };
-CUtensorMap operand_map(const Operand& o, bool bf16) {
+CUtensorMap map_of(const void* data, size_t rows, size_t columns, size_t stride, uint32_t box_rows, bool bf16) {
     CUtensorMap m;
-    const cuuint64_t dims[2] = {o.columns, o.rows}, strides[1] = {o.stride * 2};
-    const cuuint32_t box[2] = {64, o.mn ? 64u : 128u}, steps[2] = {1, 1};
-    const CUresult r = encode_fn()(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(o.data),
+    const cuuint64_t dims[2] = {columns, rows}, strides[1] = {stride * 2};
+    const cuuint32_t box[2] = {64, box_rows}, steps[2] = {1, 1};
+    const CUresult r = encode_fn()(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(data),
                                    dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) fail(ULLIS_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
     return m;
 }
+CUtensorMap operand_map(const Operand& o, bool bf16) { return map_of(o.data, o.rows, o.columns, o.stride, o.mn ? 64 : 128, bf16); }
 
 uint32_t pairs_of(const ullis_cuda_runtime* rt) { return std::max(1, rt->sm_count / 2); }
 
-template <int EPI, int ACCS>
-void launch(const Stream& s, const char* what, const Operand& a, const Operand& b, bool bf16, pg::Params p, uint32_t pairs) {
-    const auto kernel = pg::pair_gemm_kernel<EPI, ACCS>;
+template <int EPI, int ACCS, bool BF16>
+void launch_form(const Stream& s, const char* what, const pg::Maps& maps, const pg::Params& p, uint32_t pairs) {
+    const auto kernel = pg::pair_gemm_kernel<EPI, ACCS, BF16>;
     const size_t smem = pg::smem_bytes(EPI, ACCS);
-    ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const uint32_t flag = 1u << (EPI * 4 + (ACCS - 1) * 2 + BF16);
+    if (!(s.rt->pair_gemms_ready & flag)) {
+        ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        s.rt->pair_gemms_ready |= flag;
+    }
+    s.chain(what, kernel, 2 * pairs, pg::THREADS, smem, maps, p);
+}
+template <int EPI, int ACCS>
+void launch(const Stream& s, const char* what, const Operand& a, const Operand& b, bool bf16, pg::Params p, uint32_t pairs,
+            const CUtensorMap* out = nullptr) {
     p.a_mn = a.mn;
     p.b_mn = b.mn;
-    p.bf16 = bf16;
     p.stages = pg::stages_for(EPI, ACCS);
     p.status = s.status;
-    const pg::Maps maps{operand_map(a, bf16), operand_map(b, bf16)};
-    s.chain(what, kernel, 2 * pairs, pg::THREADS, smem, maps, p);
+    const pg::Maps maps{operand_map(a, bf16), operand_map(b, bf16), out ? *out : CUtensorMap{}};
+    if (bf16) launch_form<EPI, ACCS, true>(s, what, maps, p, pairs);
+    else launch_form<EPI, ACCS, false>(s, what, maps, p, pairs);
 }
 
 // How a product [M, N] over K is cut for `pairs` pairs: accumulators of 256 columns per pair (one or two) and ranges of K.
@@ -176,8 +186,9 @@ void product(const Stream& s, const char* what, const Operand& a, const Operand&
 
 // ------------------------------------------------------------------------------------------------ operands of the head
 // Rows of hidden as the operand [rows, Dp] (columns from D on and rows that do not count are 0: what a masked row holds, an
-// infinity say, stays out of the products), the rows' targets (-1: does not count, -2: a label outside the vocabulary), the weights
-// [vocab, Dp] (+/-1, or a copy of dense rows that no tensor map takes) and the largest |scale| per CTA of that part.
+// infinity say, stays out of the products), the rows' targets (-1: does not count, -2: a label outside the vocabulary) and their
+// targets' logits in f32, the weights [vocab, Dp] (+/-1, or a copy of dense rows that no tensor map takes) and the largest |scale|
+// per CTA of that part.  A warp has a row of hidden, a thread a chunk of eight weights.
 struct HeadOperands {
     const void* hidden;
     size_t stride;
@@ -186,8 +197,9 @@ struct HeadOperands {
     uint32_t ignore_id;
     uint16_t* h16;
     int32_t* target;
+    float* logit2;              // target's logit times log2 e
     const uint32_t* bits;
-    const uint16_t *dense, *scale;
+    const uint16_t *dense, *scale, *bias;
     uint16_t* w16;              // null: the dense weights are taken as they are
     float* scale_max;
     uint32_t hidden_ctas;
@@ -195,54 +207,85 @@ struct HeadOperands {
 };
 constexpr uint32_t WEIGHT_CTAS = 1024;
 
+__device__ __forceinline__ float from16(uint32_t bits, bool bf16) {
+    return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((uint16_t)bits));
+}
+// signs of eight weights from bit `bit` of `words` words on, the first in the lowest bit
+__device__ __forceinline__ uint32_t signs8(const uint32_t* bits, size_t bit, size_t words) {
+    const uint32_t shift = (uint32_t)bit & 31u;
+    uint32_t v = bits[bit >> 5] >> shift;
+    if (shift > 24 && (bit >> 5) + 1 < words) v |= bits[(bit >> 5) + 1] << (32 - shift);
+    return v;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 head_operands_kernel(const HeadOperands o) {
     chain_entry();
     const uint32_t chunks = o.Dp / 8;
+    const size_t words = ((size_t)o.vocab * o.D + 31) / 32;
     if (blockIdx.x < o.hidden_ctas) {
-        const size_t item = (size_t)blockIdx.x * THREADS + threadIdx.x;
-        const size_t row = item >> 32 ? item / chunks : (uint32_t)item / chunks;
+        const uint32_t row = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
         if (row >= o.rows) return;
-        const uint32_t c = (uint32_t)(item - row * chunks) * 8;
         int32_t target = -1;
-        if ((uint32_t)row % o.time + 1u < o.time) {   // then row + 1 is a row of the same sequence
+        if (row % o.time + 1u < o.time) {   // then row + 1 is a row of the same sequence
             const uint32_t label = o.labels[row + 1];
             if (label != o.ignore_id) target = label < o.vocab ? (int32_t)label : -2;
         }
-        if (c == 0) o.target[row] = target;
-        uint32_t w[4] = {};
-        if (target >= 0) {
-            const T* from = static_cast<const T*>(o.hidden) + row * o.stride + c;
-            if (sizeof(T) == 2 && c + 8 <= o.D && reinterpret_cast<uintptr_t>(from) % 16 == 0) {
-                const uint4 t = *reinterpret_cast<const uint4*>(from);
-                w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
-            } else {
+        float dot = 0.0f;
+        const size_t first = (size_t)max(target, 0) * o.D;   // of the target's weights
+        for (uint32_t chunk = lane; chunk < chunks; chunk += 32) {
+            const uint32_t c = chunk * 8;
+            uint32_t w[4] = {};
+            if (target >= 0) {
+                const T* from = static_cast<const T*>(o.hidden) + row * o.stride + c;
+                if (sizeof(T) == 2 && c + 8 <= o.D && reinterpret_cast<uintptr_t>(from) % 16 == 0) {
+                    const uint4 t = *reinterpret_cast<const uint4*>(from);
+                    w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
+                } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c + e < o.D) {
-                        uint16_t h;
-                        if constexpr (sizeof(T) == 4) h = __half_as_ushort(__float2half_rn(from[e]));
-                        else h = *reinterpret_cast<const uint16_t*>(from + e);
-                        w[e >> 1] |= (uint32_t)h << (16 * (e & 1));
-                    }
+                    for (int e = 0; e < 8; ++e)
+                        if (c + e < o.D) {
+                            uint16_t h;
+                            if constexpr (sizeof(T) == 4) h = __half_as_ushort(__float2half_rn(from[e]));
+                            else h = *reinterpret_cast<const uint16_t*>(from + e);
+                            w[e >> 1] |= (uint32_t)h << (16 * (e & 1));
+                        }
+                }
+                if (o.bits) {
+                    const uint32_t signs = signs8(o.bits, first + c, words);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)   // (0 past the row's end)
+                        dot += from16(((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu) ^ ((signs >> e) & 1u ? 0u : 0x8000u), o.bf16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (c + e < o.D) dot = fmaf(from16((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, o.bf16), from16(o.dense[first + c + e], o.bf16), dot);
+                }
             }
+            *reinterpret_cast<uint4*>(o.h16 + (size_t)row * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        *reinterpret_cast<uint4*>(o.h16 + row * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
+        if (lane == 0) {
+            o.target[row] = target;
+            if (target >= 0) {
+                if (o.scale) dot *= __half2float(__ushort_as_half(o.scale[target]));
+                if (o.bias) dot += __half2float(__ushort_as_half(o.bias[target]));
+            }
+            o.logit2[row] = dot * pg::LOG2E;
+        }
         return;
     }
     const uint32_t cta = blockIdx.x - o.hidden_ctas;
     const uint32_t plus = o.bf16 ? 0x3F80u : 0x3C00u;
-    const size_t items = (size_t)o.vocab * chunks, words = ((size_t)o.vocab * o.D + 31) / 32;
+    const size_t items = (size_t)o.vocab * chunks;
     float top = 0.0f;
     for (size_t item = (size_t)cta * THREADS + threadIdx.x; item < items; item += (size_t)WEIGHT_CTAS * THREADS) {
         const size_t v = item >> 32 ? item / chunks : (uint32_t)item / chunks;
         const uint32_t c = (uint32_t)(item - v * chunks) * 8;
         uint32_t w[4] = {};
         if (o.bits) {
-            const size_t bit = v * o.D + c;
-            uint32_t signs = o.bits[bit >> 5] >> (bit & 31);
-            if ((bit & 31) > 24 && (bit >> 5) + 1 < words) signs |= o.bits[(bit >> 5) + 1] << (32 - (bit & 31));
+            const uint32_t signs = signs8(o.bits, v * o.D + c, words);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (c + e < o.D) w[e >> 1] |= (plus | ((signs >> e) & 1u ? 0u : 0x8000u)) << (16 * (e & 1));
@@ -271,7 +314,7 @@ struct HeadRows {
     const float2* part;
     uint32_t rows, whole_rows, m_tiles, n_tiles, piece_tiles, slots, pairs;
     const int32_t* target;
-    const float* target_logit;
+    const float* logit2;
     float *lse2, *row_loss;
     const float* scale_max;   // null: dense weights
     float* factors;           // 2^k, 2^-k * loss_scale
@@ -296,33 +339,45 @@ head_rows_kernel(const HeadRows o) {
             o.factors[1] = exp2f((float)-k) * o.loss_scale;
         }
     }
-    const uint32_t row = blockIdx.x * 128 + threadIdx.x;
-    if (row >= o.rows) return;
-    const int32_t target = o.target[row];
-    if (target < 0) {
-        o.lse2[row] = INFINITY;
-        o.row_loss[row] = target == -1 ? 0.0f : NAN;
-        return;
-    }
+    // eight lanes to a row
+    const uint32_t row = blockIdx.x * 16 + (threadIdx.x >> 3), lane = threadIdx.x & 7;
+    if (row >= o.whole_rows) return;
     const uint32_t m = row / pg::BM;
     float top = -INFINITY, sum = 0.0f;
+    const auto add = [&](float t, float s) {
+        if (t > top) {
+            sum = sum * exp2f(top - t) + s;
+            top = t;
+        } else if (s != 0.0f) {   // (NaN too)
+            sum += s * exp2f(t - top);
+        }
+    };
     for (uint32_t first = 0, piece = 0; first < o.n_tiles; first += o.piece_tiles, ++piece) {
         const uint32_t width = min(o.piece_tiles, o.n_tiles - first);
         const pg::Share share = pg::share_of(o.m_tiles * width, o.pairs);
         const uint32_t slots = share.owner(m * width + width - 1) - share.owner(m * width) + 1;
-        for (uint32_t i = 0; i < slots * 4; ++i) {
-            const float2 t = o.part[((size_t)piece * o.slots * 4 + i) * o.whole_rows + row];
-            if (t.x > top) {
-                sum = sum * exp2f(top - t.x) + t.y;
-                top = t.x;
-            } else if (t.y != 0.0f) {   // (NaN too)
-                sum += t.y * exp2f(t.x - top);
-            }
+        const float2* part = o.part + (size_t)piece * o.slots * 4 * o.whole_rows + row;
+        for (uint32_t i = lane; i < slots * 4; i += 8) {
+            const float2 t = part[(size_t)i * o.whole_rows];
+            add(t.x, t.y);
         }
     }
+#pragma unroll
+    for (int k = 4; k > 0; k >>= 1) {   // (within a row's lanes, in a fixed order)
+        const float t = __shfl_xor_sync(0xffffffffu, top, k), s = __shfl_xor_sync(0xffffffffu, sum, k);
+        const float a = top, b = sum;
+        const bool mine_first = !(lane & k);
+        top = mine_first ? a : t;
+        sum = mine_first ? b : s;
+        add(mine_first ? t : a, mine_first ? s : b);
+    }
+    if (lane || row >= o.rows) return;
+    const int32_t target = o.target[row];
+    const float logit2 = o.logit2[row];
+    add(logit2, 1.0f);
     const float lse2 = top + log2f(sum);
-    o.lse2[row] = lse2;
-    o.row_loss[row] = (lse2 - o.target_logit[row]) * LN2;
+    o.lse2[row] = target >= 0 ? lse2 : INFINITY;
+    o.row_loss[row] = target >= 0 ? (lse2 - logit2) * LN2 : target == -1 ? 0.0f : NAN;
 }
 
 // The columns' sums of a piece out of their parts, times loss_scale.
@@ -424,6 +479,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     o.D = (uint32_t)D;
     o.Dp = (uint32_t)p.Dp;
     o.vocab = (uint32_t)V;
+    o.logit2 = reinterpret_cast<float*>(ws + p.logit);
     o.labels = h.labels;
     o.ignore_id = h.ignore_id;
     o.h16 = reinterpret_cast<uint16_t*>(ws + p.h16);
@@ -431,9 +487,10 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     o.bits = h.bits;
     o.dense = static_cast<const uint16_t*>(h.weight);
     o.scale = h.scale;
+    o.bias = h.bias;
     o.w16 = as_is ? nullptr : reinterpret_cast<uint16_t*>(ws + p.w16);
     o.scale_max = reinterpret_cast<float*>(ws + p.scale_max);
-    o.hidden_ctas = (uint32_t)ceil_div(rows * (p.Dp / 8), THREADS);
+    o.hidden_ctas = (uint32_t)ceil_div(rows, THREADS / 32);
     o.bf16 = bf16;
     const unsigned grid = o.hidden_ctas + (as_is ? 0 : WEIGHT_CTAS);
     if (h.hidden_f32) s.chain("head_operands", head_operands_kernel<float>, grid, THREADS, 0, o);
@@ -450,7 +507,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     q.piece_tiles = p.lse_tiles;
     q.slots = p.lse_slots;
     q.row_part = reinterpret_cast<float2*>(ws + p.row_part);
-    q.target_logit = reinterpret_cast<float*>(ws + p.logit);
+    q.logit2 = o.logit2;
     q.lse2 = reinterpret_cast<float*>(ws + p.lse2);
     float* factors = reinterpret_cast<float*>(ws + p.factors);
     launch<pg::LSE, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
@@ -465,13 +522,13 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     r.slots = p.lse_slots;
     r.pairs = p.pairs;
     r.target = o.target;
-    r.target_logit = q.target_logit;
+    r.logit2 = o.logit2;
     r.lse2 = reinterpret_cast<float*>(ws + p.lse2);
     r.row_loss = h.row_loss;
     r.scale_max = h.bits ? o.scale_max : nullptr;
     r.factors = factors;
     r.loss_scale = h.loss_scale;
-    s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 128), 128, 0, r);
+    s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 16), 128, 0, r);
 
     uint16_t* grad = reinterpret_cast<uint16_t*>(ws + p.grad);
     for (size_t piece = 0; piece < p.pieces; ++piece) {
@@ -483,13 +540,13 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
         g.scale = q.scale ? q.scale + v0 : nullptr;
         g.bias = q.bias ? q.bias + v0 : nullptr;
         g.factor = factors;
-        g.grad = grad;
         g.pitch = (uint32_t)p.piece;
         g.col_part = reinterpret_cast<float*>(ws + p.col_part);
         Operand wp = weight;
         wp.data = static_cast<const uint16_t*>(w16) + v0 * weight.stride;
         wp.rows = width;
-        launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs);
+        const CUtensorMap grad_map = map_of(grad, rows, p.piece, p.piece, 16, bf16);
+        launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
         if (h.g_bias || h.g_scale)
             s.chain("head_columns", head_columns_kernel, (unsigned)ceil_div(width, 256), 256, 0, static_cast<const float*>(g.col_part), g.pitch,
                     (uint32_t)p.m_tiles, n_tiles, p.pairs, (uint32_t)width, h.loss_scale, h.g_scale ? h.g_scale + v0 : nullptr,

@@ -7,11 +7,14 @@
 //    B into its own ring of shared memory; the even CTA issues the products, each CTA finds its 128 rows in its own TMEM.
 //    ACCS = 1: two accumulators take turns, the epilogue drains one while the other fills.  ACCS = 2: one of 512 columns, every
 //    element of A is fetched once for 512 columns; for products whose K is long beside the epilogue.
-//  * Warp 0 fetches, warp 1 multiplies, 16 warps are the epilogue: four to a TMEM lane quarter, 64 columns each.
+//  * Warp 0 fetches, warp 1 multiplies, 16 warps are the epilogue: four to a TMEM lane quarter, 64 columns each, with 96 registers
+//    to a thread.
 //  * The grid is persistent; which tiles a pair has follows from its number alone (Work below), so all sums have a fixed order.
 //
 // Epilogues:
-//   LSE    z = scale * acc + bias: running maximum and sum of exp over the columns, per row and quarter of the columns
+//   LSE    z = scale * acc + bias: running maximum and sum of exp over the columns but the target's, per row and quarter of the
+//          columns.  (The target's logit, whose terms have one sign where a model has learnt anything, is computed with rounding
+//          elsewhere: the loss is the difference of two large numbers, and what the tensor cores cut off would stay in it.)
 //   GRAD   g = softmax(z) - onehot, by rows as the 16-bit operand g * scale * 2^k of the products that follow, and by columns the
 //          f32 sums of g and g * acc
 //   STORE  alpha * acc in 16 bits, or into an f32 accumulator, or as one of several partial sums
@@ -36,18 +39,20 @@ constexpr uint32_t OPERAND_BYTES = 128 * BK * 2;        // one CTA's 128 rows of
 constexpr uint32_t EPI_WARPS = 16;
 constexpr int THREADS = 64 + 32 * (int)EPI_WARPS;
 constexpr uint32_t MAX_STAGES = 6, SMEM_LIMIT = 227 * 1024;
-constexpr uint32_t STAGING_BYTES = 16 * 128;            // per epilogue warp: 16 rows of 64 16-bit outputs
-constexpr uint32_t COLUMN_BYTES = 3 * 64 * 4;           // per epilogue warp: its columns' constants
+// per epilogue warp
+constexpr uint32_t STAGING_BYTES = 16 * 128;            // 16 rows of 64 16-bit outputs; GRAD has two of them
+constexpr uint32_t COLUMN_BYTES = 3 * 64 * 4;           // constants of its columns
+constexpr uint32_t ROW_BYTES = 2 * 3 * 32 * 4;          // GRAD: what its rows need, of this tile and of the next
 constexpr uint32_t SUM_BLOCKS = 16;                     // k-blocks between two rounded additions
 
 struct Maps {
     CUtensorMap a, b;
+    CUtensorMap out;           // GRAD: [M, pitch] in boxes of 64 columns x 16 rows
 };
 
 struct Params {
     uint32_t M, N, K;
     uint32_t a_mn, b_mn;       // operand with M (N) side by side
-    uint32_t bf16;
     uint32_t stages;
     uint32_t* status;
     // LSE, GRAD: columns [n_first, n_first + N) of the vocabulary
@@ -57,11 +62,10 @@ struct Params {
     uint32_t piece_tiles;      // LSE: column tiles that all pairs go through before the next ones
     uint32_t slots;            // LSE: partial sums per piece and row
     float2* row_part;          // LSE: [piece][slot][4][rows, whole tiles]
-    float* target_logit;       // LSE: [M] in units of log2 e
     const float* lse2;         // GRAD: [M] log2 of the sum of exp, +inf for a row that does not count
+    const float* logit2;       // GRAD: [M] the target's logit times log2 e
     const float* factor;       // GRAD: 2^k ; STORE: alpha
-    uint16_t* grad;            // GRAD: [M][pitch]
-    uint32_t pitch;
+    uint32_t pitch;            // GRAD: of col_part, whole tiles
     float* col_part;           // GRAD: [slot][8][2][pitch]
     // STORE, SUM
     uint32_t splits;           // of K
@@ -73,10 +77,11 @@ struct Params {
 };
 
 inline uint32_t stage_bytes(int accs) { return OPERAND_BYTES * (1 + accs); }
-inline uint32_t fixed_bytes(int epi) {
-    return 1024 /*alignment*/ + 256 /*barriers*/ + EPI_WARPS * ((epi == GRAD || epi == STORE ? STAGING_BYTES : 0u) +
-                                                               (epi == LSE || epi == GRAD ? COLUMN_BYTES : 0u));
+// Barriers first, then (on 1024 bytes) the ring, then what the epilogue warps have.
+constexpr uint32_t epi_bytes(int epi) {
+    return epi == GRAD ? 2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES : epi == STORE ? STAGING_BYTES : epi == LSE ? COLUMN_BYTES : 0u;
 }
+inline uint32_t fixed_bytes(int epi) { return 2 * 1024 /*barriers, alignment*/ + EPI_WARPS * epi_bytes(epi); }
 inline uint32_t stages_for(int epi, int accs) {
     const uint32_t fit = (SMEM_LIMIT - fixed_bytes(epi)) / stage_bytes(accs);
     return fit < MAX_STAGES ? fit : MAX_STAGES;
@@ -99,10 +104,10 @@ template <int EPI, int ACCS>
 struct Work {
     const Params& p;
     uint32_t pair, pairs, m_tiles, n_tiles, blocks;
-    uint32_t piece = 0, at = 0, end = 0, width = 0;   // LSE, GRAD
-    uint32_t job = 0;                                 // STORE, SUM
+    uint32_t piece = 0, left = 0, outer = 0, inner = 0, width = 0;   // LSE, GRAD: tiles left in the piece, (outer, inner < width) of the next
+    uint32_t job = 0;                                                // STORE, SUM
     // the tile
-    uint32_t m = 0, n = 0, k0 = 0, k1 = 0, split = 0;
+    uint32_t m = 0, n = 0, k0 = 0, k1 = 0, split = 0, in_piece = 0;
 
     __device__ Work(const Params& p_, uint32_t pair_, uint32_t pairs_) : p(p_), pair(pair_), pairs(pairs_) {
         m_tiles = (p.M + BM - 1) / BM;
@@ -110,34 +115,31 @@ struct Work {
         blocks = (p.K + BK - 1) / BK;
         k1 = blocks;
         job = pair;
-        if (EPI == LSE) open_piece();
-        if (EPI == GRAD) open(m_tiles * n_tiles);
+        if (EPI == LSE) open(m_tiles, min(p.piece_tiles, n_tiles));
+        if (EPI == GRAD) open(n_tiles, m_tiles);
     }
-    __device__ void open(uint32_t total) {
-        const Share s = share_of(total, pairs);
-        at = end = 0;
-        if (pair < s.pairs) { at = s.first(pair); end = s.first(pair + 1); }
-    }
-    __device__ void open_piece() {
-        width = min(p.piece_tiles, n_tiles - piece * p.piece_tiles);
-        open(m_tiles * width);
+    __device__ void open(uint32_t outers, uint32_t inners) {
+        const Share s = share_of(outers * inners, pairs);
+        width = inners;
+        left = 0;
+        if (pair < s.pairs) {
+            const uint32_t first = s.first(pair);
+            left = s.first(pair + 1) - first;
+            outer = first / inners;
+            inner = first - outer * inners;
+        }
     }
     __device__ bool next() {
-        if (EPI == LSE) {
-            while (at == end) {
-                if (++piece * p.piece_tiles >= n_tiles) return false;
-                open_piece();
+        if (EPI == LSE || EPI == GRAD) {
+            while (left == 0) {
+                if (EPI == GRAD || ++piece * p.piece_tiles >= n_tiles) return false;
+                open(m_tiles, min(p.piece_tiles, n_tiles - piece * p.piece_tiles));
             }
-            m = at / width;
-            n = piece * p.piece_tiles + at % width;
-            ++at;
-            return true;
-        }
-        if (EPI == GRAD) {
-            if (at == end) return false;
-            n = at / m_tiles;
-            m = at % m_tiles;
-            ++at;
+            m = EPI == LSE ? outer : inner;
+            n = EPI == LSE ? piece * p.piece_tiles + inner : outer;
+            in_piece = piece;
+            --left;
+            if (++inner == width) { inner = 0; ++outer; }
             return true;
         }
         if (job >= m_tiles * n_tiles * p.splits) return false;
@@ -165,6 +167,36 @@ __device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32])
         : "r"(taddr));
 }
 
+// the same, 32 columns
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+// Four 8 x 8 blocks of 16-bit pairs as the loads above leave them (a register each) to rows of 16 bytes; lane 8 b + i gives the
+// address of row i of block b.
+__device__ __forceinline__ void store_blocks(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem, int32_t x, int32_t y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem),
+                 "r"(x), "r"(y)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int LEFT>
+__device__ __forceinline__ void tma_store_read() {   // all but LEFT of this thread's stores have read their shared memory
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void copy_word(const void* to, const void* from, bool in) {   // global -> shared, or a zero
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(ptx::smem_u32(to)), "l"(from), "r"(in ? 4 : 0) : "memory");
+}
+
 // Descriptor of a tile with the M (N) elements side by side: atoms of 64 of them (128 bytes, swizzled) x 8 k, 1024 bytes apart
 // along k; the next 64 elements 64 k-rows, 8192 bytes, on.
 __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
@@ -176,8 +208,35 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16) {
-    if (bf16) {
+// two f32 operations per instruction
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 of_two(uint64_t r) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+    return v;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    if constexpr (BF16) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
@@ -201,35 +260,48 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile ui
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// The constants of this warp's 64 columns of the tile at n0: scale and bias times log2 e, scale * 2^k.  Columns past N have a
-// probability of 0.
-template <int EPI>
-__device__ __forceinline__ void load_columns(const Params& p, uint32_t n0, int lane, float* columns, float power) {
+// Scale and bias (FP16, two lanes' worth: columns lane and 32 + lane) of 64 columns from n0 on, on their way while the tile before
+// is worked on; and as the constants that the epilogue reads: both times log2 e, scale * 2^k.  Columns past N have a probability of 0.
+struct Columns {
+    float scale[2], bias[2];
+    __device__ void fetch(const Params& p, uint32_t n0, int lane) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t c = i * 32 + lane, n = n0 + c;
-        const bool in = n < p.N;
-        const float s = in ? half_at(p.scale, n, 1.0f) : 0.0f;
-        columns[c] = s * LOG2E;
-        columns[64 + c] = in ? half_at(p.bias, n, 0.0f) * LOG2E : -INFINITY;
-        if (EPI == GRAD) columns[128 + c] = s * power;
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t n = n0 + i * 32 + lane;
+            scale[i] = n < p.N ? half_at(p.scale, n, 1.0f) : 0.0f;
+            bias[i] = n < p.N ? half_at(p.bias, n, 0.0f) : -INFINITY;
+        }
     }
+    __device__ void keep(float* to, int lane, float power) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            to[i * 32 + lane] = scale[i] * LOG2E;
+            to[64 + i * 32 + lane] = bias[i] * LOG2E;
+            to[128 + i * 32 + lane] = scale[i] * power;
+        }
+    }
+};
+// The accumulator has been read: one arrival on the even CTA's barrier.  (With release at the scope of the cluster the arrival
+// waits for the warp's stores to memory, which this barrier says nothing of.)
+__device__ __forceinline__ void arrive_even(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-template <int EPI, int ACCS>
+template <int EPI, int ACCS, bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr uint32_t STAGE = OPERAND_BYTES * (1 + ACCS);
     const uint32_t STAGES = p.stages;
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);   // [STAGES] even CTA: both CTAs' bytes have landed
-    uint64_t* empty = full + MAX_STAGES;                                   // [STAGES] the products that read the stage are done
-    uint64_t* tmem_full = empty + MAX_STAGES;                              // [2] accumulator complete
-    uint64_t* tmem_empty = tmem_full + 2;                                  // [2] even CTA: drained in both CTAs
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem);   // [STAGES] even CTA: both CTAs' bytes have landed
+    uint64_t* empty = full + MAX_STAGES;                  // [STAGES] the products that read the stage are done
+    uint64_t* tmem_full = empty + MAX_STAGES;             // [2] accumulator complete
+    uint64_t* tmem_empty = tmem_full + 2;                 // [2] even CTA: drained in both CTAs
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
     uint32_t* s_error = tmem_slot + 1;
-    uint8_t* epi_smem = reinterpret_cast<uint8_t*>(full) + 256;
+    smem += 1024;
+    uint8_t* epi_smem = smem + STAGES * STAGE;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = ptx::cluster_ctarank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -311,7 +383,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     } else if (warp == 1) {
         // ------------------------------------------------------ products (even CTA)
         if (rank == 0 && ptx::elect_one()) {
-            const uint32_t idesc = ptx::idesc_f16(p.bf16, p.bf16, BM, BN) | p.a_mn << 15 | p.b_mn << 16;
+            const uint32_t idesc = ptx::idesc_f16(BF16, BF16, BM, BN) | p.a_mn << 15 | p.b_mn << 16;
             const uint32_t a_step = p.a_mn ? 2048u : 32u, b_step = p.b_mn ? 2048u : 32u;   // 16 k
             const uint32_t ring = ptx::smem_u32(smem);
             uint32_t it = 0, done = 0;   // k-blocks, accumulators
@@ -358,8 +430,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         // ------------------------------------------------------ epilogue (both CTAs, own rows)
         const uint32_t quarter = warp & 3, group = (uint32_t)(warp - 2) >> 2, mine = warp - 2;
         const uint32_t empty_even = ptx::cluster_map(tmem_empty, 0);
-        uint8_t* staging = epi_smem + mine * STAGING_BYTES;
-        float* columns = reinterpret_cast<float*>(epi_smem + (EPI == GRAD ? EPI_WARPS * STAGING_BYTES : 0u) + mine * COLUMN_BYTES);
+        constexpr uint32_t STAGINGS = EPI == GRAD ? 2 : EPI == STORE ? 1 : 0;
+        uint8_t* staging = epi_smem + mine * STAGINGS * STAGING_BYTES;   // on 1024 bytes
+        float* columns = reinterpret_cast<float*>(epi_smem + EPI_WARPS * STAGINGS * STAGING_BYTES + mine * COLUMN_BYTES);
         uint32_t done = 0;
         // Waits for the next accumulator; false: leave.  The loads are warp-collective: the whole warp decides.
         const auto filled = [&](uint32_t* taddr) {
@@ -376,7 +449,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         const auto drained = [&]() {
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_cluster(empty_even + 8 * (done % BUFFERS));
+            if (lane == 0) arrive_even(empty_even + 8 * (done % BUFFERS));
             ++done;
         };
         const uint32_t q2 = (lane & 3) * 2, r0 = lane >> 2;   // of the 16 x 64 form: first column of a pair, first row
@@ -393,20 +466,25 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 const size_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
                 p.row_part[(((size_t)piece_now * p.slots + slot) * 4 + group) * rows + row] = make_float2(top, sum);
             };
-            while (work.next()) {
+            Columns ahead;
+            bool more = work.next();
+            if (more) ahead.fetch(p, work.n * BN + group * 64, lane);
+            while (more) {
                 const uint32_t n0 = work.n * BN + group * 64;
-                if (work.m != m_now || work.piece != piece_now) {
+                if (work.m != m_now || work.in_piece != piece_now) {
                     leave();
                     m_now = work.m;
-                    piece_now = work.piece;
+                    piece_now = work.in_piece;
                     top = -INFINITY;
                     sum = 0.0f;
                     const uint32_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
                     target = row < p.M ? p.target[row] : -1;
                 }
                 __syncwarp();
-                load_columns<EPI>(p, n0, lane, columns, 0.0f);
+                ahead.keep(columns, lane, 0.0f);
                 __syncwarp();
+                more = work.next();
+                if (more) ahead.fetch(p, work.n * BN + group * 64, lane);
                 uint32_t taddr;
                 if (!filled(&taddr)) break;
 #pragma unroll
@@ -416,32 +494,40 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     ptx::tmem_ld_wait();
                     if (c == 1) drained();
                     const int32_t hit = target - (int32_t)(n0 + c * 32);
-                    float z[32], best = -INFINITY;
+                    uint64_t z[16];
+                    float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 s = *reinterpret_cast<const float4*>(columns + c * 32 + i);
-                        const float4 b = *reinterpret_cast<const float4*>(columns + 64 + c * 32 + i);
-                        z[i] = fmaf(__uint_as_float(r[i]), s.x, b.x);
-                        z[i + 1] = fmaf(__uint_as_float(r[i + 1]), s.y, b.y);
-                        z[i + 2] = fmaf(__uint_as_float(r[i + 2]), s.z, b.z);
-                        z[i + 3] = fmaf(__uint_as_float(r[i + 3]), s.w, b.w);
+                    for (int i = 0; i < 16; i += 2) {
+                        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(columns + c * 32 + i * 2);
+                        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(columns + 64 + c * 32 + i * 2);
+                        z[i] = fma2((uint64_t)r[i * 2 + 1] << 32 | r[i * 2], s.x, b.x);
+                        z[i + 1] = fma2((uint64_t)r[i * 2 + 3] << 32 | r[i * 2 + 2], s.y, b.y);
                     }
-                    if (hit >= 0 && hit < 32) {
+                    if (__any_sync(0xffffffffu, hit >= 0 && hit < 32)) {   // (by sums: as stores of elements z went to local memory)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (hit == i) p.target_logit[m_now * BM + rank * 128 + quarter * 32 + lane] = z[i];
+                        for (int i = 0; i < 16; ++i)
+                            z[i] = add2(z[i], two(hit == i * 2 ? -INFINITY : 0.0f, hit == i * 2 + 1 ? -INFINITY : 0.0f));
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) best = fmaxf(best, z[i]);
-                    if (best > top) {
-                        sum *= exp2_fast(top - best);   // top = -inf: 0 * 0
-                        top = best;
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 v = of_two(z[i]);
+                        best[i & 1] = fmaxf(best[i & 1], fmaxf(v.x, v.y));
                     }
-                    const float base = top == -INFINITY ? 0.0f : top;   // (a NaN among z makes the sum one)
-                    float here[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    best[0] = fmaxf(best[0], best[1]);
+                    if (best[0] > top) {
+                        sum *= exp2_fast(top - best[0]);   // top = -inf: 0 * 0
+                        top = best[0];
+                    }
+                    const float base = top == -INFINITY ? 0.0f : -top;   // (a NaN among z makes the sum one)
+                    const uint64_t base2 = two(base, base);
+                    uint64_t here[2] = {0, 0};
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) here[i & 3] += exp2_fast(z[i] - base);
-                    sum += (here[0] + here[1]) + (here[2] + here[3]);
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 v = of_two(add2(z[i], base2));
+                        here[i & 1] = add2(here[i & 1], two(exp2_fast(v.x), exp2_fast(v.y)));
+                    }
+                    const float2 all = of_two(add2(here[0], here[1]));
+                    sum += all.x + all.y;
                 }
             }
             leave();
@@ -449,95 +535,131 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             const float power = *p.factor;
             const Share all = share_of(work.m_tiles * work.n_tiles, pairs);
             uint32_t n_now = 0xFFFFFFFFu;
-            float g_sum[16], ga_sum[16];
+            uint64_t g_sum[8], ga_sum[8];   // of column pairs 8 j + q2
 #pragma unroll
-            for (int i = 0; i < 16; ++i) g_sum[i] = ga_sum[i] = 0.0f;
+            for (int j = 0; j < 8; ++j) g_sum[j] = ga_sum[j] = 0;
             const auto leave = [&]() {   // the sums of 32 rows: over the lanes that share columns, then out
                 if (n_now == 0xFFFFFFFFu) return;
                 const uint32_t slot = pair - all.owner(n_now * work.m_tiles);
                 float* to = p.col_part + (((size_t)slot * 8 + rank * 4 + quarter) * 2) * p.pitch + n_now * BN + group * 64 + q2;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float a = g_sum[i], b = ga_sum[i];
+                for (int j = 0; j < 8; ++j) {
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) {
-                        a += __shfl_xor_sync(0xffffffffu, a, o);
-                        b += __shfl_xor_sync(0xffffffffu, b, o);
+                        g_sum[j] = add2(g_sum[j], __shfl_xor_sync(0xffffffffu, g_sum[j], o));
+                        ga_sum[j] = add2(ga_sum[j], __shfl_xor_sync(0xffffffffu, ga_sum[j], o));
                     }
                     if (lane < 4) {
-                        to[(i >> 1) * 8 + (i & 1)] = a;
-                        to[p.pitch + (i >> 1) * 8 + (i & 1)] = b;
+                        *reinterpret_cast<uint64_t*>(to + j * 8) = g_sum[j];
+                        *reinterpret_cast<uint64_t*>(to + p.pitch + j * 8) = ga_sum[j];
                     }
-                    g_sum[i] = ga_sum[i] = 0.0f;
+                    g_sum[j] = ga_sum[j] = 0;
                 }
             };
-            while (work.next()) {
+            // What the rows need lies in shared memory, two tiles in turn; the next tile's is on its way while one is worked on: a
+            // word each of lse2, the target's logit and the target per lane.
+            float* row_smem = reinterpret_cast<float*>(epi_smem + EPI_WARPS * (2 * STAGING_BYTES + COLUMN_BYTES) + mine * ROW_BYTES);
+            const auto fetch = [&](uint32_t turn) {
+                const uint32_t row = work.m * BM + rank * 128 + quarter * 32 + lane;
+                const bool in = row < p.M;
+                float* to = row_smem + turn * 96 + lane;
+                copy_word(to, p.lse2 + (in ? row : 0), in);
+                copy_word(to + 32, p.logit2 + (in ? row : 0), in);
+                copy_word(to + 64, p.target + (in ? row : 0), in);
+            };
+            const uint32_t blocks_at = ptx::smem_u32(staging) + ((lane >> 3) & 1) * 1024 + (lane & 7) * 128;   // of store_blocks: block b has
+            const uint32_t block_piece = lane >> 4;                                                           // rows 8 (b % 2) .., piece b / 2
+            uint32_t turn = 0;
+            bool more = work.next();
+            if (more) fetch(0);
+            while (more) {
                 const uint32_t n0 = work.n * BN + group * 64, m0 = work.m * BM + rank * 128 + quarter * 32;
                 if (work.n != n_now) {
                     leave();
                     n_now = work.n;
                     __syncwarp();
-                    load_columns<EPI>(p, n0, lane, columns, power);
-                    __syncwarp();
+                    Columns c;
+                    c.fetch(p, n0, lane);
+                    c.keep(columns, lane, power);
                 }
-                float lse[4];
-                int32_t hit[4];
-                bool any = false;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t row = m0 + r0 + i * 8;
-                    lse[i] = row < p.M ? p.lse2[row] : INFINITY;
-                    hit[i] = (row < p.M ? p.target[row] : -1) - (int32_t)(p.n_first + n0);
-                    any |= hit[i] >= 0 && hit[i] < 64;
-                }
-                any = __any_sync(0xffffffffu, any);
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+                const float* rows = row_smem + turn * 96;
+                turn ^= 1;
+                const int32_t first = (int32_t)(p.n_first + n0);
+                const int32_t own = m0 + lane < p.M ? reinterpret_cast<const int32_t*>(rows)[64 + lane] - first : -1;
+                const bool any = __any_sync(0xffffffffu, own >= 0 && own < 64);
+                more = work.next();
+                if (more) fetch(turn);
                 uint32_t taddr;
                 if (!filled(&taddr)) break;
+                // 16 rows; TARGETS: the target of one of the warp's rows lies in its columns
                 const auto half = [&](int h, auto targets) {
-                    uint32_t r[32];
-                    tmem_ld_16x64(taddr + group * 64 + ((h * 16) << 16), r);
-                    ptx::tmem_ld_wait();
-                    if (h == 1) drained();
+                    uint32_t r[16];
+                    tmem_ld_16x32(taddr + group * 64 + ((h * 16) << 16), r);
+                    float lse[2], logit[2];
+                    int32_t at[2];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 s = *reinterpret_cast<const float2*>(columns + j * 8 + q2);
-                        const float2 b = *reinterpret_cast<const float2*>(columns + 64 + j * 8 + q2);
-                        const float2 k = *reinterpret_cast<const float2*>(columns + 128 + j * 8 + q2);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float a0 = __uint_as_float(r[j * 4 + i * 2]), a1 = __uint_as_float(r[j * 4 + i * 2 + 1]);
-                            float g0 = exp2_fast(fmaf(a0, s.x, b.x) - lse[h * 2 + i]), g1 = exp2_fast(fmaf(a1, s.y, b.y) - lse[h * 2 + i]);
-                            if (decltype(targets)::value) {
-                                if (hit[h * 2 + i] == j * 8 + (int)q2) g0 -= 1.0f;
-                                if (hit[h * 2 + i] == j * 8 + (int)q2 + 1) g1 -= 1.0f;
-                            }
-                            g_sum[j * 2] += g0;
-                            g_sum[j * 2 + 1] += g1;
-                            ga_sum[j * 2] = fmaf(g0, a0, ga_sum[j * 2]);
-                            ga_sum[j * 2 + 1] = fmaf(g1, a1, ga_sum[j * 2 + 1]);
-                            // 16-byte piece j of the row at j ^ (row % 8): neither side meets a bank conflict
-                            *reinterpret_cast<uint32_t*>(staging + (r0 + i * 8) * 128 + ((j ^ r0) << 4) + (lane & 3) * 4) =
-                                pack16(g0 * k.x, g1 * k.y, p.bf16);
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t row = h * 16 + i * 8 + r0;
+                        lse[i] = m0 + row < p.M ? -rows[row] : -INFINITY;
+                        if (decltype(targets)::value) {
+                            logit[i] = rows[32 + row] + lse[i];
+                            at[i] = reinterpret_cast<const int32_t*>(rows)[64 + row] - first - (int32_t)q2;
+                            if (m0 + row >= p.M) at[i] = -1;
                         }
                     }
+                    const uint64_t l[2] = {two(lse[0], lse[0]), two(lse[1], lse[1])};
+                    const uint32_t to = blocks_at + h * STAGING_BYTES;
+                    if (lane == 0) tma_store_read<1>();   // the store before the last has read this half
                     __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t row = i * 4 + (lane >> 3), piece = lane & 7;
-                        const uint4 v = *reinterpret_cast<const uint4*>(staging + row * 128 + ((piece ^ (row & 7)) << 4));
-                        const uint32_t gm = m0 + h * 16 + row;
-                        if (gm < p.M) *reinterpret_cast<uint4*>(p.grad + (size_t)gm * p.pitch + n0 + piece * 8) = v;
+                    for (int j = 0; j < 8; j += 2) {
+                        if (j == 4) tmem_ld_16x32(taddr + group * 64 + 32 + ((h * 16) << 16), r);
+                        if (j == 0 || j == 4) ptx::tmem_ld_wait();
+                        if (j == 4 && h == 1) drained();
+                        uint32_t w[4];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint64_t s = *reinterpret_cast<const uint64_t*>(columns + (j + u) * 8 + q2);
+                            const uint64_t b = *reinterpret_cast<const uint64_t*>(columns + 64 + (j + u) * 8 + q2);
+                            const uint64_t k = *reinterpret_cast<const uint64_t*>(columns + 128 + (j + u) * 8 + q2);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint64_t a = (uint64_t)r[(j + u) % 4 * 4 + i * 2 + 1] << 32 | r[(j + u) % 4 * 4 + i * 2];
+                                const float2 e = of_two(add2(fma2(a, s, b), l[i]));
+                                float2 gv = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                                if (decltype(targets)::value) {
+                                    if (at[i] == (j + u) * 8) gv.x = exp2_fast(logit[i]) - 1.0f;
+                                    if (at[i] == (j + u) * 8 + 1) gv.y = exp2_fast(logit[i]) - 1.0f;
+                                }
+                                const uint64_t g = two(gv.x, gv.y);
+                                g_sum[j + u] = add2(g_sum[j + u], g);
+                                ga_sum[j + u] = fma2(g, a, ga_sum[j + u]);
+                                const float2 o = of_two(mul2(g, k));
+                                w[u * 2 + i] = pack16<BF16>(o.x, o.y);
+                            }
+                        }
+                        // 16-byte piece c of row r at c ^ (r % 8), as the copy below reads it; no bank conflicts
+                        store_blocks(to + (((j + block_piece) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
                     }
+                    ptx::fence_proxy_async_smem();
                     __syncwarp();
+                    if (lane == 0) {
+                        if (m0 + h * 16 < p.M) tma_store_2d(&maps.out, ptx::smem_u32(staging) + h * STAGING_BYTES, (int32_t)n0, (int32_t)(m0 + h * 16));
+                        else asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // (the groups stay in turn)
+                    }
                 };
-                if (any) {
-                    half(0, std::true_type{});
-                    half(1, std::true_type{});
-                } else {
-                    half(0, std::false_type{});
-                    half(1, std::false_type{});
+                // one copy of the code for both halves: with two the registers ran out
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    if (any) half(h, std::true_type{});
+                    else half(h, std::false_type{});
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (lane == 0) tma_store_done();
+            __syncwarp();
             leave();
         } else if constexpr (EPI == STORE) {
             const float alpha = p.factor ? *p.factor : 1.0f;
@@ -591,7 +713,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
                             *reinterpret_cast<uint32_t*>(staging + (r0 + i * 8) * 128 + ((j ^ r0) << 4) + (lane & 3) * 4) =
-                                pack16(v[j * 4 + i * 2] * alpha, v[j * 4 + i * 2 + 1] * alpha, p.bf16);
+                                pack16<BF16>(v[j * 4 + i * 2] * alpha, v[j * 4 + i * 2 + 1] * alpha);
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {

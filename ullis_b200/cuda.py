@@ -22,7 +22,7 @@ import threading
 
 import numpy as np
 
-from .device import DeviceOps, HeadGrad, Tape  # noqa: F401
+from .device import DeviceOps, HeadGrad, Tape, declare  # noqa: F401
 from .errors import (ERR_ARG, ERR_CHECKPOINT, ERR_CUDA, ERR_DEVICE_CHECK, ERR_NCCL, ERR_NOMEM, ERR_SHAPE,  # noqa: F401
                      ERR_TIMEOUT, ERR_TOKEN, OK, UllisCudaError)
 
@@ -99,6 +99,7 @@ def load_library() -> C.CDLL:
         lib.ullis_cuda_host_free.argtypes = [C.c_void_p]
         lib.ullis_cuda_generate_state_time.restype = C.c_size_t
         lib.ullis_cuda_generate_state_time.argtypes = [C.c_void_p]
+        declare(lib)
         _LIB = lib
     return _LIB
 

@@ -32,24 +32,44 @@ class HeadGrad(NamedTuple):
     bias: object
 
 
-_DTYPES = None
+_TORCH, _DTYPES, _16, _RAW_STREAM = None, None, None, None
 
 
 def _torch():
-    import torch
+    global _TORCH, _DTYPES, _16, _RAW_STREAM
+    if _TORCH is None:
+        import torch
 
-    global _DTYPES
-    if _DTYPES is None:
         _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    return torch
+        _16 = (torch.float16, torch.bfloat16)
+        _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _TORCH = torch
+    return _TORCH
 
 
-def _z(n):
-    return C.c_size_t(n)
+_V, _Z, _I, _F, _U = C.c_void_p, C.c_size_t, C.c_int32, C.c_float, C.c_uint32
+#: Argument types of the entry points: with them ctypes takes plain numbers, a third of the time of a call of twenty arguments.
+_ARGTYPES = {
+    "tape_pack": (_V, _V, _I, _V, _Z, _Z, _Z, _V, _V),
+    "tape_unpack": (_V, _V, _I, _V, _V, _Z, _Z, _V, _Z),
+    "tape_layer_norm": (_V, _V, _I, _V, _Z, _V, _V, _Z, _Z, _V, _V, _V),
+    "tape_layer_norm_backward_workspace": (_V, _Z, _Z, _V),
+    "tape_layer_norm_backward": (_V, _V, _I, _V, _V, _V, _Z, _V, _V, _Z, _Z, _Z, _V, _V, _V, _V, _Z),
+    "tape_weight_grad_workspace": (_V, _Z, _Z, _Z, _V),
+    "tape_weight_grad": (_V, _V, _I, _V, _V, _V, _Z, _Z, _Z, _Z, _V, _V, _Z),
+    "head_ce_grad_workspace": (_V, _Z, _Z, _Z, _V),
+    "head_ce_grad": (_V, _V, _I, _V, _Z, _V, _V, _V, _V, _V, _U, _Z, _Z, _Z, _Z, _F, _V, _V, _V, _V, _V, _V, _Z),
+}
+
+
+def declare(lib) -> None:
+    for name, types in _ARGTYPES.items():
+        getattr(lib, "ullis_cuda_" + name).argtypes = types
 
 
 def _p(t):
-    return C.c_void_p(None if t is None else t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _shape_error(name, got, expected):
@@ -114,29 +134,31 @@ class DeviceOps:
             _shape_error("exponents", exponents.shape, (rows, -(-channels // 32)))
         return codes, exponents, rows, channels
 
-    def _stream_of(self):
-        return C.c_void_p(_torch().cuda.current_stream(self.device).cuda_stream)
-
-    def _new(self, shape, dtype):
-        torch = _torch()
-        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", self.device))
-
-    def _workspace(self, fn, *sizes):
-        need = C.c_size_t(0)
-        rc = fn(self._h, *sizes, C.byref(need))
-        if rc != OK:
-            raise UllisCudaError(rc, self._lib.ullis_cuda_last_error(None).decode())
-        return self._new((max(need.value, 1),), _torch().uint8), _z(need.value)
+    def _workspace(self, like, name, *sizes):
+        """(bytes of workspace from torch's allocator, how many); the size is asked for once per shape."""
+        try:
+            need = self._workspace_bytes[name, sizes]
+        except (AttributeError, KeyError):
+            value = C.c_size_t(0)
+            rc = getattr(self._lib, f"ullis_cuda_{name}_workspace")(self._h, *sizes, C.byref(value))
+            if rc != OK:
+                raise UllisCudaError(rc, self._lib.ullis_cuda_last_error(None).decode()) from None
+            need = value.value
+            known = self.__dict__.setdefault("_workspace_bytes", {})
+            if len(known) >= 4096:
+                known.clear()
+            known[name, sizes] = need
+        return like.new_empty((need,), dtype=_TORCH.uint8), need
 
     # ------------------------------------------------------------------------------------------ the 8-bit tape
     def tape_pack(self, x) -> Tape:
         """x [..., channels] (float32, float16, bfloat16) in 8 bits: one exponent per 32 channels of a row."""
         torch = _torch()
-        x, rows, channels, stride = self._matrix(x, "x", tuple(_DTYPES))
-        codes = self._new(x.shape, torch.int8)
-        exponents = self._new((rows, -(-channels // 32)), torch.uint8)
-        self._check(self._lib.ullis_cuda_tape_pack(self._h, self._stream_of(), C.c_int32(_DTYPES[x.dtype]), _p(x), _z(stride),
-                                                   _z(rows), _z(channels), _p(codes), _p(exponents)))
+        x, rows, channels, stride = self._matrix(x, "x", _DTYPES)
+        codes = x.new_empty(x.shape, dtype=torch.int8)
+        exponents = x.new_empty((rows, -(-channels // 32)), dtype=torch.uint8)
+        self._check(self._lib.ullis_cuda_tape_pack(self._h, _RAW_STREAM(self.device), _DTYPES[x.dtype], _p(x), stride,
+                                                   rows, channels, _p(codes), _p(exponents)))
         return Tape(codes, exponents)
 
     def tape_unpack(self, tape, dtype):
@@ -145,23 +167,23 @@ class DeviceOps:
         codes, exponents, rows, channels = self._tape(tape)
         if dtype not in _DTYPES:
             raise UllisCudaError(ERR_ARG, f"a tape does not unpack to {dtype}")
-        x = self._new(codes.shape, dtype)
-        self._check(self._lib.ullis_cuda_tape_unpack(self._h, self._stream_of(), C.c_int32(_DTYPES[dtype]), _p(codes), _p(exponents),
-                                                     _z(rows), _z(channels), _p(x), _z(channels)))
+        x = codes.new_empty(codes.shape, dtype=dtype)
+        self._check(self._lib.ullis_cuda_tape_unpack(self._h, _RAW_STREAM(self.device), _DTYPES[dtype], _p(codes), _p(exponents),
+                                                     rows, channels, _p(x), channels))
         return x
 
     def tape_layer_norm(self, x, weight, bias):
         """(LayerNorm(x), tape of x): weight and bias float16 [channels]; y has the shape and type of x."""
         torch = _torch()
-        x, rows, channels, stride = self._matrix(x, "x", tuple(_DTYPES))
+        x, rows, channels, stride = self._matrix(x, "x", _DTYPES)
         weight = self._vector(weight, "weight", (torch.float16,), channels)
         bias = self._vector(bias, "bias", (torch.float16,), channels)
-        y = self._new(x.shape, x.dtype)
-        codes = self._new(x.shape, torch.int8)
-        exponents = self._new((rows, -(-channels // 32)), torch.uint8)
+        y = x.new_empty(x.shape)
+        codes = x.new_empty(x.shape, dtype=torch.int8)
+        exponents = x.new_empty((rows, -(-channels // 32)), dtype=torch.uint8)
         self._check(self._lib.ullis_cuda_tape_layer_norm(
-            self._h, self._stream_of(), C.c_int32(_DTYPES[x.dtype]), _p(x), _z(stride), _p(weight), _p(bias), _z(rows),
-            _z(channels), _p(y), _p(codes), _p(exponents)))
+            self._h, _RAW_STREAM(self.device), _DTYPES[x.dtype], _p(x), stride, _p(weight), _p(bias), rows,
+            channels, _p(y), _p(codes), _p(exponents)))
         return y, Tape(codes, exponents)
 
     def tape_layer_norm_backward(self, tape, gy, weight, residual=None):
@@ -169,7 +191,7 @@ class DeviceOps:
         the gradient that comes past the norm, added to it; the gradients of weight and bias are float32."""
         torch = _torch()
         codes, exponents, rows, channels = self._tape(tape)
-        gy, g_rows, g_channels, stride = self._matrix(gy, "gy", tuple(_DTYPES))
+        gy, g_rows, g_channels, stride = self._matrix(gy, "gy", _DTYPES)
         if (g_rows, g_channels) != (rows, channels):
             _shape_error("gy", gy.shape, codes.shape)
         weight = self._vector(weight, "weight", (torch.float16,), channels)
@@ -178,28 +200,29 @@ class DeviceOps:
             residual, r_rows, r_channels, r_stride = self._matrix(residual, "residual", (gy.dtype,))
             if (r_rows, r_channels) != (rows, channels):
                 _shape_error("residual", residual.shape, gy.shape)
-        gx = self._new(gy.shape, gy.dtype)
-        g = self._new((2, channels), torch.float32)
-        work, size = self._workspace(self._lib.ullis_cuda_tape_layer_norm_backward_workspace, _z(rows), _z(channels))
+        gx = gy.new_empty(gy.shape)
+        g = gy.new_empty((2, channels), dtype=torch.float32)
+        at = g.data_ptr()
+        work, size = self._workspace(gy, "tape_layer_norm_backward", rows, channels)
         self._check(self._lib.ullis_cuda_tape_layer_norm_backward(
-            self._h, self._stream_of(), C.c_int32(_DTYPES[gy.dtype]), _p(codes), _p(exponents), _p(gy), _z(stride), _p(weight),
-            _p(residual), _z(r_stride), _z(rows), _z(channels), _p(gx), C.c_void_p(g.data_ptr()),
-            C.c_void_p(g.data_ptr() + 4 * channels), _p(work), size))
-        return gx, g[0], g[1]
+            self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], _p(codes), _p(exponents), _p(gy), stride, _p(weight),
+            _p(residual), r_stride, rows, channels, _p(gx), at,
+            at + 4 * channels, _p(work), size))
+        return (gx, *g.unbind(0))
 
     def tape_weight_grad(self, tape, gy):
         """Gradient of a linear's weights, float32 [out, in]: gy [..., out] (float16, bfloat16) transposed times what the tape
         of the linear's input stands for."""
         torch = _torch()
         codes, exponents, rows, channels = self._tape(tape)
-        gy, g_rows, out, stride = self._matrix(gy, "gy", (torch.float16, torch.bfloat16))
+        gy, g_rows, out, stride = self._matrix(gy, "gy", _16)
         if g_rows != rows:
             _shape_error("gy", gy.shape, (rows, out))
-        g = self._new((out, channels), torch.float32)
-        work, size = self._workspace(self._lib.ullis_cuda_tape_weight_grad_workspace, _z(rows), _z(channels), _z(out))
+        g = gy.new_empty((out, channels), dtype=torch.float32)
+        work, size = self._workspace(gy, "tape_weight_grad", rows, channels, out)
         self._check(self._lib.ullis_cuda_tape_weight_grad(
-            self._h, self._stream_of(), C.c_int32(_DTYPES[gy.dtype]), _p(codes), _p(exponents), _p(gy), _z(stride), _z(rows),
-            _z(channels), _z(out), _p(g), _p(work), size))
+            self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], _p(codes), _p(exponents), _p(gy), stride, rows,
+            channels, out, _p(g), _p(work), size))
         return g
 
     # ------------------------------------------------------------------------------------------ head
@@ -213,7 +236,7 @@ class DeviceOps:
         `weight` [vocab, channels] in hidden's type and no scale.  bias float16 [vocab] or None.  Gradients are of
         loss_scale * sum of row_loss; that of a packed weight is of the +/-1 values."""
         torch = _torch()
-        hidden, rows, channels, stride = self._matrix(hidden, "hidden", (torch.float16, torch.bfloat16))
+        hidden, rows, channels, stride = self._matrix(hidden, "hidden", _16)
         labels = self._vector(labels, "labels", (torch.int32,), rows)
         if time is None:
             time = hidden.shape[-2] if hidden.dim() == 3 else max(rows, 1)
@@ -234,16 +257,16 @@ class DeviceOps:
             raise UllisCudaError(ERR_ARG, "ignore_id is not a 32-bit number")
         if not 0 < int(time) < 1 << 31 or rows % int(time):
             raise UllisCudaError(ERR_SHAPE, "rows must be a multiple of time")
-        row_loss = self._new((rows,), torch.float32)
-        g_hidden = self._new(hidden.shape, hidden.dtype)
-        g_weight = self._new((vocab, channels), hidden.dtype)
-        g_scale = None if scale is None else self._new((vocab,), torch.float32)
-        g_bias = None if bias is None else self._new((vocab,), torch.float32)
-        work, size = self._workspace(self._lib.ullis_cuda_head_ce_grad_workspace, _z(rows), _z(channels), _z(vocab))
+        row_loss = hidden.new_empty((rows,), dtype=torch.float32)
+        g_hidden = hidden.new_empty(hidden.shape)
+        g_weight = hidden.new_empty((vocab, channels))
+        g_scale = None if scale is None else hidden.new_empty((vocab,), dtype=torch.float32)
+        g_bias = None if bias is None else hidden.new_empty((vocab,), dtype=torch.float32)
+        work, size = self._workspace(hidden, "head_ce_grad", rows, channels, vocab)
         packed = scale is not None
         self._check(self._lib.ullis_cuda_head_ce_grad(
-            self._h, self._stream_of(), C.c_int32(_DTYPES[hidden.dtype]), _p(hidden), _z(stride), _p(weight if packed else None),
-            _p(None if packed else weight), _p(scale), _p(bias), _p(labels), C.c_uint32(ignore & 0xFFFFFFFF), _z(rows),
-            _z(int(time)), _z(channels), _z(vocab), C.c_float(loss_scale), _p(row_loss), _p(g_hidden), _p(g_weight), _p(g_scale),
+            self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], _p(hidden), stride, _p(weight if packed else None),
+            _p(None if packed else weight), _p(scale), _p(bias), _p(labels), ignore & 0xFFFFFFFF, rows,
+            int(time), channels, vocab, float(loss_scale), _p(row_loss), _p(g_hidden), _p(g_weight), _p(g_scale),
             _p(g_bias), _p(work), size))
         return HeadGrad(row_loss, g_hidden, g_weight, g_scale, g_bias)
