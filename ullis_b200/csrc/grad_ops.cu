@@ -143,7 +143,15 @@ combine_kernel(const float* __restrict__ partial, uint32_t splits, size_t n, con
             for (int e = 0; e < 4; ++e) if (i + e < n) v[e] += from[i + e];
         }
     };
-    for (uint32_t k = 0; k < splits; ++k) add(partial + k * n);
+    if (whole) {
+#pragma unroll 8
+        for (uint32_t k = 0; k < splits; ++k) {
+            const float4 t = *reinterpret_cast<const float4*>(partial + k * n + i);
+            v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+        }
+    } else {
+        for (uint32_t k = 0; k < splits; ++k) add(partial + k * n);
+    }
     if (accum && accum_read) add(accum);
     for (int e = 0; e < 4; ++e) {
         if (i + e >= n) break;
@@ -197,7 +205,7 @@ struct HeadOperands {
     uint32_t ignore_id;
     uint16_t* h16;
     int32_t* target;
-    float* logit2;              // target's logit times log2 e
+    float *target_acc, *logit2; // the target's product; its logit times log2 e
     const uint32_t* bits;
     const uint16_t *dense, *scale, *bias;
     uint16_t* w16;              // null: the dense weights are taken as they are
@@ -268,6 +276,7 @@ head_operands_kernel(const HeadOperands o) {
         for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
         if (lane == 0) {
             o.target[row] = target;
+            o.target_acc[row] = dot;
             if (target >= 0) {
                 if (o.scale) dot *= __half2float(__ushort_as_half(o.scale[target]));
                 if (o.bias) dot += __half2float(__ushort_as_half(o.bias[target]));
@@ -326,8 +335,10 @@ head_rows_kernel(const HeadRows o) {
     if (blockIdx.x == 0) {
         __shared__ float tops[4];
         float top = o.scale_max ? 0.0f : 1.0f;
-        if (o.scale_max)
-            for (uint32_t i = threadIdx.x; i < WEIGHT_CTAS; i += 128) top = fmaxf(top, o.scale_max[i]);
+        if (o.scale_max) {
+#pragma unroll
+            for (uint32_t i = 0; i < WEIGHT_CTAS; i += 128) top = fmaxf(top, o.scale_max[i + threadIdx.x]);
+        }
         for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
         if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
         __syncthreads();
@@ -339,9 +350,8 @@ head_rows_kernel(const HeadRows o) {
             o.factors[1] = exp2f((float)-k) * o.loss_scale;
         }
     }
-    // eight lanes to a row
-    const uint32_t row = blockIdx.x * 16 + (threadIdx.x >> 3), lane = threadIdx.x & 7;
-    if (row >= o.whole_rows) return;
+    // eight rows to a warp where neighbours share sectors of the parts, with four lanes each
+    const uint32_t row = blockIdx.x * 32 + (threadIdx.x >> 5) * 8 + (threadIdx.x & 7), lane = (threadIdx.x >> 3) & 3;
     const uint32_t m = row / pg::BM;
     float top = -INFINITY, sum = 0.0f;
     const auto add = [&](float t, float s) {
@@ -357,14 +367,17 @@ head_rows_kernel(const HeadRows o) {
         const pg::Share share = pg::share_of(o.m_tiles * width, o.pairs);
         const uint32_t slots = share.owner(m * width + width - 1) - share.owner(m * width) + 1;
         const float2* part = o.part + (size_t)piece * o.slots * 4 * o.whole_rows + row;
-        for (uint32_t i = lane; i < slots * 4; i += 8) {
-            const float2 t = part[(size_t)i * o.whole_rows];
-            add(t.x, t.y);
+        for (uint32_t i = 0; i < slots; i += 8) {   // (lane: quarter of the columns)
+            float2 t[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) t[u] = i + u < slots ? part[(size_t)((i + u) * 4 + lane) * o.whole_rows] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) add(t[u].x, t[u].y);
         }
     }
 #pragma unroll
-    for (int k = 4; k > 0; k >>= 1) {   // (within a row's lanes, in a fixed order)
-        const float t = __shfl_xor_sync(0xffffffffu, top, k), s = __shfl_xor_sync(0xffffffffu, sum, k);
+    for (int k = 2; k > 0; k >>= 1) {   // (within a row's lanes, in a fixed order)
+        const float t = __shfl_xor_sync(0xffffffffu, top, 8 * k), s = __shfl_xor_sync(0xffffffffu, sum, 8 * k);
         const float a = top, b = sum;
         const bool mine_first = !(lane & k);
         top = mine_first ? a : t;
@@ -380,22 +393,31 @@ head_rows_kernel(const HeadRows o) {
     o.row_loss[row] = target >= 0 ? (lse2 - logit2) * LN2 : target == -1 ? 0.0f : NAN;
 }
 
-// The columns' sums of a piece out of their parts, times loss_scale.
+// The columns' sums of a piece out of their parts, times loss_scale.  32 columns to a CTA, a warp to each of a slot's eight parts.
 __global__ void __launch_bounds__(256)
 head_columns_kernel(const float* __restrict__ part, uint32_t pitch, uint32_t m_tiles, uint32_t n_tiles, uint32_t pairs, uint32_t columns,
                     float loss_scale, float* __restrict__ g_scale, float* __restrict__ g_bias) {
     chain_entry();
-    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= columns) return;
+    __shared__ float sums[2][8][32];
+    const uint32_t lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;   // c < pitch, whole tiles
     const pg::Share share = pg::share_of(m_tiles * n_tiles, pairs);
-    const uint32_t n = c / pg::BN, slots = share.owner(n * m_tiles + m_tiles - 1) - share.owner(n * m_tiles) + 1;
+    const uint32_t n = blockIdx.x * 32 / pg::BN, slots = share.owner(n * m_tiles + m_tiles - 1) - share.owner(n * m_tiles) + 1;
     float g = 0.0f, ga = 0.0f;
-    for (uint32_t i = 0; i < slots * 8; ++i) {
-        g += part[(size_t)i * 2 * pitch + c];
-        ga += part[((size_t)i * 2 + 1) * pitch + c];
+#pragma unroll 4
+    for (uint32_t i = 0; i < slots; ++i) {
+        const float* from = part + (size_t)(i * 8 + slice) * 2 * pitch + c;
+        g += from[0];
+        ga += from[pitch];
     }
-    if (g_bias) g_bias[c] = g * loss_scale;
-    if (g_scale) g_scale[c] = ga * loss_scale;
+    sums[0][slice][lane] = g;
+    sums[1][slice][lane] = ga;
+    __syncthreads();
+    if (slice > 1 || c >= columns) return;
+    float all = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) all += sums[slice][k][lane];
+    float* out = slice ? g_scale : g_bias;
+    if (out) out[c] = all * loss_scale;
 }
 
 // ------------------------------------------------------------------------------------------------ the head's plan
@@ -406,7 +428,7 @@ struct HeadPlan {
     size_t piece, pieces;                        // columns of a piece of g (a multiple of 256), pieces
     uint32_t col_slots;
     Cut hidden, weight;
-    size_t h16, w16, target, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, partial, bytes;
+    size_t h16, w16, target, target_acc, target_cut, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, partial, bytes;
 };
 constexpr size_t GRAD_ELEMENTS = (size_t)1 << 27;   // of a piece of g: 256 MiB
 
@@ -443,6 +465,8 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
     p.h16 = at.add(rows * p.Dp * 2);
     p.w16 = at.add(V * p.Dp * 2);
     p.target = at.add(rows * 4);
+    p.target_acc = at.add(rows * 4);
+    p.target_cut = at.add(rows * 4);
     p.lse2 = at.add(rows * 4);
     p.logit = at.add(rows * 4);
     p.factors = at.add(8);
@@ -479,6 +503,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     o.D = (uint32_t)D;
     o.Dp = (uint32_t)p.Dp;
     o.vocab = (uint32_t)V;
+    o.target_acc = reinterpret_cast<float*>(ws + p.target_acc);
     o.logit2 = reinterpret_cast<float*>(ws + p.logit);
     o.labels = h.labels;
     o.ignore_id = h.ignore_id;
@@ -507,7 +532,8 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     q.piece_tiles = p.lse_tiles;
     q.slots = p.lse_slots;
     q.row_part = reinterpret_cast<float2*>(ws + p.row_part);
-    q.logit2 = o.logit2;
+    q.target_acc = o.target_acc;
+    q.target_cut = reinterpret_cast<float*>(ws + p.target_cut);
     q.lse2 = reinterpret_cast<float*>(ws + p.lse2);
     float* factors = reinterpret_cast<float*>(ws + p.factors);
     launch<pg::LSE, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
@@ -528,7 +554,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     r.scale_max = h.bits ? o.scale_max : nullptr;
     r.factors = factors;
     r.loss_scale = h.loss_scale;
-    s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 16), 128, 0, r);
+    s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 32), 128, 0, r);
 
     uint16_t* grad = reinterpret_cast<uint16_t*>(ws + p.grad);
     for (size_t piece = 0; piece < p.pieces; ++piece) {
@@ -548,7 +574,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
         const CUtensorMap grad_map = map_of(grad, rows, p.piece, p.piece, 16, bf16);
         launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
         if (h.g_bias || h.g_scale)
-            s.chain("head_columns", head_columns_kernel, (unsigned)ceil_div(width, 256), 256, 0, static_cast<const float*>(g.col_part), g.pitch,
+            s.chain("head_columns", head_columns_kernel, (unsigned)ceil_div(width, 32), 256, 0, static_cast<const float*>(g.col_part), g.pitch,
                     (uint32_t)p.m_tiles, n_tiles, p.pairs, (uint32_t)width, h.loss_scale, h.g_scale ? h.g_scale + v0 : nullptr,
                     h.g_bias ? h.g_bias + v0 : nullptr);
         // g_hidden: over the pieces in f32
@@ -569,48 +595,67 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
 // ------------------------------------------------------------------------------------------------ weight gradient from the tape
 namespace {
 
-// The largest exponent byte of each block of 32 channels over the rows.  A thread has a block and every `slices`-th row.
+// The largest exponent byte of each block of 32 channels, over TOP_SLICES slices of the rows: top [slice][blocks].  A CTA has 32
+// blocks of a slice, eight threads share a block's rows.
+constexpr uint32_t TOP_SLICES = 32;
 __global__ void __launch_bounds__(THREADS)
-tape_exponent_max_kernel(const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t blocks, uint32_t slices, uint32_t* __restrict__ top) {
+tape_exponent_max_kernel(const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t blocks, uint8_t* __restrict__ top) {
     chain_entry();
-    const uint32_t item = blockIdx.x * THREADS + threadIdx.x, slice = item / blocks, b = item - slice * blocks;
-    if (slice >= slices) return;
+    const uint32_t slice = blockIdx.y, b = blockIdx.x * 32 + (threadIdx.x & 31);
+    const uint32_t first = (uint32_t)((uint64_t)slice * rows / TOP_SLICES), last = (uint32_t)((uint64_t)(slice + 1) * rows / TOP_SLICES);
+    __shared__ uint32_t tops[THREADS];
     uint32_t most = 0;
-    for (uint32_t r = slice; r < rows; r += slices) most = max(most, (uint32_t)exponents[(size_t)r * blocks + b]);
-    atomicMax(top + b, most);
+    if (b < blocks) {
+#pragma unroll 16
+        for (uint32_t r = first + (threadIdx.x >> 5); r < last; r += 8) most = max(most, (uint32_t)exponents[(size_t)r * blocks + b]);
+    }
+    tops[threadIdx.x] = most;
+    __syncthreads();
+    if (threadIdx.x >= 32 || b >= blocks) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) most = max(most, tops[threadIdx.x + 32 * k]);
+    top[slice * blocks + b] = (uint8_t)most;
 }
 
 // What the codes stand for as a 16-bit operand [rows, Cp].  bf16 holds every value (8 significant bits, the range of f32).  FP16
 // does not: there each block of 32 channels is shifted by a power of two common to all rows, so that its largest exponent comes to 8
 // (127 * 2^8 = 32 512), and the column's sums are shifted back.  What is lost lies 2^32 below the block's largest value.
-template <bool BF>
+// A thread has a chunk of eight columns and OPERAND_ROWS rows in turn.  VEC: as in tape.cuh.
+constexpr uint32_t OPERAND_ROWS = 4;
+template <bool BF, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 tape_operand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t C, uint32_t Cp,
-                    const uint32_t* __restrict__ top, uint16_t* __restrict__ out, float* __restrict__ col_factor) {
+                    const uint8_t* __restrict__ top, uint16_t* __restrict__ out, float* __restrict__ col_factor) {
     chain_entry();
     const uint32_t chunks = Cp / 8, blocks = (C + 31) / 32;
     const size_t item = (size_t)blockIdx.x * THREADS + threadIdx.x;
-    if (!BF && item < blocks) {
-        const uint32_t byte = top[item];
-        col_factor[item] = byte == tape::NOT_FINITE ? 1.0f : exp2f((float)((int)byte - 127 - 8));
-    }
-    const size_t row = item >> 32 ? item / chunks : (uint32_t)item / chunks;
-    if (row >= rows) return;
-    const uint32_t c = (uint32_t)(item - row * chunks) * 8, byte = exponents[row * blocks + c / 32];
-    float step = tape::power(byte);
-    if (!BF && byte != tape::NOT_FINITE) {
-        const uint32_t most = top[c / 32];
-        step = exp2f((float)((int)byte - (int)(most == tape::NOT_FINITE ? byte : most) + 8));
-    }
-    uint32_t w[4] = {};
+    const size_t group = item >> 32 ? item / chunks : (uint32_t)item / chunks, row0 = group * OPERAND_ROWS;
+    if (row0 >= rows) return;
+    const uint32_t c = (uint32_t)(item - group * chunks) * 8, b = c / 32;
+    uint32_t most = 0;
+    if (!BF) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (c + e < C) {
-            const float v = (float)(int8_t)codes[row * C + c + e] * step;
-            const uint32_t h = BF ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
-            w[e >> 1] |= h << (16 * (e & 1));
-        }
-    *reinterpret_cast<uint4*>(out + row * Cp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (uint32_t k = 0; k < TOP_SLICES; ++k) most = max(most, (uint32_t)top[k * blocks + b]);
+        if (row0 == 0 && c % 32 == 0) col_factor[b] = most == tape::NOT_FINITE ? 1.0f : exp2f((float)((int)most - 127 - 8));
+    }
+    float v[OPERAND_ROWS][8];
+#pragma unroll
+    for (uint32_t k = 0; k < OPERAND_ROWS; ++k) {
+        const size_t row = row0 + k;
+        if (row >= rows) break;
+        uint32_t byte = exponents[row * blocks + b];
+        if (!BF && byte != tape::NOT_FINITE)   // 2^(e - largest + 8)
+            byte = most == tape::NOT_FINITE ? 127u : (uint32_t)max((int)byte - (int)most + 8 + 127, 1);
+        tape::load_codes<VEC>(codes + row * C, tape::power(byte), c, C, v[k]);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < OPERAND_ROWS; ++k) {
+        if (row0 + k >= rows) break;
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pg::pack16<BF>(v[k][2 * e], v[k][2 * e + 1]);
+        *reinterpret_cast<uint4*>(out + (row0 + k) * Cp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 // 16-bit rows that no tensor map takes, with a stride of whole 16 bytes
@@ -642,7 +687,7 @@ WeightPlan weight_plan(const ullis_cuda_runtime* rt, size_t rows, size_t in, siz
     Parts at;
     p.x16 = at.add(rows * p.ip * 2);
     p.gy16 = at.add(rows * p.op * 2);
-    p.top = at.add(tape::blocks_of(in) * 4);
+    p.top = at.add(TOP_SLICES * tape::blocks_of(in));
     p.col_factor = at.add(tape::blocks_of(in) * 4);
     p.partial = at.add(partial_bytes(out, in, p.cut));
     p.bytes = at.bytes;
@@ -661,21 +706,16 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const bool bf16 = dtype == BF16;
     uint16_t* x16 = reinterpret_cast<uint16_t*>(ws + p.x16);
-    uint32_t* top = reinterpret_cast<uint32_t*>(ws + p.top);
+    uint8_t* top = ws + p.top;
     float* col_factor = reinterpret_cast<float*>(ws + p.col_factor);
     const uint32_t blocks = (uint32_t)tape::blocks_of(in);
-    const unsigned grid = (unsigned)ceil_div(rows * (p.ip / 8), THREADS);
-    if (bf16) {
-        s.chain("tape_operand", tape_operand_kernel<true>, grid, THREADS, 0, codes, exponents, (uint32_t)rows, (uint32_t)in, (uint32_t)p.ip,
-                static_cast<const uint32_t*>(top), x16, col_factor);
-    } else {
-        ULLIS_CUDA_CHECK(cudaMemsetAsync(top, 0, blocks * 4, s.stream));
-        const uint32_t slices = (uint32_t)std::min<size_t>(ceil_div(rows, 16), 4096);
-        s.chain("tape_exponent_max", tape_exponent_max_kernel, (unsigned)ceil_div((size_t)slices * blocks, THREADS), THREADS, 0, exponents,
-                (uint32_t)rows, blocks, slices, top);
-        s.chain("tape_operand", tape_operand_kernel<false>, grid, THREADS, 0, codes, exponents, (uint32_t)rows, (uint32_t)in, (uint32_t)p.ip,
-                static_cast<const uint32_t*>(top), x16, col_factor);
-    }
+    const unsigned grid = (unsigned)ceil_div(ceil_div(rows, OPERAND_ROWS) * (p.ip / 8), THREADS);
+    const bool vec = in % 8 == 0 && aligned(codes, 8);
+    if (!bf16) s.chain("tape_exponent_max", tape_exponent_max_kernel, dim3((blocks + 31) / 32, TOP_SLICES), THREADS, 0, exponents, (uint32_t)rows, blocks, top);
+    const auto operand = bf16 ? (vec ? tape_operand_kernel<true, true> : tape_operand_kernel<true, false>)
+                              : (vec ? tape_operand_kernel<false, true> : tape_operand_kernel<false, false>);
+    s.chain("tape_operand", operand, grid, THREADS, 0, codes, exponents, (uint32_t)rows, (uint32_t)in, (uint32_t)p.ip,
+            static_cast<const uint8_t*>(top), x16, col_factor);
     Operand a{gy.data, rows, out, gy.stride, true};
     if (!aligned(gy.data, 16) || gy.stride % 8) {
         uint16_t* gy16 = reinterpret_cast<uint16_t*>(ws + p.gy16);

@@ -19,7 +19,7 @@
 //          f32 sums of g and g * acc
 //   STORE  alpha * acc in 16 bits, or into an f32 accumulator, or as one of several partial sums
 //   SUM    acc in f32: the tensor cores cut off what falls below the accumulator's last bit (measured: K = 16384 1.9e-5 off in
-//          norm, 1.1e-4 where all terms have one sign; K = 1024 1e-6), so every 1024 terms the accumulator moves to registers
+//          norm, 1.1e-4 where all terms have one sign; K = 512 6e-7), so every 512 terms the accumulator moves to registers
 //          and is added there with rounding
 // Every wait is bounded and reports through the status words, as in tc_gemm_ws2.cuh.
 #pragma once
@@ -41,9 +41,10 @@ constexpr int THREADS = 64 + 32 * (int)EPI_WARPS;
 constexpr uint32_t MAX_STAGES = 6, SMEM_LIMIT = 227 * 1024;
 // per epilogue warp
 constexpr uint32_t STAGING_BYTES = 16 * 128;            // 16 rows of 64 16-bit outputs; GRAD has two of them
-constexpr uint32_t COLUMN_BYTES = 3 * 64 * 4;           // constants of its columns
-constexpr uint32_t ROW_BYTES = 2 * 3 * 32 * 4;          // GRAD: what its rows need, of this tile and of the next
-constexpr uint32_t SUM_BLOCKS = 16;                     // k-blocks between two rounded additions
+constexpr uint32_t COLUMN_BYTES = 2 * 64 * 4;           // constants of its columns
+constexpr uint32_t ROW_BYTES = 2 * 4 * 32 * 4;          // GRAD: what its rows need, of this tile and of the next
+constexpr uint32_t HIT_BYTES = 2 * 64 * 4;              // GRAD: what the targets add to the columns' sums
+constexpr uint32_t SUM_BLOCKS = 8;                      // k-blocks between two rounded additions
 
 struct Maps {
     CUtensorMap a, b;
@@ -63,7 +64,8 @@ struct Params {
     uint32_t slots;            // LSE: partial sums per piece and row
     float2* row_part;          // LSE: [piece][slot][4][rows, whole tiles]
     const float* lse2;         // GRAD: [M] log2 of the sum of exp, +inf for a row that does not count
-    const float* logit2;       // GRAD: [M] the target's logit times log2 e
+    float* target_cut;         // [M] the target's product as the tensor cores have it (LSE leaves it, GRAD takes it out) ...
+    const float* target_acc;   // GRAD: ... and with rounding
     const float* factor;       // GRAD: 2^k ; STORE: alpha
     uint32_t pitch;            // GRAD: of col_part, whole tiles
     float* col_part;           // GRAD: [slot][8][2][pitch]
@@ -79,7 +81,7 @@ struct Params {
 inline uint32_t stage_bytes(int accs) { return OPERAND_BYTES * (1 + accs); }
 // Barriers first, then (on 1024 bytes) the ring, then what the epilogue warps have.
 constexpr uint32_t epi_bytes(int epi) {
-    return epi == GRAD ? 2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES : epi == STORE ? STAGING_BYTES : epi == LSE ? COLUMN_BYTES : 0u;
+    return epi == GRAD ? 2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES + HIT_BYTES : epi == STORE ? STAGING_BYTES : epi == LSE ? COLUMN_BYTES : 0u;
 }
 inline uint32_t fixed_bytes(int epi) { return 2 * 1024 /*barriers, alignment*/ + EPI_WARPS * epi_bytes(epi); }
 inline uint32_t stages_for(int epi, int accs) {
@@ -261,7 +263,7 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile ui
 constexpr float LOG2E = 1.4426950408889634f;
 
 // Scale and bias (FP16, two lanes' worth: columns lane and 32 + lane) of 64 columns from n0 on, on their way while the tile before
-// is worked on; and as the constants that the epilogue reads: both times log2 e, scale * 2^k.  Columns past N have a probability of 0.
+// is worked on; and as the constants that the epilogue reads: both times log2 e.  Columns past N have a probability of 0.
 struct Columns {
     float scale[2], bias[2];
     __device__ void fetch(const Params& p, uint32_t n0, int lane) {
@@ -272,12 +274,11 @@ struct Columns {
             bias[i] = n < p.N ? half_at(p.bias, n, 0.0f) : -INFINITY;
         }
     }
-    __device__ void keep(float* to, int lane, float power) const {
+    __device__ void keep(float* to, int lane) const {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             to[i * 32 + lane] = scale[i] * LOG2E;
             to[64 + i * 32 + lane] = bias[i] * LOG2E;
-            to[128 + i * 32 + lane] = scale[i] * power;
         }
     }
 };
@@ -481,7 +482,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     target = row < p.M ? p.target[row] : -1;
                 }
                 __syncwarp();
-                ahead.keep(columns, lane, 0.0f);
+                ahead.keep(columns, lane);
                 __syncwarp();
                 more = work.next();
                 if (more) ahead.fetch(p, work.n * BN + group * 64, lane);
@@ -494,6 +495,13 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     ptx::tmem_ld_wait();
                     if (c == 1) drained();
                     const int32_t hit = target - (int32_t)(n0 + c * 32);
+                    const bool hits = __any_sync(0xffffffffu, hit >= 0 && hit < 32);   // of the warp's rows
+                    if (hits) {   // (by bits: chosen by an index, the accumulators went to local memory)
+                        uint32_t cut = 0;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) cut |= hit == i ? r[i] : 0u;
+                        if (hit >= 0 && hit < 32) p.target_cut[m_now * BM + rank * 128 + quarter * 32 + lane] = __uint_as_float(cut);
+                    }
                     uint64_t z[16];
                     float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -503,7 +511,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         z[i] = fma2((uint64_t)r[i * 2 + 1] << 32 | r[i * 2], s.x, b.x);
                         z[i + 1] = fma2((uint64_t)r[i * 2 + 3] << 32 | r[i * 2 + 2], s.y, b.y);
                     }
-                    if (__any_sync(0xffffffffu, hit >= 0 && hit < 32)) {   // (by sums: as stores of elements z went to local memory)
+                    if (hits) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             z[i] = add2(z[i], two(hit == i * 2 ? -INFINITY : 0.0f, hit == i * 2 + 1 ? -INFINITY : 0.0f));
@@ -532,14 +540,17 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             }
             leave();
         } else if constexpr (EPI == GRAD) {
-            const float power = *p.factor;
+            const float from_log2 = *p.factor / LOG2E;   // scale * log2 e -> scale * 2^k
             const Share all = share_of(work.m_tiles * work.n_tiles, pairs);
             uint32_t n_now = 0xFFFFFFFFu;
             uint64_t g_sum[8], ga_sum[8];   // of column pairs 8 j + q2
 #pragma unroll
             for (int j = 0; j < 8; ++j) g_sum[j] = ga_sum[j] = 0;
+            float* hits = reinterpret_cast<float*>(epi_smem + EPI_WARPS * (2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES) + mine * HIT_BYTES);
+            for (int i = lane; i < 128; i += 32) hits[i] = 0.0f;
             const auto leave = [&]() {   // the sums of 32 rows: over the lanes that share columns, then out
                 if (n_now == 0xFFFFFFFFu) return;
+                __syncwarp();
                 const uint32_t slot = pair - all.owner(n_now * work.m_tiles);
                 float* to = p.col_part + (((size_t)slot * 8 + rank * 4 + quarter) * 2) * p.pitch + n_now * BN + group * 64 + q2;
 #pragma unroll
@@ -550,22 +561,25 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         ga_sum[j] = add2(ga_sum[j], __shfl_xor_sync(0xffffffffu, ga_sum[j], o));
                     }
                     if (lane < 4) {
-                        *reinterpret_cast<uint64_t*>(to + j * 8) = g_sum[j];
-                        *reinterpret_cast<uint64_t*>(to + p.pitch + j * 8) = ga_sum[j];
+                        *reinterpret_cast<uint64_t*>(to + j * 8) = add2(g_sum[j], *reinterpret_cast<const uint64_t*>(hits + j * 8 + q2));
+                        *reinterpret_cast<uint64_t*>(to + p.pitch + j * 8) = add2(ga_sum[j], *reinterpret_cast<const uint64_t*>(hits + 64 + j * 8 + q2));
                     }
                     g_sum[j] = ga_sum[j] = 0;
                 }
+                __syncwarp();
+                for (int i = lane; i < 128; i += 32) hits[i] = 0.0f;   // (by the lane that adds to it)
             };
             // What the rows need lies in shared memory, two tiles in turn; the next tile's is on its way while one is worked on: a
-            // word each of lse2, the target's logit and the target per lane.
+            // word each of lse2, the target's two products and the target per lane.
             float* row_smem = reinterpret_cast<float*>(epi_smem + EPI_WARPS * (2 * STAGING_BYTES + COLUMN_BYTES) + mine * ROW_BYTES);
             const auto fetch = [&](uint32_t turn) {
                 const uint32_t row = work.m * BM + rank * 128 + quarter * 32 + lane;
                 const bool in = row < p.M;
-                float* to = row_smem + turn * 96 + lane;
+                float* to = row_smem + turn * 128 + lane;
                 copy_word(to, p.lse2 + (in ? row : 0), in);
-                copy_word(to + 32, p.logit2 + (in ? row : 0), in);
-                copy_word(to + 64, p.target + (in ? row : 0), in);
+                copy_word(to + 32, p.target_acc + (in ? row : 0), in);
+                copy_word(to + 64, p.target_cut + (in ? row : 0), in);
+                copy_word(to + 96, p.target + (in ? row : 0), in);
             };
             const uint32_t blocks_at = ptx::smem_u32(staging) + ((lane >> 3) & 1) * 1024 + (lane & 7) * 128;   // of store_blocks: block b has
             const uint32_t block_piece = lane >> 4;                                                           // rows 8 (b % 2) .., piece b / 2
@@ -580,42 +594,65 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     __syncwarp();
                     Columns c;
                     c.fetch(p, n0, lane);
-                    c.keep(columns, lane, power);
+                    c.keep(columns, lane);
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncwarp();
-                const float* rows = row_smem + turn * 96;
+                const float* rows = row_smem + turn * 128;
                 turn ^= 1;
-                const int32_t first = (int32_t)(p.n_first + n0);
-                const int32_t own = m0 + lane < p.M ? reinterpret_cast<const int32_t*>(rows)[64 + lane] - first : -1;
-                const bool any = __any_sync(0xffffffffu, own >= 0 && own < 64);
+                // Of this lane's row: the target's column among the warp's 64, or another number.  Its g has the product with rounding
+                // in it and the -1 of the one-hot; the loop below knows nothing of that: g goes to its place in the 16-bit block behind
+                // the loop, and what it is more than the loop's exp to the column's sums by itself.  (As comparisons within the loop the
+                // targets took a fifth of this epilogue.)  A lane has columns lane and 32 + lane, in the order of the rows.
+                const uint32_t own = m0 + lane < p.M ? reinterpret_cast<const uint32_t*>(rows)[96 + lane] - (p.n_first + n0) : 64u;
+                float own_g = 0.0f;
+                uint32_t left = __ballot_sync(0xffffffffu, own < 64u);
+                if (left) {
+                    float more_g = 0.0f, more_ga = 0.0f;
+                    if (own < 64u) {
+                        const float acc = rows[32 + lane], cut = rows[64 + lane];
+                        const float p_cut = exp2_fast(fmaf(cut, columns[own], columns[64 + own]) - rows[lane]);
+                        own_g = exp2_fast(fmaf(acc, columns[own], columns[64 + own]) - rows[lane]) - 1.0f;
+                        more_g = own_g - p_cut;
+                        more_ga = own_g * acc - p_cut * cut;
+                        own_g *= columns[own] * from_log2;
+                    }
+                    float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (; left; left &= left - 1) {
+                        const int row = __ffs(left) - 1;
+                        const uint32_t column = __shfl_sync(0xffffffffu, own, row);
+                        const float g = __shfl_sync(0xffffffffu, more_g, row), ga = __shfl_sync(0xffffffffu, more_ga, row);
+                        add[0] += column == lane ? g : 0.0f;
+                        add[1] += column == lane + 32u ? g : 0.0f;
+                        add[2] += column == lane ? ga : 0.0f;
+                        add[3] += column == lane + 32u ? ga : 0.0f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) hits[i * 32 + lane] += add[i];
+                }
                 more = work.next();
                 if (more) fetch(turn);
                 uint32_t taddr;
                 if (!filled(&taddr)) break;
-                // 16 rows; TARGETS: the target of one of the warp's rows lies in its columns
-                const auto half = [&](int h, auto targets) {
+                taddr += group * 64;
+                // 16 rows at a time, one copy of the code for both: with two the registers ran out
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
                     uint32_t r[16];
-                    tmem_ld_16x32(taddr + group * 64 + ((h * 16) << 16), r);
-                    float lse[2], logit[2];
-                    int32_t at[2];
+                    tmem_ld_16x32(taddr + ((h * 16) << 16), r);
+                    uint64_t l[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t row = h * 16 + i * 8 + r0;
-                        lse[i] = m0 + row < p.M ? -rows[row] : -INFINITY;
-                        if (decltype(targets)::value) {
-                            logit[i] = rows[32 + row] + lse[i];
-                            at[i] = reinterpret_cast<const int32_t*>(rows)[64 + row] - first - (int32_t)q2;
-                            if (m0 + row >= p.M) at[i] = -1;
-                        }
+                        const float lse = m0 + row < p.M ? -rows[row] : -INFINITY;
+                        l[i] = two(lse, lse);
                     }
-                    const uint64_t l[2] = {two(lse[0], lse[0]), two(lse[1], lse[1])};
                     const uint32_t to = blocks_at + h * STAGING_BYTES;
                     if (lane == 0) tma_store_read<1>();   // the store before the last has read this half
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
-                        if (j == 4) tmem_ld_16x32(taddr + group * 64 + 32 + ((h * 16) << 16), r);
+                        if (j == 4) tmem_ld_16x32(taddr + 32 + ((h * 16) << 16), r);
                         if (j == 0 || j == 4) ptx::tmem_ld_wait();
                         if (j == 4 && h == 1) drained();
                         uint32_t w[4];
@@ -623,17 +660,13 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         for (int u = 0; u < 2; ++u) {
                             const uint64_t s = *reinterpret_cast<const uint64_t*>(columns + (j + u) * 8 + q2);
                             const uint64_t b = *reinterpret_cast<const uint64_t*>(columns + 64 + (j + u) * 8 + q2);
-                            const uint64_t k = *reinterpret_cast<const uint64_t*>(columns + 128 + (j + u) * 8 + q2);
+                            const uint64_t k = mul2(s, two(from_log2, from_log2));
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
-                                const uint64_t a = (uint64_t)r[(j + u) % 4 * 4 + i * 2 + 1] << 32 | r[(j + u) % 4 * 4 + i * 2];
+                                const int at = (j + u) % 4 * 4 + i * 2;
+                                const uint64_t a = (uint64_t)r[at + 1] << 32 | r[at];
                                 const float2 e = of_two(add2(fma2(a, s, b), l[i]));
-                                float2 gv = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                                if (decltype(targets)::value) {
-                                    if (at[i] == (j + u) * 8) gv.x = exp2_fast(logit[i]) - 1.0f;
-                                    if (at[i] == (j + u) * 8 + 1) gv.y = exp2_fast(logit[i]) - 1.0f;
-                                }
-                                const uint64_t g = two(gv.x, gv.y);
+                                const uint64_t g = two(exp2_fast(e.x), exp2_fast(e.y));
                                 g_sum[j + u] = add2(g_sum[j + u], g);
                                 ga_sum[j + u] = fma2(g, a, ga_sum[j + u]);
                                 const float2 o = of_two(mul2(g, k));
@@ -643,18 +676,16 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         // 16-byte piece c of row r at c ^ (r % 8), as the copy below reads it; no bank conflicts
                         store_blocks(to + (((j + block_piece) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
                     }
+                    __syncwarp();
+                    if (own < 64u && lane >> 4 == h)   // this lane's row has its target here
+                        *reinterpret_cast<uint16_t*>(staging + h * STAGING_BYTES + (lane & 15) * 128 + (((own >> 3) ^ (lane & 7)) << 4) + (own & 7) * 2) =
+                            (uint16_t)pack16<BF16>(own_g, 0.0f);
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
                         if (m0 + h * 16 < p.M) tma_store_2d(&maps.out, ptx::smem_u32(staging) + h * STAGING_BYTES, (int32_t)n0, (int32_t)(m0 + h * 16));
                         else asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // (the groups stay in turn)
                     }
-                };
-                // one copy of the code for both halves: with two the registers ran out
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-                    if (any) half(h, std::true_type{});
-                    else half(h, std::false_type{});
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");

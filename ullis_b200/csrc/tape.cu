@@ -220,22 +220,25 @@ tape_layer_norm_backward_kernel(const uint8_t* __restrict__ codes, const uint8_t
     }
 }
 
-// out[c] = sum over p of part[p][c], c < 2 C: first the weights' gradient, then the biases'.  32 columns to a CTA, eight threads
-// to a column.
-__global__ void __launch_bounds__(256)
+// out[c] = sum over p of part[p][c], c < 2 C: first the weights' gradient, then the biases'.  32 columns to a CTA, 32 threads to a
+// column, their loads in flight together (eight threads one after the other: 10.8 us for 296 parts of 1024, a third of the pass).
+__global__ void __launch_bounds__(1024)
 tape_columns_kernel(const float* __restrict__ part, uint32_t parts, uint32_t C, float* __restrict__ g_weight, float* __restrict__ g_bias) {
     chain_entry();
-    __shared__ float sums[8][32];
+    __shared__ float sums[32][33];
     const uint32_t lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float acc = 0.0f;
-    if (c < 2 * C)
-        for (uint32_t p = slice; p < parts; p += 8) acc += part[(size_t)p * 2 * C + c];
+    if (c < 2 * C) {
+#pragma unroll 10
+        for (uint32_t p = slice; p < parts; p += 32) acc += part[(size_t)p * 2 * C + c];
+    }
     sums[slice][lane] = acc;
     __syncthreads();
-    if (slice || c >= 2 * C) return;
+    acc = sums[lane][slice];   // a warp per column
 #pragma unroll
-    for (int k = 1; k < 8; ++k) acc += sums[k][lane];
-    (c < C ? g_weight : g_bias)[c < C ? c : c - C] = acc;
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    const uint32_t own = blockIdx.x * 32 + slice;
+    if (lane == 0 && own < 2 * C) (own < C ? g_weight : g_bias)[own < C ? own : own - C] = acc;
 }
 
 bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -340,7 +343,7 @@ void tape_layer_norm_backward(const Stream& s, int dtype, const uint8_t* codes, 
             });
         });
     });
-    s.chain("tape_columns", tape_columns_kernel, (unsigned)((2 * channels + 31) / 32), 256, 0, part, (uint32_t)ctas, (uint32_t)channels,
+    s.chain("tape_columns", tape_columns_kernel, (unsigned)((2 * channels + 31) / 32), 1024, 0, part, (uint32_t)ctas, (uint32_t)channels,
             g_weight, g_bias);
 }
 

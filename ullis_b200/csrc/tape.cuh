@@ -112,13 +112,11 @@ __device__ __forceinline__ void store_codes(uint8_t* codes, uint32_t c, uint32_t
             if (c + i < C) codes[c + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
 }
-// What eight codes stand for; past the row's end zeros (whatever the block's exponent).
+// Eight codes times `step`; past the row's end zeros (whatever the step).
 template <bool VEC>
-__device__ __forceinline__ void load_codes(const uint8_t* codes, const uint8_t* exponents, uint32_t c, uint32_t C, float (&v)[8]) {
+__device__ __forceinline__ void load_codes(const uint8_t* codes, float step, uint32_t c, uint32_t C, float (&v)[8]) {
     uint32_t w[2] = {0u, 0u};
-    float step = 0.0f;
     if (c < C) {
-        step = power(exponents[c / BLOCK]);
         if constexpr (VEC) {
             const uint2 t = *reinterpret_cast<const uint2*>(codes + c);
             w[0] = t.x; w[1] = t.y;
@@ -131,8 +129,13 @@ __device__ __forceinline__ void load_codes(const uint8_t* codes, const uint8_t* 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float x = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * step;
-        v[i] = VEC || c + i < C ? x : 0.0f;
+        v[i] = (VEC ? c : c + i) < C ? x : 0.0f;
     }
+}
+// What they stand for.
+template <bool VEC>
+__device__ __forceinline__ void load_codes(const uint8_t* codes, const uint8_t* exponents, uint32_t c, uint32_t C, float (&v)[8]) {
+    load_codes<VEC>(codes, c < C ? power(exponents[c / BLOCK]) : 0.0f, c, C, v);
 }
 #endif
 

@@ -32,16 +32,17 @@ class HeadGrad(NamedTuple):
     bias: object
 
 
-_TORCH, _DTYPES, _16, _RAW_STREAM = None, None, None, None
+_TORCH = _RAW_STREAM = None
+_DTYPES = _16 = _F16 = _I8 = _U8 = _I32 = None   # the types that arguments may have
 
 
 def _torch():
-    global _TORCH, _DTYPES, _16, _RAW_STREAM
+    global _TORCH, _RAW_STREAM, _DTYPES, _16, _F16, _I8, _U8, _I32
     if _TORCH is None:
         import torch
 
         _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-        _16 = (torch.float16, torch.bfloat16)
+        _16, _F16, _I8, _U8, _I32 = (torch.float16, torch.bfloat16), (torch.float16,), (torch.int8,), (torch.uint8,), (torch.int32,)
         _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
             (lambda device: torch.cuda.current_stream(device).cuda_stream)
         _TORCH = torch
@@ -72,6 +73,11 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _like(t, dtype):
+    """An output of t's shape, without gaps."""
+    return _TORCH.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
 def _shape_error(name, got, expected):
     raise UllisCudaError(ERR_SHAPE, f"{name} length mismatch: got {tuple(got)}, expected {tuple(expected)}")
 
@@ -80,52 +86,60 @@ class DeviceOps:
     """Mixed into CudaRuntime."""
 
     # ------------------------------------------------------------------------------------------ arguments
+    # A call's checks are on the way of every launch: each begins with what an ordinary argument is, and only another one is
+    # looked at more closely.
     def _on_device(self, t) -> bool:
-        return t.is_cuda and t.get_device() == self.device
+        return t.get_device() == self.device          # -1 on the host
 
-    def _tensor(self, t, name, dtypes):
-        torch = _torch()
-        if not isinstance(t, torch.Tensor):
+    def _refuse(self, t, name, dtypes):
+        if not isinstance(t, _torch().Tensor):
             raise UllisCudaError(ERR_ARG, f"{name} is not a tensor")
         if not self._on_device(t):
             raise UllisCudaError(ERR_ARG, f"{name} is not on the runtime's device (cuda:{self.device})")
         if t.dtype not in dtypes:
             raise UllisCudaError(ERR_ARG, f"{name} has the type {t.dtype}, not one of {', '.join(str(d) for d in dtypes)}")
-        return t
 
     def _matrix(self, t, name, dtypes):
-        """(tensor, rows, channels, row stride) of [..., channels] with contiguous channels and evenly spaced rows."""
-        t = self._tensor(t, name, dtypes)
+        """(rows, channels, row stride) of [..., channels] with contiguous channels and evenly spaced rows."""
+        try:
+            if t.dtype in dtypes and self._on_device(t) and t.dim() == 2 and t.is_contiguous():
+                rows, channels = t.shape
+                return rows, channels, channels
+        except AttributeError:
+            pass
+        self._refuse(t, name, dtypes)
         if t.dim() < 2:
             raise UllisCudaError(ERR_SHAPE, f"{name} must have at least two dimensions")
         channels = t.shape[-1]
         if t.dim() != 2 or (channels > 1 and t.stride(1) != 1):
             if not t.is_contiguous():
                 raise UllisCudaError(ERR_SHAPE, f"{name} must have contiguous channels and, with more than two dimensions, be contiguous")
-            rows = t.numel() // channels if channels else 0
-            return t, rows, channels, channels
+            return (t.numel() // channels if channels else 0), channels, channels
         rows = t.shape[0]
         stride = t.stride(0) if rows > 1 else channels
         if stride < channels:
             raise UllisCudaError(ERR_SHAPE, f"{name} must not have overlapping rows")
-        return t, rows, channels, stride
+        return rows, channels, stride
 
     def _vector(self, t, name, dtypes, n):
-        t = self._tensor(t, name, dtypes)
+        try:
+            if t.dtype in dtypes and self._on_device(t) and t.numel() == n and t.is_contiguous():
+                return
+        except AttributeError:
+            pass
+        self._refuse(t, name, dtypes)
         if t.numel() != n:
             _shape_error(name, t.shape, (n,))
-        if not t.is_contiguous():
-            raise UllisCudaError(ERR_SHAPE, f"{name} must be contiguous")
-        return t
+        raise UllisCudaError(ERR_SHAPE, f"{name} must be contiguous")
 
     def _tape(self, tape):
-        torch = _torch()
+        _torch()
         try:
             codes, exponents = tape
         except (TypeError, ValueError):
             raise UllisCudaError(ERR_ARG, "tape is not a pair of codes and exponents") from None
-        codes = self._tensor(codes, "codes", (torch.int8,))
-        exponents = self._tensor(exponents, "exponents", (torch.uint8,))
+        self._refuse(codes, "codes", _I8)
+        self._refuse(exponents, "exponents", _U8)
         if codes.dim() < 2 or not codes.is_contiguous() or not exponents.is_contiguous():
             raise UllisCudaError(ERR_SHAPE, "codes and exponents must be contiguous, codes with at least two dimensions")
         channels = codes.shape[-1]
@@ -154,75 +168,73 @@ class DeviceOps:
     def tape_pack(self, x) -> Tape:
         """x [..., channels] (float32, float16, bfloat16) in 8 bits: one exponent per 32 channels of a row."""
         torch = _torch()
-        x, rows, channels, stride = self._matrix(x, "x", _DTYPES)
-        codes = x.new_empty(x.shape, dtype=torch.int8)
+        rows, channels, stride = self._matrix(x, "x", _DTYPES)
+        codes = _like(x, torch.int8)
         exponents = x.new_empty((rows, -(-channels // 32)), dtype=torch.uint8)
-        self._check(self._lib.ullis_cuda_tape_pack(self._h, _RAW_STREAM(self.device), _DTYPES[x.dtype], _p(x), stride,
-                                                   rows, channels, _p(codes), _p(exponents)))
+        self._check(self._lib.ullis_cuda_tape_pack(self._h, _RAW_STREAM(self.device), _DTYPES[x.dtype], x.data_ptr(), stride, rows,
+                                                   channels, codes.data_ptr(), exponents.data_ptr()))
         return Tape(codes, exponents)
 
     def tape_unpack(self, tape, dtype):
         """What the codes stand for, in `dtype`, in their shape."""
-        torch = _torch()
         codes, exponents, rows, channels = self._tape(tape)
         if dtype not in _DTYPES:
             raise UllisCudaError(ERR_ARG, f"a tape does not unpack to {dtype}")
-        x = codes.new_empty(codes.shape, dtype=dtype)
-        self._check(self._lib.ullis_cuda_tape_unpack(self._h, _RAW_STREAM(self.device), _DTYPES[dtype], _p(codes), _p(exponents),
-                                                     rows, channels, _p(x), channels))
+        x = _like(codes, dtype)
+        self._check(self._lib.ullis_cuda_tape_unpack(self._h, _RAW_STREAM(self.device), _DTYPES[dtype], codes.data_ptr(),
+                                                     exponents.data_ptr(), rows, channels, x.data_ptr(), channels))
         return x
 
     def tape_layer_norm(self, x, weight, bias):
         """(LayerNorm(x), tape of x): weight and bias float16 [channels]; y has the shape and type of x."""
         torch = _torch()
-        x, rows, channels, stride = self._matrix(x, "x", _DTYPES)
-        weight = self._vector(weight, "weight", (torch.float16,), channels)
-        bias = self._vector(bias, "bias", (torch.float16,), channels)
-        y = x.new_empty(x.shape)
-        codes = x.new_empty(x.shape, dtype=torch.int8)
+        rows, channels, stride = self._matrix(x, "x", _DTYPES)
+        self._vector(weight, "weight", _F16, channels)
+        self._vector(bias, "bias", _F16, channels)
+        y = _like(x, x.dtype)
+        codes = _like(x, torch.int8)
         exponents = x.new_empty((rows, -(-channels // 32)), dtype=torch.uint8)
         self._check(self._lib.ullis_cuda_tape_layer_norm(
-            self._h, _RAW_STREAM(self.device), _DTYPES[x.dtype], _p(x), stride, _p(weight), _p(bias), rows,
-            channels, _p(y), _p(codes), _p(exponents)))
+            self._h, _RAW_STREAM(self.device), _DTYPES[x.dtype], x.data_ptr(), stride, weight.data_ptr(), bias.data_ptr(), rows,
+            channels, y.data_ptr(), codes.data_ptr(), exponents.data_ptr()))
         return y, Tape(codes, exponents)
 
     def tape_layer_norm_backward(self, tape, gy, weight, residual=None):
         """(gx, g_weight, g_bias) of LayerNorm at what the tape stands for; gx (the type and shape of gy) has `residual`,
         the gradient that comes past the norm, added to it; the gradients of weight and bias are float32."""
-        torch = _torch()
         codes, exponents, rows, channels = self._tape(tape)
-        gy, g_rows, g_channels, stride = self._matrix(gy, "gy", _DTYPES)
-        if (g_rows, g_channels) != (rows, channels):
+        g_rows, g_channels, stride = self._matrix(gy, "gy", _DTYPES)
+        if g_rows != rows or g_channels != channels:
             _shape_error("gy", gy.shape, codes.shape)
-        weight = self._vector(weight, "weight", (torch.float16,), channels)
-        r_stride = channels
+        self._vector(weight, "weight", _F16, channels)
+        past, past_stride = None, channels
         if residual is not None:
-            residual, r_rows, r_channels, r_stride = self._matrix(residual, "residual", (gy.dtype,))
-            if (r_rows, r_channels) != (rows, channels):
+            r_rows, r_channels, past_stride = self._matrix(residual, "residual", (gy.dtype,))
+            if r_rows != rows or r_channels != channels:
                 _shape_error("residual", residual.shape, gy.shape)
-        gx = gy.new_empty(gy.shape)
-        g = gy.new_empty((2, channels), dtype=torch.float32)
+            past = residual.data_ptr()
+        gx = _like(gy, gy.dtype)
+        g = gy.new_empty((2, channels), dtype=_TORCH.float32)
         at = g.data_ptr()
         work, size = self._workspace(gy, "tape_layer_norm_backward", rows, channels)
         self._check(self._lib.ullis_cuda_tape_layer_norm_backward(
-            self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], _p(codes), _p(exponents), _p(gy), stride, _p(weight),
-            _p(residual), r_stride, rows, channels, _p(gx), at,
-            at + 4 * channels, _p(work), size))
-        return (gx, *g.unbind(0))
+            self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], codes.data_ptr(), exponents.data_ptr(), gy.data_ptr(), stride,
+            weight.data_ptr(), past, past_stride, rows, channels, gx.data_ptr(), at, at + 4 * channels, work.data_ptr(), size))
+        g_weight, g_bias = g.unbind(0)
+        return gx, g_weight, g_bias
 
     def tape_weight_grad(self, tape, gy):
         """Gradient of a linear's weights, float32 [out, in]: gy [..., out] (float16, bfloat16) transposed times what the tape
         of the linear's input stands for."""
-        torch = _torch()
         codes, exponents, rows, channels = self._tape(tape)
-        gy, g_rows, out, stride = self._matrix(gy, "gy", _16)
+        g_rows, out, stride = self._matrix(gy, "gy", _16)
         if g_rows != rows:
             _shape_error("gy", gy.shape, (rows, out))
-        g = gy.new_empty((out, channels), dtype=torch.float32)
+        g = gy.new_empty((out, channels), dtype=_TORCH.float32)
         work, size = self._workspace(gy, "tape_weight_grad", rows, channels, out)
         self._check(self._lib.ullis_cuda_tape_weight_grad(
-            self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], _p(codes), _p(exponents), _p(gy), stride, rows,
-            channels, out, _p(g), _p(work), size))
+            self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], codes.data_ptr(), exponents.data_ptr(), gy.data_ptr(), stride, rows,
+            channels, out, g.data_ptr(), work.data_ptr(), size))
         return g
 
     # ------------------------------------------------------------------------------------------ head
@@ -236,37 +248,37 @@ class DeviceOps:
         `weight` [vocab, channels] in hidden's type and no scale.  bias float16 [vocab] or None.  Gradients are of
         loss_scale * sum of row_loss; that of a packed weight is of the +/-1 values."""
         torch = _torch()
-        hidden, rows, channels, stride = self._matrix(hidden, "hidden", _16)
-        labels = self._vector(labels, "labels", (torch.int32,), rows)
+        rows, channels, stride = self._matrix(hidden, "hidden", _16)
+        self._vector(labels, "labels", _I32, rows)
         if time is None:
             time = hidden.shape[-2] if hidden.dim() == 3 else max(rows, 1)
         if scale is not None:
-            scale = self._tensor(scale, "scale", (torch.float16,))
+            self._refuse(scale, "scale", _F16)
             vocab = scale.numel()
-            scale = self._vector(scale, "scale", (torch.float16,), vocab)
-            weight = self._vector(weight, "weight", (torch.int32,), (vocab * channels + 31) // 32)
+            self._vector(scale, "scale", _F16, vocab)
+            self._vector(weight, "weight", _I32, (vocab * channels + 31) // 32)
         else:
-            weight = self._tensor(weight, "weight", (hidden.dtype,))
+            self._refuse(weight, "weight", (hidden.dtype,))
             if weight.dim() != 2 or weight.shape[1] != channels or not weight.is_contiguous():
                 _shape_error("weight", weight.shape, ("vocab", channels))
             vocab = weight.shape[0]
         if bias is not None:
-            bias = self._vector(bias, "bias", (torch.float16,), vocab)
-        ignore = int(ignore_id)
+            self._vector(bias, "bias", _F16, vocab)
+        ignore, time = int(ignore_id), int(time)
         if not -(1 << 31) <= ignore < 1 << 32:
             raise UllisCudaError(ERR_ARG, "ignore_id is not a 32-bit number")
-        if not 0 < int(time) < 1 << 31 or rows % int(time):
+        if not 0 < time < 1 << 31 or rows % time:
             raise UllisCudaError(ERR_SHAPE, "rows must be a multiple of time")
         row_loss = hidden.new_empty((rows,), dtype=torch.float32)
-        g_hidden = hidden.new_empty(hidden.shape)
+        g_hidden = _like(hidden, hidden.dtype)
         g_weight = hidden.new_empty((vocab, channels))
-        g_scale = None if scale is None else hidden.new_empty((vocab,), dtype=torch.float32)
-        g_bias = None if bias is None else hidden.new_empty((vocab,), dtype=torch.float32)
+        g_scale = None if scale is None else _like(scale, torch.float32)
+        g_bias = None if bias is None else _like(bias, torch.float32)
         work, size = self._workspace(hidden, "head_ce_grad", rows, channels, vocab)
-        packed = scale is not None
+        at = weight.data_ptr()
         self._check(self._lib.ullis_cuda_head_ce_grad(
-            self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], _p(hidden), stride, _p(weight if packed else None),
-            _p(None if packed else weight), _p(scale), _p(bias), _p(labels), ignore & 0xFFFFFFFF, rows,
-            int(time), channels, vocab, float(loss_scale), _p(row_loss), _p(g_hidden), _p(g_weight), _p(g_scale),
-            _p(g_bias), _p(work), size))
+            self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], hidden.data_ptr(), stride, at if scale is not None else None,
+            at if scale is None else None, _p(scale), _p(bias), labels.data_ptr(), ignore & 0xFFFFFFFF, rows, time, channels, vocab,
+            float(loss_scale), row_loss.data_ptr(), g_hidden.data_ptr(), g_weight.data_ptr(), _p(g_scale), _p(g_bias),
+            work.data_ptr(), size))
         return HeadGrad(row_loss, g_hidden, g_weight, g_scale, g_bias)
