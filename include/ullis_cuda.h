@@ -267,6 +267,16 @@ ULLIS_CUDA_API int32_t ullis_cuda_model_train_step(ullis_cuda_train_state* state
                                                    const uint32_t* labels, uint32_t ignore_id, size_t batch,
                                                    size_t time, float learning_rate,
                                                    ullis_cuda_train_result* result);
+/* What the steps from here on keep on the device.  tape8: the residual stream of
+ * every layer between the forward and the backward pass in 8 bits (the tape of the
+ * operators on device memory below) instead of f32, a quarter of the memory; the
+ * gradients behind it are those at the values that the tape stands for.  head_pieces:
+ * the head's loss and gradients by pieces of the vocabulary instead of from rows x
+ * vocabulary logits in f32 and two copies of their gradient in 16 bits; the same
+ * numbers to gradient rounding, and not in ULLIS_CUDA_MODE_EXACT.  Both off (0) to
+ * begin with, and then every result is what it was.  Buffers of the form that is left
+ * are freed.  ULLIS_CUDA_ERR_SHAPE for tape8 above 8192 channels. */
+ULLIS_CUDA_API int32_t ullis_cuda_train_state_set_lean(ullis_cuda_train_state* state, int32_t tape8, int32_t head_pieces);
 /* Copies a tensor of the trained model or of its carry to the host by its
  * checkpoint name ("head.bits", "blocks.0.rosa.o.latent", "embedding.residual",
  * ...; src/model.rs:3428-3466); `bytes` must be the tensor's size. */

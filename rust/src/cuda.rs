@@ -1023,6 +1023,15 @@ impl CudaTrainState<'_, '_> {
         })
     }
 
+    /// Steps that keep little on the device: the residual stream in 8 bits between the forward and the backward
+    /// pass (`tape8`), the head's loss and gradients by pieces of the vocabulary (`head_pieces`).
+    pub fn set_lean(&mut self, tape8: bool, head_pieces: bool) -> Result<()> {
+        // SAFETY: `raw` is a live handle.
+        self.model.rt.check(unsafe {
+            sys::ullis_cuda_train_state_set_lean(self.raw, i32::from(tape8), i32::from(head_pieces))
+        })
+    }
+
     /// Reads one tensor of the trained model or of its carry back by checkpoint name
     /// (`"head.bits"`, `"blocks.0.rosa.o.latent"`, `"embedding.residual"`, ...).
     pub fn read_bytes(&self, name: &str, bytes: usize) -> Result<Vec<u8>> {

@@ -237,6 +237,7 @@ unsafe extern "C" {
         learning_rate: f32,
         result: *mut ullis_cuda_train_result,
     ) -> i32;
+    pub fn ullis_cuda_train_state_set_lean(state: *mut ullis_cuda_train_state, tape8: i32, head_pieces: i32) -> i32;
     pub fn ullis_cuda_train_state_read(
         state: *mut ullis_cuda_train_state,
         name: *const c_char,

@@ -877,6 +877,14 @@ int32_t ullis_cuda_model_train_step(ullis_cuda_train_state* state, const uint32_
     return guard_model(state->m, [&] { state->step(tokens, labels, ignore_id, batch, time, learning_rate, result); });
 }
 
+int32_t ullis_cuda_train_state_set_lean(ullis_cuda_train_state* state, int32_t tape8, int32_t head_pieces) {
+    if (!state) {
+        set_global_error("train state handle is null");
+        return ULLIS_CUDA_ERR_ARG;
+    }
+    return guard_model(state->m, [&] { state->set_lean(tape8 != 0, head_pieces != 0); });
+}
+
 int32_t ullis_cuda_train_state_read(ullis_cuda_train_state* state, const char* name, void* dst, size_t bytes) {
     if (!state) {
         set_global_error("train state handle is null");

@@ -34,6 +34,15 @@ struct Rows {
     size_t stride;
 };
 
+struct Tape8 {   // a tape of [rows, channels] in a buffer of its own
+    uint8_t *codes, *exponents;
+    Tape8(DeviceBuffer& buffer, size_t rows, size_t channels) {
+        const size_t bytes = (rows * channels + 255) / 256 * 256;
+        codes = buffer.as<uint8_t>(bytes + rows * ((channels + 31) / 32));
+        exponents = codes + bytes;
+    }
+};
+
 // ---- the 8-bit tape (tape.cuh); codes [rows, channels] and exponents [rows, ceil(channels / 32)] without gaps
 void tape_pack(const Stream& s, int dtype, Rows x, size_t rows, size_t channels, uint8_t* codes, uint8_t* exponents);
 void tape_unpack(const Stream& s, int dtype, const uint8_t* codes, const uint8_t* exponents, size_t rows, size_t channels, void* x,
@@ -52,8 +61,9 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
 
 // ---- cross-entropy of a head with its gradient
 struct HeadGrad {
-    int dtype;                 // of hidden and of the 16-bit outputs: F16 or BF16; hidden F32 (hidden_f32) is rounded to F16
-    bool hidden_f32;
+    int dtype;                 // of the products' operands, hidden and the gradients: F16 or BF16
+    bool hidden_f32, out_f32;  // hidden comes in f32 (and is rounded to F16); the gradients leave in f32
+    bool fold_scale;           // F16: g_weight is that of the weights with their scale, sum of g * hidden; no g_scale
     Rows hidden;               // [rows, channels]
     const uint32_t* bits;      // packed signs, or null and
     const void* weight;        // dense [vocab, channels] of `dtype`

@@ -161,13 +161,14 @@ combine_kernel(const float* __restrict__ partial, uint32_t splits, size_t n, con
 }
 
 struct Output {
-    void* out;             // 16 bits, or null: `accum` is left
+    void* out;             // 16 bits or (f32) f32; null: `accum` is left
+    bool f32;
     float* accum;
     bool accum_read;
     const float* factor;
     float* partial;
 };
-// A 16-bit product out of `cut`
+// A product, alpha * (a . b + accum)
 void product(const Stream& s, const char* what, const Operand& a, const Operand& b, bool bf16, size_t M, size_t N, size_t K, const Cut& cut,
              const Output& o) {
     pg::Params p{};
@@ -176,6 +177,7 @@ void product(const Stream& s, const char* what, const Operand& a, const Operand&
     p.K = (uint32_t)K;
     p.splits = cut.splits;
     p.out = o.out;
+    p.out_f32 = o.f32;
     p.accum = o.accum;
     p.accum_read = o.accum_read;
     p.factor = o.factor;
@@ -186,7 +188,9 @@ void product(const Stream& s, const char* what, const Operand& a, const Operand&
     if (cut.splits == 1) return;
     const size_t n = M * N;
     const unsigned grid = (unsigned)ceil_div(n, 4 * THREADS);
-    if (bf16) s.chain("combine", combine_kernel<__nv_bfloat16>, grid, THREADS, 0, o.partial, cut.splits, n, o.factor, o.accum, (uint32_t)o.accum_read,
+    if (o.f32) s.chain("combine", combine_kernel<float>, grid, THREADS, 0, o.partial, cut.splits, n, o.factor, o.accum, (uint32_t)o.accum_read,
+                       static_cast<float*>(o.out));
+    else if (bf16) s.chain("combine", combine_kernel<__nv_bfloat16>, grid, THREADS, 0, o.partial, cut.splits, n, o.factor, o.accum, (uint32_t)o.accum_read,
                       static_cast<__nv_bfloat16*>(o.out));
     else s.chain("combine", combine_kernel<__half>, grid, THREADS, 0, o.partial, cut.splits, n, o.factor, o.accum, (uint32_t)o.accum_read,
                  static_cast<__half*>(o.out));
@@ -212,6 +216,8 @@ struct HeadOperands {
     float* scale_max;
     uint32_t hidden_ctas;
     uint32_t bf16;
+    uint32_t fold;              // weights +/-scale instead of +/-1 (FP16 has both)
+    uint32_t* status;           // hidden in f32: a finite value beyond FP16 is reported
 };
 constexpr uint32_t WEIGHT_CTAS = 1024;
 
@@ -255,8 +261,12 @@ head_operands_kernel(const HeadOperands o) {
                     for (int e = 0; e < 8; ++e)
                         if (c + e < o.D) {
                             uint16_t h;
-                            if constexpr (sizeof(T) == 4) h = __half_as_ushort(__float2half_rn(from[e]));
-                            else h = *reinterpret_cast<const uint16_t*>(from + e);
+                            if constexpr (sizeof(T) == 4) {
+                                const float v = from[e];
+                                if (fabsf(v) > 65504.0f && fabsf(v) <= 3.4028234e38f &&
+                                    atomicCAS(o.status, ULLIS_DEV_OK, ULLIS_DEV_FP16_RANGE) == ULLIS_DEV_OK) o.status[1] = row;
+                                h = __half_as_ushort(__float2half_rn(v));
+                            } else h = *reinterpret_cast<const uint16_t*>(from + e);
                             w[e >> 1] |= (uint32_t)h << (16 * (e & 1));
                         }
                 }
@@ -276,9 +286,10 @@ head_operands_kernel(const HeadOperands o) {
         for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
         if (lane == 0) {
             o.target[row] = target;
+            if (o.fold && target >= 0) dot *= __half2float(__ushort_as_half(o.scale[target]));
             o.target_acc[row] = dot;
             if (target >= 0) {
-                if (o.scale) dot *= __half2float(__ushort_as_half(o.scale[target]));
+                if (o.scale && !o.fold) dot *= __half2float(__ushort_as_half(o.scale[target]));
                 if (o.bias) dot += __half2float(__ushort_as_half(o.bias[target]));
             }
             o.logit2[row] = dot * pg::LOG2E;
@@ -295,10 +306,11 @@ head_operands_kernel(const HeadOperands o) {
         uint32_t w[4] = {};
         if (o.bits) {
             const uint32_t signs = signs8(o.bits, v * o.D + c, words);
+            const uint32_t one = o.fold ? o.scale[v] : plus;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (c + e < o.D) w[e >> 1] |= (plus | ((signs >> e) & 1u ? 0u : 0x8000u)) << (16 * (e & 1));
-            if (c == 0) top = fmaxf(top, fabsf(__half2float(__ushort_as_half(o.scale[v]))));
+                if (c + e < o.D) w[e >> 1] |= (one ^ ((signs >> e) & 1u ? 0u : 0x8000u)) << (16 * (e & 1));
+            if (c == 0 && !o.fold) top = fmaxf(top, fabsf(__half2float(__ushort_as_half(o.scale[v]))));
         } else {
             const uint16_t* from = o.dense + v * o.D + c;
 #pragma unroll
@@ -307,7 +319,7 @@ head_operands_kernel(const HeadOperands o) {
         }
         *reinterpret_cast<uint4*>(o.w16 + v * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if (!o.bits) return;
+    if (!o.bits || o.fold) return;
     __shared__ float tops[THREADS / 32];
     for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
@@ -325,7 +337,7 @@ struct HeadRows {
     const int32_t* target;
     const float* logit2;
     float *lse2, *row_loss;
-    const float* scale_max;   // null: dense weights
+    const float* scale_max;   // null: no row scales
     float* factors;           // 2^k, 2^-k * loss_scale
     float loss_scale;
 };
@@ -517,6 +529,8 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     o.scale_max = reinterpret_cast<float*>(ws + p.scale_max);
     o.hidden_ctas = (uint32_t)ceil_div(rows, THREADS / 32);
     o.bf16 = bf16;
+    o.fold = h.fold_scale;
+    o.status = s.status;
     const unsigned grid = o.hidden_ctas + (as_is ? 0 : WEIGHT_CTAS);
     if (h.hidden_f32) s.chain("head_operands", head_operands_kernel<float>, grid, THREADS, 0, o);
     else s.chain("head_operands", head_operands_kernel<__half>, grid, THREADS, 0, o);   // (moved, not read: bf16 too)
@@ -526,7 +540,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     q.M = (uint32_t)rows;
     q.N = (uint32_t)V;
     q.K = (uint32_t)D;
-    q.scale = h.bits ? h.scale : nullptr;
+    q.scale = h.bits && !h.fold_scale ? h.scale : nullptr;
     q.bias = h.bias;
     q.target = o.target;
     q.piece_tiles = p.lse_tiles;
@@ -551,7 +565,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     r.logit2 = o.logit2;
     r.lse2 = reinterpret_cast<float*>(ws + p.lse2);
     r.row_loss = h.row_loss;
-    r.scale_max = h.bits ? o.scale_max : nullptr;
+    r.scale_max = q.scale ? o.scale_max : nullptr;
     r.factors = factors;
     r.loss_scale = h.loss_scale;
     s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 32), 128, 0, r);
@@ -582,13 +596,13 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
         wp.mn = true;
         const bool last = piece + 1 == p.pieces;
         product(s, "head_g_hidden", by_rows, wp, bf16, rows, D, width, p.hidden,
-                Output{last ? h.g_hidden : nullptr, p.pieces > 1 ? reinterpret_cast<float*>(ws + p.accum) : nullptr, piece > 0, factors + 1,
+                Output{last ? h.g_hidden : nullptr, h.out_f32, p.pieces > 1 ? reinterpret_cast<float*>(ws + p.accum) : nullptr, piece > 0, factors + 1,
                        reinterpret_cast<float*>(ws + p.partial)});
         const Operand by_columns{grad, rows, width, p.piece, true};
         Operand hc = hidden;
         hc.mn = true;
         product(s, "head_g_weight", by_columns, hc, bf16, width, D, rows, p.weight,
-                Output{static_cast<uint16_t*>(h.g_weight) + v0 * D, nullptr, false, factors + 1, reinterpret_cast<float*>(ws + p.partial)});
+                Output{static_cast<uint8_t*>(h.g_weight) + v0 * D * (h.out_f32 ? 4 : 2), h.out_f32, nullptr, false, factors + 1, reinterpret_cast<float*>(ws + p.partial)});
     }
 }
 

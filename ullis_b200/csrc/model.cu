@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cstring>
 
+#include "device_ops.hpp"
 #include "kernels.hpp"
 #include "linear_tc.hpp"
 #include "safetensors.hpp"
@@ -396,9 +397,13 @@ void ullis_cuda_model::enqueue_layer(const Lane& ln, size_t l, size_t time) {
         k::binary_linear_exact(r, A, L.o.bits, L.o.scale, L.o.bias, X, rows, d, d, true);  // x += rosa out
     }
     save_tap((int)l, ULLIS_CUDA_TAP_AFTER_ROSA, X, n * 4);
-    if (train_tape)
+    if (train_tape && train_tape8) {
+        const dev::Tape8 kept(tape_after[l], rows, d);
+        dev::tape_pack(dev::Stream{r, r->stream, r->dev_status}, dev::F32, dev::Rows{X, d}, rows, d, kept.codes, kept.exponents);
+    } else if (train_tape) {
         ULLIS_CUDA_CHECK(cudaMemcpyAsync(tape_after[l].as<float>(n), X, n * 4, cudaMemcpyDeviceToDevice,
                                          r->stream));
+    }
     end(r);
 
     begin(PH_CMIX, r);

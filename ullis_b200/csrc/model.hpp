@@ -52,6 +52,7 @@ struct ullis_cuda_model {
     // training tape: the residual stream after each ROSA block and the idx bits, kept per layer
     bool train_tape = false;
     std::vector<ullis::DeviceBuffer> tape_after, tape_idx;
+    bool train_tape8 = false;   // the residual stream in 8 bits (tape.cuh): codes, then exponents, in tape_after
 
     // taps
     bool taps_enabled = false;

@@ -71,7 +71,8 @@ struct Params {
     float* col_part;           // GRAD: [slot][8][2][pitch]
     // STORE, SUM
     uint32_t splits;           // of K
-    void* out;                 // 16 bits [M][N] (STORE) or f32 [M][N] (SUM), where nothing follows
+    void* out;                 // 16 bits [M][N] (STORE) or f32 [M][N] (SUM, STORE with out_f32), where nothing follows
+    uint32_t out_f32;
     float* accum;              // f32 [M][N]; STORE: read first if `accum_read`, written unless `out` is
     uint32_t accum_read;
     float* partial;            // splits > 1: [split][M][N]
@@ -702,7 +703,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 if (!filled(&taddr)) break;
                 const uint32_t m0 = work.m * BM + rank * 128 + quarter * 32;
                 float* partial = p.splits > 1 ? p.partial + (size_t)work.split * p.M * p.N : nullptr;
-                const bool to16 = !partial && p.out;
+                const bool to16 = !partial && p.out && !p.out_f32;
 #pragma unroll 1
                 for (uint32_t part = 0; part < 2 * ACCS; ++part) {
                     const uint32_t h = part & 1, c0 = (group * ACCS + (part >> 1)) * 64, n0 = work.n * BN * ACCS + c0;
@@ -713,7 +714,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     float v[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                    const auto f32_rows = [&](float* at, bool read, bool write) {
+                    const auto f32_rows = [&](float* at, bool read, bool write, float times) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const uint32_t row = m0 + h * 16 + r0 + i * 8;
@@ -727,17 +728,18 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                                     if (c < p.N) {
                                         float2* both = reinterpret_cast<float2*>(line + c);
                                         if (read) { const float2 old = *both; x += old.x; y += old.y; }
-                                        if (write) *both = make_float2(x, y);
+                                        if (write) *both = make_float2(x * times, y * times);
                                     }
                                 } else {
-                                    if (c < p.N) { if (read) x += line[c]; if (write) line[c] = x; }
-                                    if (c + 1 < p.N) { if (read) y += line[c + 1]; if (write) line[c + 1] = y; }
+                                    if (c < p.N) { if (read) x += line[c]; if (write) line[c] = x * times; }
+                                    if (c + 1 < p.N) { if (read) y += line[c + 1]; if (write) line[c + 1] = y * times; }
                                 }
                             }
                         }
                     };
-                    if (partial) { f32_rows(partial, false, true); continue; }
-                    if (p.accum) f32_rows(p.accum, p.accum_read, !to16);
+                    if (partial) { f32_rows(partial, false, true, 1.0f); continue; }
+                    if (p.accum) f32_rows(p.accum, p.accum_read, !p.out, 1.0f);
+                    if (p.out && p.out_f32) f32_rows(static_cast<float*>(p.out), false, true, alpha);
                     if (!to16) continue;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)

@@ -22,6 +22,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "device_ops.hpp"
 #include "kernels.hpp"
 #include "linear_tc.hpp"
 #include "safetensors.hpp"
@@ -870,15 +871,22 @@ struct Step {
     void packed_update(PackedParam& p, const uint16_t* gy16t, const uint16_t* x16t, size_t rows_p, unsigned long long* flips, float* small) {
         const size_t out_f = p.weights->out, in_f = p.weights->in;
         float* G = st->gmat.as<float>(out_f * in_f);
+        tc::Partials g{G, 1};
+        if (packed_rows(p)) gemm(gy16t, x16t, G, out_f, rows_p, in_f, &g);
+        else gemm(gy16t, x16t, G, out_f, rows_p, in_f);   // a word has bits of two rows: the shares are added first
+        packed_step(p, g, flips, small);
+    }
+    static bool packed_rows(const PackedParam& p) { return p.weights->in % 32 == 0 && p.weights->out < ((size_t)1 << 31); }
+    // ... the steps from G (one share of it, unless the rows are whole words)
+    void packed_step(PackedParam& p, const tc::Partials& g, unsigned long long* flips, float* small) {
+        const size_t out_f = p.weights->out, in_f = p.weights->in;
+        const float* G = g.sums;
         uint32_t* bits = const_cast<uint32_t*>(p.weights->bits);
-        if (in_f % 32 == 0 && out_f < ((size_t)1 << 31)) {
-            tc::Partials g{};
-            gemm(gy16t, x16t, G, out_f, rows_p, in_f, &g);
+        if (packed_rows(p)) {
             rt->chain(packed_step_kernel, (unsigned)out_f, 32 * PACKED_WARPS, 0, p.latent, p.latent_residual, g.sums, g.count,
                       p.scale.w, p.scale.residual, bits, out_f * in_f, (uint32_t)in_f, gmul, ste, lr, flips);
             rt->launched("packed_step");
-        } else {   // a word has bits of two rows
-            gemm(gy16t, x16t, G, out_f, rows_p, in_f);
+        } else {
             rt->chain(g_scale_kernel, blocks_for(out_f, 8), 256, 0, G, bits, small, out_f, in_f);
             rt->launched("g_scale");
             rt->chain(latent_sgd_kernel, blocks_for(out_f * in_f, 256 * LATENT_WORDS), 256, 0, p.latent, p.latent_residual, G,
@@ -1051,6 +1059,19 @@ void ullis_cuda_train_state::read(const char* name, void* dst, size_t bytes) {
     rt->sync();
 }
 
+void ullis_cuda_train_state::set_lean(bool tape8_, bool head_pieces_) {
+    if (tape8_ && m->d > dev::TAPE_NORM_CHANNELS) fail(ULLIS_CUDA_ERR_SHAPE, "the 8-bit tape takes at most 8192 channels");
+    rt->bind();
+    rt->sync();
+    // what the other form kept goes back
+    if (tape8_ != tape8) m->tape_after.clear();
+    if (head_pieces_ != head_pieces)
+        for (DeviceBuffer* b : {&logits, &a16, &t16, &part, &lean}) b->release();
+    if (!tape8_ && !head_pieces_) lean.release();
+    tape8 = tape8_;
+    head_pieces = head_pieces_;
+}
+
 // ------------------------------------------------------------ the step
 void ullis_cuda_train_state::step(const uint32_t* tokens, const uint32_t* labels_h, uint32_t ignore_id, size_t batch,
                                   size_t time, float learning_rate, ullis_cuda_train_result* out) {
@@ -1063,6 +1084,9 @@ void ullis_cuda_train_state::step(const uint32_t* tokens, const uint32_t* labels
     for (size_t r = 0; r < rows; ++r)
         if (tokens[r] >= vocab || (labels_h[r] != ignore_id && labels_h[r] >= vocab))
             fail(ULLIS_CUDA_ERR_SHAPE, "token shape or context length is invalid");
+    const bool exact = rt->mode == ULLIS_CUDA_MODE_EXACT;
+    if (head_pieces && (exact || rt->cc_major != 10))
+        fail(ULLIS_CUDA_ERR_ARG, "a head in pieces needs ULLIS_CUDA_MODE_FAST on an sm_100 device");
     rt->bind();
 
     // rows of each distinct token, in row order, for the embedding step
@@ -1086,16 +1110,17 @@ void ullis_cuda_train_state::step(const uint32_t* tokens, const uint32_t* labels
     // forward with the tape
     m->upload_tokens(tokens, labels_h, batch, time);
     m->train_tape = true;
+    m->train_tape8 = tape8;
     try {
         m->enqueue_hidden(batch, time);
     } catch (...) {
-        m->train_tape = false;
+        m->train_tape = m->train_tape8 = false;
         throw;
     }
-    m->train_tape = false;
+    m->train_tape = m->train_tape8 = false;
 
     const size_t n = rows * d, rows_p = pad64(rows), vocab_p = pad64(vocab), d_p = pad64(d), f_p = pad64(f);
-    const bool exact = rt->mode == ULLIS_CUDA_MODE_EXACT;
+    const dev::Stream own{rt, rt->stream, rt->dev_status};
     float P = 1.0f;
     while (P < (float)(time - 1)) P *= 2.0f;
     Step s{this, rt, 1.0f / P, learning_rate, (float)(time - 1)};
@@ -1107,38 +1132,66 @@ void ullis_cuda_train_state::step(const uint32_t* tokens, const uint32_t* labels
     float* T3 = t3.as<float>(n);
     float* W1 = wide1.as<float>(rows * f);
     float* W2 = wide2.as<float>(rows * f);
-    float* LG = logits.as<float>(rows * vocab);
-    const size_t widest = std::max({f_p, vocab_p, d_p});
+    float* LG = head_pieces ? nullptr : logits.as<float>(rows * vocab);
+    const size_t head_p = head_pieces ? 0 : vocab_p;   // what the head takes of the buffers below
+    const size_t widest = std::max({f_p, head_p, d_p});
     uint16_t* A16 = a16.as<uint16_t>(rows * widest);
     uint16_t* B16 = b16.as<uint16_t>(std::max(d * rows_p, widest * std::max(f, d)));
-    uint16_t* T16 = t16.as<uint16_t>(std::max(vocab, d + 2 * f) * rows_p);
-    float* SM = small.as<float>(std::max({f, vocab, d}));   // gradients of a packed matrix's scales
+    uint16_t* T16 = t16.as<uint16_t>(std::max(head_pieces ? 0 : vocab, d + 2 * f) * rows_p);
+    float* SM = small.as<float>(std::max({f, vocab, 2 * d}));   // gradients of a packed matrix's scales
     unsigned long long* CNT = counters.as<unsigned long long>(3);
     const uint32_t* lab = m->labels.as<uint32_t>(rows);
     float* RL = m->row_loss.as<float>(rows);
     uint8_t* res = static_cast<uint8_t*>(m->result.ensure(16));
     rt->zero(CNT, 24);
     gmat.as<float>(std::max({d * f, vocab * d, d * d}));                        // sized once: no growth mid-step
-    part.as<float>((rows + 255) / 256 * std::max({f, vocab, 2 * d}));
+    part.as<float>((rows + 255) / 256 * std::max({f, head_pieces ? 0 : vocab, 2 * d}));
 
     // ---- head: logits, loss, gy (src/model.rs:3204-3257)
-    if (!tc::binary_linear(rt, H, m->head.bits, m->head.scale, m->head.bias, LG, rows, d, vocab))
-        k::binary_linear_exact(rt, H, m->head.bits, m->head.scale, m->head.bias, LG, rows, d, vocab, false);
-    rt->chain(ce_grad_kernel, (unsigned)rows, 256, 0, LG, lab, ignore_id, rows, time, vocab,
-                                                          1.0f / (float)(time - 1), P, RL, rt->dev_status);
-    rt->launched("ce_grad");
-    k::ce_reduce(rt, RL, lab, ignore_id, rows, time, reinterpret_cast<double*>(res),
-                 reinterpret_cast<unsigned long long*>(res + 8));
-    m->have_result = true;
-    if (head.bias.w) {   // not used again in this step
-        s.col_gradient(LG, nullptr, rows, vocab, COL_SUM);
-        s.col_step(head.bias, rows, learning_rate * HEAD_BIAS_LR_MULT);
+    const auto reduce_loss = [&] {
+        k::ce_reduce(rt, RL, lab, ignore_id, rows, time, reinterpret_cast<double*>(res), reinterpret_cast<unsigned long long*>(res + 8));
+        m->have_result = true;
+    };
+    if (head_pieces) {
+        dev::HeadGrad h{};
+        h.dtype = dev::F16;
+        h.hidden_f32 = h.out_f32 = h.fold_scale = true;
+        h.hidden = dev::Rows{H, d};
+        h.bits = m->head.bits;
+        h.scale = m->head.scale;
+        h.bias = m->head.bias;
+        h.labels = lab;
+        h.ignore_id = ignore_id;
+        h.rows = rows;
+        h.time = time;
+        h.channels = d;
+        h.vocab = vocab;
+        h.loss_scale = 1.0f / (float)(time - 1) * P;
+        h.row_loss = RL;
+        h.g_hidden = GX;
+        h.g_weight = gmat.as<float>(vocab * d);
+        h.g_bias = head.bias.w ? SM : nullptr;
+        dev::head_ce_grad(own, h, lean.ensure(dev::head_ce_grad_workspace(rt, rows, d, vocab)));
+        reduce_loss();
+        if (head.bias.w) s.sgd(head.bias, SM, learning_rate * HEAD_BIAS_LR_MULT);
+        s.packed_step(head, tc::Partials{gmat.as<float>(vocab * d), 1}, CNT + 0, SM);
+    } else {
+        if (!tc::binary_linear(rt, H, m->head.bits, m->head.scale, m->head.bias, LG, rows, d, vocab))
+            k::binary_linear_exact(rt, H, m->head.bits, m->head.scale, m->head.bias, LG, rows, d, vocab, false);
+        rt->chain(ce_grad_kernel, (unsigned)rows, 256, 0, LG, lab, ignore_id, rows, time, vocab,
+                                                              1.0f / (float)(time - 1), P, RL, rt->dev_status);
+        rt->launched("ce_grad");
+        reduce_loss();
+        if (head.bias.w) {   // not used again in this step
+            s.col_gradient(LG, nullptr, rows, vocab, COL_SUM);
+            s.col_step(head.bias, rows, learning_rate * HEAD_BIAS_LR_MULT);
+        }
+        s.operands(LG, m->head.scale, A16, T16, rows, vocab, rows_p);                   // (gy*scale) [rows, V], gy^T [V, rows]
+        s.unpack_transpose(m->head.bits, B16, vocab, d, vocab_p);                       // S^T [d, V]
+        s.gemm(A16, B16, GX, rows, vocab_p, d);                                         // g_hidden
+        s.operands(H, nullptr, nullptr, B16, rows, d, rows_p);                          // hidden^T [d, rows]
+        s.packed_update(head, T16, B16, rows_p, CNT + 0, SM);
     }
-    s.operands(LG, m->head.scale, A16, T16, rows, vocab, rows_p);                   // (gy*scale) [rows, V], gy^T [V, rows]
-    s.unpack_transpose(m->head.bits, B16, vocab, d, vocab_p);                       // S^T [d, V]
-    s.gemm(A16, B16, GX, rows, vocab_p, d);                                         // g_hidden
-    s.operands(H, nullptr, nullptr, B16, rows, d, rows_p);                          // hidden^T [d, rows]
-    s.packed_update(head, T16, B16, rows_p, CNT + 0, SM);
 
     // ---- ln_out
     s.ln_backward(X, GX, ln_out_w, ln_out_b, T1, false, rows, d);
@@ -1147,7 +1200,13 @@ void ullis_cuda_train_state::step(const uint32_t* tokens, const uint32_t* labels
     for (size_t li = m->layers; li-- > 0;) {
         LayerWeights& L = m->blocks[li];
         Layer& T = layers[li];
-        const float* AR = m->tape_after[li].as<float>(n);   // residual stream after the ROSA block
+        const float* AR = T3;   // residual stream after the ROSA block
+        if (tape8) {
+            const dev::Tape8 kept(m->tape_after[li], rows, d);
+            dev::tape_unpack(own, dev::F32, kept.codes, kept.exponents, rows, d, T3, d);
+        } else {
+            AR = m->tape_after[li].as<float>(n);
+        }
         // ---- CMix: recompute ln2 -> shifted -> key from the tape (src/model.rs:1050-1061)
         k::layer_norm(rt, AR, L.ln2.weight, L.ln2.bias, T1, rows, d, exact);
         k::shift_mix(rt, T1, L.ffn_x_k, nullptr, nullptr, T2, nullptr, nullptr, rows, time, d);     // shifted
@@ -1185,7 +1244,16 @@ void ullis_cuda_train_state::step(const uint32_t* tokens, const uint32_t* labels
             rt->chain(lerp_bwd_kernel<1>, blocks_for(n, 256), 256, 0, T3, L.ffn_x_k, T1, (uint32_t)rows, (uint32_t)time, (uint32_t)d);
         rt->launched("lerp_bwd");
         s.col_step(T.x_k, rows, learning_rate);                                                       // after its last use
-        s.ln_backward(AR, T1, T.ln2_w, T.ln2_b, GX, true, rows, d);
+        if (tape8) {
+            const dev::Tape8 kept(m->tape_after[li], rows, d);
+            float* g = small.as<float>(2 * d);   // of the weight, then of the bias
+            dev::tape_layer_norm_backward(own, dev::F32, kept.codes, kept.exponents, dev::Rows{T1, d}, T.ln2_w.w, dev::Rows{GX, d}, rows, d,
+                                          GX, g, g + d, lean.ensure(dev::tape_layer_norm_backward_workspace(rt, rows, d)));
+            s.sgd(T.ln2_w, g, learning_rate);
+            s.sgd(T.ln2_b, g + d, learning_rate);
+        } else {
+            s.ln_backward(AR, T1, T.ln2_w, T.ln2_b, GX, true, rows, d);
+        }
 
         // ---- ROSA: gradients stop at the q/k/v bits (src/model.rs:1494-1521)
         const uint32_t* idx = m->tape_idx[li].as<uint32_t>(1);

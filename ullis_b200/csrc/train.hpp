@@ -46,6 +46,12 @@ struct ullis_cuda_train_state {
         toks;
     uint64_t steps = 0;
 
+    // A step that keeps little (set_lean): the residual stream between forward and backward pass in 8 bits; the head's loss and
+    // gradients piece by piece of the vocabulary, without logits.
+    bool tape8 = false, head_pieces = false;
+    ullis::DeviceBuffer lean;   // workspaces of the operators that these take
+    void set_lean(bool tape8, bool head_pieces);
+
     ullis_cuda_train_state(ullis_cuda_model* model, const uint8_t* checkpoint, size_t len);
     void step(const uint32_t* tokens, const uint32_t* labels, uint32_t ignore_id, size_t batch, size_t time,
               float learning_rate, ullis_cuda_train_result* out);

@@ -51,7 +51,7 @@ ABI_SYMBOLS = (
     "ullis_cuda_rosa_pushers_create", "ullis_cuda_rosa_pushers_destroy", "ullis_cuda_rosa_pushers_reset",
     "ullis_cuda_rosa_pushers_push",
     "ullis_cuda_train_state_create", "ullis_cuda_train_state_destroy", "ullis_cuda_model_train_step",
-    "ullis_cuda_train_state_read", "ullis_cuda_train_state_install_head_unigram_prior",
+    "ullis_cuda_train_state_set_lean", "ullis_cuda_train_state_read", "ullis_cuda_train_state_install_head_unigram_prior",
     "ullis_cuda_clipped_sgd_fp16", "ullis_cuda_binaryconnect_sgd_fp16", "ullis_cuda_apply_latent_sgd",
     "ullis_cuda_rosa_qkv_1bit_bwd_e", "ullis_cuda_cmix_relu2_backward", "ullis_cuda_layer_norm_backward",
     "ullis_cuda_layer_norm", "ullis_cuda_time_shift_delta",
@@ -808,6 +808,12 @@ class CudaTrainState:
             C.byref(res)))
         return {"loss": float(res.mean_loss), "n_valid": int(res.n_valid), "flips_head": int(res.flips_head),
                 "flips_cmix": int(res.flips_cmix), "flips_rosa_o": int(res.flips_rosa_o)}
+
+    def set_lean(self, tape8: bool = True, head_pieces: bool = True) -> None:
+        """Steps that keep little: the residual stream in 8 bits between forward and backward pass (tape8), the head's loss and
+        gradients by pieces of the vocabulary without logits (head_pieces)."""
+        self.model.rt._check(self._lib.ullis_cuda_train_state_set_lean(self._h, C.c_int32(1 if tape8 else 0),
+                                                                       C.c_int32(1 if head_pieces else 0)))
 
     def install_head_unigram_prior(self, labels, ignore_id: int) -> dict:
         """UllisHeron::install_head_unigram_prior (src/model.rs:3034-3085) -> HeadUnigramInstall fields."""
