@@ -123,40 +123,36 @@ Cut cut_of(size_t M, size_t N, size_t K, uint32_t pairs, bool two) {
 }
 size_t partial_bytes(size_t M, size_t N, const Cut& c) { return c.splits > 1 ? c.splits * M * N * 4 : 0; }
 
-// The sum of `splits` arrays of n elements, in their order, times alpha (the columns' factors) as 16 bits or f32; with `accum`
-// added to it, or left there where `out` is null.
+// The sum of `splits` arrays [M][N], in their order, times alpha as 16 bits or f32; with `accum` added to it, or left there where
+// `out` is null.  Of the M rows the first *counted, if given, and row m goes to row out_rows[m] of `out`.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
-combine_kernel(const float* __restrict__ partial, uint32_t splits, size_t n, const float* __restrict__ factor, float* __restrict__ accum,
-               uint32_t accum_read, T* __restrict__ out) {
+combine_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t M, uint32_t N, const float* __restrict__ factor, float* __restrict__ accum,
+               uint32_t accum_read, T* __restrict__ out, const uint32_t* __restrict__ counted, const int32_t* __restrict__ out_rows) {
     chain_entry();
-    const size_t i = ((size_t)blockIdx.x * THREADS + threadIdx.x) * 4;
-    if (i >= n) return;
+    const size_t n = (size_t)M * N, i = ((size_t)blockIdx.x * THREADS + threadIdx.x) * 4;
+    const size_t end = counted ? min((size_t)*counted, (size_t)M) * N : n;
+    if (i >= end) return;
     const float alpha = factor ? *factor : 1.0f;
-    const bool whole = i + 4 <= n && n % 4 == 0;   // (each of the arrays on 16 bytes)
+    const bool whole = N % 4 == 0;   // four elements of one row, each of the arrays on 16 bytes
     float v[4] = {};
-    const auto add = [&](const float* from) {
-        if (whole) {
-            const float4 t = *reinterpret_cast<const float4*>(from + i);
-            v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
-        } else {
-            for (int e = 0; e < 4; ++e) if (i + e < n) v[e] += from[i + e];
-        }
-    };
     if (whole) {
 #pragma unroll 8
-        for (uint32_t k = 0; k < splits; ++k) {
-            const float4 t = *reinterpret_cast<const float4*>(partial + k * n + i);
+        for (uint32_t k = 0; k < splits + (accum && accum_read); ++k) {
+            const float4 t = *reinterpret_cast<const float4*>((k < splits ? partial + k * n : accum) + i);
             v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
         }
     } else {
-        for (uint32_t k = 0; k < splits; ++k) add(partial + k * n);
+        for (uint32_t k = 0; k < splits + (accum && accum_read); ++k)
+            for (int e = 0; e < 4; ++e)
+                if (i + e < end) v[e] += (k < splits ? partial + k * n : accum)[i + e];
     }
-    if (accum && accum_read) add(accum);
+    uint32_t row = (uint32_t)(i / N), c = (uint32_t)(i - (size_t)row * N);
     for (int e = 0; e < 4; ++e) {
-        if (i + e >= n) break;
-        if (out) out[i + e] = tape::from_float<T>(v[e] * alpha);
+        if (i + e >= end) break;
+        if (out) out[(size_t)(out_rows ? out_rows[row] : (int32_t)row) * N + c] = tape::from_float<T>(v[e] * alpha);
         else accum[i + e] = v[e];
+        if (++c == N) { c = 0; ++row; }
     }
 }
 
@@ -167,6 +163,9 @@ struct Output {
     bool accum_read;
     const float* factor;
     float* partial;
+    const uint32_t* counted;   // pair_gemm.cuh: rows of the product, or (count_k) terms of its sums
+    bool count_k;
+    const int32_t* rows;       // where its rows go
 };
 // A product, alpha * (a . b + accum)
 void product(const Stream& s, const char* what, const Operand& a, const Operand& b, bool bf16, size_t M, size_t N, size_t K, const Cut& cut,
@@ -182,31 +181,81 @@ void product(const Stream& s, const char* what, const Operand& a, const Operand&
     p.accum_read = o.accum_read;
     p.factor = o.factor;
     p.partial = o.partial;
+    p.counted = o.counted;
+    p.count_k = o.count_k;
+    p.out_rows = o.rows;
     const uint32_t pairs = (uint32_t)std::min<size_t>(pairs_of(s.rt), ceil_div(M, 256) * ceil_div(N, 256 * cut.accs) * cut.splits);
     if (cut.accs == 2) launch<pg::STORE, 2>(s, what, a, b, bf16, p, pairs);
     else launch<pg::STORE, 1>(s, what, a, b, bf16, p, pairs);
     if (cut.splits == 1) return;
-    const size_t n = M * N;
-    const unsigned grid = (unsigned)ceil_div(n, 4 * THREADS);
-    if (o.f32) s.chain("combine", combine_kernel<float>, grid, THREADS, 0, o.partial, cut.splits, n, o.factor, o.accum, (uint32_t)o.accum_read,
-                       static_cast<float*>(o.out));
-    else if (bf16) s.chain("combine", combine_kernel<__nv_bfloat16>, grid, THREADS, 0, o.partial, cut.splits, n, o.factor, o.accum, (uint32_t)o.accum_read,
-                      static_cast<__nv_bfloat16*>(o.out));
-    else s.chain("combine", combine_kernel<__half>, grid, THREADS, 0, o.partial, cut.splits, n, o.factor, o.accum, (uint32_t)o.accum_read,
-                 static_cast<__half*>(o.out));
+    const unsigned grid = (unsigned)ceil_div(M * N, 4 * THREADS);
+    const auto combine = [&](auto kernel, auto* out) {
+        s.chain("combine", kernel, grid, THREADS, 0, static_cast<const float*>(o.partial), cut.splits, (uint32_t)M, (uint32_t)N, o.factor, o.accum,
+                (uint32_t)o.accum_read, out, o.count_k ? nullptr : o.counted, o.rows);
+    };
+    if (o.f32) combine(combine_kernel<float>, static_cast<float*>(o.out));
+    else if (bf16) combine(combine_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(o.out));
+    else combine(combine_kernel<__half>, static_cast<__half*>(o.out));
 }
 
 // ------------------------------------------------------------------------------------------------ operands of the head
-// Rows of hidden as the operand [rows, Dp] (columns from D on and rows that do not count are 0: what a masked row holds, an
-// infinity say, stays out of the products), the rows' targets (-1: does not count, -2: a label outside the vocabulary) and their
-// targets' logits in f32, the weights [vocab, Dp] (+/-1, or a copy of dense rows that no tensor map takes) and the largest |scale|
-// per CTA of that part.  A warp has a row of hidden, a thread a chunk of eight weights.
+// Which rows count: place[row] = the row's place among those that do, or -1 - its place among those that do not; list[place] = row
+// and how many there are.  A CTA has 1024 rows and counts those before them by itself (all labels are a few KB that lie in L2; one
+// CTA with a run of rows per warp took 18 us for 16 384).
+struct HeadLabels {
+    const uint32_t* labels;
+    uint32_t ignore_id, rows, time, vocab;
+    // the target of a row, -1 where it does not count (the last of its sequence, an ignored label), -2 for a label outside the vocabulary
+    __device__ int32_t target(uint32_t row) const {
+        const uint32_t label = labels[min(row + 1u, rows - 1u)];   // (always read, so that several are on their way)
+        if (row % time + 1u >= time || label == ignore_id) return -1;
+        return label < vocab ? (int32_t)label : -2;
+    }
+};
+__global__ void __launch_bounds__(1024)
+head_list_kernel(const HeadLabels l, int32_t* __restrict__ place, int32_t* __restrict__ list, uint32_t* __restrict__ counted) {
+    chain_entry();
+    __shared__ uint32_t counts[2][32];   // per warp: of the rows before, of its own
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = blockIdx.x * 1024, row = first + threadIdx.x;
+    uint32_t n = 0;
+#pragma unroll 8
+    for (uint32_t r = threadIdx.x; r < first; r += 1024) n += l.target(r) >= 0;
+    const bool mine = row < l.rows && l.target(row) >= 0;
+    const uint32_t mask = __ballot_sync(0xffffffffu, mine);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (lane == 0) {
+        counts[0][warp] = n;
+        counts[1][warp] = __popc(mask);
+    }
+    __syncthreads();
+    uint32_t at = counts[0][lane] + (lane < warp ? counts[1][lane] : 0u);   // counted before this warp's rows
+    uint32_t all = counts[0][lane] + counts[1][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        at += __shfl_xor_sync(0xffffffffu, at, o);
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    at += __popc(mask & ((1u << lane) - 1u));
+    if (mine) list[at] = (int32_t)row;
+    if (row < l.rows) place[row] = mine ? (int32_t)at : -1 - (int32_t)(row - at);
+    if (threadIdx.x == 0 && blockIdx.x + 1 == gridDim.x) *counted = all;
+}
+
+// The rows of hidden that count, one behind the other, as the operand [., Dp] (columns from D on 0, and rows up to a whole tile: what
+// other rows hold, an infinity say, stays out of the products), their targets, their targets' products and logits in f32, zeros (or
+// a NaN) for the others' losses and gradients; the weights [vocab, Dp] (+/-1, or a copy of dense rows that no tensor map takes) and
+// the largest |scale| per CTA of that part.  A warp has a row of hidden, a thread a chunk of eight weights.
 struct HeadOperands {
     const void* hidden;
     size_t stride;
-    uint32_t rows, time, D, Dp, vocab;
-    const uint32_t* labels;
-    uint32_t ignore_id;
+    uint32_t rows, D, Dp, vocab;
+    HeadLabels labels;
+    const int32_t* place;
+    const uint32_t* counted;
+    float* row_loss;
+    void* g_hidden;             // [rows, D]
+    uint32_t g_bytes;           // of a row of it
     uint16_t* h16;
     int32_t* target;
     float *target_acc, *logit2; // the target's product; its logit times log2 e
@@ -241,58 +290,64 @@ head_operands_kernel(const HeadOperands o) {
     if (blockIdx.x < o.hidden_ctas) {
         const uint32_t row = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
         if (row >= o.rows) return;
-        int32_t target = -1;
-        if (row % o.time + 1u < o.time) {   // then row + 1 is a row of the same sequence
-            const uint32_t label = o.labels[row + 1];
-            if (label != o.ignore_id) target = label < o.vocab ? (int32_t)label : -2;
+        const int32_t place = o.place[row], target = o.labels.target(row);
+        if (place < 0) {
+            if (lane == 0) o.row_loss[row] = target == -1 ? 0.0f : NAN;
+            uint8_t* g = static_cast<uint8_t*>(o.g_hidden) + (size_t)row * o.g_bytes;
+            if (o.g_bytes % 16 == 0 && reinterpret_cast<uintptr_t>(o.g_hidden) % 16 == 0) {
+                for (uint32_t i = lane * 16; i < o.g_bytes; i += 512) *reinterpret_cast<uint4*>(g + i) = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+                for (uint32_t i = lane * 2; i < o.g_bytes; i += 64) *reinterpret_cast<uint16_t*>(g + i) = 0;
+            }
+            const uint32_t counted = *o.counted, pad = counted + (uint32_t)(-1 - place);   // a row behind the last, for each such row
+            if (pad < (counted + pg::BM - 1) / pg::BM * pg::BM)
+                for (uint32_t chunk = lane; chunk < chunks; chunk += 32)
+                    *reinterpret_cast<uint4*>(o.h16 + (size_t)pad * o.Dp + chunk * 8) = make_uint4(0u, 0u, 0u, 0u);
+            return;
         }
         float dot = 0.0f;
-        const size_t first = (size_t)max(target, 0) * o.D;   // of the target's weights
+        const size_t first = (size_t)target * o.D;   // of the target's weights
         for (uint32_t chunk = lane; chunk < chunks; chunk += 32) {
             const uint32_t c = chunk * 8;
             uint32_t w[4] = {};
-            if (target >= 0) {
-                const T* from = static_cast<const T*>(o.hidden) + row * o.stride + c;
-                if (sizeof(T) == 2 && c + 8 <= o.D && reinterpret_cast<uintptr_t>(from) % 16 == 0) {
-                    const uint4 t = *reinterpret_cast<const uint4*>(from);
-                    w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
-                } else {
+            const T* from = static_cast<const T*>(o.hidden) + row * o.stride + c;
+            if (sizeof(T) == 2 && c + 8 <= o.D && reinterpret_cast<uintptr_t>(from) % 16 == 0) {
+                const uint4 t = *reinterpret_cast<const uint4*>(from);
+                w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c + e < o.D) {
-                            uint16_t h;
-                            if constexpr (sizeof(T) == 4) {
-                                const float v = from[e];
-                                if (fabsf(v) > 65504.0f && fabsf(v) <= 3.4028234e38f &&
-                                    atomicCAS(o.status, ULLIS_DEV_OK, ULLIS_DEV_FP16_RANGE) == ULLIS_DEV_OK) o.status[1] = row;
-                                h = __half_as_ushort(__float2half_rn(v));
-                            } else h = *reinterpret_cast<const uint16_t*>(from + e);
-                            w[e >> 1] |= (uint32_t)h << (16 * (e & 1));
-                        }
-                }
-                if (o.bits) {
-                    const uint32_t signs = signs8(o.bits, first + c, words);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)   // (0 past the row's end)
-                        dot += from16(((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu) ^ ((signs >> e) & 1u ? 0u : 0x8000u), o.bf16);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c + e < o.D) dot = fmaf(from16((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, o.bf16), from16(o.dense[first + c + e], o.bf16), dot);
-                }
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < o.D) {
+                        uint16_t h;
+                        if constexpr (sizeof(T) == 4) {
+                            const float v = from[e];
+                            if (fabsf(v) > 65504.0f && fabsf(v) <= 3.4028234e38f &&
+                                atomicCAS(o.status, ULLIS_DEV_OK, ULLIS_DEV_FP16_RANGE) == ULLIS_DEV_OK) o.status[1] = row;
+                            h = __half_as_ushort(__float2half_rn(v));
+                        } else h = *reinterpret_cast<const uint16_t*>(from + e);
+                        w[e >> 1] |= (uint32_t)h << (16 * (e & 1));
+                    }
             }
-            *reinterpret_cast<uint4*>(o.h16 + (size_t)row * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (o.bits) {
+                const uint32_t signs = signs8(o.bits, first + c, words);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)   // (0 past the row's end)
+                    dot += from16(((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu) ^ ((signs >> e) & 1u ? 0u : 0x8000u), o.bf16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < o.D) dot = fmaf(from16((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, o.bf16), from16(o.dense[first + c + e], o.bf16), dot);
+            }
+            *reinterpret_cast<uint4*>(o.h16 + (size_t)place * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
         if (lane == 0) {
-            o.target[row] = target;
-            if (o.fold && target >= 0) dot *= __half2float(__ushort_as_half(o.scale[target]));
-            o.target_acc[row] = dot;
-            if (target >= 0) {
-                if (o.scale && !o.fold) dot *= __half2float(__ushort_as_half(o.scale[target]));
-                if (o.bias) dot += __half2float(__ushort_as_half(o.bias[target]));
-            }
-            o.logit2[row] = dot * pg::LOG2E;
+            o.target[place] = target;
+            if (o.fold) dot *= __half2float(__ushort_as_half(o.scale[target]));
+            o.target_acc[place] = dot;
+            if (o.scale && !o.fold) dot *= __half2float(__ushort_as_half(o.scale[target]));
+            if (o.bias) dot += __half2float(__ushort_as_half(o.bias[target]));
+            o.logit2[place] = dot * pg::LOG2E;
         }
         return;
     }
@@ -333,8 +388,10 @@ head_operands_kernel(const HeadOperands o) {
 // log2 sum exp of every row out of its parts, the row's loss, and (first CTA) the powers of two of g * scale.
 struct HeadRows {
     const float2* part;
-    uint32_t rows, whole_rows, m_tiles, n_tiles, piece_tiles, slots, pairs;
-    const int32_t* target;
+    size_t part_piece;
+    const uint32_t* counted;
+    const int32_t* list;
+    uint32_t n_tiles, piece_tiles, pairs;
     const float* logit2;
     float *lse2, *row_loss;
     const float* scale_max;   // null: no row scales
@@ -364,7 +421,8 @@ head_rows_kernel(const HeadRows o) {
     }
     // eight rows to a warp where neighbours share sectors of the parts, with four lanes each
     const uint32_t row = blockIdx.x * 32 + (threadIdx.x >> 5) * 8 + (threadIdx.x & 7), lane = (threadIdx.x >> 3) & 3;
-    const uint32_t m = row / pg::BM;
+    const uint32_t rows = *o.counted, m = row / pg::BM, m_tiles = (rows + pg::BM - 1) / pg::BM, whole_rows = m_tiles * pg::BM;
+    if (m >= m_tiles) return;   // (a CTA's rows are all of one tile)
     float top = -INFINITY, sum = 0.0f;
     const auto add = [&](float t, float s) {
         if (t > top) {
@@ -376,13 +434,13 @@ head_rows_kernel(const HeadRows o) {
     };
     for (uint32_t first = 0, piece = 0; first < o.n_tiles; first += o.piece_tiles, ++piece) {
         const uint32_t width = min(o.piece_tiles, o.n_tiles - first);
-        const pg::Share share = pg::share_of(o.m_tiles * width, o.pairs);
+        const pg::Share share = pg::share_of(m_tiles * width, o.pairs);
         const uint32_t slots = share.owner(m * width + width - 1) - share.owner(m * width) + 1;
-        const float2* part = o.part + (size_t)piece * o.slots * 4 * o.whole_rows + row;
+        const float2* part = o.part + piece * o.part_piece + row;
         for (uint32_t i = 0; i < slots; i += 8) {   // (lane: quarter of the columns)
             float2 t[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) t[u] = i + u < slots ? part[(size_t)((i + u) * 4 + lane) * o.whole_rows] : make_float2(-INFINITY, 0.0f);
+            for (int u = 0; u < 8; ++u) t[u] = i + u < slots ? part[(size_t)((i + u) * 4 + lane) * whole_rows] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
             for (int u = 0; u < 8; ++u) add(t[u].x, t[u].y);
         }
@@ -396,24 +454,27 @@ head_rows_kernel(const HeadRows o) {
         sum = mine_first ? b : s;
         add(mine_first ? t : a, mine_first ? s : b);
     }
-    if (lane || row >= o.rows) return;
-    const int32_t target = o.target[row];
+    if (lane || row >= rows) return;
     const float logit2 = o.logit2[row];
     add(logit2, 1.0f);
     const float lse2 = top + log2f(sum);
-    o.lse2[row] = target >= 0 ? lse2 : INFINITY;
-    o.row_loss[row] = target >= 0 ? (lse2 - logit2) * LN2 : target == -1 ? 0.0f : NAN;
+    o.lse2[row] = lse2;
+    o.row_loss[o.list[row]] = (lse2 - logit2) * LN2;
 }
 
 // The columns' sums of a piece out of their parts, times loss_scale.  32 columns to a CTA, a warp to each of a slot's eight parts.
 __global__ void __launch_bounds__(256)
-head_columns_kernel(const float* __restrict__ part, uint32_t pitch, uint32_t m_tiles, uint32_t n_tiles, uint32_t pairs, uint32_t columns,
-                    float loss_scale, float* __restrict__ g_scale, float* __restrict__ g_bias) {
+head_columns_kernel(const float* __restrict__ part, uint32_t pitch, const uint32_t* __restrict__ counted, uint32_t n_tiles, uint32_t pairs,
+                    uint32_t columns, float loss_scale, float* __restrict__ g_scale, float* __restrict__ g_bias) {
     chain_entry();
     __shared__ float sums[2][8][32];
     const uint32_t lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;   // c < pitch, whole tiles
-    const pg::Share share = pg::share_of(m_tiles * n_tiles, pairs);
-    const uint32_t n = blockIdx.x * 32 / pg::BN, slots = share.owner(n * m_tiles + m_tiles - 1) - share.owner(n * m_tiles) + 1;
+    const uint32_t m_tiles = (*counted + pg::BM - 1) / pg::BM, n = blockIdx.x * 32 / pg::BN;
+    uint32_t slots = 0;
+    if (m_tiles) {
+        const pg::Share share = pg::share_of(m_tiles * n_tiles, pairs);
+        slots = share.owner(n * m_tiles + m_tiles - 1) - share.owner(n * m_tiles) + 1;
+    }
     float g = 0.0f, ga = 0.0f;
 #pragma unroll 4
     for (uint32_t i = 0; i < slots; ++i) {
@@ -436,20 +497,18 @@ head_columns_kernel(const float* __restrict__ part, uint32_t pitch, uint32_t m_t
 struct HeadPlan {
     size_t Dp, m_tiles, n_tiles;
     uint32_t pairs;
-    uint32_t lse_tiles, lse_pieces, lse_slots;   // column tiles of a piece, pieces, parts per row in one
+    uint32_t lse_tiles, lse_pieces;              // column tiles of a piece, pieces
+    size_t row_part_piece;                       // parts of the rows' sums in a piece
     size_t piece, pieces;                        // columns of a piece of g (a multiple of 256), pieces
     uint32_t col_slots;
     Cut hidden, weight;
-    size_t h16, w16, target, target_acc, target_cut, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, partial, bytes;
+    size_t h16, w16, counted, place, list, target, target_acc, target_cut, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, partial, bytes;
 };
 constexpr size_t GRAD_ELEMENTS = (size_t)1 << 27;   // of a piece of g: 256 MiB
 
-uint32_t most_slots(uint32_t outer, uint32_t inner, uint32_t pairs) {
-    const pg::Share s = pg::share_of(outer * inner, pairs);
-    uint32_t most = 1;
-    for (uint32_t o = 0; o < outer; ++o) most = std::max(most, s.owner(o * inner + inner - 1) - s.owner(o * inner) + 1);
-    return most;
-}
+// How many pairs at most have a part of `inner` tiles in a row, where outer * inner tiles are shared out (pg::Share): with x = tiles per
+// pair they begin at floor(c x), of which inner / x + 1 lie in a run of `inner`, and one begins before it.
+size_t most_slots(size_t outer, uint32_t pairs) { return pairs / outer + 2; }
 
 HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V) {
     HeadPlan p{};
@@ -460,22 +519,24 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
     // weights of a piece: up to 32 MiB, a quarter of L2
     p.lse_tiles = (uint32_t)std::min(p.n_tiles, std::max<size_t>(8, ((size_t)32 << 20) / (pg::BN * p.Dp * 2)));
     p.lse_pieces = (uint32_t)ceil_div(p.n_tiles, p.lse_tiles);
-    p.lse_slots = most_slots((uint32_t)p.m_tiles, p.lse_tiles, p.pairs);
-    const uint32_t rest = (uint32_t)(p.n_tiles - (p.lse_pieces - 1) * (size_t)p.lse_tiles);
-    p.lse_slots = std::max(p.lse_slots, most_slots((uint32_t)p.m_tiles, rest, p.pairs));
+    // [slot][4][rows] for any number of row tiles m that turns out to count: most_slots(m) * m <= pairs + 2 m
+    p.row_part_piece = (p.pairs + 2 * p.m_tiles) * 4 * pg::BM;
     const size_t most = std::max<size_t>(1, GRAD_ELEMENTS / (p.m_tiles * pg::BM) / pg::BN);   // column tiles of a piece
     p.pieces = ceil_div(p.n_tiles, most);
     const size_t tiles = ceil_div(p.n_tiles, p.pieces);
     p.pieces = ceil_div(p.n_tiles, tiles);
     p.piece = tiles * pg::BN;
     const size_t last = p.n_tiles - (p.pieces - 1) * tiles;
-    p.col_slots = std::max(most_slots((uint32_t)tiles, (uint32_t)p.m_tiles, p.pairs), most_slots((uint32_t)last, (uint32_t)p.m_tiles, p.pairs));
+    p.col_slots = (uint32_t)std::min(p.m_tiles, most_slots(last, p.pairs));   // (of one tile at least)
     const size_t width = std::min(p.piece, V);
     p.hidden = cut_of(rows, D, width, p.pairs, true);
     p.weight = cut_of(width, D, rows, p.pairs, true);
     Parts at;
     p.h16 = at.add(rows * p.Dp * 2);
     p.w16 = at.add(V * p.Dp * 2);
+    p.counted = at.add(4);
+    p.place = at.add(rows * 4);
+    p.list = at.add(rows * 4);
     p.target = at.add(rows * 4);
     p.target_acc = at.add(rows * 4);
     p.target_cut = at.add(rows * 4);
@@ -483,7 +544,7 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
     p.logit = at.add(rows * 4);
     p.factors = at.add(8);
     p.scale_max = at.add(WEIGHT_CTAS * 4);
-    p.row_part = at.add((size_t)p.lse_pieces * p.lse_slots * 4 * p.m_tiles * pg::BM * 8);
+    p.row_part = at.add(p.lse_pieces * p.row_part_piece * 8);
     p.grad = at.add(rows * p.piece * 2);
     p.col_part = at.add((size_t)p.col_slots * 16 * p.piece * 4);
     p.accum = at.add(p.pieces > 1 ? rows * D * 4 : 0);
@@ -507,18 +568,26 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     const bool as_is = !h.bits && D % 8 == 0 && aligned(h.weight, 16);
     const void* w16 = as_is ? h.weight : static_cast<const void*>(ws + p.w16);
 
+    const uint32_t* counted = reinterpret_cast<uint32_t*>(ws + p.counted);
+    const int32_t *place = reinterpret_cast<int32_t*>(ws + p.place), *list = reinterpret_cast<int32_t*>(ws + p.list);
+    const HeadLabels labels{h.labels, h.ignore_id, (uint32_t)rows, (uint32_t)h.time, (uint32_t)V};
+    s.chain("head_list", head_list_kernel, (unsigned)ceil_div(rows, 1024), 1024, 0, labels, const_cast<int32_t*>(place), const_cast<int32_t*>(list), const_cast<uint32_t*>(counted));
+
     HeadOperands o{};
     o.hidden = h.hidden.data;
     o.stride = h.hidden.stride;
     o.rows = (uint32_t)rows;
-    o.time = (uint32_t)h.time;
     o.D = (uint32_t)D;
     o.Dp = (uint32_t)p.Dp;
     o.vocab = (uint32_t)V;
     o.target_acc = reinterpret_cast<float*>(ws + p.target_acc);
     o.logit2 = reinterpret_cast<float*>(ws + p.logit);
-    o.labels = h.labels;
-    o.ignore_id = h.ignore_id;
+    o.labels = labels;
+    o.place = place;
+    o.counted = counted;
+    o.row_loss = h.row_loss;
+    o.g_hidden = h.g_hidden;
+    o.g_bytes = (uint32_t)(D * (h.out_f32 ? 4 : 2));
     o.h16 = reinterpret_cast<uint16_t*>(ws + p.h16);
     o.target = reinterpret_cast<int32_t*>(ws + p.target);
     o.bits = h.bits;
@@ -544,7 +613,8 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     q.bias = h.bias;
     q.target = o.target;
     q.piece_tiles = p.lse_tiles;
-    q.slots = p.lse_slots;
+    q.counted = counted;
+    q.row_part_piece = p.row_part_piece;
     q.row_part = reinterpret_cast<float2*>(ws + p.row_part);
     q.target_acc = o.target_acc;
     q.target_cut = reinterpret_cast<float*>(ws + p.target_cut);
@@ -554,14 +624,12 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
 
     HeadRows r{};
     r.part = q.row_part;
-    r.rows = (uint32_t)rows;
-    r.whole_rows = (uint32_t)(p.m_tiles * pg::BM);
-    r.m_tiles = (uint32_t)p.m_tiles;
+    r.part_piece = p.row_part_piece;
+    r.counted = counted;
+    r.list = list;
     r.n_tiles = (uint32_t)p.n_tiles;
     r.piece_tiles = p.lse_tiles;
-    r.slots = p.lse_slots;
     r.pairs = p.pairs;
-    r.target = o.target;
     r.logit2 = o.logit2;
     r.lse2 = reinterpret_cast<float*>(ws + p.lse2);
     r.row_loss = h.row_loss;
@@ -589,7 +657,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
         launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
         if (h.g_bias || h.g_scale)
             s.chain("head_columns", head_columns_kernel, (unsigned)ceil_div(width, 32), 256, 0, static_cast<const float*>(g.col_part), g.pitch,
-                    (uint32_t)p.m_tiles, n_tiles, p.pairs, (uint32_t)width, h.loss_scale, h.g_scale ? h.g_scale + v0 : nullptr,
+                    counted, n_tiles, p.pairs, (uint32_t)width, h.loss_scale, h.g_scale ? h.g_scale + v0 : nullptr,
                     h.g_bias ? h.g_bias + v0 : nullptr);
         // g_hidden: over the pieces in f32
         const Operand by_rows{grad, rows, width, p.piece, false};
@@ -597,12 +665,13 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
         const bool last = piece + 1 == p.pieces;
         product(s, "head_g_hidden", by_rows, wp, bf16, rows, D, width, p.hidden,
                 Output{last ? h.g_hidden : nullptr, h.out_f32, p.pieces > 1 ? reinterpret_cast<float*>(ws + p.accum) : nullptr, piece > 0, factors + 1,
-                       reinterpret_cast<float*>(ws + p.partial)});
+                       reinterpret_cast<float*>(ws + p.partial), counted, false, list});
         const Operand by_columns{grad, rows, width, p.piece, true};
         Operand hc = hidden;
         hc.mn = true;
         product(s, "head_g_weight", by_columns, hc, bf16, width, D, rows, p.weight,
-                Output{static_cast<uint8_t*>(h.g_weight) + v0 * D * (h.out_f32 ? 4 : 2), h.out_f32, nullptr, false, factors + 1, reinterpret_cast<float*>(ws + p.partial)});
+                Output{static_cast<uint8_t*>(h.g_weight) + v0 * D * (h.out_f32 ? 4 : 2), h.out_f32, nullptr, false, factors + 1, reinterpret_cast<float*>(ws + p.partial),
+                       counted, true, nullptr});
     }
 }
 
@@ -750,7 +819,7 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
     launch<pg::SUM, 1>(s, "tape_weight_grad", a, b, bf16, q, pairs);
     if (p.cut.splits > 1)
         s.chain("combine", combine_kernel<float>, (unsigned)ceil_div(out * in, 4 * THREADS), THREADS, 0, static_cast<const float*>(q.partial), p.cut.splits,
-                out * in, static_cast<const float*>(nullptr), static_cast<float*>(nullptr), 0u, g);
+                (uint32_t)out, (uint32_t)in, nullptr, nullptr, 0u, g, nullptr, nullptr);
 }
 
 }  // namespace dev

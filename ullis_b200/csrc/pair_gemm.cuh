@@ -56,13 +56,17 @@ struct Params {
     uint32_t a_mn, b_mn;       // operand with M (N) side by side
     uint32_t stages;
     uint32_t* status;
+    // How many of the rows of a batch count is known on the device only: M (count_k: K) is *counted and at most what it says above,
+    // which the arrays are laid out for.  null: it is what it says.
+    const uint32_t* counted;
+    uint32_t count_k;
     // LSE, GRAD: columns [n_first, n_first + N) of the vocabulary
     const uint16_t *scale, *bias;   // FP16 or null, of the first column
     const int32_t* target;          // [M] column of the vocabulary, or negative
     uint32_t n_first;
     uint32_t piece_tiles;      // LSE: column tiles that all pairs go through before the next ones
-    uint32_t slots;            // LSE: partial sums per piece and row
-    float2* row_part;          // LSE: [piece][slot][4][rows, whole tiles]
+    float2* row_part;          // LSE: [piece] of [slot][4][rows that count, whole tiles]
+    size_t row_part_piece;     // elements of a piece
     const float* lse2;         // GRAD: [M] log2 of the sum of exp, +inf for a row that does not count
     float* target_cut;         // [M] the target's product as the tensor cores have it (LSE leaves it, GRAD takes it out) ...
     const float* target_acc;   // GRAD: ... and with rounding
@@ -73,6 +77,7 @@ struct Params {
     uint32_t splits;           // of K
     void* out;                 // 16 bits [M][N] (STORE) or f32 [M][N] (SUM, STORE with out_f32), where nothing follows
     uint32_t out_f32;
+    const int32_t* out_rows;   // STORE: the row of `out` that row m goes to, or null
     float* accum;              // f32 [M][N]; STORE: read first if `accum_read`, written unless `out` is
     uint32_t accum_read;
     float* partial;            // splits > 1: [split][M][N]
@@ -106,16 +111,18 @@ __host__ __device__ inline Share share_of(uint32_t total, uint32_t pairs) { retu
 template <int EPI, int ACCS>
 struct Work {
     const Params& p;
-    uint32_t pair, pairs, m_tiles, n_tiles, blocks;
+    uint32_t pair, pairs, M, m_tiles, n_tiles, blocks;
     uint32_t piece = 0, left = 0, outer = 0, inner = 0, width = 0;   // LSE, GRAD: tiles left in the piece, (outer, inner < width) of the next
     uint32_t job = 0;                                                // STORE, SUM
-    // the tile
+    // the tile; of K the k-blocks [k0, k1), none where there are fewer than ranges (its sum is 0 and nobody waits for it)
     uint32_t m = 0, n = 0, k0 = 0, k1 = 0, split = 0, in_piece = 0;
 
     __device__ Work(const Params& p_, uint32_t pair_, uint32_t pairs_) : p(p_), pair(pair_), pairs(pairs_) {
-        m_tiles = (p.M + BM - 1) / BM;
+        const uint32_t counted = p.counted ? *p.counted : 0xFFFFFFFFu;
+        M = p.count_k ? p.M : min(p.M, counted);
+        m_tiles = (M + BM - 1) / BM;
         n_tiles = (p.N + BN * ACCS - 1) / (BN * ACCS);
-        blocks = (p.K + BK - 1) / BK;
+        blocks = ((p.count_k ? min(p.K, counted) : p.K) + BK - 1) / BK;
         k1 = blocks;
         job = pair;
         if (EPI == LSE) open(m_tiles, min(p.piece_tiles, n_tiles));
@@ -125,7 +132,7 @@ struct Work {
         const Share s = share_of(outers * inners, pairs);
         width = inners;
         left = 0;
-        if (pair < s.pairs) {
+        if (pair < s.pairs) {   // (no pair has a share of nothing)
             const uint32_t first = s.first(pair);
             left = s.first(pair + 1) - first;
             outer = first / inners;
@@ -454,6 +461,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             if (lane == 0) arrive_even(empty_even + 8 * (done % BUFFERS));
             ++done;
         };
+        const uint32_t M = work.M;
         const uint32_t q2 = (lane & 3) * 2, r0 = lane >> 2;   // of the 16 x 64 form: first column of a pair, first row
 
         if constexpr (EPI == LSE) {
@@ -466,7 +474,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 const uint32_t width = min(p.piece_tiles, work.n_tiles - piece_now * p.piece_tiles);
                 const uint32_t slot = pair - share_of(work.m_tiles * width, pairs).owner(m_now * width);
                 const size_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
-                p.row_part[(((size_t)piece_now * p.slots + slot) * 4 + group) * rows + row] = make_float2(top, sum);
+                p.row_part[piece_now * p.row_part_piece + (size_t)(slot * 4 + group) * rows + row] = make_float2(top, sum);
             };
             Columns ahead;
             bool more = work.next();
@@ -480,7 +488,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     top = -INFINITY;
                     sum = 0.0f;
                     const uint32_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
-                    target = row < p.M ? p.target[row] : -1;
+                    target = row < M ? p.target[row] : -1;
                 }
                 __syncwarp();
                 ahead.keep(columns, lane);
@@ -575,7 +583,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             float* row_smem = reinterpret_cast<float*>(epi_smem + EPI_WARPS * (2 * STAGING_BYTES + COLUMN_BYTES) + mine * ROW_BYTES);
             const auto fetch = [&](uint32_t turn) {
                 const uint32_t row = work.m * BM + rank * 128 + quarter * 32 + lane;
-                const bool in = row < p.M;
+                const bool in = row < M;
                 float* to = row_smem + turn * 128 + lane;
                 copy_word(to, p.lse2 + (in ? row : 0), in);
                 copy_word(to + 32, p.target_acc + (in ? row : 0), in);
@@ -605,7 +613,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 // in it and the -1 of the one-hot; the loop below knows nothing of that: g goes to its place in the 16-bit block behind
                 // the loop, and what it is more than the loop's exp to the column's sums by itself.  (As comparisons within the loop the
                 // targets took a fifth of this epilogue.)  A lane has columns lane and 32 + lane, in the order of the rows.
-                const uint32_t own = m0 + lane < p.M ? reinterpret_cast<const uint32_t*>(rows)[96 + lane] - (p.n_first + n0) : 64u;
+                const uint32_t own = m0 + lane < M ? reinterpret_cast<const uint32_t*>(rows)[96 + lane] - (p.n_first + n0) : 64u;
                 float own_g = 0.0f;
                 uint32_t left = __ballot_sync(0xffffffffu, own < 64u);
                 if (left) {
@@ -645,7 +653,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t row = h * 16 + i * 8 + r0;
-                        const float lse = m0 + row < p.M ? -rows[row] : -INFINITY;
+                        const float lse = m0 + row < M ? -rows[row] : -INFINITY;
                         l[i] = two(lse, lse);
                     }
                     const uint32_t to = blocks_at + h * STAGING_BYTES;
@@ -699,27 +707,30 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             const bool wide = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
             uint16_t* out = static_cast<uint16_t*>(p.out);
             while (work.next()) {
-                uint32_t taddr;
-                if (!filled(&taddr)) break;
+                uint32_t taddr = 0;
+                const bool none = work.k0 == work.k1;
+                if (!none && !filled(&taddr)) break;
                 const uint32_t m0 = work.m * BM + rank * 128 + quarter * 32;
                 float* partial = p.splits > 1 ? p.partial + (size_t)work.split * p.M * p.N : nullptr;
                 const bool to16 = !partial && p.out && !p.out_f32;
 #pragma unroll 1
                 for (uint32_t part = 0; part < 2 * ACCS; ++part) {
                     const uint32_t h = part & 1, c0 = (group * ACCS + (part >> 1)) * 64, n0 = work.n * BN * ACCS + c0;
-                    uint32_t r[32];
-                    tmem_ld_16x64(taddr + c0 + ((h * 16) << 16), r);
-                    ptx::tmem_ld_wait();
-                    if (part == 2 * ACCS - 1) drained();
+                    uint32_t r[32] = {};
+                    if (!none) {
+                        tmem_ld_16x64(taddr + c0 + ((h * 16) << 16), r);
+                        ptx::tmem_ld_wait();
+                        if (part == 2 * ACCS - 1) drained();
+                    }
                     float v[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                    const auto f32_rows = [&](float* at, bool read, bool write, float times) {
+                    const auto f32_rows = [&](float* at, const int32_t* rows, bool read, bool write, float times) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const uint32_t row = m0 + h * 16 + r0 + i * 8;
-                            if (row >= p.M) continue;
-                            float* line = at + (size_t)row * p.N;
+                            if (row >= M) continue;
+                            float* line = at + (size_t)(rows ? rows[row] : row) * p.N;
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
                                 const uint32_t c = n0 + j * 8 + q2;
@@ -737,9 +748,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             }
                         }
                     };
-                    if (partial) { f32_rows(partial, false, true, 1.0f); continue; }
-                    if (p.accum) f32_rows(p.accum, p.accum_read, !p.out, 1.0f);
-                    if (p.out && p.out_f32) f32_rows(static_cast<float*>(p.out), false, true, alpha);
+                    if (partial) { f32_rows(partial, nullptr, false, true, 1.0f); continue; }
+                    if (p.accum) f32_rows(p.accum, nullptr, p.accum_read, !p.out, 1.0f);
+                    if (p.out && p.out_f32) f32_rows(static_cast<float*>(p.out), p.out_rows, false, true, alpha);
                     if (!to16) continue;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
@@ -752,8 +763,8 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t row = i * 4 + (lane >> 3), piece = lane & 7, gm = m0 + h * 16 + row, c = n0 + piece * 8;
                         const uint4 w = *reinterpret_cast<const uint4*>(staging + row * 128 + ((piece ^ (row & 7)) << 4));
-                        if (gm >= p.M || c >= p.N) continue;
-                        uint16_t* to = out + (size_t)gm * p.N + c;
+                        if (gm >= M || c >= p.N) continue;
+                        uint16_t* to = out + (size_t)(p.out_rows ? p.out_rows[gm] : gm) * p.N + c;
                         if (wide) {
                             *reinterpret_cast<uint4*>(to) = w;
                         } else {
@@ -798,7 +809,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t row = m0 + r0 + i * 8;
-                    if (row >= p.M) continue;
+                    if (row >= M) continue;
                     float* line = out + (size_t)row * p.N;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
