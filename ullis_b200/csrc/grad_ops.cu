@@ -166,8 +166,9 @@ struct Output {
     const uint32_t* counted;   // pair_gemm.cuh: rows of the product, or (count_k) terms of its sums
     bool count_k;
     const int32_t* rows;       // where its rows go
+    bool beside;               // pair_gemm.cuh
 };
-// A product, alpha * (a . b + accum)
+// A product, alpha * (a . b + accum) ...
 void product(const Stream& s, const char* what, const Operand& a, const Operand& b, bool bf16, size_t M, size_t N, size_t K, const Cut& cut,
              const Output& o) {
     pg::Params p{};
@@ -184,18 +185,22 @@ void product(const Stream& s, const char* what, const Operand& a, const Operand&
     p.counted = o.counted;
     p.count_k = o.count_k;
     p.out_rows = o.rows;
+    p.beside = o.beside;
     const uint32_t pairs = (uint32_t)std::min<size_t>(pairs_of(s.rt), ceil_div(M, 256) * ceil_div(N, 256 * cut.accs) * cut.splits);
     if (cut.accs == 2) launch<pg::STORE, 2>(s, what, a, b, bf16, p, pairs);
     else launch<pg::STORE, 1>(s, what, a, b, bf16, p, pairs);
+}
+// ... and the sum of its ranges of K, if there are several
+void combine(const Stream& s, bool bf16, size_t M, size_t N, const Cut& cut, const Output& o) {
     if (cut.splits == 1) return;
     const unsigned grid = (unsigned)ceil_div(M * N, 4 * THREADS);
-    const auto combine = [&](auto kernel, auto* out) {
+    const auto launch = [&](auto kernel, auto* out) {
         s.chain("combine", kernel, grid, THREADS, 0, static_cast<const float*>(o.partial), cut.splits, (uint32_t)M, (uint32_t)N, o.factor, o.accum,
                 (uint32_t)o.accum_read, out, o.count_k ? nullptr : o.counted, o.rows);
     };
-    if (o.f32) combine(combine_kernel<float>, static_cast<float*>(o.out));
-    else if (bf16) combine(combine_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(o.out));
-    else combine(combine_kernel<__half>, static_cast<__half*>(o.out));
+    if (o.f32) launch(combine_kernel<float>, static_cast<float*>(o.out));
+    else if (bf16) launch(combine_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(o.out));
+    else launch(combine_kernel<__half>, static_cast<__half*>(o.out));
 }
 
 // ------------------------------------------------------------------------------------------------ operands of the head
@@ -251,8 +256,9 @@ struct HeadOperands {
     size_t stride;
     uint32_t rows, D, Dp, vocab;
     HeadLabels labels;
-    const int32_t* place;
-    const uint32_t* counted;
+    const int32_t* place;       // null: each CTA finds its rows' places itself (few rows), and leaves `list` and `counted`
+    int32_t* list;
+    uint32_t* counted;
     float* row_loss;
     void* g_hidden;             // [rows, D]
     uint32_t g_bytes;           // of a row of it
@@ -288,9 +294,46 @@ head_operands_kernel(const HeadOperands o) {
     const uint32_t chunks = o.Dp / 8;
     const size_t words = ((size_t)o.vocab * o.D + 31) / 32;
     if (blockIdx.x < o.hidden_ctas) {
-        const uint32_t row = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-        if (row >= o.rows) return;
-        const int32_t place = o.place[row], target = o.labels.target(row);
+        constexpr uint32_t ROWS = THREADS / 32;
+        const uint32_t first_row = blockIdx.x * ROWS, warp = threadIdx.x >> 5, row = first_row + warp, lane = threadIdx.x & 31;
+        const int32_t target = row < o.rows ? o.labels.target(row) : -1;
+        int32_t place = 0;
+        uint32_t counted = 0;
+        if (o.place) {
+            if (row >= o.rows) return;
+            place = o.place[row];
+            counted = *o.counted;
+        } else {
+            __shared__ uint32_t before[ROWS], all[ROWS], own[ROWS];
+            uint32_t n = 0, total = 0;
+#pragma unroll 4
+            for (uint32_t r = threadIdx.x; r < o.rows; r += THREADS) {
+                const uint32_t counts = o.labels.target(r) >= 0;
+                total += counts;
+                n += r < first_row ? counts : 0u;
+            }
+#pragma unroll
+            for (int k = 16; k > 0; k >>= 1) {
+                n += __shfl_xor_sync(0xffffffffu, n, k);
+                total += __shfl_xor_sync(0xffffffffu, total, k);
+            }
+            if (lane == 0) {
+                before[warp] = n;
+                all[warp] = total;
+                own[warp] = target >= 0;
+            }
+            __syncthreads();
+            uint32_t at = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < ROWS; ++w) {
+                at += before[w] + (w < warp ? own[w] : 0u);
+                counted += all[w];
+            }
+            if (blockIdx.x == 0 && threadIdx.x == 0) *o.counted = counted;
+            if (row >= o.rows) return;
+            place = target >= 0 ? (int32_t)at : -1 - (int32_t)(row - at);
+            if (target >= 0 && lane == 0) o.list[at] = (int32_t)row;
+        }
         if (place < 0) {
             if (lane == 0) o.row_loss[row] = target == -1 ? 0.0f : NAN;
             uint8_t* g = static_cast<uint8_t*>(o.g_hidden) + (size_t)row * o.g_bytes;
@@ -299,7 +342,7 @@ head_operands_kernel(const HeadOperands o) {
             } else {
                 for (uint32_t i = lane * 2; i < o.g_bytes; i += 64) *reinterpret_cast<uint16_t*>(g + i) = 0;
             }
-            const uint32_t counted = *o.counted, pad = counted + (uint32_t)(-1 - place);   // a row behind the last, for each such row
+            const uint32_t pad = counted + (uint32_t)(-1 - place);   // a row behind the last, for each such row
             if (pad < (counted + pg::BM - 1) / pg::BM * pg::BM)
                 for (uint32_t chunk = lane; chunk < chunks; chunk += 32)
                     *reinterpret_cast<uint4*>(o.h16 + (size_t)pad * o.Dp + chunk * 8) = make_uint4(0u, 0u, 0u, 0u);
@@ -419,8 +462,8 @@ head_rows_kernel(const HeadRows o) {
             o.factors[1] = exp2f((float)-k) * o.loss_scale;
         }
     }
-    // eight rows to a warp where neighbours share sectors of the parts, with four lanes each
-    const uint32_t row = blockIdx.x * 32 + (threadIdx.x >> 5) * 8 + (threadIdx.x & 7), lane = (threadIdx.x >> 3) & 3;
+    // two rows to a warp; a row's sixteen lanes: a quarter of the columns, every fourth slot
+    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5) * 2 + (threadIdx.x & 1), lane = (threadIdx.x >> 1) & 15, quarter = lane & 3;
     const uint32_t rows = *o.counted, m = row / pg::BM, m_tiles = (rows + pg::BM - 1) / pg::BM, whole_rows = m_tiles * pg::BM;
     if (m >= m_tiles) return;   // (a CTA's rows are all of one tile)
     float top = -INFINITY, sum = 0.0f;
@@ -437,17 +480,17 @@ head_rows_kernel(const HeadRows o) {
         const pg::Share share = pg::share_of(m_tiles * width, o.pairs);
         const uint32_t slots = share.owner(m * width + width - 1) - share.owner(m * width) + 1;
         const float2* part = o.part + piece * o.part_piece + row;
-        for (uint32_t i = 0; i < slots; i += 8) {   // (lane: quarter of the columns)
-            float2 t[8];
+        for (uint32_t i = lane >> 2; i < slots; i += 16) {
+            float2 t[4];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) t[u] = i + u < slots ? part[(size_t)((i + u) * 4 + lane) * whole_rows] : make_float2(-INFINITY, 0.0f);
+            for (int u = 0; u < 4; ++u) t[u] = i + 4 * u < slots ? part[(size_t)((i + 4 * u) * 4 + quarter) * whole_rows] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) add(t[u].x, t[u].y);
+            for (int u = 0; u < 4; ++u) add(t[u].x, t[u].y);
         }
     }
 #pragma unroll
-    for (int k = 2; k > 0; k >>= 1) {   // (within a row's lanes, in a fixed order)
-        const float t = __shfl_xor_sync(0xffffffffu, top, 8 * k), s = __shfl_xor_sync(0xffffffffu, sum, 8 * k);
+    for (int k = 8; k > 0; k >>= 1) {   // (within a row's lanes, in a fixed order)
+        const float t = __shfl_xor_sync(0xffffffffu, top, 2 * k), s = __shfl_xor_sync(0xffffffffu, sum, 2 * k);
         const float a = top, b = sum;
         const bool mine_first = !(lane & k);
         top = mine_first ? a : t;
@@ -502,9 +545,9 @@ struct HeadPlan {
     size_t piece, pieces;                        // columns of a piece of g (a multiple of 256), pieces
     uint32_t col_slots;
     Cut hidden, weight;
-    size_t h16, w16, counted, place, list, target, target_acc, target_cut, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, partial, bytes;
+    size_t h16, w16, counted, place, list, target, target_acc, target_cut, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, hidden_partial, weight_partial, bytes;
 };
-constexpr size_t GRAD_ELEMENTS = (size_t)1 << 27;   // of a piece of g: 256 MiB
+constexpr size_t GRAD_ELEMENTS = (size_t)1 << 28;   // of a piece of g: 512 MiB
 
 // How many pairs at most have a part of `inner` tiles in a row, where outer * inner tiles are shared out (pg::Share): with x = tiles per
 // pair they begin at floor(c x), of which inner / x + 1 lie in a run of `inner`, and one begins before it.
@@ -548,7 +591,8 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
     p.grad = at.add(rows * p.piece * 2);
     p.col_part = at.add((size_t)p.col_slots * 16 * p.piece * 4);
     p.accum = at.add(p.pieces > 1 ? rows * D * 4 : 0);
-    p.partial = at.add(std::max(partial_bytes(rows, D, p.hidden), partial_bytes(width, D, p.weight)));
+    p.hidden_partial = at.add(partial_bytes(rows, D, p.hidden));
+    p.weight_partial = at.add(partial_bytes(width, D, p.weight));
     p.bytes = at.bytes;
     return p;
 }
@@ -568,10 +612,14 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     const bool as_is = !h.bits && D % 8 == 0 && aligned(h.weight, 16);
     const void* w16 = as_is ? h.weight : static_cast<const void*>(ws + p.w16);
 
-    const uint32_t* counted = reinterpret_cast<uint32_t*>(ws + p.counted);
-    const int32_t *place = reinterpret_cast<int32_t*>(ws + p.place), *list = reinterpret_cast<int32_t*>(ws + p.list);
+    uint32_t* counted = reinterpret_cast<uint32_t*>(ws + p.counted);
+    int32_t *place = reinterpret_cast<int32_t*>(ws + p.place), *list = reinterpret_cast<int32_t*>(ws + p.list);
     const HeadLabels labels{h.labels, h.ignore_id, (uint32_t)rows, (uint32_t)h.time, (uint32_t)V};
-    s.chain("head_list", head_list_kernel, (unsigned)ceil_div(rows, 1024), 1024, 0, labels, const_cast<int32_t*>(place), const_cast<int32_t*>(list), const_cast<uint32_t*>(counted));
+    // Few rows find their places where they are gathered, each CTA of eight from all labels.  us of a call in a graph, 256 channels
+    // and a vocabulary of 1024, so / with the list by a launch of its own: 32 rows 31.6 / 32.4, 512 35.3 / 36.0, 2048 42.4 / 42.0,
+    // 8192 62.0 / 55.0, 16 384 115 / 86.
+    const bool listed = rows > 1024;
+    if (listed) s.chain("head_list", head_list_kernel, (unsigned)ceil_div(rows, 1024), 1024, 0, labels, place, list, counted);
 
     HeadOperands o{};
     o.hidden = h.hidden.data;
@@ -583,7 +631,8 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     o.target_acc = reinterpret_cast<float*>(ws + p.target_acc);
     o.logit2 = reinterpret_cast<float*>(ws + p.logit);
     o.labels = labels;
-    o.place = place;
+    o.place = listed ? place : nullptr;
+    o.list = list;
     o.counted = counted;
     o.row_loss = h.row_loss;
     o.g_hidden = h.g_hidden;
@@ -636,7 +685,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     r.scale_max = q.scale ? o.scale_max : nullptr;
     r.factors = factors;
     r.loss_scale = h.loss_scale;
-    s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 32), 128, 0, r);
+    s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 8), 128, 0, r);
 
     uint16_t* grad = reinterpret_cast<uint16_t*>(ws + p.grad);
     for (size_t piece = 0; piece < p.pieces; ++piece) {
@@ -655,23 +704,40 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
         wp.rows = width;
         const CUtensorMap grad_map = map_of(grad, rows, p.piece, p.piece, 16, bf16);
         launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
-        if (h.g_bias || h.g_scale)
+        // What follows reads g and nothing of one another: few rows leave room for all three at once.
+        const bool columns = h.g_bias || h.g_scale;
+        if (columns)
             s.chain("head_columns", head_columns_kernel, (unsigned)ceil_div(width, 32), 256, 0, static_cast<const float*>(g.col_part), g.pitch,
                     counted, n_tiles, p.pairs, (uint32_t)width, h.loss_scale, h.g_scale ? h.g_scale + v0 : nullptr,
                     h.g_bias ? h.g_bias + v0 : nullptr);
-        // g_hidden: over the pieces in f32
-        const Operand by_rows{grad, rows, width, p.piece, false};
-        wp.mn = true;
-        const bool last = piece + 1 == p.pieces;
-        product(s, "head_g_hidden", by_rows, wp, bf16, rows, D, width, p.hidden,
-                Output{last ? h.g_hidden : nullptr, h.out_f32, p.pieces > 1 ? reinterpret_cast<float*>(ws + p.accum) : nullptr, piece > 0, factors + 1,
-                       reinterpret_cast<float*>(ws + p.partial), counted, false, list});
         const Operand by_columns{grad, rows, width, p.piece, true};
         Operand hc = hidden;
         hc.mn = true;
-        product(s, "head_g_weight", by_columns, hc, bf16, width, D, rows, p.weight,
-                Output{static_cast<uint8_t*>(h.g_weight) + v0 * D * (h.out_f32 ? 4 : 2), h.out_f32, nullptr, false, factors + 1, reinterpret_cast<float*>(ws + p.partial),
-                       counted, true, nullptr});
+        Output w{};
+        w.out = static_cast<uint8_t*>(h.g_weight) + v0 * D * (h.out_f32 ? 4 : 2);
+        w.f32 = h.out_f32;
+        w.factor = factors + 1;
+        w.partial = reinterpret_cast<float*>(ws + p.weight_partial);
+        w.counted = counted;
+        w.count_k = true;
+        w.beside = columns;
+        product(s, "head_g_weight", by_columns, hc, bf16, width, D, rows, p.weight, w);
+        // g_hidden: over the pieces in f32
+        const Operand by_rows{grad, rows, width, p.piece, false};
+        wp.mn = true;
+        Output d{};
+        d.out = piece + 1 == p.pieces ? h.g_hidden : nullptr;
+        d.f32 = h.out_f32;
+        d.accum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.accum) : nullptr;
+        d.accum_read = piece > 0;
+        d.factor = factors + 1;
+        d.partial = reinterpret_cast<float*>(ws + p.hidden_partial);
+        d.counted = counted;
+        d.rows = list;
+        d.beside = true;
+        product(s, "head_g_hidden", by_rows, wp, bf16, rows, D, width, p.hidden, d);
+        combine(s, bf16, width, D, p.weight, w);
+        combine(s, bf16, rows, D, p.hidden, d);
     }
 }
 

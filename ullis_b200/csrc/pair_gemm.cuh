@@ -75,6 +75,7 @@ struct Params {
     float* col_part;           // GRAD: [slot][8][2][pitch]
     // STORE, SUM
     uint32_t splits;           // of K
+    uint32_t beside;           // STORE: nothing of the kernel before this one is read or written, only of those before that
     void* out;                 // 16 bits [M][N] (STORE) or f32 [M][N] (SUM, STORE with out_f32), where nothing follows
     uint32_t out_f32;
     const int32_t* out_rows;   // STORE: the row of `out` that row m goes to, or null
@@ -177,14 +178,34 @@ __device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32])
         : "r"(taddr));
 }
 
-// the same, 32 columns
-__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+// the same, 16 columns
+__device__ __forceinline__ void tmem_ld_16x16(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+// 32 lanes x 16 columns, a row per thread
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
+}
+// All loads so far have landed; the registers that the last one wrote are named, so that nothing is read from them before.
+__device__ __forceinline__ void tmem_landed(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_landed(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
 }
 
 // Four 8 x 8 blocks of 16-bit pairs as the loads above leave them (a register each) to rows of 16 bytes; lane 8 b + i gives the
@@ -333,7 +354,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         ptx::tmem_alloc_pair(tmem_slot, 512);
         ptx::tmem_relinquish_pair();
     }
-    chain_entry();
+    // A kernel with `beside` runs beside the one before: that one has waited for those before it, or this one would not have been
+    // launched, and it is waited for at the end, so that whoever waits for this kernel has waited for both.
+    if (EPI == STORE && p.beside) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    else chain_entry();
     ptx::tc_fence_before_sync();
     __syncthreads();
     ptx::cluster_sync_all();
@@ -497,36 +521,40 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 if (more) ahead.fetch(p, work.n * BN + group * 64, lane);
                 uint32_t taddr;
                 if (!filled(&taddr)) break;
+                // 16 columns are on their way while 16 are worked on
+                taddr += group * 64;
+                uint32_t r[2][16];
+                tmem_ld_32x16(taddr, r[0]);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t r[32];
-                    ptx::tmem_ld_32x32(taddr + group * 64 + c * 32, r);
-                    ptx::tmem_ld_wait();
-                    if (c == 1) drained();
-                    const int32_t hit = target - (int32_t)(n0 + c * 32);
-                    const bool hits = __any_sync(0xffffffffu, hit >= 0 && hit < 32);   // of the warp's rows
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t(&now)[16] = r[c & 1];
+                    tmem_landed(now);
+                    if (c < 3) tmem_ld_32x16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
+                    else drained();
+                    const int32_t hit = target - (int32_t)(n0 + c * 16);
+                    const bool hits = __any_sync(0xffffffffu, hit >= 0 && hit < 16);   // of the warp's rows
                     if (hits) {   // (by bits: chosen by an index, the accumulators went to local memory)
                         uint32_t cut = 0;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) cut |= hit == i ? r[i] : 0u;
-                        if (hit >= 0 && hit < 32) p.target_cut[m_now * BM + rank * 128 + quarter * 32 + lane] = __uint_as_float(cut);
+                        for (int i = 0; i < 16; ++i) cut |= hit == i ? now[i] : 0u;
+                        if (hit >= 0 && hit < 16) p.target_cut[m_now * BM + rank * 128 + quarter * 32 + lane] = __uint_as_float(cut);
                     }
-                    uint64_t z[16];
+                    uint64_t z[8];
                     float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(columns + c * 32 + i * 2);
-                        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(columns + 64 + c * 32 + i * 2);
-                        z[i] = fma2((uint64_t)r[i * 2 + 1] << 32 | r[i * 2], s.x, b.x);
-                        z[i + 1] = fma2((uint64_t)r[i * 2 + 3] << 32 | r[i * 2 + 2], s.y, b.y);
+                    for (int i = 0; i < 8; i += 2) {
+                        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(columns + c * 16 + i * 2);
+                        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(columns + 64 + c * 16 + i * 2);
+                        z[i] = fma2((uint64_t)now[i * 2 + 1] << 32 | now[i * 2], s.x, b.x);
+                        z[i + 1] = fma2((uint64_t)now[i * 2 + 3] << 32 | now[i * 2 + 2], s.y, b.y);
                     }
                     if (hits) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
+                        for (int i = 0; i < 8; ++i)
                             z[i] = add2(z[i], two(hit == i * 2 ? -INFINITY : 0.0f, hit == i * 2 + 1 ? -INFINITY : 0.0f));
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
+                    for (int i = 0; i < 8; ++i) {
                         const float2 v = of_two(z[i]);
                         best[i & 1] = fmaxf(best[i & 1], fmaxf(v.x, v.y));
                     }
@@ -539,7 +567,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     const uint64_t base2 = two(base, base);
                     uint64_t here[2] = {0, 0};
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
+                    for (int i = 0; i < 8; ++i) {
                         const float2 v = of_two(add2(z[i], base2));
                         here[i & 1] = add2(here[i & 1], two(exp2_fast(v.x), exp2_fast(v.y)));
                     }
@@ -647,8 +675,8 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 // 16 rows at a time, one copy of the code for both: with two the registers ran out
 #pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t r[16];
-                    tmem_ld_16x32(taddr + ((h * 16) << 16), r);
+                    uint32_t r[2][8];   // 16 columns are on their way while 16 are worked on
+                    tmem_ld_16x16(taddr + ((h * 16) << 16), r[0]);
                     uint64_t l[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -661,9 +689,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
-                        if (j == 4) tmem_ld_16x32(taddr + 32 + ((h * 16) << 16), r);
-                        if (j == 0 || j == 4) ptx::tmem_ld_wait();
-                        if (j == 4 && h == 1) drained();
+                        uint32_t(&now)[8] = r[j / 2 & 1];
+                        tmem_landed(now);
+                        if (j < 6) tmem_ld_16x16(taddr + (j + 2) * 8 + ((h * 16) << 16), r[(j / 2 + 1) & 1]);
+                        else if (h == 1) drained();
                         uint32_t w[4];
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
@@ -672,8 +701,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             const uint64_t k = mul2(s, two(from_log2, from_log2));
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
-                                const int at = (j + u) % 4 * 4 + i * 2;
-                                const uint64_t a = (uint64_t)r[at + 1] << 32 | r[at];
+                                const uint64_t a = (uint64_t)now[u * 4 + i * 2 + 1] << 32 | now[u * 4 + i * 2];
                                 const float2 e = of_two(add2(fma2(a, s, b), l[i]));
                                 const uint64_t g = two(exp2_fast(e.x), exp2_fast(e.y));
                                 g_sum[j + u] = add2(g_sum[j + u], g);
@@ -834,6 +862,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc_pair(tmem_base, 512);
     }
+    if (EPI == STORE && p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (threadIdx.x == 0 && *s_error) {
         volatile uint32_t* status = p.status;   // a caller's stream: pinned host memory
         status[1] = 64u + *s_error;

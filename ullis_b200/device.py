@@ -74,8 +74,8 @@ def _p(t):
 
 
 def _like(t, dtype):
-    """An output of t's shape, without gaps."""
-    return _TORCH.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+    """An output of t's shape, without gaps.  (Sizes as single numbers: torch takes a tuple of them twice as long.)"""
+    return _TORCH.empty_like(t, dtype=dtype) if t.is_contiguous() else _TORCH.empty(*t.shape, dtype=dtype, device=t.device)
 
 
 def _shape_error(name, got, expected):
@@ -162,7 +162,7 @@ class DeviceOps:
             if len(known) >= 4096:
                 known.clear()
             known[name, sizes] = need
-        return like.new_empty((need,), dtype=_TORCH.uint8), need
+        return _TORCH.empty(need, dtype=_TORCH.uint8, device=like.device), need
 
     # ------------------------------------------------------------------------------------------ the 8-bit tape
     def tape_pack(self, x) -> Tape:
@@ -170,7 +170,7 @@ class DeviceOps:
         torch = _torch()
         rows, channels, stride = self._matrix(x, "x", _DTYPES)
         codes = _like(x, torch.int8)
-        exponents = x.new_empty((rows, -(-channels // 32)), dtype=torch.uint8)
+        exponents = torch.empty(rows, -(-channels // 32), dtype=torch.uint8, device=x.device)
         self._check(self._lib.ullis_cuda_tape_pack(self._h, _RAW_STREAM(self.device), _DTYPES[x.dtype], x.data_ptr(), stride, rows,
                                                    channels, codes.data_ptr(), exponents.data_ptr()))
         return Tape(codes, exponents)
@@ -193,7 +193,7 @@ class DeviceOps:
         self._vector(bias, "bias", _F16, channels)
         y = _like(x, x.dtype)
         codes = _like(x, torch.int8)
-        exponents = x.new_empty((rows, -(-channels // 32)), dtype=torch.uint8)
+        exponents = torch.empty(rows, -(-channels // 32), dtype=torch.uint8, device=x.device)
         self._check(self._lib.ullis_cuda_tape_layer_norm(
             self._h, _RAW_STREAM(self.device), _DTYPES[x.dtype], x.data_ptr(), stride, weight.data_ptr(), bias.data_ptr(), rows,
             channels, y.data_ptr(), codes.data_ptr(), exponents.data_ptr()))
@@ -214,13 +214,12 @@ class DeviceOps:
                 _shape_error("residual", residual.shape, gy.shape)
             past = residual.data_ptr()
         gx = _like(gy, gy.dtype)
-        g = gy.new_empty((2, channels), dtype=_TORCH.float32)
-        at = g.data_ptr()
+        g_weight, g_bias = _like(weight, _TORCH.float32), _like(weight, _TORCH.float32)
         work, size = self._workspace(gy, "tape_layer_norm_backward", rows, channels)
         self._check(self._lib.ullis_cuda_tape_layer_norm_backward(
             self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], codes.data_ptr(), exponents.data_ptr(), gy.data_ptr(), stride,
-            weight.data_ptr(), past, past_stride, rows, channels, gx.data_ptr(), at, at + 4 * channels, work.data_ptr(), size))
-        g_weight, g_bias = g.unbind(0)
+            weight.data_ptr(), past, past_stride, rows, channels, gx.data_ptr(), g_weight.data_ptr(),
+            g_bias.data_ptr(), work.data_ptr(), size))
         return gx, g_weight, g_bias
 
     def tape_weight_grad(self, tape, gy):
@@ -230,7 +229,7 @@ class DeviceOps:
         g_rows, out, stride = self._matrix(gy, "gy", _16)
         if g_rows != rows:
             _shape_error("gy", gy.shape, (rows, out))
-        g = gy.new_empty((out, channels), dtype=_TORCH.float32)
+        g = _TORCH.empty(out, channels, dtype=_TORCH.float32, device=gy.device)
         work, size = self._workspace(gy, "tape_weight_grad", rows, channels, out)
         self._check(self._lib.ullis_cuda_tape_weight_grad(
             self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], codes.data_ptr(), exponents.data_ptr(), gy.data_ptr(), stride, rows,
@@ -269,9 +268,9 @@ class DeviceOps:
             raise UllisCudaError(ERR_ARG, "ignore_id is not a 32-bit number")
         if not 0 < time < 1 << 31 or rows % time:
             raise UllisCudaError(ERR_SHAPE, "rows must be a multiple of time")
-        row_loss = hidden.new_empty((rows,), dtype=torch.float32)
+        row_loss = torch.empty(rows, dtype=torch.float32, device=hidden.device)
         g_hidden = _like(hidden, hidden.dtype)
-        g_weight = hidden.new_empty((vocab, channels))
+        g_weight = torch.empty(vocab, channels, dtype=hidden.dtype, device=hidden.device)
         g_scale = None if scale is None else _like(scale, torch.float32)
         g_bias = None if bias is None else _like(bias, torch.float32)
         work, size = self._workspace(hidden, "head_ce_grad", rows, channels, vocab)
