@@ -503,9 +503,12 @@ ULLIS_CUDA_API int32_t ullis_cuda_tape_weight_grad(ullis_cuda_runtime* rt, void*
  * behind g_scale and g_bias are f32; g * scale is rounded to hidden's type for the
  * two gradient products, which accumulate in f32.  What rows hold that do not count
  * (infinities, NaN) has no effect.  A label outside the vocabulary makes its row's
- * loss NaN and gives no gradient.  Rows must be a multiple of `time`. */
+ * loss NaN and gives no gradient.  Rows must be a multiple of `time`.
+ * copies_weight: 1 for a packed head, and for a dense one whose rows do not all start
+ * on 16 bytes (channels no multiple of 8, or weight unaligned): the workspace then
+ * holds the weights as an operand of the products. */
 ULLIS_CUDA_API int32_t ullis_cuda_head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels,
-                                                         size_t vocab, size_t* bytes);
+                                                         size_t vocab, int32_t copies_weight, size_t* bytes);
 ULLIS_CUDA_API int32_t ullis_cuda_head_ce_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype,
                                                const void* hidden, size_t hidden_stride, const uint32_t* bits,
                                                const void* weight, const uint16_t* scale, const uint16_t* bias,

@@ -524,6 +524,7 @@ unsafe extern "C" {
         rows: usize,
         channels: usize,
         vocab: usize,
+        copies_weight: i32,
         bytes: *mut usize,
     ) -> i32;
     pub fn ullis_cuda_head_ce_grad(

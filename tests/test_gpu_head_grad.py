@@ -150,6 +150,26 @@ def test_a_vocabulary_in_several_pieces(cuda_rt, packed, dtype):
     check(call(cuda_rt, s), formulas(s))
 
 
+@pytest.mark.parametrize("packed,dtype", [(True, "bf16"), (False, "f16")])
+def test_a_vocabulary_in_several_pieces_of_the_largest_size(cuda_rt, packed, dtype):
+    """More than 2^28 logits, which the workspace holds of one piece."""
+    s = inputs(16384 + 40, 16384 + 40, 64, 16500, dtype, packed, 0.02)
+    check(call(cuda_rt, s), formulas(s))
+
+
+def test_drawn_sizes(cuda_rt):
+    import random
+    rng = random.Random(7)
+    for seed in range(40):
+        time = rng.choice([1, 2, 3, 31, 64, 65, 127, 200, 333])
+        rows = time * rng.randint(1, max(1, 900 // time))
+        d = rng.choice([1, 3, 8, 15, 16, 40, 64, 65, 96, 128, 250, 264])
+        vocab = rng.choice([1, 2, 5, 63, 64, 65, 255, 256, 257, 500, 777, 1024, 1500])
+        s = inputs(rows, time, d, vocab, rng.choice(["f16", "bf16"]), rng.random() < 0.5, rng.choice([0.0, 0.1, 0.5, 0.9]), seed=seed,
+                   bias=rng.random() < 0.7)
+        check(call(cuda_rt, s), formulas(s))
+
+
 def test_scales_of_every_size(cuda_rt):
     s = inputs(200, 200, 64, 600, "f16", True)
     s["scale"][::7] = 0.0

@@ -203,6 +203,29 @@ def test_two_graphs_replayed_at_once(cuda_rt):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+def test_gx_in_the_place_of_the_other_gradient(cuda_rt):
+    """The C entry point takes residual for gx."""
+    import ctypes as C
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 2)):
+        for rows, c in ((3000, 512), (37, 100), (9, 2048)):
+            x, gy = activations(rows, c, dtype, 1), activations(rows, c, dtype, 2)
+            res, w = activations(rows, c, dtype, 3), torch.ones(c, device="cuda").half()
+            tape = cuda_rt.tape_pack(x)
+            want = cuda_rt.tape_layer_norm_backward(tape, gy, w, residual=res)
+            g = torch.empty(2, c, device="cuda")
+            need = C.c_size_t(0)
+            assert cuda_rt._lib.ullis_cuda_tape_layer_norm_backward_workspace(cuda_rt._h, rows, c, C.byref(need)) == cuda.OK
+            work = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+            fn = cuda_rt._lib.ullis_cuda_tape_layer_norm_backward
+            stream = torch.cuda.current_stream().cuda_stream
+            args = (tape.codes.data_ptr(), tape.exponents.data_ptr(), gy.data_ptr(), c, w.data_ptr(), res.data_ptr())
+            end = (rows, c, res.data_ptr(), g[0].data_ptr(), g[1].data_ptr(), work.data_ptr())
+            assert fn(cuda_rt._h, stream, code, *args, c + 8, *end, need) == cuda.ERR_ARG      # rows that do not lie on one another
+            assert fn(cuda_rt._h, stream, code, *args, c, *end, C.c_size_t(need.value - 1)) == cuda.ERR_SHAPE
+            assert fn(cuda_rt._h, stream, code, *args, c, *end, need) == cuda.OK
+            assert torch.equal(res, want[0]) and torch.equal(g[0], want[1]) and torch.equal(g[1], want[2])
+
+
 def test_offsets_past_32_bits(cuda_rt):
     c, stride = 96, 2 ** 32 + 16
     base = torch.empty(stride + c, dtype=torch.bfloat16, device="cuda")

@@ -228,10 +228,11 @@ int32_t ullis_cuda_tape_weight_grad(ullis_cuda_runtime* rt, void* cuda_stream, i
     });
 }
 
-int32_t ullis_cuda_head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, size_t* bytes) {
+int32_t ullis_cuda_head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab,
+                                          int32_t copies_weight, size_t* bytes) {
     return workspace_of(rt, bytes, [&] {
         need_head(rows, channels, vocab);
-        return dev::head_ce_grad_workspace(rt, rows, channels, vocab);
+        return dev::head_ce_grad_workspace(rt, rows, channels, vocab, copies_weight != 0);
     });
 }
 
@@ -269,7 +270,7 @@ int32_t ullis_cuda_head_ce_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32
         need_array(labels, "labels", 4);
         need_array(row_loss, "row_loss", 4);
         need_array(g_hidden, "g_hidden", 2);
-        need_workspace(workspace, workspace_bytes, dev::head_ce_grad_workspace(rt, rows, channels, vocab));
+        need_workspace(workspace, workspace_bytes, dev::head_ce_grad_workspace(rt, rows, channels, vocab, dev::head_copies_weight(weight, channels)));
         need_sm100(rt);
         dev::HeadGrad h{};
         h.dtype = dtype;

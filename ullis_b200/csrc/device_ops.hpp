@@ -78,7 +78,8 @@ struct HeadGrad {
     void* g_weight;            // [vocab, channels]
     float *g_scale, *g_bias;   // [vocab], nullable
 };
-size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab);
+bool head_copies_weight(const void* dense, size_t channels);   // whether the workspace holds the weights as an operand (null: packed)
+size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, bool copies_weight);
 void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace);
 
 }  // namespace dev

@@ -553,7 +553,7 @@ constexpr size_t GRAD_ELEMENTS = (size_t)1 << 28;   // of a piece of g: 512 MiB
 // pair they begin at floor(c x), of which inner / x + 1 lie in a run of `inner`, and one begins before it.
 size_t most_slots(size_t outer, uint32_t pairs) { return pairs / outer + 2; }
 
-HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V) {
+HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V, bool copies_weight) {
     HeadPlan p{};
     p.pairs = pairs_of(rt);
     p.Dp = up(D, 8);
@@ -576,7 +576,7 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
     p.weight = cut_of(width, D, rows, p.pairs, true);
     Parts at;
     p.h16 = at.add(rows * p.Dp * 2);
-    p.w16 = at.add(V * p.Dp * 2);
+    p.w16 = at.add(copies_weight ? V * p.Dp * 2 : 0);
     p.counted = at.add(4);
     p.place = at.add(rows * 4);
     p.list = at.add(rows * 4);
@@ -599,17 +599,19 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
 
 }  // namespace
 
-size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab) {
-    return rows ? head_plan(rt, rows, channels, vocab).bytes : 0;
+size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, bool copies_weight) {
+    return rows ? head_plan(rt, rows, channels, vocab, copies_weight).bytes : 0;
 }
 
+// Dense weights that a tensor map takes are read where they are.
+bool head_copies_weight(const void* dense, size_t channels) { return !dense || channels % 8 != 0 || !aligned(dense, 16); }
+
 void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
-    const HeadPlan p = head_plan(s.rt, h.rows, h.channels, h.vocab);
+    const bool as_is = !head_copies_weight(h.weight, h.channels);
+    const HeadPlan p = head_plan(s.rt, h.rows, h.channels, h.vocab, !as_is);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const bool bf16 = h.dtype == BF16;
     const size_t rows = h.rows, D = h.channels, V = h.vocab;
-    // dense weights that a tensor map takes are read where they are
-    const bool as_is = !h.bits && D % 8 == 0 && aligned(h.weight, 16);
     const void* w16 = as_is ? h.weight : static_cast<const void*>(ws + p.w16);
 
     uint32_t* counted = reinterpret_cast<uint32_t*>(ws + p.counted);

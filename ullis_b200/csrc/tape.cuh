@@ -7,7 +7,7 @@
 // 8-bit operand goes through the tensor cores as the number it stands for.  A block with a value that is not finite has the
 // byte 255 and stands for NaN throughout.
 //
-// Kernels take a row in chunks of eight channels, one per thread, four threads to a block.
+// Kernels take a row in chunks of 16 bytes, one per thread: four channels in f32, eight in 16 bits.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -16,7 +16,7 @@
 namespace ullis {
 namespace tape {
 
-constexpr uint32_t BLOCK = 32, CHUNK = 8;
+constexpr uint32_t BLOCK = 32;
 constexpr uint32_t NOT_FINITE = 255;
 
 __host__ __device__ inline size_t blocks_of(size_t channels) { return (channels + BLOCK - 1) / BLOCK; }
@@ -44,98 +44,146 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight channels from c on of a row of `C`; past its end zeros.  VEC: rows start on 16 bytes and C is a multiple of 8, so a
-// chunk is whole or absent.
+// The channels of a chunk as they lie in memory: 16 bytes, so that neighbouring threads read and write neighbouring pieces.
+template <typename T>
+constexpr int CHUNK = 16 / (int)sizeof(T);
+template <typename T>
+struct Raw {
+    uint4 q;
+    __device__ __forceinline__ void unpack(float (&v)[CHUNK<T>]) const {
+        const T* t = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int i = 0; i < CHUNK<T>; ++i) v[i] = to_float(t[i]);
+    }
+};
+// From channel c on of a row of `C`; past its end zeros.  VEC: rows start on 16 bytes and C is a multiple of 8, so a chunk is whole or
+// absent.
 template <bool VEC, typename T>
-__device__ __forceinline__ void load8(const T* row, uint32_t c, uint32_t C, float (&v)[8]) {
+__device__ __forceinline__ Raw<T> load_raw(const T* row, uint32_t c, uint32_t C) {
+    Raw<T> r;
+    r.q = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (VEC) {
+        if (c < C) r.q = *reinterpret_cast<const uint4*>(row + c);
+    } else {
+        T* t = reinterpret_cast<T*>(&r.q);
+#pragma unroll
+        for (int i = 0; i < CHUNK<T>; ++i)
+            if (c + i < C) t[i] = row[c + i];
+    }
+    return r;
+}
+// N FP16 numbers (weights), N = 4 or 8
+template <bool VEC, int N>
+__device__ __forceinline__ void load_halves(const uint16_t* row, uint32_t c, uint32_t C, float (&v)[N]) {
+    uint32_t w[N / 2] = {};
     if constexpr (VEC) {
         if (c < C) {
-            if constexpr (sizeof(T) == 4) {
-                const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
-                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-                v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            if constexpr (N == 8) {
+                const uint4 t = *reinterpret_cast<const uint4*>(row + c);
+                w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
             } else {
-                const uint4 w = *reinterpret_cast<const uint4*>(row + c);
-                const T* t = reinterpret_cast<const T*>(&w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = to_float(t[i]);
+                const uint2 t = *reinterpret_cast<const uint2*>(row + c);
+                w[0] = t.x; w[1] = t.y;
             }
-            return;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < C ? to_float(row[c + i]) : 0.0f;
+        for (int i = 0; i < N; ++i)
+            if (c + i < C) w[i >> 1] |= (uint32_t)row[c + i] << (16 * (i & 1));
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __half2float(__ushort_as_half((uint16_t)(w[i >> 1] >> (16 * (i & 1)))));
 }
 template <bool VEC, typename T>
-__device__ __forceinline__ void store8(T* row, uint32_t c, uint32_t C, const float (&v)[8]) {
+__device__ __forceinline__ void store_chunk(T* row, uint32_t c, uint32_t C, const float (&v)[CHUNK<T>]) {
     if constexpr (VEC) {
         if (c >= C) return;
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(row + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            uint4 w;
-            T* t = reinterpret_cast<T*>(&w);
+        uint4 w;
+        T* t = reinterpret_cast<T*>(&w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = from_float<T>(v[i]);
-            *reinterpret_cast<uint4*>(row + c) = w;
-        }
+        for (int i = 0; i < CHUNK<T>; ++i) t[i] = from_float<T>(v[i]);
+        *reinterpret_cast<uint4*>(row + c) = w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < CHUNK<T>; ++i)
             if (c + i < C) row[c + i] = from_float<T>(v[i]);
     }
 }
-// The exponent byte of the block whose four chunks the four lanes of a quad hold.
-__device__ __forceinline__ uint32_t quad_exponent(const float (&v)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);   // of NaN too: above infinity
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    return exponent_byte(top);
+// The exponent byte of the block whose chunks of N channels lie in 32 / N neighbouring lanes.
+__device__ __forceinline__ float larger(float a, float b) {   // of a and |b|, NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
 }
-template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* codes, uint32_t c, uint32_t C, const float (&v)[8], float inverse) {
-    uint32_t w[2] = {0u, 0u};
+template <int N>
+__device__ __forceinline__ uint32_t block_exponent(const float (&v)[N]) {
+    float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        w[i >> 2] |= (uint32_t)(min(max(__float2int_rn(v[i] * inverse), -127), 127) & 0xFF) << (8 * (i & 3));   // (0 for NaN)
+    for (int i = 0; i < N; ++i) top = larger(top, v[i]);
+    uint32_t bits = __float_as_uint(top) & 0x7FFFFFFFu;   // (of NaN: above infinity)
+#pragma unroll
+    for (int o = 1; o < (int)BLOCK / N; o <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    return exponent_byte(bits);
+}
+// Codes of a block with this exponent byte.  x * 2^-e + 1.5 * 2^23 is rounded to whole numbers by the addition (ties to even; the
+// product is exact), and its lowest byte is the code: an FMA instead of a multiplication and a conversion, which goes at a quarter
+// of its rate and, with the two bounds, made LayerNorm with the tape issue-bound (131072 x 512 bf16 78 us, so 60).
+template <int N>
+__device__ __forceinline__ void codes_of(const float (&v)[N], uint32_t byte, uint32_t (&w)[N / 4]) {
+    const float inverse = inverse_power(byte);
+    uint32_t r[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = __float_as_uint(fmaf(v[i], inverse, 12582912.0f));
+    if (byte >= 248u) {   // the last exponent, above which lies what no code reaches, or not finite: hardly ever
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = byte == NOT_FINITE ? 0u : (uint32_t)min(max(__float2int_rn(v[i] * inverse), -127), 127);
+    }
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k)
+        w[k] = __byte_perm(__byte_perm(r[k * 4], r[k * 4 + 1], 0x0040), __byte_perm(r[k * 4 + 2], r[k * 4 + 3], 0x0040), 0x5410);
+}
+template <bool VEC, int N>
+__device__ __forceinline__ void store_codes(uint8_t* codes, uint32_t c, uint32_t C, const float (&v)[N], uint32_t byte) {
+    uint32_t w[N / 4];
+    codes_of(v, byte, w);
     if constexpr (VEC) {
-        if (c < C) *reinterpret_cast<uint2*>(codes + c) = make_uint2(w[0], w[1]);
+        if (c >= C) return;
+        if constexpr (N == 8) *reinterpret_cast<uint2*>(codes + c) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(codes + c) = w[0];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < N; ++i)
             if (c + i < C) codes[c + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
 }
-// Eight codes times `step`; past the row's end zeros (whatever the step).
-template <bool VEC>
-__device__ __forceinline__ void load_codes(const uint8_t* codes, float step, uint32_t c, uint32_t C, float (&v)[8]) {
-    uint32_t w[2] = {0u, 0u};
-    if (c < C) {
-        if constexpr (VEC) {
-            const uint2 t = *reinterpret_cast<const uint2*>(codes + c);
-            w[0] = t.x; w[1] = t.y;
-        } else {
+// N codes times `step`; past the row's end zeros (whatever the step).
+template <int N>
+__device__ __forceinline__ void values_of(const uint32_t (&w)[N / 4], float step, float (&v)[N]) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < C) w[i >> 2] |= (uint32_t)codes[c + i] << (8 * (i & 3));
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * step;
-        v[i] = (VEC ? c : c + i) < C ? x : 0.0f;
-    }
+    for (int i = 0; i < N; ++i) v[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * step;
 }
-// What they stand for.
-template <bool VEC>
-__device__ __forceinline__ void load_codes(const uint8_t* codes, const uint8_t* exponents, uint32_t c, uint32_t C, float (&v)[8]) {
-    load_codes<VEC>(codes, c < C ? power(exponents[c / BLOCK]) : 0.0f, c, C, v);
+template <bool VEC, int N>
+__device__ __forceinline__ void load_codes(const uint8_t* codes, float step, uint32_t c, uint32_t C, float (&v)[N]) {
+    uint32_t w[N / 4] = {};
+    if constexpr (VEC) {
+        if (c < C) {
+            if constexpr (N == 8) {
+                const uint2 t = *reinterpret_cast<const uint2*>(codes + c);
+                w[0] = t.x; w[1] = t.y;
+            } else {
+                w[0] = *reinterpret_cast<const uint32_t*>(codes + c);
+            }
+        }
+        values_of(w, c < C ? step : 0.0f, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (c + i < C) w[i >> 2] |= (uint32_t)codes[c + i] << (8 * (i & 3));
+        values_of(w, step, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (c + i >= C) v[i] = 0.0f;
+    }
 }
 #endif
 

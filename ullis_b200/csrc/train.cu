@@ -1171,7 +1171,7 @@ void ullis_cuda_train_state::step(const uint32_t* tokens, const uint32_t* labels
         h.g_hidden = GX;
         h.g_weight = gmat.as<float>(vocab * d);
         h.g_bias = head.bias.w ? SM : nullptr;
-        dev::head_ce_grad(own, h, lean.ensure(dev::head_ce_grad_workspace(rt, rows, d, vocab)));
+        dev::head_ce_grad(own, h, lean.ensure(dev::head_ce_grad_workspace(rt, rows, d, vocab, true)));
         reduce_loss();
         if (head.bias.w) s.sgd(head.bias, SM, learning_rate * HEAD_BIAS_LR_MULT);
         s.packed_step(head, tc::Partials{gmat.as<float>(vocab * d), 1}, CNT + 0, SM);

@@ -59,7 +59,7 @@ _ARGTYPES = {
     "tape_layer_norm_backward": (_V, _V, _I, _V, _V, _V, _Z, _V, _V, _Z, _Z, _Z, _V, _V, _V, _V, _Z),
     "tape_weight_grad_workspace": (_V, _Z, _Z, _Z, _V),
     "tape_weight_grad": (_V, _V, _I, _V, _V, _V, _Z, _Z, _Z, _Z, _V, _V, _Z),
-    "head_ce_grad_workspace": (_V, _Z, _Z, _Z, _V),
+    "head_ce_grad_workspace": (_V, _Z, _Z, _Z, _I, _V),
     "head_ce_grad": (_V, _V, _I, _V, _Z, _V, _V, _V, _V, _V, _U, _Z, _Z, _Z, _Z, _F, _V, _V, _V, _V, _V, _V, _Z),
 }
 
@@ -273,8 +273,9 @@ class DeviceOps:
         g_weight = torch.empty(vocab, channels, dtype=hidden.dtype, device=hidden.device)
         g_scale = None if scale is None else _like(scale, torch.float32)
         g_bias = None if bias is None else _like(bias, torch.float32)
-        work, size = self._workspace(hidden, "head_ce_grad", rows, channels, vocab)
         at = weight.data_ptr()
+        copies = scale is not None or channels % 8 != 0 or at % 16 != 0
+        work, size = self._workspace(hidden, "head_ce_grad", rows, channels, vocab, int(copies))
         self._check(self._lib.ullis_cuda_head_ce_grad(
             self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], hidden.data_ptr(), stride, at if scale is not None else None,
             at if scale is None else None, _p(scale), _p(bias), labels.data_ptr(), ignore & 0xFFFFFFFF, rows, time, channels, vocab,
