@@ -190,6 +190,37 @@ def test_a_softmax_that_is_almost_one_hot(cuda_rt):
         check(call(cuda_rt, s), want)
 
 
+def test_rows_that_are_sure_have_small_gradients(cuda_rt):
+    """Gradients of rows whose loss is 1e-8 to 1e-4, to a relative bound.  Hidden states are multiples of 1/8 and weights +-1, so
+    the products are exact in any order, and a logit in units of ln 2, below 64, is off by the roundings of its scale and its
+    bias and of itself, 3 * 2^-24 * 64.  A target's 1 - p, and p of another column, take two logits and a sum of 400
+    terms: off by less than 2 * 1.2e-5 * ln 2 + 80 * 2^-24 + 2^-21 < 2^-14 relatively."""
+    g = torch.Generator("cuda").manual_seed(5)
+    rows, d, vocab = 600, 1000, 400
+    s = inputs(rows, rows, d, vocab, "bf16", True, lean=2.0)
+    s["hidden"] = ((torch.randn(rows, d, generator=g, device="cuda") * 8).round() / 8).clamp(-6, 6)
+    s["hidden"] += 2.0 * signs(s["weight"], vocab, d)[torch.roll(s["labels"], -1).long()].float()
+    s["hidden"] = s["hidden"].bfloat16()
+    assert torch.equal(s["hidden"].float() * 8, (s["hidden"].float() * 8).round())
+    s["scale"].clamp_(max=0.0155)
+    got = call(cuda_rt, s)
+    a = s["hidden"].double() @ signs(s["weight"], vocab, d).t()
+    z = a * s["scale"].double() + s["bias"].double()
+    assert z.abs().max() / math.log(2.0) < 64
+    after, at = torch.roll(s["labels"], -1).long(), torch.arange(rows, device="cuda")
+    rest = torch.exp(z).scatter(1, after[:, None], 0.0)
+    hit = torch.exp(z.gather(1, after[:, None])[:, 0])
+    p = rest / (rest.sum(1) + hit)[:, None]
+    p[at, after] = -rest.sum(1) / (rest.sum(1) + hit)
+    p[-1] = 0.0
+    loss = torch.log1p(rest.sum(1) / hit)[:-1]
+    assert 1e-12 < loss.min() and loss.median() < 1e-4
+    assert ((got.row_loss[:-1].double() - loss).abs() <= 2.0 ** -14 * loss).all()
+    for x, value in ((got.bias, p), (got.scale, p * a)):
+        off = (2.0 ** -14 + U * (16 + rows)) * value.abs().sum(0)
+        assert ((x.double() - value.sum(0)).abs() <= off).all()
+
+
 @pytest.mark.parametrize("packed", [True, False], ids=["packed", "dense"])
 def test_masked_rows_hold_anything(cuda_rt, packed):
     s = inputs(260, 130, 64, 500, "bf16", packed, 0.4)

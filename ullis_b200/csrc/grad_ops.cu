@@ -388,9 +388,10 @@ head_operands_kernel(const HeadOperands o) {
             o.target[place] = target;
             if (o.fold) dot *= __half2float(__ushort_as_half(o.scale[target]));
             o.target_acc[place] = dot;
-            if (o.scale && !o.fold) dot *= __half2float(__ushort_as_half(o.scale[target]));
-            if (o.bias) dot += __half2float(__ushort_as_half(o.bias[target]));
-            o.logit2[place] = dot * pg::LOG2E;
+            // rounded as the epilogues round theirs: the difference of two logits is then what it is
+            const float scale = o.scale && !o.fold ? __half2float(__ushort_as_half(o.scale[target])) : 1.0f;
+            const float bias = o.bias ? __half2float(__ushort_as_half(o.bias[target])) : 0.0f;
+            o.logit2[place] = fmaf(dot, scale * pg::LOG2E, bias * pg::LOG2E);
         }
         return;
     }
@@ -436,7 +437,7 @@ struct HeadRows {
     const int32_t* list;
     uint32_t n_tiles, piece_tiles, pairs;
     const float* logit2;
-    float *lse2, *row_loss;
+    float *lse2, *target_g, *row_loss;
     const float* scale_max;   // null: no row scales
     float* factors;           // 2^k, 2^-k * loss_scale
     float loss_scale;
@@ -499,10 +500,23 @@ head_rows_kernel(const HeadRows o) {
     }
     if (lane || row >= rows) return;
     const float logit2 = o.logit2[row];
-    add(logit2, 1.0f);
-    const float lse2 = top + log2f(sum);
-    o.lse2[row] = lse2;
-    o.row_loss[o.list[row]] = (lse2 - logit2) * LN2;
+    // The loss and the target's 1 - p from the sum of the other columns, which a sum with the target in it has lost where a row is sure
+    float more, loss, g;   // (more: lse2 over the larger of logit2 and top)
+    if (top <= logit2) {
+        const float others = sum * exp2f(top - logit2);
+        loss = log1pf(others) + (logit2 - logit2);   // (NaN where that is infinite)
+        g = -others / (1.0f + others);
+        more = loss * pg::LOG2E;
+        top = logit2;
+    } else {
+        const float all = sum + exp2f(logit2 - top);
+        more = log2f(all);
+        loss = ((top - logit2) + more) * LN2;
+        g = -sum / all;
+    }
+    o.lse2[row] = top + more;
+    o.target_g[row] = g;
+    o.row_loss[o.list[row]] = loss;
 }
 
 // The columns' sums of a piece out of their parts, times loss_scale.  32 columns to a CTA, a warp to each of a slot's eight parts.
@@ -545,7 +559,7 @@ struct HeadPlan {
     size_t piece, pieces;                        // columns of a piece of g (a multiple of 256), pieces
     uint32_t col_slots;
     Cut hidden, weight;
-    size_t h16, w16, counted, place, list, target, target_acc, target_cut, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, hidden_partial, weight_partial, bytes;
+    size_t h16, w16, counted, place, list, target, target_acc, target_g, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, hidden_partial, weight_partial, bytes;
 };
 constexpr size_t GRAD_ELEMENTS = (size_t)1 << 28;   // of a piece of g: 512 MiB
 
@@ -582,7 +596,7 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
     p.list = at.add(rows * 4);
     p.target = at.add(rows * 4);
     p.target_acc = at.add(rows * 4);
-    p.target_cut = at.add(rows * 4);
+    p.target_g = at.add(rows * 4);
     p.lse2 = at.add(rows * 4);
     p.logit = at.add(rows * 4);
     p.factors = at.add(8);
@@ -668,7 +682,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     q.row_part_piece = p.row_part_piece;
     q.row_part = reinterpret_cast<float2*>(ws + p.row_part);
     q.target_acc = o.target_acc;
-    q.target_cut = reinterpret_cast<float*>(ws + p.target_cut);
+    q.target_g = reinterpret_cast<float*>(ws + p.target_g);
     q.lse2 = reinterpret_cast<float*>(ws + p.lse2);
     float* factors = reinterpret_cast<float*>(ws + p.factors);
     launch<pg::LSE, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
@@ -683,6 +697,7 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     r.pairs = p.pairs;
     r.logit2 = o.logit2;
     r.lse2 = reinterpret_cast<float*>(ws + p.lse2);
+    r.target_g = reinterpret_cast<float*>(ws + p.target_g);
     r.row_loss = h.row_loss;
     r.scale_max = q.scale ? o.scale_max : nullptr;
     r.factors = factors;

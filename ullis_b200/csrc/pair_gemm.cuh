@@ -43,7 +43,6 @@ constexpr uint32_t MAX_STAGES = 6, SMEM_LIMIT = 227 * 1024;
 constexpr uint32_t STAGING_BYTES = 16 * 128;            // 16 rows of 64 16-bit outputs; GRAD has two of them
 constexpr uint32_t COLUMN_BYTES = 2 * 64 * 4;           // constants of its columns
 constexpr uint32_t ROW_BYTES = 2 * 4 * 32 * 4;          // GRAD: what its rows need, of this tile and of the next
-constexpr uint32_t HIT_BYTES = 2 * 64 * 4;              // GRAD: what the targets add to the columns' sums
 constexpr uint32_t SUM_BLOCKS = 8;                      // k-blocks between two rounded additions
 
 struct Maps {
@@ -68,8 +67,8 @@ struct Params {
     float2* row_part;          // LSE: [piece] of [slot][4][rows that count, whole tiles]
     size_t row_part_piece;     // elements of a piece
     const float* lse2;         // GRAD: [M] log2 of the sum of exp, +inf for a row that does not count
-    float* target_cut;         // [M] the target's product as the tensor cores have it (LSE leaves it, GRAD takes it out) ...
-    const float* target_acc;   // GRAD: ... and with rounding
+    const float* target_acc;   // GRAD: [M] the target's product, added with rounding
+    const float* target_g;     // GRAD: [M] its probability - 1
     const float* factor;       // GRAD: 2^k ; STORE: alpha
     uint32_t pitch;            // GRAD: of col_part, whole tiles
     float* col_part;           // GRAD: [slot][8][2][pitch]
@@ -88,7 +87,7 @@ struct Params {
 inline uint32_t stage_bytes(int accs) { return OPERAND_BYTES * (1 + accs); }
 // Barriers first, then (on 1024 bytes) the ring, then what the epilogue warps have.
 constexpr uint32_t epi_bytes(int epi) {
-    return epi == GRAD ? 2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES + HIT_BYTES : epi == STORE ? STAGING_BYTES : epi == LSE ? COLUMN_BYTES : 0u;
+    return epi == GRAD ? 2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES : epi == STORE ? STAGING_BYTES : epi == LSE ? COLUMN_BYTES : 0u;
 }
 inline uint32_t fixed_bytes(int epi) { return 2 * 1024 /*barriers, alignment*/ + EPI_WARPS * epi_bytes(epi); }
 inline uint32_t stages_for(int epi, int accs) {
@@ -533,12 +532,6 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     else drained();
                     const int32_t hit = target - (int32_t)(n0 + c * 16);
                     const bool hits = __any_sync(0xffffffffu, hit >= 0 && hit < 16);   // of the warp's rows
-                    if (hits) {   // (by bits: chosen by an index, the accumulators went to local memory)
-                        uint32_t cut = 0;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) cut |= hit == i ? now[i] : 0u;
-                        if (hit >= 0 && hit < 16) p.target_cut[m_now * BM + rank * 128 + quarter * 32 + lane] = __uint_as_float(cut);
-                    }
                     uint64_t z[8];
                     float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -583,11 +576,8 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             uint64_t g_sum[8], ga_sum[8];   // of column pairs 8 j + q2
 #pragma unroll
             for (int j = 0; j < 8; ++j) g_sum[j] = ga_sum[j] = 0;
-            float* hits = reinterpret_cast<float*>(epi_smem + EPI_WARPS * (2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES) + mine * HIT_BYTES);
-            for (int i = lane; i < 128; i += 32) hits[i] = 0.0f;
             const auto leave = [&]() {   // the sums of 32 rows: over the lanes that share columns, then out
                 if (n_now == 0xFFFFFFFFu) return;
-                __syncwarp();
                 const uint32_t slot = pair - all.owner(n_now * work.m_tiles);
                 float* to = p.col_part + (((size_t)slot * 8 + rank * 4 + quarter) * 2) * p.pitch + n_now * BN + group * 64 + q2;
 #pragma unroll
@@ -598,16 +588,14 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         ga_sum[j] = add2(ga_sum[j], __shfl_xor_sync(0xffffffffu, ga_sum[j], o));
                     }
                     if (lane < 4) {
-                        *reinterpret_cast<uint64_t*>(to + j * 8) = add2(g_sum[j], *reinterpret_cast<const uint64_t*>(hits + j * 8 + q2));
-                        *reinterpret_cast<uint64_t*>(to + p.pitch + j * 8) = add2(ga_sum[j], *reinterpret_cast<const uint64_t*>(hits + 64 + j * 8 + q2));
+                        *reinterpret_cast<uint64_t*>(to + j * 8) = g_sum[j];
+                        *reinterpret_cast<uint64_t*>(to + p.pitch + j * 8) = ga_sum[j];
                     }
                     g_sum[j] = ga_sum[j] = 0;
                 }
-                __syncwarp();
-                for (int i = lane; i < 128; i += 32) hits[i] = 0.0f;   // (by the lane that adds to it)
             };
             // What the rows need lies in shared memory, two tiles in turn; the next tile's is on its way while one is worked on: a
-            // word each of lse2, the target's two products and the target per lane.
+            // word each of lse2, the target's product, its g and the target per lane.
             float* row_smem = reinterpret_cast<float*>(epi_smem + EPI_WARPS * (2 * STAGING_BYTES + COLUMN_BYTES) + mine * ROW_BYTES);
             const auto fetch = [&](uint32_t turn) {
                 const uint32_t row = work.m * BM + rank * 128 + quarter * 32 + lane;
@@ -615,7 +603,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 float* to = row_smem + turn * 128 + lane;
                 copy_word(to, p.lse2 + (in ? row : 0), in);
                 copy_word(to + 32, p.target_acc + (in ? row : 0), in);
-                copy_word(to + 64, p.target_cut + (in ? row : 0), in);
+                copy_word(to + 64, p.target_g + (in ? row : 0), in);
                 copy_word(to + 96, p.target + (in ? row : 0), in);
             };
             const uint32_t blocks_at = ptx::smem_u32(staging) + ((lane >> 3) & 1) * 1024 + (lane & 7) * 128;   // of store_blocks: block b has
@@ -637,52 +625,28 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 __syncwarp();
                 const float* rows = row_smem + turn * 128;
                 turn ^= 1;
-                // Of this lane's row: the target's column among the warp's 64, or another number.  Its g has the product with rounding
-                // in it and the -1 of the one-hot; the loop below knows nothing of that: g goes to its place in the 16-bit block behind
-                // the loop, and what it is more than the loop's exp to the column's sums by itself.  (As comparisons within the loop the
-                // targets took a fifth of this epilogue.)  A lane has columns lane and 32 + lane, in the order of the rows.
-                const uint32_t own = m0 + lane < M ? reinterpret_cast<const uint32_t*>(rows)[96 + lane] - (p.n_first + n0) : 64u;
-                float own_g = 0.0f;
-                uint32_t left = __ballot_sync(0xffffffffu, own < 64u);
-                if (left) {
-                    float more_g = 0.0f, more_ga = 0.0f;
-                    if (own < 64u) {
-                        const float acc = rows[32 + lane], cut = rows[64 + lane];
-                        const float p_cut = exp2_fast(fmaf(cut, columns[own], columns[64 + own]) - rows[lane]);
-                        own_g = exp2_fast(fmaf(acc, columns[own], columns[64 + own]) - rows[lane]) - 1.0f;
-                        more_g = own_g - p_cut;
-                        more_ga = own_g * acc - p_cut * cut;
-                        own_g *= columns[own] * from_log2;
-                    }
-                    float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    for (; left; left &= left - 1) {
-                        const int row = __ffs(left) - 1;
-                        const uint32_t column = __shfl_sync(0xffffffffu, own, row);
-                        const float g = __shfl_sync(0xffffffffu, more_g, row), ga = __shfl_sync(0xffffffffu, more_ga, row);
-                        add[0] += column == lane ? g : 0.0f;
-                        add[1] += column == lane + 32u ? g : 0.0f;
-                        add[2] += column == lane ? ga : 0.0f;
-                        add[3] += column == lane + 32u ? ga : 0.0f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) hits[i * 32 + lane] += add[i];
-                }
+                const uint32_t first = p.n_first + n0;
+                const bool any = __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
                 more = work.next();
                 if (more) fetch(turn);
                 uint32_t taddr;
                 if (!filled(&taddr)) break;
                 taddr += group * 64;
-                // 16 rows at a time, one copy of the code for both: with two the registers ran out
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
+                // 16 rows at a time, one copy of the code for both: with two the registers ran out.  TARGETS: the target of one of the
+                // warp's rows lies in its columns.  Its product and its g are the row's: lse2 is a number of the size of the logits, off
+                // by 2e-6 where those are 36, and a model that is sure leaves a g of that size.
+                const auto half = [&](int h, auto targets) {
                     uint32_t r[2][8];   // 16 columns are on their way while 16 are worked on
                     tmem_ld_16x16(taddr + ((h * 16) << 16), r[0]);
                     uint64_t l[2];
+                    uint32_t at[2];   // the target's column less q2
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t row = h * 16 + i * 8 + r0;
                         const float lse = m0 + row < M ? -rows[row] : -INFINITY;
                         l[i] = two(lse, lse);
+                        if (decltype(targets)::value)
+                            at[i] = m0 + row < M ? reinterpret_cast<const uint32_t*>(rows)[96 + row] - first - q2 : 0x80000000u;
                     }
                     const uint32_t to = blocks_at + h * STAGING_BYTES;
                     if (lane == 0) tma_store_read<1>();   // the store before the last has read this half
@@ -701,9 +665,16 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             const uint64_t k = mul2(s, two(from_log2, from_log2));
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
-                                const uint64_t a = (uint64_t)now[u * 4 + i * 2 + 1] << 32 | now[u * 4 + i * 2];
+                                uint64_t a = (uint64_t)now[u * 4 + i * 2 + 1] << 32 | now[u * 4 + i * 2];
                                 const float2 e = of_two(add2(fma2(a, s, b), l[i]));
-                                const uint64_t g = two(exp2_fast(e.x), exp2_fast(e.y));
+                                uint64_t g = two(exp2_fast(e.x), exp2_fast(e.y));
+                                if (decltype(targets)::value) {
+                                    const uint32_t row = h * 16 + i * 8 + r0;
+                                    const bool x = at[i] == (uint32_t)(j + u) * 8, y = at[i] == (uint32_t)(j + u) * 8 + 1;
+                                    const float2 av = of_two(a), gv = of_two(g);
+                                    a = two(x ? rows[32 + row] : av.x, y ? rows[32 + row] : av.y);
+                                    g = two(x ? rows[64 + row] : gv.x, y ? rows[64 + row] : gv.y);
+                                }
                                 g_sum[j + u] = add2(g_sum[j + u], g);
                                 ga_sum[j + u] = fma2(g, a, ga_sum[j + u]);
                                 const float2 o = of_two(mul2(g, k));
@@ -713,16 +684,17 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         // 16-byte piece c of row r at c ^ (r % 8), as the copy below reads it; no bank conflicts
                         store_blocks(to + (((j + block_piece) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
                     }
-                    __syncwarp();
-                    if (own < 64u && lane >> 4 == h)   // this lane's row has its target here
-                        *reinterpret_cast<uint16_t*>(staging + h * STAGING_BYTES + (lane & 15) * 128 + (((own >> 3) ^ (lane & 7)) << 4) + (own & 7) * 2) =
-                            (uint16_t)pack16<BF16>(own_g, 0.0f);
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
                         if (m0 + h * 16 < p.M) tma_store_2d(&maps.out, ptx::smem_u32(staging) + h * STAGING_BYTES, (int32_t)n0, (int32_t)(m0 + h * 16));
                         else asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // (the groups stay in turn)
                     }
+                };
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    if (any) half(h, std::true_type{});
+                    else half(h, std::false_type{});
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
