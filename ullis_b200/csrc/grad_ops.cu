@@ -98,7 +98,9 @@ void launch(const Stream& s, const char* what, const Operand& a, const Operand& 
 
 // How a product [M, N] over K is cut for `pairs` pairs: accumulators of 256 columns per pair (one or two) and ranges of K.
 // Estimated in k-blocks (256 x 256 x 64 on a pair, 0.3 us): rounds * (k-blocks + an epilogue nothing overlaps) and, with several
-// ranges, their sums written and read once more at 4 TB/s.
+// ranges, their sums written and read once more: at 8 TB/s for a product that runs alone, whose sums stay in L2 (2048 x 512 x 2048
+// takes 20.1 us in three ranges, 21.8 in one, which 4 TB/s would choose), at 4 TB/s for the head's two beside one another (at 8 a
+// ragged batch of 7655 x 256 x 10007, half of its rows not counted, takes 167 us instead of 137).
 struct Cut {
     uint32_t accs, splits;
 };
@@ -112,7 +114,7 @@ Cut cut_of(size_t M, size_t N, size_t K, uint32_t pairs, bool two) {
             const double rounds = (double)ceil_div(tiles * splits, pairs);
             const double epilogue = accs == 2 ? 10.0 : 1.0;
             double cost = rounds * (ceil_div(blocks, splits) * accs + epilogue) + 4.0;
-            if (splits > 1) cost += (2.0 * splits + 1.0) * M * N * 4.0 / 4e6 / 0.3 + 8.0;
+            if (splits > 1) cost += (2.0 * splits + 1.0) * M * N * 4.0 / (two ? 4e6 : 8e6) / 0.3 + 8.0;
             if (cost < least) {
                 least = cost;
                 best = Cut{accs, splits};
@@ -761,26 +763,31 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
 // ------------------------------------------------------------------------------------------------ weight gradient from the tape
 namespace {
 
-// The largest exponent byte of each block of 32 channels, over TOP_SLICES slices of the rows: top [slice][blocks].  A CTA has 32
-// blocks of a slice, eight threads share a block's rows.
+// The largest exponent byte of each block of 32 channels, over TOP_SLICES slices of the rows: top [blocks][slices].  A CTA has 32
+// blocks of a slice.  WIDE: a thread reads four blocks' bytes in one word, and 32 rows are on their way at a time instead of 8.
 constexpr uint32_t TOP_SLICES = 32;
+template <bool WIDE>
 __global__ void __launch_bounds__(THREADS)
 tape_exponent_max_kernel(const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t blocks, uint8_t* __restrict__ top) {
     chain_entry();
-    const uint32_t slice = blockIdx.y, b = blockIdx.x * 32 + (threadIdx.x & 31);
+    constexpr uint32_t LANES = WIDE ? 8 : 32, STEP = THREADS / LANES;
+    const uint32_t slice = blockIdx.y, lane = threadIdx.x % LANES, b = blockIdx.x * 32 + lane * (32 / LANES);
     const uint32_t first = (uint32_t)((uint64_t)slice * rows / TOP_SLICES), last = (uint32_t)((uint64_t)(slice + 1) * rows / TOP_SLICES);
     __shared__ uint32_t tops[THREADS];
     uint32_t most = 0;
     if (b < blocks) {
-#pragma unroll 16
-        for (uint32_t r = first + (threadIdx.x >> 5); r < last; r += 8) most = max(most, (uint32_t)exponents[(size_t)r * blocks + b]);
+#pragma unroll 8
+        for (uint32_t r = first + threadIdx.x / LANES; r < last; r += STEP) {
+            const uint8_t* at = exponents + (size_t)r * blocks + b;
+            most = __vmaxu4(most, WIDE ? *reinterpret_cast<const uint32_t*>(at) : (uint32_t)*at);
+        }
     }
     tops[threadIdx.x] = most;
     __syncthreads();
-    if (threadIdx.x >= 32 || b >= blocks) return;
+    if (threadIdx.x >= LANES || b >= blocks) return;
 #pragma unroll
-    for (int k = 1; k < 8; ++k) most = max(most, tops[threadIdx.x + 32 * k]);
-    top[slice * blocks + b] = (uint8_t)most;
+    for (uint32_t k = 1; k < STEP; ++k) most = __vmaxu4(most, tops[threadIdx.x + LANES * k]);
+    for (uint32_t k = 0; k < 32 / LANES; ++k) top[(b + k) * TOP_SLICES + slice] = (uint8_t)(most >> 8 * k);
 }
 
 // What the codes stand for as a 16-bit operand [rows, Cp].  bf16 holds every value (8 significant bits, the range of f32).  FP16
@@ -800,8 +807,10 @@ tape_operand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict
     const uint32_t c = (uint32_t)(item - group * chunks) * 8, b = c / 32;
     uint32_t most = 0;
     if (!BF) {
-#pragma unroll
-        for (uint32_t k = 0; k < TOP_SLICES; ++k) most = max(most, (uint32_t)top[k * blocks + b]);
+        const uint4 u = reinterpret_cast<const uint4*>(top + b * TOP_SLICES)[0], w = reinterpret_cast<const uint4*>(top + b * TOP_SLICES)[1];
+        most = __vmaxu4(__vmaxu4(__vmaxu4(u.x, u.y), __vmaxu4(u.z, u.w)), __vmaxu4(__vmaxu4(w.x, w.y), __vmaxu4(w.z, w.w)));
+        most = __vmaxu4(most, most >> 16);
+        most = max(most & 0xff, most >> 8 & 0xff);
         if (row0 == 0 && c % 32 == 0) col_factor[b] = most == tape::NOT_FINITE ? 1.0f : exp2f((float)((int)most - 127 - 8));
     }
     float v[OPERAND_ROWS][8];
@@ -877,7 +886,9 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
     const uint32_t blocks = (uint32_t)tape::blocks_of(in);
     const unsigned grid = (unsigned)ceil_div(ceil_div(rows, OPERAND_ROWS) * (p.ip / 8), THREADS);
     const bool vec = in % 8 == 0 && aligned(codes, 8);
-    if (!bf16) s.chain("tape_exponent_max", tape_exponent_max_kernel, dim3((blocks + 31) / 32, TOP_SLICES), THREADS, 0, exponents, (uint32_t)rows, blocks, top);
+    const bool wide = blocks % 4 == 0 && aligned(exponents, 4);
+    if (!bf16)
+        s.chain("tape_exponent_max", wide ? tape_exponent_max_kernel<true> : tape_exponent_max_kernel<false>, dim3((blocks + 31) / 32, TOP_SLICES), THREADS, 0, exponents, (uint32_t)rows, blocks, top);
     const auto operand = bf16 ? (vec ? tape_operand_kernel<true, true> : tape_operand_kernel<true, false>)
                               : (vec ? tape_operand_kernel<false, true> : tape_operand_kernel<false, false>);
     s.chain("tape_operand", operand, grid, THREADS, 0, codes, exponents, (uint32_t)rows, (uint32_t)in, (uint32_t)p.ip,
