@@ -12,6 +12,9 @@
 // hold most of it (FP16 from 2^-24 to 65504), and the products are multiplied by 2^-k * loss_scale at the end.  The rounding of
 // g * scale to 16 bits is the same that the training step's operands have (half a step: 2^-11 in FP16, 2^-8 in bf16, independent
 // from term to term); g_scale and g_bias are sums of what was not rounded.
+//
+// Beside the products a call of 16384 x 512 x 8192 takes 7.6 us to list the rows that count, 11.4 to bring both operands into 16
+// bits, 5.6 for the rows' sums and 4.7 for the columns': reads and writes of what they name, bound by their latency.
 #include <algorithm>
 
 #include <cudaTypedefs.h>
@@ -793,7 +796,8 @@ tape_exponent_max_kernel(const uint8_t* __restrict__ exponents, uint32_t rows, u
 // What the codes stand for as a 16-bit operand [rows, Cp].  bf16 holds every value (8 significant bits, the range of f32).  FP16
 // does not: there each block of 32 channels is shifted by a power of two common to all rows, so that its largest exponent comes to 8
 // (127 * 2^8 = 32 512), and the column's sums are shifted back.  What is lost lies 2^32 below the block's largest value.
-// A thread has a chunk of eight columns and OPERAND_ROWS rows in turn.  VEC: as in tape.cuh.
+// A thread has a chunk of eight columns and OPERAND_ROWS rows in turn.  VEC: as in tape.cuh.  16384 x 512 in bf16 9.1 us (25 MB), 7655
+// x 2048 in FP16 12.8 (47 MB), its largest exponents 6.7.
 constexpr uint32_t OPERAND_ROWS = 4;
 template <bool BF, bool VEC>
 __global__ void __launch_bounds__(THREADS)
