@@ -503,7 +503,7 @@ ULLIS_CUDA_API int32_t ullis_cuda_tape_weight_grad(ullis_cuda_runtime* rt, void*
  * behind g_scale and g_bias are f32; g * scale is rounded to hidden's type for the
  * two gradient products, which accumulate in f32.  What rows hold that do not count
  * (infinities, NaN) has no effect.  A label outside the vocabulary makes its row's
- * loss NaN and gives no gradient.  Rows must be a multiple of `time`.
+ * loss NaN and gives no gradient.  Rows must be a multiple of `time`, at most 2^24.
  * copies_weight: 1 for a packed head, and for a dense one whose rows do not all start
  * on 16 bytes (channels no multiple of 8, or weight unaligned): the workspace then
  * holds the weights as an operand of the products. */

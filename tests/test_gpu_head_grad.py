@@ -388,3 +388,24 @@ def test_refusals_of_the_library(cuda_rt):
     assert rc(bits=None, weight=s["hidden"], scale=None) == cuda.ERR_ARG      # g_scale without scales
     torch.cuda.synchronize()
     assert not out.any()
+
+
+def test_more_rows_than_the_list_is_made_for(cuda_rt):
+    import ctypes as C
+    size = C.c_size_t(7)
+    fn = cuda_rt._lib.ullis_cuda_head_ce_grad_workspace
+    assert fn(cuda_rt._h, 1 << 24, 8, 100, 1, C.byref(size)) == cuda.OK and size.value > 0
+    assert fn(cuda_rt._h, (1 << 24) + 1, 8, 100, 1, C.byref(size)) == cuda.ERR_SHAPE and size.value == 0
+
+
+def test_offsets_past_32_bits(cuda_rt):
+    """More than 2^32 elements of hidden and of its gradient; rows that count at both ends, NaN in all others."""
+    rows, d, vocab, time = 2 ** 22 + 128, 1032, 70, 64
+    s = inputs(256, time, d, vocab, "bf16", True)
+    ends = torch.cat([torch.arange(128), torch.arange(rows - 128, rows)]).cuda()
+    big = dict(s, hidden=torch.full((rows, d), float("nan"), dtype=torch.bfloat16, device="cuda"),
+               labels=torch.full((rows,), -1, dtype=torch.int32, device="cuda"))
+    big["hidden"][ends], big["labels"][ends] = s["hidden"], s["labels"]
+    got = call(cuda_rt, big)
+    assert not got.hidden[128:-128].any() and not got.row_loss[128:-128].any()
+    check(got._replace(hidden=got.hidden[ends], row_loss=got.row_loss[ends]), formulas(s))

@@ -236,6 +236,30 @@ def test_offsets_past_32_bits(cuda_rt):
     assert torch.equal(tape.codes, codes) and torch.equal(tape.exponents, byte)
 
 
+def test_more_than_2_to_the_32_elements(cuda_rt):
+    """Rows at both ends as a call of those rows alone has them; the sums over rows have nothing of the others, whose gy is 0."""
+    rows, c, t = 2 ** 22 + 128, 1032, torch.bfloat16
+    g = torch.Generator("cuda").manual_seed(3)
+    x, gy, past = (torch.randn(256, c, generator=g, device="cuda").to(t) for _ in range(3))
+    w = (1 + 0.1 * torch.randn(c, generator=g, device="cuda")).half()
+    ends = torch.cat([torch.arange(128), torch.arange(rows - 128, rows)]).cuda()
+    big_x, big_gy = torch.ones(rows, c, dtype=t, device="cuda"), torch.zeros(rows, c, dtype=t, device="cuda")
+    big_x[ends], big_gy[ends] = x, gy
+    y, tape = cuda_rt.tape_layer_norm(big_x, w, w)
+    big_x[ends] = past
+    got = cuda_rt.tape_layer_norm_backward(tape, big_gy, w, residual=big_x)
+    small_y, small_tape = cuda_rt.tape_layer_norm(x, w, w)
+    want = cuda_rt.tape_layer_norm_backward(small_tape, gy, w, residual=past)
+    assert torch.equal(y[ends], small_y) and torch.equal(tape.codes[ends], small_tape.codes)
+    assert torch.equal(tape.exponents[ends], small_tape.exponents) and torch.equal(got[0][ends], want[0])
+    # 256 terms gy * xh, |xh| < 8, in two orders, each sum off by 2^-24 of its terms' sizes per addition
+    for a, b in zip(got[1:], want[1:]):
+        assert ((a - b).abs() <= 2 * 256 * 2.0 ** -24 * 8 * gy.float().abs().sum(0)).all()
+    assert torch.equal(cuda_rt.tape_unpack(tape, t)[ends], cuda_rt.tape_unpack(small_tape, t))
+    packed = cuda_rt.tape_pack(big_x)
+    assert torch.equal(packed.codes[ends], cuda_rt.tape_pack(past).codes)
+
+
 def test_refusals_of_the_library(cuda_rt):
     x = torch.zeros(2, 9000, device="cuda")
     w = torch.zeros(9000, device="cuda").half()

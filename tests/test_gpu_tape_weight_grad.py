@@ -134,3 +134,15 @@ def test_norm_linear_and_head_together(cuda_rt):
     # 8-bit inputs, and four 16-bit roundings on the way: half a step of 2^-7 is the largest of them
     for name, got, want in (("x", gx, kept.grad), ("norm weight", gw, wd.grad), ("norm bias", gb, bd.grad), ("linear", g_lin, ld.grad)):
         assert (got.double() - want).norm() <= 4 * 2.0 ** -7 * want.norm(), name
+
+
+def test_offsets_past_32_bits(cuda_rt):
+    """More than 2^32 elements of both operands; what is not zero lies at both ends."""
+    rows, i, o = 2 ** 22 + 128, 1030, 1040
+    small, gy = tape_of(256, i), torch.randn(256, o, device="cuda").half()
+    ends = torch.cat([torch.arange(128), torch.arange(rows - 128, rows)]).cuda()
+    codes = torch.zeros(rows, i, dtype=torch.int8, device="cuda")
+    exponents = torch.full((rows, small[1].shape[1]), 127, dtype=torch.uint8, device="cuda")
+    big = torch.zeros(rows, o, dtype=torch.float16, device="cuda")
+    codes[ends], exponents[ends], big[ends] = small[0], small[1], gy
+    check(cuda_rt.tape_weight_grad((codes, exponents), big), gy, small)

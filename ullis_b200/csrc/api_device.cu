@@ -113,6 +113,8 @@ void need_head(size_t rows, size_t channels, size_t vocab) {
     const char* what = "head cross-entropy";
     need_sizes(rows, channels, what);
     need_sizes(rows, vocab, what);
+    // (each 1024 rows of the list of those that count look at all labels before them)
+    if (rows > (size_t)1 << 24) fail(ULLIS_CUDA_ERR_SHAPE, std::string(what) + " takes at most 2^24 rows");
     need_tiles(rows, vocab, what);
     need_tiles(rows, channels, what);
     need_tiles(vocab, channels, what);

@@ -242,7 +242,8 @@ class DeviceOps:
         """Next-token cross-entropy of a head with its gradient; logits are never kept.
 
         hidden [..., channels] float16 or bfloat16; labels int32, one per row (a negative id and `ignore_id` are taken as the
-        unsigned 32-bit number they are); `time` rows to a sequence (default: all, or with three dimensions the second).  A
+        unsigned 32-bit number they are); `time` rows to a sequence (default: all, or with three dimensions the second; at
+        most 2^24 in all).  A
         packed head is `weight` int32 words of sign bits in checkpoint order with `scale` float16 [vocab]; a dense one is
         `weight` [vocab, channels] in hidden's type and no scale.  bias float16 [vocab] or None.  Gradients are of
         loss_scale * sum of row_loss; that of a packed weight is of the +/-1 values."""
