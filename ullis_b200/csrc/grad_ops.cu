@@ -104,6 +104,8 @@ void launch(const Stream& s, const char* what, const Operand& a, const Operand& 
 // ranges, their sums written and read once more: at 8 TB/s for a product that runs alone, whose sums stay in L2 (2048 x 512 x 2048
 // takes 20.1 us in three ranges, 21.8 in one, which 4 TB/s would choose), at 4 TB/s for the head's two beside one another (at 8 a
 // ragged batch of 7655 x 256 x 10007, half of its rows not counted, takes 167 us instead of 137).
+// Two accumulators fetch A half as often, which counts where the power limit sets the clock: a head of 16384 x 512 x 8192 takes
+// 500 us instead of 507 over seconds, 429 instead of 434 before the limit acts.
 struct Cut {
     uint32_t accs, splits;
 };
@@ -116,7 +118,8 @@ Cut cut_of(size_t M, size_t N, size_t K, uint32_t pairs, bool two) {
         for (uint32_t splits = 1; splits <= std::min<size_t>(16, std::max<size_t>(1, blocks / 4)); ++splits) {
             const double rounds = (double)ceil_div(tiles * splits, pairs);
             const double epilogue = accs == 2 ? 10.0 : 1.0;
-            double cost = rounds * (ceil_div(blocks, splits) * accs + epilogue) + 4.0;
+            const double k_blocks = (double)ceil_div(blocks, splits) * (accs == 2 ? 1.9 : 1.0);
+            double cost = rounds * (k_blocks + epilogue) + 4.0;
             if (splits > 1) cost += (2.0 * splits + 1.0) * M * N * 4.0 / (two ? 4e6 : 8e6) / 0.3 + 8.0;
             if (cost < least) {
                 least = cost;
