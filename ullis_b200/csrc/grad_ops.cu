@@ -799,9 +799,9 @@ tape_exponent_max_kernel(const uint8_t* __restrict__ exponents, uint32_t rows, u
 // What the codes stand for as a 16-bit operand [rows, Cp].  bf16 holds every value (8 significant bits, the range of f32).  FP16
 // does not: there each block of 32 channels is shifted by a power of two common to all rows, so that its largest exponent comes to 8
 // (127 * 2^8 = 32 512), and the column's sums are shifted back.  What is lost lies 2^32 below the block's largest value.
-// A thread has a chunk of eight columns and OPERAND_ROWS rows in turn.  VEC: as in tape.cuh.  16384 x 512 in bf16 9.1 us (25 MB), 7655
-// x 2048 in FP16 12.8 (47 MB), its largest exponents 6.7.
-constexpr uint32_t OPERAND_ROWS = 4;
+// A thread has a chunk of eight columns and OPERAND_ROWS rows in turn.  VEC: as in tape.cuh.  16384 x 512 in bf16 7.4 us (25 MB), 7655
+// x 2048 in FP16 9.7 (47 MB), its largest exponents 6.7; with four rows 9.1 and 12.8, with sixteen a whole call is 2 % slower again.
+constexpr uint32_t OPERAND_ROWS = 8;
 template <bool BF, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 tape_operand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t C, uint32_t Cp,
@@ -823,8 +823,7 @@ tape_operand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict
     float v[OPERAND_ROWS][8];
 #pragma unroll
     for (uint32_t k = 0; k < OPERAND_ROWS; ++k) {
-        const size_t row = row0 + k;
-        if (row >= rows) break;
+        const size_t row = min(row0 + k, (size_t)rows - 1);   // (no branch between the loads)
         uint32_t byte = exponents[row * blocks + b];
         if (!BF && byte != tape::NOT_FINITE)   // 2^(e - largest + 8)
             byte = most == tape::NOT_FINITE ? 127u : (uint32_t)max((int)byte - (int)most + 8 + 127, 1);
