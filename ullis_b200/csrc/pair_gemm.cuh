@@ -21,11 +21,11 @@
 //   SUM    acc in f32: the tensor cores cut off what falls below the accumulator's last bit (measured: K = 16384 1.9e-5 off in
 //          norm, 1.1e-4 where all terms have one sign; K = 512 6e-7), so every 512 terms the accumulator moves to registers
 //          and is added there with rounding
-// Measured at 16384 x 512 x 8192 in FP16 (137 GFLOP each, cold caches): LSE 105 us, GRAD 125, the two STOREs 99 and 107; SUM at
-// 512 x 16384 x 2048 in bf16 35 us for 34 GFLOP.  The tensor pipe is busy 66, 55, 68 and 48 % of the time.  The products of
-// such a call take the pipe 113 thousand cycles, a loop without an epilogue 148 (the same without the loads of A: neither L2 nor the
-// ring bounds it), LSE 174, GRAD 211: there it is the exp and the sums of the 16 epilogue warps, 36 and 45 % of the issue slots; a
-// STORE has 64 tiles for 74 pairs.
+// Measured at 16384 x 512 x 8192 in FP16 (137 GFLOP each, cold caches): LSE 106 us, GRAD 125, STORE 105 (one accumulator at a time)
+// and 95 (two); SUM at 2048 x 16384 -> 512 in bf16 35 us for 34 GFLOP.  The tensor pipe is busy 65, 54, 69, 70 and 48 % of the
+// time.  The products of such a call take the pipe 113 thousand cycles, a loop without an epilogue 148 (the same without the loads of
+// A: neither L2 nor the ring bounds it), LSE 177, GRAD 211: there it is the exp and the sums of the 16 epilogue warps, 36 and 45 %
+// of the issue slots; a STORE has 64 tiles for 74 pairs.
 // Every wait is bounded and reports through the status words, as in tc_gemm_ws2.cuh.
 #pragma once
 #include <cuda_bf16.h>
