@@ -364,6 +364,39 @@ def test_graphs_streams_and_the_same_result_every_time(cuda_rt):
     cuda_rt.synchronize()
 
 
+@pytest.mark.parametrize("rows,vocab", [(96, 700), (2600, 3000)])
+def test_a_graph_replayed_with_other_inputs(cuda_rt, rows, vocab):
+    """How many rows count, and which, is known on the device only; and whatever lies in the workspace, nothing of it shows."""
+    first, second = (inputs(rows, rows // 2, 72, vocab, "bf16", True, ignored, seed=k) for k, ignored in ((1, 0.8), (2, 0.1)))
+    want = [call(cuda_rt, s) for s in (first, second)]
+    held = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in first.items()}
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = call(cuda_rt, held)
+        dirt = torch.full((1 << 28,), 0xFF, dtype=torch.uint8, device="cuda")   # NaN in f32 and 16 bits, over what the call gave back
+    for k in (0, 1, 0, 1, 1):
+        for name, v in (first, second)[k].items():
+            if isinstance(v, torch.Tensor):
+                held[name].copy_(v)
+        g.replay()
+        for a, b in zip(got, want[k]):
+            assert torch.equal(a, b)
+    del dirt
+
+
+@pytest.mark.parametrize("rows,vocab", [(5, 40), (96, 700), (2600, 3000), (9000, 16400)])
+def test_nothing_depends_on_what_the_workspace_held(cuda_rt, rows, vocab):
+    s = inputs(rows, rows, 72, vocab, "f16", True, 0.3, seed=9)
+    want = call(cuda_rt, s)
+    for byte in (0xFF, 0x7B):     # NaN; large numbers
+        torch.cuda.empty_cache()
+        dirt = torch.full((1 << 30,), byte, dtype=torch.uint8, device="cuda")
+        del dirt                  # the next blocks come out of it
+        for a, b in zip(call(cuda_rt, s), want):
+            assert torch.equal(a, b)
+
+
 def test_refusals_of_the_library(cuda_rt):
     s = inputs(64, 64, 64, 300, "f16", True)
     with pytest.raises(cuda.UllisCudaError) as e:

@@ -104,6 +104,19 @@ def test_zero_rows_and_leading_dimensions(cuda_rt):
     assert torch.equal(cuda_rt.tape_weight_grad(tape, gy), cuda_rt.tape_weight_grad(flat, gy.reshape(150, 24)))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", [(70, 40, 30), (5000, 100, 300), (20000, 512, 512)], ids=str)
+def test_nothing_depends_on_what_the_workspace_held(cuda_rt, case, dtype):
+    rows, i, o = case
+    tape, gy = tape_of(rows, i, 1), torch.randn(rows, o, device="cuda").to(TYPES[dtype])
+    want = cuda_rt.tape_weight_grad(tape, gy)
+    for byte in (0xFF, 0x7B):     # NaN; large numbers
+        torch.cuda.empty_cache()
+        dirt = torch.full((1 << 29,), byte, dtype=torch.uint8, device="cuda")
+        del dirt                  # the next blocks come out of it
+        assert torch.equal(cuda_rt.tape_weight_grad(tape, gy), want)
+
+
 def test_norm_linear_and_head_together(cuda_rt):
     """Norm, linear and head of a small model from the 8-bit tape: every gradient as autograd gives it in 64 bits at the values that
     the tape keeps."""
