@@ -1,5 +1,7 @@
 """CudaRuntime.tape_weight_grad against the product in 64 bits.  Products of 16-bit numbers and codes are exact in f32; within 1024
 rows the tensor cores cut off each addition (2^-23 per term), everything else is added with rounding (2^-24)."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -90,6 +92,29 @@ def test_rows_with_gaps_and_odd_starts(cuda_rt, offset, stride):
     got = cuda_rt.tape_weight_grad(tape, gy)
     assert torch.equal(got, cuda_rt.tape_weight_grad(tape, gy.contiguous()))
     check(got, gy, tape)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("inputs", [64, 63])
+@pytest.mark.parametrize("rows,ranges", [(200, False), (20000, True)])
+def test_an_output_that_starts_anywhere(cuda_rt, rows, ranges, inputs, dtype):
+    """g at every offset into a buffer (the entry point asks for the alignment of its elements), with one range of K, which the product
+    writes itself, and with several, whose sum is."""
+    out = 40
+    tape, gy = tape_of(rows, inputs, 1), torch.randn(rows, out, device="cuda").to(TYPES[dtype])
+    want = cuda_rt.tape_weight_grad(tape, gy)
+    size = C.c_size_t(0)
+    assert cuda_rt._lib.ullis_cuda_tape_weight_grad_workspace(cuda_rt._h, rows, inputs, out, C.byref(size)) == cuda.OK
+    work = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+    for offset in (0, 1, 2, 3):
+        g = torch.full((out * inputs + 8,), 7.0, device="cuda")
+        before = cuda_rt.launch_count
+        assert cuda_rt._lib.ullis_cuda_tape_weight_grad(
+            cuda_rt._h, torch.cuda.current_stream().cuda_stream, {"f16": 1, "bf16": 2}[dtype], tape[0].data_ptr(), tape[1].data_ptr(),
+            gy.data_ptr(), out, rows, inputs, out, g.data_ptr() + 4 * offset, work.data_ptr(), size.value) == cuda.OK
+        assert cuda_rt.launch_count - before == (3 if dtype == "f16" else 2) + ranges
+        assert torch.equal(g[offset:offset + out * inputs].view(out, inputs), want)
+        assert (g[:offset] == 7.0).all() and (g[offset + out * inputs:] == 7.0).all()
 
 
 def test_zero_rows_and_leading_dimensions(cuda_rt):

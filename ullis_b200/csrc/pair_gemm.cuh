@@ -295,6 +295,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile ui
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Whether two columns of every row of an f32 array of `columns` lie on 8 bytes: a caller's array is aligned to its elements only.
+__device__ __forceinline__ bool rows_of_pairs(const void* array, uint32_t columns) {
+    return (columns & 1) == 0 && (reinterpret_cast<uintptr_t>(array) & 7) == 0;
+}
+
 // Scale and bias (FP16, two lanes' worth: columns lane and 32 + lane) of 64 columns from n0 on, on their way while the tile before
 // is worked on; and as the constants that the epilogue reads: both times log2 e.  Columns past N have a probability of 0.
 struct Columns {
@@ -708,7 +713,6 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             leave();
         } else if constexpr (EPI == STORE) {
             const float alpha = p.factor ? *p.factor : 1.0f;
-            const bool pairs_ok = (p.N & 1) == 0;   // two columns of an f32 row lie on 8 bytes
             const bool wide = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
             uint16_t* out = static_cast<uint16_t*>(p.out);
             while (work.next()) {
@@ -731,6 +735,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
                     const auto f32_rows = [&](float* at, const int32_t* rows, bool read, bool write, float times) {
+                        const bool pairs_ok = rows_of_pairs(at, p.N);
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const uint32_t row = m0 + h * 16 + r0 + i * 8;
@@ -784,7 +789,6 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             }
         } else {
             static_assert(EPI != SUM || ACCS == 1, "");
-            const bool pairs_ok = (p.N & 1) == 0;
             bool ok = true;
             while (ok && work.next()) {
                 float v[64];
@@ -811,6 +815,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 for (int i = 0; i < 2; ++i)
                     if (p.col_factor && n0 + i * 32 < p.N) f[i] = p.col_factor[n0 / 32 + i];
                 float* out = p.splits > 1 ? p.partial + (size_t)work.split * p.M * p.N : static_cast<float*>(p.out);
+                const bool pairs_ok = rows_of_pairs(out, p.N);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t row = m0 + r0 + i * 8;
