@@ -74,6 +74,99 @@ def test_blocks_of_every_exponent(cuda_rt, dtype):
     assert ((got - want).abs() <= U * 1100 * sizes + 2.0 ** -149 * 512).all()
 
 
+def close(got, gy, tape):
+    """512 terms at a time with what the tensor cores cut off; then those sums with rounding, at most two for 512 rows (gy in two
+    parts, the smaller one below 2^-8 of the other: 1 + 2^-7 times the sizes)."""
+    rows = gy.shape[0]
+    want, sizes = gy.double().t() @ values(*tape), gy.double().abs().t() @ values(*tape).abs()
+    off = (1 + 2.0 ** -7) * U * (2 * min(rows, 512) + 32 + 2 * rows / 512) * sizes + 2.0 ** -149 * rows
+    bad = ~((got.double() - want).abs() <= off)
+    assert not bad.any(), (int(bad.sum()), got[bad][:4].tolist(), want[bad][:4].tolist(), off[bad][:4].tolist())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", [(300, 96, 72), (300, 70, 7), (2100, 264, 300), (20000, 64, 8)], ids=str)
+def test_a_row_far_above_the_others(cuda_rt, case, dtype):
+    """What a row of very large values holds has no effect where its gy is 0, and no more than its own where gy is not."""
+    rows, i, o = case
+    g = torch.Generator("cuda").manual_seed(4)
+    codes, exponents = tape_of(rows, i, 2)
+    gy = (1e-2 * torch.randn(rows, o, generator=g, device="cuda")).to(TYPES[dtype])
+    for binades, at in ((33, 0), (45, rows - 1), (70, rows // 2), (100, 17)):
+        high = exponents.clone()
+        high[at] += binades
+        masked = gy.clone()
+        masked[at] = 0.0
+        got = cuda_rt.tape_weight_grad((codes, high), masked)
+        close(got, masked, (codes, high))
+        assert got.abs().min() > 0.0
+        masked[at, ::3] = 6e-5                   # the other outputs still have nothing of that row
+        close(cuda_rt.tape_weight_grad((codes, high), masked), masked, (codes, high))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_exponents_all_over(cuda_rt, dtype):
+    """Every exponent of a tape in one block, beside a block that 16 bits hold and one that lies at the range's end."""
+    g = torch.Generator("cuda").manual_seed(6)
+    codes = torch.randint(-127, 128, (1500, 100), generator=g, device="cuda").to(torch.int8)
+    exponents = torch.randint(1, 249, (1500, 4), generator=g, device="cuda").to(torch.uint8)
+    exponents[:, 1] = 130
+    exponents[:, 3] = torch.where(exponents[:, 3] > 120, 248, 216).to(torch.uint8)
+    gy = (2.0 ** -10 * torch.randn(1500, 300, generator=g, device="cuda")).to(TYPES[dtype])
+    close(cuda_rt.tape_weight_grad((codes, exponents), gy), gy, (codes, exponents))
+    # rows of nothing, whose exponent is the lowest, take no block out of 16 bits
+    codes[::2], exponents[::2], exponents[1::2] = 0, 1, 130
+    got = cuda_rt.tape_weight_grad((codes, exponents), gy)
+    close(got, gy, (codes, exponents))
+    exponents[::2] = 130
+    assert torch.equal(got, cuda_rt.tape_weight_grad((codes, exponents), gy))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset,stride", [(0, 136), (3, 136), (0, 131)])
+def test_far_values_in_a_few_blocks(cuda_rt, offset, stride, dtype):
+    """Some stretches of some columns need more than FP16, their neighbours do not; and gy may have to be copied."""
+    codes, exponents = tape_of(3000, 600, 3)
+    exponents[1100, 2] += 60                     # rows 1024 .. 1535, columns 0 .. 255
+    exponents[2999, 18] += 50                    # the last rows, the last columns
+    base = torch.full((3000 * stride + offset + 130,), float("nan"), device="cuda").to(TYPES[dtype])
+    gy = base.as_strided((3000, 130), (stride, 1), offset)
+    gy.copy_(torch.randn(3000, 130, device="cuda"))
+    gy[1100] = 0.0
+    gy[2999, ::2] = 0.0
+    got = cuda_rt.tape_weight_grad((codes, exponents), gy)
+    close(got, gy, (codes, exponents))
+    assert torch.equal(got, cuda_rt.tape_weight_grad((codes, exponents), gy.contiguous()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_codes_of_the_lowest_exponent(cuda_rt, dtype):
+    """A block of zeros has it too: what is not 0 there counts where nothing else does."""
+    codes, exponents = tape_of(100, 96, 8)
+    gy = torch.zeros(100, 40, device="cuda").to(TYPES[dtype])
+    exponents[41], gy[41] = 1, 1000.0
+    codes[7], exponents[7] = 0, 1
+    got = cuda_rt.tape_weight_grad((codes, exponents), gy)
+    close(got, gy, (codes, exponents))
+    assert torch.equal(got != 0, (codes[41] != 0).expand(40, 96))
+
+
+def test_infinite_gradients_with_far_values(cuda_rt):
+    """An infinity in gy is one in every product it is in, however gy is held: 0 times it is NaN, anything else infinite."""
+    for high in (0, 60):
+        codes, exponents = tape_of(200, 64, 8)
+        codes[9, :4] = torch.tensor([0, 1, -1, 127], dtype=torch.int8)
+        exponents[100] += high
+        gy = (1e-2 * torch.randn(200, 8, device="cuda")).half()
+        gy[9, 2], gy[9, 3] = float("inf"), -float("inf")
+        got = cuda_rt.tape_weight_grad((codes, exponents), gy)
+        inf = float("inf")
+        assert torch.isnan(got[2:4, 0]).all()
+        assert got[2, 1:4].tolist() == [inf, -inf, inf] and got[3, 1:4].tolist() == [-inf, inf, -inf]
+        keep = torch.tensor([0, 1, 4, 5, 6, 7], device="cuda")
+        close(got[keep], gy[:, keep], (codes, exponents))
+
+
 def test_a_block_that_is_not_finite(cuda_rt):
     codes, exponents = tape_of(100, 96, 5)
     exponents[17, 1] = 255
@@ -112,7 +205,7 @@ def test_an_output_that_starts_anywhere(cuda_rt, rows, ranges, inputs, dtype):
         assert cuda_rt._lib.ullis_cuda_tape_weight_grad(
             cuda_rt._h, torch.cuda.current_stream().cuda_stream, {"f16": 1, "bf16": 2}[dtype], tape[0].data_ptr(), tape[1].data_ptr(),
             gy.data_ptr(), out, rows, inputs, out, g.data_ptr() + 4 * offset, work.data_ptr(), size.value) == cuda.OK
-        assert cuda_rt.launch_count - before == (3 if dtype == "f16" else 2) + ranges
+        assert cuda_rt.launch_count - before == 2 + ranges          # operand, product, and the sum
         assert torch.equal(g[offset:offset + out * inputs].view(out, inputs), want)
         assert (g[:offset] == 7.0).all() and (g[offset + out * inputs:] == 7.0).all()
 

@@ -106,6 +106,7 @@ void launch(const Stream& s, const char* what, const Operand& a, const Operand& 
 // ragged batch of 7655 x 256 x 10007, half of its rows not counted, takes 167 us instead of 137).
 // Two accumulators fetch A half as often, which counts where the power limit sets the clock: a head of 16384 x 512 x 8192 takes
 // 500 us instead of 507 over seconds, 429 instead of 434 before the limit acts.
+// (two: a product of the head, else a SUM, whose ranges are whole stretches of K)
 struct Cut {
     uint32_t accs, splits;
 };
@@ -118,7 +119,8 @@ Cut cut_of(size_t M, size_t N, size_t K, uint32_t pairs, bool two) {
         for (uint32_t splits = 1; splits <= std::min<size_t>(16, std::max<size_t>(1, blocks / 4)); ++splits) {
             const double rounds = (double)ceil_div(tiles * splits, pairs);
             const double epilogue = accs == 2 ? 10.0 : 1.0;
-            const double k_blocks = (double)ceil_div(blocks, splits) * (accs == 2 ? 1.9 : 1.0);
+            const size_t most = two ? ceil_div(blocks, splits) : std::min(blocks, ceil_div(ceil_div(blocks, pg::SUM_BLOCKS), splits) * pg::SUM_BLOCKS);
+            const double k_blocks = (double)most * (accs == 2 ? 1.9 : 1.0);
             double cost = rounds * (k_blocks + epilogue) + 4.0;
             if (splits > 1) cost += (2.0 * splits + 1.0) * M * N * 4.0 / (two ? 4e6 : 8e6) / 0.3 + 8.0;
             if (cost < least) {
@@ -769,73 +771,173 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
 // ------------------------------------------------------------------------------------------------ weight gradient from the tape
 namespace {
 
-// The largest exponent byte of each block of 32 channels, over TOP_SLICES slices of the rows: top [blocks][slices].  A CTA has 32
-// blocks of a slice.  WIDE: a thread reads four blocks' bytes in one word, and 32 rows are on their way at a time instead of 8.
-constexpr uint32_t TOP_SLICES = 32;
-template <bool WIDE>
-__global__ void __launch_bounds__(THREADS)
-tape_exponent_max_kernel(const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t blocks, uint8_t* __restrict__ top) {
-    chain_entry();
-    constexpr uint32_t LANES = WIDE ? 8 : 32, STEP = THREADS / LANES;
-    const uint32_t slice = blockIdx.y, lane = threadIdx.x % LANES, b = blockIdx.x * 32 + lane * (32 / LANES);
-    const uint32_t first = (uint32_t)((uint64_t)slice * rows / TOP_SLICES), last = (uint32_t)((uint64_t)(slice + 1) * rows / TOP_SLICES);
-    __shared__ uint32_t tops[THREADS];
-    uint32_t most = 0;
-    if (b < blocks) {
-#pragma unroll 8
-        for (uint32_t r = first + threadIdx.x / LANES; r < last; r += STEP) {
-            const uint8_t* at = exponents + (size_t)r * blocks + b;
-            most = __vmaxu4(most, WIDE ? *reinterpret_cast<const uint32_t*>(at) : (uint32_t)*at);
+// What the codes stand for as a 16-bit operand [rows, Cp].  A thread has a chunk of eight columns and OPERAND_ROWS rows.  VEC: as in
+// tape.cuh.
+constexpr int OPERAND_ROWS = 8;
+template <bool VEC>
+struct OperandRows {
+    uint32_t codes[OPERAND_ROWS][2], bytes[OPERAND_ROWS];
+    __device__ __forceinline__ void load(const uint8_t* __restrict__ from, const uint8_t* __restrict__ exponents, size_t row0, uint32_t rows,
+                                         uint32_t c, uint32_t C) {
+        const uint32_t blocks = (C + 31) / 32, b = c / 32;
+#pragma unroll
+        for (int k = 0; k < OPERAND_ROWS; ++k) {
+            const size_t row = min(row0 + k, (size_t)rows - 1);   // (no branch between the loads)
+            bytes[k] = exponents[row * blocks + b];
+            tape::raw_codes<VEC, 8>(from + row * C, c, C, codes[k]);
         }
     }
-    tops[threadIdx.x] = most;
-    __syncthreads();
-    if (threadIdx.x >= LANES || b >= blocks) return;
+};
+template <bool BF>
+__device__ __forceinline__ void store_operand(uint16_t* to, const uint32_t (&codes)[2], uint32_t byte) {
+    float v[8];
+    tape::values_of(codes, tape::power(byte), v);
+    uint32_t w[4];
 #pragma unroll
-    for (uint32_t k = 1; k < STEP; ++k) most = __vmaxu4(most, tops[threadIdx.x + LANES * k]);
-    for (uint32_t k = 0; k < 32 / LANES; ++k) top[(b + k) * TOP_SLICES + slice] = (uint8_t)(most >> 8 * k);
+    for (int e = 0; e < 4; ++e) w[e] = pg::pack16<BF>(v[2 * e], v[2 * e + 1]);
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// What the codes stand for as a 16-bit operand [rows, Cp].  bf16 holds every value (8 significant bits, the range of f32).  FP16
-// does not: there each block of 32 channels is shifted by a power of two common to all rows, so that its largest exponent comes to 8
-// (127 * 2^8 = 32 512), and the column's sums are shifted back.  What is lost lies 2^32 below the block's largest value.
-// A thread has a chunk of eight columns and OPERAND_ROWS rows in turn.  VEC: as in tape.cuh.  16384 x 512 in bf16 7.4 us (25 MB), 7655
-// x 2048 in FP16 9.7 (47 MB), its largest exponents 6.7; with four rows 9.1 and 12.8, with sixteen a whole call is 2 % slower again.
-constexpr uint32_t OPERAND_ROWS = 8;
-template <bool BF, bool VEC>
+// bf16 holds every value: 8 significant bits, the range of f32.  16384 x 512: 5.8 us (25 MB).
+template <bool VEC>
 __global__ void __launch_bounds__(THREADS)
-tape_operand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t C, uint32_t Cp,
-                    const uint8_t* __restrict__ top, uint16_t* __restrict__ out, float* __restrict__ col_factor) {
+tape_operand_bf16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t C, uint32_t Cp,
+                         uint16_t* __restrict__ out) {
     chain_entry();
-    const uint32_t chunks = Cp / 8, blocks = (C + 31) / 32;
+    const uint32_t chunks = Cp / 8;
     const size_t item = (size_t)blockIdx.x * THREADS + threadIdx.x;
     const size_t group = item >> 32 ? item / chunks : (uint32_t)item / chunks, row0 = group * OPERAND_ROWS;
     if (row0 >= rows) return;
-    const uint32_t c = (uint32_t)(item - group * chunks) * 8, b = c / 32;
-    uint32_t most = 0;
-    if (!BF) {
-        const uint4 u = reinterpret_cast<const uint4*>(top + b * TOP_SLICES)[0], w = reinterpret_cast<const uint4*>(top + b * TOP_SLICES)[1];
-        most = __vmaxu4(__vmaxu4(__vmaxu4(u.x, u.y), __vmaxu4(u.z, u.w)), __vmaxu4(__vmaxu4(w.x, w.y), __vmaxu4(w.z, w.w)));
-        most = __vmaxu4(most, most >> 16);
-        most = max(most & 0xff, most >> 8 & 0xff);
-        if (row0 == 0 && c % 32 == 0) col_factor[b] = most == tape::NOT_FINITE ? 1.0f : exp2f((float)((int)most - 127 - 8));
-    }
-    float v[OPERAND_ROWS][8];
+    const uint32_t c = (uint32_t)(item - group * chunks) * 8;
+    OperandRows<VEC> o;
+    o.load(codes, exponents, row0, rows, c, C);
 #pragma unroll
-    for (uint32_t k = 0; k < OPERAND_ROWS; ++k) {
-        const size_t row = min(row0 + k, (size_t)rows - 1);   // (no branch between the loads)
-        uint32_t byte = exponents[row * blocks + b];
-        if (!BF && byte != tape::NOT_FINITE)   // 2^(e - largest + 8)
-            byte = most == tape::NOT_FINITE ? 127u : (uint32_t)max((int)byte - (int)most + 8 + 127, 1);
-        tape::load_codes<VEC>(codes + row * C, tape::power(byte), c, C, v[k]);
-    }
+    for (int k = 0; k < OPERAND_ROWS; ++k)
+        if (row0 + k < rows) store_operand<true>(out + (row0 + k) * Cp + c, o.codes[k], o.bytes[k]);
+}
+
+// FP16 does not: there the codes of 32 channels and a stretch of 512 rows, whose sums SUM adds up with rounding anyway, are shifted by a
+// power of two in common, so that their largest exponent comes to 8 (127 * 2^8 = 32 512), and the sums are shifted back.  FP16's last
+// bit, 2^-24, is then that of a code whose exponent lies 32 below the largest.  Where a smaller one turns up (a row of very large values is
+// enough, a padded one whose gy is 0 too), the 256 columns that a product's tile has of the stretch go to bf16 after all, and gy's rows
+// into the sum of two bf16 matrices, which 11 bits always are: the same products, exact again, with twice the operations.
+// A CTA has 64 rows of 256 columns and looks at the exponents of the whole stretch (4 KB, in L2).  BYTES8: a row's eight start on 8 bytes.
+// 7655 x 2048: 12.2 us (47 MB); the largest exponents of all rows by a kernel before it took 6.5 and 9.4, and held 32 binades.
+constexpr uint32_t STRETCH = pg::SUM_BLOCKS * pg::BK, F16_ROWS = THREADS / 32 * OPERAND_ROWS;
+static_assert(STRETCH % F16_ROWS == 0 && STRETCH / 32 <= 32 && THREADS == 8 * 32 && pg::BN == 256, "");
+
+struct GyRows {   // gy [rows, O] as two bf16 matrices side by side, [rows, 2 Op]
+    const uint16_t* gy;
+    size_t stride;
+    uint32_t O, Op;
+    uint16_t* out;
+    // the nearest bf16 number, and what is left (at most 3 bits; 0 where that is not finite)
+    __device__ __noinline__ void in_parts(size_t first, size_t last) const {
+        const uint32_t chunks = Op / 8;
+        const size_t items = (last - first) * chunks;
+        for (size_t i = threadIdx.x; i < items; i += THREADS) {
+            const size_t row = first + i / chunks;
+            const uint32_t c = (uint32_t)(i % chunks) * 8;
+            uint32_t w[2][4];
 #pragma unroll
-    for (uint32_t k = 0; k < OPERAND_ROWS; ++k) {
+            for (int e = 0; e < 4; ++e) {
+                float high[2], low[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float v = c + 2 * e + k < O ? __half2float(__ushort_as_half(gy[row * stride + c + 2 * e + k])) : 0.0f;
+                    high[k] = __bfloat162float(__float2bfloat16_rn(v));
+                    low[k] = isfinite(v) ? v - high[k] : 0.0f;
+                }
+                w[0][e] = pg::pack16<true>(high[0], high[1]);
+                w[1][e] = pg::pack16<true>(low[0], low[1]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                *reinterpret_cast<uint4*>(out + (row * 2 + k) * Op + c) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+        }
+    }
+};
+template <bool VEC, bool BYTES8>
+__global__ void __launch_bounds__(THREADS)
+tape_operand_f16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t C, uint32_t Cp,
+                        uint16_t* __restrict__ out, float* __restrict__ col_factor, uint32_t* __restrict__ parts, const GyRows gy) {
+    chain_entry();
+    const uint32_t tiles = (C + pg::BN - 1) / pg::BN, blocks = (C + 31) / 32;
+    const uint32_t tile = blockIdx.x % tiles, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b0 = tile * 8;
+    const size_t first = (size_t)(blockIdx.x / tiles) * F16_ROWS, row0 = first + warp * OPERAND_ROWS;
+    const size_t stretch = first / STRETCH, end = min((stretch + 1) * STRETCH, (size_t)rows);
+    const uint32_t c = tile * pg::BN + lane * 8;
+    const bool mine = row0 < rows && c < Cp;
+    OperandRows<VEC> o;
+    if (mine) o.load(codes, exponents, row0, rows, c, C);
+    // A warp for each of the tile's eight blocks: the largest exponent byte of the stretch, and the smallest of those whose codes are not
+    // all 0 (255: none).  A block of zeros has the lowest byte there is, 1: only where that turns up are codes read.
+    __shared__ __align__(8) uint8_t bytes[STRETCH][8];   // 0: no row or no block there
+    __shared__ uint32_t range[2][8];
+#pragma unroll
+    for (uint32_t r = threadIdx.x; r < STRETCH; r += THREADS) {
+        const size_t row = stretch * STRETCH + r;
+        const uint8_t* at = exponents + row * blocks + b0;
+        uint2 e = make_uint2(0u, 0u);
+        if (BYTES8) {
+            if (row < end) e = *reinterpret_cast<const uint2*>(at);
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+                if (row < end && b0 + k < blocks) (k < 4 ? e.x : e.y) |= (uint32_t)at[k] << 8 * (k & 3);
+        }
+        *reinterpret_cast<uint2*>(bytes[r]) = e;
+    }
+    __syncthreads();
+    uint32_t largest = 0, smallest = 255, ones = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < STRETCH / 32; ++i) {
+        const uint32_t e = bytes[i * 32 + lane][warp];
+        largest = max(largest, e);
+        smallest = min(smallest, e > 1 ? e : 255u);
+        ones |= (uint32_t)(e == 1) << i;
+    }
+    while (ones) {
+        const size_t row = stretch * STRETCH + (__ffs(ones) - 1) * 32 + lane;
+        ones &= ones - 1;
+        uint32_t any = 0;
+        for (uint32_t i = 0; i < 4; ++i) {
+            uint32_t w[2];
+            tape::raw_codes<VEC, 8>(codes + row * C, (b0 + warp) * 32 + i * 8, C, w);
+            any |= w[0] | w[1];
+        }
+        if (any) smallest = 1;
+    }
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    smallest = __reduce_min_sync(0xffffffffu, smallest);
+    if (lane == 0) {
+        range[0][warp] = largest;
+        range[1][warp] = smallest;
+    }
+    __syncthreads();
+    largest = range[0][lane & 7];   // of block b0 + lane % 8
+    smallest = range[1][lane & 7];
+    const bool exact = __any_sync(0xffffffffu, largest != tape::NOT_FINITE && smallest + 32 < largest);   // (the same for all warps)
+    if (first % STRETCH == 0 && threadIdx.x < 8) {
+        if (b0 + lane < blocks)
+            col_factor[stretch * blocks + b0 + lane] = exact || largest == tape::NOT_FINITE ? 1.0f : exp2f((float)((int)largest - 127 - 8));
+        if (lane == 0) parts[stretch * tiles + tile] = exact;
+    }
+    if (exact) gy.in_parts(first, min(first + F16_ROWS, (size_t)rows));
+    const uint32_t own = __shfl_sync(0xffffffffu, largest, lane >> 2);   // the largest of this thread's block
+    if (!mine) return;
+#pragma unroll
+    for (int k = 0; k < OPERAND_ROWS; ++k) {
         if (row0 + k >= rows) break;
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = pg::pack16<BF>(v[k][2 * e], v[k][2 * e + 1]);
-        *reinterpret_cast<uint4*>(out + (row0 + k) * Cp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        uint16_t* to = out + (row0 + k) * Cp + c;
+        uint32_t byte = o.bytes[k];
+        if (exact) {
+            store_operand<true>(to, o.codes[k], byte);
+        } else {
+            if (byte != tape::NOT_FINITE)   // 2^(e - largest + 8)
+                byte = own == tape::NOT_FINITE ? 127u : (uint32_t)max((int)byte - (int)own + 8 + 127, 1);
+            store_operand<false>(to, o.codes[k], byte);
+        }
     }
 }
 
@@ -858,7 +960,7 @@ rows16_kernel(const uint16_t* __restrict__ x, size_t stride, uint32_t rows, uint
 struct WeightPlan {
     size_t ip, op;
     Cut cut;
-    size_t x16, gy16, top, col_factor, partial, bytes;
+    size_t x16, gy16, gy_parts, col_factor, parts, partial, bytes;
 };
 WeightPlan weight_plan(const ullis_cuda_runtime* rt, size_t rows, size_t in, size_t out) {
     WeightPlan p{};
@@ -868,8 +970,9 @@ WeightPlan weight_plan(const ullis_cuda_runtime* rt, size_t rows, size_t in, siz
     Parts at;
     p.x16 = at.add(rows * p.ip * 2);
     p.gy16 = at.add(rows * p.op * 2);
-    p.top = at.add(TOP_SLICES * tape::blocks_of(in));
-    p.col_factor = at.add(tape::blocks_of(in) * 4);
+    p.gy_parts = at.add(rows * 2 * p.op * 2);
+    p.col_factor = at.add(ceil_div(rows, STRETCH) * tape::blocks_of(in) * 4);
+    p.parts = at.add(ceil_div(rows, STRETCH) * ceil_div(in, pg::BN) * 4);
     p.partial = at.add(partial_bytes(out, in, p.cut));
     p.bytes = at.bytes;
     return p;
@@ -887,24 +990,28 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const bool bf16 = dtype == BF16;
     uint16_t* x16 = reinterpret_cast<uint16_t*>(ws + p.x16);
-    uint8_t* top = ws + p.top;
+    uint16_t* gy16 = reinterpret_cast<uint16_t*>(ws + p.gy16);
     float* col_factor = reinterpret_cast<float*>(ws + p.col_factor);
-    const uint32_t blocks = (uint32_t)tape::blocks_of(in);
-    const unsigned grid = (unsigned)ceil_div(ceil_div(rows, OPERAND_ROWS) * (p.ip / 8), THREADS);
-    const bool vec = in % 8 == 0 && aligned(codes, 8);
-    const bool wide = blocks % 4 == 0 && aligned(exponents, 4);
-    if (!bf16)
-        s.chain("tape_exponent_max", wide ? tape_exponent_max_kernel<true> : tape_exponent_max_kernel<false>, dim3((blocks + 31) / 32, TOP_SLICES), THREADS, 0, exponents, (uint32_t)rows, blocks, top);
-    const auto operand = bf16 ? (vec ? tape_operand_kernel<true, true> : tape_operand_kernel<true, false>)
-                              : (vec ? tape_operand_kernel<false, true> : tape_operand_kernel<false, false>);
-    s.chain("tape_operand", operand, grid, THREADS, 0, codes, exponents, (uint32_t)rows, (uint32_t)in, (uint32_t)p.ip,
-            static_cast<const uint8_t*>(top), x16, col_factor);
+    uint32_t* parts = reinterpret_cast<uint32_t*>(ws + p.parts);
     Operand a{gy.data, rows, out, gy.stride, true};
+    uint16_t* gy_parts = reinterpret_cast<uint16_t*>(ws + p.gy_parts);
     if (!aligned(gy.data, 16) || gy.stride % 8) {
-        uint16_t* gy16 = reinterpret_cast<uint16_t*>(ws + p.gy16);
         s.chain("rows16", rows16_kernel, (unsigned)ceil_div(rows * (p.op / 8), THREADS), THREADS, 0, static_cast<const uint16_t*>(gy.data),
                 gy.stride, (uint32_t)rows, (uint32_t)out, (uint32_t)p.op, gy16);
         a = Operand{gy16, rows, out, p.op, true};
+    }
+    const bool vec = in % 8 == 0 && aligned(codes, 8);
+    if (bf16) {
+        s.chain("tape_operand", vec ? tape_operand_bf16_kernel<true> : tape_operand_bf16_kernel<false>,
+                (unsigned)ceil_div(ceil_div(rows, OPERAND_ROWS) * (p.ip / 8), THREADS), THREADS, 0, codes, exponents, (uint32_t)rows, (uint32_t)in,
+                (uint32_t)p.ip, x16);
+    } else {
+        const bool bytes8 = tape::blocks_of(in) % 8 == 0 && aligned(exponents, 8);
+        const auto operand = vec ? (bytes8 ? tape_operand_f16_kernel<true, true> : tape_operand_f16_kernel<true, false>)
+                                 : (bytes8 ? tape_operand_f16_kernel<false, true> : tape_operand_f16_kernel<false, false>);
+        s.chain("tape_operand", operand, (unsigned)(ceil_div(rows, F16_ROWS) * ceil_div(in, pg::BN)), THREADS, 0, codes, exponents, (uint32_t)rows,
+                (uint32_t)in, (uint32_t)p.ip, x16, col_factor, parts,
+                GyRows{static_cast<const uint16_t*>(gy.data), gy.stride, (uint32_t)out, (uint32_t)p.op, gy_parts});
     }
     const Operand b{x16, rows, in, p.ip, true};
     pg::Params q{};
@@ -914,9 +1021,14 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
     q.splits = p.cut.splits;
     q.out = g;
     q.partial = reinterpret_cast<float*>(ws + p.partial);
-    q.col_factor = bf16 ? nullptr : col_factor;
+    if (!bf16) {
+        q.col_factor = col_factor;
+        q.parts = parts;
+        q.parts_at = (uint32_t)p.op;
+    }
+    const CUtensorMap in_parts = operand_map(Operand{gy_parts, rows, 2 * p.op, 2 * p.op, true}, true);
     const uint32_t pairs = (uint32_t)std::min<size_t>(pairs_of(s.rt), ceil_div(out, 256) * ceil_div(in, 256) * p.cut.splits);
-    launch<pg::SUM, 1>(s, "tape_weight_grad", a, b, bf16, q, pairs);
+    launch<pg::SUM, 1>(s, "tape_weight_grad", a, b, bf16, q, pairs, &in_parts);
     if (p.cut.splits > 1)
         s.chain("combine", combine_kernel<float>, (unsigned)ceil_div(out * in, 4 * THREADS), THREADS, 0, static_cast<const float*>(q.partial), p.cut.splits,
                 (uint32_t)out, (uint32_t)in, nullptr, nullptr, 0u, g, nullptr, nullptr);

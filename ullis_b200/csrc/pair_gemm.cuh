@@ -20,7 +20,8 @@
 //   STORE  alpha * acc in 16 bits, or into an f32 accumulator, or as one of several partial sums
 //   SUM    acc in f32: the tensor cores cut off what falls below the accumulator's last bit (measured: K = 16384 1.9e-5 off in
 //          norm, 1.1e-4 where all terms have one sign; K = 512 6e-7), so every 512 terms the accumulator moves to registers
-//          and is added there with rounding
+//          and is added there with rounding, in FP16 with a factor per 32 columns.  A stretch of 512 terms whose B does not fit into
+//          FP16 comes in bf16, and goes through the accumulator twice, for the two bf16 parts of A
 // Measured at 16384 x 512 x 8192 in FP16 (137 GFLOP each, cold caches): LSE 106 us, GRAD 125, STORE 105 (one accumulator at a time)
 // and 95 (two); SUM at 2048 x 16384 -> 512 in bf16 35 us for 34 GFLOP.  The tensor pipe is busy 65, 54, 69, 70 and 48 % of the
 // time.  The products of such a call take the pipe 113 thousand cycles, a loop without an epilogue 148 (the same without the loads of
@@ -48,11 +49,11 @@ constexpr uint32_t MAX_STAGES = 6, SMEM_LIMIT = 227 * 1024;
 constexpr uint32_t STAGING_BYTES = 16 * 128;            // 16 rows of 64 16-bit outputs; GRAD has two of them
 constexpr uint32_t COLUMN_BYTES = 2 * 64 * 4;           // constants of its columns
 constexpr uint32_t ROW_BYTES = 2 * 4 * 32 * 4;          // GRAD: what its rows need, of this tile and of the next
-constexpr uint32_t SUM_BLOCKS = 8;                      // k-blocks between two rounded additions
+constexpr uint32_t SUM_BLOCKS = 8;                      // k-blocks of a stretch of K, after which SUM adds with rounding
 
 struct Maps {
     CUtensorMap a, b;
-    CUtensorMap out;           // GRAD: [M, pitch] in boxes of 64 columns x 16 rows
+    CUtensorMap out;           // GRAD: [M, pitch] in boxes of 64 columns x 16 rows; SUM: A in two bf16 parts (Params::parts)
 };
 
 struct Params {
@@ -86,7 +87,12 @@ struct Params {
     float* accum;              // f32 [M][N]; STORE: read first if `accum_read`, written unless `out` is
     uint32_t accum_read;
     float* partial;            // splits > 1: [split][M][N]
-    const float* col_factor;   // SUM: [ceil(N / 32)] or null
+    // SUM, FP16: for each stretch of K and 32 columns what its sums are multiplied by, [stretch][ceil(N / 32)], and for each stretch
+    // and tile of columns, [stretch][n_tiles], a word that is not 0 where B lies there in bf16 instead of FP16: A is then the sum of two
+    // bf16 matrices, columns [0, M) and [parts_at, parts_at + M) of maps.out, and the product goes through the stretch once with each
+    const float* col_factor;
+    const uint32_t* parts;
+    uint32_t parts_at;
 };
 
 inline uint32_t stage_bytes(int accs) { return OPERAND_BYTES * (1 + accs); }
@@ -133,6 +139,9 @@ struct Work {
         if (EPI == LSE) open(m_tiles, min(p.piece_tiles, n_tiles));
         if (EPI == GRAD) open(n_tiles, m_tiles);
     }
+    // where the stretch from k-block kb on ends (STORE: the range), and whether A comes in two parts there
+    __device__ uint32_t stretch_end(uint32_t kb) const { return EPI == SUM ? min(k1, kb + SUM_BLOCKS) : k1; }
+    __device__ bool in_parts(uint32_t kb) const { return kb < k1 && p.parts[kb / SUM_BLOCKS * n_tiles + n]; }
     __device__ void open(uint32_t outers, uint32_t inners) {
         const Share s = share_of(outers * inners, pairs);
         width = inners;
@@ -162,8 +171,9 @@ struct Work {
         split = job % p.splits;
         m = tile / n_tiles;
         n = tile % n_tiles;
-        k0 = (uint32_t)((uint64_t)split * blocks / p.splits);
-        k1 = (uint32_t)((uint64_t)(split + 1) * blocks / p.splits);
+        const uint32_t step = EPI == SUM ? SUM_BLOCKS : 1u, steps = (blocks + step - 1) / step;   // SUM: whole stretches
+        k0 = (uint32_t)((uint64_t)split * steps / p.splits) * step;
+        k1 = min(blocks, (uint32_t)((uint64_t)(split + 1) * steps / p.splits) * step);
         job += pairs;
         return true;
     }
@@ -373,6 +383,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
     constexpr uint32_t BUFFERS = ACCS == 1 ? 2 : 1;
+    constexpr bool BY_STRETCH = EPI == SUM && !BF16;   // stretches of K with a type and a factor of their own
     Work<EPI, ACCS> work(p, pair, pairs);
 
     if (warp == 0) {
@@ -383,7 +394,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             bool ok = true;
             while (ok && work.next()) {
                 const int32_t m0 = (int32_t)(work.m * BM + rank * 128), n0 = (int32_t)(work.n * BN * ACCS + rank * 128);
-                for (uint32_t kb = work.k0; kb < work.k1; ++kb, ++it) {
+                uint32_t last = BY_STRETCH ? work.stretch_end(work.k0) : work.k1;
+                bool parts = BY_STRETCH && work.in_parts(work.k0), ahead = BY_STRETCH && work.in_parts(last), second = false;
+                for (uint32_t kb = work.k0; kb < work.k1; ++it) {
                     const uint32_t s = it % STAGES;
                     if (it >= STAGES && !wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, s_error)) {
                         atomicCAS(s_error, 0u, 1u);
@@ -391,12 +404,13 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         break;
                     }
                     uint8_t* st = smem + s * STAGE;
-                    const int32_t k = (int32_t)(kb * BK);
+                    const int32_t k = (int32_t)(kb * BK), ma = BY_STRETCH && second ? m0 + (int32_t)p.parts_at : m0;
+                    const CUtensorMap* map_a = BY_STRETCH && parts ? &maps.out : &maps.a;
                     const uint32_t bar = full_even + 8 * s;
                     if (rank == 0) ptx::mbar_arrive_expect_tx(&full[s], 2 * STAGE);
                     if (p.a_mn) {
-                        ptx::tma_load_2d_pair(st, &maps.a, bar, m0, k);
-                        ptx::tma_load_2d_pair(st + 8192, &maps.a, bar, m0 + 64, k);
+                        ptx::tma_load_2d_pair(st, map_a, bar, ma, k);
+                        ptx::tma_load_2d_pair(st + 8192, map_a, bar, ma + 64, k);
                     } else {
                         ptx::tma_load_2d_pair(st, &maps.a, bar, k, m0);
                     }
@@ -410,6 +424,16 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         } else {
                             ptx::tma_load_2d_pair(bt, &maps.b, bar, k, nb);
                         }
+                    }
+                    if (++kb < last) continue;
+                    if (BY_STRETCH && parts && !second) {   // through the stretch again
+                        second = true;
+                        kb = (last - 1) / SUM_BLOCKS * SUM_BLOCKS;
+                    } else if (BY_STRETCH) {
+                        second = false;
+                        parts = ahead;
+                        last = work.stretch_end(kb);
+                        ahead = work.in_parts(last);
                     }
                 }
             }
@@ -425,14 +449,17 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     } else if (warp == 1) {
         // ------------------------------------------------------ products (even CTA)
         if (rank == 0 && ptx::elect_one()) {
-            const uint32_t idesc = ptx::idesc_f16(BF16, BF16, BM, BN) | p.a_mn << 15 | p.b_mn << 16;
+            const uint32_t layout = p.a_mn << 15 | p.b_mn << 16;
             const uint32_t a_step = p.a_mn ? 2048u : 32u, b_step = p.b_mn ? 2048u : 32u;   // 16 k
             const uint32_t ring = ptx::smem_u32(smem);
             uint32_t it = 0, done = 0;   // k-blocks, accumulators
             bool ok = true;
             while (ok && work.next()) {
+                bool parts = BY_STRETCH && work.in_parts(work.k0);
                 for (uint32_t kb = work.k0; kb < work.k1 && ok;) {
-                    const uint32_t last = EPI == SUM ? min(work.k1, kb + SUM_BLOCKS) : work.k1;
+                    const uint32_t last = work.stretch_end(kb), todo = (last - kb) * (parts ? 2 : 1);
+                    const uint32_t idesc = ptx::idesc_f16(BF16 || parts, BF16 || parts, BM, BN) | layout;
+                    const bool ahead = BY_STRETCH && work.in_parts(last);
                     const uint32_t buf = done % BUFFERS;
                     if (done >= BUFFERS && !wait(&tmem_empty[buf], ((done / BUFFERS) & 1u) ^ 1u, s_error)) {
                         atomicCAS(s_error, 0u, 2u);
@@ -441,7 +468,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     }
                     ptx::tc_fence_after_sync();
                     bool add = false;
-                    for (; kb < last; ++kb, ++it) {
+                    for (uint32_t i = 0; i < todo; ++i, ++it) {
                         const uint32_t s = it % STAGES;
                         if (!wait(&full[s], (it / STAGES) & 1u, s_error)) {
                             atomicCAS(s_error, 0u, 3u);
@@ -454,10 +481,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         for (uint32_t k4 = 0; k4 < BK / 16; ++k4) {
                             const uint64_t da = p.a_mn ? smem_desc_mn(a + k4 * a_step) : ptx::smem_desc_sw128(a + k4 * a_step);
 #pragma unroll
-                            for (int i = 0; i < ACCS; ++i) {
-                                const uint32_t bi = b + i * OPERAND_BYTES + k4 * b_step;
+                            for (int acc = 0; acc < ACCS; ++acc) {
+                                const uint32_t bi = b + acc * OPERAND_BYTES + k4 * b_step;
                                 const uint64_t db = p.b_mn ? smem_desc_mn(bi) : ptx::smem_desc_sw128(bi);
-                                ptx::mma_f16_ss_pair(tmem_base + (ACCS == 1 ? buf : i) * BN, da, db, idesc, add || k4);
+                                ptx::mma_f16_ss_pair(tmem_base + (ACCS == 1 ? buf : acc) * BN, da, db, idesc, add || k4);
                             }
                         }
                         add = true;
@@ -465,6 +492,8 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     }
                     ptx::mma_commit_pair(&tmem_full[buf]);   // on the way out too: the epilogues do not wait in vain
                     ++done;
+                    kb = last;
+                    parts = ahead;
                 }
             }
         }
@@ -794,8 +823,15 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 float v[64];
 #pragma unroll
                 for (int i = 0; i < 64; ++i) v[i] = 0.0f;
-                for (uint32_t kb = work.k0; kb < work.k1; kb += SUM_BLOCKS) {
+                const uint32_t m0 = work.m * BM + rank * 128 + quarter * 32, n0 = work.n * BN + group * 64, blocks32 = (p.N + 31) / 32;
+                for (uint32_t kb = work.k0; kb < work.k1; kb = work.stretch_end(kb)) {
                     uint32_t taddr;
+                    float f[2];
+                    if constexpr (BY_STRETCH) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            f[i] = n0 + i * 32 < p.N ? p.col_factor[(size_t)(kb / SUM_BLOCKS) * blocks32 + n0 / 32 + i] : 0.0f;
+                    }
                     ok = filled(&taddr);
                     if (!ok) break;
 #pragma unroll
@@ -805,15 +841,13 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         ptx::tmem_ld_wait();
                         if (h == 1) drained();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[h * 32 + i] += __uint_as_float(r[i]);
+                        for (int i = 0; i < 32; ++i) {
+                            float& sum = v[h * 32 + i];
+                            sum = BY_STRETCH ? fmaf(__uint_as_float(r[i]), f[i >> 4], sum) : sum + __uint_as_float(r[i]);   // (f: powers of two)
+                        }
                     }
                 }
                 if (!ok) break;
-                const uint32_t m0 = work.m * BM + rank * 128 + quarter * 32, n0 = work.n * BN + group * 64;
-                float f[2] = {1.0f, 1.0f};
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (p.col_factor && n0 + i * 32 < p.N) f[i] = p.col_factor[n0 / 32 + i];
                 float* out = p.splits > 1 ? p.partial + (size_t)work.split * p.M * p.N : static_cast<float*>(p.out);
                 const bool pairs_ok = rows_of_pairs(out, p.N);
 #pragma unroll
@@ -825,7 +859,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     for (int j = 0; j < 8; ++j) {
                         const uint32_t c = n0 + j * 8 + q2;
                         const int at = (i >> 1) * 32 + j * 4 + (i & 1) * 2;
-                        const float x = v[at] * f[j >> 2], y = v[at + 1] * f[j >> 2];
+                        const float x = v[at], y = v[at + 1];
                         if (pairs_ok) {
                             if (c < p.N) *reinterpret_cast<float2*>(line + c) = make_float2(x, y);
                         } else {

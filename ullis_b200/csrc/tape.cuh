@@ -163,8 +163,9 @@ __device__ __forceinline__ void values_of(const uint32_t (&w)[N / 4], float step
     for (int i = 0; i < N; ++i) v[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * step;
 }
 template <bool VEC, int N>
-__device__ __forceinline__ void load_codes(const uint8_t* codes, float step, uint32_t c, uint32_t C, float (&v)[N]) {
-    uint32_t w[N / 4] = {};
+__device__ __forceinline__ void raw_codes(const uint8_t* codes, uint32_t c, uint32_t C, uint32_t (&w)[N / 4]) {
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) w[k] = 0;
     if constexpr (VEC) {
         if (c < C) {
             if constexpr (N == 8) {
@@ -174,11 +175,19 @@ __device__ __forceinline__ void load_codes(const uint8_t* codes, float step, uin
                 w[0] = *reinterpret_cast<const uint32_t*>(codes + c);
             }
         }
-        values_of(w, c < C ? step : 0.0f, v);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (c + i < C) w[i >> 2] |= (uint32_t)codes[c + i] << (8 * (i & 3));
+    }
+}
+template <bool VEC, int N>
+__device__ __forceinline__ void load_codes(const uint8_t* codes, float step, uint32_t c, uint32_t C, float (&v)[N]) {
+    uint32_t w[N / 4];
+    raw_codes<VEC, N>(codes, c, C, w);
+    if constexpr (VEC) {
+        values_of(w, c < C ? step : 0.0f, v);
+    } else {
         values_of(w, step, v);
 #pragma unroll
         for (int i = 0; i < N; ++i)
