@@ -394,25 +394,22 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             bool ok = true;
             while (ok && work.next()) {
                 const int32_t m0 = (int32_t)(work.m * BM + rank * 128), n0 = (int32_t)(work.n * BN * ACCS + rank * 128);
-                uint32_t last = BY_STRETCH ? work.stretch_end(work.k0) : work.k1;
-                bool parts = BY_STRETCH && work.in_parts(work.k0), ahead = BY_STRETCH && work.in_parts(last), second = false;
-                for (uint32_t kb = work.k0; kb < work.k1; ++it) {
+                const auto fetch = [&](uint32_t kb, const CUtensorMap* map_a, int32_t ma) {
                     const uint32_t s = it % STAGES;
                     if (it >= STAGES && !wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, s_error)) {
                         atomicCAS(s_error, 0u, 1u);
                         ok = false;
-                        break;
+                        return;
                     }
                     uint8_t* st = smem + s * STAGE;
-                    const int32_t k = (int32_t)(kb * BK), ma = BY_STRETCH && second ? m0 + (int32_t)p.parts_at : m0;
-                    const CUtensorMap* map_a = BY_STRETCH && parts ? &maps.out : &maps.a;
+                    const int32_t k = (int32_t)(kb * BK);
                     const uint32_t bar = full_even + 8 * s;
                     if (rank == 0) ptx::mbar_arrive_expect_tx(&full[s], 2 * STAGE);
                     if (p.a_mn) {
                         ptx::tma_load_2d_pair(st, map_a, bar, ma, k);
                         ptx::tma_load_2d_pair(st + 8192, map_a, bar, ma + 64, k);
                     } else {
-                        ptx::tma_load_2d_pair(st, &maps.a, bar, k, m0);
+                        ptx::tma_load_2d_pair(st, map_a, bar, k, ma);
                     }
 #pragma unroll
                     for (int i = 0; i < ACCS; ++i) {
@@ -425,15 +422,23 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             ptx::tma_load_2d_pair(bt, &maps.b, bar, k, nb);
                         }
                     }
-                    if (++kb < last) continue;
-                    if (BY_STRETCH && parts && !second) {   // through the stretch again
-                        second = true;
-                        kb = (last - 1) / SUM_BLOCKS * SUM_BLOCKS;
-                    } else if (BY_STRETCH) {
-                        second = false;
+                    ++it;
+                };
+                if constexpr (BY_STRETCH) {
+                    bool parts = work.in_parts(work.k0);
+                    for (uint32_t from = work.k0; from < work.k1 && ok;) {
+                        const uint32_t last = work.stretch_end(from);
+                        const bool ahead = work.in_parts(last);
+                        for (uint32_t kb = from; kb < last && ok; ++kb) fetch(kb, parts ? &maps.out : &maps.a, m0);
+                        if (parts)
+                            for (uint32_t kb = from; kb < last && ok; ++kb) fetch(kb, &maps.out, m0 + (int32_t)p.parts_at);
+                        from = last;
                         parts = ahead;
-                        last = work.stretch_end(kb);
-                        ahead = work.in_parts(last);
+                    }
+                } else {
+                    for (uint32_t kb = work.k0; kb < work.k1; ++kb) {
+                        fetch(kb, &maps.a, m0);
+                        if (!ok) break;
                     }
                 }
             }
@@ -449,17 +454,18 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     } else if (warp == 1) {
         // ------------------------------------------------------ products (even CTA)
         if (rank == 0 && ptx::elect_one()) {
-            const uint32_t layout = p.a_mn << 15 | p.b_mn << 16;
+            const uint32_t idesc_own = ptx::idesc_f16(BF16, BF16, BM, BN) | p.a_mn << 15 | p.b_mn << 16;
+            const uint32_t idesc_bf16 = ptx::idesc_f16(true, true, BM, BN) | p.a_mn << 15 | p.b_mn << 16;
             const uint32_t a_step = p.a_mn ? 2048u : 32u, b_step = p.b_mn ? 2048u : 32u;   // 16 k
             const uint32_t ring = ptx::smem_u32(smem);
             uint32_t it = 0, done = 0;   // k-blocks, accumulators
             bool ok = true;
             while (ok && work.next()) {
-                bool parts = BY_STRETCH && work.in_parts(work.k0);
+                bool parts = BY_STRETCH && work.in_parts(work.k0);   // this stretch's products in bf16, and twice as many
                 for (uint32_t kb = work.k0; kb < work.k1 && ok;) {
-                    const uint32_t last = work.stretch_end(kb), todo = (last - kb) * (parts ? 2 : 1);
-                    const uint32_t idesc = ptx::idesc_f16(BF16 || parts, BF16 || parts, BM, BN) | layout;
+                    const uint32_t last = EPI == SUM ? work.stretch_end(kb) : work.k1, idesc = BY_STRETCH && parts ? idesc_bf16 : idesc_own;
                     const bool ahead = BY_STRETCH && work.in_parts(last);
+                    const uint32_t end = BY_STRETCH && parts ? 2 * last - kb : last;
                     const uint32_t buf = done % BUFFERS;
                     if (done >= BUFFERS && !wait(&tmem_empty[buf], ((done / BUFFERS) & 1u) ^ 1u, s_error)) {
                         atomicCAS(s_error, 0u, 2u);
@@ -468,7 +474,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     }
                     ptx::tc_fence_after_sync();
                     bool add = false;
-                    for (uint32_t i = 0; i < todo; ++i, ++it) {
+                    for (; kb < end; ++kb, ++it) {
                         const uint32_t s = it % STAGES;
                         if (!wait(&full[s], (it / STAGES) & 1u, s_error)) {
                             atomicCAS(s_error, 0u, 3u);
@@ -481,10 +487,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         for (uint32_t k4 = 0; k4 < BK / 16; ++k4) {
                             const uint64_t da = p.a_mn ? smem_desc_mn(a + k4 * a_step) : ptx::smem_desc_sw128(a + k4 * a_step);
 #pragma unroll
-                            for (int acc = 0; acc < ACCS; ++acc) {
-                                const uint32_t bi = b + acc * OPERAND_BYTES + k4 * b_step;
+                            for (int i = 0; i < ACCS; ++i) {
+                                const uint32_t bi = b + i * OPERAND_BYTES + k4 * b_step;
                                 const uint64_t db = p.b_mn ? smem_desc_mn(bi) : ptx::smem_desc_sw128(bi);
-                                ptx::mma_f16_ss_pair(tmem_base + (ACCS == 1 ? buf : acc) * BN, da, db, idesc, add || k4);
+                                ptx::mma_f16_ss_pair(tmem_base + (ACCS == 1 ? buf : i) * BN, da, db, idesc, add || k4);
                             }
                         }
                         add = true;
@@ -492,8 +498,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     }
                     ptx::mma_commit_pair(&tmem_full[buf]);   // on the way out too: the epilogues do not wait in vain
                     ++done;
-                    kb = last;
-                    parts = ahead;
+                    if (BY_STRETCH) {
+                        kb = last;
+                        parts = ahead;
+                    }
                 }
             }
         }
@@ -742,6 +750,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             leave();
         } else if constexpr (EPI == STORE) {
             const float alpha = p.factor ? *p.factor : 1.0f;
+            const bool pairs_ok = rows_of_pairs(p.out_f32 ? p.out : nullptr, p.N);   // (the other f32 arrays lie in the workspace)
             const bool wide = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
             uint16_t* out = static_cast<uint16_t*>(p.out);
             while (work.next()) {
@@ -764,7 +773,6 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
                     const auto f32_rows = [&](float* at, const int32_t* rows, bool read, bool write, float times) {
-                        const bool pairs_ok = rows_of_pairs(at, p.N);
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const uint32_t row = m0 + h * 16 + r0 + i * 8;
