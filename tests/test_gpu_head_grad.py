@@ -157,6 +157,40 @@ def test_a_vocabulary_in_several_pieces_of_the_largest_size(cuda_rt, packed, dty
     check(call(cuda_rt, s), formulas(s))
 
 
+def lost(got, want):
+    """Mean relative error of sums, positive where they are too small; what rounds them to 16 bits has a mean of 0."""
+    return ((want - got.double()) / want).mean().item()
+
+
+@pytest.mark.parametrize("over", ["rows", "vocabulary"])
+def test_long_sums_of_one_sign(cuda_rt, over):
+    """What the tensor cores cut off of a sum does not grow with its length.  All logits are 0 and every probability 1 / vocab, in FP16 the
+    number p; so the weights' gradient is p times the sum of the rows of h (no weights, h in [1, 2)), the hidden states' p times that of the
+    weights (no h, weights in [1, 2), the target's 0), all terms of one sign.  Of 1024 sums, each rounded by half a step of FP16 at most,
+    the mean is off by 2^-11 / sqrt(3 * 1024) < 1e-5 (one sigma); what is lost has to stay below 2^-12, the smallest half step there is."""
+    d, found = 1024, {}
+    for length in (16000, 65000, 200000) if over == "rows" else (16000, 65000):
+        g = torch.Generator("cuda").manual_seed(length)
+        rows, vocab = (length + 1, 4000) if over == "rows" else (4096, length)
+        # (2^14: what the call multiplies g by in FP16; an f32 probability rounds to the same number)
+        p, near = (torch.tensor([x * 2.0 ** 14 / vocab for x in (1.0, 1 - 1e-5, 1 + 1e-5)], dtype=torch.float64).half().split([1, 2]))
+        assert (near == p).all()
+        ones = (1 + torch.randint(0, 1024, (length, d), generator=g, device="cuda") / 1024).half()
+        if over == "rows":
+            hidden = torch.cat([ones, torch.full_like(ones[:1], float("nan"))])
+            weight = torch.zeros(vocab, d, dtype=torch.float16, device="cuda")
+        else:
+            hidden = torch.zeros(rows, d, dtype=torch.float16, device="cuda")
+            weight = ones
+            weight[0] = 0.0
+        r = cuda_rt.head_ce_grad(hidden, weight, torch.zeros(rows, dtype=torch.int32, device="cuda"), time=rows)
+        got = r.weight[1:] if over == "rows" else r.hidden[:-1]
+        assert torch.equal(got, got[:1].expand_as(got))
+        found[length] = lost(got[0], ones.sum(0, dtype=torch.float64) * (p.item() * 2.0 ** -14))
+    assert max(found.values()) <= 1.25 * found[16000] + 5e-5, found
+    assert max(found.values()) <= 2.0 ** -12, found
+
+
 def test_drawn_sizes(cuda_rt):
     import random
     rng = random.Random(7)

@@ -99,7 +99,8 @@ void need_codes(const uint8_t* codes, const uint8_t* exponents) {
     need_array(exponents, "exponents", 1);
 }
 
-// The tiles of a product are counted in 32 bits (up to 16 ranges of K each).
+// The tiles of a product are counted in 32 bits, each with up to 16 ranges of K; more, of 2^14 terms and up to 2^10, only the head takes,
+// where K is above 2^18 and the other side of its piece of g below 2^10.
 void need_tiles(size_t m, size_t n, const char* what) {
     if ((m + 255) / 256 * ((n + 255) / 256) >= ((size_t)1 << 27)) fail(ULLIS_CUDA_ERR_SHAPE, std::string(what) + " shape overflow");
 }

@@ -107,16 +107,21 @@ void launch(const Stream& s, const char* what, const Operand& a, const Operand& 
 // Two accumulators fetch A half as often, which counts where the power limit sets the clock: a head of 16384 x 512 x 8192 takes
 // 500 us instead of 507 over seconds, 429 instead of 434 before the limit acts.
 // (two: a product of the head, else a SUM, whose ranges are whole stretches of K)
+// A product of the head has no more than LONGEST k-blocks in one accumulator, whose additions the tensor cores cut off: sums of 16 384
+// terms of one sign are 1.0e-4 too small, of 65 536 4.3e-4, and half a step of FP16 is 2.4e-4 to 4.9e-4.  (4096 x 512 x 131072, whose hidden
+// gradient has four ranges for it instead of two: 2.08 ms, with two 2.07.)
 struct Cut {
     uint32_t accs, splits;
 };
+constexpr size_t LONGEST = 16384 / pg::BK;
 Cut cut_of(size_t M, size_t N, size_t K, uint32_t pairs, bool two) {
     const size_t blocks = std::max<size_t>(1, ceil_div(K, pg::BK));
+    const size_t fewest = two ? ceil_div(blocks, LONGEST) : 1;
     Cut best{1, 1};
     double least = 1e300;
     for (uint32_t accs = 1; accs <= (two && N > 256 ? 2u : 1u); ++accs) {
         const size_t tiles = ceil_div(M, 256) * ceil_div(N, 256 * accs);
-        for (uint32_t splits = 1; splits <= std::min<size_t>(16, std::max<size_t>(1, blocks / 4)); ++splits) {
+        for (uint32_t splits = (uint32_t)fewest; splits <= std::max(fewest, std::min<size_t>(16, std::max<size_t>(1, blocks / 4))); ++splits) {
             const double rounds = (double)ceil_div(tiles * splits, pairs);
             const double epilogue = accs == 2 ? 10.0 : 1.0;
             const size_t most = two ? ceil_div(blocks, splits) : std::min(blocks, ceil_div(ceil_div(blocks, pg::SUM_BLOCKS), splits) * pg::SUM_BLOCKS);
