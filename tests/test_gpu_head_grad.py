@@ -157,6 +157,19 @@ def test_a_vocabulary_in_several_pieces_of_the_largest_size(cuda_rt, packed, dty
     check(call(cuda_rt, s), formulas(s))
 
 
+@pytest.mark.parametrize("rows,d,vocab,packed,dtype", [(4096, 64, 70000, True, "f16"), (4000, 66, 70000, False, "bf16"),
+                                                       (40000, 40, 8000, True, "bf16"), (40000, 33, 8000, False, "f16")])
+def test_sums_over_pieces_and_ranges(cuda_rt, rows, d, vocab, packed, dtype):
+    """Two pieces of the vocabulary, and one of the gradient products in several ranges of its sums: the hidden states' (few rows, a large
+    vocabulary), whose sum over the pieces lies in f32 between them, or the weights' (many rows).  The launches show that it is so:
+    list, operands, log sum exp, rows' losses; for each piece the gradient, columns' sums, two products and the sum of the ranges."""
+    s = inputs(rows, rows // 8, d, vocab, dtype, packed, 0.1, seed=vocab + d)
+    before = cuda_rt.launch_count
+    got = call(cuda_rt, s)
+    assert cuda_rt.launch_count - before == 4 + 2 * 5
+    check(got, formulas(s))
+
+
 def lost(got, want):
     """Mean relative error of sums, positive where they are too small; what rounds them to 16 bits has a mean of 0."""
     return ((want - got.double()) / want).mean().item()
