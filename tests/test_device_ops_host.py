@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from ullis_b200 import cuda
+from ullis_b200 import cuda, device
 from ullis_b200.device import DeviceOps
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -116,6 +116,33 @@ REFUSED = {
     "norm backward: residual's rows": (lambda rt: rt.tape_layer_norm_backward(
         codes(), torch.zeros(4, 64), torch.zeros(64, dtype=H), residual=torch.zeros(3, 64)), cuda.ERR_SHAPE),
 }
+
+
+class Taking(Fake):
+    """Every call of the library succeeds; the last one's arguments are kept."""
+
+    class _Lib:
+        def __getattr__(self, name):
+            def call(*arguments):
+                Taking.arguments = arguments
+                return cuda.OK
+            return call
+
+    _lib = _Lib()
+
+    def _check(self, rc):
+        assert rc == cuda.OK
+
+
+@pytest.mark.parametrize("shape,time", [((3, 0, 64), 1), ((0, 5, 64), 5), ((0, 64), 1), ((3, 4, 64), 4), ((12, 64), 12)])
+def test_the_time_that_a_shape_gives(monkeypatch, shape, time):
+    """Zero rows are no error, whichever of the leading sizes is 0."""
+    device._torch()
+    monkeypatch.setattr(device, "_RAW_STREAM", lambda d: 0)
+    rows = shape[0] if len(shape) == 2 else shape[0] * shape[1]
+    r = Taking().head_ce_grad(torch.zeros(shape, dtype=H), dense(), torch.zeros(shape[:-1], dtype=torch.int32))
+    assert Taking.arguments[11:14] == (rows, time, 64) and rows % time == 0
+    assert r.hidden.shape == shape and r.row_loss.shape == (rows,) and r.weight.shape == (9, 64)
 
 
 @pytest.mark.parametrize("call,code", REFUSED.values(), ids=REFUSED.keys())

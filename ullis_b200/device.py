@@ -2,8 +2,8 @@
 
 Tensors lie on the runtime's device; kernels go to torch's current stream of that device, outputs and workspaces come from
 torch's allocator on it, and nothing waits for the device, so the calls may be captured into a graph.  A tensor that belongs to
-another stream is ordered and kept alive by the caller, as for any torch operation.  Arguments that the operator does not take
-raise `UllisCudaError`.  The arithmetic, the 8-bit tape and the limits are described at the entry points of
+another stream is ordered and kept alive by the caller, as for any torch operation.  Autograd does not see the calls: inputs may
+require gradients, outputs track nothing.  Arguments that the operator does not take raise `UllisCudaError`.  The arithmetic, the 8-bit tape and the limits are described at the entry points of
 include/ullis_cuda.h.
 """
 from __future__ import annotations
@@ -251,7 +251,7 @@ class DeviceOps:
         rows, channels, stride = self._matrix(hidden, "hidden", _16)
         self._vector(labels, "labels", _I32, rows)
         if time is None:
-            time = hidden.shape[-2] if hidden.dim() == 3 else max(rows, 1)
+            time = max(1, hidden.shape[-2] if hidden.dim() == 3 else rows)
         if scale is not None:
             self._refuse(scale, "scale", _F16)
             vocab = scale.numel()
