@@ -132,6 +132,9 @@ ULLIS_CUDA_API void ullis_cuda_host_free(void* block);
  * "a kernel gave up waiting" as the message; the runtime stays usable.  The reference's counterpart of the path
  * is the command-buffer error check after waitUntilCompleted (src/metal.rs:736-738). */
 ULLIS_CUDA_API int32_t ullis_cuda_runtime_wait_selftest(ullis_cuda_runtime* rt, uint32_t polls);
+/* The same on a caller's stream, where a kernel that gives up is reported to a later call: returns ULLIS_CUDA_OK, and
+ * once the stream has been waited for, the next call on the runtime returns ULLIS_CUDA_ERR_TIMEOUT. */
+ULLIS_CUDA_API int32_t ullis_cuda_runtime_wait_selftest_on(ullis_cuda_runtime* rt, void* cuda_stream, uint32_t polls);
 /* Compute capability check: 1 when the device is sm_100 class. */
 ULLIS_CUDA_API int32_t ullis_cuda_runtime_is_sm100(const ullis_cuda_runtime* rt);
 
@@ -435,9 +438,12 @@ ULLIS_CUDA_API int32_t ullis_cuda_rosa_sam_static(int32_t device, void* cuda_str
  *    caller's and free again when the stream has passed the call (two graphs that
  *    may run at once need one each).  The current device is left as it was.
  *  - A refused call (ULLIS_CUDA_ERR_ARG, ULLIS_CUDA_ERR_SHAPE) has enqueued nothing.
- *    Should a kernel give up waiting, which none does in working order, the next
- *    call on the runtime or ullis_cuda_runtime_synchronize returns
- *    ULLIS_CUDA_ERR_TIMEOUT, and the outputs of the call that it belonged to are void.
+ *    Should a kernel give up waiting, which none does in working order, the next call
+ *    on the runtime, or on a model or state of it, after that kernel has ended
+ *    returns ULLIS_CUDA_ERR_TIMEOUT (once; it does nothing else), and the outputs of
+ *    the call that the kernel belonged to are void.  Whoever wants to be sure of the
+ *    outputs waits for `cuda_stream` and then calls ullis_cuda_runtime_synchronize,
+ *    which by itself waits for the runtime's own stream only.
  *  - Zero rows are no error: nothing but sums over rows, which are zero, is written.
  *
  * The 8-bit tape of x [rows, channels]: blocks of 32 consecutive channels of a row

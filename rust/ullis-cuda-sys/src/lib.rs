@@ -119,6 +119,11 @@ unsafe extern "C" {
     pub fn ullis_cuda_host_alloc(rt: *mut ullis_cuda_runtime, bytes: usize, out: *mut *mut c_void) -> i32;
     pub fn ullis_cuda_host_free(block: *mut c_void);
     pub fn ullis_cuda_runtime_wait_selftest(rt: *mut ullis_cuda_runtime, polls: u32) -> i32;
+    pub fn ullis_cuda_runtime_wait_selftest_on(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        polls: u32,
+    ) -> i32;
     pub fn ullis_cuda_runtime_is_sm100(rt: *const ullis_cuda_runtime) -> i32;
     pub fn ullis_cuda_model_load_safetensors(
         rt: *mut ullis_cuda_runtime,

@@ -36,6 +36,7 @@ int32_t guard(ullis_cuda_runtime* rt, F&& body) {
     };
     try {
         rt->bind();
+        rt->throw_on_async_status();   // of a kernel on a caller's stream
         body();
         return ULLIS_CUDA_OK;
     } catch (const Error& e) {

@@ -125,6 +125,13 @@ void need_head(size_t rows, size_t channels, size_t vocab) {
 
 extern "C" {
 
+int32_t ullis_cuda_runtime_wait_selftest_on(ullis_cuda_runtime* rt, void* cuda_stream, uint32_t polls) {
+    return on_stream(rt, cuda_stream, [&](const dev::Stream& s) {
+        if (polls == 0 || polls > (1u << 20)) fail(ULLIS_CUDA_ERR_ARG, "polls must be in 1..2^20");
+        dev::wait_selftest(s, polls);
+    });
+}
+
 int32_t ullis_cuda_tape_pack(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const void* x, size_t x_stride, size_t rows,
                              size_t channels, uint8_t* codes, uint8_t* exponents) {
     return on_stream(rt, cuda_stream, [&](const dev::Stream& s) {

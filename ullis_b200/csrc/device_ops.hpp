@@ -43,6 +43,9 @@ struct Tape8 {   // a tape of [rows, channels] in a buffer of its own
     }
 };
 
+// One CTA waits on a barrier that nothing arrives on, `polls` times, and says so as the products do.
+void wait_selftest(const Stream& s, uint32_t polls);
+
 // ---- the 8-bit tape (tape.cuh); codes [rows, channels] and exponents [rows, ceil(channels / 32)] without gaps
 void tape_pack(const Stream& s, int dtype, Rows x, size_t rows, size_t channels, uint8_t* codes, uint8_t* exponents);
 void tape_unpack(const Stream& s, int dtype, const uint8_t* codes, const uint8_t* exponents, size_t rows, size_t channels, void* x,

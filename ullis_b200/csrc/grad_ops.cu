@@ -773,6 +773,24 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------ a wait that runs out
+namespace {
+__global__ void wait_selftest_kernel(uint32_t polls, uint32_t* status) {
+    __shared__ __align__(8) uint64_t bar;
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(&bar, 1);
+        ptx::fence_mbar_init();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && !ptx::mbar_wait(&bar, 0, polls)) pg::report_wait(status, 99u);   // site: self-test
+}
+}  // namespace
+
+void wait_selftest(const Stream& s, uint32_t polls) {
+    wait_selftest_kernel<<<1, 32, 0, s.stream>>>(polls, s.status);
+    s.launched("wait_selftest");
+}
+
 // ------------------------------------------------------------------------------------------------ weight gradient from the tape
 namespace {
 

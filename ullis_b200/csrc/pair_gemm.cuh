@@ -303,6 +303,13 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile ui
     return false;
 }
 
+// A wait at `site` has run out.  On a caller's stream `status` is pinned host memory.
+__device__ __forceinline__ void report_wait(volatile uint32_t* status, uint32_t site) {
+    status[1] = site;
+    __threadfence_system();
+    status[0] = ULLIS_DEV_WAIT_TIMEOUT;
+}
+
 constexpr float LOG2E = 1.4426950408889634f;
 
 // Whether two columns of every row of an f32 array of `columns` lie on 8 bytes: a caller's array is aligned to its elements only.
@@ -887,12 +894,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         ptx::tmem_dealloc_pair(tmem_base, 512);
     }
     if (EPI == STORE && p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (threadIdx.x == 0 && *s_error) {
-        volatile uint32_t* status = p.status;   // a caller's stream: pinned host memory
-        status[1] = 64u + *s_error;
-        __threadfence_system();
-        status[0] = ULLIS_DEV_WAIT_TIMEOUT;
-    }
+    if (threadIdx.x == 0 && *s_error) report_wait(p.status, 64u + *s_error);
 }
 
 }  // namespace pg

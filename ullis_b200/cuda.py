@@ -58,7 +58,8 @@ ABI_SYMBOLS = (
     "ullis_cuda_binary_linear", "ullis_cuda_fp16_linear", "ullis_cuda_sign_pack_bits", "ullis_cuda_cmix_relu2",
     "ullis_cuda_residual_add", "ullis_cuda_rosa_qkv_1bit_fwd", "ullis_cuda_rosa_block_forward",
     "ullis_cuda_cmix_block_forward", "ullis_cuda_streamed_ce", "ullis_cuda_rosa_sam_static",
-    "ullis_cuda_runtime_sam_counts", "ullis_cuda_runtime_wait_selftest", "ullis_cuda_host_alloc",
+    "ullis_cuda_runtime_sam_counts", "ullis_cuda_runtime_wait_selftest", "ullis_cuda_runtime_wait_selftest_on",
+    "ullis_cuda_host_alloc",
     "ullis_cuda_host_free", "ullis_cuda_model_read_loss_global", "ullis_cuda_dp_rendezvous",
     "ullis_cuda_dp_unique_id", "ullis_cuda_dp_init",
     "ullis_cuda_dp_allreduce_loss", "ullis_cuda_dp_finalize",
@@ -553,6 +554,10 @@ class CudaRuntime(DeviceOps):
         """Makes a bounded device wait run out (ullis_cuda_runtime_wait_selftest): always raises, ERR_TIMEOUT
         when the error path works."""
         self._check(self._lib.ullis_cuda_runtime_wait_selftest(self._h, C.c_uint32(polls)))
+
+    def wait_selftest_on(self, stream: int, polls: int = 2000) -> None:
+        """The same on a caller's stream (a cudaStream_t): once that has been waited for, the next call raises ERR_TIMEOUT."""
+        self._check(self._lib.ullis_cuda_runtime_wait_selftest_on(self._h, C.c_void_p(stream), C.c_uint32(polls)))
 
     def sam_counts(self) -> dict:
         """Streams of the last ROSA match: total, without a closed form, through the constant-q form."""

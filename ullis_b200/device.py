@@ -3,8 +3,9 @@
 Tensors lie on the runtime's device; kernels go to torch's current stream of that device, outputs and workspaces come from
 torch's allocator on it, and nothing waits for the device, so the calls may be captured into a graph.  A tensor that belongs to
 another stream is ordered and kept alive by the caller, as for any torch operation.  Autograd does not see the calls: inputs may
-require gradients, outputs track nothing.  Arguments that the operator does not take raise `UllisCudaError`.  The arithmetic, the 8-bit tape and the limits are described at the entry points of
-include/ullis_cuda.h.
+require gradients, outputs track nothing.  Arguments that the operator does not take raise `UllisCudaError`, and so does the next
+call of the runtime after a kernel that gave up waiting (none does in working order).  The arithmetic, the 8-bit tape and the
+limits are described at the entry points of include/ullis_cuda.h.
 """
 from __future__ import annotations
 
