@@ -59,6 +59,20 @@ def test_terms_of_one_sign(cuda_rt):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_what_is_cut_off_does_not_grow_with_the_rows(cuda_rt, dtype):
+    """Sums of one sign over 512 rows, and over 32 times as many: no more than 512 terms are added up without rounding, so what is lost
+    of a sum is what is lost of its parts.  Their 32 additions are off by 2^-25 each, up and down."""
+    lost = []
+    for rows in (512, 16384):
+        codes, exponents = tape_of(rows, 512, 3)
+        gy = torch.rand(rows, 512, device="cuda").to(TYPES[dtype])
+        want = gy.double().t() @ values(codes.abs(), exponents)
+        got = cuda_rt.tape_weight_grad((codes.abs(), exponents), gy)
+        lost.append(((want - got.double()) / want).mean().item())
+    assert 0.0 < lost[1] <= 1.25 * lost[0] + 2.0 ** -24, lost
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_blocks_of_every_exponent(cuda_rt, dtype):
     """A block's exponents 30 binades apart lose nothing in FP16; blocks of very different size do not meet."""
     codes, _ = tape_of(512, 160, 1)
