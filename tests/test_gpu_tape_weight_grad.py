@@ -249,6 +249,51 @@ def test_nothing_depends_on_what_the_workspace_held(cuda_rt, case, dtype):
         assert torch.equal(cuda_rt.tape_weight_grad(tape, gy), want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_graph_replayed_with_other_inputs(cuda_rt, dtype):
+    """Which stretches need more than FP16 is known on the device only; and whatever lies in the workspace, nothing of it shows."""
+    def inputs(seed, far):
+        codes, exponents = tape_of(1400, 264, seed)
+        exponents[600] += far                    # rows 512 .. 1023
+        gy = torch.randn(1400, 96, device="cuda").to(TYPES[dtype])
+        gy[600] = 0.0
+        return [codes, exponents, gy]
+
+    cases = [inputs(1, 0), inputs(2, 60), inputs(3, 0)]
+    want = [cuda_rt.tape_weight_grad((c, e), gy) for c, e, gy in cases]
+    held = [t.clone() for t in cases[0]]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = cuda_rt.tape_weight_grad((held[0], held[1]), held[2])
+        dirt = torch.full((1 << 26,), 0xFF, dtype=torch.uint8, device="cuda")   # over what the call gave back
+    for k in (0, 1, 2, 1, 1, 0):
+        for t, v in zip(held, cases[k]):
+            t.copy_(v)
+        g.replay()
+        assert torch.equal(got, want[k])
+        close(got, cases[k][2], cases[k][:2])
+    del dirt
+
+
+def test_calls_on_two_streams_at_once(cuda_rt):
+    tape = [tape_of(9000, 512, seed) for seed in (1, 2)]
+    tape[1][1][77] += 60
+    gy = [torch.randn(9000, 384, device="cuda").half() for _ in range(2)]
+    gy[1][77] = 0.0
+    want = [cuda_rt.tape_weight_grad(t, g) for t, g in zip(tape, gy)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(cuda_rt.tape_weight_grad(tape[k], gy[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(x, want[k]) for x in got[k])
+    cuda_rt.synchronize()
+
+
 def test_norm_linear_and_head_together(cuda_rt):
     """Norm, linear and head of a small model from the 8-bit tape: every gradient as autograd gives it in 64 bits at the values that
     the tape keeps."""
