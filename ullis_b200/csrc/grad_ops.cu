@@ -102,10 +102,10 @@ void launch(const Stream& s, const char* what, const Operand& a, const Operand& 
 // How a product [M, N] over K is cut for `pairs` pairs: accumulators of 256 columns per pair (one or two) and ranges of K.
 // Estimated in k-blocks (256 x 256 x 64 on a pair, 0.3 us): rounds * (k-blocks + an epilogue nothing overlaps) and, with several
 // ranges, their sums written and read once more: at 8 TB/s for a product that runs alone, whose sums stay in L2 (2048 x 512 x 2048
-// takes 20.1 us in three ranges, 21.8 in one, which 4 TB/s would choose), at 4 TB/s for the head's two beside one another (at 8 a
-// ragged batch of 7655 x 256 x 10007, half of its rows not counted, takes 167 us instead of 137).
+// takes 20.9 us in four ranges, 21.2 in one, which 4 TB/s would choose), at 4 TB/s for the head's two beside one another (at 8 a
+// ragged batch of 7655 x 256 x 10007, half of its rows not counted, takes 148 us instead of 117).
 // Two accumulators fetch A half as often, which counts where the power limit sets the clock: a head of 16384 x 512 x 8192 takes
-// 500 us instead of 507 over seconds, 429 instead of 434 before the limit acts.
+// 487 us instead of 494 over seconds, 430 instead of 437 before the limit acts.
 // (two: a product of the head, else a SUM, whose ranges are whole stretches of K)
 // A product of the head has no more than LONGEST k-blocks in one accumulator, whose additions the tensor cores cut off: sums of 16 384
 // terms of one sign are 1.0e-4 too small, of 65 536 4.3e-4, and half a step of FP16 is 2.4e-4 to 4.9e-4.  (4096 x 512 x 131072, whose hidden
