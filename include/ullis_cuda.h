@@ -511,7 +511,10 @@ ULLIS_CUDA_API int32_t ullis_cuda_tape_weight_grad(ullis_cuda_runtime* rt, void*
  * only) and g_bias [vocab] f32, both nullable.  log sum exp, losses and the sums
  * behind g_scale and g_bias are f32; g * scale is rounded to hidden's type for the
  * two gradient products, which accumulate in f32, at most 16384 terms at a time on the
- * tensor cores, which cut off (1e-4 of a sum of one sign).  What rows hold that do not count
+ * tensor cores, which cut off (1e-4 of a sum of one sign).  So do the logits but the
+ * target's, which is added with rounding: terms of one sign come out 1e-6 of their sum
+ * too small at 1024 channels, as far off as f32 sums, 3e-6 at 2048, 3e-5 at 8192, and
+ * the row's loss by that times the logit.  What rows hold that do not count
  * (infinities, NaN) has no effect.  A label outside the vocabulary makes its row's
  * loss NaN and gives no gradient.  Rows must be a multiple of `time`, at most 2^24.
  * copies_weight: 1 for a packed head, and for a dense one whose rows do not all start
