@@ -93,6 +93,7 @@ void launch(const Stream& s, const char* what, const Operand& a, const Operand& 
     p.a_mn = a.mn;
     p.b_mn = b.mn;
     p.stages = pg::stages_for(EPI, ACCS);
+    p.pairs_ok = p.N % 2 == 0 && (!(EPI == pg::SUM || p.out_f32) || aligned(p.out, 8));   // (all others are parts of the workspace)
     p.status = s.status;
     const pg::Maps maps{operand_map(a, bf16), operand_map(b, bf16), out ? *out : CUtensorMap{}};
     if (bf16) launch_form<EPI, ACCS, true>(s, what, maps, p, pairs);
@@ -102,7 +103,7 @@ void launch(const Stream& s, const char* what, const Operand& a, const Operand& 
 // How a product [M, N] over K is cut for `pairs` pairs: accumulators of 256 columns per pair (one or two) and ranges of K.
 // Estimated in k-blocks (256 x 256 x 64 on a pair, 0.3 us): rounds * (k-blocks + an epilogue nothing overlaps) and, with several
 // ranges, their sums written and read once more: at 8 TB/s for a product that runs alone, whose sums stay in L2 (2048 x 512 x 2048
-// takes 20.9 us in four ranges, 21.2 in one, which 4 TB/s would choose), at 4 TB/s for the head's two beside one another (at 8 a
+// takes 1.5 % less in four ranges than in one, which 4 TB/s would choose), at 4 TB/s for the head's two beside one another (at 8 a
 // ragged batch of 7655 x 256 x 10007, half of its rows not counted, takes 148 us instead of 117).
 // Two accumulators fetch A half as often, which counts where the power limit sets the clock: a head of 16384 x 512 x 8192 takes
 // 487 us instead of 494 over seconds, 430 instead of 437 before the limit acts.
@@ -883,7 +884,8 @@ struct GyRows {   // gy [rows, O] as two bf16 matrices side by side, [rows, 2 Op
 template <bool VEC, bool BYTES8>
 __global__ void __launch_bounds__(THREADS)
 tape_operand_f16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, uint32_t rows, uint32_t C, uint32_t Cp,
-                        uint16_t* __restrict__ out, float* __restrict__ col_factor, uint32_t* __restrict__ parts, const GyRows gy) {
+                        uint16_t* __restrict__ out, float* __restrict__ col_factor, uint8_t* __restrict__ parts, uint32_t parts_pitch,
+                        const GyRows gy) {
     chain_entry();
     const uint32_t tiles = (C + pg::BN - 1) / pg::BN, blocks = (C + 31) / 32;
     const uint32_t tile = blockIdx.x % tiles, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b0 = tile * 8;
@@ -944,7 +946,7 @@ tape_operand_f16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __rest
     if (first % STRETCH == 0 && threadIdx.x < 8) {
         if (b0 + lane < blocks)
             col_factor[stretch * blocks + b0 + lane] = exact || largest == tape::NOT_FINITE ? 1.0f : exp2f((float)((int)largest - 127 - 8));
-        if (lane == 0) parts[stretch * tiles + tile] = exact;
+        if (lane == 0) parts[(size_t)tile * parts_pitch + stretch] = exact;
     }
     if (exact) gy.in_parts(first, min(first + F16_ROWS, (size_t)rows));
     const uint32_t own = __shfl_sync(0xffffffffu, largest, lane >> 2);   // the largest of this thread's block
@@ -983,7 +985,7 @@ rows16_kernel(const uint16_t* __restrict__ x, size_t stride, uint32_t rows, uint
 struct WeightPlan {
     size_t ip, op;
     Cut cut;
-    size_t x16, gy16, gy_parts, col_factor, parts, partial, bytes;
+    size_t x16, gy16, gy_parts, col_factor, parts_pitch, parts, partial, bytes;
 };
 WeightPlan weight_plan(const ullis_cuda_runtime* rt, size_t rows, size_t in, size_t out) {
     WeightPlan p{};
@@ -995,7 +997,8 @@ WeightPlan weight_plan(const ullis_cuda_runtime* rt, size_t rows, size_t in, siz
     p.gy16 = at.add(rows * p.op * 2);
     p.gy_parts = at.add(rows * 2 * p.op * 2);
     p.col_factor = at.add(ceil_div(rows, STRETCH) * tape::blocks_of(in) * 4);
-    p.parts = at.add(ceil_div(rows, STRETCH) * ceil_div(in, pg::BN) * 4);
+    p.parts_pitch = up(ceil_div(rows, STRETCH), 8);
+    p.parts = at.add(p.parts_pitch * ceil_div(in, pg::BN));
     p.partial = at.add(partial_bytes(out, in, p.cut));
     p.bytes = at.bytes;
     return p;
@@ -1015,7 +1018,7 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
     uint16_t* x16 = reinterpret_cast<uint16_t*>(ws + p.x16);
     uint16_t* gy16 = reinterpret_cast<uint16_t*>(ws + p.gy16);
     float* col_factor = reinterpret_cast<float*>(ws + p.col_factor);
-    uint32_t* parts = reinterpret_cast<uint32_t*>(ws + p.parts);
+    uint8_t* parts = ws + p.parts;
     Operand a{gy.data, rows, out, gy.stride, true};
     uint16_t* gy_parts = reinterpret_cast<uint16_t*>(ws + p.gy_parts);
     if (!aligned(gy.data, 16) || gy.stride % 8) {
@@ -1033,7 +1036,7 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
         const auto operand = vec ? (bytes8 ? tape_operand_f16_kernel<true, true> : tape_operand_f16_kernel<true, false>)
                                  : (bytes8 ? tape_operand_f16_kernel<false, true> : tape_operand_f16_kernel<false, false>);
         s.chain("tape_operand", operand, (unsigned)(ceil_div(rows, F16_ROWS) * ceil_div(in, pg::BN)), THREADS, 0, codes, exponents, (uint32_t)rows,
-                (uint32_t)in, (uint32_t)p.ip, x16, col_factor, parts,
+                (uint32_t)in, (uint32_t)p.ip, x16, col_factor, parts, (uint32_t)p.parts_pitch,
                 GyRows{static_cast<const uint16_t*>(gy.data), gy.stride, (uint32_t)out, (uint32_t)p.op, gy_parts});
     }
     const Operand b{x16, rows, in, p.ip, true};
@@ -1047,6 +1050,7 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
     if (!bf16) {
         q.col_factor = col_factor;
         q.parts = parts;
+        q.parts_pitch = (uint32_t)p.parts_pitch;
         q.parts_at = (uint32_t)p.op;
     }
     const CUtensorMap in_parts = operand_map(Operand{gy_parts, rows, 2 * p.op, 2 * p.op, true}, true);

@@ -87,12 +87,14 @@ struct Params {
     float* accum;              // f32 [M][N]; STORE: read first if `accum_read`, written unless `out` is
     uint32_t accum_read;
     float* partial;            // splits > 1: [split][M][N]
-    // SUM, FP16: for each stretch of K and 32 columns what its sums are multiplied by, [stretch][ceil(N / 32)], and for each stretch
-    // and tile of columns, [stretch][n_tiles], a word that is not 0 where B lies there in bf16 instead of FP16: A is then the sum of two
-    // bf16 matrices, columns [0, M) and [parts_at, parts_at + M) of maps.out, and the product goes through the stretch once with each
+    uint32_t pairs_ok;         // two columns of every row of its f32 arrays lie on 8 bytes (`out` is aligned to its elements only)
+    // SUM, FP16: for each stretch of K and 32 columns what its sums are multiplied by, [stretch][ceil(N / 32)], and for each tile of
+    // columns and stretch, [n_tiles][parts_pitch, a multiple of 8], a byte that is not 0 where B lies there in bf16 instead of FP16: A is
+    // then the sum of two bf16 matrices, columns [0, M) and [parts_at, parts_at + M) of maps.out, and the product goes through the
+    // stretch once with each
     const float* col_factor;
-    const uint32_t* parts;
-    uint32_t parts_at;
+    const uint8_t* parts;
+    uint32_t parts_pitch, parts_at;
 };
 
 inline uint32_t stage_bytes(int accs) { return OPERAND_BYTES * (1 + accs); }
@@ -139,9 +141,8 @@ struct Work {
         if (EPI == LSE) open(m_tiles, min(p.piece_tiles, n_tiles));
         if (EPI == GRAD) open(n_tiles, m_tiles);
     }
-    // where the stretch from k-block kb on ends (STORE: the range), and whether A comes in two parts there
+    // where the stretch from k-block kb on ends (STORE: the range)
     __device__ uint32_t stretch_end(uint32_t kb) const { return EPI == SUM ? min(k1, kb + SUM_BLOCKS) : k1; }
-    __device__ bool in_parts(uint32_t kb) const { return kb < k1 && p.parts[kb / SUM_BLOCKS * n_tiles + n]; }
     __device__ void open(uint32_t outers, uint32_t inners) {
         const Share s = share_of(outers * inners, pairs);
         width = inners;
@@ -179,6 +180,21 @@ struct Work {
     }
 };
 
+// Whether A comes in two parts in the stretch of k-block kb of a tile: eight stretches to a load (one each took 6 of 113 us at 16384 x
+// 2048 -> 2048, whatever the distance between the load and its use).
+struct InParts {
+    uint64_t eight = 0;
+    uint32_t held = 0xFFFFFFFFu;
+    __device__ bool operator()(const Params& p, uint32_t n, uint32_t kb) {
+        const uint32_t stretch = kb / SUM_BLOCKS;
+        if (stretch / 8 != held) {
+            held = stretch / 8;
+            eight = *reinterpret_cast<const uint64_t*>(p.parts + (size_t)n * p.parts_pitch + held * 8);
+        }
+        return (eight >> 8 * (stretch % 8) & 0xFFu) != 0;
+    }
+};
+
 // 16 lanes x 64 columns: register 4 j + i of thread t has row t / 4 + 8 (i / 2), column 8 j + 2 (t % 4) + i % 2
 __device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
@@ -192,7 +208,15 @@ __device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32])
         : "r"(taddr));
 }
 
-// the same, 16 columns
+// the same, 32 and 16 columns
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_ld_16x16(uint32_t taddr, uint32_t (&r)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
@@ -312,11 +336,6 @@ __device__ __forceinline__ void report_wait(volatile uint32_t* status, uint32_t 
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// Whether two columns of every row of an f32 array of `columns` lie on 8 bytes: a caller's array is aligned to its elements only.
-__device__ __forceinline__ bool rows_of_pairs(const void* array, uint32_t columns) {
-    return (columns & 1) == 0 && (reinterpret_cast<uintptr_t>(array) & 7) == 0;
-}
-
 // Scale and bias (FP16, two lanes' worth: columns lane and 32 + lane) of 64 columns from n0 on, on their way while the tile before
 // is worked on; and as the constants that the epilogue reads: both times log2 e.  Columns past N have a probability of 0.
 struct Columns {
@@ -432,15 +451,14 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     ++it;
                 };
                 if constexpr (BY_STRETCH) {
-                    bool parts = work.in_parts(work.k0);
+                    InParts in_parts;
                     for (uint32_t from = work.k0; from < work.k1 && ok;) {
                         const uint32_t last = work.stretch_end(from);
-                        const bool ahead = work.in_parts(last);
+                        const bool parts = in_parts(p, work.n, from);
                         for (uint32_t kb = from; kb < last && ok; ++kb) fetch(kb, parts ? &maps.out : &maps.a, m0);
                         if (parts)
                             for (uint32_t kb = from; kb < last && ok; ++kb) fetch(kb, &maps.out, m0 + (int32_t)p.parts_at);
                         from = last;
-                        parts = ahead;
                     }
                 } else {
                     for (uint32_t kb = work.k0; kb < work.k1; ++kb) {
@@ -468,10 +486,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             uint32_t it = 0, done = 0;   // k-blocks, accumulators
             bool ok = true;
             while (ok && work.next()) {
-                bool parts = BY_STRETCH && work.in_parts(work.k0);   // this stretch's products in bf16, and twice as many
+                InParts in_parts;
                 for (uint32_t kb = work.k0; kb < work.k1 && ok;) {
+                    const bool parts = BY_STRETCH && in_parts(p, work.n, kb);   // this stretch's products in bf16, and twice as many
                     const uint32_t last = EPI == SUM ? work.stretch_end(kb) : work.k1, idesc = BY_STRETCH && parts ? idesc_bf16 : idesc_own;
-                    const bool ahead = BY_STRETCH && work.in_parts(last);
                     const uint32_t end = BY_STRETCH && parts ? 2 * last - kb : last;
                     const uint32_t buf = done % BUFFERS;
                     if (done >= BUFFERS && !wait(&tmem_empty[buf], ((done / BUFFERS) & 1u) ^ 1u, s_error)) {
@@ -505,10 +523,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     }
                     ptx::mma_commit_pair(&tmem_full[buf]);   // on the way out too: the epilogues do not wait in vain
                     ++done;
-                    if (BY_STRETCH) {
-                        kb = last;
-                        parts = ahead;
-                    }
+                    if (BY_STRETCH) kb = last;
                 }
             }
         }
@@ -757,7 +772,6 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             leave();
         } else if constexpr (EPI == STORE) {
             const float alpha = p.factor ? *p.factor : 1.0f;
-            const bool pairs_ok = rows_of_pairs(p.out_f32 ? p.out : nullptr, p.N);   // (the other f32 arrays lie in the workspace)
             const bool wide = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
             uint16_t* out = static_cast<uint16_t*>(p.out);
             while (work.next()) {
@@ -789,7 +803,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             for (int j = 0; j < 8; ++j) {
                                 const uint32_t c = n0 + j * 8 + q2;
                                 float &x = v[j * 4 + i * 2], &y = v[j * 4 + i * 2 + 1];
-                                if (pairs_ok) {
+                                if (p.pairs_ok) {
                                     if (c < p.N) {
                                         float2* both = reinterpret_cast<float2*>(line + c);
                                         if (read) { const float2 old = *both; x += old.x; y += old.y; }
@@ -850,21 +864,20 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     ok = filled(&taddr);
                     if (!ok) break;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t r[32];
-                        tmem_ld_16x64(taddr + group * 64 + ((h * 16) << 16), r);
-                        ptx::tmem_ld_wait();
-                        if (h == 1) drained();
+                    for (int part = 0; part < 4; ++part) {   // 16 rows of 32 columns: with 64 at a time registers spill (47.5 us, so 45.8)
+                        uint32_t r[16];
+                        tmem_ld_16x32(taddr + group * 64 + (part & 1) * 32 + ((part >> 1) * 16 << 16), r);
+                        tmem_landed(r);
+                        if (part == 3) drained();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float& sum = v[h * 32 + i];
-                            sum = BY_STRETCH ? fmaf(__uint_as_float(r[i]), f[i >> 4], sum) : sum + __uint_as_float(r[i]);   // (f: powers of two)
+                        for (int i = 0; i < 16; ++i) {
+                            float& sum = v[part * 16 + i];
+                            sum = BY_STRETCH ? fmaf(__uint_as_float(r[i]), f[part & 1], sum) : sum + __uint_as_float(r[i]);   // (f: powers of two)
                         }
                     }
                 }
                 if (!ok) break;
                 float* out = p.splits > 1 ? p.partial + (size_t)work.split * p.M * p.N : static_cast<float*>(p.out);
-                const bool pairs_ok = rows_of_pairs(out, p.N);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t row = m0 + r0 + i * 8;
@@ -875,7 +888,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         const uint32_t c = n0 + j * 8 + q2;
                         const int at = (i >> 1) * 32 + j * 4 + (i & 1) * 2;
                         const float x = v[at], y = v[at + 1];
-                        if (pairs_ok) {
+                        if (p.pairs_ok) {
                             if (c < p.N) *reinterpret_cast<float2*>(line + c) = make_float2(x, y);
                         } else {
                             if (c < p.N) line[c] = x;

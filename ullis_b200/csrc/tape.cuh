@@ -176,9 +176,11 @@ __device__ __forceinline__ void raw_codes(const uint8_t* codes, uint32_t c, uint
             }
         }
     } else {
+        uint32_t t[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (c + i < C) w[i >> 2] |= (uint32_t)codes[c + i] << (8 * (i & 3));
+        for (int i = 0; i < N; ++i) t[i] = c + i < C ? codes[c + i] : 0u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i >> 2] |= t[i] << (8 * (i & 3));
     }
 }
 template <bool VEC, int N>
