@@ -497,6 +497,26 @@ ULLIS_CUDA_API int32_t ullis_cuda_tape_weight_grad(ullis_cuda_runtime* rt, void*
                                                    size_t gy_stride, size_t rows, size_t in_features, size_t out_features,
                                                    float* g, void* workspace, size_t workspace_bytes);
 
+/* Embedding lookup (UllisHeron::hidden's first step, src/model.rs:2644-2664): y
+ * [rows, channels] (dtype) = scale * table[tokens[row]], rounded once from f32; table
+ * [vocab, channels] of table_dtype.  The row of `ignore_id` is zero, that of any other
+ * token outside the vocabulary NaN. */
+ULLIS_CUDA_API int32_t ullis_cuda_embed(ullis_cuda_runtime* rt, void* cuda_stream, int32_t table_dtype, const void* table,
+                                        size_t table_stride, const uint32_t* tokens, uint32_t ignore_id, float scale,
+                                        size_t rows, size_t channels, size_t vocab, int32_t dtype, void* y);
+/* Its gradient (src/model.rs:2980-2987): g [vocab, channels] f32 = scale * the sum of
+ * gy [rows, channels] (dtype) over the rows with that token, zero for tokens that none
+ * has; rows of ignore_id and of tokens outside the vocabulary count for nothing, and gy
+ * is not read there.  Tokens are sorted on the device; sums are f32, a token's rows in
+ * rising order in pieces that depend on the sizes and on where its rows lie among the
+ * sorted ones alone, so that a call gives the same result every time. */
+ULLIS_CUDA_API int32_t ullis_cuda_embed_grad_workspace(const ullis_cuda_runtime* rt, int32_t dtype, size_t rows,
+                                                       size_t channels, size_t vocab, size_t* bytes);
+ULLIS_CUDA_API int32_t ullis_cuda_embed_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const uint32_t* tokens,
+                                             uint32_t ignore_id, const void* gy, size_t gy_stride, size_t rows,
+                                             size_t channels, size_t vocab, float scale, float* g, void* workspace,
+                                             size_t workspace_bytes);
+
 /* Next-token cross-entropy of a head with its gradient and without logits
  * (apply_head_ce, src/model.rs:3132-3275; row rule src/model.rs:27-39): row m counts
  * unless it is the last of its `time` rows or labels[m + 1] == ignore_id.

@@ -524,6 +524,45 @@ unsafe extern "C" {
         workspace: *mut c_void,
         workspace_bytes: usize,
     ) -> i32;
+    pub fn ullis_cuda_embed(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        table_dtype: i32,
+        table: *const c_void,
+        table_stride: usize,
+        tokens: *const u32,
+        ignore_id: u32,
+        scale: f32,
+        rows: usize,
+        channels: usize,
+        vocab: usize,
+        dtype: i32,
+        y: *mut c_void,
+    ) -> i32;
+    pub fn ullis_cuda_embed_grad_workspace(
+        rt: *const ullis_cuda_runtime,
+        dtype: i32,
+        rows: usize,
+        channels: usize,
+        vocab: usize,
+        bytes: *mut usize,
+    ) -> i32;
+    pub fn ullis_cuda_embed_grad(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        dtype: i32,
+        tokens: *const u32,
+        ignore_id: u32,
+        gy: *const c_void,
+        gy_stride: usize,
+        rows: usize,
+        channels: usize,
+        vocab: usize,
+        scale: f32,
+        g: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+    ) -> i32;
     pub fn ullis_cuda_head_ce_grad_workspace(
         rt: *const ullis_cuda_runtime,
         rows: usize,

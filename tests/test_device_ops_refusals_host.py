@@ -1,0 +1,40 @@
+"""What the Python layer of embedding, top logits and distillation refuses before it calls the library; no device needed."""
+import numpy as np
+import pytest
+import torch
+
+from test_device_ops_host import Fake
+
+from ullis_b200 import cuda
+
+H, F, I32 = torch.float16, torch.float32, torch.int32
+
+
+def ids(*shape):
+    return torch.zeros(*shape, dtype=I32)
+
+
+REFUSED = {
+    "embed: an array": (lambda rt: rt.embed(np.zeros((4, 64), np.float32), ids(3)), cuda.ERR_ARG),
+    "embed: table's type": (lambda rt: rt.embed(torch.zeros(4, 64, dtype=torch.float64), ids(3)), cuda.ERR_ARG),
+    "embed: table's dimensions": (lambda rt: rt.embed(torch.zeros(2, 4, 64), ids(3)), cuda.ERR_SHAPE),
+    "embed: a transposed table": (lambda rt: rt.embed(torch.zeros(64, 4).t(), ids(3)), cuda.ERR_SHAPE),
+    "embed: 64-bit tokens": (lambda rt: rt.embed(torch.zeros(4, 64), ids(3).long()), cuda.ERR_ARG),
+    "embed: tokens on another device": (lambda rt: rt.embed(torch.zeros(4, 64), torch.zeros(3, dtype=I32, device="meta")), cuda.ERR_ARG),
+    "embed: tokens with gaps": (lambda rt: rt.embed(torch.zeros(4, 64), ids(6)[::2]), cuda.ERR_SHAPE),
+    "embed: to integers": (lambda rt: rt.embed(torch.zeros(4, 64), ids(3), dtype=I32), cuda.ERR_ARG),
+    "embed: ignore_id": (lambda rt: rt.embed(torch.zeros(4, 64), ids(3), ignore_id=1 << 32), cuda.ERR_ARG),
+    "embed gradient: tokens": (lambda rt: rt.embed_grad(ids(5), torch.zeros(4, 64), 9), cuda.ERR_SHAPE),
+    "embed gradient: 64-bit tokens": (lambda rt: rt.embed_grad(ids(4).long(), torch.zeros(4, 64), 9), cuda.ERR_ARG),
+    "embed gradient: gy's type": (lambda rt: rt.embed_grad(ids(4), torch.zeros(4, 64, dtype=torch.float64), 9), cuda.ERR_ARG),
+    "embed gradient: one dimension": (lambda rt: rt.embed_grad(ids(4), torch.zeros(4), 9), cuda.ERR_SHAPE),
+    "embed gradient: no vocabulary": (lambda rt: rt.embed_grad(ids(4), torch.zeros(4, 64), 0), cuda.ERR_SHAPE),
+    "embed gradient: ignore_id": (lambda rt: rt.embed_grad(ids(4), torch.zeros(4, 64), 9, ignore_id=-(1 << 31) - 1), cuda.ERR_ARG),
+}
+
+
+@pytest.mark.parametrize("call,code", REFUSED.values(), ids=REFUSED.keys())
+def test_refused_before_the_library_is_called(call, code):
+    with pytest.raises(cuda.UllisCudaError) as e:
+        call(Fake())
+    assert e.value.code == code

@@ -110,6 +110,15 @@ void need_product(size_t rows, size_t in_features, size_t out_features) {
     need_sizes(rows, out_features, what);
     need_tiles(out_features, in_features, what);
 }
+void need_embed(size_t rows, size_t channels, size_t vocab) {
+    const char* what = "embedding";
+    need_sizes(rows, channels, what);
+    if (vocab == 0) fail(ULLIS_CUDA_ERR_SHAPE, "embedding dimensions must be non-zero");
+    if (vocab >= (size_t)1 << 31) fail(ULLIS_CUDA_ERR_SHAPE, "embedding shape overflow");
+}
+void need_scale(float scale) {
+    if (!std::isfinite(scale)) fail(ULLIS_CUDA_ERR_ARG, "scale is not finite");
+}
 void need_head(size_t rows, size_t channels, size_t vocab) {
     const char* what = "head cross-entropy";
     need_sizes(rows, channels, what);
@@ -235,6 +244,51 @@ int32_t ullis_cuda_tape_weight_grad(ullis_cuda_runtime* rt, void* cuda_stream, i
         need_workspace(workspace, workspace_bytes, dev::tape_weight_grad_workspace(rt, rows, in_features, out_features));
         need_sm100(rt);
         dev::tape_weight_grad(s, dtype, codes, exponents, dev::Rows{gy, gy_stride}, rows, in_features, out_features, g, workspace);
+    });
+}
+
+int32_t ullis_cuda_embed(ullis_cuda_runtime* rt, void* cuda_stream, int32_t table_dtype, const void* table, size_t table_stride,
+                         const uint32_t* tokens, uint32_t ignore_id, float scale, size_t rows, size_t channels, size_t vocab, int32_t dtype,
+                         void* y) {
+    return on_stream(rt, cuda_stream, [&](const dev::Stream& s) {
+        need_dtype(table_dtype, true);
+        need_dtype(dtype, true);
+        need_embed(rows, channels, vocab);
+        need_stride(table_stride, channels, "table");
+        need_scale(scale);
+        if (rows == 0) return;
+        need_array(table, "table", dev::size_of(table_dtype));
+        need_array(tokens, "tokens", 4);
+        need_array(y, "y", dev::size_of(dtype));
+        dev::embed(s, table_dtype, dev::Rows{table, table_stride}, tokens, ignore_id, scale, rows, channels, vocab, dtype, y);
+    });
+}
+
+int32_t ullis_cuda_embed_grad_workspace(const ullis_cuda_runtime* rt, int32_t dtype, size_t rows, size_t channels, size_t vocab, size_t* bytes) {
+    return workspace_of(rt, bytes, [&] {
+        need_dtype(dtype, true);
+        need_embed(rows, channels, vocab);
+        return dev::embed_grad_workspace(rt, dtype, rows, channels);
+    });
+}
+
+int32_t ullis_cuda_embed_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const uint32_t* tokens, uint32_t ignore_id,
+                              const void* gy, size_t gy_stride, size_t rows, size_t channels, size_t vocab, float scale, float* g,
+                              void* workspace, size_t workspace_bytes) {
+    return on_stream(rt, cuda_stream, [&](const dev::Stream& s) {
+        need_dtype(dtype, true);
+        need_embed(rows, channels, vocab);
+        need_stride(gy_stride, channels, "gy");
+        need_scale(scale);
+        need_array(g, "g", 4);
+        if (rows == 0) {
+            ULLIS_CUDA_CHECK(cudaMemsetAsync(g, 0, vocab * channels * 4, s.stream));
+            return;
+        }
+        need_array(tokens, "tokens", 4);
+        need_array(gy, "gy", dev::size_of(dtype));
+        need_workspace(workspace, workspace_bytes, dev::embed_grad_workspace(rt, dtype, rows, channels));
+        dev::embed_grad(s, dtype, tokens, ignore_id, dev::Rows{gy, gy_stride}, rows, channels, vocab, scale, g, workspace);
     });
 }
 

@@ -60,6 +60,9 @@ _ARGTYPES = {
     "tape_layer_norm_backward": (_V, _V, _I, _V, _V, _V, _Z, _V, _V, _Z, _Z, _Z, _V, _V, _V, _V, _Z),
     "tape_weight_grad_workspace": (_V, _Z, _Z, _Z, _V),
     "tape_weight_grad": (_V, _V, _I, _V, _V, _V, _Z, _Z, _Z, _Z, _V, _V, _Z),
+    "embed": (_V, _V, _I, _V, _Z, _V, _U, _F, _Z, _Z, _Z, _I, _V),
+    "embed_grad_workspace": (_V, _I, _Z, _Z, _Z, _V),
+    "embed_grad": (_V, _V, _I, _V, _U, _V, _Z, _Z, _Z, _Z, _F, _V, _V, _Z),
     "head_ce_grad_workspace": (_V, _Z, _Z, _Z, _I, _V),
     "head_ce_grad": (_V, _V, _I, _V, _Z, _V, _V, _V, _V, _V, _U, _Z, _Z, _Z, _Z, _F, _V, _V, _V, _V, _V, _V, _Z),
 }
@@ -77,6 +80,13 @@ def _p(t):
 def _like(t, dtype):
     """An output of t's shape, without gaps.  (Sizes as single numbers: torch takes a tuple of them twice as long.)"""
     return _TORCH.empty_like(t, dtype=dtype) if t.is_contiguous() else _TORCH.empty(*t.shape, dtype=dtype, device=t.device)
+
+
+def _id32(ignore_id):
+    ignore = int(ignore_id)
+    if not -(1 << 31) <= ignore < 1 << 32:
+        raise UllisCudaError(ERR_ARG, "ignore_id is not a 32-bit number")
+    return ignore & 0xFFFFFFFF
 
 
 def _shape_error(name, got, expected):
@@ -122,6 +132,12 @@ class DeviceOps:
             raise UllisCudaError(ERR_SHAPE, f"{name} must not have overlapping rows")
         return rows, channels, stride
 
+    def _ids(self, t, name):
+        """int32 without gaps, of any shape."""
+        self._refuse(t, name, _I32)
+        if not t.is_contiguous():
+            raise UllisCudaError(ERR_SHAPE, f"{name} must be contiguous")
+
     def _vector(self, t, name, dtypes, n):
         try:
             if t.dtype in dtypes and self._on_device(t) and t.numel() == n and t.is_contiguous():
@@ -132,6 +148,12 @@ class DeviceOps:
         if t.numel() != n:
             _shape_error(name, t.shape, (n,))
         raise UllisCudaError(ERR_SHAPE, f"{name} must be contiguous")
+
+    def _table(self, table):
+        vocab, channels, stride = self._matrix(table, "table", _DTYPES)
+        if table.dim() != 2:
+            raise UllisCudaError(ERR_SHAPE, "table must have two dimensions")
+        return vocab, channels, stride
 
     def _tape(self, tape):
         _torch()
@@ -235,6 +257,42 @@ class DeviceOps:
         self._check(self._lib.ullis_cuda_tape_weight_grad(
             self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], codes.data_ptr(), exponents.data_ptr(), gy.data_ptr(), stride, rows,
             channels, out, g.data_ptr(), work.data_ptr(), size))
+        return g
+
+    # ------------------------------------------------------------------------------------------ embedding
+    def embed(self, table, tokens, *, scale: float = 1.0, dtype=None, ignore_id: int = 0xFFFFFFFF):
+        """scale * table[tokens], [*tokens.shape, channels] in `dtype` (default: the table's type).
+
+        table [vocab, channels] float32, float16 or bfloat16; tokens int32 of any shape (a negative id and `ignore_id` are taken as
+        the unsigned 32-bit number they are).  The row of `ignore_id` is zero, that of any other id outside the table NaN."""
+        torch = _torch()
+        vocab, channels, stride = self._table(table)
+        self._ids(tokens, "tokens")
+        dtype = table.dtype if dtype is None else dtype
+        if dtype not in _DTYPES:
+            raise UllisCudaError(ERR_ARG, f"an embedding has no type {dtype}")
+        y = torch.empty(*tokens.shape, channels, dtype=dtype, device=tokens.device)
+        self._check(self._lib.ullis_cuda_embed(
+            self._h, _RAW_STREAM(self.device), _DTYPES[table.dtype], table.data_ptr(), stride, tokens.data_ptr(), _id32(ignore_id),
+            float(scale), tokens.numel(), channels, vocab, _DTYPES[dtype], y.data_ptr()))
+        return y
+
+    def embed_grad(self, tokens, gy, vocab: int, *, scale: float = 1.0, ignore_id: int = 0xFFFFFFFF):
+        """Gradient of `embed`'s table, float32 [vocab, channels]: scale * the sum of gy [*tokens.shape, channels] (float32, float16,
+        bfloat16) over the rows of each token.  `ignore_id` and ids outside the table add nothing."""
+        torch = _torch()
+        rows, channels, stride = self._matrix(gy, "gy", _DTYPES)
+        self._ids(tokens, "tokens")
+        if tokens.numel() != rows:
+            _shape_error("tokens", tokens.shape, gy.shape[:-1])
+        vocab = int(vocab)
+        if vocab <= 0:
+            raise UllisCudaError(ERR_SHAPE, "vocab must be positive")
+        g = torch.empty(vocab, channels, dtype=torch.float32, device=gy.device)
+        work, size = self._workspace(gy, "embed_grad", _DTYPES[gy.dtype], rows, channels, vocab)
+        self._check(self._lib.ullis_cuda_embed_grad(
+            self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], tokens.data_ptr(), _id32(ignore_id), gy.data_ptr(), stride, rows,
+            channels, vocab, float(scale), g.data_ptr(), work.data_ptr(), size))
         return g
 
     # ------------------------------------------------------------------------------------------ head
