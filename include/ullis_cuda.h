@@ -517,6 +517,13 @@ ULLIS_CUDA_API int32_t ullis_cuda_embed_grad(ullis_cuda_runtime* rt, void* cuda_
                                              size_t channels, size_t vocab, float scale, float* g, void* workspace,
                                              size_t workspace_bytes);
 
+/* The k largest logits of every row, in falling order, equal ones (-0 and 0 are) by
+ * rising column: ids [rows, k] their columns, top [rows, k] (dtype) the logits (a -0
+ * comes back as 0).  NaN is above all others.  k is at least 1 and at most vocab and 256. */
+ULLIS_CUDA_API int32_t ullis_cuda_top_logits(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const void* logits,
+                                             size_t logits_stride, size_t rows, size_t vocab, size_t k, int32_t* ids,
+                                             void* top);
+
 /* Next-token cross-entropy of a head with its gradient and without logits
  * (apply_head_ce, src/model.rs:3132-3275; row rule src/model.rs:27-39): row m counts
  * unless it is the last of its `time` rows or labels[m + 1] == ignore_id.

@@ -563,6 +563,18 @@ unsafe extern "C" {
         workspace: *mut c_void,
         workspace_bytes: usize,
     ) -> i32;
+    pub fn ullis_cuda_top_logits(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        dtype: i32,
+        logits: *const c_void,
+        logits_stride: usize,
+        rows: usize,
+        vocab: usize,
+        k: usize,
+        ids: *mut i32,
+        top: *mut c_void,
+    ) -> i32;
     pub fn ullis_cuda_head_ce_grad_workspace(
         rt: *const ullis_cuda_runtime,
         rows: usize,

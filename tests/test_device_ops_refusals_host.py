@@ -30,6 +30,13 @@ REFUSED = {
     "embed gradient: one dimension": (lambda rt: rt.embed_grad(ids(4), torch.zeros(4), 9), cuda.ERR_SHAPE),
     "embed gradient: no vocabulary": (lambda rt: rt.embed_grad(ids(4), torch.zeros(4, 64), 0), cuda.ERR_SHAPE),
     "embed gradient: ignore_id": (lambda rt: rt.embed_grad(ids(4), torch.zeros(4, 64), 9, ignore_id=-(1 << 31) - 1), cuda.ERR_ARG),
+    "top: integers": (lambda rt: rt.top_logits(ids(4, 64), 3), cuda.ERR_ARG),
+    "top: one dimension": (lambda rt: rt.top_logits(torch.zeros(64), 3), cuda.ERR_SHAPE),
+    "top: none": (lambda rt: rt.top_logits(torch.zeros(4, 64), 0), cuda.ERR_SHAPE),
+    "top: more than there are": (lambda rt: rt.top_logits(torch.zeros(4, 64), 65), cuda.ERR_SHAPE),
+    "top: more than 256": (lambda rt: rt.top_logits(torch.zeros(4, 640), 257), cuda.ERR_SHAPE),
+    "top: rows on top of each other": (lambda rt: rt.top_logits(torch.zeros(1, 64).expand(4, 64), 3), cuda.ERR_SHAPE),
+    "top: transposed": (lambda rt: rt.top_logits(torch.zeros(64, 4).t(), 3), cuda.ERR_SHAPE),
 }
 
 

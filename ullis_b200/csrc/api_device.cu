@@ -1,5 +1,6 @@
 // extern "C" entry points of the operators on device memory (include/ullis_cuda.h): checks of the arguments, the caller's stream
 // and device.  No C++ exception leaves this file.
+#include <algorithm>
 #include <cmath>
 #include <exception>
 #include <new>
@@ -289,6 +290,22 @@ int32_t ullis_cuda_embed_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t
         need_array(gy, "gy", dev::size_of(dtype));
         need_workspace(workspace, workspace_bytes, dev::embed_grad_workspace(rt, dtype, rows, channels));
         dev::embed_grad(s, dtype, tokens, ignore_id, dev::Rows{gy, gy_stride}, rows, channels, vocab, scale, g, workspace);
+    });
+}
+
+int32_t ullis_cuda_top_logits(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const void* logits, size_t logits_stride, size_t rows,
+                              size_t vocab, size_t k, int32_t* ids, void* top) {
+    return on_stream(rt, cuda_stream, [&](const dev::Stream& s) {
+        need_dtype(dtype, true);
+        need_sizes(rows, vocab, "top logits");
+        if (k == 0 || k > vocab || k > dev::TOP_MOST)
+            fail(ULLIS_CUDA_ERR_SHAPE, "top logits: k must be at least 1 and at most " + std::to_string(std::min(vocab, dev::TOP_MOST)));
+        need_stride(logits_stride, vocab, "logits");
+        if (rows == 0) return;
+        need_array(logits, "logits", dev::size_of(dtype));
+        need_array(ids, "ids", 4);
+        need_array(top, "top", dev::size_of(dtype));
+        dev::top_logits(s, dtype, dev::Rows{logits, logits_stride}, rows, vocab, k, ids, top);
     });
 }
 

@@ -70,6 +70,10 @@ size_t embed_grad_workspace(const ullis_cuda_runtime* rt, int dtype, size_t rows
 void embed_grad(const Stream& s, int dtype, const uint32_t* tokens, uint32_t ignore_id, Rows gy, size_t rows, size_t channels, size_t vocab,
                 float scale, float* g, void* workspace);
 
+// ---- the k largest of every row in falling order, equal ones by rising column (top.cu): ids and out [rows, k]
+constexpr size_t TOP_MOST = 256;
+void top_logits(const Stream& s, int dtype, Rows logits, size_t rows, size_t vocab, size_t k, int32_t* ids, void* out);
+
 // ---- cross-entropy of a head with its gradient
 struct HeadGrad {
     int dtype;                 // of the products' operands, hidden and the gradients: F16 or BF16

@@ -22,7 +22,7 @@ import threading
 
 import numpy as np
 
-from .device import DeviceOps, HeadGrad, Tape, declare  # noqa: F401
+from .device import DeviceOps, HeadGrad, Tape, TopLogits, declare  # noqa: F401
 from .errors import (ERR_ARG, ERR_CHECKPOINT, ERR_CUDA, ERR_DEVICE_CHECK, ERR_NCCL, ERR_NOMEM, ERR_SHAPE,  # noqa: F401
                      ERR_TIMEOUT, ERR_TOKEN, OK, UllisCudaError)
 
@@ -66,7 +66,7 @@ ABI_SYMBOLS = (
     "ullis_cuda_tape_pack", "ullis_cuda_tape_unpack", "ullis_cuda_tape_layer_norm",
     "ullis_cuda_tape_layer_norm_backward_workspace", "ullis_cuda_tape_layer_norm_backward",
     "ullis_cuda_tape_weight_grad_workspace", "ullis_cuda_tape_weight_grad", "ullis_cuda_head_ce_grad_workspace",
-    "ullis_cuda_head_ce_grad",
+    "ullis_cuda_head_ce_grad", "ullis_cuda_embed", "ullis_cuda_embed_grad_workspace", "ullis_cuda_embed_grad", "ullis_cuda_top_logits",
 )
 
 

@@ -33,6 +33,13 @@ class HeadGrad(NamedTuple):
     bias: object
 
 
+class TopLogits(NamedTuple):
+    """ids int32 and logits (the type they were taken from) [..., k]."""
+
+    ids: object
+    logits: object
+
+
 _TORCH = _RAW_STREAM = None
 _DTYPES = _16 = _F16 = _I8 = _U8 = _I32 = None   # the types that arguments may have
 
@@ -63,6 +70,7 @@ _ARGTYPES = {
     "embed": (_V, _V, _I, _V, _Z, _V, _U, _F, _Z, _Z, _Z, _I, _V),
     "embed_grad_workspace": (_V, _I, _Z, _Z, _Z, _V),
     "embed_grad": (_V, _V, _I, _V, _U, _V, _Z, _Z, _Z, _Z, _F, _V, _V, _Z),
+    "top_logits": (_V, _V, _I, _V, _Z, _Z, _Z, _Z, _V, _V),
     "head_ce_grad_workspace": (_V, _Z, _Z, _Z, _I, _V),
     "head_ce_grad": (_V, _V, _I, _V, _Z, _V, _V, _V, _V, _V, _U, _Z, _Z, _Z, _Z, _F, _V, _V, _V, _V, _V, _V, _Z),
 }
@@ -271,10 +279,11 @@ class DeviceOps:
         dtype = table.dtype if dtype is None else dtype
         if dtype not in _DTYPES:
             raise UllisCudaError(ERR_ARG, f"an embedding has no type {dtype}")
+        ignore = _id32(ignore_id)
         y = torch.empty(*tokens.shape, channels, dtype=dtype, device=tokens.device)
         self._check(self._lib.ullis_cuda_embed(
-            self._h, _RAW_STREAM(self.device), _DTYPES[table.dtype], table.data_ptr(), stride, tokens.data_ptr(), _id32(ignore_id),
-            float(scale), tokens.numel(), channels, vocab, _DTYPES[dtype], y.data_ptr()))
+            self._h, _RAW_STREAM(self.device), _DTYPES[table.dtype], table.data_ptr(), stride, tokens.data_ptr(), ignore, float(scale),
+            tokens.numel(), channels, vocab, _DTYPES[dtype], y.data_ptr()))
         return y
 
     def embed_grad(self, tokens, gy, vocab: int, *, scale: float = 1.0, ignore_id: int = 0xFFFFFFFF):
@@ -285,15 +294,31 @@ class DeviceOps:
         self._ids(tokens, "tokens")
         if tokens.numel() != rows:
             _shape_error("tokens", tokens.shape, gy.shape[:-1])
-        vocab = int(vocab)
-        if vocab <= 0:
-            raise UllisCudaError(ERR_SHAPE, "vocab must be positive")
+        vocab, ignore = int(vocab), _id32(ignore_id)
+        if not 0 < vocab < 1 << 31:
+            raise UllisCudaError(ERR_SHAPE, "vocab must be positive and below 2^31")
         g = torch.empty(vocab, channels, dtype=torch.float32, device=gy.device)
         work, size = self._workspace(gy, "embed_grad", _DTYPES[gy.dtype], rows, channels, vocab)
         self._check(self._lib.ullis_cuda_embed_grad(
-            self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], tokens.data_ptr(), _id32(ignore_id), gy.data_ptr(), stride, rows,
+            self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], tokens.data_ptr(), ignore, gy.data_ptr(), stride, rows,
             channels, vocab, float(scale), g.data_ptr(), work.data_ptr(), size))
         return g
+
+    # ------------------------------------------------------------------------------------------ a teacher's logits
+    def top_logits(self, logits, k: int) -> TopLogits:
+        """The k largest of logits [..., vocab] (float32, float16, bfloat16) in falling order, equal ones by rising id; NaN is
+        above all others.  k at most 256."""
+        torch = _torch()
+        rows, vocab, stride = self._matrix(logits, "logits", _DTYPES)
+        k = int(k)
+        if not 0 < k <= min(vocab, 256):
+            raise UllisCudaError(ERR_SHAPE, f"top logits: k must be at least 1 and at most {min(vocab, 256)}")
+        shape = (*logits.shape[:-1], k)
+        ids = torch.empty(shape, dtype=torch.int32, device=logits.device)
+        top = torch.empty(shape, dtype=logits.dtype, device=logits.device)
+        self._check(self._lib.ullis_cuda_top_logits(self._h, _RAW_STREAM(self.device), _DTYPES[logits.dtype], logits.data_ptr(), stride,
+                                                    rows, vocab, k, ids.data_ptr(), top.data_ptr()))
+        return TopLogits(ids, top)
 
     # ------------------------------------------------------------------------------------------ head
     def head_ce_grad(self, hidden, weight, labels, *, scale=None, bias=None, ignore_id: int = 0xFFFFFFFF, time=None,
@@ -323,9 +348,7 @@ class DeviceOps:
             vocab = weight.shape[0]
         if bias is not None:
             self._vector(bias, "bias", _F16, vocab)
-        ignore, time = int(ignore_id), int(time)
-        if not -(1 << 31) <= ignore < 1 << 32:
-            raise UllisCudaError(ERR_ARG, "ignore_id is not a 32-bit number")
+        ignore, time = _id32(ignore_id), int(time)
         if not 0 < time < 1 << 31 or rows % time:
             raise UllisCudaError(ERR_SHAPE, "rows must be a multiple of time")
         row_loss = torch.empty(rows, dtype=torch.float32, device=hidden.device)
@@ -338,7 +361,7 @@ class DeviceOps:
         work, size = self._workspace(hidden, "head_ce_grad", rows, channels, vocab, int(copies))
         self._check(self._lib.ullis_cuda_head_ce_grad(
             self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], hidden.data_ptr(), stride, at if scale is not None else None,
-            at if scale is None else None, _p(scale), _p(bias), labels.data_ptr(), ignore & 0xFFFFFFFF, rows, time, channels, vocab,
+            at if scale is None else None, _p(scale), _p(bias), labels.data_ptr(), ignore, rows, time, channels, vocab,
             float(loss_scale), row_loss.data_ptr(), g_hidden.data_ptr(), g_weight.data_ptr(), _p(g_scale), _p(g_bias),
             work.data_ptr(), size))
         return HeadGrad(row_loss, g_hidden, g_weight, g_scale, g_bias)
