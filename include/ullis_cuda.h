@@ -557,6 +557,36 @@ ULLIS_CUDA_API int32_t ullis_cuda_head_ce_grad(ullis_cuda_runtime* rt, void* cud
                                                void* g_hidden, void* g_weight, float* g_scale, float* g_bias,
                                                void* workspace, size_t workspace_bytes);
 
+/* A head's distillation from a teacher's largest logits, with its gradient and without
+ * the student's logits.  Entries top_ids, top_logits [rows, top] (top_dtype; top at most
+ * 256) of a row m speak of the token after it; a negative id is no entry, an id that
+ * comes twice in a row has the sum of both probabilities, and a logit of -infinity has
+ * none.  With z as in ullis_cuda_head_ce_grad, T the temperature, p = softmax(top_logits
+ * / T) over the row's entries and y = labels[m + 1],
+ *   row_loss = (1 - alpha) * (log sum exp z - z[y])
+ *              + alpha * T^2 * sum p * (log p - z / T + log sum exp (z / T)),
+ *   g = loss_scale * ((1 - alpha) * (softmax(z) - onehot(y)) + alpha * T * (softmax(z / T) - p)).
+ * With labels a row counts as in ullis_cuda_head_ce_grad, for both parts; one without an
+ * entry above -infinity has the first part alone.  labels NULL: the second part alone,
+ * and a row counts if it has such an entry.  A row that counts and has an id of the
+ * vocabulary's size or above, or a logit of NaN or +infinity, has a loss of NaN and gives
+ * no gradient; negative ids' logits are not looked at.  alpha in 0 .. 1, temperature in
+ * 1/128 .. 128.  Arguments, outputs and limits otherwise as for ullis_cuda_head_ce_grad;
+ * the logits of entries keep what the tensor cores leave of them, and losses are sums of
+ * terms none of which is negative but alpha * T^2 * sum p * log p. */
+ULLIS_CUDA_API int32_t ullis_cuda_head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels,
+                                                              size_t vocab, size_t top, int32_t has_labels,
+                                                              int32_t copies_weight, size_t* bytes);
+ULLIS_CUDA_API int32_t ullis_cuda_head_distill_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype,
+                                                    const void* hidden, size_t hidden_stride, const uint32_t* bits,
+                                                    const void* weight, const uint16_t* scale, const uint16_t* bias,
+                                                    const int32_t* top_ids, int32_t top_dtype, const void* top_logits,
+                                                    size_t top, float alpha, float temperature, const uint32_t* labels,
+                                                    uint32_t ignore_id, size_t rows, size_t time, size_t channels,
+                                                    size_t vocab, float loss_scale, float* row_loss, void* g_hidden,
+                                                    void* g_weight, float* g_scale, float* g_bias, void* workspace,
+                                                    size_t workspace_bytes);
+
 /* ------------------------------------------------------------ data parallel
  * Sequences are independent; ranks own disjoint blocks of sequences and only
  * {loss_sum, n_valid} is summed across ranks (NCCL all-reduce, 16 bytes).

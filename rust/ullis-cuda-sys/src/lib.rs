@@ -608,6 +608,47 @@ unsafe extern "C" {
         workspace: *mut c_void,
         workspace_bytes: usize,
     ) -> i32;
+    pub fn ullis_cuda_head_distill_grad_workspace(
+        rt: *const ullis_cuda_runtime,
+        rows: usize,
+        channels: usize,
+        vocab: usize,
+        top: usize,
+        has_labels: i32,
+        copies_weight: i32,
+        bytes: *mut usize,
+    ) -> i32;
+    pub fn ullis_cuda_head_distill_grad(
+        rt: *mut ullis_cuda_runtime,
+        cuda_stream: *mut c_void,
+        dtype: i32,
+        hidden: *const c_void,
+        hidden_stride: usize,
+        bits: *const u32,
+        weight: *const c_void,
+        scale: *const u16,
+        bias: *const u16,
+        top_ids: *const i32,
+        top_dtype: i32,
+        top_logits: *const c_void,
+        top: usize,
+        alpha: f32,
+        temperature: f32,
+        labels: *const u32,
+        ignore_id: u32,
+        rows: usize,
+        time: usize,
+        channels: usize,
+        vocab: usize,
+        loss_scale: f32,
+        row_loss: *mut f32,
+        g_hidden: *mut c_void,
+        g_weight: *mut c_void,
+        g_scale: *mut f32,
+        g_bias: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+    ) -> i32;
     pub fn ullis_cuda_dp_unique_id(id: *mut u8) -> i32;
     pub fn ullis_cuda_dp_rendezvous(
         dir: *const c_char,

@@ -131,6 +131,43 @@ void need_head(size_t rows, size_t channels, size_t vocab) {
     need_tiles(vocab, channels, what);
 }
 
+// What both calls of a head ask of their arguments; false: no rows, and the sums over them are written.
+bool need_head_grad(const dev::Stream& s, const dev::HeadGrad& h) {
+    need_dtype(h.dtype, false);
+    need_head(h.rows, h.channels, h.vocab);
+    if (h.time == 0 || h.time >= ((size_t)1 << 31) || h.rows % h.time) fail(ULLIS_CUDA_ERR_SHAPE, "rows must be a multiple of time");
+    need_stride(h.hidden.stride, h.channels, "hidden");
+    if (!std::isfinite(h.loss_scale)) fail(ULLIS_CUDA_ERR_ARG, "loss_scale is not finite");
+    if ((h.bits != nullptr) == (h.weight != nullptr)) fail(ULLIS_CUDA_ERR_ARG, "a head is either packed (bits) or dense (weight)");
+    if ((h.bits != nullptr) != (h.scale != nullptr)) fail(ULLIS_CUDA_ERR_ARG, "a packed head has row scales, a dense one none");
+    if (h.g_scale && !h.scale) fail(ULLIS_CUDA_ERR_ARG, "g_scale without row scales");
+    if (h.bits) {
+        need_array(h.bits, "bits", 4);
+        need_array(h.scale, "scale", 2);
+    } else {
+        need_array(h.weight, "weight", 2);
+    }
+    if (h.bias) need_array(h.bias, "bias", 2);
+    need_array(h.g_weight, "g_weight", 2);
+    if (h.g_scale) need_array(h.g_scale, "g_scale", 4);
+    if (h.g_bias) need_array(h.g_bias, "g_bias", 4);
+    if (h.rows == 0) {
+        ULLIS_CUDA_CHECK(cudaMemsetAsync(h.g_weight, 0, h.vocab * h.channels * 2, s.stream));
+        if (h.g_scale) ULLIS_CUDA_CHECK(cudaMemsetAsync(h.g_scale, 0, h.vocab * 4, s.stream));
+        if (h.g_bias) ULLIS_CUDA_CHECK(cudaMemsetAsync(h.g_bias, 0, h.vocab * 4, s.stream));
+        return false;
+    }
+    need_array(h.hidden.data, "hidden", 2);
+    need_array(h.row_loss, "row_loss", 4);
+    need_array(h.g_hidden, "g_hidden", 2);
+    return true;
+}
+void need_distill(size_t top, float alpha, float temperature) {
+    if (top == 0 || top > dev::DISTILL_MOST) fail(ULLIS_CUDA_ERR_SHAPE, "head distillation takes 1 to 256 entries of a row");
+    if (!(alpha >= 0.0f && alpha <= 1.0f)) fail(ULLIS_CUDA_ERR_ARG, "alpha must be in 0 .. 1");
+    if (!(temperature >= 0.0078125f && temperature <= 128.0f)) fail(ULLIS_CUDA_ERR_ARG, "temperature must be in 1/128 .. 128");
+}
+
 }  // namespace
 
 extern "C" {
@@ -323,56 +360,44 @@ int32_t ullis_cuda_head_ce_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32
                                 float loss_scale, float* row_loss, void* g_hidden, void* g_weight, float* g_scale, float* g_bias,
                                 void* workspace, size_t workspace_bytes) {
     return on_stream(rt, cuda_stream, [&](const dev::Stream& s) {
-        need_dtype(dtype, false);
-        need_head(rows, channels, vocab);
-        if (time == 0 || time >= ((size_t)1 << 31) || rows % time) fail(ULLIS_CUDA_ERR_SHAPE, "rows must be a multiple of time");
-        need_stride(hidden_stride, channels, "hidden");
-        if (!std::isfinite(loss_scale)) fail(ULLIS_CUDA_ERR_ARG, "loss_scale is not finite");
-        if ((bits != nullptr) == (weight != nullptr)) fail(ULLIS_CUDA_ERR_ARG, "a head is either packed (bits) or dense (weight)");
-        if ((bits != nullptr) != (scale != nullptr)) fail(ULLIS_CUDA_ERR_ARG, "a packed head has row scales, a dense one none");
-        if (g_scale && !scale) fail(ULLIS_CUDA_ERR_ARG, "g_scale without row scales");
-        if (bits) {
-            need_array(bits, "bits", 4);
-            need_array(scale, "scale", 2);
-        } else {
-            need_array(weight, "weight", 2);
-        }
-        if (bias) need_array(bias, "bias", 2);
-        need_array(g_weight, "g_weight", 2);
-        if (g_scale) need_array(g_scale, "g_scale", 4);
-        if (g_bias) need_array(g_bias, "g_bias", 4);
-        if (rows == 0) {
-            ULLIS_CUDA_CHECK(cudaMemsetAsync(g_weight, 0, vocab * channels * 2, s.stream));
-            if (g_scale) ULLIS_CUDA_CHECK(cudaMemsetAsync(g_scale, 0, vocab * 4, s.stream));
-            if (g_bias) ULLIS_CUDA_CHECK(cudaMemsetAsync(g_bias, 0, vocab * 4, s.stream));
-            return;
-        }
-        need_array(hidden, "hidden", 2);
+        const dev::HeadGrad h{dtype, false,     false, false, {hidden, hidden_stride}, bits,     weight,   scale,    bias,    labels, ignore_id,
+                              rows,  time,      channels, vocab, loss_scale,           row_loss, g_hidden, g_weight, g_scale, g_bias};
+        if (!need_head_grad(s, h)) return;
         need_array(labels, "labels", 4);
-        need_array(row_loss, "row_loss", 4);
-        need_array(g_hidden, "g_hidden", 2);
         need_workspace(workspace, workspace_bytes, dev::head_ce_grad_workspace(rt, rows, channels, vocab, dev::head_copies_weight(weight, channels)));
         need_sm100(rt);
-        dev::HeadGrad h{};
-        h.dtype = dtype;
-        h.hidden = dev::Rows{hidden, hidden_stride};
-        h.bits = bits;
-        h.weight = weight;
-        h.scale = scale;
-        h.bias = bias;
-        h.labels = labels;
-        h.ignore_id = ignore_id;
-        h.rows = rows;
-        h.time = time;
-        h.channels = channels;
-        h.vocab = vocab;
-        h.loss_scale = loss_scale;
-        h.row_loss = row_loss;
-        h.g_hidden = g_hidden;
-        h.g_weight = g_weight;
-        h.g_scale = g_scale;
-        h.g_bias = g_bias;
         dev::head_ce_grad(s, h, workspace);
+    });
+}
+
+int32_t ullis_cuda_head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, size_t top,
+                                               int32_t has_labels, int32_t copies_weight, size_t* bytes) {
+    return workspace_of(rt, bytes, [&] {
+        need_head(rows, channels, vocab);
+        need_distill(top, 1.0f, 1.0f);
+        return dev::head_distill_grad_workspace(rt, rows, channels, vocab, top, has_labels != 0, copies_weight != 0);
+    });
+}
+
+int32_t ullis_cuda_head_distill_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t dtype, const void* hidden, size_t hidden_stride,
+                                     const uint32_t* bits, const void* weight, const uint16_t* scale, const uint16_t* bias,
+                                     const int32_t* top_ids, int32_t top_dtype, const void* top_logits, size_t top, float alpha,
+                                     float temperature, const uint32_t* labels, uint32_t ignore_id, size_t rows, size_t time,
+                                     size_t channels, size_t vocab, float loss_scale, float* row_loss, void* g_hidden, void* g_weight,
+                                     float* g_scale, float* g_bias, void* workspace, size_t workspace_bytes) {
+    return on_stream(rt, cuda_stream, [&](const dev::Stream& s) {
+        const dev::HeadGrad h{dtype, false,     false, false, {hidden, hidden_stride}, bits,     weight,   scale,    bias,    labels, ignore_id,
+                              rows,  time,      channels, vocab, loss_scale,           row_loss, g_hidden, g_weight, g_scale, g_bias};
+        need_dtype(top_dtype, true);
+        need_distill(top, alpha, temperature);
+        if (!need_head_grad(s, h)) return;
+        if (labels) need_array(labels, "labels", 4);
+        need_array(top_ids, "top_ids", 4);
+        need_array(top_logits, "top_logits", dev::size_of(top_dtype));
+        need_workspace(workspace, workspace_bytes,
+                       dev::head_distill_grad_workspace(rt, rows, channels, vocab, top, labels != nullptr, dev::head_copies_weight(weight, channels)));
+        need_sm100(rt);
+        dev::head_distill_grad(s, h, dev::Distill{top_ids, top_logits, top_dtype, top, alpha, temperature}, workspace);
     });
 }
 

@@ -97,5 +97,19 @@ bool head_copies_weight(const void* dense, size_t channels);   // whether the wo
 size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, bool copies_weight);
 void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace);
 
+// ---- distillation: the same outputs for (1 - alpha) * cross-entropy (labels may be null: without) + alpha * T^2 * KL(teacher || student)
+// over the teacher's entries [rows, top]
+struct Distill {
+    const int32_t* ids;        // negative: no entry
+    const void* logits;        // of `dtype`: F32, F16 or BF16
+    int dtype;
+    size_t top;
+    float alpha, temperature;
+};
+constexpr size_t DISTILL_MOST = 256;   // entries of a row
+size_t head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, size_t top, bool labels,
+                                   bool copies_weight);
+void head_distill_grad(const Stream& s, const HeadGrad& h, const Distill& d, void* workspace);
+
 }  // namespace dev
 }  // namespace ullis

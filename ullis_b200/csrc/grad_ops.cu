@@ -16,10 +16,12 @@
 // Beside the products a call of 16384 x 512 x 8192 takes 7.6 us to list the rows that count, 11.4 to bring both operands into 16
 // bits, 5.6 for the rows' sums and 4.7 for the columns': reads and writes of what they name, bound by their latency.
 #include <algorithm>
+#include <cmath>
 
 #include <cudaTypedefs.h>
 
 #include "device_ops.hpp"
+#include "head_entries.cuh"
 #include "pair_gemm.cuh"
 #include "tape.cuh"
 
@@ -28,7 +30,6 @@ namespace dev {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr float LN2 = 0.6931471805599453f;
 
 size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 size_t ceil_div(size_t n, size_t by) { return (n + by - 1) / by; }
@@ -222,17 +223,7 @@ void combine(const Stream& s, bool bf16, size_t M, size_t N, const Cut& cut, con
 // ------------------------------------------------------------------------------------------------ operands of the head
 // Which rows count: place[row] = the row's place among those that do, or -1 - its place among those that do not; list[place] = row
 // and how many there are.  A CTA has 1024 rows and counts those before them by itself (all labels are a few KB that lie in L2; one
-// CTA with a run of rows per warp took 18 us for 16 384).
-struct HeadLabels {
-    const uint32_t* labels;
-    uint32_t ignore_id, rows, time, vocab;
-    // the target of a row, -1 where it does not count (the last of its sequence, an ignored label), -2 for a label outside the vocabulary
-    __device__ int32_t target(uint32_t row) const {
-        const uint32_t label = labels[min(row + 1u, rows - 1u)];   // (always read, so that several are on their way)
-        if (row % time + 1u >= time || label == ignore_id) return -1;
-        return label < vocab ? (int32_t)label : -2;
-    }
-};
+// CTA with a run of rows per warp took 18 us for 16 384).  HeadLabels: head_entries.cuh.
 __global__ void __launch_bounds__(1024)
 head_list_kernel(const HeadLabels l, int32_t* __restrict__ place, int32_t* __restrict__ list, uint32_t* __restrict__ counted) {
     chain_entry();
@@ -280,7 +271,7 @@ struct HeadOperands {
     uint32_t g_bytes;           // of a row of it
     uint16_t* h16;
     int32_t* target;
-    float *target_acc, *logit2; // the target's product; its logit times log2 e
+    float *target_acc, *logit2; // the target's product; its logit times log2 e.  Both null: not wanted
     const uint32_t* bits;
     const uint16_t *dense, *scale, *bias;
     uint16_t* w16;              // null: the dense weights are taken as they are
@@ -387,7 +378,8 @@ head_operands_kernel(const HeadOperands o) {
                         w[e >> 1] |= (uint32_t)h << (16 * (e & 1));
                     }
             }
-            if (o.bits) {
+            if (!o.target_acc) {
+            } else if (o.bits) {
                 const uint32_t signs = signs8(o.bits, first + c, words);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)   // (0 past the row's end)
@@ -400,8 +392,8 @@ head_operands_kernel(const HeadOperands o) {
             *reinterpret_cast<uint4*>(o.h16 + (size_t)place * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
-        if (lane == 0) {
-            o.target[place] = target;
+        if (lane == 0) o.target[place] = target;
+        if (lane == 0 && o.target_acc) {
             if (o.fold) dot *= __half2float(__ushort_as_half(o.scale[target]));
             o.target_acc[place] = dot;
             // rounded as the epilogues round theirs: the difference of two logits is then what it is
@@ -535,10 +527,11 @@ head_rows_kernel(const HeadRows o) {
     o.row_loss[o.list[row]] = loss;
 }
 
-// The columns' sums of a piece out of their parts, times loss_scale.  32 columns to a CTA, a warp to each of a slot's eight parts.
+// The columns' sums of a piece out of their parts, and of `stretches` that the entries add, times loss_scale.  32 columns to a CTA, a warp to each of a slot's eight parts.
 __global__ void __launch_bounds__(256)
 head_columns_kernel(const float* __restrict__ part, uint32_t pitch, const uint32_t* __restrict__ counted, uint32_t n_tiles, uint32_t pairs,
-                    uint32_t columns, float loss_scale, float* __restrict__ g_scale, float* __restrict__ g_bias) {
+                    uint32_t columns, float loss_scale, const float* __restrict__ more, size_t more_pitch, uint32_t stretches,
+                    float* __restrict__ g_scale, float* __restrict__ g_bias) {
     chain_entry();
     __shared__ float sums[2][8][32];
     const uint32_t lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;   // c < pitch, whole tiles
@@ -562,8 +555,11 @@ head_columns_kernel(const float* __restrict__ part, uint32_t pitch, const uint32
     float all = 0.0f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) all += sums[slice][k][lane];
+    float entries = 0.0f;
+#pragma unroll 4
+    for (uint32_t i = 0; i < stretches; ++i) entries += more[((size_t)i * 2 + slice) * more_pitch + c];
     float* out = slice ? g_scale : g_bias;
-    if (out) out[c] = all * loss_scale;
+    if (out) out[c] = (all + entries) * loss_scale;
 }
 
 // ------------------------------------------------------------------------------------------------ the head's plan
@@ -575,6 +571,9 @@ struct HeadPlan {
     size_t piece, pieces;                        // columns of a piece of g (a multiple of 256), pieces
     uint32_t col_slots;
     Cut hidden, weight;
+    // with entries: K1 to a row that counts, sorted by blocks of 32 rows and groups of 64 columns
+    size_t K1, blocks, groups, stretch, stretches;
+    size_t state, entry_bits, entry_column, entry_weight, entry_logits, entry_place, offsets, constant, second_lse2, row_part2, column_sums;
     size_t h16, w16, counted, place, list, target, target_acc, target_g, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, hidden_partial, weight_partial, bytes;
 };
 constexpr size_t GRAD_ELEMENTS = (size_t)1 << 28;   // of a piece of g: 512 MiB
@@ -583,8 +582,9 @@ constexpr size_t GRAD_ELEMENTS = (size_t)1 << 28;   // of a piece of g: 512 MiB
 // pair they begin at floor(c x), of which inner / x + 1 lie in a run of `inner`, and one begins before it.
 size_t most_slots(size_t outer, uint32_t pairs) { return pairs / outer + 2; }
 
-HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V, bool copies_weight) {
+HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V, bool copies_weight, size_t K1 = 0) {
     HeadPlan p{};
+    p.K1 = K1;
     p.pairs = pairs_of(rt);
     p.Dp = up(D, 8);
     p.m_tiles = ceil_div(rows, pg::BM);
@@ -623,6 +623,25 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
     p.accum = at.add(p.pieces > 1 ? rows * D * 4 : 0);
     p.hidden_partial = at.add(partial_bytes(rows, D, p.hidden));
     p.weight_partial = at.add(partial_bytes(width, D, p.weight));
+    if (K1) {
+        p.blocks = ceil_div(rows, BLOCK_ROWS);
+        p.groups = p.n_tiles * (pg::BN / GROUP_COLUMNS);
+        // Blocks of rows whose entries' column sums a CTA takes: 32, and at most 64 such parts.
+        p.stretch = std::max<size_t>(32, ceil_div(p.blocks, 64));
+        p.stretches = ceil_div(p.blocks, p.stretch);
+        const size_t entries = p.blocks * BLOCK_ROWS * K1;
+        p.state = at.add(rows * 4);
+        p.entry_bits = at.add(entries * 4);
+        p.entry_column = at.add(entries * 4);
+        p.entry_weight = at.add(entries * 4);
+        p.entry_logits = at.add(entries * 8);
+        p.entry_place = at.add(entries * 2);
+        p.offsets = at.add(p.blocks * (p.groups + 1) * 2);
+        p.constant = at.add(rows * 4);
+        p.second_lse2 = at.add(rows * 4);
+        p.row_part2 = at.add(p.lse_pieces * p.row_part_piece * 4);
+        p.column_sums = at.add(p.stretches * 2 * p.n_tiles * pg::BN * 4);
+    }
     p.bytes = at.bytes;
     return p;
 }
@@ -636,9 +655,25 @@ size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t 
 // Dense weights that a tensor map takes are read where they are.
 bool head_copies_weight(const void* dense, size_t channels) { return !dense || channels % 8 != 0 || !aligned(dense, 16); }
 
-void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
+size_t head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, size_t top, bool labels,
+                                   bool copies_weight) {
+    return rows ? head_plan(rt, rows, channels, vocab, copies_weight, top + labels).bytes : 0;
+}
+
+namespace {
+
+template <typename T>
+void launch_entries_list(const Stream& s, const Teacher& t, size_t blocks, const int32_t* target, const int32_t* list, const uint32_t* counted,
+                         const EntryLists& lists) {
+    const size_t smem = BLOCK_ROWS * t.K1 * 12;
+    if (smem > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(entries_list_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    s.chain("entries_list", entries_list_kernel<T>, (unsigned)blocks, 512, smem, t, target, list, counted, lists);
+}
+
+// `d`: null, or what the target is spread over.
+void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* workspace) {
     const bool as_is = !head_copies_weight(h.weight, h.channels);
-    const HeadPlan p = head_plan(s.rt, h.rows, h.channels, h.vocab, !as_is);
+    const HeadPlan p = head_plan(s.rt, h.rows, h.channels, h.vocab, !as_is, d ? d->top + (h.labels != nullptr) : 0);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const bool bf16 = h.dtype == BF16;
     const size_t rows = h.rows, D = h.channels, V = h.vocab;
@@ -646,7 +681,33 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
 
     uint32_t* counted = reinterpret_cast<uint32_t*>(ws + p.counted);
     int32_t *place = reinterpret_cast<int32_t*>(ws + p.place), *list = reinterpret_cast<int32_t*>(ws + p.list);
-    const HeadLabels labels{h.labels, h.ignore_id, (uint32_t)rows, (uint32_t)h.time, (uint32_t)V};
+    HeadLabels labels{h.labels, h.ignore_id, (uint32_t)rows, (uint32_t)h.time, (uint32_t)V, nullptr};
+    Teacher teacher{};
+    EntryLists lists{};
+    bool two = false;
+    if (d) {
+        teacher.ids = d->ids;
+        teacher.logits = d->logits;
+        teacher.K = (uint32_t)d->top;
+        teacher.K1 = (uint32_t)p.K1;
+        teacher.alpha = d->alpha;
+        teacher.hard = h.labels ? (float)(1.0 - (double)d->alpha) : 0.0f;
+        teacher.temperature = d->alpha > 0.0f ? d->temperature : 1.0f;
+        two = teacher.hard > 0.0f && teacher.temperature != 1.0f;
+        teacher.first = two ? 1.0f : 1.0f / teacher.temperature;
+        teacher.second = two ? 1.0f / teacher.temperature : 0.0f;
+        lists.bits = reinterpret_cast<uint32_t*>(ws + p.entry_bits);
+        lists.column = reinterpret_cast<uint32_t*>(ws + p.entry_column);
+        lists.weight = reinterpret_cast<float*>(ws + p.entry_weight);
+        lists.offsets = reinterpret_cast<uint16_t*>(ws + p.offsets);
+        lists.groups1 = (uint32_t)p.groups + 1;
+        lists.place = reinterpret_cast<uint16_t*>(ws + p.entry_place);
+        lists.constant = reinterpret_cast<float*>(ws + p.constant);
+        int32_t* state = reinterpret_cast<int32_t*>(ws + p.state);
+        const auto kernel = d->dtype == F32 ? entries_state_kernel<float> : d->dtype == F16 ? entries_state_kernel<__half> : entries_state_kernel<__nv_bfloat16>;
+        s.chain("entries_state", kernel, (unsigned)ceil_div(rows, 8), 256, 0, labels, teacher, (uint32_t)rows, (uint32_t)V, state);
+        labels.ready = state;
+    }
     // Few rows find their places where they are gathered, each CTA of eight from all labels.  us of a call in a graph, 256 channels
     // and a vocabulary of 1024, so / with the list by a launch of its own: 32 rows 31.6 / 32.4, 512 35.3 / 36.0, 2048 42.4 / 42.0,
     // 8192 62.0 / 55.0, 16 384 115 / 86.
@@ -660,8 +721,8 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     o.D = (uint32_t)D;
     o.Dp = (uint32_t)p.Dp;
     o.vocab = (uint32_t)V;
-    o.target_acc = reinterpret_cast<float*>(ws + p.target_acc);
-    o.logit2 = reinterpret_cast<float*>(ws + p.logit);
+    o.target_acc = d ? nullptr : reinterpret_cast<float*>(ws + p.target_acc);
+    o.logit2 = d ? nullptr : reinterpret_cast<float*>(ws + p.logit);
     o.labels = labels;
     o.place = listed ? place : nullptr;
     o.list = list;
@@ -701,7 +762,23 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     q.target_g = reinterpret_cast<float*>(ws + p.target_g);
     q.lse2 = reinterpret_cast<float*>(ws + p.lse2);
     float* factors = reinterpret_cast<float*>(ws + p.factors);
-    launch<pg::LSE, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+    if (d) {
+        q.offsets = lists.offsets;
+        q.groups1 = lists.groups1;
+        q.block_entries = (uint32_t)(BLOCK_ROWS * p.K1);
+        q.entries = lists.bits;
+        q.entry_logits = reinterpret_cast<float2*>(ws + p.entry_logits);
+        q.column_factor = teacher.first;
+        q.second_factor = teacher.second;
+        q.row_part2 = reinterpret_cast<float*>(ws + p.row_part2);
+        q.second_lse2 = reinterpret_cast<float*>(ws + p.second_lse2);
+        const auto list_kernel = d->dtype == F32 ? launch_entries_list<float> : d->dtype == F16 ? launch_entries_list<__half> : launch_entries_list<__nv_bfloat16>;
+        list_kernel(s, teacher, p.blocks, o.target, list, counted, lists);
+        if (two) launch<pg::LSE_ENTRIES_2, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+        else launch<pg::LSE_ENTRIES, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+    } else {
+        launch<pg::LSE, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+    }
 
     HeadRows r{};
     r.part = q.row_part;
@@ -718,7 +795,40 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
     r.scale_max = q.scale ? o.scale_max : nullptr;
     r.factors = factors;
     r.loss_scale = h.loss_scale;
-    s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 8), 128, 0, r);
+    const bool columns = h.g_bias || h.g_scale;
+    if (d) {
+        EntryRows e{};
+        e.teacher = teacher;
+        e.lists = lists;
+        e.part = r.part;
+        e.part2 = q.row_part2;
+        e.part_piece = r.part_piece;
+        e.counted = counted;
+        e.list = list;
+        e.n_tiles = r.n_tiles;
+        e.piece_tiles = r.piece_tiles;
+        e.pairs = r.pairs;
+        e.logits = q.entry_logits;
+        e.scale = q.scale;
+        e.scale_max = r.scale_max;
+        e.n_scale_max = WEIGHT_CTAS;
+        e.bf16 = bf16;
+        e.headroom = (uint32_t)std::max(0, (int)std::ceil(std::log2(std::max(1e-30f, teacher.hard + teacher.alpha * teacher.temperature))));
+        e.lse2 = r.lse2;
+        e.second_lse2 = reinterpret_cast<float*>(ws + p.second_lse2);
+        e.row_loss = r.row_loss;
+        e.factors = factors;
+        e.loss_scale = r.loss_scale;
+        e.blocks = (uint32_t)p.blocks;
+        e.stretch = (uint32_t)p.stretch;
+        e.stretches = (uint32_t)p.stretches;
+        e.column_sums = reinterpret_cast<float*>(ws + p.column_sums);
+        e.column_pitch = p.n_tiles * pg::BN;
+        s.chain("entries_rows", entries_rows_kernel, (unsigned)(p.blocks + (columns ? p.groups * p.stretches : 0)), ROWS_THREADS, 0, e);
+        q.entries = lists.column;
+    } else {
+        s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 8), 128, 0, r);
+    }
 
     uint16_t* grad = reinterpret_cast<uint16_t*>(ws + p.grad);
     for (size_t piece = 0; piece < p.pieces; ++piece) {
@@ -736,13 +846,15 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
         wp.data = static_cast<const uint16_t*>(w16) + v0 * weight.stride;
         wp.rows = width;
         const CUtensorMap grad_map = map_of(grad, rows, p.piece, p.piece, 16, bf16);
-        launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
+        if (two) launch<pg::GRAD_ENTRIES_2, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
+        else if (d) launch<pg::GRAD_ENTRIES, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
+        else launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
         // What follows reads g and nothing of one another: few rows leave room for all three at once.
-        const bool columns = h.g_bias || h.g_scale;
         if (columns)
             s.chain("head_columns", head_columns_kernel, (unsigned)ceil_div(width, 32), 256, 0, static_cast<const float*>(g.col_part), g.pitch,
-                    counted, n_tiles, p.pairs, (uint32_t)width, h.loss_scale, h.g_scale ? h.g_scale + v0 : nullptr,
-                    h.g_bias ? h.g_bias + v0 : nullptr);
+                    counted, n_tiles, p.pairs, (uint32_t)width, h.loss_scale,
+                    d ? reinterpret_cast<const float*>(ws + p.column_sums) + v0 : nullptr, p.n_tiles * pg::BN, (uint32_t)p.stretches,
+                    h.g_scale ? h.g_scale + v0 : nullptr, h.g_bias ? h.g_bias + v0 : nullptr);
         const Operand by_columns{grad, rows, width, p.piece, true};
         Operand hc = hidden;
         hc.mn = true;
@@ -758,21 +870,26 @@ void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) {
         // g_hidden: over the pieces in f32
         const Operand by_rows{grad, rows, width, p.piece, false};
         wp.mn = true;
-        Output d{};
-        d.out = piece + 1 == p.pieces ? h.g_hidden : nullptr;
-        d.f32 = h.out_f32;
-        d.accum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.accum) : nullptr;
-        d.accum_read = piece > 0;
-        d.factor = factors + 1;
-        d.partial = reinterpret_cast<float*>(ws + p.hidden_partial);
-        d.counted = counted;
-        d.rows = list;
-        d.beside = true;
-        product(s, "head_g_hidden", by_rows, wp, bf16, rows, D, width, p.hidden, d);
+        Output x{};
+        x.out = piece + 1 == p.pieces ? h.g_hidden : nullptr;
+        x.f32 = h.out_f32;
+        x.accum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.accum) : nullptr;
+        x.accum_read = piece > 0;
+        x.factor = factors + 1;
+        x.partial = reinterpret_cast<float*>(ws + p.hidden_partial);
+        x.counted = counted;
+        x.rows = list;
+        x.beside = true;
+        product(s, "head_g_hidden", by_rows, wp, bf16, rows, D, width, p.hidden, x);
         combine(s, bf16, width, D, p.weight, w);
-        combine(s, bf16, rows, D, p.hidden, d);
+        combine(s, bf16, rows, D, p.hidden, x);
     }
 }
+
+}  // namespace
+
+void head_ce_grad(const Stream& s, const HeadGrad& h, void* workspace) { head_grad(s, h, nullptr, workspace); }
+void head_distill_grad(const Stream& s, const HeadGrad& h, const Distill& d, void* workspace) { head_grad(s, h, &d, workspace); }
 
 // ------------------------------------------------------------------------------------------------ a wait that runs out
 namespace {

@@ -1,0 +1,372 @@
+// Which rows of a head's batch count, and, for distillation, the teacher's entries: their probabilities, their order for the epilogues of
+// pair_gemm.cuh, and what comes of them between the two products.
+//
+// Of a row that counts, with z the student's logits, T the temperature, p = softmax(t / T) over its entries (a negative id is none,
+// t = -infinity has p = 0), y its label and alpha the teacher's share,
+//   loss = (1 - alpha) * (lse(z) - z[y]) + alpha * T^2 * sum p * (log p - z / T + lse(z / T)),
+//   g = (1 - alpha) * softmax(z) + alpha * T * softmax(z / T) - w,  w = alpha * T * p at the entries, 1 - alpha more at y:
+// a label is one more entry, and an id that comes twice in a row is one entry with both weights.  With top the largest logit,
+//   loss = (1 - alpha) * (lse(z) - top) + alpha * T^2 * (lse(z / T) - top / T) + sum w * (top - z) + alpha * T^2 * sum p * log p,
+// none of whose terms but the last is negative.  Without labels the first parts are left out; where only one of the softmaxes has a
+// share, or T = 1, one is computed, and z and top below are those at its temperature.
+//
+// The rows that count are taken 32 at a time, and their entries sorted by groups of 64 columns and within them by entry_bits: what an
+// epilogue warp has of a tile then lies in a row, and entries of one column beside one another.  Sums go by that order: a call gives the
+// same result every time.
+#pragma once
+#include "pair_gemm.cuh"
+#include "tape.cuh"
+
+namespace ullis {
+namespace dev {
+namespace {
+
+constexpr float LN2 = 0.6931471805599453f;
+constexpr uint32_t BLOCK_ROWS = 32, GROUP_COLUMNS = 64;
+constexpr uint32_t NO_PLACE = 0xFFFFu;   // of an entry that is none, among those of its block
+
+struct HeadLabels {
+    const uint32_t* labels;
+    uint32_t ignore_id, rows, time, vocab;
+    const int32_t* ready;   // the answers (distillation: entries_state_kernel), or null
+    // the target of a row, -1 where it does not count (the last of its sequence, an ignored label), -2 for a label outside the vocabulary
+    __device__ int32_t target(uint32_t row) const {
+        if (ready) return ready[min(row, rows - 1u)];
+        const uint32_t label = labels[min(row + 1u, rows - 1u)];   // (always read, so that several are on their way)
+        if (row % time + 1u >= time || label == ignore_id) return -1;
+        return label < vocab ? (int32_t)label : -2;
+    }
+};
+
+struct Teacher {
+    const int32_t* ids;       // [rows, K]
+    const void* logits;       // [rows, K]
+    uint32_t K, K1;           // K1: with the label's entry
+    float alpha, hard;        // the teacher's share and, with labels, 1 - alpha (else 0)
+    float temperature;
+    // what is computed: 1 / the temperature of the first softmax, and of the second over the first's (0: none)
+    float first, second;
+};
+
+// The state of every row: HeadLabels::target's numbers (0 without labels).  A warp has a row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+entries_state_kernel(const HeadLabels labels, const Teacher t, uint32_t rows, uint32_t vocab, int32_t* __restrict__ state) {
+    chain_entry();
+    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    bool any = false, bad = false;
+    const size_t at = (size_t)row * t.K;
+#pragma unroll 4
+    for (uint32_t k = lane; k < t.K; k += 32) {
+        const int32_t id = t.ids[at + k];
+        const float v = tape::to_float(static_cast<const T*>(t.logits)[at + k]);
+        if (id < 0) continue;
+        any |= v != -INFINITY;
+        bad |= (uint32_t)id >= vocab || !(v < INFINITY);
+    }
+    any = __any_sync(0xffffffffu, any);
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane) return;
+    int32_t s = labels.labels ? labels.target(row) : any || bad ? 0 : -1;
+    if (s >= 0 && bad) s = -2;
+    state[row] = s;
+}
+
+struct EntryLists {
+    // by block of 32 rows that count: 32 * K1 places, and groups1 offsets among them
+    uint32_t* bits;            // entry_bits (and ENTRY_DEAD)
+    uint32_t* column;          // of the vocabulary; later what GRAD takes: bits and above them the 16-bit g * scale * 2^k
+    float* weight;             // w, of a dead one 0
+    uint16_t* offsets;
+    uint32_t groups1;
+    // by row that counts
+    uint16_t* place;           // [row][K1], in the block's list
+    float* constant;           // alpha * T^2 * sum p * log p; without entries NAN, which marks that
+};
+template <typename T>
+__global__ void __launch_bounds__(512)
+entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const int32_t* __restrict__ list, const uint32_t* __restrict__ counted,
+                    const EntryLists o) {
+    chain_entry();
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    const uint32_t first = blockIdx.x * BLOCK_ROWS, rows = *counted, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (first >= rows) return;
+    const uint32_t n_rows = min(BLOCK_ROWS, rows - first), n = n_rows * t.K1;
+    uint64_t* keys = reinterpret_cast<uint64_t*>(smem_raw);             // column group, entry_bits, the entry's number
+    float* weight = reinterpret_cast<float*>(keys + BLOCK_ROWS * t.K1);   // by the entry's number
+    const auto key_of = [](uint32_t row, uint32_t column, uint32_t number) {
+        return (uint64_t)((column / GROUP_COLUMNS) * pg::ENTRY_PLACES | pg::entry_bits(row, column)) << 32 | number;
+    };
+    for (uint32_t r = warp; r < n_rows; r += 16) {
+        const size_t at = (size_t)list[first + r] * t.K;
+        const T* logits = static_cast<const T*>(t.logits) + at;
+        float top = -INFINITY;
+        for (uint32_t k = lane; k < t.K; k += 32) top = fmaxf(top, t.ids[at + k] < 0 ? -INFINITY : tape::to_float(logits[k]));
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const bool has = top != -INFINITY;
+        float sum = 0.0f;
+        for (uint32_t k = lane; k < t.K; k += 32)
+            if (has && t.ids[at + k] >= 0) sum += expf((tape::to_float(logits[k]) - top) / t.temperature);
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const float log_sum = logf(sum);
+        float entropy = 0.0f;
+        for (uint32_t k = lane; k < t.K; k += 32) {
+            const uint32_t number = r * t.K1 + k;
+            const int32_t id = t.ids[at + k];
+            uint64_t key = ~0ull;
+            if (has && id >= 0) {
+                const float x = (tape::to_float(logits[k]) - top) / t.temperature, p = expf(x) / sum;
+                if (p > 0.0f) entropy += p * (x - log_sum);
+                weight[number] = t.alpha * t.temperature * p;
+                key = key_of(r, (uint32_t)id, number);
+            }
+            keys[number] = key;
+        }
+        for (int d = 16; d > 0; d >>= 1) entropy += __shfl_xor_sync(0xffffffffu, entropy, d);
+        if (lane == 0) {
+            o.constant[first + r] = has ? t.alpha * t.temperature * t.temperature * entropy : NAN;
+            if (t.K1 > t.K) {
+                keys[r * t.K1 + t.K] = key_of(r, (uint32_t)target[first + r], r * t.K1 + t.K);
+                weight[r * t.K1 + t.K] = t.hard;
+            }
+        }
+    }
+    for (uint32_t run = 2; run < 2 * n; run <<= 1) {
+        for (uint32_t half = run >> 1; half > 0; half >>= 1) {
+            __syncthreads();
+            for (uint32_t i = threadIdx.x;; i += 512) {
+                const uint32_t a = (i & ~(half - 1)) * 2 + (i & (half - 1));
+                if (a >= n) break;
+                const uint32_t b = half == run >> 1 ? a ^ (run - 1) : a + half;   // (the first step of a run mirrors: all runs rise)
+                if (b >= n) continue;
+                const uint64_t x = keys[a], y = keys[b];
+                if (x > y) {
+                    keys[a] = y;
+                    keys[b] = x;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const size_t base = (size_t)blockIdx.x * BLOCK_ROWS * t.K1;
+    for (uint32_t i = threadIdx.x; i < n; i += 512) {
+        const uint64_t key = keys[i];
+        if (key == ~0ull) continue;
+        const uint32_t at = (uint32_t)(key >> 32), number = (uint32_t)key;
+        const bool dead = i > 0 && (uint32_t)(keys[i - 1] >> 32) == at;
+        float w = 0.0f;
+        if (!dead)
+            for (uint32_t j = i; j < n && (uint32_t)(keys[j] >> 32) == at; ++j) w += weight[(uint32_t)keys[j]];
+        o.bits[base + i] = (at & (pg::ENTRY_PLACES - 1)) | (dead ? pg::ENTRY_DEAD : 0u);
+        o.column[base + i] = at / pg::ENTRY_PLACES * GROUP_COLUMNS + pg::entry_column(at);
+        o.weight[base + i] = w;
+        o.place[(size_t)first * t.K1 + number] = (uint16_t)i;
+    }
+    // (the numbers of entries that are none come with none of the keys)
+    for (uint32_t r = warp; r < n_rows; r += 16) {
+        const size_t at = (size_t)list[first + r] * t.K;
+        const bool has = o.constant[first + r] == o.constant[first + r];
+        for (uint32_t k = lane; k < t.K; k += 32)
+            if (!has || t.ids[at + k] < 0) o.place[(size_t)first * t.K1 + r * t.K1 + k] = (uint16_t)NO_PLACE;
+    }
+    for (uint32_t g = threadIdx.x; g < o.groups1; g += 512) {
+        const uint64_t limit = (uint64_t)g * pg::ENTRY_PLACES << 32;
+        uint32_t low = 0, high = n;
+        while (low < high) {
+            const uint32_t middle = (low + high) >> 1;
+            if (keys[middle] < limit) low = middle + 1;
+            else high = middle;
+        }
+        o.offsets[(size_t)blockIdx.x * o.groups1 + g] = (uint16_t)low;
+    }
+}
+
+// Between the products.  The first CTAs have a block of 32 rows each: log2 sum exp of its rows out of their parts (sixteen lanes to a
+// row), less the logarithm of the softmax's share so that GRAD's exp has it as a factor; the losses; and of every entry the 16-bit
+// g * scale * 2^k that GRAD puts in its place.  The others sum -w and -w * product by columns: 64 columns and a stretch of blocks each,
+// over runs of one column in a word of 32 entries, then over the words and blocks of a warp, then over the warps.
+struct EntryRows {
+    Teacher teacher;
+    EntryLists lists;
+    const float2* part;
+    const float* part2;
+    size_t part_piece;
+    const uint32_t* counted;
+    const int32_t* list;
+    uint32_t n_tiles, piece_tiles, pairs;
+    const float2* logits;      // of entries: product, logit
+    const uint16_t* scale;     // or null
+    const float* scale_max;    // null: no row scales
+    uint32_t n_scale_max;
+    uint32_t bf16, headroom;   // 2^headroom: bound of the softmaxes' shares
+    float *lse2, *second_lse2, *row_loss, *factors;
+    float loss_scale;
+    uint32_t blocks;           // of rows, CTAs
+    uint32_t stretch, stretches;
+    float* column_sums;        // [stretches][2][groups of 64]
+    size_t column_pitch;
+};
+constexpr uint32_t ROWS_THREADS = 512, ROWS_WARPS = ROWS_THREADS / 32;
+__global__ void __launch_bounds__(ROWS_THREADS)
+entries_rows_kernel(const EntryRows o) {
+    chain_entry();
+    const Teacher& t = o.teacher;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = *o.counted;
+    const size_t block_entries = (size_t)BLOCK_ROWS * t.K1;
+    if (blockIdx.x >= o.blocks) {
+        __shared__ float sums[ROWS_WARPS][2][GROUP_COLUMNS];
+        const uint32_t group = (blockIdx.x - o.blocks) / o.stretches, stretch = (blockIdx.x - o.blocks) % o.stretches;
+        for (uint32_t i = lane; i < 2 * GROUP_COLUMNS; i += 32) sums[warp][0][i] = 0.0f;
+        __syncwarp();
+        const uint32_t end = min((stretch + 1) * o.stretch, (rows + BLOCK_ROWS - 1) / BLOCK_ROWS);
+        for (uint32_t b = stretch * o.stretch + warp; b < end; b += ROWS_WARPS) {
+            const uint16_t* at = o.lists.offsets + (size_t)b * o.lists.groups1 + group;
+            const uint32_t last = at[1];
+            for (uint32_t i0 = at[0]; i0 < last; i0 += 32) {
+                const uint32_t i = i0 + lane;
+                const bool in = i < last;
+                const uint32_t run = in ? (o.lists.bits[b * block_entries + i] & (pg::ENTRY_PLACES - 1)) >> 4 : 0xFFFFFFFFu;   // half, column
+                const float w = in ? -o.lists.weight[b * block_entries + i] : 0.0f;
+                float g = w, ga = w != 0.0f ? w * o.logits[b * block_entries + i].x : 0.0f;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t other = __shfl_up_sync(0xffffffffu, run, d);
+                    const float u = __shfl_up_sync(0xffffffffu, g, d), v = __shfl_up_sync(0xffffffffu, ga, d);
+                    if ((int)lane >= d && other == run) {
+                        g += u;
+                        ga += v;
+                    }
+                }
+                const uint32_t next = __shfl_down_sync(0xffffffffu, run, 1);
+                const bool ends = in && (lane == 31 || next != run);
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {   // (a column may end a run of either)
+                    if (ends && run >> 6 == half) {
+                        sums[warp][0][run & 63u] += g;
+                        sums[warp][1][run & 63u] += ga;
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x < 2 * GROUP_COLUMNS) {
+            const uint32_t which = threadIdx.x / GROUP_COLUMNS, c = threadIdx.x % GROUP_COLUMNS;
+            float all = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < ROWS_WARPS; ++w) all += sums[w][which][c];
+            o.column_sums[((size_t)stretch * 2 + which) * o.column_pitch + group * GROUP_COLUMNS + c] = all;
+        }
+        return;
+    }
+    __shared__ float tops[ROWS_WARPS], row_lse[2][BLOCK_ROWS];
+    // the power of two of g * scale
+    float largest = o.scale_max ? 0.0f : 1.0f;
+    if (o.scale_max)
+        for (uint32_t i = threadIdx.x; i < o.n_scale_max; i += ROWS_THREADS) largest = fmaxf(largest, o.scale_max[i]);
+    for (int d = 16; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, d));
+    if (lane == 0) tops[warp] = largest;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < ROWS_WARPS; ++w) largest = fmaxf(largest, tops[w]);
+    const int exponent = (int)(__float_as_uint(largest) >> 23) - 127;
+    const int power = largest > 0.0f && exponent < 128 ? 14 - exponent - (int)o.headroom : 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        o.factors[0] = exp2f((float)power);
+        o.factors[1] = exp2f((float)-power) * o.loss_scale;
+    }
+    const uint32_t first = blockIdx.x * BLOCK_ROWS;
+    if (first >= rows) return;
+    const bool two = t.second != 0.0f;
+    // two rows to a warp; a row's sixteen lanes: a quarter of the columns, every fourth slot
+    const uint32_t r = warp * 2 + (lane & 1), row = first + r, part_lane = lane >> 1, quarter = part_lane & 3;
+    const uint32_t m = row / pg::BM, m_tiles = (rows + pg::BM - 1) / pg::BM, whole_rows = m_tiles * pg::BM;   // (32 rows: of one tile)
+    float top = -INFINITY, sum = 0.0f, sum2 = 0.0f;
+    const auto add = [&](float u, float s, float s2) {
+        if (u > top) {
+            sum = sum * exp2f(top - u) + s;
+            if (two) sum2 = sum2 * exp2f((top - u) * t.second) + s2;
+            top = u;
+        } else if (s != 0.0f) {   // (NaN too)
+            sum += s * exp2f(u - top);
+            if (two) sum2 += s2 * exp2f((u - top) * t.second);
+        }
+    };
+    for (uint32_t begin = 0, piece = 0; begin < o.n_tiles; begin += o.piece_tiles, ++piece) {
+        const uint32_t width = min(o.piece_tiles, o.n_tiles - begin);
+        const pg::Share share = pg::share_of(m_tiles * width, o.pairs);
+        const uint32_t slots = share.owner(m * width + width - 1) - share.owner(m * width) + 1;
+        const size_t at = piece * o.part_piece + row;
+#pragma unroll 4
+        for (uint32_t i = part_lane >> 2; i < slots; i += 4) {
+            const size_t from = at + (size_t)(i * 4 + quarter) * whole_rows;
+            const float2 p = o.part[from];
+            add(p.x, p.y, two ? o.part2[from] : 0.0f);
+        }
+    }
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) {   // (within a row's lanes, in a fixed order)
+        const float u = __shfl_xor_sync(0xffffffffu, top, 2 * k), s = __shfl_xor_sync(0xffffffffu, sum, 2 * k);
+        const float s2 = __shfl_xor_sync(0xffffffffu, sum2, 2 * k);
+        const float a = top, b = sum, b2 = sum2;
+        const bool mine_first = !(part_lane & k);
+        top = mine_first ? a : u;
+        sum = mine_first ? b : s;
+        sum2 = mine_first ? b2 : s2;
+        add(mine_first ? u : a, mine_first ? s : b, mine_first ? s2 : b2);
+    }
+    const bool in = row < rows;
+    float off = 0.0f;   // sum of w * (top - z)
+    if (in) {
+#pragma unroll 4
+        for (uint32_t k = part_lane; k < t.K1; k += 16) {
+            const uint32_t i = o.lists.place[(size_t)row * t.K1 + k];
+            if (i == NO_PLACE) continue;
+            const float w = o.lists.weight[blockIdx.x * block_entries + i];
+            if (w != 0.0f) off += w * (top - o.logits[blockIdx.x * block_entries + i].y);
+        }
+    }
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) off += __shfl_xor_sync(0xffffffffu, off, 2 * k);
+    if (in && part_lane == 0) {
+        const float constant = o.lists.constant[row];
+        const bool has = constant == constant;
+        const float soft = has ? t.alpha * t.temperature : 0.0f, soft2 = soft * t.temperature;   // of the gradient and of the loss
+        const float more = log2f(sum);
+        float loss, lse = top + more, second = 0.0f;
+        if (two) {
+            const float more2 = log2f(sum2);
+            loss = t.hard * more + soft2 * more2;
+            lse -= log2f(t.hard);
+            second = top * t.second + more2 - log2f(soft);   // (no entries: infinity, whose exp is 0)
+        } else {
+            loss = (t.hard + soft2) * more;
+            if (t.hard + soft == 0.0f) loss = 0.0f;
+            lse -= log2f(t.hard + soft);
+            off /= t.first;
+        }
+        o.row_loss[o.list[row]] = (loss + off) * LN2 + (has ? constant : 0.0f);
+        o.lse2[row] = lse;
+        row_lse[0][r] = lse;
+        if (two) o.second_lse2[row] = second;
+        row_lse[1][r] = second;
+    }
+    __syncthreads();
+    const float times = exp2f((float)power);
+    const uint32_t n = o.lists.offsets[(size_t)blockIdx.x * o.lists.groups1 + o.lists.groups1 - 1];
+#pragma unroll 2
+    for (uint32_t j = threadIdx.x; j < n; j += ROWS_THREADS) {
+        const size_t i = blockIdx.x * block_entries + j;
+        const uint32_t bits = o.lists.bits[i], column = o.lists.column[i], of = pg::entry_row(bits);
+        const float w = o.lists.weight[i], z = o.logits[i].y;
+        float g = exp2f(z - row_lse[0][of]);
+        if (two) g += exp2f(fmaf(z, t.second, -row_lse[1][of]));
+        g = (g - w) * times * pg::half_at(o.scale, column, 1.0f);
+        o.lists.column[i] = bits | (o.bf16 ? (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(g)) : (uint32_t)__half_as_ushort(__float2half_rn(g))) << 16;
+    }
+}
+
+}  // namespace
+}  // namespace dev
+}  // namespace ullis

@@ -17,6 +17,10 @@
 //          elsewhere: the loss is the difference of two large numbers, and what the tensor cores cut off would stay in it.)
 //   GRAD   g = softmax(z) - onehot, by rows as the 16-bit operand g * scale * 2^k of the products that follow, and by columns the
 //          f32 sums of g and g * acc
+//   LSE_ENTRIES, GRAD_ENTRIES  the same for a target that is spread over a list of columns per row (entries), at one temperature or
+//          (.._2) as a sum over two.  LSE leaves the product and the logit of every entry, GRAD writes softmax(z) and, over it, what
+//          a kernel between the two has made of the entries.  Entries lie by blocks of 32 rows and groups of 64 columns, which
+//          are what an epilogue warp has of a tile
 //   STORE  alpha * acc in 16 bits, or into an f32 accumulator, or as one of several partial sums
 //   SUM    acc in f32: the tensor cores cut off what falls below the accumulator's last bit (measured: K = 16384 1.9e-5 off in
 //          norm, 1.1e-4 where all terms have one sign; K = 512 6e-7), so every 512 terms the accumulator moves to registers
@@ -38,7 +42,10 @@
 namespace ullis {
 namespace pg {
 
-enum { LSE = 0, GRAD = 1, STORE = 2, SUM = 3 };
+enum { LSE = 0, GRAD = 1, STORE = 2, SUM = 3, LSE_ENTRIES = 4, GRAD_ENTRIES = 5, LSE_ENTRIES_2 = 6, GRAD_ENTRIES_2 = 7 };
+__host__ __device__ constexpr int kind_of(int epi) { return epi >= LSE_ENTRIES ? epi & 1 : epi; }   // LSE, GRAD, STORE or SUM
+__host__ __device__ constexpr bool has_entries(int epi) { return epi >= LSE_ENTRIES; }
+__host__ __device__ constexpr bool has_two(int epi) { return epi >= LSE_ENTRIES_2; }
 
 constexpr uint32_t BM = 256, BN = 256, BK = 64;         // of a pair, per accumulator
 constexpr uint32_t OPERAND_BYTES = 128 * BK * 2;        // one CTA's 128 rows of A, or of one accumulator's B
@@ -49,6 +56,7 @@ constexpr uint32_t MAX_STAGES = 6, SMEM_LIMIT = 227 * 1024;
 constexpr uint32_t STAGING_BYTES = 16 * 128;            // 16 rows of 64 16-bit outputs; GRAD has two of them
 constexpr uint32_t COLUMN_BYTES = 2 * 64 * 4;           // constants of its columns
 constexpr uint32_t ROW_BYTES = 2 * 4 * 32 * 4;          // GRAD: what its rows need, of this tile and of the next
+constexpr uint32_t EXTRACT_PITCH = 20, EXTRACT_BYTES = 32 * EXTRACT_PITCH * 4;   // LSE_ENTRIES: 16 columns of 32 rows, rows 80 bytes apart
 constexpr uint32_t SUM_BLOCKS = 8;                      // k-blocks of a stretch of K, after which SUM adds with rounding
 
 struct Maps {
@@ -76,6 +84,16 @@ struct Params {
     const float* target_acc;   // GRAD: [M] the target's product, added with rounding
     const float* target_g;     // GRAD: [M] its probability - 1
     const float* factor;       // GRAD: 2^k ; STORE: alpha
+    // .._ENTRIES: entries of block b of 32 rows and group n of 64 columns of the vocabulary: [b * block_entries + offsets[b * groups1 + n],
+    // .. + offsets[b * groups1 + n + 1])
+    const uint16_t* offsets;
+    uint32_t groups1, block_entries;
+    const uint32_t* entries;   // LSE: entry_bits; GRAD: with the 16-bit g * scale * 2^k above them
+    float2* entry_logits;      // LSE: the entry's product, and its logit as the epilogues have it
+    float column_factor;       // 1 / the temperature of the first (only) softmax
+    float second_factor;       // .._2: 1 / the temperature of the second
+    float* row_part2;          // .._2: LSE: the second sums beside row_part's
+    const float* second_lse2;  // .._2: GRAD: as lse2
     uint32_t pitch;            // GRAD: of col_part, whole tiles
     float* col_part;           // GRAD: [slot][8][2][pitch]
     // STORE, SUM
@@ -100,7 +118,10 @@ struct Params {
 inline uint32_t stage_bytes(int accs) { return OPERAND_BYTES * (1 + accs); }
 // Barriers first, then (on 1024 bytes) the ring, then what the epilogue warps have.
 constexpr uint32_t epi_bytes(int epi) {
-    return epi == GRAD ? 2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES : epi == STORE ? STAGING_BYTES : epi == LSE ? COLUMN_BYTES : 0u;
+    return kind_of(epi) == GRAD    ? 2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES
+           : kind_of(epi) == STORE ? STAGING_BYTES
+           : kind_of(epi) == LSE   ? COLUMN_BYTES + (has_entries(epi) ? EXTRACT_BYTES : 0u)
+                                   : 0u;
 }
 inline uint32_t fixed_bytes(int epi) { return 2 * 1024 /*barriers, alignment*/ + EPI_WARPS * epi_bytes(epi); }
 inline uint32_t stages_for(int epi, int accs) {
@@ -117,12 +138,20 @@ struct Share {
 };
 __host__ __device__ inline Share share_of(uint32_t total, uint32_t pairs) { return Share{total, total < pairs ? total : pairs}; }
 
+// An entry's place in its 32 rows and 64 columns, 0 .. 2^11 in the order of the list: the second sixteen rows last, then by
+// columns.  ENTRY_DEAD: an earlier one of the list has the same place and stands for both.
+constexpr uint32_t ENTRY_PLACES = 2048, ENTRY_DEAD = ENTRY_PLACES, NO_ENTRY = 0xFFFFFFFFu;
+__host__ __device__ inline uint32_t entry_bits(uint32_t row, uint32_t column) { return (row & 16u) << 6 | (column & 63u) << 4 | (row & 15u); }
+__device__ __forceinline__ uint32_t entry_row(uint32_t bits) { return (bits >> 6 & 16u) | (bits & 15u); }
+__device__ __forceinline__ uint32_t entry_column(uint32_t bits) { return bits >> 4 & 63u; }
+
 // What a pair computes, tile by tile; every warp of the pair goes through the same list.
 //  LSE   piece after piece of the columns (whose B stays in L2); in a piece the tiles of 256 rows follow one another
 //  GRAD  tiles of 256 columns follow one another
 //  STORE, SUM  jobs of one tile and one range of K, dealt out in turn
 template <int EPI, int ACCS>
 struct Work {
+    static constexpr int KIND = kind_of(EPI);
     const Params& p;
     uint32_t pair, pairs, M, m_tiles, n_tiles, blocks;
     uint32_t piece = 0, left = 0, outer = 0, inner = 0, width = 0;   // LSE, GRAD: tiles left in the piece, (outer, inner < width) of the next
@@ -138,11 +167,11 @@ struct Work {
         blocks = ((p.count_k ? min(p.K, counted) : p.K) + BK - 1) / BK;
         k1 = blocks;
         job = pair;
-        if (EPI == LSE) open(m_tiles, min(p.piece_tiles, n_tiles));
-        if (EPI == GRAD) open(n_tiles, m_tiles);
+        if (KIND == LSE) open(m_tiles, min(p.piece_tiles, n_tiles));
+        if (KIND == GRAD) open(n_tiles, m_tiles);
     }
     // where the stretch from k-block kb on ends (STORE: the range)
-    __device__ uint32_t stretch_end(uint32_t kb) const { return EPI == SUM ? min(k1, kb + SUM_BLOCKS) : k1; }
+    __device__ uint32_t stretch_end(uint32_t kb) const { return KIND == SUM ? min(k1, kb + SUM_BLOCKS) : k1; }
     __device__ void open(uint32_t outers, uint32_t inners) {
         const Share s = share_of(outers * inners, pairs);
         width = inners;
@@ -155,13 +184,13 @@ struct Work {
         }
     }
     __device__ bool next() {
-        if (EPI == LSE || EPI == GRAD) {
+        if (KIND == LSE || KIND == GRAD) {
             while (left == 0) {
-                if (EPI == GRAD || ++piece * p.piece_tiles >= n_tiles) return false;
+                if (KIND == GRAD || ++piece * p.piece_tiles >= n_tiles) return false;
                 open(m_tiles, min(p.piece_tiles, n_tiles - piece * p.piece_tiles));
             }
-            m = EPI == LSE ? outer : inner;
-            n = EPI == LSE ? piece * p.piece_tiles + inner : outer;
+            m = KIND == LSE ? outer : inner;
+            n = KIND == LSE ? piece * p.piece_tiles + inner : outer;
             in_piece = piece;
             --left;
             if (++inner == width) { inner = 0; ++outer; }
@@ -172,7 +201,7 @@ struct Work {
         split = job % p.splits;
         m = tile / n_tiles;
         n = tile % n_tiles;
-        const uint32_t step = EPI == SUM ? SUM_BLOCKS : 1u, steps = (blocks + step - 1) / step;   // SUM: whole stretches
+        const uint32_t step = KIND == SUM ? SUM_BLOCKS : 1u, steps = (blocks + step - 1) / step;   // SUM: whole stretches
         k0 = (uint32_t)((uint64_t)split * steps / p.splits) * step;
         k1 = min(blocks, (uint32_t)((uint64_t)(split + 1) * steps / p.splits) * step);
         job += pairs;
@@ -348,14 +377,28 @@ struct Columns {
             bias[i] = n < p.N ? half_at(p.bias, n, 0.0f) : -INFINITY;
         }
     }
-    __device__ void keep(float* to, int lane) const {
+    __device__ void keep(float* to, int lane, float log2e = LOG2E) const {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            to[i * 32 + lane] = scale[i] * LOG2E;
-            to[64 + i * 32 + lane] = bias[i] * LOG2E;
+            to[i * 32 + lane] = scale[i] * log2e;
+            to[64 + i * 32 + lane] = bias[i] * log2e;
         }
     }
 };
+// The entries of a warp's 32 rows and 64 columns: where they lie (on its way a tile ahead) and the first of them.
+struct Entries {
+    uint32_t first, count;
+    __device__ void find(const Params& p, uint32_t row, uint32_t column, uint32_t M) {
+        first = count = 0;
+        if (row < M) {
+            const uint16_t* at = p.offsets + (size_t)(row / 32) * p.groups1 + column / 64;
+            first = at[0];
+            count = at[1];   // (the end, until they are fetched)
+        }
+    }
+    __device__ const uint32_t* list(const Params& p, uint32_t row) const { return p.entries + (size_t)(row / 32) * p.block_entries + first; }
+};
+constexpr int ENTRIES_HELD = 2;   // words of 32 entries that are fetched before the accumulator is there
 // The accumulator has been read: one arrival on the even CTA's barrier.  (With release at the scope of the cluster the arrival
 // waits for the warp's stores to memory, which this barrier says nothing of.)
 __device__ __forceinline__ void arrive_even(uint32_t cluster_addr) {
@@ -365,6 +408,8 @@ __device__ __forceinline__ void arrive_even(uint32_t cluster_addr) {
 template <int EPI, int ACCS, bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+    constexpr int KIND = kind_of(EPI);
+    constexpr bool ENTRIES = has_entries(EPI), TWO = has_two(EPI);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr uint32_t STAGE = OPERAND_BYTES * (1 + ACCS);
@@ -401,7 +446,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     }
     // A kernel with `beside` runs beside the one before: that one has waited for those before it, or this one would not have been
     // launched, and it is waited for at the end, so that whoever waits for this kernel has waited for both.
-    if (EPI == STORE && p.beside) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (KIND == STORE && p.beside) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     else chain_entry();
     ptx::tc_fence_before_sync();
     __syncthreads();
@@ -409,7 +454,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
     constexpr uint32_t BUFFERS = ACCS == 1 ? 2 : 1;
-    constexpr bool BY_STRETCH = EPI == SUM && !BF16;   // stretches of K with a type and a factor of their own
+    constexpr bool BY_STRETCH = KIND == SUM && !BF16;   // stretches of K with a type and a factor of their own
     Work<EPI, ACCS> work(p, pair, pairs);
 
     if (warp == 0) {
@@ -489,7 +534,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 InParts in_parts;
                 for (uint32_t kb = work.k0; kb < work.k1 && ok;) {
                     const bool parts = BY_STRETCH && in_parts(p, work.n, kb);   // this stretch's products in bf16, and twice as many
-                    const uint32_t last = EPI == SUM ? work.stretch_end(kb) : work.k1, idesc = BY_STRETCH && parts ? idesc_bf16 : idesc_own;
+                    const uint32_t last = KIND == SUM ? work.stretch_end(kb) : work.k1, idesc = BY_STRETCH && parts ? idesc_bf16 : idesc_own;
                     const uint32_t end = BY_STRETCH && parts ? 2 * last - kb : last;
                     const uint32_t buf = done % BUFFERS;
                     if (done >= BUFFERS && !wait(&tmem_empty[buf], ((done / BUFFERS) & 1u) ^ 1u, s_error)) {
@@ -531,7 +576,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         // ------------------------------------------------------ epilogue (both CTAs, own rows)
         const uint32_t quarter = warp & 3, group = (uint32_t)(warp - 2) >> 2, mine = warp - 2;
         const uint32_t empty_even = ptx::cluster_map(tmem_empty, 0);
-        constexpr uint32_t STAGINGS = EPI == GRAD ? 2 : EPI == STORE ? 1 : 0;
+        constexpr uint32_t STAGINGS = KIND == GRAD ? 2 : KIND == STORE ? 1 : 0;
         uint8_t* staging = epi_smem + mine * STAGINGS * STAGING_BYTES;   // on 1024 bytes
         float* columns = reinterpret_cast<float*>(epi_smem + EPI_WARPS * STAGINGS * STAGING_BYTES + mine * COLUMN_BYTES);
         uint32_t done = 0;
@@ -556,37 +601,57 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         const uint32_t M = work.M;
         const uint32_t q2 = (lane & 3) * 2, r0 = lane >> 2;   // of the 16 x 64 form: first column of a pair, first row
 
-        if constexpr (EPI == LSE) {
+        if constexpr (KIND == LSE) {
             const uint32_t rows = work.m_tiles * BM;
             uint32_t m_now = 0xFFFFFFFFu, piece_now = 0;
-            float top = -INFINITY, sum = 0.0f;
+            float top = -INFINITY, sum = 0.0f, sum2 = 0.0f;
             int32_t target = -1;
             const auto leave = [&]() {
                 if (m_now == 0xFFFFFFFFu) return;
                 const uint32_t width = min(p.piece_tiles, work.n_tiles - piece_now * p.piece_tiles);
                 const uint32_t slot = pair - share_of(work.m_tiles * width, pairs).owner(m_now * width);
                 const size_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
-                p.row_part[piece_now * p.row_part_piece + (size_t)(slot * 4 + group) * rows + row] = make_float2(top, sum);
+                const size_t at = piece_now * p.row_part_piece + (size_t)(slot * 4 + group) * rows + row;
+                p.row_part[at] = make_float2(top, sum);
+                if (TWO) p.row_part2[at] = sum2;
             };
+            const float log2e = ENTRIES ? LOG2E * p.column_factor : LOG2E;
+            float* extract = columns + EPI_WARPS * COLUMN_BYTES / 4 - mine * (COLUMN_BYTES / 4) + mine * (EXTRACT_BYTES / 4);   // ENTRIES
             Columns ahead;
+            Entries entries{};
+            const auto fetch = [&]() {
+                ahead.fetch(p, work.n * BN + group * 64, lane);
+                if (ENTRIES) entries.find(p, work.m * BM + rank * 128 + quarter * 32, work.n * BN + group * 64, M);
+            };
             bool more = work.next();
-            if (more) ahead.fetch(p, work.n * BN + group * 64, lane);
+            if (more) fetch();
             while (more) {
                 const uint32_t n0 = work.n * BN + group * 64;
+                const uint32_t* list = nullptr;
+                float2* logits = nullptr;
+                uint32_t n_entries = 0, held[ENTRIES_HELD];
+                if (ENTRIES) {
+                    const uint32_t row = work.m * BM + rank * 128 + quarter * 32;
+                    list = entries.list(p, row);
+                    logits = p.entry_logits + (list - p.entries);
+                    n_entries = entries.count - entries.first;
+#pragma unroll
+                    for (int b = 0; b < ENTRIES_HELD; ++b) held[b] = b * 32 + lane < n_entries ? list[b * 32 + lane] : NO_ENTRY;
+                }
                 if (work.m != m_now || work.in_piece != piece_now) {
                     leave();
                     m_now = work.m;
                     piece_now = work.in_piece;
                     top = -INFINITY;
-                    sum = 0.0f;
+                    sum = sum2 = 0.0f;
                     const uint32_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
-                    target = row < M ? p.target[row] : -1;
+                    if (!ENTRIES) target = row < M ? p.target[row] : -1;
                 }
                 __syncwarp();
-                ahead.keep(columns, lane);
+                ahead.keep(columns, lane, log2e);
                 __syncwarp();
                 more = work.next();
-                if (more) ahead.fetch(p, work.n * BN + group * 64, lane);
+                if (more) fetch();
                 uint32_t taddr;
                 if (!filled(&taddr)) break;
                 // 16 columns are on their way while 16 are worked on
@@ -599,8 +664,32 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     tmem_landed(now);
                     if (c < 3) tmem_ld_32x16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
                     else drained();
+                    if constexpr (ENTRIES) {
+                        bool mine = false;
+#pragma unroll
+                        for (int b = 0; b < ENTRIES_HELD; ++b) mine |= held[b] != NO_ENTRY && entry_column(held[b]) / 16 == c;
+                        if (__any_sync(0xffffffffu, mine) || n_entries > ENTRIES_HELD * 32) {
+                            float4* to = reinterpret_cast<float4*>(extract + lane * EXTRACT_PITCH);   // (no bank conflicts)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                to[i] = make_float4(__uint_as_float(now[i * 4]), __uint_as_float(now[i * 4 + 1]), __uint_as_float(now[i * 4 + 2]),
+                                                    __uint_as_float(now[i * 4 + 3]));
+                            __syncwarp();
+                            const auto take = [&](uint32_t i, uint32_t bits) {
+                                const uint32_t column = entry_column(bits);
+                                if (bits == NO_ENTRY || column / 16 != c) return;
+                                const float a = extract[entry_row(bits) * EXTRACT_PITCH + column % 16];
+                                logits[i] = make_float2(a, fmaf(a, columns[column], columns[64 + column]));
+                            };
+#pragma unroll
+                            for (int b = 0; b < ENTRIES_HELD; ++b) take(b * 32 + lane, held[b]);
+#pragma unroll 4
+                            for (uint32_t i = ENTRIES_HELD * 32 + lane; i < n_entries; i += 32) take(i, list[i]);
+                            __syncwarp();
+                        }
+                    }
                     const int32_t hit = target - (int32_t)(n0 + c * 16);
-                    const bool hits = __any_sync(0xffffffffu, hit >= 0 && hit < 16);   // of the warp's rows
+                    const bool hits = !ENTRIES && __any_sync(0xffffffffu, hit >= 0 && hit < 16);   // of the warp's rows
                     uint64_t z[8];
                     float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -623,23 +712,35 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     best[0] = fmaxf(best[0], best[1]);
                     if (best[0] > top) {
                         sum *= exp2_fast(top - best[0]);   // top = -inf: 0 * 0
+                        if (TWO) sum2 *= exp2_fast((top - best[0]) * p.second_factor);
                         top = best[0];
                     }
                     const float base = top == -INFINITY ? 0.0f : -top;   // (a NaN among z makes the sum one)
                     const uint64_t base2 = two(base, base);
-                    uint64_t here[2] = {0, 0};
+                    uint64_t here[2] = {0, 0}, here2[2] = {0, 0};
+                    const uint64_t second = two(p.second_factor, p.second_factor);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float2 v = of_two(add2(z[i], base2));
+                        const uint64_t less = add2(z[i], base2);
+                        const float2 v = of_two(less);
                         here[i & 1] = add2(here[i & 1], two(exp2_fast(v.x), exp2_fast(v.y)));
+                        if (TWO) {
+                            const float2 u = of_two(mul2(less, second));
+                            here2[i & 1] = add2(here2[i & 1], two(exp2_fast(u.x), exp2_fast(u.y)));
+                        }
                     }
                     const float2 all = of_two(add2(here[0], here[1]));
                     sum += all.x + all.y;
+                    if (TWO) {
+                        const float2 all2 = of_two(add2(here2[0], here2[1]));
+                        sum2 += all2.x + all2.y;
+                    }
                 }
             }
             leave();
-        } else if constexpr (EPI == GRAD) {
-            const float from_log2 = *p.factor / LOG2E;   // scale * log2 e -> scale * 2^k
+        } else if constexpr (KIND == GRAD) {
+            const float log2e = ENTRIES ? LOG2E * p.column_factor : LOG2E;
+            const float from_log2 = *p.factor / log2e;   // scale * log2 e -> scale * 2^k
             const Share all = share_of(work.m_tiles * work.n_tiles, pairs);
             uint32_t n_now = 0xFFFFFFFFu;
             uint64_t g_sum[8], ga_sum[8];   // of column pairs 8 j + q2
@@ -671,6 +772,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 const bool in = row < M;
                 float* to = row_smem + turn * 128 + lane;
                 copy_word(to, p.lse2 + (in ? row : 0), in);
+                if (ENTRIES) {
+                    if (TWO) copy_word(to + 32, p.second_lse2 + (in ? row : 0), in);
+                    return;
+                }
                 copy_word(to + 32, p.target_acc + (in ? row : 0), in);
                 copy_word(to + 64, p.target_g + (in ? row : 0), in);
                 copy_word(to + 96, p.target + (in ? row : 0), in);
@@ -678,26 +783,41 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             const uint32_t blocks_at = ptx::smem_u32(staging) + ((lane >> 3) & 1) * 1024 + (lane & 7) * 128;   // of store_blocks: block b has
             const uint32_t block_piece = lane >> 4;                                                           // rows 8 (b % 2) .., piece b / 2
             uint32_t turn = 0;
+            Entries entries{};
             bool more = work.next();
-            if (more) fetch(0);
+            if (more) {
+                fetch(0);
+                if (ENTRIES) entries.find(p, work.m * BM + rank * 128 + quarter * 32, p.n_first + work.n * BN + group * 64, M);
+            }
             while (more) {
                 const uint32_t n0 = work.n * BN + group * 64, m0 = work.m * BM + rank * 128 + quarter * 32;
+                const uint32_t* list = nullptr;
+                uint32_t n_entries = 0, held[ENTRIES_HELD];
+                if (ENTRIES) {
+                    list = entries.list(p, m0);
+                    n_entries = entries.count - entries.first;
+#pragma unroll
+                    for (int b = 0; b < ENTRIES_HELD; ++b) held[b] = b * 32 + lane < n_entries ? list[b * 32 + lane] : NO_ENTRY;
+                }
                 if (work.n != n_now) {
                     leave();
                     n_now = work.n;
                     __syncwarp();
                     Columns c;
                     c.fetch(p, n0, lane);
-                    c.keep(columns, lane);
+                    c.keep(columns, lane, log2e);
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncwarp();
                 const float* rows = row_smem + turn * 128;
                 turn ^= 1;
                 const uint32_t first = p.n_first + n0;
-                const bool any = __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
+                const bool any = !ENTRIES && __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
                 more = work.next();
-                if (more) fetch(turn);
+                if (more) {
+                    fetch(turn);
+                    if (ENTRIES) entries.find(p, work.m * BM + rank * 128 + quarter * 32, p.n_first + work.n * BN + group * 64, M);
+                }
                 uint32_t taddr;
                 if (!filled(&taddr)) break;
                 taddr += group * 64;
@@ -707,13 +827,17 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 const auto half = [&](int h, auto targets) {
                     uint32_t r[2][8];   // 16 columns are on their way while 16 are worked on
                     tmem_ld_16x16(taddr + ((h * 16) << 16), r[0]);
-                    uint64_t l[2];
+                    uint64_t l[2], l2[2];
                     uint32_t at[2];   // the target's column less q2
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t row = h * 16 + i * 8 + r0;
                         const float lse = m0 + row < M ? -rows[row] : -INFINITY;
                         l[i] = two(lse, lse);
+                        if (TWO) {
+                            const float lse2 = m0 + row < M ? -rows[32 + row] : -INFINITY;
+                            l2[i] = two(lse2, lse2);
+                        }
                         if (decltype(targets)::value)
                             at[i] = m0 + row < M ? reinterpret_cast<const uint32_t*>(rows)[96 + row] - first - q2 : 0x80000000u;
                     }
@@ -735,8 +859,13 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 uint64_t a = (uint64_t)now[u * 4 + i * 2 + 1] << 32 | now[u * 4 + i * 2];
-                                const float2 e = of_two(add2(fma2(a, s, b), l[i]));
+                                const uint64_t z = fma2(a, s, b);
+                                const float2 e = of_two(add2(z, l[i]));
                                 uint64_t g = two(exp2_fast(e.x), exp2_fast(e.y));
+                                if (TWO) {
+                                    const float2 e2 = of_two(fma2(z, two(p.second_factor, p.second_factor), l2[i]));
+                                    g = add2(g, two(exp2_fast(e2.x), exp2_fast(e2.y)));
+                                }
                                 if (decltype(targets)::value) {
                                     const uint32_t row = h * 16 + i * 8 + r0;
                                     const bool x = at[i] == (uint32_t)(j + u) * 8, y = at[i] == (uint32_t)(j + u) * 8 + 1;
@@ -752,6 +881,19 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         }
                         // 16-byte piece c of row r at c ^ (r % 8), as the copy below reads it; no bank conflicts
                         store_blocks(to + (((j + block_piece) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+                    }
+                    if constexpr (ENTRIES) {
+                        __syncwarp();
+                        const auto put = [&](uint32_t bits) {
+                            if ((bits & ENTRY_DEAD) || (bits >> 10 & 1u) != (uint32_t)h) return;
+                            const uint32_t row = bits & 15u, column = entry_column(bits);
+                            *reinterpret_cast<uint16_t*>(staging + h * STAGING_BYTES + row * 128 + ((column / 8 ^ (row & 7)) << 4) + column % 8 * 2) =
+                                (uint16_t)(bits >> 16);
+                        };
+#pragma unroll
+                        for (int b = 0; b < ENTRIES_HELD; ++b) put(held[b]);
+#pragma unroll 4
+                        for (uint32_t i = ENTRIES_HELD * 32 + lane; i < n_entries; i += 32) put(list[i]);
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
@@ -770,7 +912,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             if (lane == 0) tma_store_done();
             __syncwarp();
             leave();
-        } else if constexpr (EPI == STORE) {
+        } else if constexpr (KIND == STORE) {
             const float alpha = p.factor ? *p.factor : 1.0f;
             const bool wide = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
             uint16_t* out = static_cast<uint16_t*>(p.out);
@@ -846,7 +988,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 }
             }
         } else {
-            static_assert(EPI != SUM || ACCS == 1, "");
+            static_assert(KIND != SUM || ACCS == 1, "");
             bool ok = true;
             while (ok && work.next()) {
                 float v[64];
@@ -906,7 +1048,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc_pair(tmem_base, 512);
     }
-    if (EPI == STORE && p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (KIND == STORE && p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (threadIdx.x == 0 && *s_error) report_wait(p.status, 64u + *s_error);
 }
 

@@ -67,6 +67,7 @@ ABI_SYMBOLS = (
     "ullis_cuda_tape_layer_norm_backward_workspace", "ullis_cuda_tape_layer_norm_backward",
     "ullis_cuda_tape_weight_grad_workspace", "ullis_cuda_tape_weight_grad", "ullis_cuda_head_ce_grad_workspace",
     "ullis_cuda_head_ce_grad", "ullis_cuda_embed", "ullis_cuda_embed_grad_workspace", "ullis_cuda_embed_grad", "ullis_cuda_top_logits",
+    "ullis_cuda_head_distill_grad_workspace", "ullis_cuda_head_distill_grad",
 )
 
 

@@ -71,6 +71,8 @@ _ARGTYPES = {
     "embed_grad_workspace": (_V, _I, _Z, _Z, _Z, _V),
     "embed_grad": (_V, _V, _I, _V, _U, _V, _Z, _Z, _Z, _Z, _F, _V, _V, _Z),
     "top_logits": (_V, _V, _I, _V, _Z, _Z, _Z, _Z, _V, _V),
+    "head_distill_grad_workspace": (_V, _Z, _Z, _Z, _Z, _I, _I, _V),
+    "head_distill_grad": (_V, _V, _I, _V, _Z, _V, _V, _V, _V, _V, _I, _V, _Z, _F, _F, _V, _U, _Z, _Z, _Z, _Z, _F, _V, _V, _V, _V, _V, _V, _Z),
     "head_ce_grad_workspace": (_V, _Z, _Z, _Z, _I, _V),
     "head_ce_grad": (_V, _V, _I, _V, _Z, _V, _V, _V, _V, _V, _U, _Z, _Z, _Z, _Z, _F, _V, _V, _V, _V, _V, _V, _Z),
 }
@@ -331,11 +333,73 @@ class DeviceOps:
         packed head is `weight` int32 words of sign bits in checkpoint order with `scale` float16 [vocab]; a dense one is
         `weight` [vocab, channels] in hidden's type and no scale.  bias float16 [vocab] or None.  Gradients are of
         loss_scale * sum of row_loss; that of a packed weight is of the +/-1 values."""
-        torch = _torch()
+        _torch()
         rows, channels, stride = self._matrix(hidden, "hidden", _16)
         self._vector(labels, "labels", _I32, rows)
+        vocab = self._head(hidden, channels, weight, scale, bias)
+        ignore, time = _id32(ignore_id), self._time(hidden, rows, time)
+        outputs, copies = self._head_outputs(hidden, rows, channels, vocab, weight, scale, bias)
+        at = weight.data_ptr()
+        work, size = self._workspace(hidden, "head_ce_grad", rows, channels, vocab, copies)
+        self._check(self._lib.ullis_cuda_head_ce_grad(
+            self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], hidden.data_ptr(), stride, at if scale is not None else None,
+            at if scale is None else None, _p(scale), _p(bias), labels.data_ptr(), ignore, rows, time, channels, vocab,
+            float(loss_scale), *(_p(t) for t in outputs), work.data_ptr(), size))
+        return outputs
+
+    def head_distill_grad(self, hidden, weight, top_ids, top_logits, *, scale=None, bias=None, labels=None, alpha: float = 1.0,
+                          temperature: float = 1.0, ignore_id: int = 0xFFFFFFFF, time=None, loss_scale: float = 1.0) -> HeadGrad:
+        """A head's distillation from a teacher's largest logits, with its gradient; the student's logits are never kept.
+
+        hidden, weight, scale, bias, ignore_id, time, loss_scale and what is returned are `head_ce_grad`'s.  top_ids int32 and
+        top_logits (float32, float16, bfloat16) [..., k], k at most 256: what the teacher says of the token after each row, as
+        `top_logits` gives it; a negative id is no entry, and one that comes twice has the sum of both probabilities.  The
+        teacher's distribution is softmax(top_logits / temperature) over a row's entries, and
+
+            row_loss = (1 - alpha) * cross-entropy(label) + alpha * temperature^2 * KL(teacher, softmax(logits / temperature)).
+
+        With `labels` a row counts as in `head_ce_grad`, for both parts; one without entries has the first part alone.  Without
+        labels there is the second part alone, and a row counts if it has entries.  alpha in 0..1, temperature in 1/128..128."""
+        _torch()
+        rows, channels, stride = self._matrix(hidden, "hidden", _16)
+        if labels is not None:
+            self._vector(labels, "labels", _I32, rows)
+        self._refuse(top_ids, "top_ids", _I32)
+        self._refuse(top_logits, "top_logits", _DTYPES)
+        top = top_ids.shape[-1] if top_ids.dim() else 0
+        if not 0 < top <= 256:
+            raise UllisCudaError(ERR_SHAPE, "head distillation takes 1 to 256 entries of a row")
+        if top_ids.shape != top_logits.shape:
+            _shape_error("top_logits", top_logits.shape, top_ids.shape)
+        if top_ids.numel() != rows * top:
+            _shape_error("top_ids", top_ids.shape, (rows, top))
+        if not (top_ids.is_contiguous() and top_logits.is_contiguous()):
+            raise UllisCudaError(ERR_SHAPE, "top_ids and top_logits must be contiguous")
+        alpha, temperature = float(alpha), float(temperature)
+        if not 0.0 <= alpha <= 1.0 or not 1 / 128 <= temperature <= 128:
+            raise UllisCudaError(ERR_ARG, "alpha must be in 0 .. 1, temperature in 1/128 .. 128")
+        vocab = self._head(hidden, channels, weight, scale, bias)
+        ignore, time = _id32(ignore_id), self._time(hidden, rows, time)
+        outputs, copies = self._head_outputs(hidden, rows, channels, vocab, weight, scale, bias)
+        at = weight.data_ptr()
+        work, size = self._workspace(hidden, "head_distill_grad", rows, channels, vocab, top, int(labels is not None), copies)
+        self._check(self._lib.ullis_cuda_head_distill_grad(
+            self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], hidden.data_ptr(), stride, at if scale is not None else None,
+            at if scale is None else None, _p(scale), _p(bias), top_ids.data_ptr(), _DTYPES[top_logits.dtype], top_logits.data_ptr(), top,
+            alpha, temperature, _p(labels), ignore, rows, time, channels, vocab, float(loss_scale), *(_p(t) for t in outputs),
+            work.data_ptr(), size))
+        return outputs
+
+    def _time(self, hidden, rows, time) -> int:
         if time is None:
             time = max(1, hidden.shape[-2] if hidden.dim() == 3 else rows)
+        time = int(time)
+        if not 0 < time < 1 << 31 or rows % time:
+            raise UllisCudaError(ERR_SHAPE, "rows must be a multiple of time")
+        return time
+
+    def _head(self, hidden, channels, weight, scale, bias) -> int:
+        """The vocabulary of a packed or dense head."""
         if scale is not None:
             self._refuse(scale, "scale", _F16)
             vocab = scale.numel()
@@ -348,20 +412,12 @@ class DeviceOps:
             vocab = weight.shape[0]
         if bias is not None:
             self._vector(bias, "bias", _F16, vocab)
-        ignore, time = _id32(ignore_id), int(time)
-        if not 0 < time < 1 << 31 or rows % time:
-            raise UllisCudaError(ERR_SHAPE, "rows must be a multiple of time")
-        row_loss = torch.empty(rows, dtype=torch.float32, device=hidden.device)
-        g_hidden = _like(hidden, hidden.dtype)
-        g_weight = torch.empty(vocab, channels, dtype=hidden.dtype, device=hidden.device)
-        g_scale = None if scale is None else _like(scale, torch.float32)
-        g_bias = None if bias is None else _like(bias, torch.float32)
-        at = weight.data_ptr()
-        copies = scale is not None or channels % 8 != 0 or at % 16 != 0
-        work, size = self._workspace(hidden, "head_ce_grad", rows, channels, vocab, int(copies))
-        self._check(self._lib.ullis_cuda_head_ce_grad(
-            self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], hidden.data_ptr(), stride, at if scale is not None else None,
-            at if scale is None else None, _p(scale), _p(bias), labels.data_ptr(), ignore, rows, time, channels, vocab,
-            float(loss_scale), row_loss.data_ptr(), g_hidden.data_ptr(), g_weight.data_ptr(), _p(g_scale), _p(g_bias),
-            work.data_ptr(), size))
-        return HeadGrad(row_loss, g_hidden, g_weight, g_scale, g_bias)
+        return vocab
+
+    def _head_outputs(self, hidden, rows, channels, vocab, weight, scale, bias):
+        """(where the gradients go, whether the workspace holds the weights)."""
+        empty, f32, device = _TORCH.empty, _TORCH.float32, hidden.device
+        outputs = HeadGrad(empty(rows, dtype=f32, device=device), _like(hidden, hidden.dtype),
+                           empty(vocab, channels, dtype=hidden.dtype, device=device), None if scale is None else _like(scale, f32),
+                           None if bias is None else _like(bias, f32))
+        return outputs, int(scale is not None or channels % 8 != 0 or weight.data_ptr() % 16 != 0)
