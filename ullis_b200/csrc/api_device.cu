@@ -306,7 +306,7 @@ int32_t ullis_cuda_embed_grad_workspace(const ullis_cuda_runtime* rt, int32_t dt
     return workspace_of(rt, bytes, [&] {
         need_dtype(dtype, true);
         need_embed(rows, channels, vocab);
-        return dev::embed_grad_workspace(rt, dtype, rows, channels);
+        return dev::embed_grad_workspace(rt, rows, channels);
     });
 }
 
@@ -325,7 +325,7 @@ int32_t ullis_cuda_embed_grad(ullis_cuda_runtime* rt, void* cuda_stream, int32_t
         }
         need_array(tokens, "tokens", 4);
         need_array(gy, "gy", dev::size_of(dtype));
-        need_workspace(workspace, workspace_bytes, dev::embed_grad_workspace(rt, dtype, rows, channels));
+        need_workspace(workspace, workspace_bytes, dev::embed_grad_workspace(rt, rows, channels));
         dev::embed_grad(s, dtype, tokens, ignore_id, dev::Rows{gy, gy_stride}, rows, channels, vocab, scale, g, workspace);
     });
 }

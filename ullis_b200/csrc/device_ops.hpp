@@ -66,7 +66,7 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
 // its gradient g [vocab, channels] f32, which workspace is for
 void embed(const Stream& s, int table_dtype, Rows table, const uint32_t* tokens, uint32_t ignore_id, float scale, size_t rows, size_t channels,
            size_t vocab, int dtype, void* y);
-size_t embed_grad_workspace(const ullis_cuda_runtime* rt, int dtype, size_t rows, size_t channels);
+size_t embed_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels);
 void embed_grad(const Stream& s, int dtype, const uint32_t* tokens, uint32_t ignore_id, Rows gy, size_t rows, size_t channels, size_t vocab,
                 float scale, float* g, void* workspace);
 

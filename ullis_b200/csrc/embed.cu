@@ -6,6 +6,7 @@
 // The gradient's sums have a fixed order, with no atomics: the rows of a token in rising order, in pieces where there are many.
 #include <algorithm>
 
+#include "block_sort.cuh"
 #include "device_ops.hpp"
 #include "tape.cuh"
 
@@ -19,23 +20,24 @@ size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 size_t ceil_div(size_t n, size_t by) { return (n + by - 1) / by; }
 bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-// N channels from c on of a row of C, past its end zeros.  VEC: whole or absent, on their own size.
-template <bool VEC, int N, typename T>
+// A lane's N channels of a row: side by side from c on, read and written at once where they lie on their own size (WIDE), else
+// GAP apart, so that neighbouring threads have neighbouring channels; past the row's end zeros.
+template <bool WIDE, int N, int GAP, typename T>
 __device__ __forceinline__ void load_channels(const T* row, uint32_t c, uint32_t C, float (&v)[N]) {
-    __align__(16) T t[N];
-    if constexpr (VEC) {
+    if constexpr (WIDE) {
+        __align__(16) T t[N];
         if constexpr (sizeof(T) * N == 16) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(row + c);
         else *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(row + c);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = tape::to_float(t[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = c + i < C ? tape::to_float(row[c + i]) : 0.0f;
+        for (int i = 0; i < N; ++i) v[i] = c + i * GAP < C ? tape::to_float(row[c + i * GAP]) : 0.0f;
     }
 }
-template <bool VEC, int N, typename T>
+template <bool WIDE, int N, int GAP, typename T>
 __device__ __forceinline__ void store_channels(T* row, uint32_t c, uint32_t C, const float (&v)[N]) {
-    if constexpr (VEC) {
+    if constexpr (WIDE) {
         __align__(16) T t[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) t[i] = tape::from_float<T>(v[i]);
@@ -45,22 +47,19 @@ __device__ __forceinline__ void store_channels(T* row, uint32_t c, uint32_t C, c
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (c + i < C) row[c + i] = tape::from_float<T>(v[i]);
+            if (c + i * GAP < C) row[c + i * GAP] = tape::from_float<T>(v[i]);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ lookup
 constexpr int PER_THREAD = 2;   // chunks, their loads in flight together
-// A thread has chunks of as many channels as the wider type has in 16 bytes.
-template <typename A, typename B>
-constexpr int WIDTH = 16 / (int)(sizeof(A) > sizeof(B) ? sizeof(A) : sizeof(B));
-
-template <typename T, typename Y, bool VEC>
+// A thread has chunks of N channels.
+template <typename T, typename Y, int N>
 __global__ void __launch_bounds__(THREADS)
 embed_kernel(const T* __restrict__ table, size_t stride, const uint32_t* __restrict__ tokens, uint32_t ignore_id, float scale, uint32_t rows,
              uint32_t C, uint32_t vocab, uint32_t per_row, Y* __restrict__ y) {
     chain_entry();
-    constexpr int N = WIDTH<T, Y>;
+    constexpr bool WIDE = N > 1;
     size_t row[PER_THREAD];
     uint32_t c[PER_THREAD], token[PER_THREAD];
     float v[PER_THREAD][N];
@@ -75,7 +74,7 @@ embed_kernel(const T* __restrict__ table, size_t stride, const uint32_t* __restr
     for (int k = 0; k < PER_THREAD; ++k) {
         const float other = token[k] == ignore_id ? 0.0f : NAN;
         if (token[k] != ignore_id && token[k] < vocab) {
-            load_channels<VEC>(table + token[k] * stride, c[k], C, v[k]);
+            load_channels<WIDE, N, 1>(table + token[k] * stride, c[k], C, v[k]);
 #pragma unroll
             for (int i = 0; i < N; ++i) v[k][i] *= scale;
         } else {
@@ -85,17 +84,25 @@ embed_kernel(const T* __restrict__ table, size_t stride, const uint32_t* __restr
     }
 #pragma unroll
     for (int k = 0; k < PER_THREAD; ++k)
-        if (row[k] < rows) store_channels<VEC>(y + row[k] * C, c[k], C, v[k]);
+        if (row[k] < rows) store_channels<WIDE, N, 1>(y + row[k] * C, c[k], C, v[k]);
 }
 
+template <typename T, typename Y, int N>
+bool embed_by(const Stream& s, Rows table, const uint32_t* tokens, uint32_t ignore_id, float scale, size_t rows, size_t C, size_t vocab, void* y) {
+    if (C % N || table.stride % N || !aligned(table.data, N * sizeof(T)) || !aligned(y, N * sizeof(Y))) return false;
+    const uint32_t per_row = (uint32_t)(C / N);
+    s.chain("embed", embed_kernel<T, Y, N>, (unsigned)ceil_div(rows * per_row, PER_THREAD * THREADS), THREADS, 0, static_cast<const T*>(table.data),
+            table.stride, tokens, ignore_id, scale, (uint32_t)rows, (uint32_t)C, (uint32_t)vocab, per_row, static_cast<Y*>(y));
+    return true;
+}
+// As many channels to a chunk as the wider type has in 16 bytes; 16-bit rows on 8 bytes half of them; others one.
 template <typename T, typename Y>
 void embed_as(const Stream& s, Rows table, const uint32_t* tokens, uint32_t ignore_id, float scale, size_t rows, size_t C, size_t vocab, void* y) {
-    constexpr int N = WIDTH<T, Y>;
-    const bool vec = C % N == 0 && table.stride % N == 0 && aligned(table.data, N * sizeof(T)) && aligned(y, N * sizeof(Y));
-    const uint32_t per_row = (uint32_t)ceil_div(C, N);
-    s.chain("embed", vec ? embed_kernel<T, Y, true> : embed_kernel<T, Y, false>, (unsigned)ceil_div(rows * per_row, PER_THREAD * THREADS), THREADS,
-            0, static_cast<const T*>(table.data), table.stride, tokens, ignore_id, scale, (uint32_t)rows, (uint32_t)C, (uint32_t)vocab, per_row,
-            static_cast<Y*>(y));
+    constexpr int N = 16 / (int)(sizeof(T) > sizeof(Y) ? sizeof(T) : sizeof(Y));
+    if (embed_by<T, Y, N>(s, table, tokens, ignore_id, scale, rows, C, vocab, y)) return;
+    if constexpr (N == 8)
+        if (embed_by<T, Y, 4>(s, table, tokens, ignore_id, scale, rows, C, vocab, y)) return;
+    embed_by<T, Y, 1>(s, table, tokens, ignore_id, scale, rows, C, vocab, y);
 }
 template <typename T>
 void embed_from(const Stream& s, int dtype, Rows table, const uint32_t* tokens, uint32_t ignore_id, float scale, size_t rows, size_t C,
@@ -124,12 +131,12 @@ __device__ __forceinline__ uint32_t below(const uint32_t* list, uint32_t n, uint
 // threads per row of gy, the groups' sums added in their order.
 constexpr uint32_t FEW = 1024;
 
-template <typename T, bool VEC>
+template <typename T, int N>
 __global__ void __launch_bounds__(THREADS)
 embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, const T* __restrict__ gy, size_t stride, uint32_t rows, uint32_t C,
                       uint32_t vocab, float scale, float* __restrict__ g) {
     chain_entry();
-    constexpr int N = tape::CHUNK<T>;
+    constexpr bool WIDE = N > 1;
     __shared__ uint32_t found_token[FEW], found_row[FEW], token_at[FEW], row_at[FEW], warp_counts[THREADS / 32];
     __shared__ float sums[THREADS][N + 1];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -182,7 +189,7 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
                 for (; k + 3 * groups < end; k += 4 * groups) {
                     float v[4][N];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) load_channels<VEC>(gy + row_at[k + u * groups] * stride, c, C, v[u]);
+                    for (int u = 0; u < 4; ++u) load_channels<WIDE, N, 1>(gy + row_at[k + u * groups] * stride, c, C, v[u]);
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -190,7 +197,7 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
                 }
                 for (; k < end; k += groups) {
                     float v[N];
-                    load_channels<VEC>(gy + row_at[k] * stride, c, C, v);
+                    load_channels<WIDE, N, 1>(gy + row_at[k] * stride, c, C, v);
 #pragma unroll
                     for (int e = 0; e < N; ++e) sum[e] += v[e];
                 }
@@ -221,73 +228,97 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
 // Tokens are sorted by chunks in shared memory (beside which other CTAs write the table's zeros), an element's place among all is its
 // place in its chunk and what searches in the others give, and warps sum runs of rows in that order, a fixed number of
 // places each whatever the tokens are: a run that ends in another warp's places leaves a part of its sum, and a last launch adds those.
-constexpr uint32_t SORT_THREADS = 1024;
+constexpr uint32_t SORT_EACH = 8;   // keys to a thread
 
 // Keys token << BITS | place, padded with the largest.
 template <typename K, uint32_t BITS>
-__global__ void __launch_bounds__(SORT_THREADS)
+__global__ void __launch_bounds__((1u << BITS) / SORT_EACH)
 embed_sort_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, uint32_t rows, uint32_t vocab, uint32_t chunks,
                   uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row, float* __restrict__ g, size_t elements) {
     chain_entry();
-    constexpr uint32_t SIZE = 1u << BITS;
+    constexpr uint32_t SIZE = 1u << BITS, SORT_THREADS = SIZE / SORT_EACH;
     if (blockIdx.x >= chunks) {
         const size_t at = (size_t)(blockIdx.x - chunks) * SORT_THREADS + threadIdx.x, step = (size_t)(gridDim.x - chunks) * SORT_THREADS;
         size_t quads = 0;
         if (reinterpret_cast<uintptr_t>(g) % 16 == 0) {
             quads = elements / 4;
+#pragma unroll 4
             for (size_t i = at; i < quads; i += step) reinterpret_cast<float4*>(g)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         for (size_t i = quads * 4 + at; i < elements; i += step) g[i] = 0.0f;
         return;
     }
-    extern __shared__ uint8_t smem_raw[];
-    K* keys = reinterpret_cast<K*>(smem_raw);
-    const uint32_t base = blockIdx.x * SIZE;
-    for (uint32_t i = threadIdx.x; i < SIZE; i += SORT_THREADS) {
-        K key = ~(K)0;
-        if (base + i < rows) {
-            uint32_t token = tokens[base + i];
-            if (token == ignore_id || token > vocab) token = vocab;   // behind all others
-            key = (K)token << BITS | i;
-        }
-        keys[i] = key;
-    }
-    for (uint32_t run = 2; run <= SIZE; run <<= 1) {
-        for (uint32_t half = run >> 1; half > 0; half >>= 1) {
-            __syncthreads();
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    const uint32_t base = blockIdx.x * SIZE, first = threadIdx.x * SORT_EACH;
+    K keys[SORT_EACH];
 #pragma unroll
-            for (uint32_t i = threadIdx.x; i < SIZE / 2; i += SORT_THREADS) {
-                // the first step of a run compares mirrored places, so that all runs rise
-                const uint32_t low = (i & ~(half - 1)) * 2 + (i & (half - 1));
-                const uint32_t high = half == run >> 1 ? low ^ (run - 1) : low + half;
-                const K a = keys[low], b = keys[high];
-                if (a > b) {
-                    keys[low] = b;
-                    keys[high] = a;
-                }
-            }
+    for (uint32_t i = 0; i < SORT_EACH; ++i) {
+        keys[i] = ~(K)0;
+        if (base + first + i < rows) {
+            uint32_t token = tokens[base + first + i];
+            if (token == ignore_id || token > vocab) token = vocab;   // behind all others
+            keys[i] = (K)token << BITS | (first + i);
         }
     }
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < SIZE && base + i < rows; i += SORT_THREADS) {
-        sorted_token[base + i] = (uint32_t)(keys[i] >> BITS);
-        sorted_row[base + i] = base + (uint32_t)(keys[i] & (SIZE - 1));
+    block_sort<K, SORT_EACH, SORT_THREADS>(keys, reinterpret_cast<K*>(smem_raw));
+#pragma unroll
+    for (uint32_t i = 0; i < SORT_EACH; ++i) {
+        if (base + first + i >= rows) break;
+        sorted_token[base + first + i] = (uint32_t)(keys[i] >> BITS);
+        sorted_row[base + first + i] = base + (uint32_t)(keys[i] & (SIZE - 1));
     }
 }
 
+// A warp has 32 elements of a chunk, whose tokens lie close together.  Its lanes search the places of the first and the last of them
+// in 32 other chunks at once; what lies between two such places, mostly less than a warp's width, is fetched and searched by shuffles.
 __global__ void __launch_bounds__(THREADS)
 embed_rank_kernel(const uint32_t* __restrict__ chunk_token, const uint32_t* __restrict__ chunk_row, uint32_t rows, uint32_t size, uint32_t chunks,
                   uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row) {
     chain_entry();
-    const uint32_t i = blockIdx.x * THREADS + threadIdx.x;
-    if (i >= rows) return;
-    const uint32_t own = i / size, token = chunk_token[i];
+    constexpr uint32_t ALL = 0xffffffffu;
+    const uint32_t first = (blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5)) * 32, lane = threadIdx.x & 31;
+    if (first >= rows) return;
+    const uint32_t i = min(first + lane, rows - 1), own = first / size, token = chunk_token[i];   // (a warp's are of one chunk)
+    const uint32_t row = chunk_row[i], from = __shfl_sync(ALL, token, 0), to = __shfl_sync(ALL, token, 31);
     uint32_t rank = i - own * size;
-#pragma unroll 4
-    for (uint32_t c = 0; c < chunks; ++c)
-        if (c != own) rank += below(chunk_token + c * size, min(size, rows - c * size), token, c < own);
-    sorted_token[rank] = token;
-    sorted_row[rank] = chunk_row[i];
+    for (uint32_t c0 = 0; c0 < chunks; c0 += 32) {
+        uint32_t low = 0, high = 0;
+        const uint32_t c = c0 + lane;
+        if (c < chunks && c != own) {
+            const uint32_t n = min(size, rows - c * size);
+            low = below(chunk_token + c * size, n, from, c < own);
+            high = below(chunk_token + c * size, n, to, c < own);
+        }
+        const uint32_t end = min(32u, chunks - c0);
+        const auto fetch = [&](uint32_t k) {
+            const uint32_t begin = __shfl_sync(ALL, low, k), stop = __shfl_sync(ALL, high, k);
+            return begin + lane < stop ? chunk_token[(c0 + k) * size + begin + lane] : 0xFFFFFFFFu;
+        };
+        uint32_t next = fetch(0);
+        for (uint32_t k = 0; k < end; ++k) {
+            const uint32_t begin = __shfl_sync(ALL, low, k), stop = __shfl_sync(ALL, high, k), here = next;
+            if (k + 1 < end) next = fetch(k + 1);
+            rank += begin;
+            if (begin == stop) continue;
+            const uint32_t limit = token + (c0 + k < own);
+            if (stop - begin <= 32) {
+                uint32_t at = 0;
+#pragma unroll
+                for (uint32_t step = 16; step > 0; step >>= 1) {
+                    const uint32_t value = __shfl_sync(ALL, here, at + step - 1);
+                    at += value < limit ? step : 0u;
+                }
+                at += __shfl_sync(ALL, here, at) < limit;   // (31 of 32 have been told apart)
+                rank += at;
+            } else {
+                rank += below(chunk_token + (c0 + k) * size + begin, stop - begin, token, c0 + k < own);
+            }
+        }
+    }
+    if (first + lane < rows) {
+        sorted_token[rank] = token;
+        sorted_row[rank] = row;
+    }
 }
 
 struct GradSums {
@@ -299,11 +330,10 @@ struct GradSums {
     float *g, *head, *tail;        // parts of sums that began before a warp's places, and that go on behind them: [warp][C]
 };
 // A warp has `places` (a power of two, at most 32) places of the sorted order and 32 chunks of channels.
-template <typename T, bool VEC>
+template <typename T, int N, bool WIDE>
 __global__ void __launch_bounds__(THREADS)
 embed_sums_kernel(const GradSums o) {
     chain_entry();
-    constexpr int N = tape::CHUNK<T>;
     const uint32_t lane = threadIdx.x & 31;
     const size_t warp = (size_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
     const uint32_t tile = (uint32_t)(warp / o.blocks), block = (uint32_t)(warp - (size_t)tile * o.blocks);
@@ -312,7 +342,7 @@ embed_sums_kernel(const GradSums o) {
     const uint32_t n = min(o.places, o.rows - first), at = first + min(lane, n - 1);
     const uint32_t my_token = o.token[at], my_row = o.row[at];
     const uint32_t before = first > 0 ? o.token[first - 1] : 0xFFFFFFFFu, after = first + n < o.rows ? o.token[first + n] : 0xFFFFFFFFu;
-    const uint32_t c = (block * 32 + lane) * N;
+    const uint32_t c = block * 32 * N + lane * (WIDE ? N : 1);
     const bool in = c < o.C;
     const T* gy = static_cast<const T*>(o.gy);
     float sum[N] = {};
@@ -324,7 +354,7 @@ embed_sums_kernel(const GradSums o) {
         for (int u = 0; u < AHEAD; ++u) {
             const uint32_t k = min(k0 + u, n - 1);
             const uint32_t token = __shfl_sync(0xffffffffu, my_token, k), row = __shfl_sync(0xffffffffu, my_row, k);
-            if (in && token < o.vocab && k0 + u < n) load_channels<VEC>(gy + row * o.stride, c, o.C, v[u]);
+            if (in && token < o.vocab && k0 + u < n) load_channels<WIDE, N, 32>(gy + row * o.stride, c, o.C, v[u]);
             else
 #pragma unroll
                 for (int e = 0; e < N; ++e) v[u][e] = 0.0f;
@@ -344,7 +374,7 @@ embed_sums_kernel(const GradSums o) {
                 const float times = whole ? o.scale : 1.0f;
 #pragma unroll
                 for (int e = 0; e < N; ++e) sum[e] *= times;
-                store_channels<VEC>(to, c, o.C, sum);
+                store_channels<WIDE, N, 32>(to, c, o.C, sum);
             }
 #pragma unroll
             for (int e = 0; e < N; ++e) sum[e] = 0.0f;
@@ -353,42 +383,69 @@ embed_sums_kernel(const GradSums o) {
     }
 }
 
-// The sums that several warps have parts of: the tail of the warp they began in and the heads of those after it, in their order, by
-// eight warps a stretch each.  A CTA has 128 channels of what began in one warp's places.
+// The sums that several warps have parts of: the tail of the warp they began in and the heads of those after it, in their order.  A CTA
+// has 128 channels of what began in the places of eight warps: sums of few parts a warp each, then those of many one after the other, by
+// eight warps a stretch of the parts each.
+constexpr uint32_t FEW_PARTS = 16;
 __global__ void __launch_bounds__(THREADS)
-embed_join_kernel(const GradSums o) {
+embed_join_kernel(const GradSums o, uint32_t tiles) {
     chain_entry();
-    const uint32_t per_tile = (o.C + 127) / 128, tile = blockIdx.x / per_tile, block = blockIdx.x - tile * per_tile;
-    const uint32_t first = tile * o.places, next = first + o.places;   // (a last warp's sums go on nowhere)
-    const uint32_t token = o.token[next - 1];
-    if (token >= o.vocab || o.token[next] != token || (first > 0 && o.token[first - 1] == token)) return;
-    // one behind the last warp with a part: warps whose first place has the token
-    uint32_t low = tile + 1, high = (o.rows + o.places - 1) / o.places;
-    while (low < high) {
-        const uint32_t middle = (low + high) >> 1;
-        if (o.token[middle * o.places] == token) low = middle + 1;
-        else high = middle;
+    constexpr uint32_t WARPS = THREADS / 32;
+    __shared__ uint32_t all_parts[WARPS];
+    __shared__ float sums[WARPS][128];
+    const uint32_t per_tile = (o.C + 127) / 128, block = blockIdx.x % per_tile, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t first_tile = blockIdx.x / per_tile * WARPS, tile = first_tile + warp, c = block * 128 + lane;
+    uint32_t parts = 0;   // heads
+    if (tile + 1 < tiles) {   // (the last warp's sums go on nowhere)
+        const uint32_t first = tile * o.places, next = first + o.places, token = o.token[next - 1];
+        if (token < o.vocab && o.token[next] == token && !(first > 0 && o.token[first - 1] == token)) {
+            // warps whose first place has the token: 32 of them at a time
+            for (uint32_t t = tile + 1;; t += 32) {
+                const bool more = t + lane < tiles && o.token[(t + lane) * o.places] == token;
+                const uint32_t mask = __ballot_sync(0xffffffffu, more);
+                parts += __popc(mask);
+                if (mask != 0xffffffffu) break;
+            }
+        }
     }
-    const uint32_t parts = low - tile - 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = block * 128 + lane;
-    const uint32_t from = (uint32_t)((uint64_t)warp * parts / 8), to = (uint32_t)((uint64_t)(warp + 1) * parts / 8);
-    __shared__ float sums[8][128];
-    float sum[4] = {};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (warp == 0 && c + 32 * e < o.C) sum[e] = o.tail[(size_t)tile * o.C + c + 32 * e];
+    const auto add = [&](float (&sum)[4], uint32_t of, uint32_t from, uint32_t to) {   // heads [from, to) of the sum that began in warp `of`
 #pragma unroll 4
-    for (uint32_t k = from; k < to; ++k)
+        for (uint32_t k = from; k < to; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + 32 * e < o.C) sum[e] += o.head[(size_t)(of + 1 + k) * o.C + c + 32 * e];
+    };
+    const auto tail = [&](float (&sum)[4], uint32_t of, bool wanted) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = wanted && c + 32 * e < o.C ? o.tail[(size_t)of * o.C + c + 32 * e] : 0.0f;
+    };
+    float sum[4];
+    if (parts > 0 && parts <= FEW_PARTS) {
+        tail(sum, tile, true);
+        add(sum, tile, 0, parts);
+        float* to = o.g + (size_t)o.token[tile * o.places + o.places - 1] * o.C;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (c + 32 * e < o.C) sum[e] += o.head[(size_t)(tile + 1 + k) * o.C + c + 32 * e];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sums[warp][lane + 32 * e] = sum[e];
+            if (c + 32 * e < o.C) to[c + 32 * e] = sum[e] * o.scale;
+    }
+    if (lane == 0) all_parts[warp] = parts;
     __syncthreads();
-    if (threadIdx.x >= 128 || block * 128 + threadIdx.x >= o.C) return;
-    float all = sums[0][threadIdx.x];
+    for (uint32_t w = 0; w < WARPS; ++w) {
+        const uint32_t n = all_parts[w], of = first_tile + w;
+        if (n <= FEW_PARTS) continue;
+        tail(sum, of, warp == 0);
+        add(sum, of, (uint32_t)((uint64_t)warp * n / WARPS), (uint32_t)((uint64_t)(warp + 1) * n / WARPS));
 #pragma unroll
-    for (int w = 1; w < 8; ++w) all += sums[w][threadIdx.x];
-    o.g[(size_t)token * o.C + block * 128 + threadIdx.x] = all * o.scale;
+        for (int e = 0; e < 4; ++e) sums[warp][lane + 32 * e] = sum[e];
+        __syncthreads();
+        if (threadIdx.x < 128 && block * 128 + threadIdx.x < o.C) {
+            float all = sums[0][threadIdx.x];
+#pragma unroll
+            for (uint32_t k = 1; k < WARPS; ++k) all += sums[k][threadIdx.x];
+            o.g[(size_t)o.token[of * o.places + o.places - 1] * o.C + block * 128 + threadIdx.x] = all * o.scale;
+        }
+        __syncthreads();
+    }
 }
 
 struct GradPlan {
@@ -396,14 +453,15 @@ struct GradPlan {
     uint32_t bits, chunks, places, blocks;
     size_t tiles, chunk_token, chunk_row, token, row, head, tail, bytes;
 };
-GradPlan grad_plan(const ullis_cuda_runtime* rt, int dtype, size_t rows, size_t C) {
+GradPlan grad_plan(const ullis_cuda_runtime* rt, size_t rows, size_t C) {
     GradPlan p{};
     p.few = rows <= FEW;
     if (p.few) return p;
-    p.bits = rows <= 32768 ? 11 : 13;
+    // Chunks of 2048 are sorted faster than those of 8192 by more than the search in four times as many takes, up to 64 of them.
+    p.bits = rows <= 131072 ? 11 : 13;
     p.chunks = (uint32_t)ceil_div(rows, (size_t)1 << p.bits);
-    p.blocks = (uint32_t)ceil_div(C, 32 * (16 / size_of(dtype)));
-    // sixteen warps to an SM before a warp has more places than 4
+    // Places of a warp: as many as leave sixteen warps to an SM, each with 128 channels.
+    p.blocks = (uint32_t)ceil_div(C, 128);
     p.places = 32;
     while (p.places > 4 && ceil_div(rows, p.places) * p.blocks < (size_t)rt->sm_count * 16) p.places /= 2;
     p.tiles = ceil_div(rows, p.places);
@@ -424,23 +482,25 @@ GradPlan grad_plan(const ullis_cuda_runtime* rt, int dtype, size_t rows, size_t 
 }
 
 template <typename K, uint32_t BITS>
-void launch_sort(const Stream& s, unsigned grid, const uint32_t* tokens, uint32_t ignore_id, size_t rows, size_t vocab, uint32_t chunks,
+void launch_sort(const Stream& s, unsigned zeros, const uint32_t* tokens, uint32_t ignore_id, size_t rows, size_t vocab, uint32_t chunks,
                  uint32_t* token, uint32_t* row, float* g, size_t elements) {
     const auto kernel = embed_sort_kernel<K, BITS>;
     constexpr size_t SMEM = sizeof(K) << BITS;
     if (SMEM > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
-    s.chain("embed_sort", kernel, grid, SORT_THREADS, SMEM, tokens, ignore_id, (uint32_t)rows, (uint32_t)vocab, chunks, token, row, g, elements);
+    s.chain("embed_sort", kernel, chunks + zeros, (1u << BITS) / SORT_EACH, SMEM, tokens, ignore_id, (uint32_t)rows, (uint32_t)vocab, chunks, token,
+            row, g, elements);
 }
 
 template <typename T>
-void embed_grad_as(const Stream& s, int dtype, const uint32_t* tokens, uint32_t ignore_id, Rows gy, size_t rows, size_t C, size_t vocab, float scale,
-                   float* g, void* workspace) {
-    const GradPlan p = grad_plan(s.rt, dtype, rows, C);
-    constexpr int N = tape::CHUNK<T>;
-    const bool vec = C % N == 0 && gy.stride % N == 0 && aligned(gy.data, 16) && aligned(g, 16);
+void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, Rows gy, size_t rows, size_t C, size_t vocab, float scale, float* g,
+                   void* workspace) {
+    const GradPlan p = grad_plan(s.rt, rows, C);
+    constexpr int N = 16 / (int)sizeof(T);
+    const auto on = [&](size_t n) { return C % n == 0 && gy.stride % n == 0 && aligned(gy.data, n * sizeof(T)) && aligned(g, 16); };
+    const bool wide = on(N);
     if (p.few) {
         const unsigned grid = (unsigned)std::min<size_t>(vocab, (size_t)s.rt->sm_count * 8);
-        s.chain("embed_grad_few", vec ? embed_grad_few_kernel<T, true> : embed_grad_few_kernel<T, false>, grid, THREADS, 0, tokens, ignore_id,
+        s.chain("embed_grad_few", wide ? embed_grad_few_kernel<T, N> : embed_grad_few_kernel<T, 1>, grid, THREADS, 0, tokens, ignore_id,
                 static_cast<const T*>(gy.data), gy.stride, (uint32_t)rows, (uint32_t)C, (uint32_t)vocab, scale, g);
         return;
     }
@@ -449,11 +509,11 @@ void embed_grad_as(const Stream& s, int dtype, const uint32_t* tokens, uint32_t 
     uint32_t *chunk_token = p.chunks > 1 ? reinterpret_cast<uint32_t*>(ws + p.chunk_token) : token;
     uint32_t *chunk_row = p.chunks > 1 ? reinterpret_cast<uint32_t*>(ws + p.chunk_row) : row;
     const size_t elements = vocab * C;
-    const unsigned zeros = (unsigned)std::min<size_t>((size_t)s.rt->sm_count * 2, ceil_div(elements, 4 * SORT_THREADS));
+    const unsigned zeros = (unsigned)std::min<size_t>((size_t)s.rt->sm_count * 8, ceil_div(elements, 4096));
     const bool narrow = (vocab + 1) >> (32 - p.bits) == 0;   // the largest key is that of the padding
     const auto sort = p.bits == 11 ? (narrow ? launch_sort<uint32_t, 11> : launch_sort<uint64_t, 11>)
                                    : (narrow ? launch_sort<uint32_t, 13> : launch_sort<uint64_t, 13>);
-    sort(s, p.chunks + zeros, tokens, ignore_id, rows, vocab, p.chunks, chunk_token, chunk_row, g, elements);
+    sort(s, zeros, tokens, ignore_id, rows, vocab, p.chunks, chunk_token, chunk_row, g, elements);
     if (p.chunks > 1)
         s.chain("embed_rank", embed_rank_kernel, (unsigned)ceil_div(rows, THREADS), THREADS, 0, static_cast<const uint32_t*>(chunk_token),
                 static_cast<const uint32_t*>(chunk_row), (uint32_t)rows, 1u << p.bits, p.chunks, token, row);
@@ -466,13 +526,19 @@ void embed_grad_as(const Stream& s, int dtype, const uint32_t* tokens, uint32_t 
     o.C = (uint32_t)C;
     o.vocab = (uint32_t)vocab;
     o.places = p.places;
-    o.blocks = p.blocks;
     o.scale = scale;
     o.g = g;
     o.head = reinterpret_cast<float*>(ws + p.head);
     o.tail = reinterpret_cast<float*>(ws + p.tail);
-    s.chain("embed_sums", vec ? embed_sums_kernel<T, true> : embed_sums_kernel<T, false>, (unsigned)ceil_div(p.tiles * p.blocks, THREADS / 32), THREADS, 0, o);
-    if (p.tiles > 1) s.chain("embed_join", embed_join_kernel, (unsigned)((p.tiles - 1) * ceil_div(C, 128)), THREADS, 0, o);
+    const auto sums = [&](auto kernel, int each) {
+        o.blocks = (uint32_t)ceil_div(C, 32 * each);
+        s.chain("embed_sums", kernel, (unsigned)ceil_div(p.tiles * o.blocks, THREADS / 32), THREADS, 0, o);
+    };
+    if (wide) sums(embed_sums_kernel<T, N, true>, N);
+    else if (N == 8 && on(4)) sums(embed_sums_kernel<T, N == 8 ? 4 : N, true>, 4);
+    else sums(embed_sums_kernel<T, 4, false>, 4);
+    if (p.tiles > 1)
+        s.chain("embed_join", embed_join_kernel, (unsigned)(ceil_div(p.tiles - 1, THREADS / 32) * ceil_div(C, 128)), THREADS, 0, o, (uint32_t)p.tiles);
 }
 
 }  // namespace
@@ -484,15 +550,15 @@ void embed(const Stream& s, int table_dtype, Rows table, const uint32_t* tokens,
     else embed_from<__nv_bfloat16>(s, dtype, table, tokens, ignore_id, scale, rows, channels, vocab, y);
 }
 
-size_t embed_grad_workspace(const ullis_cuda_runtime* rt, int dtype, size_t rows, size_t channels) {
-    return rows ? grad_plan(rt, dtype, rows, channels).bytes : 0;
+size_t embed_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels) {
+    return rows ? grad_plan(rt, rows, channels).bytes : 0;
 }
 
 void embed_grad(const Stream& s, int dtype, const uint32_t* tokens, uint32_t ignore_id, Rows gy, size_t rows, size_t channels, size_t vocab,
                 float scale, float* g, void* workspace) {
-    if (dtype == F32) embed_grad_as<float>(s, dtype, tokens, ignore_id, gy, rows, channels, vocab, scale, g, workspace);
-    else if (dtype == F16) embed_grad_as<__half>(s, dtype, tokens, ignore_id, gy, rows, channels, vocab, scale, g, workspace);
-    else embed_grad_as<__nv_bfloat16>(s, dtype, tokens, ignore_id, gy, rows, channels, vocab, scale, g, workspace);
+    if (dtype == F32) embed_grad_as<float>(s, tokens, ignore_id, gy, rows, channels, vocab, scale, g, workspace);
+    else if (dtype == F16) embed_grad_as<__half>(s, tokens, ignore_id, gy, rows, channels, vocab, scale, g, workspace);
+    else embed_grad_as<__nv_bfloat16>(s, tokens, ignore_id, gy, rows, channels, vocab, scale, g, workspace);
 }
 
 }  // namespace dev

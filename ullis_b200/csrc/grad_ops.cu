@@ -636,7 +636,7 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
         p.entry_weight = at.add(entries * 4);
         p.entry_logits = at.add(entries * 8);
         p.entry_place = at.add(entries * 2);
-        p.offsets = at.add(p.blocks * (p.groups + 1) * 2);
+        p.offsets = at.add(p.blocks * (2 * p.groups + 1) * 2);
         p.constant = at.add(rows * 4);
         p.second_lse2 = at.add(rows * 4);
         p.row_part2 = at.add(p.lse_pieces * p.row_part_piece * 4);
@@ -662,12 +662,25 @@ size_t head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, si
 
 namespace {
 
+template <typename T, int E>
+void launch_entries_list_of(const Stream& s, const Teacher& t, size_t blocks, const int32_t* target, const int32_t* list, const uint32_t* counted,
+                            const EntryLists& lists) {
+    const auto kernel = entries_list_kernel<T, E>;
+    const size_t smem = (E * LIST_THREADS + 2 * BLOCK_ROWS * t.K) * 4;
+    if (smem > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    s.chain("entries_list", kernel, (unsigned)blocks, LIST_THREADS, smem, t, target, list, counted, lists);
+}
 template <typename T>
 void launch_entries_list(const Stream& s, const Teacher& t, size_t blocks, const int32_t* target, const int32_t* list, const uint32_t* counted,
                          const EntryLists& lists) {
-    const size_t smem = BLOCK_ROWS * t.K1 * 12;
-    if (smem > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(entries_list_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    s.chain("entries_list", entries_list_kernel<T>, (unsigned)blocks, 512, smem, t, target, list, counted, lists);
+    const uint32_t each = BLOCK_ROWS * t.K;   // keys of a block
+    const auto launch = each <= LIST_THREADS       ? launch_entries_list_of<T, 1>
+                        : each <= 2 * LIST_THREADS ? launch_entries_list_of<T, 2>
+                        : each <= 4 * LIST_THREADS ? launch_entries_list_of<T, 4>
+                        : each <= 8 * LIST_THREADS ? launch_entries_list_of<T, 8>
+                                                   : launch_entries_list_of<T, 16>;
+    static_assert(BLOCK_ROWS * DISTILL_MOST <= 16 * LIST_THREADS, "");
+    launch(s, t, blocks, target, list, counted, lists);
 }
 
 // `d`: null, or what the target is spread over.
@@ -700,7 +713,7 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         lists.column = reinterpret_cast<uint32_t*>(ws + p.entry_column);
         lists.weight = reinterpret_cast<float*>(ws + p.entry_weight);
         lists.offsets = reinterpret_cast<uint16_t*>(ws + p.offsets);
-        lists.groups1 = (uint32_t)p.groups + 1;
+        lists.groups1 = 2 * (uint32_t)p.groups + 1;
         lists.place = reinterpret_cast<uint16_t*>(ws + p.entry_place);
         lists.constant = reinterpret_cast<float*>(ws + p.constant);
         int32_t* state = reinterpret_cast<int32_t*>(ws + p.state);

@@ -10,10 +10,13 @@
 // none of whose terms but the last is negative.  Without labels the first parts are left out; where only one of the softmaxes has a
 // share, or T = 1, one is computed, and z and top below are those at its temperature.
 //
+// A label that is an entry already adds its weight there (so every id of a row has one live entry), else it is one more.
+//
 // The rows that count are taken 32 at a time, and their entries sorted by groups of 64 columns and within them by entry_bits: what an
 // epilogue warp has of a tile then lies in a row, and entries of one column beside one another.  Sums go by that order: a call gives the
 // same result every time.
 #pragma once
+#include "block_sort.cuh"
 #include "pair_gemm.cuh"
 #include "tape.cuh"
 
@@ -74,111 +77,157 @@ entries_state_kernel(const HeadLabels labels, const Teacher t, uint32_t rows, ui
 }
 
 struct EntryLists {
-    // by block of 32 rows that count: 32 * K1 places, and groups1 offsets among them
+    // by block of 32 rows that count: 32 * K1 places, and groups1 = 2 groups + 1 offsets among them, for each group that of its first
+    // sixteen rows and of the others
     uint32_t* bits;            // entry_bits (and ENTRY_DEAD)
     uint32_t* column;          // of the vocabulary; later what GRAD takes: bits and above them the 16-bit g * scale * 2^k
     float* weight;             // w, of a dead one 0
     uint16_t* offsets;
     uint32_t groups1;
     // by row that counts
-    uint16_t* place;           // [row][K1], in the block's list
+    uint16_t* place;           // [row][K1], in the block's list, of those that have a weight there
     float* constant;           // alpha * T^2 * sum p * log p; without entries NAN, which marks that
 };
-template <typename T>
-__global__ void __launch_bounds__(512)
+constexpr uint32_t LIST_THREADS = 512;
+constexpr uint32_t NO_KEY = 0xFFFFFFFFu;   // a key: group of columns, entry_bits
+
+// How many of a rising list are below `limit`.
+__device__ __forceinline__ uint32_t keys_below(const uint32_t* list, uint32_t n, uint32_t limit) {
+    uint32_t at = 0;
+    while (n > 0) {
+        const uint32_t half = n >> 1;
+        const bool right = list[at + half] < limit;
+        at += right ? half + 1 : 0u;
+        n = right ? n - half - 1 : half;
+    }
+    return at;
+}
+
+// A CTA has a block of rows.  The teacher's entries are sorted as keys alone (each then finds its place by a search), and the labels that
+// are not among them, a warp's width at most, merged into them.  E: keys to a thread, 32 K <= 512 E.
+template <typename T, int E>
+__global__ void __launch_bounds__(LIST_THREADS)
 entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const int32_t* __restrict__ list, const uint32_t* __restrict__ counted,
                     const EntryLists o) {
     chain_entry();
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+    constexpr uint32_t N = E * LIST_THREADS, WARPS = LIST_THREADS / 32;
+    extern __shared__ __align__(16) uint32_t smem_keys[];
+    __shared__ uint32_t row_label[BLOCK_ROWS], more[BLOCK_ROWS];   // the label's key; those of labels that are no entry, in order
     const uint32_t first = blockIdx.x * BLOCK_ROWS, rows = *counted, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (first >= rows) return;
-    const uint32_t n_rows = min(BLOCK_ROWS, rows - first), n = n_rows * t.K1;
-    uint64_t* keys = reinterpret_cast<uint64_t*>(smem_raw);             // column group, entry_bits, the entry's number
-    float* weight = reinterpret_cast<float*>(keys + BLOCK_ROWS * t.K1);   // by the entry's number
-    const auto key_of = [](uint32_t row, uint32_t column, uint32_t number) {
-        return (uint64_t)((column / GROUP_COLUMNS) * pg::ENTRY_PLACES | pg::entry_bits(row, column)) << 32 | number;
-    };
-    for (uint32_t r = warp; r < n_rows; r += 16) {
+    const uint32_t n_rows = min(BLOCK_ROWS, rows - first), n = n_rows * t.K;
+    const bool labels = t.K1 > t.K;
+    uint32_t* sorted = smem_keys;                                    // [N]
+    uint32_t* keys = sorted + N;                                     // [row][K]
+    float* weight = reinterpret_cast<float*>(keys + BLOCK_ROWS * t.K);   // [row][K]
+    const auto key_of = [](uint32_t row, uint32_t column) { return column / GROUP_COLUMNS * pg::ENTRY_PLACES | pg::entry_bits(row, column); };
+    for (uint32_t r = warp; r < n_rows; r += WARPS) {
         const size_t at = (size_t)list[first + r] * t.K;
         const T* logits = static_cast<const T*>(t.logits) + at;
         float top = -INFINITY;
-        for (uint32_t k = lane; k < t.K; k += 32) top = fmaxf(top, t.ids[at + k] < 0 ? -INFINITY : tape::to_float(logits[k]));
+#pragma unroll 4
+        for (uint32_t k = lane; k < t.K; k += 32) {
+            const float v = tape::to_float(logits[k]);
+            top = fmaxf(top, t.ids[at + k] < 0 ? -INFINITY : v);
+        }
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         const bool has = top != -INFINITY;
         float sum = 0.0f;
-        for (uint32_t k = lane; k < t.K; k += 32)
-            if (has && t.ids[at + k] >= 0) sum += expf((tape::to_float(logits[k]) - top) / t.temperature);
+        for (uint32_t k = lane; k < t.K; k += 32) {
+            const int32_t id = t.ids[at + k];
+            const bool is = has && id >= 0;
+            const float e = is ? expf((tape::to_float(logits[k]) - top) / t.temperature) : 0.0f;
+            sum += e;
+            keys[r * t.K + k] = is ? key_of(r, (uint32_t)id) : NO_KEY;
+            weight[r * t.K + k] = e;
+        }
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const float log_sum = logf(sum);
+        const float log_sum = logf(sum), share = t.alpha * t.temperature;
         float entropy = 0.0f;
         for (uint32_t k = lane; k < t.K; k += 32) {
-            const uint32_t number = r * t.K1 + k;
-            const int32_t id = t.ids[at + k];
-            uint64_t key = ~0ull;
-            if (has && id >= 0) {
-                const float x = (tape::to_float(logits[k]) - top) / t.temperature, p = expf(x) / sum;
-                if (p > 0.0f) entropy += p * (x - log_sum);
-                weight[number] = t.alpha * t.temperature * p;
-                key = key_of(r, (uint32_t)id, number);
-            }
-            keys[number] = key;
+            const float p = has ? weight[r * t.K + k] / sum : 0.0f;
+            if (p > 0.0f) entropy += p * ((tape::to_float(logits[k]) - top) / t.temperature - log_sum);
+            weight[r * t.K + k] = share * p;
         }
         for (int d = 16; d > 0; d >>= 1) entropy += __shfl_xor_sync(0xffffffffu, entropy, d);
         if (lane == 0) {
-            o.constant[first + r] = has ? t.alpha * t.temperature * t.temperature * entropy : NAN;
-            if (t.K1 > t.K) {
-                keys[r * t.K1 + t.K] = key_of(r, (uint32_t)target[first + r], r * t.K1 + t.K);
-                weight[r * t.K1 + t.K] = t.hard;
-            }
-        }
-    }
-    for (uint32_t run = 2; run < 2 * n; run <<= 1) {
-        for (uint32_t half = run >> 1; half > 0; half >>= 1) {
-            __syncthreads();
-            for (uint32_t i = threadIdx.x;; i += 512) {
-                const uint32_t a = (i & ~(half - 1)) * 2 + (i & (half - 1));
-                if (a >= n) break;
-                const uint32_t b = half == run >> 1 ? a ^ (run - 1) : a + half;   // (the first step of a run mirrors: all runs rise)
-                if (b >= n) continue;
-                const uint64_t x = keys[a], y = keys[b];
-                if (x > y) {
-                    keys[a] = y;
-                    keys[b] = x;
-                }
-            }
+            o.constant[first + r] = has ? share * t.temperature * entropy : NAN;
+            row_label[r] = labels ? key_of(r, (uint32_t)target[first + r]) : NO_KEY;
         }
     }
     __syncthreads();
+    uint32_t v[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = threadIdx.x * E + i < n ? keys[threadIdx.x * E + i] : NO_KEY;
+    block_sort<uint32_t, E, LIST_THREADS>(v, sorted);
+#pragma unroll
+    for (int i = 0; i < E; ++i) sorted[threadIdx.x * E + i] = v[i];
+    __syncthreads();
+    const uint32_t valid = keys_below(sorted, N, NO_KEY);
+    if (warp == 0) {
+        uint32_t key = labels && lane < n_rows ? row_label[lane] : NO_KEY;
+        const uint32_t at = keys_below(sorted, valid, key);
+        if (at < valid && sorted[at] == key) key = NO_KEY;
+#pragma unroll
+        for (uint32_t run = 2; run <= 32; run <<= 1)
+#pragma unroll
+            for (uint32_t step = run >> 1; step > 0; step >>= 1) {
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, key, step);
+                key = ((lane & step) == 0) == ((lane & run) == 0) ? min(key, other) : max(key, other);
+            }
+        more[lane] = key;
+    }
+    __syncthreads();
     const size_t base = (size_t)blockIdx.x * BLOCK_ROWS * t.K1;
-    for (uint32_t i = threadIdx.x; i < n; i += 512) {
-        const uint64_t key = keys[i];
-        if (key == ~0ull) continue;
-        const uint32_t at = (uint32_t)(key >> 32), number = (uint32_t)key;
-        const bool dead = i > 0 && (uint32_t)(keys[i - 1] >> 32) == at;
-        float w = 0.0f;
-        if (!dead)
-            for (uint32_t j = i; j < n && (uint32_t)(keys[j] >> 32) == at; ++j) w += weight[(uint32_t)keys[j]];
-        o.bits[base + i] = (at & (pg::ENTRY_PLACES - 1)) | (dead ? pg::ENTRY_DEAD : 0u);
-        o.column[base + i] = at / pg::ENTRY_PLACES * GROUP_COLUMNS + pg::entry_column(at);
-        o.weight[base + i] = w;
-        o.place[(size_t)first * t.K1 + number] = (uint16_t)i;
+    // an entry's place: the teacher's and the labels' before it
+    const auto shift = [&](uint32_t key) { return labels ? keys_below(more, BLOCK_ROWS, key) : 0u; };
+    const auto leave = [&](uint32_t place, uint32_t key, bool dead) {
+        o.bits[base + place] = (key & (pg::ENTRY_PLACES - 1)) | (dead ? pg::ENTRY_DEAD : 0u);
+        o.column[base + place] = key / pg::ENTRY_PLACES * GROUP_COLUMNS + pg::entry_column(key);
+    };
+    for (uint32_t i = threadIdx.x; i < valid; i += LIST_THREADS) {
+        const uint32_t key = sorted[i], place = i + shift(key);
+        const bool dead = i > 0 && sorted[i - 1] == key;
+        leave(place, key, dead);
+        if (dead) o.weight[base + place] = 0.0f;
     }
-    // (the numbers of entries that are none come with none of the keys)
-    for (uint32_t r = warp; r < n_rows; r += 16) {
-        const size_t at = (size_t)list[first + r] * t.K;
-        const bool has = o.constant[first + r] == o.constant[first + r];
-        for (uint32_t k = lane; k < t.K; k += 32)
-            if (!has || t.ids[at + k] < 0) o.place[(size_t)first * t.K1 + r * t.K1 + k] = (uint16_t)NO_PLACE;
-    }
-    for (uint32_t g = threadIdx.x; g < o.groups1; g += 512) {
-        const uint64_t limit = (uint64_t)g * pg::ENTRY_PLACES << 32;
-        uint32_t low = 0, high = n;
-        while (low < high) {
-            const uint32_t middle = (low + high) >> 1;
-            if (keys[middle] < limit) low = middle + 1;
-            else high = middle;
+    for (uint32_t i = threadIdx.x; i < n; i += LIST_THREADS) {
+        const uint32_t key = keys[i], r = i / t.K, k = i - r * t.K;
+        uint16_t* place = o.place + (size_t)(first + r) * t.K1 + k;
+        if (key == NO_KEY) {
+            *place = (uint16_t)NO_PLACE;
+            continue;
         }
-        o.offsets[(size_t)blockIdx.x * o.groups1 + g] = (uint16_t)low;
+        const uint32_t at = keys_below(sorted, valid, key), to = at + shift(key);
+        float w = weight[i];
+        if (at + 1 < valid && sorted[at + 1] == key) {   // it comes again: the first of them has the sum
+            bool mine = true;
+            w = 0.0f;
+            for (uint32_t j = 0; j < t.K; ++j)
+                if (keys[r * t.K + j] == key) {
+                    mine &= j >= k;
+                    w += weight[r * t.K + j];
+                }
+            if (!mine) {
+                *place = (uint16_t)NO_PLACE;
+                continue;
+            }
+        }
+        *place = (uint16_t)to;
+        o.weight[base + to] = row_label[r] == key ? w + t.hard : w;
+    }
+    if (labels && threadIdx.x < n_rows) {
+        const uint32_t key = row_label[threadIdx.x], at = keys_below(sorted, valid, key), to = at + shift(key);
+        const bool entry = at < valid && sorted[at] == key;
+        o.place[(size_t)(first + threadIdx.x) * t.K1 + t.K] = (uint16_t)(entry ? NO_PLACE : to);
+        if (!entry) {
+            leave(to, key, false);
+            o.weight[base + to] = t.hard;
+        }
+    }
+    for (uint32_t g = threadIdx.x; g < o.groups1; g += LIST_THREADS) {
+        const uint32_t limit = g * (pg::ENTRY_PLACES / 2);
+        o.offsets[(size_t)blockIdx.x * o.groups1 + g] = (uint16_t)(keys_below(sorted, valid, limit) + shift(limit));
     }
 }
 
@@ -221,8 +270,8 @@ entries_rows_kernel(const EntryRows o) {
         __syncwarp();
         const uint32_t end = min((stretch + 1) * o.stretch, (rows + BLOCK_ROWS - 1) / BLOCK_ROWS);
         for (uint32_t b = stretch * o.stretch + warp; b < end; b += ROWS_WARPS) {
-            const uint16_t* at = o.lists.offsets + (size_t)b * o.lists.groups1 + group;
-            const uint32_t last = at[1];
+            const uint16_t* at = o.lists.offsets + (size_t)b * o.lists.groups1 + 2 * group;
+            const uint32_t last = at[2];
             for (uint32_t i0 = at[0]; i0 < last; i0 += 32) {
                 const uint32_t i = i0 + lane;
                 const bool in = i < last;

@@ -84,8 +84,8 @@ struct Params {
     const float* target_acc;   // GRAD: [M] the target's product, added with rounding
     const float* target_g;     // GRAD: [M] its probability - 1
     const float* factor;       // GRAD: 2^k ; STORE: alpha
-    // .._ENTRIES: entries of block b of 32 rows and group n of 64 columns of the vocabulary: [b * block_entries + offsets[b * groups1 + n],
-    // .. + offsets[b * groups1 + n + 1])
+    // .._ENTRIES: entries of block b of 32 rows and group n of 64 columns of the vocabulary: those of its first sixteen rows at
+    // b * block_entries + [offsets[b * groups1 + 2 n], offsets[.. + 1]), the others up to offsets[.. + 2]
     const uint16_t* offsets;
     uint32_t groups1, block_entries;
     const uint32_t* entries;   // LSE: entry_bits; GRAD: with the 16-bit g * scale * 2^k above them
@@ -387,18 +387,30 @@ struct Columns {
 };
 // The entries of a warp's 32 rows and 64 columns: where they lie (on its way a tile ahead) and the first of them.
 struct Entries {
-    uint32_t first, count;
+    uint32_t first, middle, end;
     __device__ void find(const Params& p, uint32_t row, uint32_t column, uint32_t M) {
-        first = count = 0;
+        first = middle = end = 0;
         if (row < M) {
-            const uint16_t* at = p.offsets + (size_t)(row / 32) * p.groups1 + column / 64;
+            const uint16_t* at = p.offsets + (size_t)(row / 32) * p.groups1 + column / 64 * 2;
             first = at[0];
-            count = at[1];   // (the end, until they are fetched)
+            middle = at[1];
+            end = at[2];
         }
     }
     __device__ const uint32_t* list(const Params& p, uint32_t row) const { return p.entries + (size_t)(row / 32) * p.block_entries + first; }
 };
 constexpr int ENTRIES_HELD = 2;   // words of 32 entries that are fetched before the accumulator is there
+// The others, in groups of words that are on their way together.
+template <int WORDS, typename F>
+__device__ __forceinline__ void more_entries(const uint32_t* list, uint32_t from, uint32_t to, int lane, F&& use) {
+    for (uint32_t i = from + lane; i - lane < to; i += 32 * WORDS) {
+        uint32_t w[WORDS];
+#pragma unroll
+        for (int u = 0; u < WORDS; ++u) w[u] = i + u * 32 < to ? list[i + u * 32] : NO_ENTRY;
+#pragma unroll
+        for (int u = 0; u < WORDS; ++u) use(i + u * 32, w[u]);
+    }
+}
 // The accumulator has been read: one arrival on the even CTA's barrier.  (With release at the scope of the cluster the arrival
 // waits for the warp's stores to memory, which this barrier says nothing of.)
 __device__ __forceinline__ void arrive_even(uint32_t cluster_addr) {
@@ -634,7 +646,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     const uint32_t row = work.m * BM + rank * 128 + quarter * 32;
                     list = entries.list(p, row);
                     logits = p.entry_logits + (list - p.entries);
-                    n_entries = entries.count - entries.first;
+                    n_entries = entries.end - entries.first;
 #pragma unroll
                     for (int b = 0; b < ENTRIES_HELD; ++b) held[b] = b * 32 + lane < n_entries ? list[b * 32 + lane] : NO_ENTRY;
                 }
@@ -683,8 +695,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             };
 #pragma unroll
                             for (int b = 0; b < ENTRIES_HELD; ++b) take(b * 32 + lane, held[b]);
-#pragma unroll 4
-                            for (uint32_t i = ENTRIES_HELD * 32 + lane; i < n_entries; i += 32) take(i, list[i]);
+                            more_entries<4>(list, ENTRIES_HELD * 32, n_entries, lane, take);
                             __syncwarp();
                         }
                     }
@@ -792,12 +803,13 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             while (more) {
                 const uint32_t n0 = work.n * BN + group * 64, m0 = work.m * BM + rank * 128 + quarter * 32;
                 const uint32_t* list = nullptr;
-                uint32_t n_entries = 0, held[ENTRIES_HELD];
+                uint32_t n_upper = 0, n_entries = 0, held[2];   // held: the first of either half
                 if (ENTRIES) {
                     list = entries.list(p, m0);
-                    n_entries = entries.count - entries.first;
-#pragma unroll
-                    for (int b = 0; b < ENTRIES_HELD; ++b) held[b] = b * 32 + lane < n_entries ? list[b * 32 + lane] : NO_ENTRY;
+                    n_upper = entries.middle - entries.first;
+                    n_entries = entries.end - entries.first;
+                    held[0] = lane < n_upper ? list[lane] : NO_ENTRY;
+                    held[1] = n_upper + lane < n_entries ? list[n_upper + lane] : NO_ENTRY;
                 }
                 if (work.n != n_now) {
                     leave();
@@ -884,16 +896,14 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     }
                     if constexpr (ENTRIES) {
                         __syncwarp();
-                        const auto put = [&](uint32_t bits) {
-                            if ((bits & ENTRY_DEAD) || (bits >> 10 & 1u) != (uint32_t)h) return;
+                        const auto put = [&](uint32_t, uint32_t bits) {
+                            if (bits & ENTRY_DEAD) return;
                             const uint32_t row = bits & 15u, column = entry_column(bits);
                             *reinterpret_cast<uint16_t*>(staging + h * STAGING_BYTES + row * 128 + ((column / 8 ^ (row & 7)) << 4) + column % 8 * 2) =
                                 (uint16_t)(bits >> 16);
                         };
-#pragma unroll
-                        for (int b = 0; b < ENTRIES_HELD; ++b) put(held[b]);
-#pragma unroll 4
-                        for (uint32_t i = ENTRIES_HELD * 32 + lane; i < n_entries; i += 32) put(list[i]);
+                        put(0, h ? held[1] : held[0]);
+                        more_entries<8>(list, (h ? n_upper : 0u) + 32, h ? n_entries : n_upper, lane, put);
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
