@@ -379,3 +379,12 @@ def test_a_step_from_teacher_to_table(cuda_rt):
     sizes = inv * (dx + dx.mean(1, keepdim=True) + xh * (dx * xh).mean(1, keepdim=True))
     off = torch.zeros_like(t64).index_add_(0, at, sizes) * scale * (4 * 64 + 32 + 520) * U
     assert ((got.double() - t64).abs() <= off).all()
+
+
+@pytest.mark.parametrize("vocab", [(1 << 19) - 256, (1 << 19) + 70])
+def test_large_vocabularies(cuda_rt, vocab):
+    """Sort keys of the entries in 32 bits up to 524 032 columns, in 64 beyond them."""
+    s = student(70, 70, 8, vocab, "bf16", False, 30, seed=2)
+    s["top_ids"][:, 4] = vocab - 1 - torch.arange(70, device="cuda").to(torch.int32) % 3
+    s["top_ids"][::2, 9] = s["top_ids"][::2, 4]
+    check(call(cuda_rt, s), formulas(s))

@@ -7,11 +7,6 @@
 namespace ullis {
 namespace dev {
 
-template <typename K>
-__device__ __forceinline__ K sort_smaller(K a, K b) { return a < b ? a : b; }
-template <typename K>
-__device__ __forceinline__ K sort_larger(K a, K b) { return a < b ? b : a; }
-
 // Thread t has keys t * E .. of them; `shared` has room for E * THREADS keys and is free before and after.
 template <typename K, int E, int THREADS>
 __device__ __forceinline__ void block_sort(K (&v)[E], K* shared) {
@@ -25,9 +20,10 @@ __device__ __forceinline__ void block_sort(K (&v)[E], K* shared) {
             for (int i = 0; i < E; ++i) {
                 if (i & step) continue;
                 const bool rising = ((first + i) & run) == 0;
-                const K a = v[i], b = v[i | step], low = sort_smaller(a, b), high = sort_larger(a, b);
-                v[i] = rising ? low : high;
-                v[i | step] = rising ? high : low;
+                const K a = v[i], b = v[i | step];
+                const bool keep = (a < b) == rising;
+                v[i] = keep ? a : b;
+                v[i | step] = keep ? b : a;
             }
         }
     };
@@ -44,7 +40,7 @@ __device__ __forceinline__ void block_sort(K (&v)[E], K* shared) {
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
                     const K other = __shfl_xor_sync(0xffffffffu, v[i], apart);
-                    v[i] = smaller ? sort_smaller(v[i], other) : sort_larger(v[i], other);
+                    v[i] = (v[i] < other) == smaller ? v[i] : other;
                 }
             } else {
 #pragma unroll
@@ -53,7 +49,7 @@ __device__ __forceinline__ void block_sort(K (&v)[E], K* shared) {
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
                     const K other = shared[i * THREADS + (t ^ apart)];
-                    v[i] = smaller ? sort_smaller(v[i], other) : sort_larger(v[i], other);
+                    v[i] = (v[i] < other) == smaller ? v[i] : other;
                 }
                 __syncthreads();
             }

@@ -5,6 +5,7 @@
 // Both are bound by memory: the lookup reads a table row and writes a row, the gradient reads gy once and writes the table once.
 // The gradient's sums have a fixed order, with no atomics: the rows of a token in rising order, in pieces where there are many.
 #include <algorithm>
+#include <type_traits>
 
 #include "block_sort.cuh"
 #include "device_ops.hpp"
@@ -23,17 +24,24 @@ bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p
 // A lane's N channels of a row: side by side from c on, read and written at once where they lie on their own size (WIDE), else
 // GAP apart, so that neighbouring threads have neighbouring channels; past the row's end zeros.
 template <bool WIDE, int N, int GAP, typename T>
-__device__ __forceinline__ void load_channels(const T* row, uint32_t c, uint32_t C, float (&v)[N]) {
-    if constexpr (WIDE) {
-        __align__(16) T t[N];
-        if constexpr (sizeof(T) * N == 16) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(row + c);
-        else *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(row + c);
+struct Channels {
+    __align__(WIDE ? sizeof(T) * N : sizeof(T)) T t[N];
+    __device__ __forceinline__ void load(const T* row, uint32_t c, uint32_t C) {
+        if constexpr (WIDE) {
+            using Word = std::conditional_t<sizeof(T) * N == 16, uint4, uint2>;
+            *reinterpret_cast<Word*>(t) = c < C ? *reinterpret_cast<const Word*>(row + c) : Word{};
+        } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = tape::to_float(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = c + i * GAP < C ? tape::to_float(row[c + i * GAP]) : 0.0f;
+            for (int i = 0; i < N; ++i) t[i] = c + i * GAP < C ? row[c + i * GAP] : tape::from_float<T>(0.0f);
+        }
     }
+};
+template <bool WIDE, int N, int GAP, typename T>
+__device__ __forceinline__ void load_channels(const T* row, uint32_t c, uint32_t C, float (&v)[N]) {
+    Channels<WIDE, N, GAP, T> r;
+    r.load(row, c, C);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = tape::to_float(r.t[i]);
 }
 template <bool WIDE, int N, int GAP, typename T>
 __device__ __forceinline__ void store_channels(T* row, uint32_t c, uint32_t C, const float (&v)[N]) {
@@ -229,12 +237,14 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
 // place in its chunk and what searches in the others give, and warps sum runs of rows in that order, a fixed number of
 // places each whatever the tokens are: a run that ends in another warp's places leaves a part of its sum, and a last launch adds those.
 constexpr uint32_t SORT_EACH = 8;   // keys to a thread
+constexpr uint32_t WINDOW = 8;      // of sorted tokens, the last of which are kept apart
 
 // Keys token << BITS | place, padded with the largest.
 template <typename K, uint32_t BITS>
 __global__ void __launch_bounds__((1u << BITS) / SORT_EACH)
 embed_sort_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, uint32_t rows, uint32_t vocab, uint32_t chunks,
-                  uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row, float* __restrict__ g, size_t elements) {
+                  uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row, uint32_t* __restrict__ samples,
+                  float* __restrict__ g, size_t elements) {
     chain_entry();
     constexpr uint32_t SIZE = 1u << BITS, SORT_THREADS = SIZE / SORT_EACH;
     if (blockIdx.x >= chunks) {
@@ -263,59 +273,62 @@ embed_sort_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, uint3
     block_sort<K, SORT_EACH, SORT_THREADS>(keys, reinterpret_cast<K*>(smem_raw));
 #pragma unroll
     for (uint32_t i = 0; i < SORT_EACH; ++i) {
-        if (base + first + i >= rows) break;
+        if (i % WINDOW == WINDOW - 1) samples[(base + first + i) / WINDOW] = (uint32_t)(keys[i] >> BITS);
         sorted_token[base + first + i] = (uint32_t)(keys[i] >> BITS);
         sorted_row[base + first + i] = base + (uint32_t)(keys[i] & (SIZE - 1));
     }
 }
 
-// A warp has 32 elements of a chunk, whose tokens lie close together.  Its lanes search the places of the first and the last of them
-// in 32 other chunks at once; what lies between two such places, mostly less than a warp's width, is fetched and searched by shuffles.
+// An element's place: how many elements of every other chunk come before it.  The last token of every eight of a chunk lies in shared
+// memory, where the eight are found; they are a sector of memory, read at once.  Four chunks are searched side by side, so that
+// their reads wait for memory together.  (Steps of a search in memory are a sector each: 33 us for 38 chunks of 2048, so 8.)
+constexpr uint32_t SAMPLES_HELD = 16384;
 __global__ void __launch_bounds__(THREADS)
-embed_rank_kernel(const uint32_t* __restrict__ chunk_token, const uint32_t* __restrict__ chunk_row, uint32_t rows, uint32_t size, uint32_t chunks,
-                  uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row) {
+embed_rank_kernel(const uint32_t* __restrict__ chunk_token, const uint32_t* __restrict__ chunk_row, const uint32_t* __restrict__ samples,
+                  uint32_t rows, uint32_t size, uint32_t chunks, uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row) {
     chain_entry();
-    constexpr uint32_t ALL = 0xffffffffu;
-    const uint32_t first = (blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5)) * 32, lane = threadIdx.x & 31;
-    if (first >= rows) return;
-    const uint32_t i = min(first + lane, rows - 1), own = first / size, token = chunk_token[i];   // (a warp's are of one chunk)
-    const uint32_t row = chunk_row[i], from = __shfl_sync(ALL, token, 0), to = __shfl_sync(ALL, token, 31);
+    constexpr uint32_t TOGETHER = 4;
+    extern __shared__ __align__(16) uint32_t held[];
+    const uint32_t i = blockIdx.x * THREADS + threadIdx.x, per_chunk = size / WINDOW, chunks_held = SAMPLES_HELD / per_chunk;
+    const uint32_t own = i / size, token = chunk_token[i], row = chunk_row[i];   // (whole chunks are there)
     uint32_t rank = i - own * size;
-    for (uint32_t c0 = 0; c0 < chunks; c0 += 32) {
-        uint32_t low = 0, high = 0;
-        const uint32_t c = c0 + lane;
-        if (c < chunks && c != own) {
-            const uint32_t n = min(size, rows - c * size);
-            low = below(chunk_token + c * size, n, from, c < own);
-            high = below(chunk_token + c * size, n, to, c < own);
-        }
-        const uint32_t end = min(32u, chunks - c0);
-        const auto fetch = [&](uint32_t k) {
-            const uint32_t begin = __shfl_sync(ALL, low, k), stop = __shfl_sync(ALL, high, k);
-            return begin + lane < stop ? chunk_token[(c0 + k) * size + begin + lane] : 0xFFFFFFFFu;
-        };
-        uint32_t next = fetch(0);
-        for (uint32_t k = 0; k < end; ++k) {
-            const uint32_t begin = __shfl_sync(ALL, low, k), stop = __shfl_sync(ALL, high, k), here = next;
-            if (k + 1 < end) next = fetch(k + 1);
-            rank += begin;
-            if (begin == stop) continue;
-            const uint32_t limit = token + (c0 + k < own);
-            if (stop - begin <= 32) {
-                uint32_t at = 0;
+    for (uint32_t c0 = 0; c0 < chunks; c0 += chunks_held) {
+        const uint32_t n = min(chunks_held, chunks - c0);
+        if (c0) __syncthreads();
+        for (uint32_t k = threadIdx.x * 4; k < n * per_chunk; k += THREADS * 4)
+            *reinterpret_cast<uint4*>(held + k) = *reinterpret_cast<const uint4*>(samples + (size_t)c0 * per_chunk + k);
+        __syncthreads();
+        for (uint32_t k0 = 0; k0 < n; k0 += TOGETHER) {
+            uint32_t at[TOGETHER], limit[TOGETHER];
+            uint4 eight[TOGETHER][2];
 #pragma unroll
-                for (uint32_t step = 16; step > 0; step >>= 1) {
-                    const uint32_t value = __shfl_sync(ALL, here, at + step - 1);
-                    at += value < limit ? step : 0u;
-                }
-                at += __shfl_sync(ALL, here, at) < limit;   // (31 of 32 have been told apart)
-                rank += at;
-            } else {
-                rank += below(chunk_token + (c0 + k) * size + begin, stop - begin, token, c0 + k < own);
+            for (uint32_t u = 0; u < TOGETHER; ++u) {
+                const uint32_t c = c0 + k0 + u;
+                // (tokens that are the same come first in earlier chunks; of the own one and of those behind the last nothing counts)
+                limit[u] = c == own || k0 + u >= n ? 0u : token + (c < own);
+                at[u] = min(k0 + u, n - 1) * per_chunk;
+            }
+            for (uint32_t step = per_chunk / 2; step > 0; step >>= 1)
+#pragma unroll
+                for (uint32_t u = 0; u < TOGETHER; ++u)
+                    if (held[at[u] + step - 1] < limit[u]) at[u] += step;
+#pragma unroll
+            for (uint32_t u = 0; u < TOGETHER; ++u) {   // (a chunk's last eight, where all eights end below the limit)
+                const uint4* from = reinterpret_cast<const uint4*>(chunk_token + ((size_t)c0 * per_chunk + at[u]) * WINDOW);
+                eight[u][0] = from[0];
+                eight[u][1] = from[1];
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < TOGETHER; ++u) {
+                if (limit[u] == 0) continue;
+                rank += (at[u] - (k0 + u) * per_chunk) * WINDOW;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    rank += (eight[u][h].x < limit[u]) + (eight[u][h].y < limit[u]) + (eight[u][h].z < limit[u]) + (eight[u][h].w < limit[u]);
             }
         }
     }
-    if (first + lane < rows) {
+    if (i < rows) {
         sorted_token[rank] = token;
         sorted_row[rank] = row;
     }
@@ -347,17 +360,14 @@ embed_sums_kernel(const GradSums o) {
     const T* gy = static_cast<const T*>(o.gy);
     float sum[N] = {};
     bool began_here = __shfl_sync(0xffffffffu, my_token, 0) != before;
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = 8;   // rows on their way (16 of 8 bytes: 121 registers, and 82 us instead of 42 for 76550 x 500 bf16)
     for (uint32_t k0 = 0; k0 < n; k0 += AHEAD) {
-        float v[AHEAD][N];
+        Channels<WIDE, N, 32, T> v[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const uint32_t k = min(k0 + u, n - 1);
             const uint32_t token = __shfl_sync(0xffffffffu, my_token, k), row = __shfl_sync(0xffffffffu, my_row, k);
-            if (in && token < o.vocab && k0 + u < n) load_channels<WIDE, N, 32>(gy + row * o.stride, c, o.C, v[u]);
-            else
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[u][e] = 0.0f;
+            v[u].load(gy + row * o.stride, c, in && token < o.vocab && k0 + u < n ? o.C : 0u);
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
@@ -366,7 +376,7 @@ embed_sums_kernel(const GradSums o) {
             const uint32_t token = __shfl_sync(0xffffffffu, my_token, k), next_lane = __shfl_sync(0xffffffffu, my_token, min(k + 1, n - 1));
             const uint32_t next = k + 1 < n ? next_lane : after;
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] += v[u][e];
+            for (int e = 0; e < N; ++e) sum[e] += tape::to_float(v[u].t[e]);
             if (token == next && k + 1 < n) continue;
             if (in && token < o.vocab) {
                 const bool whole = began_here && token != next;
@@ -386,7 +396,7 @@ embed_sums_kernel(const GradSums o) {
 // The sums that several warps have parts of: the tail of the warp they began in and the heads of those after it, in their order.  A CTA
 // has 128 channels of what began in the places of eight warps: sums of few parts a warp each, then those of many one after the other, by
 // eight warps a stretch of the parts each.
-constexpr uint32_t FEW_PARTS = 16;
+constexpr uint32_t FEW_PARTS = 4;
 __global__ void __launch_bounds__(THREADS)
 embed_join_kernel(const GradSums o, uint32_t tiles) {
     chain_entry();
@@ -451,7 +461,7 @@ embed_join_kernel(const GradSums o, uint32_t tiles) {
 struct GradPlan {
     bool few;
     uint32_t bits, chunks, places, blocks;
-    size_t tiles, chunk_token, chunk_row, token, row, head, tail, bytes;
+    size_t tiles, samples, chunk_token, chunk_row, token, row, head, tail, bytes;
 };
 GradPlan grad_plan(const ullis_cuda_runtime* rt, size_t rows, size_t C) {
     GradPlan p{};
@@ -471,10 +481,12 @@ GradPlan grad_plan(const ullis_cuda_runtime* rt, size_t rows, size_t C) {
         at += up(n, 256);
         return here;
     };
-    p.chunk_token = add(p.chunks > 1 ? rows * 4 : 0);
-    p.chunk_row = add(p.chunks > 1 ? rows * 4 : 0);
-    p.token = add(rows * 4);
-    p.row = add(rows * 4);
+    const size_t whole = (size_t)p.chunks << p.bits;   // the padding of the last chunk with it
+    p.samples = add(whole / WINDOW * 4);
+    p.chunk_token = add(p.chunks > 1 ? whole * 4 : 0);
+    p.chunk_row = add(p.chunks > 1 ? whole * 4 : 0);
+    p.token = add(whole * 4);
+    p.row = add(whole * 4);
     p.head = add(p.tiles * C * 4);
     p.tail = add(p.tiles * C * 4);
     p.bytes = at;
@@ -483,12 +495,12 @@ GradPlan grad_plan(const ullis_cuda_runtime* rt, size_t rows, size_t C) {
 
 template <typename K, uint32_t BITS>
 void launch_sort(const Stream& s, unsigned zeros, const uint32_t* tokens, uint32_t ignore_id, size_t rows, size_t vocab, uint32_t chunks,
-                 uint32_t* token, uint32_t* row, float* g, size_t elements) {
+                 uint32_t* token, uint32_t* row, uint32_t* samples, float* g, size_t elements) {
     const auto kernel = embed_sort_kernel<K, BITS>;
     constexpr size_t SMEM = sizeof(K) << BITS;
     if (SMEM > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
     s.chain("embed_sort", kernel, chunks + zeros, (1u << BITS) / SORT_EACH, SMEM, tokens, ignore_id, (uint32_t)rows, (uint32_t)vocab, chunks, token,
-            row, g, elements);
+            row, samples, g, elements);
 }
 
 template <typename T>
@@ -508,15 +520,19 @@ void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, 
     uint32_t *token = reinterpret_cast<uint32_t*>(ws + p.token), *row = reinterpret_cast<uint32_t*>(ws + p.row);
     uint32_t *chunk_token = p.chunks > 1 ? reinterpret_cast<uint32_t*>(ws + p.chunk_token) : token;
     uint32_t *chunk_row = p.chunks > 1 ? reinterpret_cast<uint32_t*>(ws + p.chunk_row) : row;
+    uint32_t* samples = reinterpret_cast<uint32_t*>(ws + p.samples);
     const size_t elements = vocab * C;
     const unsigned zeros = (unsigned)std::min<size_t>((size_t)s.rt->sm_count * 8, ceil_div(elements, 4096));
     const bool narrow = (vocab + 1) >> (32 - p.bits) == 0;   // the largest key is that of the padding
     const auto sort = p.bits == 11 ? (narrow ? launch_sort<uint32_t, 11> : launch_sort<uint64_t, 11>)
                                    : (narrow ? launch_sort<uint32_t, 13> : launch_sort<uint64_t, 13>);
-    sort(s, zeros, tokens, ignore_id, rows, vocab, p.chunks, chunk_token, chunk_row, g, elements);
-    if (p.chunks > 1)
-        s.chain("embed_rank", embed_rank_kernel, (unsigned)ceil_div(rows, THREADS), THREADS, 0, static_cast<const uint32_t*>(chunk_token),
-                static_cast<const uint32_t*>(chunk_row), (uint32_t)rows, 1u << p.bits, p.chunks, token, row);
+    sort(s, zeros, tokens, ignore_id, rows, vocab, p.chunks, chunk_token, chunk_row, samples, g, elements);
+    if (p.chunks > 1) {
+        const size_t held = std::min<size_t>(SAMPLES_HELD, ((size_t)p.chunks << p.bits) / WINDOW) * 4;
+        if (held > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(embed_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)held));
+        s.chain("embed_rank", embed_rank_kernel, (unsigned)ceil_div(rows, THREADS), THREADS, held, static_cast<const uint32_t*>(chunk_token),
+                static_cast<const uint32_t*>(chunk_row), static_cast<const uint32_t*>(samples), (uint32_t)rows, 1u << p.bits, p.chunks, token, row);
+    }
     GradSums o{};
     o.token = token;
     o.row = row;

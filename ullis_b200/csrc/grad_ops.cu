@@ -662,11 +662,11 @@ size_t head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, si
 
 namespace {
 
-template <typename T, int E>
+template <typename T, typename Key, int E>
 void launch_entries_list_of(const Stream& s, const Teacher& t, size_t blocks, const int32_t* target, const int32_t* list, const uint32_t* counted,
                             const EntryLists& lists) {
-    const auto kernel = entries_list_kernel<T, E>;
-    const size_t smem = (E * LIST_THREADS + 2 * BLOCK_ROWS * t.K) * 4;
+    const auto kernel = entries_list_kernel<T, Key, E>;
+    const size_t smem = E * LIST_THREADS * sizeof(Key) + BLOCK_ROWS * t.K * 4;
     if (smem > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     s.chain("entries_list", kernel, (unsigned)blocks, LIST_THREADS, smem, t, target, list, counted, lists);
 }
@@ -674,12 +674,14 @@ template <typename T>
 void launch_entries_list(const Stream& s, const Teacher& t, size_t blocks, const int32_t* target, const int32_t* list, const uint32_t* counted,
                          const EntryLists& lists) {
     const uint32_t each = BLOCK_ROWS * t.K;   // keys of a block
-    const auto launch = each <= LIST_THREADS       ? launch_entries_list_of<T, 1>
-                        : each <= 2 * LIST_THREADS ? launch_entries_list_of<T, 2>
-                        : each <= 4 * LIST_THREADS ? launch_entries_list_of<T, 4>
-                        : each <= 8 * LIST_THREADS ? launch_entries_list_of<T, 8>
-                                                   : launch_entries_list_of<T, 16>;
-    static_assert(BLOCK_ROWS * DISTILL_MOST <= 16 * LIST_THREADS, "");
+    // keys: 8 bits for an entry's number, 11 for its place in a group, the others for the group
+    const auto launch = lists.groups1 / 2 >= 1u << 13  ? launch_entries_list_of<T, uint64_t, 16>
+                        : each <= LIST_THREADS       ? launch_entries_list_of<T, uint32_t, 1>
+                        : each <= 2 * LIST_THREADS ? launch_entries_list_of<T, uint32_t, 2>
+                        : each <= 4 * LIST_THREADS ? launch_entries_list_of<T, uint32_t, 4>
+                        : each <= 8 * LIST_THREADS ? launch_entries_list_of<T, uint32_t, 8>
+                                                   : launch_entries_list_of<T, uint32_t, 16>;
+    static_assert(BLOCK_ROWS * DISTILL_MOST <= 16 * LIST_THREADS && DISTILL_MOST <= 256, "");
     launch(s, t, blocks, target, list, counted, lists);
 }
 

@@ -89,10 +89,10 @@ struct EntryLists {
     float* constant;           // alpha * T^2 * sum p * log p; without entries NAN, which marks that
 };
 constexpr uint32_t LIST_THREADS = 512;
-constexpr uint32_t NO_KEY = 0xFFFFFFFFu;   // a key: group of columns, entry_bits
 
 // How many of a rising list are below `limit`.
-__device__ __forceinline__ uint32_t keys_below(const uint32_t* list, uint32_t n, uint32_t limit) {
+template <typename Key>
+__device__ __forceinline__ uint32_t keys_below(const Key* list, uint32_t n, Key limit) {
     uint32_t at = 0;
     while (n > 0) {
         const uint32_t half = n >> 1;
@@ -103,131 +103,118 @@ __device__ __forceinline__ uint32_t keys_below(const uint32_t* list, uint32_t n,
     return at;
 }
 
-// A CTA has a block of rows.  The teacher's entries are sorted as keys alone (each then finds its place by a search), and the labels that
-// are not among them, a warp's width at most, merged into them.  E: keys to a thread, 32 K <= 512 E.
-template <typename T, int E>
+// A CTA has a block of rows.  The teacher's entries are sorted by spot (group of columns and entry_bits) and the entry's number in its row
+// below it, in 32 bits up to 524 032 columns; the labels that are no entries, at most a warp's width, are merged into them.  E: keys to
+// a thread, 32 K <= 512 E.
+template <typename T, typename Key, int E>
 __global__ void __launch_bounds__(LIST_THREADS)
 entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const int32_t* __restrict__ list, const uint32_t* __restrict__ counted,
                     const EntryLists o) {
     chain_entry();
-    constexpr uint32_t N = E * LIST_THREADS, WARPS = LIST_THREADS / 32;
-    extern __shared__ __align__(16) uint32_t smem_keys[];
-    __shared__ uint32_t row_label[BLOCK_ROWS], more[BLOCK_ROWS];   // the label's key; those of labels that are no entry, in order
+    constexpr uint32_t N = E * LIST_THREADS, WARPS = LIST_THREADS / 32, NUMBER_BITS = 8, NO_SPOT = 0xFFFFFFFFu;
+    constexpr Key NO_KEY = ~(Key)0;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    __shared__ uint32_t row_label[BLOCK_ROWS], more[BLOCK_ROWS];   // the label's spot; those of labels that are no entries, rising
     const uint32_t first = blockIdx.x * BLOCK_ROWS, rows = *counted, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (first >= rows) return;
     const uint32_t n_rows = min(BLOCK_ROWS, rows - first), n = n_rows * t.K;
     const bool labels = t.K1 > t.K;
-    uint32_t* sorted = smem_keys;                                    // [N]
-    uint32_t* keys = sorted + N;                                     // [row][K]
-    float* weight = reinterpret_cast<float*>(keys + BLOCK_ROWS * t.K);   // [row][K]
-    const auto key_of = [](uint32_t row, uint32_t column) { return column / GROUP_COLUMNS * pg::ENTRY_PLACES | pg::entry_bits(row, column); };
+    Key* sorted = reinterpret_cast<Key*>(smem_raw);                  // [N]
+    float* weight = reinterpret_cast<float*>(sorted + N);            // [row][K]
+    const auto spot_of = [](uint32_t row, uint32_t column) { return column / GROUP_COLUMNS * pg::ENTRY_PLACES | pg::entry_bits(row, column); };
+    const float times = 1.0f / t.temperature, share = t.alpha * t.temperature;
     for (uint32_t r = warp; r < n_rows; r += WARPS) {
         const size_t at = (size_t)list[first + r] * t.K;
         const T* logits = static_cast<const T*>(t.logits) + at;
+        uint16_t* place = o.place + (size_t)(first + r) * t.K1;
         float top = -INFINITY;
-#pragma unroll 4
+#pragma unroll 2
         for (uint32_t k = lane; k < t.K; k += 32) {
             const float v = tape::to_float(logits[k]);
             top = fmaxf(top, t.ids[at + k] < 0 ? -INFINITY : v);
         }
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         const bool has = top != -INFINITY;
-        float sum = 0.0f;
+        float sum = 0.0f, sum_x = 0.0f;
+#pragma unroll 2
         for (uint32_t k = lane; k < t.K; k += 32) {
             const int32_t id = t.ids[at + k];
             const bool is = has && id >= 0;
-            const float e = is ? expf((tape::to_float(logits[k]) - top) / t.temperature) : 0.0f;
+            const float x = (tape::to_float(logits[k]) - top) * times, e = is ? expf(x) : 0.0f;
             sum += e;
-            keys[r * t.K + k] = is ? key_of(r, (uint32_t)id) : NO_KEY;
+            if (e > 0.0f) sum_x += e * x;
+            sorted[r * t.K + k] = is ? (Key)spot_of(r, (uint32_t)id) << NUMBER_BITS | k : NO_KEY;
+            if (!is) place[k] = (uint16_t)NO_PLACE;
             weight[r * t.K + k] = e;
         }
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const float log_sum = logf(sum), share = t.alpha * t.temperature;
-        float entropy = 0.0f;
-        for (uint32_t k = lane; k < t.K; k += 32) {
-            const float p = has ? weight[r * t.K + k] / sum : 0.0f;
-            if (p > 0.0f) entropy += p * ((tape::to_float(logits[k]) - top) / t.temperature - log_sum);
-            weight[r * t.K + k] = share * p;
+        for (int d = 16; d > 0; d >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            sum_x += __shfl_xor_sync(0xffffffffu, sum_x, d);
         }
-        for (int d = 16; d > 0; d >>= 1) entropy += __shfl_xor_sync(0xffffffffu, entropy, d);
+        const float each = share / sum;
+        if (has)
+            for (uint32_t k = lane; k < t.K; k += 32) weight[r * t.K + k] *= each;
         if (lane == 0) {
-            o.constant[first + r] = has ? share * t.temperature * entropy : NAN;
-            row_label[r] = labels ? key_of(r, (uint32_t)target[first + r]) : NO_KEY;
+            // sum of p * log p, with log p = x - log sum
+            o.constant[first + r] = has ? share * t.temperature * (sum_x / sum - logf(sum)) : NAN;
+            row_label[r] = labels ? spot_of(r, (uint32_t)target[first + r]) : NO_SPOT;
         }
     }
     __syncthreads();
-    uint32_t v[E];
+    Key v[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = threadIdx.x * E + i < n ? keys[threadIdx.x * E + i] : NO_KEY;
-    block_sort<uint32_t, E, LIST_THREADS>(v, sorted);
+    for (int i = 0; i < E; ++i) v[i] = threadIdx.x * E + i < n ? sorted[threadIdx.x * E + i] : NO_KEY;
+    __syncthreads();
+    block_sort<Key, E, LIST_THREADS>(v, sorted);
 #pragma unroll
     for (int i = 0; i < E; ++i) sorted[threadIdx.x * E + i] = v[i];
     __syncthreads();
     const uint32_t valid = keys_below(sorted, N, NO_KEY);
+    const auto find = [&](uint32_t spot) { return keys_below(sorted, valid, (Key)spot << NUMBER_BITS); };
+    const auto is_at = [&](uint32_t i, uint32_t spot) { return i < valid && (uint32_t)(sorted[i] >> NUMBER_BITS) == spot; };
     if (warp == 0) {
-        uint32_t key = labels && lane < n_rows ? row_label[lane] : NO_KEY;
-        const uint32_t at = keys_below(sorted, valid, key);
-        if (at < valid && sorted[at] == key) key = NO_KEY;
+        uint32_t spot = labels && lane < n_rows ? row_label[lane] : NO_SPOT;
+        if (spot != NO_SPOT && is_at(find(spot), spot)) spot = NO_SPOT;
 #pragma unroll
         for (uint32_t run = 2; run <= 32; run <<= 1)
 #pragma unroll
             for (uint32_t step = run >> 1; step > 0; step >>= 1) {
-                const uint32_t other = __shfl_xor_sync(0xffffffffu, key, step);
-                key = ((lane & step) == 0) == ((lane & run) == 0) ? min(key, other) : max(key, other);
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, spot, step);
+                spot = ((lane & step) == 0) == ((lane & run) == 0) ? min(spot, other) : max(spot, other);
             }
-        more[lane] = key;
+        more[lane] = spot;
     }
     __syncthreads();
     const size_t base = (size_t)blockIdx.x * BLOCK_ROWS * t.K1;
-    // an entry's place: the teacher's and the labels' before it
-    const auto shift = [&](uint32_t key) { return labels ? keys_below(more, BLOCK_ROWS, key) : 0u; };
-    const auto leave = [&](uint32_t place, uint32_t key, bool dead) {
-        o.bits[base + place] = (key & (pg::ENTRY_PLACES - 1)) | (dead ? pg::ENTRY_DEAD : 0u);
-        o.column[base + place] = key / pg::ENTRY_PLACES * GROUP_COLUMNS + pg::entry_column(key);
+    const auto labels_below = [&](uint32_t spot) { return labels ? keys_below(more, BLOCK_ROWS, spot) : 0u; };
+    const auto leave = [&](uint32_t place, uint32_t spot, uint32_t dead, float w) {
+        o.bits[base + place] = (spot & (pg::ENTRY_PLACES - 1)) | dead;
+        o.column[base + place] = spot / pg::ENTRY_PLACES * GROUP_COLUMNS + pg::entry_column(spot);
+        o.weight[base + place] = w;
     };
     for (uint32_t i = threadIdx.x; i < valid; i += LIST_THREADS) {
-        const uint32_t key = sorted[i], place = i + shift(key);
-        const bool dead = i > 0 && sorted[i - 1] == key;
-        leave(place, key, dead);
-        if (dead) o.weight[base + place] = 0.0f;
-    }
-    for (uint32_t i = threadIdx.x; i < n; i += LIST_THREADS) {
-        const uint32_t key = keys[i], r = i / t.K, k = i - r * t.K;
-        uint16_t* place = o.place + (size_t)(first + r) * t.K1 + k;
-        if (key == NO_KEY) {
-            *place = (uint16_t)NO_PLACE;
-            continue;
+        const Key key = sorted[i];
+        const uint32_t spot = (uint32_t)(key >> NUMBER_BITS), r = pg::entry_row(spot), k = (uint32_t)key & ((1u << NUMBER_BITS) - 1);
+        const uint32_t place = i + labels_below(spot);
+        const bool dead = i > 0 && is_at(i - 1, spot);   // the first of its spot has the sum
+        float w = 0.0f;
+        if (!dead) {
+            w = weight[r * t.K + k];
+            for (uint32_t j = i + 1; is_at(j, spot); ++j) w += weight[r * t.K + ((uint32_t)sorted[j] & ((1u << NUMBER_BITS) - 1))];
+            if (row_label[r] == spot) w += t.hard;
         }
-        const uint32_t at = keys_below(sorted, valid, key), to = at + shift(key);
-        float w = weight[i];
-        if (at + 1 < valid && sorted[at + 1] == key) {   // it comes again: the first of them has the sum
-            bool mine = true;
-            w = 0.0f;
-            for (uint32_t j = 0; j < t.K; ++j)
-                if (keys[r * t.K + j] == key) {
-                    mine &= j >= k;
-                    w += weight[r * t.K + j];
-                }
-            if (!mine) {
-                *place = (uint16_t)NO_PLACE;
-                continue;
-            }
-        }
-        *place = (uint16_t)to;
-        o.weight[base + to] = row_label[r] == key ? w + t.hard : w;
+        leave(place, spot, dead ? pg::ENTRY_DEAD : 0u, w);
+        o.place[(size_t)(first + r) * t.K1 + k] = (uint16_t)(dead ? NO_PLACE : place);
     }
     if (labels && threadIdx.x < n_rows) {
-        const uint32_t key = row_label[threadIdx.x], at = keys_below(sorted, valid, key), to = at + shift(key);
-        const bool entry = at < valid && sorted[at] == key;
-        o.place[(size_t)(first + threadIdx.x) * t.K1 + t.K] = (uint16_t)(entry ? NO_PLACE : to);
-        if (!entry) {
-            leave(to, key, false);
-            o.weight[base + to] = t.hard;
-        }
+        const uint32_t spot = row_label[threadIdx.x], at = find(spot), place = at + labels_below(spot);
+        const bool entry = is_at(at, spot);
+        o.place[(size_t)(first + threadIdx.x) * t.K1 + t.K] = (uint16_t)(entry ? NO_PLACE : place);
+        if (!entry) leave(place, spot, 0u, t.hard);
     }
     for (uint32_t g = threadIdx.x; g < o.groups1; g += LIST_THREADS) {
-        const uint32_t limit = g * (pg::ENTRY_PLACES / 2);
-        o.offsets[(size_t)blockIdx.x * o.groups1 + g] = (uint16_t)(keys_below(sorted, valid, limit) + shift(limit));
+        const uint32_t spot = g * (pg::ENTRY_PLACES / 2);
+        o.offsets[(size_t)blockIdx.x * o.groups1 + g] = (uint16_t)(find(spot) + labels_below(spot));
     }
 }
 
