@@ -7,11 +7,12 @@
 namespace ullis {
 namespace dev {
 
-// Thread t has keys t * E .. of them; `shared` has room for E * THREADS keys and is free before and after.
+// Thread t of THREADS has keys t * E .. of them; `shared` has room for E * THREADS keys and is free before and after (32 threads, a
+// warp: none is needed, and nobody waits).
 template <typename K, int E, int THREADS>
-__device__ __forceinline__ void block_sort(K (&v)[E], K* shared) {
+__device__ __forceinline__ void block_sort(K (&v)[E], K* shared, uint32_t t) {
     constexpr uint32_t N = (uint32_t)E * THREADS;
-    const uint32_t t = threadIdx.x, first = t * E;
+    const uint32_t first = t * E;
     const auto within = [&](uint32_t run) {   // the steps over fewer than E keys; runs of at most E keys have no others
 #pragma unroll
         for (int step = E / 2; step > 0; step >>= 1) {
@@ -36,13 +37,13 @@ __device__ __forceinline__ void block_sort(K (&v)[E], K* shared) {
         for (uint32_t step = run >> 1; step >= (uint32_t)E; step >>= 1) {
             const uint32_t apart = step / E;
             const bool smaller = ((t & apart) == 0) == rising;
-            if (apart < 32) {
+            if (THREADS == 32 || apart < 32) {
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
                     const K other = __shfl_xor_sync(0xffffffffu, v[i], apart);
                     v[i] = (v[i] < other) == smaller ? v[i] : other;
                 }
-            } else {
+            } else if constexpr (THREADS > 32) {
 #pragma unroll
                 for (int i = 0; i < E; ++i) shared[i * THREADS + t] = v[i];
                 __syncthreads();

@@ -270,7 +270,7 @@ embed_sort_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, uint3
             keys[i] = (K)token << BITS | (first + i);
         }
     }
-    block_sort<K, SORT_EACH, SORT_THREADS>(keys, reinterpret_cast<K*>(smem_raw));
+    block_sort<K, SORT_EACH, SORT_THREADS>(keys, reinterpret_cast<K*>(smem_raw), threadIdx.x);
 #pragma unroll
     for (uint32_t i = 0; i < SORT_EACH; ++i) {
         if (i % WINDOW == WINDOW - 1) samples[(base + first + i) / WINDOW] = (uint32_t)(keys[i] >> BITS);

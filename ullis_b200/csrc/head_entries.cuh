@@ -165,7 +165,7 @@ entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const i
 #pragma unroll
     for (int i = 0; i < E; ++i) v[i] = threadIdx.x * E + i < n ? sorted[threadIdx.x * E + i] : NO_KEY;
     __syncthreads();
-    block_sort<Key, E, LIST_THREADS>(v, sorted);
+    block_sort<Key, E, LIST_THREADS>(v, sorted, threadIdx.x);
 #pragma unroll
     for (int i = 0; i < E; ++i) sorted[threadIdx.x * E + i] = v[i];
     __syncthreads();
