@@ -20,6 +20,25 @@ struct Stream {   // where a call's kernels go
         rt->launch_on(stream, true, kernel, grid, block, smem, P(args)...);
         launched(what);
     }
+    // The same with clusters of `ctas` CTAs.
+    template <typename... P, typename... A>
+    void chain_cluster(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, unsigned ctas, A... args) const {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attrs[2] = {};
+        attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[0].val.programmaticStreamSerializationAllowed = 1;
+        attrs[1].id = cudaLaunchAttributeClusterDimension;
+        attrs[1].val.clusterDim.x = ctas;
+        attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+        cfg.gridDim = grid;
+        cfg.blockDim = block;
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cfg.attrs = attrs;
+        cfg.numAttrs = 2;
+        ULLIS_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+        launched(what);
+    }
     void launched(const char* what) const {
         if (stream == rt->stream) { rt->launched(what); return; }   // (timing marks are events on that stream)
         ++rt->launches;

@@ -233,71 +233,97 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
 }
 
 // ------------------------------------------------------------------------------------------------ gradient of many rows
-// Tokens are sorted by chunks in shared memory (beside which other CTAs write the table's zeros), an element's place among all is its
-// place in its chunk and what searches in the others give, and warps sum runs of rows in that order, a fixed number of
-// places each whatever the tokens are: a run that ends in another warp's places leaves a part of its sum, and a last launch adds those.
-constexpr uint32_t SORT_EACH = 8;   // keys to a thread
+// Tokens are sorted by chunks, each by a cluster; with more chunks than one an element's place among all is its place in its chunk and
+// what searches in the others give.  Beside both other CTAs write the table's zeros, which costs nothing there (zeros for the rows alone
+// that no chunk has, found by the same searches: 76550 x 500 into 50021 rows 108 us instead of 82).  Then warps sum runs of rows in that order, a fixed number
+// of places each whatever the tokens are: a run that ends in another warp's places leaves a part of its sum, and a last launch adds those.
+constexpr uint32_t SORT_EACH = 8, SORT_THREADS = 256, SORT_CTA = SORT_EACH * SORT_THREADS;   // keys to a thread, of a CTA
+constexpr uint32_t MOST_CTAS = 8;   // of a cluster
 constexpr uint32_t WINDOW = 8;      // of sorted tokens, the last of which are kept apart
 
-// Keys token << BITS | place, padded with the largest.
-template <typename K, uint32_t BITS>
-__global__ void __launch_bounds__((1u << BITS) / SORT_EACH)
-embed_sort_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, uint32_t rows, uint32_t vocab, uint32_t chunks,
-                  uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row, uint32_t* __restrict__ samples,
-                  float* __restrict__ g, size_t elements) {
-    chain_entry();
-    constexpr uint32_t SIZE = 1u << BITS, SORT_THREADS = SIZE / SORT_EACH;
-    if (blockIdx.x >= chunks) {
-        const size_t at = (size_t)(blockIdx.x - chunks) * SORT_THREADS + threadIdx.x, step = (size_t)(gridDim.x - chunks) * SORT_THREADS;
-        size_t quads = 0;
-        if (reinterpret_cast<uintptr_t>(g) % 16 == 0) {
-            quads = elements / 4;
+// Zeros for `elements` of g, by threads `at`, `at` + `step` ...
+__device__ __forceinline__ void write_zeros(float* g, size_t elements, size_t at, size_t step) {
+    size_t quads = 0;
+    if (reinterpret_cast<uintptr_t>(g) % 16 == 0) {
+        quads = elements / 4;
 #pragma unroll 4
-            for (size_t i = at; i < quads; i += step) reinterpret_cast<float4*>(g)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-        for (size_t i = quads * 4 + at; i < elements; i += step) g[i] = 0.0f;
+        for (size_t i = at; i < quads; i += step) reinterpret_cast<float4*>(g)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (size_t i = quads * 4 + at; i < elements; i += step) g[i] = 0.0f;
+}
+
+// Keys token * size of the chunk + place, padded with the largest.  A chunk is what a cluster's CTAs hold.
+template <typename K>
+__global__ void __launch_bounds__(SORT_THREADS)
+embed_sort_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, uint32_t rows, uint32_t vocab, uint32_t bits, uint32_t sort_ctas,
+                  uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row, uint32_t* __restrict__ samples,
+                  float* __restrict__ g, size_t zeros) {
+    chain_entry();
+    if (blockIdx.x >= sort_ctas) {   // (whole clusters)
+        write_zeros(g, zeros, (size_t)(blockIdx.x - sort_ctas) * SORT_THREADS + threadIdx.x, (size_t)(gridDim.x - sort_ctas) * SORT_THREADS);
         return;
     }
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    const uint32_t base = blockIdx.x * SIZE, first = threadIdx.x * SORT_EACH;
+    __shared__ __align__(16) K buffers[3 * SORT_CTA];
+    uint32_t rank, ctas;
+    asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %cluster_nctaid.x;" : "=r"(ctas));
+    const uint32_t first = blockIdx.x * SORT_CTA + threadIdx.x * SORT_EACH, in_chunk = first & ((1u << bits) - 1);
     K keys[SORT_EACH];
 #pragma unroll
     for (uint32_t i = 0; i < SORT_EACH; ++i) {
         keys[i] = ~(K)0;
-        if (base + first + i < rows) {
-            uint32_t token = tokens[base + first + i];
+        if (first + i < rows) {
+            uint32_t token = tokens[first + i];
             if (token == ignore_id || token > vocab) token = vocab;   // behind all others
-            keys[i] = (K)token << BITS | (first + i);
+            keys[i] = (K)token << bits | (in_chunk + i);
         }
     }
-    block_sort<K, SORT_EACH, SORT_THREADS>(keys, reinterpret_cast<K*>(smem_raw), threadIdx.x);
+    cluster_sort<K, SORT_EACH, SORT_THREADS>(keys, buffers, buffers + SORT_CTA, rank, ctas);
+    uint32_t token[SORT_EACH], row[SORT_EACH];
 #pragma unroll
     for (uint32_t i = 0; i < SORT_EACH; ++i) {
-        if (i % WINDOW == WINDOW - 1) samples[(base + first + i) / WINDOW] = (uint32_t)(keys[i] >> BITS);
-        sorted_token[base + first + i] = (uint32_t)(keys[i] >> BITS);
-        sorted_row[base + first + i] = base + (uint32_t)(keys[i] & (SIZE - 1));
+        token[i] = (uint32_t)(keys[i] >> bits);
+        row[i] = (first - in_chunk) + (uint32_t)(keys[i] & ((K)1 << bits) - 1);
     }
+#pragma unroll
+    for (uint32_t i = 0; i < SORT_EACH; i += 4) {
+        *reinterpret_cast<uint4*>(sorted_token + first + i) = make_uint4(token[i], token[i + 1], token[i + 2], token[i + 3]);
+        *reinterpret_cast<uint4*>(sorted_row + first + i) = make_uint4(row[i], row[i + 1], row[i + 2], row[i + 3]);
+    }
+    static_assert(SORT_EACH == WINDOW, "");
+    samples[first / WINDOW] = token[WINDOW - 1];
 }
 
 // An element's place: how many elements of every other chunk come before it.  The last token of every eight of a chunk lies in shared
 // memory, where the eight are found; they are a sector of memory, read at once.  Four chunks are searched side by side, so that
 // their reads wait for memory together.  (Steps of a search in memory are a sector each: 33 us for 38 chunks of 2048, so 8.)
-constexpr uint32_t SAMPLES_HELD = 16384;
-__global__ void __launch_bounds__(THREADS)
+constexpr uint32_t CHUNK_BITS = 14, SAMPLES_HELD = 16384;
+static_assert(1u << CHUNK_BITS == MOST_CTAS * SORT_CTA, "");
+__global__ void __launch_bounds__(THREADS, 3)
 embed_rank_kernel(const uint32_t* __restrict__ chunk_token, const uint32_t* __restrict__ chunk_row, const uint32_t* __restrict__ samples,
-                  uint32_t rows, uint32_t size, uint32_t chunks, uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row) {
+                  uint32_t rows, uint32_t chunks, uint32_t* __restrict__ sorted_token, uint32_t* __restrict__ sorted_row, float* __restrict__ g,
+                  size_t zeros) {
     chain_entry();
-    constexpr uint32_t TOGETHER = 4;
+    constexpr uint32_t TOGETHER = 4, size = 1u << CHUNK_BITS, per_chunk = size / WINDOW, chunks_held = SAMPLES_HELD / per_chunk;
     extern __shared__ __align__(16) uint32_t held[];
-    const uint32_t i = blockIdx.x * THREADS + threadIdx.x, per_chunk = size / WINDOW, chunks_held = SAMPLES_HELD / per_chunk;
+    const uint32_t rank_ctas = (rows + THREADS - 1) / THREADS;
+    const auto hold = [&](uint32_t c0, uint32_t n) {
+        __syncthreads();
+#pragma unroll 8
+        for (uint32_t k = threadIdx.x * 4; k < n * per_chunk; k += THREADS * 4)
+            *reinterpret_cast<uint4*>(held + k) = *reinterpret_cast<const uint4*>(samples + (size_t)c0 * per_chunk + k);
+        __syncthreads();
+    };
+    if (blockIdx.x >= rank_ctas) {
+        write_zeros(g, zeros, (size_t)(blockIdx.x - rank_ctas) * THREADS + threadIdx.x, (size_t)(gridDim.x - rank_ctas) * THREADS);
+        return;
+    }
+    const uint32_t i = blockIdx.x * THREADS + threadIdx.x;
     const uint32_t own = i / size, token = chunk_token[i], row = chunk_row[i];   // (whole chunks are there)
     uint32_t rank = i - own * size;
     for (uint32_t c0 = 0; c0 < chunks; c0 += chunks_held) {
         const uint32_t n = min(chunks_held, chunks - c0);
-        if (c0) __syncthreads();
-        for (uint32_t k = threadIdx.x * 4; k < n * per_chunk; k += THREADS * 4)
-            *reinterpret_cast<uint4*>(held + k) = *reinterpret_cast<const uint4*>(samples + (size_t)c0 * per_chunk + k);
-        __syncthreads();
+        hold(c0, n);
         for (uint32_t k0 = 0; k0 < n; k0 += TOGETHER) {
             uint32_t at[TOGETHER], limit[TOGETHER];
             uint4 eight[TOGETHER][2];
@@ -308,6 +334,7 @@ embed_rank_kernel(const uint32_t* __restrict__ chunk_token, const uint32_t* __re
                 limit[u] = c == own || k0 + u >= n ? 0u : token + (c < own);
                 at[u] = min(k0 + u, n - 1) * per_chunk;
             }
+#pragma unroll
             for (uint32_t step = per_chunk / 2; step > 0; step >>= 1)
 #pragma unroll
                 for (uint32_t u = 0; u < TOGETHER; ++u)
@@ -342,11 +369,12 @@ struct GradSums {
     float scale;
     float *g, *head, *tail;        // parts of sums that began before a warp's places, and that go on behind them: [warp][C]
 };
-// A warp has `places` (a power of two, at most 32) places of the sorted order and 32 chunks of channels.
-template <typename T, int N, bool WIDE>
+// A warp has `places` (a power of two, at most 32) places of the sorted order and 256 channels, a lane BLOCKS times N of them.
+template <typename T, int N, int BLOCKS, bool WIDE>
 __global__ void __launch_bounds__(THREADS)
 embed_sums_kernel(const GradSums o) {
     chain_entry();
+    constexpr uint32_t ALL = 0xffffffffu;
     const uint32_t lane = threadIdx.x & 31;
     const size_t warp = (size_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
     const uint32_t tile = (uint32_t)(warp / o.blocks), block = (uint32_t)(warp - (size_t)tile * o.blocks);
@@ -355,39 +383,47 @@ embed_sums_kernel(const GradSums o) {
     const uint32_t n = min(o.places, o.rows - first), at = first + min(lane, n - 1);
     const uint32_t my_token = o.token[at], my_row = o.row[at];
     const uint32_t before = first > 0 ? o.token[first - 1] : 0xFFFFFFFFu, after = first + n < o.rows ? o.token[first + n] : 0xFFFFFFFFu;
-    const uint32_t c = block * 32 * N + lane * (WIDE ? N : 1);
-    const bool in = c < o.C;
+    const uint32_t right = __shfl_down_sync(ALL, my_token, 1);
+    const uint32_t ends = __ballot_sync(ALL, lane < n && my_token != (lane + 1 < n ? right : after));   // places that a run ends at
+    const uint32_t live = __ballot_sync(ALL, lane < n && my_token < o.vocab);
+    const uint32_t c = block * (32 * N * BLOCKS) + lane * (WIDE ? N : 1);   // and 32 * N further on for each block
     const T* gy = static_cast<const T*>(o.gy);
-    float sum[N] = {};
-    bool began_here = __shfl_sync(0xffffffffu, my_token, 0) != before;
-    constexpr int AHEAD = 8;   // rows on their way (16 of 8 bytes: 121 registers, and 82 us instead of 42 for 76550 x 500 bf16)
+    float sum[BLOCKS][N] = {};
+    bool began_here = __shfl_sync(ALL, my_token, 0) != before;
+    constexpr int AHEAD = 32 / (BLOCKS * N * (int)sizeof(T) / 4);   // rows on their way: 32 registers of them
     for (uint32_t k0 = 0; k0 < n; k0 += AHEAD) {
-        Channels<WIDE, N, 32, T> v[AHEAD];
+        Channels<WIDE, N, 32, T> v[AHEAD][BLOCKS];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const uint32_t k = min(k0 + u, n - 1);
-            const uint32_t token = __shfl_sync(0xffffffffu, my_token, k), row = __shfl_sync(0xffffffffu, my_row, k);
-            v[u].load(gy + row * o.stride, c, in && token < o.vocab && k0 + u < n ? o.C : 0u);
+            const T* from = gy + __shfl_sync(ALL, my_row, k0 + u) * o.stride;
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) v[u][b].load(from, c + b * 32 * N, live >> (k0 + u) & 1u ? o.C : 0u);
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const uint32_t k = k0 + u;
             if (k >= n) break;
-            const uint32_t token = __shfl_sync(0xffffffffu, my_token, k), next_lane = __shfl_sync(0xffffffffu, my_token, min(k + 1, n - 1));
-            const uint32_t next = k + 1 < n ? next_lane : after;
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] += tape::to_float(v[u].t[e]);
-            if (token == next && k + 1 < n) continue;
-            if (in && token < o.vocab) {
-                const bool whole = began_here && token != next;
-                float* to = whole ? o.g + (size_t)token * o.C : (began_here ? o.tail : o.head) + (size_t)tile * o.C;
+            for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[b][e] += tape::to_float(v[u][b].t[e]);
+            const bool end = ends >> k & 1u;
+            if (!end && k + 1 < n) continue;
+            if (live >> k & 1u) {
+                const bool whole = began_here && end;
+                float* to = whole ? o.g + (size_t)__shfl_sync(ALL, my_token, k) * o.C : (began_here ? o.tail : o.head) + (size_t)tile * o.C;
                 const float times = whole ? o.scale : 1.0f;
 #pragma unroll
-                for (int e = 0; e < N; ++e) sum[e] *= times;
-                store_channels<WIDE, N, 32>(to, c, o.C, sum);
+                for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sum[b][e] *= times;
+                    if (c + b * 32 * N < o.C) store_channels<WIDE, N, 32>(to, c + b * 32 * N, o.C, sum[b]);
+                }
             }
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] = 0.0f;
+            for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[b][e] = 0.0f;
             began_here = true;
         }
     }
@@ -397,46 +433,59 @@ embed_sums_kernel(const GradSums o) {
 // has 128 channels of what began in the places of eight warps: sums of few parts a warp each, then those of many one after the other, by
 // eight warps a stretch of the parts each.
 constexpr uint32_t FEW_PARTS = 4;
+template <bool WIDE>
 __global__ void __launch_bounds__(THREADS)
 embed_join_kernel(const GradSums o, uint32_t tiles) {
     chain_entry();
     constexpr uint32_t WARPS = THREADS / 32;
     __shared__ uint32_t all_parts[WARPS];
-    __shared__ float sums[WARPS][128];
+    __shared__ float sums[WARPS][4][32];
     const uint32_t per_tile = (o.C + 127) / 128, block = blockIdx.x % per_tile, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t first_tile = blockIdx.x / per_tile * WARPS, tile = first_tile + warp, c = block * 128 + lane;
+    const uint32_t first_tile = blockIdx.x / per_tile * WARPS, tile = first_tile + warp, c = block * 128 + lane * (WIDE ? 4 : 1);
+    const auto first_token = [&](uint32_t t) { return o.token[(size_t)t * o.places]; };
     uint32_t parts = 0;   // heads
     if (tile + 1 < tiles) {   // (the last warp's sums go on nowhere)
-        const uint32_t first = tile * o.places, next = first + o.places, token = o.token[next - 1];
-        if (token < o.vocab && o.token[next] == token && !(first > 0 && o.token[first - 1] == token)) {
-            // warps whose first place has the token: 32 of them at a time
-            for (uint32_t t = tile + 1;; t += 32) {
-                const bool more = t + lane < tiles && o.token[(t + lane) * o.places] == token;
-                const uint32_t mask = __ballot_sync(0xffffffffu, more);
-                parts += __popc(mask);
-                if (mask != 0xffffffffu) break;
+        const uint32_t first = tile * o.places, token = o.token[first + o.places - 1], next = o.token[first + o.places];
+        const uint32_t before = first > 0 ? o.token[first - 1] : 0xFFFFFFFFu;
+        if (token < o.vocab && next == token && before != token) {
+            // one behind the last warp whose first place has the token: 32 looks at once
+            uint32_t low = tile + 1, high = tiles;   // low has it, high has not or is none
+            while (high - low > 1) {
+                const uint32_t step = (high - low + 31) / 32, at = low + lane * step;
+                const uint32_t mask = __ballot_sync(0xffffffffu, at < high && first_token(min(at, high - 1)) == token);   // (lanes from 0 on)
+                const uint32_t last = 31 - __clz(mask);
+                high = min(high, low + (last + 1) * step);
+                low += last * step;
             }
+            parts = high - tile - 1;
         }
     }
+    using Part = Channels<WIDE, 4, 32, float>;
     const auto add = [&](float (&sum)[4], uint32_t of, uint32_t from, uint32_t to) {   // heads [from, to) of the sum that began in warp `of`
-#pragma unroll 4
-        for (uint32_t k = from; k < to; ++k)
+        constexpr uint32_t AHEAD = 8;
+        for (uint32_t k = from; k < to; k += AHEAD) {
+            Part part[AHEAD];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (c + 32 * e < o.C) sum[e] += o.head[(size_t)(of + 1 + k) * o.C + c + 32 * e];
+            for (uint32_t u = 0; u < AHEAD; ++u) part[u].load(o.head + (size_t)(of + 1 + k + u) * o.C, c, k + u < to ? o.C : 0u);
+#pragma unroll
+            for (uint32_t u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += part[u].t[e];
+        }
     };
     const auto tail = [&](float (&sum)[4], uint32_t of, bool wanted) {
+        load_channels<WIDE, 4, 32>(o.tail + (size_t)of * o.C, c, wanted ? o.C : 0u, sum);
+    };
+    const auto leave = [&](float (&sum)[4], uint32_t of) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = wanted && c + 32 * e < o.C ? o.tail[(size_t)of * o.C + c + 32 * e] : 0.0f;
+        for (int e = 0; e < 4; ++e) sum[e] *= o.scale;
+        if (c < o.C) store_channels<WIDE, 4, 32>(o.g + (size_t)o.token[(size_t)of * o.places + o.places - 1] * o.C, c, o.C, sum);
     };
     float sum[4];
     if (parts > 0 && parts <= FEW_PARTS) {
         tail(sum, tile, true);
         add(sum, tile, 0, parts);
-        float* to = o.g + (size_t)o.token[tile * o.places + o.places - 1] * o.C;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + 32 * e < o.C) to[c + 32 * e] = sum[e] * o.scale;
+        leave(sum, tile);
     }
     if (lane == 0) all_parts[warp] = parts;
     __syncthreads();
@@ -446,13 +495,14 @@ embed_join_kernel(const GradSums o, uint32_t tiles) {
         tail(sum, of, warp == 0);
         add(sum, of, (uint32_t)((uint64_t)warp * n / WARPS), (uint32_t)((uint64_t)(warp + 1) * n / WARPS));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sums[warp][lane + 32 * e] = sum[e];
+        for (int e = 0; e < 4; ++e) sums[warp][e][lane] = sum[e];
         __syncthreads();
-        if (threadIdx.x < 128 && block * 128 + threadIdx.x < o.C) {
-            float all = sums[0][threadIdx.x];
+        if (warp == 0) {
 #pragma unroll
-            for (uint32_t k = 1; k < WARPS; ++k) all += sums[k][threadIdx.x];
-            o.g[(size_t)o.token[of * o.places + o.places - 1] * o.C + block * 128 + threadIdx.x] = all * o.scale;
+            for (uint32_t k = 1; k < WARPS; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += sums[k][e][lane];
+            leave(sum, of);
         }
         __syncthreads();
     }
@@ -467,11 +517,12 @@ GradPlan grad_plan(const ullis_cuda_runtime* rt, size_t rows, size_t C) {
     GradPlan p{};
     p.few = rows <= FEW;
     if (p.few) return p;
-    // Chunks of 2048 are sorted faster than those of 8192 by more than the search in four times as many takes, up to 64 of them.
-    p.bits = rows <= 131072 ? 11 : 13;
+    // One chunk of as many CTAs as hold the rows, or several of eight CTAs.
+    p.bits = 11;
+    while (p.bits < CHUNK_BITS && (size_t)1 << p.bits < rows) ++p.bits;
     p.chunks = (uint32_t)ceil_div(rows, (size_t)1 << p.bits);
-    // Places of a warp: as many as leave sixteen warps to an SM, each with 128 channels.
-    p.blocks = (uint32_t)ceil_div(C, 128);
+    // Places of a warp: as many as leave sixteen warps to an SM.
+    p.blocks = (uint32_t)ceil_div(C, 256);
     p.places = 32;
     while (p.places > 4 && ceil_div(rows, p.places) * p.blocks < (size_t)rt->sm_count * 16) p.places /= 2;
     p.tiles = ceil_div(rows, p.places);
@@ -493,16 +544,6 @@ GradPlan grad_plan(const ullis_cuda_runtime* rt, size_t rows, size_t C) {
     return p;
 }
 
-template <typename K, uint32_t BITS>
-void launch_sort(const Stream& s, unsigned zeros, const uint32_t* tokens, uint32_t ignore_id, size_t rows, size_t vocab, uint32_t chunks,
-                 uint32_t* token, uint32_t* row, uint32_t* samples, float* g, size_t elements) {
-    const auto kernel = embed_sort_kernel<K, BITS>;
-    constexpr size_t SMEM = sizeof(K) << BITS;
-    if (SMEM > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
-    s.chain("embed_sort", kernel, chunks + zeros, (1u << BITS) / SORT_EACH, SMEM, tokens, ignore_id, (uint32_t)rows, (uint32_t)vocab, chunks, token,
-            row, samples, g, elements);
-}
-
 template <typename T>
 void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, Rows gy, size_t rows, size_t C, size_t vocab, float scale, float* g,
                    void* workspace) {
@@ -522,16 +563,20 @@ void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, 
     uint32_t *chunk_row = p.chunks > 1 ? reinterpret_cast<uint32_t*>(ws + p.chunk_row) : row;
     uint32_t* samples = reinterpret_cast<uint32_t*>(ws + p.samples);
     const size_t elements = vocab * C;
-    const unsigned zeros = (unsigned)std::min<size_t>((size_t)s.rt->sm_count * 8, ceil_div(elements, 4096));
+    // (32 MB beside the sort)
+    const size_t zeros = p.chunks > 1 ? std::min(elements, (size_t)8 << 20) : elements;
+    const auto zero_ctas = [&](size_t n) { return std::min<size_t>((size_t)s.rt->sm_count * 8, ceil_div(n, 4096)); };
     const bool narrow = (vocab + 1) >> (32 - p.bits) == 0;   // the largest key is that of the padding
-    const auto sort = p.bits == 11 ? (narrow ? launch_sort<uint32_t, 11> : launch_sort<uint64_t, 11>)
-                                   : (narrow ? launch_sort<uint32_t, 13> : launch_sort<uint64_t, 13>);
-    sort(s, zeros, tokens, ignore_id, rows, vocab, p.chunks, chunk_token, chunk_row, samples, g, elements);
+    const uint32_t ctas = (1u << p.bits) / SORT_CTA, sort_ctas = p.chunks * ctas;
+    const auto sort = narrow ? embed_sort_kernel<uint32_t> : embed_sort_kernel<uint64_t>;
+    s.chain_cluster("embed_sort", sort, sort_ctas + (unsigned)ceil_div(zero_ctas(zeros), ctas) * ctas, SORT_THREADS, 0, ctas, tokens, ignore_id,
+                    (uint32_t)rows, (uint32_t)vocab, p.bits, sort_ctas, chunk_token, chunk_row, samples, g, zeros);
     if (p.chunks > 1) {
         const size_t held = std::min<size_t>(SAMPLES_HELD, ((size_t)p.chunks << p.bits) / WINDOW) * 4;
         if (held > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(embed_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)held));
-        s.chain("embed_rank", embed_rank_kernel, (unsigned)ceil_div(rows, THREADS), THREADS, held, static_cast<const uint32_t*>(chunk_token),
-                static_cast<const uint32_t*>(chunk_row), static_cast<const uint32_t*>(samples), (uint32_t)rows, 1u << p.bits, p.chunks, token, row);
+        s.chain("embed_rank", embed_rank_kernel, (unsigned)(ceil_div(rows, THREADS) + zero_ctas(elements - zeros)), THREADS, held,
+                static_cast<const uint32_t*>(chunk_token), static_cast<const uint32_t*>(chunk_row), static_cast<const uint32_t*>(samples),
+                (uint32_t)rows, p.chunks, token, row, g + zeros, elements - zeros);
     }
     GradSums o{};
     o.token = token;
@@ -546,15 +591,13 @@ void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, 
     o.g = g;
     o.head = reinterpret_cast<float*>(ws + p.head);
     o.tail = reinterpret_cast<float*>(ws + p.tail);
-    const auto sums = [&](auto kernel, int each) {
-        o.blocks = (uint32_t)ceil_div(C, 32 * each);
-        s.chain("embed_sums", kernel, (unsigned)ceil_div(p.tiles * o.blocks, THREADS / 32), THREADS, 0, o);
-    };
-    if (wide) sums(embed_sums_kernel<T, N, true>, N);
-    else if (N == 8 && on(4)) sums(embed_sums_kernel<T, N == 8 ? 4 : N, true>, 4);
-    else sums(embed_sums_kernel<T, 4, false>, 4);
+    o.blocks = p.blocks;
+    const auto sums = [&](auto kernel) { s.chain("embed_sums", kernel, (unsigned)ceil_div(p.tiles * p.blocks, THREADS / 32), THREADS, 0, o); };
+    if (wide) sums(embed_sums_kernel<T, N, 8 / N, true>);
+    else if (N == 8 && on(4)) sums(embed_sums_kernel<T, 4, 2, true>);
+    else sums(embed_sums_kernel<T, 4, 2, false>);
     if (p.tiles > 1)
-        s.chain("embed_join", embed_join_kernel, (unsigned)(ceil_div(p.tiles - 1, THREADS / 32) * ceil_div(C, 128)), THREADS, 0, o, (uint32_t)p.tiles);
+        s.chain("embed_join", C % 4 == 0 && aligned(g, 16) ? embed_join_kernel<true> : embed_join_kernel<false>, (unsigned)(ceil_div(p.tiles - 1, THREADS / 32) * ceil_div(C, 128)), THREADS, 0, o, (uint32_t)p.tiles);
 }
 
 }  // namespace
