@@ -234,20 +234,20 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
 
 // ------------------------------------------------------------------------------------------------ gradient of many rows
 // Tokens are sorted by chunks, each by a cluster; with more chunks than one an element's place among all is its place in its chunk and
-// what searches in the others give.  Beside both other CTAs write the table's zeros, which costs nothing there (zeros for the rows alone
-// that no chunk has, found by the same searches: 76550 x 500 into 50021 rows 108 us instead of 82).  Then warps sum runs of rows in that order, a fixed number
+// what searches in the others give.  Beside the last of these launches other CTAs write the table's zeros, which costs little there
+// (zeros for the rows alone that no chunk has, found by the same searches: 76550 x 500 into 50021 rows 108 us instead of 82).  Then warps sum runs of rows in that order, a fixed number
 // of places each whatever the tokens are: a run that ends in another warp's places leaves a part of its sum, and a last launch adds those.
 constexpr uint32_t SORT_EACH = 8, SORT_THREADS = 256, SORT_CTA = SORT_EACH * SORT_THREADS;   // keys to a thread, of a CTA
 constexpr uint32_t MOST_CTAS = 8;   // of a cluster
 constexpr uint32_t WINDOW = 8;      // of sorted tokens, the last of which are kept apart
 
-// Zeros for `elements` of g, by threads `at`, `at` + `step` ...
+// Zeros for `elements` of g, by threads `at`, `at` + `step` ...; the first to leave L2.
 __device__ __forceinline__ void write_zeros(float* g, size_t elements, size_t at, size_t step) {
     size_t quads = 0;
     if (reinterpret_cast<uintptr_t>(g) % 16 == 0) {
         quads = elements / 4;
 #pragma unroll 4
-        for (size_t i = at; i < quads; i += step) reinterpret_cast<float4*>(g)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (size_t i = at; i < quads; i += step) __stcs(reinterpret_cast<float4*>(g) + i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
     }
     for (size_t i = quads * 4 + at; i < elements; i += step) g[i] = 0.0f;
 }
@@ -380,24 +380,40 @@ embed_sums_kernel(const GradSums o) {
     const uint32_t tile = (uint32_t)(warp / o.blocks), block = (uint32_t)(warp - (size_t)tile * o.blocks);
     const uint32_t first = tile * o.places;
     if (first >= o.rows) return;
-    const uint32_t n = min(o.places, o.rows - first), at = first + min(lane, n - 1);
+    const uint32_t there = min(o.places, o.rows - first), at = first + min(lane, there - 1);
     const uint32_t my_token = o.token[at], my_row = o.row[at];
-    const uint32_t before = first > 0 ? o.token[first - 1] : 0xFFFFFFFFu, after = first + n < o.rows ? o.token[first + n] : 0xFFFFFFFFu;
+    const uint32_t before = first > 0 ? o.token[first - 1] : 0xFFFFFFFFu, after = first + there < o.rows ? o.token[first + there] : 0xFFFFFFFFu;
     const uint32_t right = __shfl_down_sync(ALL, my_token, 1);
-    const uint32_t ends = __ballot_sync(ALL, lane < n && my_token != (lane + 1 < n ? right : after));   // places that a run ends at
-    const uint32_t live = __ballot_sync(ALL, lane < n && my_token < o.vocab);
-    const uint32_t c = block * (32 * N * BLOCKS) + lane * (WIDE ? N : 1);   // and 32 * N further on for each block
+    const uint32_t ends = __ballot_sync(ALL, lane < there && my_token != (lane + 1 < there ? right : after));   // places that a run ends at
+    const uint32_t n = __popc(__ballot_sync(ALL, lane < there && my_token < o.vocab));   // (those that do not count come last)
+    // What a lane reads of a row; past the row's end something of it that is not kept.
+    const uint32_t c = block * (32 * N * BLOCKS) + lane * (WIDE ? N : 1);
+    uint32_t from[BLOCKS][WIDE ? 1 : N];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int e = 0; e < (WIDE ? 1 : N); ++e) {
+            const uint32_t channel = c + b * 32 * N + e * 32;
+            from[b][e] = channel < o.C ? channel : 0u;
+        }
     const T* gy = static_cast<const T*>(o.gy);
     float sum[BLOCKS][N] = {};
     bool began_here = __shfl_sync(ALL, my_token, 0) != before;
-    constexpr int AHEAD = 32 / (BLOCKS * N * (int)sizeof(T) / 4);   // rows on their way: 32 registers of them
+    constexpr int AHEAD = WIDE ? 32 / (BLOCKS * N * (int)sizeof(T) / 4) : 4;   // rows on their way: 32 registers of them
     for (uint32_t k0 = 0; k0 < n; k0 += AHEAD) {
         Channels<WIDE, N, 32, T> v[AHEAD][BLOCKS];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const T* from = gy + __shfl_sync(ALL, my_row, k0 + u) * o.stride;
+        for (int u = 0; u < AHEAD; ++u) {   // (behind the last: that row again)
+            const T* row = gy + __shfl_sync(ALL, my_row, k0 + u) * o.stride;
 #pragma unroll
-            for (int b = 0; b < BLOCKS; ++b) v[u][b].load(from, c + b * 32 * N, live >> (k0 + u) & 1u ? o.C : 0u);
+            for (int b = 0; b < BLOCKS; ++b) {
+                if constexpr (WIDE) {
+                    v[u][b].load(row, from[b][0], 0xFFFFFFFFu);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v[u][b].t[e] = row[from[b][e]];
+                }
+            }
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
@@ -409,21 +425,17 @@ embed_sums_kernel(const GradSums o) {
                 for (int e = 0; e < N; ++e) sum[b][e] += tape::to_float(v[u][b].t[e]);
             const bool end = ends >> k & 1u;
             if (!end && k + 1 < n) continue;
-            if (live >> k & 1u) {
-                const bool whole = began_here && end;
-                float* to = whole ? o.g + (size_t)__shfl_sync(ALL, my_token, k) * o.C : (began_here ? o.tail : o.head) + (size_t)tile * o.C;
-                const float times = whole ? o.scale : 1.0f;
+            const bool whole = began_here && end;
+            float* to = whole ? o.g + (size_t)__shfl_sync(ALL, my_token, k) * o.C : (began_here ? o.tail : o.head) + (size_t)tile * o.C;
+            const float times = whole ? o.scale : 1.0f;
 #pragma unroll
-                for (int b = 0; b < BLOCKS; ++b) {
+            for (int b = 0; b < BLOCKS; ++b) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) sum[b][e] *= times;
-                    if (c + b * 32 * N < o.C) store_channels<WIDE, N, 32>(to, c + b * 32 * N, o.C, sum[b]);
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < BLOCKS; ++b)
+                for (int e = 0; e < N; ++e) sum[b][e] *= times;
+                if (c + b * 32 * N < o.C) store_channels<WIDE, N, 32>(to, c + b * 32 * N, o.C, sum[b]);
 #pragma unroll
                 for (int e = 0; e < N; ++e) sum[b][e] = 0.0f;
+            }
             began_here = true;
         }
     }
@@ -563,8 +575,7 @@ void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, 
     uint32_t *chunk_row = p.chunks > 1 ? reinterpret_cast<uint32_t*>(ws + p.chunk_row) : row;
     uint32_t* samples = reinterpret_cast<uint32_t*>(ws + p.samples);
     const size_t elements = vocab * C;
-    // (32 MB beside the sort)
-    const size_t zeros = p.chunks > 1 ? std::min(elements, (size_t)8 << 20) : elements;
+    const size_t zeros = p.chunks > 1 ? 0 : elements;   // beside the sort if it is the only launch before the sums
     const auto zero_ctas = [&](size_t n) { return std::min<size_t>((size_t)s.rt->sm_count * 8, ceil_div(n, 4096)); };
     const bool narrow = (vocab + 1) >> (32 - p.bits) == 0;   // the largest key is that of the padding
     const uint32_t ctas = (1u << p.bits) / SORT_CTA, sort_ctas = p.chunks * ctas;
