@@ -388,3 +388,12 @@ def test_large_vocabularies(cuda_rt, vocab):
     s["top_ids"][:, 4] = vocab - 1 - torch.arange(70, device="cuda").to(torch.int32) % 3
     s["top_ids"][::2, 9] = s["top_ids"][::2, 4]
     check(call(cuda_rt, s), formulas(s))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [2.0, 4.0, 1.9999999, 3.0])
+def test_temperatures_that_are_squared(cuda_rt, temperature, dtype):
+    """At 2 and 4 the first softmax comes of the second's squares; sure rows, whose other columns' exps are far below 1, with them."""
+    for lean in (1.0, 8.0):
+        s = student(700, 100, 96, 1500, dtype, True, 24, temperature=temperature, lean=lean, seed=11, absent=0.2)
+        check(call(cuda_rt, s), formulas(s))

@@ -14,17 +14,11 @@ template <typename K, int E, int THREADS>
 __device__ __forceinline__ void sort_steps(K (&v)[E], K* shared, uint32_t t, uint32_t base, uint32_t run, uint32_t step) {
     const uint32_t first = base + t * E;
     const bool rising = (first & run) == 0;   // (of runs of more than E keys: the same for all of a thread's)
+    if constexpr (THREADS > 32) {
 #pragma unroll 1
-    for (; step >= (uint32_t)E; step >>= 1) {
-        const uint32_t apart = step / E;
-        const bool smaller = ((t & apart) == 0) == rising;
-        if (THREADS == 32 || apart < 32) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const K other = __shfl_xor_sync(0xffffffffu, v[i], apart);
-                v[i] = (v[i] < other) == smaller ? v[i] : other;
-            }
-        } else if constexpr (THREADS > 32) {
+        for (; step >= 32u * E; step >>= 1) {
+            const uint32_t apart = step / E;
+            const bool smaller = ((t & apart) == 0) == rising;
 #pragma unroll
             for (int i = 0; i < E; ++i) shared[i * THREADS + t] = v[i];
             __syncthreads();
@@ -34,6 +28,16 @@ __device__ __forceinline__ void sort_steps(K (&v)[E], K* shared, uint32_t t, uin
                 v[i] = (v[i] < other) == smaller ? v[i] : other;
             }
             __syncthreads();
+        }
+    }
+#pragma unroll
+    for (uint32_t apart = 16; apart > 0; apart >>= 1) {
+        if (step < apart * E) continue;
+        const bool smaller = ((t & apart) == 0) == rising;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const K other = __shfl_xor_sync(0xffffffffu, v[i], apart);
+            v[i] = (v[i] < other) == smaller ? v[i] : other;
         }
     }
 #pragma unroll

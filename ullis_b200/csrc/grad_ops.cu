@@ -81,7 +81,8 @@ template <int EPI, int ACCS, bool BF16>
 void launch_form(const Stream& s, const char* what, const pg::Maps& maps, const pg::Params& p, uint32_t pairs) {
     const auto kernel = pg::pair_gemm_kernel<EPI, ACCS, BF16>;
     const size_t smem = pg::smem_bytes(EPI, ACCS);
-    const uint32_t flag = 1u << (EPI * 4 + (ACCS - 1) * 2 + BF16);
+    static_assert(pg::FORMS * 4 <= 64, "");
+    const uint64_t flag = 1ull << (EPI * 4 + (ACCS - 1) * 2 + BF16);
     if (!(s.rt->pair_gemms_ready & flag)) {
         ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         s.rt->pair_gemms_ready |= flag;
@@ -700,6 +701,7 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
     Teacher teacher{};
     EntryLists lists{};
     bool two = false;
+    int squarings = 0;
     if (d) {
         teacher.ids = d->ids;
         teacher.logits = d->logits;
@@ -709,6 +711,7 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         teacher.hard = h.labels ? (float)(1.0 - (double)d->alpha) : 0.0f;
         teacher.temperature = d->alpha > 0.0f ? d->temperature : 1.0f;
         two = teacher.hard > 0.0f && teacher.temperature != 1.0f;
+        squarings = two && teacher.temperature == 2.0f ? 1 : two && teacher.temperature == 4.0f ? 2 : 0;
         teacher.first = two ? 1.0f : 1.0f / teacher.temperature;
         teacher.second = two ? 1.0f / teacher.temperature : 0.0f;
         lists.bits = reinterpret_cast<uint32_t*>(ws + p.entry_bits);
@@ -783,13 +786,15 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         q.block_entries = (uint32_t)(BLOCK_ROWS * p.K1);
         q.entries = lists.bits;
         q.entry_logits = reinterpret_cast<float2*>(ws + p.entry_logits);
-        q.column_factor = teacher.first;
+        q.column_factor = squarings ? teacher.second : teacher.first;
         q.second_factor = teacher.second;
         q.row_part2 = reinterpret_cast<float*>(ws + p.row_part2);
         q.second_lse2 = reinterpret_cast<float*>(ws + p.second_lse2);
         const auto list_kernel = d->dtype == F32 ? launch_entries_list<float> : d->dtype == F16 ? launch_entries_list<__half> : launch_entries_list<__nv_bfloat16>;
         list_kernel(s, teacher, p.blocks, o.target, list, counted, lists);
-        if (two) launch<pg::LSE_ENTRIES_2, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+        if (squarings == 1) launch<8, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+        else if (squarings == 2) launch<10, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+        else if (two) launch<pg::LSE_ENTRIES_2, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
         else launch<pg::LSE_ENTRIES, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
     } else {
         launch<pg::LSE, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
@@ -861,7 +866,9 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         wp.data = static_cast<const uint16_t*>(w16) + v0 * weight.stride;
         wp.rows = width;
         const CUtensorMap grad_map = map_of(grad, rows, p.piece, p.piece, 16, bf16);
-        if (two) launch<pg::GRAD_ENTRIES_2, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
+        if (squarings == 1) launch<9, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
+        else if (squarings == 2) launch<11, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
+        else if (two) launch<pg::GRAD_ENTRIES_2, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
         else if (d) launch<pg::GRAD_ENTRIES, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
         else launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
         // What follows reads g and nothing of one another: few rows leave room for all three at once.

@@ -268,6 +268,7 @@ entries_rows_kernel(const EntryRows o) {
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
                     const uint32_t other = __shfl_up_sync(0xffffffffu, run, d);
+                    if (!__any_sync(0xffffffffu, in && (int)lane >= d && other == run)) break;   // (nor further apart)
                     const float u = __shfl_up_sync(0xffffffffu, g, d), v = __shfl_up_sync(0xffffffffu, ga, d);
                     if ((int)lane >= d && other == run) {
                         g += u;
@@ -396,8 +397,8 @@ entries_rows_kernel(const EntryRows o) {
         const size_t i = blockIdx.x * block_entries + j;
         const uint32_t bits = o.lists.bits[i], column = o.lists.column[i], of = pg::entry_row(bits);
         const float w = o.lists.weight[i], z = o.logits[i].y;
-        float g = exp2f(z - row_lse[0][of]);
-        if (two) g += exp2f(fmaf(z, t.second, -row_lse[1][of]));
+        float g = pg::exp2_fast(z - row_lse[0][of]);
+        if (two) g += pg::exp2_fast(fmaf(z, t.second, -row_lse[1][of]));
         g = (g - w) * times * pg::half_at(o.scale, column, 1.0f);
         o.lists.column[i] = bits | (o.bf16 ? (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(g)) : (uint32_t)__half_as_ushort(__float2half_rn(g))) << 16;
     }

@@ -42,10 +42,13 @@
 namespace ullis {
 namespace pg {
 
-enum { LSE = 0, GRAD = 1, STORE = 2, SUM = 3, LSE_ENTRIES = 4, GRAD_ENTRIES = 5, LSE_ENTRIES_2 = 6, GRAD_ENTRIES_2 = 7 };
+enum { LSE = 0, GRAD = 1, STORE = 2, SUM = 3, LSE_ENTRIES = 4, GRAD_ENTRIES = 5, LSE_ENTRIES_2 = 6, GRAD_ENTRIES_2 = 7, FORMS = 12 };
 __host__ __device__ constexpr int kind_of(int epi) { return epi >= LSE_ENTRIES ? epi & 1 : epi; }   // LSE, GRAD, STORE or SUM
 __host__ __device__ constexpr bool has_entries(int epi) { return epi >= LSE_ENTRIES; }
 __host__ __device__ constexpr bool has_two(int epi) { return epi >= LSE_ENTRIES_2; }
+// 8, 9: .._ENTRIES_2 at a second temperature of 2; 10, 11: of 4.  The exp of the first softmax is the second's squared once or twice:
+// half the exps.  16384 x 512 x 8192 in FP16: LSE 134 us so 117, GRAD 167 so 151.
+__host__ __device__ constexpr int squarings(int epi) { return epi >= 8 ? (epi - 6) / 2 : 0; }
 
 constexpr uint32_t BM = 256, BN = 256, BK = 64;         // of a pair, per accumulator
 constexpr uint32_t OPERAND_BYTES = 128 * BK * 2;        // one CTA's 128 rows of A, or of one accumulator's B
@@ -56,6 +59,8 @@ constexpr uint32_t MAX_STAGES = 6, SMEM_LIMIT = 227 * 1024;
 constexpr uint32_t STAGING_BYTES = 16 * 128;            // 16 rows of 64 16-bit outputs; GRAD has two of them
 constexpr uint32_t COLUMN_BYTES = 2 * 64 * 4;           // constants of its columns
 constexpr uint32_t ROW_BYTES = 2 * 4 * 32 * 4;          // GRAD: what its rows need, of this tile and of the next
+constexpr uint32_t ROW_WORDS_ENTRIES = 2 * 32;          // GRAD_ENTRIES: half as much a tile, and
+constexpr uint32_t HALF_ENTRIES = 256;                  // the entries of 16 rows and its columns, where they are no more
 constexpr uint32_t EXTRACT_PITCH = 20, EXTRACT_BYTES = 32 * EXTRACT_PITCH * 4;   // LSE_ENTRIES: 16 columns of 32 rows, rows 80 bytes apart
 constexpr uint32_t SUM_BLOCKS = 8;                      // k-blocks of a stretch of K, after which SUM adds with rounding
 
@@ -90,7 +95,7 @@ struct Params {
     uint32_t groups1, block_entries;
     const uint32_t* entries;   // LSE: entry_bits; GRAD: with the 16-bit g * scale * 2^k above them
     float2* entry_logits;      // LSE: the entry's product, and its logit as the epilogues have it
-    float column_factor;       // 1 / the temperature of the first (only) softmax
+    float column_factor;       // 1 / the temperature that the epilogues' logits are at: of the first (only) softmax, with squarings of the second
     float second_factor;       // .._2: 1 / the temperature of the second
     float* row_part2;          // .._2: LSE: the second sums beside row_part's
     const float* second_lse2;  // .._2: GRAD: as lse2
@@ -118,7 +123,7 @@ struct Params {
 inline uint32_t stage_bytes(int accs) { return OPERAND_BYTES * (1 + accs); }
 // Barriers first, then (on 1024 bytes) the ring, then what the epilogue warps have.
 constexpr uint32_t epi_bytes(int epi) {
-    return kind_of(epi) == GRAD    ? 2 * STAGING_BYTES + COLUMN_BYTES + ROW_BYTES
+    return kind_of(epi) == GRAD    ? 2 * STAGING_BYTES + COLUMN_BYTES + (has_entries(epi) ? (2 * ROW_WORDS_ENTRIES + HALF_ENTRIES) * 4 : ROW_BYTES)
            : kind_of(epi) == STORE ? STAGING_BYTES
            : kind_of(epi) == LSE   ? COLUMN_BYTES + (has_entries(epi) ? EXTRACT_BYTES : 0u)
                                    : 0u;
@@ -399,7 +404,7 @@ struct Entries {
     }
     __device__ const uint32_t* list(const Params& p, uint32_t row) const { return p.entries + (size_t)(row / 32) * p.block_entries + first; }
 };
-constexpr int ENTRIES_HELD = 2;   // words of 32 entries that are fetched before the accumulator is there
+constexpr int ENTRIES_HELD = 2;   // LSE: words of 32 entries that are fetched before the accumulator is there
 // The others, in groups of words that are on their way together.
 template <int WORDS, typename F>
 __device__ __forceinline__ void more_entries(const uint32_t* list, uint32_t from, uint32_t to, int lane, F&& use) {
@@ -422,6 +427,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
     constexpr int KIND = kind_of(EPI);
     constexpr bool ENTRIES = has_entries(EPI), TWO = has_two(EPI);
+    constexpr int SQUARINGS = squarings(EPI);
+    constexpr float SECOND = (float)(1 << SQUARINGS);   // with squarings: the second temperature
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr uint32_t STAGE = OPERAND_BYTES * (1 + ACCS);
@@ -624,7 +631,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 const uint32_t slot = pair - share_of(work.m_tiles * width, pairs).owner(m_now * width);
                 const size_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
                 const size_t at = piece_now * p.row_part_piece + (size_t)(slot * 4 + group) * rows + row;
-                p.row_part[at] = make_float2(top, sum);
+                p.row_part[at] = make_float2(top * SECOND, sum);   // (top: at the first temperature)
                 if (TWO) p.row_part2[at] = sum2;
             };
             const float log2e = ENTRIES ? LOG2E * p.column_factor : LOG2E;
@@ -691,7 +698,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                                 const uint32_t column = entry_column(bits);
                                 if (bits == NO_ENTRY || column / 16 != c) return;
                                 const float a = extract[entry_row(bits) * EXTRACT_PITCH + column % 16];
-                                logits[i] = make_float2(a, fmaf(a, columns[column], columns[64 + column]));
+                                logits[i] = make_float2(a, fmaf(a, columns[column], columns[64 + column]) * SECOND);
                             };
 #pragma unroll
                             for (int b = 0; b < ENTRIES_HELD; ++b) take(b * 32 + lane, held[b]);
@@ -722,8 +729,16 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     }
                     best[0] = fmaxf(best[0], best[1]);
                     if (best[0] > top) {
-                        sum *= exp2_fast(top - best[0]);   // top = -inf: 0 * 0
-                        if (TWO) sum2 *= exp2_fast((top - best[0]) * p.second_factor);
+                        if constexpr (SQUARINGS > 0) {
+                            float less = exp2_fast(top - best[0]);
+                            sum2 *= less;
+#pragma unroll
+                            for (int k = 0; k < SQUARINGS; ++k) less *= less;
+                            sum *= less;
+                        } else {
+                            sum *= exp2_fast(top - best[0]);   // top = -inf: 0 * 0
+                            if (TWO) sum2 *= exp2_fast((top - best[0]) * p.second_factor);
+                        }
                         top = best[0];
                     }
                     const float base = top == -INFINITY ? 0.0f : -top;   // (a NaN among z makes the sum one)
@@ -734,8 +749,14 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     for (int i = 0; i < 8; ++i) {
                         const uint64_t less = add2(z[i], base2);
                         const float2 v = of_two(less);
-                        here[i & 1] = add2(here[i & 1], two(exp2_fast(v.x), exp2_fast(v.y)));
-                        if (TWO) {
+                        uint64_t e = two(exp2_fast(v.x), exp2_fast(v.y));
+                        if constexpr (SQUARINGS > 0) {
+                            here2[i & 1] = add2(here2[i & 1], e);
+#pragma unroll
+                            for (int k = 0; k < SQUARINGS; ++k) e = mul2(e, e);
+                        }
+                        here[i & 1] = add2(here[i & 1], e);
+                        if (TWO && SQUARINGS == 0) {
                             const float2 u = of_two(mul2(less, second));
                             here2[i & 1] = add2(here2[i & 1], two(exp2_fast(u.x), exp2_fast(u.y)));
                         }
@@ -777,11 +798,13 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             };
             // What the rows need lies in shared memory, two tiles in turn; the next tile's is on its way while one is worked on: a
             // word each of lse2, the target's product, its g and the target per lane.
-            float* row_smem = reinterpret_cast<float*>(epi_smem + EPI_WARPS * (2 * STAGING_BYTES + COLUMN_BYTES) + mine * ROW_BYTES);
+            constexpr uint32_t MINE = epi_bytes(EPI) - 2 * STAGING_BYTES - COLUMN_BYTES, TURN = ENTRIES ? ROW_WORDS_ENTRIES : 128;
+            float* row_smem = reinterpret_cast<float*>(epi_smem + EPI_WARPS * (2 * STAGING_BYTES + COLUMN_BYTES) + mine * MINE);
+            const uint32_t* half_smem = reinterpret_cast<const uint32_t*>(row_smem + 2 * ROW_WORDS_ENTRIES);   // ENTRIES
             const auto fetch = [&](uint32_t turn) {
                 const uint32_t row = work.m * BM + rank * 128 + quarter * 32 + lane;
                 const bool in = row < M;
-                float* to = row_smem + turn * 128 + lane;
+                float* to = row_smem + turn * TURN + lane;
                 copy_word(to, p.lse2 + (in ? row : 0), in);
                 if (ENTRIES) {
                     if (TWO) copy_word(to + 32, p.second_lse2 + (in ? row : 0), in);
@@ -803,14 +826,18 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             while (more) {
                 const uint32_t n0 = work.n * BN + group * 64, m0 = work.m * BM + rank * 128 + quarter * 32;
                 const uint32_t* list = nullptr;
-                uint32_t n_upper = 0, n_entries = 0, held[2];   // held: the first of either half
+                uint32_t n_half[2] = {0, 0};
                 if (ENTRIES) {
                     list = entries.list(p, m0);
-                    n_upper = entries.middle - entries.first;
-                    n_entries = entries.end - entries.first;
-                    held[0] = lane < n_upper ? list[lane] : NO_ENTRY;
-                    held[1] = n_upper + lane < n_entries ? list[n_upper + lane] : NO_ENTRY;
+                    n_half[0] = entries.middle - entries.first;
+                    n_half[1] = entries.end - entries.middle;
                 }
+                // ENTRIES: the entries of a half on their way to shared memory, while its logits are worked on
+                const auto bring = [&](int h) {
+                    const uint32_t n = min(h ? n_half[1] : n_half[0], HALF_ENTRIES);
+                    const uint32_t* from = list + (h ? n_half[0] : 0u);
+                    for (uint32_t i = lane; i < n; i += 32) copy_word(half_smem + i, from + i, true);
+                };
                 if (work.n != n_now) {
                     leave();
                     n_now = work.n;
@@ -821,7 +848,8 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncwarp();
-                const float* rows = row_smem + turn * 128;
+                if (ENTRIES) bring(0);   // (all have been put that lay there)
+                const float* rows = row_smem + turn * TURN;
                 turn ^= 1;
                 const uint32_t first = p.n_first + n0;
                 const bool any = !ENTRIES && __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
@@ -844,10 +872,12 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t row = h * 16 + i * 8 + r0;
-                        const float lse = m0 + row < M ? -rows[row] : -INFINITY;
+                        const float lse = m0 + row < M ? -rows[row] / SECOND : -INFINITY;
                         l[i] = two(lse, lse);
                         if (TWO) {
-                            const float lse2 = m0 + row < M ? -rows[32 + row] : -INFINITY;
+                            float lse2 = m0 + row < M ? -rows[32 + row] : -INFINITY;
+                            // squarings: with v = exp of the logit less the first sum's, g = v^SECOND + v * exp(that sum less the second's)
+                            if (SQUARINGS > 0) lse2 = m0 + row < M ? exp2_fast(lse2 - lse) : 0.0f;
                             l2[i] = two(lse2, lse2);
                         }
                         if (decltype(targets)::value)
@@ -874,7 +904,12 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                                 const uint64_t z = fma2(a, s, b);
                                 const float2 e = of_two(add2(z, l[i]));
                                 uint64_t g = two(exp2_fast(e.x), exp2_fast(e.y));
-                                if (TWO) {
+                                if constexpr (SQUARINGS > 0) {
+                                    const uint64_t v = g;
+#pragma unroll
+                                    for (int t = 0; t < SQUARINGS; ++t) g = mul2(g, g);
+                                    g = fma2(v, l2[i], g);
+                                } else if (TWO) {
                                     const float2 e2 = of_two(fma2(z, two(p.second_factor, p.second_factor), l2[i]));
                                     g = add2(g, two(exp2_fast(e2.x), exp2_fast(e2.y)));
                                 }
@@ -895,6 +930,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         store_blocks(to + (((j + block_piece) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
                     }
                     if constexpr (ENTRIES) {
+                        asm volatile("cp.async.wait_all;" ::: "memory");
                         __syncwarp();
                         const auto put = [&](uint32_t, uint32_t bits) {
                             if (bits & ENTRY_DEAD) return;
@@ -902,8 +938,11 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             *reinterpret_cast<uint16_t*>(staging + h * STAGING_BYTES + row * 128 + ((column / 8 ^ (row & 7)) << 4) + column % 8 * 2) =
                                 (uint16_t)(bits >> 16);
                         };
-                        put(0, h ? held[1] : held[0]);
-                        more_entries<8>(list, (h ? n_upper : 0u) + 32, h ? n_entries : n_upper, lane, put);
+                        const uint32_t n = h ? n_half[1] : n_half[0];
+                        for (uint32_t i = lane; i < min(n, HALF_ENTRIES); i += 32) put(i, half_smem[i]);
+                        more_entries<8>(list + (h ? n_half[0] : 0u), HALF_ENTRIES, n, lane, put);
+                        __syncwarp();
+                        if (h == 0) bring(1);
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
