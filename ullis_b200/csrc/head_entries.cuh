@@ -256,35 +256,62 @@ entries_rows_kernel(const EntryRows o) {
         for (uint32_t i = lane; i < 2 * GROUP_COLUMNS; i += 32) sums[warp][0][i] = 0.0f;
         __syncwarp();
         const uint32_t end = min((stretch + 1) * o.stretch, (rows + BLOCK_ROWS - 1) / BLOCK_ROWS);
-        for (uint32_t b = stretch * o.stretch + warp; b < end; b += ROWS_WARPS) {
-            const uint16_t* at = o.lists.offsets + (size_t)b * o.lists.groups1 + 2 * group;
-            const uint32_t last = at[2];
-            for (uint32_t i0 = at[0]; i0 < last; i0 += 32) {
-                const uint32_t i = i0 + lane;
-                const bool in = i < last;
-                const uint32_t run = in ? (o.lists.bits[b * block_entries + i] & (pg::ENTRY_PLACES - 1)) >> 4 : 0xFFFFFFFFu;   // half, column
-                const float w = in ? -o.lists.weight[b * block_entries + i] : 0.0f;
-                float g = w, ga = w != 0.0f ? w * o.logits[b * block_entries + i].x : 0.0f;
+        // block by block, 32 entries at a time, the next of them on their way
+        uint32_t block = stretch * o.stretch + warp, at = 0, last = 0;
+        struct {
+            uint32_t run;
+            float w, product;
+            bool in;
+        } now, next;
+        const auto open = [&]() {   // the next block that has any
+            while (at >= last && block < end) {
+                const uint16_t* offsets = o.lists.offsets + (size_t)block * o.lists.groups1 + 2 * group;
+                at = offsets[0];
+                last = offsets[2];
+                if (at < last) break;
+                block += ROWS_WARPS;
+            }
+        };
+        const auto fetch = [&]() {
+            next.in = false;
+            if (block >= end) return false;
+            next.in = at + lane < last;
+            const size_t i = block * block_entries + at + lane;
+            next.run = next.in ? (o.lists.bits[i] & (pg::ENTRY_PLACES - 1)) >> 4 : 0xFFFFFFFFu;   // half, column
+            next.w = next.in ? -o.lists.weight[i] : 0.0f;
+            next.product = next.in ? o.logits[i].x : 0.0f;
+            at += 32;
+            if (at >= last) {
+                block += ROWS_WARPS;
+                open();
+            }
+            return true;
+        };
+        open();
+        bool more = fetch();
+        while (more) {
+            now = next;
+            more = fetch();
+            float g = now.w, ga = now.w != 0.0f ? now.w * now.product : 0.0f;
 #pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const uint32_t other = __shfl_up_sync(0xffffffffu, run, d);
-                    if (!__any_sync(0xffffffffu, in && (int)lane >= d && other == run)) break;   // (nor further apart)
-                    const float u = __shfl_up_sync(0xffffffffu, g, d), v = __shfl_up_sync(0xffffffffu, ga, d);
-                    if ((int)lane >= d && other == run) {
-                        g += u;
-                        ga += v;
-                    }
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t other = __shfl_up_sync(0xffffffffu, now.run, d);
+                if (!__any_sync(0xffffffffu, now.in && (int)lane >= d && other == now.run)) break;   // (nor further apart)
+                const float u = __shfl_up_sync(0xffffffffu, g, d), v = __shfl_up_sync(0xffffffffu, ga, d);
+                if ((int)lane >= d && other == now.run) {
+                    g += u;
+                    ga += v;
                 }
-                const uint32_t next = __shfl_down_sync(0xffffffffu, run, 1);
-                const bool ends = in && (lane == 31 || next != run);
+            }
+            const uint32_t right = __shfl_down_sync(0xffffffffu, now.run, 1);
+            const bool ends = now.in && (lane == 31 || right != now.run);
 #pragma unroll
-                for (uint32_t half = 0; half < 2; ++half) {   // (a column may end a run of either)
-                    if (ends && run >> 6 == half) {
-                        sums[warp][0][run & 63u] += g;
-                        sums[warp][1][run & 63u] += ga;
-                    }
-                    __syncwarp();
+            for (uint32_t half = 0; half < 2; ++half) {   // (a column may end a run of either)
+                if (ends && now.run >> 6 == half) {
+                    sums[warp][0][now.run & 63u] += g;
+                    sums[warp][1][now.run & 63u] += ga;
                 }
+                __syncwarp();
             }
         }
         __syncthreads();
