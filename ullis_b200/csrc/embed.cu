@@ -148,6 +148,9 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
     __shared__ uint32_t found_token[FEW], found_row[FEW], token_at[FEW], row_at[FEW], warp_counts[THREADS / 32];
     __shared__ float sums[THREADS][N + 1];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t tokens_here[FEW / THREADS];   // on their way beside the zeros
+#pragma unroll
+    for (uint32_t k = 0; k < FEW / THREADS; ++k) tokens_here[k] = k * THREADS + threadIdx.x < rows ? tokens[k * THREADS + threadIdx.x] : ignore_id;
     const size_t first = (size_t)blockIdx.x * C, step = (size_t)gridDim.x * C;
     if (C % 4 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0) {
         for (size_t at = first; at < (size_t)vocab * C; at += step)
@@ -157,8 +160,10 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
             for (uint32_t c = threadIdx.x; c < C; c += THREADS) g[at + c] = 0.0f;
     }
     uint32_t count = 0;
-    for (uint32_t base = 0; base < rows; base += THREADS) {   // (in the order of the rows)
-        const uint32_t r = base + threadIdx.x, token = r < rows ? tokens[r] : ignore_id;
+#pragma unroll
+    for (uint32_t k = 0; k < FEW / THREADS; ++k) {   // (in the order of the rows)
+        const uint32_t r = k * THREADS + threadIdx.x, token = tokens_here[k];
+        if (k * THREADS >= rows) break;
         const bool mine = token != ignore_id && token < vocab && token % gridDim.x == blockIdx.x;
         const uint32_t mask = __ballot_sync(0xffffffffu, mine);
         if (lane == 0) warp_counts[warp] = __popc(mask);

@@ -144,6 +144,11 @@ class DeviceOps:
 
     def _ids(self, t, name):
         """int32 without gaps, of any shape."""
+        try:
+            if t.dtype in _I32 and self._on_device(t) and t.is_contiguous():
+                return
+        except AttributeError:
+            pass
         self._refuse(t, name, _I32)
         if not t.is_contiguous():
             raise UllisCudaError(ERR_SHAPE, f"{name} must be contiguous")
@@ -158,12 +163,6 @@ class DeviceOps:
         if t.numel() != n:
             _shape_error(name, t.shape, (n,))
         raise UllisCudaError(ERR_SHAPE, f"{name} must be contiguous")
-
-    def _table(self, table):
-        vocab, channels, stride = self._matrix(table, "table", _DTYPES)
-        if table.dim() != 2:
-            raise UllisCudaError(ERR_SHAPE, "table must have two dimensions")
-        return vocab, channels, stride
 
     def _tape(self, tape):
         _torch()
@@ -195,7 +194,7 @@ class DeviceOps:
             if len(known) >= 4096:
                 known.clear()
             known[name, sizes] = need
-        return _TORCH.empty(need, dtype=_TORCH.uint8, device=like.device), need
+        return _TORCH.empty(need, dtype=_TORCH.uint8, device=like.device) if need else None, need
 
     # ------------------------------------------------------------------------------------------ the 8-bit tape
     def tape_pack(self, x) -> Tape:
@@ -252,7 +251,7 @@ class DeviceOps:
         self._check(self._lib.ullis_cuda_tape_layer_norm_backward(
             self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], codes.data_ptr(), exponents.data_ptr(), gy.data_ptr(), stride,
             weight.data_ptr(), past, past_stride, rows, channels, gx.data_ptr(), g_weight.data_ptr(),
-            g_bias.data_ptr(), work.data_ptr(), size))
+            g_bias.data_ptr(), _p(work), size))
         return gx, g_weight, g_bias
 
     def tape_weight_grad(self, tape, gy):
@@ -266,7 +265,7 @@ class DeviceOps:
         work, size = self._workspace(gy, "tape_weight_grad", rows, channels, out)
         self._check(self._lib.ullis_cuda_tape_weight_grad(
             self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], codes.data_ptr(), exponents.data_ptr(), gy.data_ptr(), stride, rows,
-            channels, out, g.data_ptr(), work.data_ptr(), size))
+            channels, out, g.data_ptr(), _p(work), size))
         return g
 
     # ------------------------------------------------------------------------------------------ embedding
@@ -276,13 +275,15 @@ class DeviceOps:
         table [vocab, channels] float32, float16 or bfloat16; tokens int32 of any shape (a negative id and `ignore_id` are taken as
         the unsigned 32-bit number they are).  The row of `ignore_id` is zero, that of any other id outside the table NaN."""
         torch = _torch()
-        vocab, channels, stride = self._table(table)
+        vocab, channels, stride = self._matrix(table, "table", _DTYPES)
+        if table.dim() != 2:
+            raise UllisCudaError(ERR_SHAPE, "table must have two dimensions")
         self._ids(tokens, "tokens")
         dtype = table.dtype if dtype is None else dtype
         if dtype not in _DTYPES:
             raise UllisCudaError(ERR_ARG, f"an embedding has no type {dtype}")
         ignore = _id32(ignore_id)
-        y = torch.empty(*tokens.shape, channels, dtype=dtype, device=tokens.device)
+        y = torch.empty(*tokens.shape, channels, dtype=dtype, device=table.device)
         self._check(self._lib.ullis_cuda_embed(
             self._h, _RAW_STREAM(self.device), _DTYPES[table.dtype], table.data_ptr(), stride, tokens.data_ptr(), ignore, float(scale),
             tokens.numel(), channels, vocab, _DTYPES[dtype], y.data_ptr()))
@@ -303,7 +304,7 @@ class DeviceOps:
         work, size = self._workspace(gy, "embed_grad", _DTYPES[gy.dtype], rows, channels, vocab)
         self._check(self._lib.ullis_cuda_embed_grad(
             self._h, _RAW_STREAM(self.device), _DTYPES[gy.dtype], tokens.data_ptr(), ignore, gy.data_ptr(), stride, rows,
-            channels, vocab, float(scale), g.data_ptr(), work.data_ptr(), size))
+            channels, vocab, float(scale), g.data_ptr(), _p(work), size))
         return g
 
     # ------------------------------------------------------------------------------------------ a teacher's logits
@@ -315,9 +316,9 @@ class DeviceOps:
         k = int(k)
         if not 0 < k <= min(vocab, 256):
             raise UllisCudaError(ERR_SHAPE, f"top logits: k must be at least 1 and at most {min(vocab, 256)}")
-        shape = (*logits.shape[:-1], k)
-        ids = torch.empty(shape, dtype=torch.int32, device=logits.device)
-        top = torch.empty(shape, dtype=logits.dtype, device=logits.device)
+        lead, device = logits.shape[:-1], logits.device
+        ids = torch.empty(*lead, k, dtype=torch.int32, device=device)
+        top = torch.empty(*lead, k, dtype=logits.dtype, device=device)
         self._check(self._lib.ullis_cuda_top_logits(self._h, _RAW_STREAM(self.device), _DTYPES[logits.dtype], logits.data_ptr(), stride,
                                                     rows, vocab, k, ids.data_ptr(), top.data_ptr()))
         return TopLogits(ids, top)
@@ -344,7 +345,7 @@ class DeviceOps:
         self._check(self._lib.ullis_cuda_head_ce_grad(
             self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], hidden.data_ptr(), stride, at if scale is not None else None,
             at if scale is None else None, _p(scale), _p(bias), labels.data_ptr(), ignore, rows, time, channels, vocab,
-            float(loss_scale), *(_p(t) for t in outputs), work.data_ptr(), size))
+            float(loss_scale), *(_p(t) for t in outputs), _p(work), size))
         return outputs
 
     def head_distill_grad(self, hidden, weight, top_ids, top_logits, *, scale=None, bias=None, labels=None, alpha: float = 1.0,
@@ -364,17 +365,15 @@ class DeviceOps:
         rows, channels, stride = self._matrix(hidden, "hidden", _16)
         if labels is not None:
             self._vector(labels, "labels", _I32, rows)
-        self._refuse(top_ids, "top_ids", _I32)
-        self._refuse(top_logits, "top_logits", _DTYPES)
+        self._ids(top_ids, "top_ids")
         top = top_ids.shape[-1] if top_ids.dim() else 0
         if not 0 < top <= 256:
             raise UllisCudaError(ERR_SHAPE, "head distillation takes 1 to 256 entries of a row")
-        if top_ids.shape != top_logits.shape:
-            _shape_error("top_logits", top_logits.shape, top_ids.shape)
         if top_ids.numel() != rows * top:
             _shape_error("top_ids", top_ids.shape, (rows, top))
-        if not (top_ids.is_contiguous() and top_logits.is_contiguous()):
-            raise UllisCudaError(ERR_SHAPE, "top_ids and top_logits must be contiguous")
+        self._vector(top_logits, "top_logits", _DTYPES, rows * top)
+        if top_logits.shape != top_ids.shape:
+            _shape_error("top_logits", top_logits.shape, top_ids.shape)
         alpha, temperature = float(alpha), float(temperature)
         if not 0.0 <= alpha <= 1.0 or not 1 / 128 <= temperature <= 128:
             raise UllisCudaError(ERR_ARG, "alpha must be in 0 .. 1, temperature in 1/128 .. 128")
@@ -387,7 +386,7 @@ class DeviceOps:
             self._h, _RAW_STREAM(self.device), _DTYPES[hidden.dtype], hidden.data_ptr(), stride, at if scale is not None else None,
             at if scale is None else None, _p(scale), _p(bias), top_ids.data_ptr(), _DTYPES[top_logits.dtype], top_logits.data_ptr(), top,
             alpha, temperature, _p(labels), ignore, rows, time, channels, vocab, float(loss_scale), *(_p(t) for t in outputs),
-            work.data_ptr(), size))
+            _p(work), size))
         return outputs
 
     def _time(self, hidden, rows, time) -> int:
