@@ -6,8 +6,13 @@
 // the chunks that hold something as large go into a queue, and 32 of them at a time are looked at element by element, a lane each, so that
 // the rare ones cost a warp no more than they are.  Keys that are not below the bound are kept in shared memory.
 // The bound begins as the k-th largest maximum of the first 512 chunks (k of them hold something as large) and rises whenever
-// the buffer is full: bits of the new bound are found from the top by counting.  Where there are few rows several warps share one and
-// the first of them goes through what the others have kept.
+// the buffer is full: bits of the new bound are found from the top by counting.  Where there are few rows several warps share one; the least
+// of the bounds that each finds for its share of the k holds for all of them, and the first goes through what the others have kept.
+//
+// Bound by memory on long rows and by instructions on short ones: 4096 x 131072 bf16, k = 64 195 us (1.07 GB, 5.5 TB/s); 16384 x 8192 f32 132 us
+// (537 MB, 4.1 TB/s; 5000 warp instructions to a row, of which the reading takes 800: the first bound 600, the queue's chunks 1000, raising and
+// sorting 1600).  Tried and slower there: tiles of 2 or 8 chunks (155, 127 but 220 on the long rows), a sample of 8 or 32 (139), a buffer of
+// 384 keys (149), the next tiles prefetched into L2 (127, long rows 214).  k = 128 and 256 keep two and four times as much: 250, 476 us.
 #include <algorithm>
 
 #include "block_sort.cuh"
@@ -18,7 +23,7 @@ namespace ullis {
 namespace dev {
 namespace {
 
-constexpr uint32_t MOST_WARPS = 8, TILE = 4, SAMPLE = 16;   // chunks per lane: of a tile; looked at for the first bound
+constexpr uint32_t MOST_WARPS = 16, TILE = 4, SAMPLE = 16;   // chunks per lane: of a tile; looked at for the first bound
 constexpr uint32_t FULL = 0xffffffffu;
 
 size_t ceil_div(size_t n, size_t by) { return (n + by - 1) / by; }
@@ -121,7 +126,7 @@ struct Best {
 struct Top {
     const void* logits;
     size_t stride;
-    uint32_t rows, vocab, k, warps;   // warps to a row: 1, 2, 4 or 8
+    uint32_t rows, vocab, k, warps;   // warps to a row: 1, 2, 4, 8 or 16
     int32_t* ids;
     void* out;
 };
@@ -172,7 +177,7 @@ struct Most<__nv_bfloat16> {
 constexpr uint32_t QUEUE = 64;   // chunk numbers of a warp
 
 template <typename T, uint32_t CAP>
-__global__ void __launch_bounds__(MOST_WARPS * 32, CAP <= 256 ? 4 : 2)
+__global__ void __launch_bounds__(MOST_WARPS * 32, CAP <= 256 ? 2 : 1)
 top_kernel(const Top o) {
     chain_entry();
     constexpr int N = tape::CHUNK<T>, E = CAP / 128;   // E: keys to a lane when they are sorted
@@ -181,121 +186,126 @@ top_kernel(const Top o) {
     uint64_t* all_keys = reinterpret_cast<uint64_t*>(smem_raw);   // [warp][CAP]
     __shared__ uint32_t counts[MOST_WARPS], queues[MOST_WARPS][QUEUE];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % o.warps;
-    const size_t row = (size_t)blockIdx.x * (blockDim.x / 32 / o.warps) + warp / o.warps;
-    const bool live = row < o.rows;
+    const size_t mine = (size_t)blockIdx.x * (blockDim.x / 32 / o.warps) + warp / o.warps, row = min(mine, (size_t)o.rows - 1);   // (the last again)
     Best<CAP> best{all_keys + warp * CAP, o.k, lane};
-    if (live) {
-        const T* from = static_cast<const T*>(o.logits) + row * o.stride;
-        // chunks on 16 bytes; the first and the last may reach out of the row
-        const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(from) % 16) / sizeof(T), chunks = (o.vocab + off + N - 1) / N;
-        const uint32_t begin = (uint32_t)((uint64_t)chunks * part / o.warps), end = (uint32_t)((uint64_t)chunks * (part + 1) / o.warps);
-        const uint32_t first_whole = off ? 1 : 0, behind_whole = (o.vocab + off) / N;   // [..): chunks that lie in the row
-        const T* aligned = from - off;
-        const auto load = [&](uint32_t chunk) {
-            tape::Raw<T> raw;
-            if (chunk >= first_whole && chunk < behind_whole && chunk < end) {
-                raw.q = *reinterpret_cast<const uint4*>(aligned + (size_t)chunk * N);
-            } else {
-                T* t = reinterpret_cast<T*>(&raw.q);
+    const T* from = static_cast<const T*>(o.logits) + row * o.stride;
+    // chunks on 16 bytes; the first and the last may reach out of the row
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(from) % 16) / sizeof(T), chunks = (o.vocab + off + N - 1) / N;
+    const uint32_t begin = (uint32_t)((uint64_t)chunks * part / o.warps), end = (uint32_t)((uint64_t)chunks * (part + 1) / o.warps);
+    const uint32_t first_whole = off ? 1 : 0, behind_whole = (o.vocab + off) / N;   // [..): chunks that lie in the row
+    const T* aligned = from - off;
+    const auto load = [&](uint32_t chunk) {
+        tape::Raw<T> raw;
+        if (chunk >= first_whole && chunk < behind_whole && chunk < end) {
+            raw.q = *reinterpret_cast<const uint4*>(aligned + (size_t)chunk * N);
+        } else {
+            T* t = reinterpret_cast<T*>(&raw.q);
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const uint32_t column = chunk * N + e - off;   // (above the row's length where it lies before the row)
-                    t[e] = chunk < end && column < o.vocab ? from[column] : tape::from_float<T>(-INFINITY);
-                }
-            }
-            return raw;
-        };
-        uint32_t* queue = queues[warp];
-        uint32_t queued = 0;
-        auto bound = Most<T>::bound(best.least);
-        // The first of the queue, up to 32, element by element.
-        const auto look = [&]() {
-            __syncwarp();
-            const uint32_t n = min(queued, 32u), chunk = lane < n ? queue[lane] : 0u;
-            const uint32_t left = lane + 32 < queued ? queue[lane + 32] : 0u;
-            const tape::Raw<T> raw = load(chunk);
-            float v[N];
-            raw.unpack(v);
-            uint32_t pass = 0;
-#pragma unroll
-            for (int e = 0; e < N; ++e) pass |= (uint32_t)(lane < n && chunk * N + e - off < o.vocab && !(v[e] < best.least)) << e;
-            while (__any_sync(FULL, pass != 0)) {
-                const uint32_t e = __ffs(pass) - 1;   // (of none: no element)
-                float value = v[0];
-#pragma unroll
-                for (uint32_t i = 1; i < N; ++i) value = e == i ? v[i] : value;
-                best.add(pass ? (uint64_t)order_of(value) << 32 | (0xFFFFFFFFu - (chunk * N + e - off)) : 0u);
-                pass &= pass - 1;
-            }
-            if (lane + 32 < queued) queue[lane] = left;
-            queued -= n;
-            bound = Most<T>::bound(best.least);
-        };
-        const uint32_t whole_end = min(end, behind_whole);
-        if (end - begin > o.k) {
-            // a first bound: bits from the top while k chunk maxima are not below it, until not many more are
-            uint32_t high[SAMPLE], largest = 0, smallest = FULL;
-#pragma unroll
-            for (uint32_t u = 0; u < SAMPLE; ++u) {
-                const uint32_t chunk = begin + u * 32 + lane;
-                high[u] = chunk >= first_whole && chunk < whole_end ? order_of(Most<T>(*reinterpret_cast<const uint4*>(aligned + (size_t)chunk * N)).value()) : 0u;
-                largest = max(largest, high[u]);
-                smallest = min(smallest, high[u]);
-            }
-            uint32_t bit, t = common(largest, smallest, &bit);
-            for (uint32_t left = FULL; bit >= 0x1000u && left > o.k + o.k / 8; bit >>= 1) {
-                uint32_t n = 0;
-#pragma unroll
-                for (uint32_t u = 0; u < SAMPLE; ++u) n += high[u] >= (t | bit);
-                n = __reduce_add_sync(FULL, n);
-                if (n >= o.k) {
-                    t |= bit;
-                    left = n;
-                }
-            }
-            if (t) {
-                best.set_bound((uint64_t)t << 32);
-                bound = Most<T>::bound(best.least);
+            for (int e = 0; e < N; ++e) {
+                const uint32_t column = chunk * N + e - off;   // (above the row's length where it lies before the row)
+                t[e] = chunk < end && column < o.vocab ? from[column] : tape::from_float<T>(-INFINITY);
             }
         }
-        for (uint32_t tile = begin; tile < end; tile += TILE * 32) {
-            tape::Raw<T> raw[TILE];
-            if (tile >= first_whole && tile + TILE * 32 <= whole_end) {
-                const T* at = aligned + (size_t)(tile + lane) * N;
+        return raw;
+    };
+    uint32_t* queue = queues[warp];
+    uint32_t queued = 0;
+    auto bound = Most<T>::bound(best.least);
+    // The first of the queue, up to 32, element by element.
+    const auto look = [&]() {
+        __syncwarp();
+        const uint32_t n = min(queued, 32u), chunk = lane < n ? queue[lane] : 0u;
+        const uint32_t left = lane + 32 < queued ? queue[lane + 32] : 0u;
+        const tape::Raw<T> raw = load(chunk);
+        float v[N];
+        raw.unpack(v);
+        uint32_t pass = 0;
 #pragma unroll
-                for (uint32_t u = 0; u < TILE; ++u) raw[u].q = *reinterpret_cast<const uint4*>(at + u * 32 * N);
-            } else {
+        for (int e = 0; e < N; ++e) pass |= (uint32_t)(lane < n && chunk * N + e - off < o.vocab && !(v[e] < best.least)) << e;
+        while (__any_sync(FULL, pass != 0)) {
+            const uint32_t e = __ffs(pass) - 1;   // (of none: no element)
+            float value = v[0];
 #pragma unroll
-                for (uint32_t u = 0; u < TILE; ++u) raw[u] = load(tile + u * 32 + lane);
-            }
-            uint32_t pass = 0;   // a bit per chunk
+            for (uint32_t i = 1; i < N; ++i) value = e == i ? v[i] : value;
+            best.add(pass ? (uint64_t)order_of(value) << 32 | (0xFFFFFFFFu - (chunk * N + e - off)) : 0u);
+            pass &= pass - 1;
+        }
+        if (lane + 32 < queued) queue[lane] = left;
+        queued -= n;
+        bound = Most<T>::bound(best.least);
+    };
+    const uint32_t whole_end = min(end, behind_whole);
+    // A first bound: bits from the top while `need` chunk maxima are not below it, until not many more are.  Of several warps each looks
+    // for its share of the k, and no bound is above the least of theirs.
+    const uint32_t need = (o.k + o.warps - 1) / o.warps;
+    uint32_t t = 0;
+    if (end - begin > need) {
+        uint32_t high[SAMPLE], largest = 0, smallest = FULL;
 #pragma unroll
-            for (uint32_t u = 0; u < TILE; ++u) pass |= (uint32_t)Most<T>(raw[u].q).reaches(bound) << u;
-            for (;;) {   // (a round for each of the most that a lane has: in the middle of a long row none or one)
-                const uint32_t mask = __ballot_sync(FULL, pass != 0);
-                if (!mask) break;
-                if (pass) queue[queued + __popc(mask & ((1u << lane) - 1u))] = tile + (__ffs(pass) - 1) * 32 + lane;
-                pass &= pass - 1;
-                queued += __popc(mask);
-                if (queued >= 32) look();
+        for (uint32_t u = 0; u < SAMPLE; ++u) {
+            const uint32_t chunk = begin + u * 32 + lane;
+            high[u] = chunk >= first_whole && chunk < whole_end ? order_of(Most<T>(*reinterpret_cast<const uint4*>(aligned + (size_t)chunk * N)).value()) : 0u;
+            largest = max(largest, high[u]);
+            smallest = min(smallest, high[u]);
+        }
+        uint32_t bit;
+        t = common(largest, smallest, &bit);
+        for (uint32_t left = FULL; bit >= 0x1000u && left > need + need / 8; bit >>= 1) {
+            uint32_t n = 0;
+#pragma unroll
+            for (uint32_t u = 0; u < SAMPLE; ++u) n += high[u] >= (t | bit);
+            n = __reduce_add_sync(FULL, n);
+            if (n >= need) {
+                t |= bit;
+                left = n;
             }
         }
-        while (queued) look();
-        best.keep(max(o.k, LEFT));
     }
+    if (o.warps > 1) {
+        if (lane == 0) counts[warp] = t;
+        __syncthreads();
+        for (uint32_t w = 0; w < o.warps; ++w) t = min(t, counts[warp - part + w]);
+        __syncthreads();
+    }
+    if (t) {
+        best.set_bound((uint64_t)t << 32);
+        bound = Most<T>::bound(best.least);
+    }
+    for (uint32_t tile = begin; tile < end; tile += TILE * 32) {
+        tape::Raw<T> raw[TILE];
+        if (tile >= first_whole && tile + TILE * 32 <= whole_end) {
+            const T* at = aligned + (size_t)(tile + lane) * N;
+#pragma unroll
+            for (uint32_t u = 0; u < TILE; ++u) raw[u].q = *reinterpret_cast<const uint4*>(at + u * 32 * N);
+        } else {
+#pragma unroll
+            for (uint32_t u = 0; u < TILE; ++u) raw[u] = load(tile + u * 32 + lane);
+        }
+        uint32_t pass = 0;   // a bit per chunk
+#pragma unroll
+        for (uint32_t u = 0; u < TILE; ++u) pass |= (uint32_t)Most<T>(raw[u].q).reaches(bound) << u;
+        for (;;) {   // (a round for each of the most that a lane has: in the middle of a long row none or one)
+            const uint32_t mask = __ballot_sync(FULL, pass != 0);
+            if (!mask) break;
+            if (pass) queue[queued + __popc(mask & ((1u << lane) - 1u))] = tile + (__ffs(pass) - 1) * 32 + lane;
+            pass &= pass - 1;
+            queued += __popc(mask);
+            if (queued >= 32) look();
+        }
+    }
+    while (queued) look();
+    best.keep(max(o.k, LEFT));
     if (o.warps > 1) {
         if (lane == 0) counts[warp] = best.count;
         __syncthreads();
         if (part) return;
-        if (live) {
-            for (uint32_t w = 1; w < o.warps; ++w) {
-                const uint32_t n = counts[warp + w];
-                for (uint32_t i = 0; i < n; i += 32) best.add(i + lane < n ? all_keys[(warp + w) * CAP + i + lane] : 0u);
-            }
-            best.keep(max(o.k, LEFT));
+        for (uint32_t w = 1; w < o.warps; ++w) {
+            const uint32_t n = counts[warp + w];
+            for (uint32_t i = 0; i < n; i += 32) best.add(i + lane < n ? all_keys[(warp + w) * CAP + i + lane] : 0u);
         }
+        best.keep(max(o.k, LEFT));
     }
-    if (!live) return;
+    if (mine >= o.rows) return;
     // in falling order: the complements in rising order
     uint64_t v[E];
     __syncwarp();
@@ -336,10 +346,11 @@ void top_logits(const Stream& s, int dtype, Rows logits, size_t rows, size_t voc
     o.k = (uint32_t)k;
     o.ids = ids;
     o.out = out;
-    // warps enough for every SM, of whole tiles each
+    // Warps enough for every SM, of four tiles each at least.  us with up to 8 / 16: 1 x 131072 f32, k = 64 28.6 / 22.0, k = 256 51 / 38;
+    // 32 x 131072 bf16 32 / 26.
     const size_t tiles = ceil_div(vocab * size_of(dtype), TILE * 32 * 16);
     o.warps = 1;
-    while (o.warps < MOST_WARPS && rows * o.warps < (size_t)s.rt->sm_count * 16 && tiles >= 2 * o.warps) o.warps *= 2;
+    while (o.warps < MOST_WARPS && rows * o.warps < (size_t)s.rt->sm_count * 16 && tiles >= 4 * o.warps) o.warps *= 2;
     if (dtype == F32) launch_by_k<float>(s, o);
     else if (dtype == F16) launch_by_k<__half>(s, o);
     else launch_by_k<__nv_bfloat16>(s, o);
