@@ -214,3 +214,80 @@ def test_the_gradient_is_that_of_the_lookup(cuda_rt):
     # embed's outputs and table + h are rounded to f32, the sums of the gradient too
     sizes = (gy.double().abs() * (both[0].abs() + both[1].abs())).sum() + 2008 * (gy.double().abs() * 3.0 * h.double().abs()[tokens.long()]).sum()
     assert abs(left - right) <= 4 * U * sizes
+
+
+@pytest.mark.parametrize("rows,vocab,kind", [(140_000, 3000, "words"), (300_001, 50, "even"), (300_001, 200_000, "words"), (131_073, 7, "same")])
+def test_gradient_of_many_chunks(cuda_rt, rows, vocab, kind):
+    """Rows in more chunks than a CTA holds the samples of at once, tokens with tens of thousands of rows."""
+    g = torch.Generator("cuda").manual_seed(rows)
+    tokens = draw_tokens(rows, vocab, kind, g)
+    tokens[::1001] = IGNORED
+    gy = torch.randn(rows, 12, generator=g, device="cuda").bfloat16()
+    check_grad(cuda_rt.embed_grad(tokens, gy, vocab), tokens, gy, vocab)
+
+
+def test_past_32_bits_of_elements(cuda_rt):
+    """Tables, gradients and rows beyond 2^32 elements."""
+    vocab, d = 8_400_000, 512                                  # 4.3e9
+    table = torch.zeros(vocab, d, dtype=torch.float16, device="cuda")
+    at = torch.tensor([0, 1, 4_194_304, 8_388_607, 8_388_608, vocab - 1], device="cuda")
+    table[at] = (torch.arange(6, device="cuda")[:, None] + 1 + torch.arange(d, device="cuda") / 1024).half()
+    tokens = at.repeat(300).to(torch.int32)                    # 1800 rows: sorted; 6: few
+    for t in (tokens, tokens[:6]):
+        assert torch.equal(cuda_rt.embed(table, t), table[t.long()])
+        gy = torch.ones(t.numel(), d, device="cuda").half()
+        g = cuda_rt.embed_grad(t, gy, vocab)
+        assert (g[at] == t.numel() // 6).all() and float(g.sum(dtype=torch.float64)) == t.numel() * d
+        del g
+    del table
+    rows = vocab                                               # gy beyond 2^32
+    gy = torch.zeros(rows, d, dtype=torch.float16, device="cuda")
+    gy[at] = 1.0
+    tokens = (torch.arange(rows, device="cuda") % 1000).to(torch.int32)
+    g = cuda_rt.embed_grad(tokens, gy, 1000)
+    want = torch.zeros(1000, device="cuda").index_add_(0, at % 1000, torch.ones(6, device="cuda"))
+    assert torch.equal(g, want[:, None].expand(1000, d))
+    y = cuda_rt.embed(torch.arange(1000, device="cuda")[:, None].expand(1000, d).half().contiguous(), tokens)
+    assert (y[at, 7] == (at % 1000).half()).all() and float(y[-1].float().sum()) == ((rows - 1) % 1000) * d   # (in f32: FP16 has no 511 488)
+
+
+def test_the_library_refuses(cuda_rt):
+    """Statuses of the entry points themselves; nothing is written."""
+    import ctypes as C
+    lib, h, stream = cuda_rt._lib, cuda_rt._h, torch.cuda.current_stream().cuda_stream
+    t = torch.zeros(8, 16, device="cuda")
+    tok = torch.zeros(2000, dtype=torch.int32, device="cuda")
+    gy, out = torch.zeros(2000, 16, device="cuda"), torch.full((2000, 16), 77.0, device="cuda")
+
+    def embed(dtype=0, table=t.data_ptr(), stride=16, tokens=tok.data_ptr(), scale=1.0, rows=8, c=16, vocab=8, out_dtype=0, y=out.data_ptr()):
+        return lib.ullis_cuda_embed(h, stream, dtype, table, stride, tokens, 0xFFFFFFFF, scale, rows, c, vocab, out_dtype, y)
+
+    assert embed() == cuda.OK
+    out.fill_(77.0)
+    for bad in (dict(dtype=3), dict(out_dtype=-1), dict(scale=float("nan")), dict(table=None), dict(tokens=None), dict(y=None),
+                dict(tokens=tok.data_ptr() + 2), dict(table=t.data_ptr() + 1)):
+        assert embed(**bad) == cuda.ERR_ARG, bad
+    for bad in (dict(stride=15), dict(c=0), dict(vocab=0), dict(rows=1 << 31), dict(c=1 << 24, stride=1 << 24), dict(vocab=1 << 31)):
+        assert embed(**bad) == cuda.ERR_SHAPE, bad
+    assert lib.ullis_cuda_embed(None, stream, 0, t.data_ptr(), 16, tok.data_ptr(), 0, 1.0, 8, 16, 8, 0, out.data_ptr()) == cuda.ERR_ARG
+    need = C.c_size_t(0)
+    assert lib.ullis_cuda_embed_grad_workspace(h, 0, 2000, 16, 8, C.byref(need)) == cuda.OK
+    work = torch.zeros(need.value + 256, dtype=torch.uint8, device="cuda")
+
+    def grad(dtype=0, tokens=tok.data_ptr(), x=gy.data_ptr(), stride=16, rows=2000, c=16, vocab=8, scale=1.0, g=out.data_ptr(), w=work.data_ptr(),
+             size=need.value):
+        return lib.ullis_cuda_embed_grad(h, stream, dtype, tokens, 0xFFFFFFFF, x, stride, rows, c, vocab, scale, g, w, size)
+
+    for bad in (dict(dtype=9), dict(scale=float("inf")), dict(tokens=None), dict(x=None), dict(g=None), dict(w=None), dict(w=work.data_ptr() + 4),
+                dict(g=out.data_ptr() + 2)):
+        assert grad(**bad) == cuda.ERR_ARG, bad
+    for bad in (dict(stride=8), dict(size=need.value - 1), dict(vocab=0), dict(c=0)):
+        assert grad(**bad) == cuda.ERR_SHAPE, bad
+    torch.cuda.synchronize()
+    assert (out == 77).all()
+    assert grad() == cuda.OK
+    ids, top = torch.zeros(8, 300, dtype=torch.int32, device="cuda"), torch.zeros(8, 300, device="cuda")
+    for k, vocab, stride, code in ((0, 16, 16, cuda.ERR_SHAPE), (17, 16, 16, cuda.ERR_SHAPE), (257, 1000, 1000, cuda.ERR_SHAPE), (4, 16, 15, cuda.ERR_SHAPE),
+                                   (4, 16, 16, cuda.OK)):
+        assert lib.ullis_cuda_top_logits(h, stream, 0, t.data_ptr(), stride, 8, vocab, k, ids.data_ptr(), top.data_ptr()) == code
+    assert lib.ullis_cuda_top_logits(h, stream, 0, t.data_ptr(), 16, 8, 16, 4, None, top.data_ptr()) == cuda.ERR_ARG

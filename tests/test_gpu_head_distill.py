@@ -397,3 +397,49 @@ def test_temperatures_that_are_squared(cuda_rt, temperature, dtype):
     for lean in (1.0, 8.0):
         s = student(700, 100, 96, 1500, dtype, True, 24, temperature=temperature, lean=lean, seed=11, absent=0.2)
         check(call(cuda_rt, s), formulas(s))
+
+
+def test_the_library_refuses(cuda_rt):
+    """Statuses of the entry point itself; nothing is written."""
+    import ctypes as C
+    s = student(40, 20, 64, 300, "f16", False, 8, seed=7)
+    need = C.c_size_t(0)
+    lib, h = cuda_rt._lib, cuda_rt._h
+    for top, code in ((0, cuda.ERR_SHAPE), (257, cuda.ERR_SHAPE), (8, cuda.OK)):
+        assert lib.ullis_cuda_head_distill_grad_workspace(h, 40, 64, 300, top, 1, 0, C.byref(need)) == code
+    work = torch.zeros(need.value, dtype=torch.uint8, device="cuda")
+    outs = [torch.full((n,), 77, dtype=t, device="cuda") for n, t in ((40, torch.float32), (40 * 64, torch.float16), (300 * 64, torch.float16), (300, torch.float32))]
+
+    def go(dtype=1, ids=s["top_ids"].data_ptr(), top_dtype=0, logits=s["top_logits"].data_ptr(), top=8, alpha=0.5, temperature=2.0,
+           labels=s["labels"].data_ptr(), time=20, weight=s["weight"].data_ptr(), loss_scale=1.0, size=need.value, g_scale=None):
+        return lib.ullis_cuda_head_distill_grad(h, torch.cuda.current_stream().cuda_stream, dtype, s["hidden"].data_ptr(), 64, None, weight, None,
+                                                s["bias"].data_ptr(), ids, top_dtype, logits, top, alpha, temperature, labels, 0xFFFFFFFF, 40, time, 64,
+                                                300, loss_scale, outs[0].data_ptr(), outs[1].data_ptr(), outs[2].data_ptr(), g_scale, outs[3].data_ptr(),
+                                                work.data_ptr(), size)
+
+    nan, inf = float("nan"), float("inf")
+    for bad in (dict(dtype=0), dict(top_dtype=5), dict(ids=None), dict(logits=None), dict(logits=s["top_logits"].data_ptr() + 1), dict(alpha=-0.1),
+                dict(alpha=1.1), dict(alpha=nan), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=nan), dict(temperature=inf),
+                dict(temperature=129.0), dict(weight=None), dict(loss_scale=inf), dict(labels=s["labels"].data_ptr() + 1), dict(g_scale=outs[3].data_ptr())):
+        assert go(**bad) == cuda.ERR_ARG, bad
+    for bad in (dict(top=0), dict(top=257), dict(time=3), dict(time=0), dict(size=need.value - 1)):
+        assert go(**bad) == cuda.ERR_SHAPE, bad
+    torch.cuda.synchronize()
+    assert all((o == 77).all() for o in outs)
+    assert go() == cuda.OK
+    torch.cuda.synchronize()
+    assert all(not (o == 77).all() for o in outs)
+
+
+@pytest.mark.parametrize("labels", [True, False])
+def test_small_shares(cuda_rt, labels):
+    """A small alpha without labels, a low temperature: FP16 keeps as many bits of small gradients as of large ones."""
+    s = student(300, 100, 64, 700, "f16", True, 12, labels=labels, alpha=1.0 if labels else 0.01, temperature=1 / 64, seed=9)
+    got, want = call(cuda_rt, s), formulas(s)
+    check(got, want)
+    value, _ = want["hidden"]
+    # the operand's rounding, half a step of each term; what leaves is 6e-6, where FP16 has steps of 2^-24: half of one more
+    assert ((got.hidden.double() - value).abs() <= 2.0 ** -9 * value.abs().max() + 2.0 ** -25).all()
+    # the same gradients lifted by the loss scale to where FP16 has all its bits
+    got, (value, _) = call(cuda_rt, s, loss_scale=8192.0), formulas(s, loss_scale=8192.0)["hidden"]
+    assert ((got.hidden.double() - value).abs() <= 2.0 ** -9 * value.abs().max() + 2.0 ** -25).all()

@@ -240,8 +240,8 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
 // ------------------------------------------------------------------------------------------------ gradient of many rows
 // Tokens are sorted by chunks, each by a cluster; with more chunks than one an element's place among all is its place in its chunk and
 // what searches in the others give.  Beside the last of these launches other CTAs write the table's zeros, which costs little there
-// (zeros for the rows alone that no chunk has, found by the same searches: 76550 x 500 into 50021 rows 108 us instead of 82).  Then warps sum runs of rows in that order, a fixed number
-// of places each whatever the tokens are: a run that ends in another warp's places leaves a part of its sum, and a last launch adds those.
+// (zeros for the rows alone that no chunk has, found by the same searches: 76550 x 500 into 50021 rows 108 us instead of 82).  Then warps
+// sum runs of rows in that order, a fixed number of places each whatever the tokens are: a run that ends in another warp's places leaves a part of its sum, and a last launch adds those.
 constexpr uint32_t SORT_EACH = 8, SORT_THREADS = 256, SORT_CTA = SORT_EACH * SORT_THREADS;   // keys to a thread, of a CTA
 constexpr uint32_t MOST_CTAS = 8;   // of a cluster
 constexpr uint32_t WINDOW = 8;      // of sorted tokens, the last of which are kept apart
@@ -612,8 +612,10 @@ void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, 
     if (wide) sums(embed_sums_kernel<T, N, 8 / N, true>);
     else if (N == 8 && on(4)) sums(embed_sums_kernel<T, 4, 2, true>);
     else sums(embed_sums_kernel<T, 4, 2, false>);
-    if (p.tiles > 1)
-        s.chain("embed_join", C % 4 == 0 && aligned(g, 16) ? embed_join_kernel<true> : embed_join_kernel<false>, (unsigned)(ceil_div(p.tiles - 1, THREADS / 32) * ceil_div(C, 128)), THREADS, 0, o, (uint32_t)p.tiles);
+    if (p.tiles > 1) {
+        const auto join = C % 4 == 0 && aligned(g, 16) ? embed_join_kernel<true> : embed_join_kernel<false>;
+        s.chain("embed_join", join, (unsigned)(ceil_div(p.tiles - 1, THREADS / 32) * ceil_div(C, 128)), THREADS, 0, o, (uint32_t)p.tiles);
+    }
 }
 
 }  // namespace

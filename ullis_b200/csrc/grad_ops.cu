@@ -833,7 +833,8 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         e.scale_max = r.scale_max;
         e.n_scale_max = WEIGHT_CTAS;
         e.bf16 = bf16;
-        e.headroom = (uint32_t)std::max(0, (int)std::ceil(std::log2(std::max(1e-30f, teacher.hard + teacher.alpha * teacher.temperature))));
+        // |g| is at most both shares: up to 2^7, and far below 1 for a small alpha or temperature, which FP16 would lose bits of
+        e.headroom = std::max(-14, (int)std::ceil(std::log2(std::max(1e-30f, teacher.hard + teacher.alpha * teacher.temperature))));
         e.lse2 = r.lse2;
         e.second_lse2 = reinterpret_cast<float*>(ws + p.second_lse2);
         e.row_loss = r.row_loss;

@@ -235,7 +235,8 @@ struct EntryRows {
     const uint16_t* scale;     // or null
     const float* scale_max;    // null: no row scales
     uint32_t n_scale_max;
-    uint32_t bf16, headroom;   // 2^headroom: bound of the softmaxes' shares
+    uint32_t bf16;
+    int headroom;              // 2^headroom: bound of the softmaxes' shares
     float *lse2, *second_lse2, *row_loss, *factors;
     float loss_scale;
     uint32_t blocks;           // of rows, CTAs
@@ -335,7 +336,7 @@ entries_rows_kernel(const EntryRows o) {
 #pragma unroll
     for (uint32_t w = 0; w < ROWS_WARPS; ++w) largest = fmaxf(largest, tops[w]);
     const int exponent = (int)(__float_as_uint(largest) >> 23) - 127;
-    const int power = largest > 0.0f && exponent < 128 ? 14 - exponent - (int)o.headroom : 0;
+    const int power = largest > 0.0f && exponent < 128 ? 14 - exponent - o.headroom : 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         o.factors[0] = exp2f((float)power);
         o.factors[1] = exp2f((float)-power) * o.loss_scale;

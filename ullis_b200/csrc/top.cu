@@ -10,8 +10,7 @@
 // of the bounds that each finds for its share of the k holds for all of them, and the first goes through what the others have kept.
 //
 // Bound by memory on long rows and by instructions on short ones: 4096 x 131072 bf16, k = 64 195 us (1.07 GB, 5.5 TB/s); 16384 x 8192 f32 132 us
-// (537 MB, 4.1 TB/s; 5000 warp instructions to a row, of which the reading takes 800: the first bound 600, the queue's chunks 1000, raising and
-// sorting 1600).  Tried and slower there: tiles of 2 or 8 chunks (155, 127 but 220 on the long rows), a sample of 8 or 32 (139), a buffer of
+// (537 MB, 4.1 TB/s; some 5000 warp instructions to a row, a fifth of them for reading it by count, the others for what is kept).  Tried and slower there: tiles of 2 or 8 chunks (155, 127 but 220 on the long rows), a sample of 8 or 32 (139), a buffer of
 // 384 keys (149), the next tiles prefetched into L2 (127, long rows 214).  k = 128 and 256 keep two and four times as much: 250, 476 us.
 #include <algorithm>
 
@@ -244,7 +243,8 @@ top_kernel(const Top o) {
 #pragma unroll
         for (uint32_t u = 0; u < SAMPLE; ++u) {
             const uint32_t chunk = begin + u * 32 + lane;
-            high[u] = chunk >= first_whole && chunk < whole_end ? order_of(Most<T>(*reinterpret_cast<const uint4*>(aligned + (size_t)chunk * N)).value()) : 0u;
+            const bool whole = chunk >= first_whole && chunk < whole_end;
+            high[u] = whole ? order_of(Most<T>(*reinterpret_cast<const uint4*>(aligned + (size_t)chunk * N)).value()) : 0u;
             largest = max(largest, high[u]);
             smallest = min(smallest, high[u]);
         }
