@@ -42,8 +42,8 @@ def student(rows, time, d, vocab, dtype, packed, k, *, labels=True, alpha=0.5, t
     return s
 
 
-def formulas(s, ignore_id=-1, loss_scale=1.0):
-    """{output: (value, tolerance)} in 64 bits."""
+def formulas(s, ignore_id=-1, loss_scale=1.0, operand=None):
+    """{output: (value, tolerance)} in 64 bits.  operand: how far g * scale is rounded, half a step of hidden's type."""
     h, t = s["hidden"].double(), s["hidden"].dtype
     rows, d = h.shape
     packed = s["scale"] is not None
@@ -109,7 +109,7 @@ def formulas(s, ignore_id=-1, loss_scale=1.0):
     sizes = dense + w
     g_off = g_off + 2 * U * sizes
     half = torch.finfo(t).eps / 2
-    gs, gs_off = g * scale, g_off * scale.abs() + half * (g * scale).abs()
+    gs, gs_off = g * scale, g_off * scale.abs() + (half if operand is None else operand) * (g * scale).abs()
     if t == torch.float16:                         # below 2^-14 FP16 has steps of 2^-24; the largest scale and share lie at 2^14
         room = max(0, math.ceil(math.log2(max(1e-30, float(hard.max()) + alpha * tau))))
         biggest = 2.0 ** (14 - room - math.floor(math.log2(max(scale.abs().max().item(), 2.0 ** -24))))
@@ -443,3 +443,23 @@ def test_small_shares(cuda_rt, labels):
     # the same gradients lifted by the loss scale to where FP16 has all its bits
     got, (value, _) = call(cuda_rt, s, loss_scale=8192.0), formulas(s, loss_scale=8192.0)["hidden"]
     assert ((got.hidden.double() - value).abs() <= 2.0 ** -9 * value.abs().max() + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("packed", [True, False], ids=["packed", "dense"])
+@pytest.mark.parametrize("rows,time,d,vocab,k,more", [
+    (32, 32, 256, 8192, 16, dict()), (1, 1, 64, 300, 1, dict(labels=False)), (128, 16, 100, 513, 40, dict(ignored=0.4, temperature=3.0)),
+    (127, 127, 72, 1000, 5, dict(labels=False, absent=0.5, temperature=1.0)), (100, 50, 64, 77, 30, dict(hot=True)), (16, 4, 8, 70_000, 3, dict())])
+def test_few_rows_keep_more_of_their_gradients(cuda_rt, rows, time, d, vocab, k, more, packed, dtype):
+    """Up to 128 rows g * scale is the sum of two 16-bit numbers: off by half a step of half a step."""
+    s = student(rows, time, d, vocab, dtype, packed, k, seed=rows, **more)
+    half = torch.finfo(TYPES[dtype]).eps / 2
+    check(call(cuda_rt, s), formulas(s, operand=half * half))
+
+
+def test_few_rows_by_pieces_of_the_vocabulary(cuda_rt):
+    """So few rows that their logits reach 2^28 only beyond 2^20 columns."""
+    s = student(4, 4, 8, (1 << 20) + 300, "f16", False, 6, seed=2)
+    s["top_ids"][:, 1] = (1 << 20) + 17
+    half = torch.finfo(torch.float16).eps / 2
+    check(call(cuda_rt, s), formulas(s, operand=half * half))

@@ -142,33 +142,44 @@ Cut cut_of(size_t M, size_t N, size_t K, uint32_t pairs, bool two) {
 size_t partial_bytes(size_t M, size_t N, const Cut& c) { return c.splits > 1 ? c.splits * M * N * 4 : 0; }
 
 // The sum of `splits` arrays [M][N], in their order, times alpha as 16 bits or f32; with `accum` added to it, or left there where
-// `out` is null.  Of the M rows the first *counted, if given, and row m goes to row out_rows[m] of `out`.
+// `out` is null.  Of the M rows the first *counted, if given, and row m goes to row out_rows[m] of `out`.  twice: of `out` a row is the sum of
+// two that follow on one another.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 combine_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t M, uint32_t N, const float* __restrict__ factor, float* __restrict__ accum,
-               uint32_t accum_read, T* __restrict__ out, const uint32_t* __restrict__ counted, const int32_t* __restrict__ out_rows) {
+               uint32_t accum_read, T* __restrict__ out, const uint32_t* __restrict__ counted, const int32_t* __restrict__ out_rows, uint32_t twice) {
     chain_entry();
     const size_t n = (size_t)M * N, i = ((size_t)blockIdx.x * THREADS + threadIdx.x) * 4;
-    const size_t end = counted ? min((size_t)*counted, (size_t)M) * N : n;
+    const size_t end = (counted ? min((size_t)*counted, (size_t)M) * N : n) >> twice;
     if (i >= end) return;
     const float alpha = factor ? *factor : 1.0f;
     const bool whole = N % 4 == 0;   // four elements of one row, each of the arrays on 16 bytes
+    uint32_t row = (uint32_t)(i / N), c = (uint32_t)(i - (size_t)row * N);
     float v[4] = {};
-    if (whole) {
+    const uint32_t arrays = splits + (accum && accum_read);
+    if (whole && twice) {
+        const size_t at = i + (size_t)row * N;   // rows 2 row and 2 row + 1
 #pragma unroll 8
-        for (uint32_t k = 0; k < splits + (accum && accum_read); ++k) {
+        for (uint32_t k = 0; k < arrays; ++k) {
+            const float* from = (k < splits ? partial + k * n : accum) + at;
+            const float4 t = *reinterpret_cast<const float4*>(from), u = *reinterpret_cast<const float4*>(from + N);
+            v[0] += t.x + u.x; v[1] += t.y + u.y; v[2] += t.z + u.z; v[3] += t.w + u.w;
+        }
+    } else if (whole) {
+#pragma unroll 8
+        for (uint32_t k = 0; k < arrays; ++k) {
             const float4 t = *reinterpret_cast<const float4*>((k < splits ? partial + k * n : accum) + i);
             v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
         }
     } else {
-        for (uint32_t k = 0; k < splits + (accum && accum_read); ++k)
+        for (uint32_t k = 0; k < arrays; ++k)
             for (int e = 0; e < 4; ++e)
-                if (i + e < end) v[e] += (k < splits ? partial + k * n : accum)[i + e];
+                for (uint32_t t = 0; t <= twice && i + e < end; ++t)
+                    v[e] += (k < splits ? partial + k * n : accum)[i + e + ((i + e) / N * twice + t) * N];
     }
-    uint32_t row = (uint32_t)(i / N), c = (uint32_t)(i - (size_t)row * N);
     for (int e = 0; e < 4; ++e) {
         if (i + e >= end) break;
-        if (out) out[(size_t)(out_rows ? out_rows[row] : (int32_t)row) * N + c] = tape::from_float<T>(v[e] * alpha);
+        if (out) out[(size_t)(out_rows ? out_rows[row << twice] : (int32_t)row) * N + c] = tape::from_float<T>(v[e] * alpha);
         else accum[i + e] = v[e];
         if (++c == N) { c = 0; ++row; }
     }
@@ -185,6 +196,7 @@ struct Output {
     bool count_k;
     const int32_t* rows;       // where its rows go
     bool beside;               // pair_gemm.cuh
+    bool twice;                // combine_kernel, where `out` is written
 };
 // A product, alpha * (a . b + accum) ...
 void product(const Stream& s, const char* what, const Operand& a, const Operand& b, bool bf16, size_t M, size_t N, size_t K, const Cut& cut,
@@ -214,7 +226,7 @@ void combine(const Stream& s, bool bf16, size_t M, size_t N, const Cut& cut, con
     const unsigned grid = (unsigned)ceil_div(M * N, 4 * THREADS);
     const auto launch = [&](auto kernel, auto* out) {
         s.chain("combine", kernel, grid, THREADS, 0, static_cast<const float*>(o.partial), cut.splits, (uint32_t)M, (uint32_t)N, o.factor, o.accum,
-                (uint32_t)o.accum_read, out, o.count_k ? nullptr : o.counted, o.rows);
+                (uint32_t)o.accum_read, out, o.count_k ? nullptr : o.counted, o.rows, (uint32_t)(o.twice && o.out));
     };
     if (o.f32) launch(combine_kernel<float>, static_cast<float*>(o.out));
     else if (bf16) launch(combine_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(o.out));
@@ -280,6 +292,7 @@ struct HeadOperands {
     uint32_t hidden_ctas;
     uint32_t bf16;
     uint32_t fold;              // weights +/-scale instead of +/-1 (FP16 has both)
+    uint32_t twice;             // 1: every row that counts has two places, one behind the other (few rows; `place` is null)
     uint32_t* status;           // hidden in f32: a finite value beyond FP16 is reported
 };
 constexpr uint32_t WEIGHT_CTAS = 1024;
@@ -337,10 +350,10 @@ head_operands_kernel(const HeadOperands o) {
                 at += before[w] + (w < warp ? own[w] : 0u);
                 counted += all[w];
             }
-            if (blockIdx.x == 0 && threadIdx.x == 0) *o.counted = counted;
+            if (blockIdx.x == 0 && threadIdx.x == 0) *o.counted = counted << o.twice;
             if (row >= o.rows) return;
             place = target >= 0 ? (int32_t)at : -1 - (int32_t)(row - at);
-            if (target >= 0 && lane == 0) o.list[at] = (int32_t)row;
+            if (target >= 0 && lane <= o.twice) o.list[(at << o.twice) + lane] = (int32_t)row;
         }
         if (place < 0) {
             if (lane == 0) o.row_loss[row] = target == -1 ? 0.0f : NAN;
@@ -350,10 +363,12 @@ head_operands_kernel(const HeadOperands o) {
             } else {
                 for (uint32_t i = lane * 2; i < o.g_bytes; i += 64) *reinterpret_cast<uint16_t*>(g + i) = 0;
             }
-            const uint32_t pad = counted + (uint32_t)(-1 - place);   // a row behind the last, for each such row
-            if (pad < (counted + pg::BM - 1) / pg::BM * pg::BM)
-                for (uint32_t chunk = lane; chunk < chunks; chunk += 32)
-                    *reinterpret_cast<uint4*>(o.h16 + (size_t)pad * o.Dp + chunk * 8) = make_uint4(0u, 0u, 0u, 0u);
+            for (uint32_t t = 0; t <= o.twice; ++t) {
+                const uint32_t pad = ((counted + (uint32_t)(-1 - place)) << o.twice) + t;   // a row behind the last, for each such row
+                if (pad < ((counted << o.twice) + pg::BM - 1) / pg::BM * pg::BM)
+                    for (uint32_t chunk = lane; chunk < chunks; chunk += 32)
+                        *reinterpret_cast<uint4*>(o.h16 + (size_t)pad * o.Dp + chunk * 8) = make_uint4(0u, 0u, 0u, 0u);
+            }
             return;
         }
         float dot = 0.0f;
@@ -390,10 +405,11 @@ head_operands_kernel(const HeadOperands o) {
                 for (int e = 0; e < 8; ++e)
                     if (c + e < o.D) dot = fmaf(from16((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu, o.bf16), from16(o.dense[first + c + e], o.bf16), dot);
             }
-            *reinterpret_cast<uint4*>(o.h16 + (size_t)place * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (uint32_t t = 0; t <= o.twice; ++t)
+                *reinterpret_cast<uint4*>(o.h16 + (((size_t)place << o.twice) + t) * o.Dp + c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
-        if (lane == 0) o.target[place] = target;
+        if (lane <= o.twice) o.target[(place << o.twice) + lane] = target;
         if (lane == 0 && o.target_acc) {
             if (o.fold) dot *= __half2float(__ushort_as_half(o.scale[target]));
             o.target_acc[place] = dot;
@@ -583,7 +599,7 @@ constexpr size_t GRAD_ELEMENTS = (size_t)1 << 28;   // of a piece of g: 512 MiB
 // pair they begin at floor(c x), of which inner / x + 1 lie in a run of `inner`, and one begins before it.
 size_t most_slots(size_t outer, uint32_t pairs) { return pairs / outer + 2; }
 
-HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V, bool copies_weight, size_t K1 = 0) {
+HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V, bool copies_weight, size_t K1 = 0, bool twice = false) {
     HeadPlan p{};
     p.K1 = K1;
     p.pairs = pairs_of(rt);
@@ -604,6 +620,7 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
     p.col_slots = (uint32_t)std::min(p.m_tiles, most_slots(last, p.pairs));   // (of one tile at least)
     const size_t width = std::min(p.piece, V);
     p.hidden = cut_of(rows, D, width, p.pairs, true);
+    if (twice) p.hidden.splits = std::max(2u, p.hidden.splits);   // (combine_kernel adds the two rows)
     p.weight = cut_of(width, D, rows, p.pairs, true);
     Parts at;
     p.h16 = at.add(rows * p.Dp * 2);
@@ -656,9 +673,14 @@ size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t 
 // Dense weights that a tensor map takes are read where they are.
 bool head_copies_weight(const void* dense, size_t channels) { return !dense || channels % 8 != 0 || !aligned(dense, 16); }
 
+// A distilled row's gradient is a handful of terms, whose roundings to 16 bits do not average out over few rows.  Up to 128 rows, which
+// with two places each are one tile of the products all the same, g * scale goes in as the sum of two 16-bit numbers (GRAD, Params::residual):
+// its rounding is then far below that of what leaves.  (32 x 256 x 8192, FP16, 16 entries: g_hidden off by 2.1e-4 in norm instead of 3.2e-4;
+// 57 us so 60.)
+constexpr size_t RESIDUAL_ROWS = 128;
 size_t head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, size_t top, bool labels,
                                    bool copies_weight) {
-    return rows ? head_plan(rt, rows, channels, vocab, copies_weight, top + labels).bytes : 0;
+    return rows ? head_plan(rt, rows << (rows <= RESIDUAL_ROWS), channels, vocab, copies_weight, top + labels, rows <= RESIDUAL_ROWS).bytes : 0;
 }
 
 namespace {
@@ -689,10 +711,12 @@ void launch_entries_list(const Stream& s, const Teacher& t, size_t blocks, const
 // `d`: null, or what the target is spread over.
 void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* workspace) {
     const bool as_is = !head_copies_weight(h.weight, h.channels);
-    const HeadPlan p = head_plan(s.rt, h.rows, h.channels, h.vocab, !as_is, d ? d->top + (h.labels != nullptr) : 0);
+    const uint32_t twice = d && h.rows <= RESIDUAL_ROWS;
+    const HeadPlan p = head_plan(s.rt, h.rows << twice, h.channels, h.vocab, !as_is, d ? d->top + (h.labels != nullptr) : 0, twice);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const bool bf16 = h.dtype == BF16;
-    const size_t rows = h.rows, D = h.channels, V = h.vocab;
+    const size_t D = h.channels, V = h.vocab;
+    size_t rows = h.rows;   // (later: of the operands)
     const void* w16 = as_is ? h.weight : static_cast<const void*>(ws + p.w16);
 
     uint32_t* counted = reinterpret_cast<uint32_t*>(ws + p.counted);
@@ -759,11 +783,13 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
     o.hidden_ctas = (uint32_t)ceil_div(rows, THREADS / 32);
     o.bf16 = bf16;
     o.fold = h.fold_scale;
+    o.twice = twice;
     o.status = s.status;
     const unsigned grid = o.hidden_ctas + (as_is ? 0 : WEIGHT_CTAS);
     if (h.hidden_f32) s.chain("head_operands", head_operands_kernel<float>, grid, THREADS, 0, o);
     else s.chain("head_operands", head_operands_kernel<__half>, grid, THREADS, 0, o);   // (moved, not read: bf16 too)
 
+    rows <<= twice;
     const Operand hidden{o.h16, rows, D, p.Dp, false}, weight{w16, V, D, as_is ? D : p.Dp, false};
     pg::Params q{};
     q.M = (uint32_t)rows;
@@ -790,6 +816,7 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         q.second_factor = teacher.second;
         q.row_part2 = reinterpret_cast<float*>(ws + p.row_part2);
         q.second_lse2 = reinterpret_cast<float*>(ws + p.second_lse2);
+        q.residual = twice;
         const auto list_kernel = d->dtype == F32 ? launch_entries_list<float> : d->dtype == F16 ? launch_entries_list<__half> : launch_entries_list<__nv_bfloat16>;
         list_kernel(s, teacher, p.blocks, o.target, list, counted, lists);
         if (squarings == 1) launch<8, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
@@ -833,6 +860,7 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         e.scale_max = r.scale_max;
         e.n_scale_max = WEIGHT_CTAS;
         e.bf16 = bf16;
+        e.residual = twice;
         // |g| is at most both shares: up to 2^7, and far below 1 for a small alpha or temperature, which FP16 would lose bits of
         e.headroom = std::max(-14, (int)std::ceil(std::log2(std::max(1e-30f, teacher.hard + teacher.alpha * teacher.temperature))));
         e.lse2 = r.lse2;
@@ -903,6 +931,7 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         x.counted = counted;
         x.rows = list;
         x.beside = true;
+        x.twice = twice;
         product(s, "head_g_hidden", by_rows, wp, bf16, rows, D, width, p.hidden, x);
         combine(s, bf16, width, D, p.weight, w);
         combine(s, bf16, rows, D, p.hidden, x);
@@ -1198,7 +1227,7 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
     launch<pg::SUM, 1>(s, "tape_weight_grad", a, b, bf16, q, pairs, &in_parts);
     if (p.cut.splits > 1)
         s.chain("combine", combine_kernel<float>, (unsigned)ceil_div(out * in, 4 * THREADS), THREADS, 0, static_cast<const float*>(q.partial), p.cut.splits,
-                (uint32_t)out, (uint32_t)in, nullptr, nullptr, 0u, g, nullptr, nullptr);
+                (uint32_t)out, (uint32_t)in, nullptr, nullptr, 0u, g, nullptr, nullptr, 0u);
 }
 
 }  // namespace dev

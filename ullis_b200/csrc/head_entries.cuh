@@ -235,7 +235,7 @@ struct EntryRows {
     const uint16_t* scale;     // or null
     const float* scale_max;    // null: no row scales
     uint32_t n_scale_max;
-    uint32_t bf16;
+    uint32_t bf16, residual;   // residual: of two places that follow on one another the second has what rounding takes from the first's g
     int headroom;              // 2^headroom: bound of the softmaxes' shares
     float *lse2, *second_lse2, *row_loss, *factors;
     float loss_scale;
@@ -278,8 +278,9 @@ entries_rows_kernel(const EntryRows o) {
             if (block >= end) return false;
             next.in = at + lane < last;
             const size_t i = block * block_entries + at + lane;
-            next.run = next.in ? (o.lists.bits[i] & (pg::ENTRY_PLACES - 1)) >> 4 : 0xFFFFFFFFu;   // half, column
-            next.w = next.in ? -o.lists.weight[i] : 0.0f;
+            const uint32_t bits = next.in ? o.lists.bits[i] : 0u;
+            next.w = next.in && !(o.residual & bits) ? -o.lists.weight[i] : 0.0f;   // (bits & 1: the second of two places)
+            next.run = next.in ? (bits & (pg::ENTRY_PLACES - 1)) >> 4 : 0xFFFFFFFFu;   // half, column
             next.product = next.in ? o.logits[i].x : 0.0f;
             at += 32;
             if (at >= last) {
@@ -411,7 +412,7 @@ entries_rows_kernel(const EntryRows o) {
             lse -= log2f(t.hard + soft);
             off /= t.first;
         }
-        o.row_loss[o.list[row]] = (loss + off) * LN2 + (has ? constant : 0.0f);
+        if (!(o.residual & row)) o.row_loss[o.list[row]] = (loss + off) * LN2 + (has ? constant : 0.0f);
         o.lse2[row] = lse;
         row_lse[0][r] = lse;
         if (two) o.second_lse2[row] = second;
@@ -419,6 +420,9 @@ entries_rows_kernel(const EntryRows o) {
     }
     __syncthreads();
     const float times = exp2f((float)power);
+    const auto to_bits = [&](float v) {
+        return o.bf16 ? (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v)) : (uint32_t)__half_as_ushort(__float2half_rn(v));
+    };
     const uint32_t n = o.lists.offsets[(size_t)blockIdx.x * o.lists.groups1 + o.lists.groups1 - 1];
 #pragma unroll 2
     for (uint32_t j = threadIdx.x; j < n; j += ROWS_THREADS) {
@@ -428,7 +432,9 @@ entries_rows_kernel(const EntryRows o) {
         float g = pg::exp2_fast(z - row_lse[0][of]);
         if (two) g += pg::exp2_fast(fmaf(z, t.second, -row_lse[1][of]));
         g = (g - w) * times * pg::half_at(o.scale, column, 1.0f);
-        o.lists.column[i] = bits | (o.bf16 ? (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(g)) : (uint32_t)__half_as_ushort(__float2half_rn(g))) << 16;
+        uint32_t g16 = to_bits(g);
+        if (o.residual & bits) g16 = to_bits(g - (o.bf16 ? __uint_as_float(g16 << 16) : __half2float(__ushort_as_half((uint16_t)g16))));
+        o.lists.column[i] = bits | g16 << 16;
     }
 }
 

@@ -97,6 +97,8 @@ struct Params {
     float2* entry_logits;      // LSE: the entry's product, and its logit as the epilogues have it
     float column_factor;       // 1 / the temperature that the epilogues' logits are at: of the first (only) softmax, with squarings of the second
     float second_factor;       // .._2: 1 / the temperature of the second
+    uint32_t residual;         // GRAD: rows 2 m and 2 m + 1 are the same; the second has what rounding to 16 bits takes from the first's g, and
+                               // is in no sum over the columns
     float* row_part2;          // .._2: LSE: the second sums beside row_part's
     const float* second_lse2;  // .._2: GRAD: as lse2
     uint32_t pitch;            // GRAD: of col_part, whole tiles
@@ -345,6 +347,11 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     }
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack16(uint32_t w) {
+    if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 __device__ __forceinline__ float half_at(const uint16_t* p, uint32_t i, float missing) {
     return p ? __half2float(__ushort_as_half(p[i])) : missing;
@@ -852,7 +859,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 const float* rows = row_smem + turn * TURN;
                 turn ^= 1;
                 const uint32_t first = p.n_first + n0;
-                const bool any = !ENTRIES && __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
+                const bool any = ENTRIES ? p.residual != 0 : __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
                 more = work.next();
                 if (more) {
                     fetch(turn);
@@ -864,7 +871,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 // 16 rows at a time, one copy of the code for both: with two the registers ran out.  TARGETS: the target of one of the
                 // warp's rows lies in its columns.  Its product and its g are the row's: lse2 is a number of the size of the logits, off
                 // by 2e-6 where those are 36, and a model that is sure leaves a g of that size.
-                const auto half = [&](int h, auto targets) {
+                // (ENTRIES: with a residual)
+                const auto half = [&](int h, auto special) {
+                    constexpr bool TARGETS = decltype(special)::value && !ENTRIES, RESIDUAL = decltype(special)::value && ENTRIES;
                     uint32_t r[2][8];   // 16 columns are on their way while 16 are worked on
                     tmem_ld_16x16(taddr + ((h * 16) << 16), r[0]);
                     uint64_t l[2], l2[2];
@@ -880,7 +889,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             if (SQUARINGS > 0) lse2 = m0 + row < M ? exp2_fast(lse2 - lse) : 0.0f;
                             l2[i] = two(lse2, lse2);
                         }
-                        if (decltype(targets)::value)
+                        if (TARGETS)
                             at[i] = m0 + row < M ? reinterpret_cast<const uint32_t*>(rows)[96 + row] - first - q2 : 0x80000000u;
                     }
                     const uint32_t to = blocks_at + h * STAGING_BYTES;
@@ -913,17 +922,22 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                                     const float2 e2 = of_two(fma2(z, two(p.second_factor, p.second_factor), l2[i]));
                                     g = add2(g, two(exp2_fast(e2.x), exp2_fast(e2.y)));
                                 }
-                                if (decltype(targets)::value) {
+                                if (TARGETS) {
                                     const uint32_t row = h * 16 + i * 8 + r0;
                                     const bool x = at[i] == (uint32_t)(j + u) * 8, y = at[i] == (uint32_t)(j + u) * 8 + 1;
                                     const float2 av = of_two(a), gv = of_two(g);
                                     a = two(x ? rows[32 + row] : av.x, y ? rows[32 + row] : av.y);
                                     g = two(x ? rows[64 + row] : gv.x, y ? rows[64 + row] : gv.y);
                                 }
-                                g_sum[j + u] = add2(g_sum[j + u], g);
-                                ga_sum[j + u] = fma2(g, a, ga_sum[j + u]);
+                                const uint64_t counts = RESIDUAL && (r0 & 1) ? 0 : g;
+                                g_sum[j + u] = add2(g_sum[j + u], counts);
+                                ga_sum[j + u] = fma2(counts, a, ga_sum[j + u]);
                                 const float2 o = of_two(mul2(g, k));
                                 w[u * 2 + i] = pack16<BF16>(o.x, o.y);
+                                if (RESIDUAL && (r0 & 1)) {
+                                    const float2 r = unpack16<BF16>(w[u * 2 + i]);
+                                    w[u * 2 + i] = pack16<BF16>(o.x - r.x, o.y - r.y);
+                                }
                             }
                         }
                         // 16-byte piece c of row r at c ^ (r % 8), as the copy below reads it; no bank conflicts
