@@ -463,3 +463,20 @@ def test_few_rows_by_pieces_of_the_vocabulary(cuda_rt):
     s["top_ids"][:, 1] = (1 << 20) + 17
     half = torch.finfo(torch.float16).eps / 2
     check(call(cuda_rt, s), formulas(s, operand=half * half))
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 3.0])
+def test_columns_that_a_bias_masks(cuda_rt, temperature):
+    """A bias of -infinity takes columns out: the others' results are those of the smaller vocabulary, the masked ones' gradients are zero."""
+    s = student(400, 100, 64, 1100, "bf16", False, 9, temperature=temperature, seed=14)
+    s["labels"] = s["labels"] % 800
+    s["top_ids"] = s["top_ids"] % 800
+    s["bias"][800:] = -math.inf
+    small = dict(s, weight=s["weight"][:800].contiguous(), bias=s["bias"][:800].contiguous())
+    got, want = call(cuda_rt, s), formulas(small)
+    assert (got.weight[800:] == 0).all() and (got.bias[800:] == 0).all()
+    check(got._replace(weight=got.weight[:800], bias=got.bias[:800]), want)
+    # a masked column that the teacher has: its row's loss is infinite, as the formula's, and no number is lost
+    s["top_ids"][5, 0] = 900
+    got = call(cuda_rt, s)
+    assert got.row_loss[5] == math.inf and int(got.row_loss.isinf().sum()) == 1 and got.hidden.isfinite().all() and got.weight.isfinite().all()
