@@ -572,8 +572,9 @@ ULLIS_CUDA_API int32_t ullis_cuda_head_ce_grad(ullis_cuda_runtime* rt, void* cud
  * vocabulary's size or above, or a logit of NaN or +infinity, has a loss of NaN and gives
  * no gradient; negative ids' logits are not looked at.  alpha in 0 .. 1, temperature in
  * 1/128 .. 128.  Arguments, outputs and limits otherwise as for ullis_cuda_head_ce_grad;
- * the logits of entries keep what the tensor cores leave of them, and losses are sums of
- * terms none of which is negative but alpha * T^2 * sum p * log p. */
+ * the target whose logit is added with rounding is the label, without labels the entry
+ * of the largest logit.  Losses are sums of terms none of which is negative but alpha *
+ * T^2 * sum p * log p. */
 ULLIS_CUDA_API int32_t ullis_cuda_head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels,
                                                               size_t vocab, size_t top, int32_t has_labels,
                                                               int32_t copies_weight, size_t* bytes);

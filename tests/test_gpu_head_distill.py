@@ -480,3 +480,33 @@ def test_columns_that_a_bias_masks(cuda_rt, temperature):
     s["top_ids"][5, 0] = 900
     got = call(cuda_rt, s)
     assert got.row_loss[5] == math.inf and int(got.row_loss.isinf().sum()) == 1 and got.hidden.isfinite().all() and got.weight.isfinite().all()
+
+
+@pytest.mark.parametrize("labels,alpha,temperature", [(True, 0.5, 2.0), (True, 0.3, 3.0), (True, 0.6, 1.0), (False, 1.0, 1.0), (False, 1.0, 2.5)])
+@pytest.mark.parametrize("rows", [64, 1300])
+def test_a_target_of_one_sign(cuda_rt, rows, labels, alpha, temperature):
+    """The target's logit (the label's, or the teacher's likeliest) is a sum of 4096 positive terms, every other logit zero.  The target is added
+    with rounding: a lane's 128 terms one after the other and five steps between lanes, 133 * 2^-24 of the sum at most, of which the tensor
+    cores would cut off 2.7e-5.  The loss moves by (1 - alpha) * (1 - q) + alpha * T * (1 - q_T) of that, the bias's gradient by
+    (1 - alpha) * q * (1 - q) + alpha * q_T * (1 - q_T), at most a quarter a row."""
+    d, vocab = 4096, 400
+    g = torch.Generator("cuda").manual_seed(rows)
+    hidden = (0.5 + torch.rand(rows, d, generator=g, device="cuda")).half()
+    weight = torch.zeros(vocab, d, dtype=torch.float16, device="cuda")
+    weight[7] = ((0.5 + torch.rand(d, generator=g, device="cuda")) * (math.log(vocab) * temperature / d)).half()
+    ids = torch.tensor([300, 7, -1], dtype=torch.int32, device="cuda").repeat(rows, 1)
+    said = torch.tensor([-40.0 * temperature, 2.0, 90.0], device="cuda").repeat(rows, 1)
+    token = torch.full((rows,), 7, dtype=torch.int32, device="cuda") if labels else None
+    s = dict(hidden=hidden, weight=weight, scale=None, bias=torch.zeros(vocab, dtype=torch.float16, device="cuda"), labels=token, time=rows,
+             top_ids=ids, top_logits=said, alpha=alpha, temperature=temperature)
+    got, want = call(cuda_rt, s), formulas(s)
+    z = (hidden.double() @ weight[7].double())
+    hard = (1.0 - alpha) if labels else 0.0
+    off = 133 * U * z
+    q, q_t = torch.sigmoid(z - math.log(vocab - 1)), torch.sigmoid(z / temperature - math.log(vocab - 1))
+    steps = 2.0 ** -20 * (1.0 + temperature ** 2)   # exp, log and the sums of the loss's terms, of sizes up to 1 and T^2 times a few
+    bound = (hard * (1 - q) + alpha * temperature * (1 - q_t)) * off + 8 * steps
+    assert ((got.row_loss.double() - want["row_loss"][0]).abs() <= bound).all()
+    bias = want["bias"][0][7]
+    moves = ((hard * q * (1 - q) + alpha * q_t * (1 - q_t)) * off).sum() + (hard + alpha * temperature) * rows * 2.0 ** -20
+    assert abs(got.bias[7].double() - bias) <= moves

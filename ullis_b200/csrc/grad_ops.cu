@@ -284,7 +284,8 @@ struct HeadOperands {
     uint32_t g_bytes;           // of a row of it
     uint16_t* h16;
     int32_t* target;
-    float *target_acc, *logit2; // the target's product; its logit times log2 e.  Both null: not wanted
+    float *target_acc, *logit2; // the target's product; its logit times log2 e (or what the first softmax takes)
+    float log2e;
     const uint32_t* bits;
     const uint16_t *dense, *scale, *bias;
     uint16_t* w16;              // null: the dense weights are taken as they are
@@ -394,8 +395,7 @@ head_operands_kernel(const HeadOperands o) {
                         w[e >> 1] |= (uint32_t)h << (16 * (e & 1));
                     }
             }
-            if (!o.target_acc) {
-            } else if (o.bits) {
+            if (o.bits) {
                 const uint32_t signs = signs8(o.bits, first + c, words);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)   // (0 past the row's end)
@@ -410,13 +410,14 @@ head_operands_kernel(const HeadOperands o) {
         }
         for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
         if (lane <= o.twice) o.target[(place << o.twice) + lane] = target;
-        if (lane == 0 && o.target_acc) {
+        if (lane <= o.twice) {
+            const uint32_t at = (place << o.twice) + lane;
             if (o.fold) dot *= __half2float(__ushort_as_half(o.scale[target]));
-            o.target_acc[place] = dot;
+            o.target_acc[at] = dot;
             // rounded as the epilogues round theirs: the difference of two logits is then what it is
             const float scale = o.scale && !o.fold ? __half2float(__ushort_as_half(o.scale[target])) : 1.0f;
             const float bias = o.bias ? __half2float(__ushort_as_half(o.bias[target])) : 0.0f;
-            o.logit2[place] = fmaf(dot, scale * pg::LOG2E, bias * pg::LOG2E);
+            o.logit2[at] = fmaf(dot, scale * o.log2e, bias * o.log2e);
         }
         return;
     }
@@ -590,7 +591,7 @@ struct HeadPlan {
     Cut hidden, weight;
     // with entries: K1 to a row that counts, sorted by blocks of 32 rows and groups of 64 columns
     size_t K1, blocks, groups, stretch, stretches;
-    size_t state, entry_bits, entry_column, entry_weight, entry_logits, entry_place, offsets, constant, second_lse2, row_part2, column_sums;
+    size_t state, entry_bits, entry_column, entry_weight, entry_logits, entry_place, offsets, constant, entry_target, second_lse2, row_part2, column_sums;
     size_t h16, w16, counted, place, list, target, target_acc, target_g, lse2, logit, factors, scale_max, row_part, grad, col_part, accum, hidden_partial, weight_partial, bytes;
 };
 constexpr size_t GRAD_ELEMENTS = (size_t)1 << 28;   // of a piece of g: 512 MiB
@@ -656,6 +657,7 @@ HeadPlan head_plan(const ullis_cuda_runtime* rt, size_t rows, size_t D, size_t V
         p.entry_place = at.add(entries * 2);
         p.offsets = at.add(p.blocks * (2 * p.groups + 1) * 2);
         p.constant = at.add(rows * 4);
+        p.entry_target = at.add(rows * 2);
         p.second_lse2 = at.add(rows * 4);
         p.row_part2 = at.add(p.lse_pieces * p.row_part_piece * 4);
         p.column_sums = at.add(p.stretches * 2 * p.n_tiles * pg::BN * 4);
@@ -745,6 +747,7 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         lists.groups1 = 2 * (uint32_t)p.groups + 1;
         lists.place = reinterpret_cast<uint16_t*>(ws + p.entry_place);
         lists.constant = reinterpret_cast<float*>(ws + p.constant);
+        lists.target = reinterpret_cast<uint16_t*>(ws + p.entry_target);
         int32_t* state = reinterpret_cast<int32_t*>(ws + p.state);
         const auto kernel = d->dtype == F32 ? entries_state_kernel<float> : d->dtype == F16 ? entries_state_kernel<__half> : entries_state_kernel<__nv_bfloat16>;
         s.chain("entries_state", kernel, (unsigned)ceil_div(rows, 8), 256, 0, labels, teacher, (uint32_t)rows, (uint32_t)V, state);
@@ -763,8 +766,9 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
     o.D = (uint32_t)D;
     o.Dp = (uint32_t)p.Dp;
     o.vocab = (uint32_t)V;
-    o.target_acc = d ? nullptr : reinterpret_cast<float*>(ws + p.target_acc);
-    o.logit2 = d ? nullptr : reinterpret_cast<float*>(ws + p.logit);
+    o.target_acc = reinterpret_cast<float*>(ws + p.target_acc);
+    o.logit2 = reinterpret_cast<float*>(ws + p.logit);
+    o.log2e = d ? pg::LOG2E * teacher.first : pg::LOG2E;
     o.labels = labels;
     o.place = listed ? place : nullptr;
     o.list = list;
@@ -843,8 +847,8 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
     r.factors = factors;
     r.loss_scale = h.loss_scale;
     const bool columns = h.g_bias || h.g_scale;
+    EntryRows e{};
     if (d) {
-        EntryRows e{};
         e.teacher = teacher;
         e.lists = lists;
         e.part = r.part;
@@ -856,6 +860,8 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         e.piece_tiles = r.piece_tiles;
         e.pairs = r.pairs;
         e.logits = q.entry_logits;
+        e.target_acc = o.target_acc;
+        e.target_logit = o.logit2;
         e.scale = q.scale;
         e.scale_max = r.scale_max;
         e.n_scale_max = WEIGHT_CTAS;
@@ -868,12 +874,11 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         e.row_loss = r.row_loss;
         e.factors = factors;
         e.loss_scale = r.loss_scale;
-        e.blocks = (uint32_t)p.blocks;
         e.stretch = (uint32_t)p.stretch;
         e.stretches = (uint32_t)p.stretches;
         e.column_sums = reinterpret_cast<float*>(ws + p.column_sums);
         e.column_pitch = p.n_tiles * pg::BN;
-        s.chain("entries_rows", entries_rows_kernel, (unsigned)(p.blocks + (columns ? p.groups * p.stretches : 0)), ROWS_THREADS, 0, e);
+        s.chain("entries_rows", entries_rows_kernel, (unsigned)p.blocks, ROWS_THREADS, 0, e);
         q.entries = lists.column;
     } else {
         s.chain("head_rows", head_rows_kernel, (unsigned)ceil_div(rows, 8), 128, 0, r);
@@ -900,6 +905,8 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         else if (two) launch<pg::GRAD_ENTRIES_2, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
         else if (d) launch<pg::GRAD_ENTRIES, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
         else launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
+        if (d && columns && piece == 0)
+            s.chain("entries_columns", entries_columns_kernel, (unsigned)(p.groups * p.stretches), COLUMNS_THREADS, 0, e);
         // What follows reads g and nothing of one another: few rows leave room for all three at once.
         if (columns)
             s.chain("head_columns", head_columns_kernel, (unsigned)ceil_div(width, 32), 256, 0, static_cast<const float*>(g.col_part), g.pitch,

@@ -14,9 +14,9 @@
 //
 // The rows that count are taken 32 at a time, and their entries sorted by groups of 64 columns and within them by entry_bits: what an
 // epilogue warp has of a tile then lies in a row, and entries of one column beside one another.  Sums go by that order: a call gives the
-// same result every time.  What this costs beside the products, us with 64 entries in each of 16384 rows: states 6.5, lists 39, entries_rows 28,
-// and 15 more in GRAD, whose pairs with the first columns have hundreds of entries to a tile (a teacher's favourites).  All three kernels
-// are bound by instructions (50 to 70 % of the slots) and the latency between them.
+// same result every time.  What this costs beside the products, us with 64 entries in each of 16384 rows: states 7, lists 39,
+// entries_rows 22, entries_columns 24 (some of it behind GRAD), and 15 more in GRAD, whose pairs with the first columns have hundreds of entries
+// to a tile (a teacher's favourites).  All four kernels are bound by instructions (40 to 70 % of the slots) and the latency between them.
 #pragma once
 #include "block_sort.cuh"
 #include "pair_gemm.cuh"
@@ -53,35 +53,43 @@ struct Teacher {
     float first, second;
 };
 
-// The state of every row: HeadLabels::target's numbers (0 without labels).  A warp has a row.
+// The state of every row: HeadLabels::target's numbers; without labels its target is the entry that the teacher holds for the likeliest.  The
+// target is the column whose logit is computed with rounding beside the products: its terms have one sign where a student has learnt
+// anything, and what the tensor cores cut off would stay in the loss and the sums over the columns.  A warp has a row.
 template <typename T>
 __global__ void __launch_bounds__(256)
 entries_state_kernel(const HeadLabels labels, const Teacher t, uint32_t rows, uint32_t vocab, int32_t* __restrict__ state) {
     chain_entry();
     const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= rows) return;
-    bool any = false, bad = false;
+    bool bad = false;
+    uint32_t best = 0, best_id = 0;   // of what lies above -infinity: a number that rises with the logit
     const size_t at = (size_t)row * t.K;
 #pragma unroll 4
     for (uint32_t k = lane; k < t.K; k += 32) {
         const int32_t id = t.ids[at + k];
         const float v = tape::to_float(static_cast<const T*>(t.logits)[at + k]);
         if (id < 0) continue;
-        any |= v != -INFINITY;
         bad |= (uint32_t)id >= vocab || !(v < INFINITY);
+        const uint32_t raw = __float_as_uint(v), order = v > -INFINITY ? raw ^ ((uint32_t)((int32_t)raw >> 31) | 0x80000000u) : 0u;
+        if (order > best) {
+            best = order;
+            best_id = (uint32_t)id;
+        }
     }
-    any = __any_sync(0xffffffffu, any);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    best_id = __reduce_min_sync(0xffffffffu, best == top ? best_id : 0xFFFFFFFFu);
     bad = __any_sync(0xffffffffu, bad);
     if (lane) return;
-    int32_t s = labels.labels ? labels.target(row) : any || bad ? 0 : -1;
-    if (s >= 0 && bad) s = -2;
+    int32_t s = labels.labels ? labels.target(row) : top ? (int32_t)best_id : -1;
+    if (bad && (s >= 0 || !labels.labels)) s = -2;
     state[row] = s;
 }
 
 struct EntryLists {
     // by block of 32 rows that count: 32 * K1 places, and groups1 = 2 groups + 1 offsets among them, for each group that of its first
     // sixteen rows and of the others
-    uint32_t* bits;            // entry_bits (and ENTRY_DEAD)
+    uint32_t* bits;            // entry_bits (and ENTRY_DEAD, ENTRY_TARGET)
     uint32_t* column;          // of the vocabulary; later what GRAD takes: bits and above them the 16-bit g * scale * 2^k
     float* weight;             // w, of a dead one 0
     uint16_t* offsets;
@@ -89,6 +97,7 @@ struct EntryLists {
     // by row that counts
     uint16_t* place;           // [row][K1], in the block's list, of those that have a weight there
     float* constant;           // alpha * T^2 * sum p * log p; without entries NAN, which marks that
+    uint16_t* target;          // the place of the target's entry
 };
 constexpr uint32_t LIST_THREADS = 512;
 
@@ -117,7 +126,7 @@ entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const i
     constexpr uint32_t N = E * LIST_THREADS, WARPS = LIST_THREADS / 32, NUMBER_BITS = 8, NO_SPOT = 0xFFFFFFFFu;
     constexpr Key NO_KEY = ~(Key)0;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    __shared__ uint32_t row_label[BLOCK_ROWS], more[BLOCK_ROWS];   // the label's spot; those of labels that are no entries, rising
+    __shared__ uint32_t row_target[BLOCK_ROWS], row_label[BLOCK_ROWS], more[BLOCK_ROWS];   // spots; more: of labels that are no entries, rising
     const uint32_t first = blockIdx.x * BLOCK_ROWS, rows = *counted, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (first >= rows) return;
     const uint32_t n_rows = min(BLOCK_ROWS, rows - first), n = n_rows * t.K;
@@ -160,7 +169,8 @@ entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const i
         if (lane == 0) {
             // sum of p * log p, with log p = x - log sum
             o.constant[first + r] = has ? share * t.temperature * (sum_x / sum - logf(sum)) : NAN;
-            row_label[r] = labels ? spot_of(r, (uint32_t)target[first + r]) : NO_SPOT;
+            row_target[r] = spot_of(r, (uint32_t)target[first + r]);
+            row_label[r] = labels ? row_target[r] : NO_SPOT;
         }
     }
     __syncthreads();
@@ -190,8 +200,11 @@ entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const i
     __syncthreads();
     const size_t base = (size_t)blockIdx.x * BLOCK_ROWS * t.K1;
     const auto labels_below = [&](uint32_t spot) { return labels ? keys_below(more, BLOCK_ROWS, spot) : 0u; };
-    const auto leave = [&](uint32_t place, uint32_t spot, uint32_t dead, float w) {
-        o.bits[base + place] = (spot & (pg::ENTRY_PLACES - 1)) | dead;
+    const auto leave = [&](uint32_t place, uint32_t spot, bool dead, float w) {
+        const uint32_t r = pg::entry_row(spot);
+        const bool is_target = !dead && row_target[r] == spot;
+        o.bits[base + place] = (spot & (pg::ENTRY_PLACES - 1)) | (dead ? pg::ENTRY_DEAD : 0u) | (is_target ? pg::ENTRY_TARGET : 0u);
+        if (is_target) o.target[first + r] = (uint16_t)place;
         o.column[base + place] = spot / pg::ENTRY_PLACES * GROUP_COLUMNS + pg::entry_column(spot);
         o.weight[base + place] = w;
     };
@@ -206,14 +219,14 @@ entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const i
             for (uint32_t j = i + 1; is_at(j, spot); ++j) w += weight[r * t.K + ((uint32_t)sorted[j] & ((1u << NUMBER_BITS) - 1))];
             if (row_label[r] == spot) w += t.hard;
         }
-        leave(place, spot, dead ? pg::ENTRY_DEAD : 0u, w);
+        leave(place, spot, dead, w);
         o.place[(size_t)(first + r) * t.K1 + k] = (uint16_t)(dead ? NO_PLACE : place);
     }
     if (labels && threadIdx.x < n_rows) {
         const uint32_t spot = row_label[threadIdx.x], at = find(spot), place = at + labels_below(spot);
         const bool entry = is_at(at, spot);
         o.place[(size_t)(first + threadIdx.x) * t.K1 + t.K] = (uint16_t)(entry ? NO_PLACE : place);
-        if (!entry) leave(place, spot, 0u, t.hard);
+        if (!entry) leave(place, spot, false, t.hard);
     }
     for (uint32_t g = threadIdx.x; g < o.groups1; g += LIST_THREADS) {
         const uint32_t spot = g * (pg::ENTRY_PLACES / 2);
@@ -221,10 +234,10 @@ entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const i
     }
 }
 
-// Between the products.  The first CTAs have a block of 32 rows each: log2 sum exp of its rows out of their parts (sixteen lanes to a
-// row), less the logarithm of the softmax's share so that GRAD's exp has it as a factor; the losses; and of every entry the 16-bit
-// g * scale * 2^k that GRAD puts in its place.  The others sum -w and -w * product by columns: 64 columns and a stretch of blocks each,
-// over runs of one column in a word of 32 entries, then over the words and blocks of a warp, then over the warps.
+// Between the products.  A CTA has a block of 32 rows: log2 sum exp of its rows out of their parts (sixteen lanes to a row) and their
+// targets' logits, less the logarithm of the softmax's share so that GRAD's exp has it as a factor; the losses; and of every entry the
+// 16-bit g * scale * 2^k that GRAD puts in its place, and what it adds to GRAD's sums over its column: -w and -w * product, and at the
+// target the difference that rounding makes to the probability and the product too.
 struct EntryRows {
     Teacher teacher;
     EntryLists lists;
@@ -234,7 +247,8 @@ struct EntryRows {
     const uint32_t* counted;
     const int32_t* list;
     uint32_t n_tiles, piece_tiles, pairs;
-    const float2* logits;      // of entries: product, logit
+    float2* logits;            // of entries: product, logit; after it what the entry adds to GRAD's sums over its column
+    const float *target_acc, *target_logit;   // by row: the same of its target, with rounding
     const uint16_t* scale;     // or null
     const float* scale_max;    // null: no row scales
     uint32_t n_scale_max;
@@ -242,94 +256,80 @@ struct EntryRows {
     int headroom;              // 2^headroom: bound of the softmaxes' shares
     float *lse2, *second_lse2, *row_loss, *factors;
     float loss_scale;
-    uint32_t blocks;           // of rows, CTAs
-    uint32_t stretch, stretches;
+    // entries_columns
+    uint32_t stretch, stretches;   // blocks of a CTA
     float* column_sums;        // [stretches][2][groups of 64]
     size_t column_pitch;
 };
 constexpr uint32_t ROWS_THREADS = 512, ROWS_WARPS = ROWS_THREADS / 32;
-__global__ void __launch_bounds__(ROWS_THREADS)
+constexpr uint32_t COLUMNS_THREADS = 256, COLUMNS_WARPS = COLUMNS_THREADS / 32, WORDS = 4;
+
+// Sums of exp over a row's columns: the parts that one of sixteen lanes has, then the target's.
+struct RowSums {
+    float top = -INFINITY, sum = 0.0f, sum2 = 0.0f;
+    __device__ void add(const EntryRows& o, float u, float s, float s2) {
+        const float second = o.teacher.second;
+        if (u > top) {
+            sum = sum * exp2f(top - u) + s;
+            if (second != 0.0f) sum2 = sum2 * exp2f((top - u) * second) + s2;
+            top = u;
+        } else if (s != 0.0f) {   // (NaN too)
+            sum += s * exp2f(u - top);
+            if (second != 0.0f) sum2 += s2 * exp2f((u - top) * second);
+        }
+    }
+    __device__ void parts(const EntryRows& o, uint32_t rows, uint32_t row, uint32_t lane) {
+        const uint32_t m = row / pg::BM, m_tiles = (rows + pg::BM - 1) / pg::BM, whole_rows = m_tiles * pg::BM;
+        for (uint32_t begin = 0, piece = 0; begin < o.n_tiles; begin += o.piece_tiles, ++piece) {
+            const uint32_t width = min(o.piece_tiles, o.n_tiles - begin);
+            const pg::Share share = pg::share_of(m_tiles * width, o.pairs);
+            const uint32_t slots = share.owner(m * width + width - 1) - share.owner(m * width) + 1;
+            const size_t at = piece * o.part_piece + row;
+#pragma unroll 4
+            for (uint32_t i = lane; i < slots * 4; i += 16) {   // a slot's quarters of the columns
+                const size_t from = at + (size_t)i * whole_rows;
+                const float2 p = o.part[from];
+                add(o, p.x, p.y, o.teacher.second != 0.0f ? o.part2[from] : 0.0f);
+            }
+        }
+    }
+    // log2 of both sums over all columns, less `top` (times the second's factor).  Where the target is the largest, from what the others add
+    // to its 1, which a sum with it has lost where a row is sure.
+    __device__ float2 logs(const EntryRows& o, float target) {
+        const float second = o.teacher.second;
+        if (target >= top) {
+            const float others = sum * exp2f(top - target), others2 = sum2 * exp2f((top - target) * second);
+            top = target;
+            return make_float2(log1pf(others) * pg::LOG2E, second != 0.0f ? log1pf(others2) * pg::LOG2E : 0.0f);
+        }
+        return make_float2(log2f(sum + exp2f(target - top)), second != 0.0f ? log2f(sum2 + exp2f((target - top) * second)) : 0.0f);
+    }
+    // ... and with the shares taken off, what GRAD takes from a logit (times the second's factor) before its exp
+    struct Lse {
+        float first, second;
+        __device__ float probability(const EntryRows& o, float z) const {   // (both shares times theirs)
+            float g = pg::exp2_fast(z - first);
+            if (o.teacher.second != 0.0f) g += pg::exp2_fast(fmaf(z, o.teacher.second, -second));
+            return g;
+        }
+    };
+    __device__ Lse lse(const EntryRows& o, float2 logs, bool has) const {
+        const Teacher& t = o.teacher;
+        const float soft = has ? t.alpha * t.temperature : 0.0f;
+        if (t.second != 0.0f)   // (no entries: infinity, whose exp is 0)
+            return Lse{top + logs.x - log2f(t.hard), top * t.second + logs.y - log2f(soft)};
+        return Lse{top + logs.x - log2f(t.hard + soft), 0.0f};
+    }
+};
+__global__ void __launch_bounds__(ROWS_THREADS, 2)
 entries_rows_kernel(const EntryRows o) {
     chain_entry();
     const Teacher& t = o.teacher;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = *o.counted;
     const size_t block_entries = (size_t)BLOCK_ROWS * t.K1;
-    if (blockIdx.x >= o.blocks) {
-        __shared__ float sums[ROWS_WARPS][2][GROUP_COLUMNS];
-        const uint32_t group = (blockIdx.x - o.blocks) / o.stretches, stretch = (blockIdx.x - o.blocks) % o.stretches;
-        for (uint32_t i = lane; i < 2 * GROUP_COLUMNS; i += 32) sums[warp][0][i] = 0.0f;
-        __syncwarp();
-        const uint32_t end = min((stretch + 1) * o.stretch, (rows + BLOCK_ROWS - 1) / BLOCK_ROWS);
-        // block by block, 32 entries at a time, the next of them on their way
-        uint32_t block = stretch * o.stretch + warp, at = 0, last = 0;
-        struct {
-            uint32_t run;
-            float w, product;
-            bool in;
-        } now, next;
-        const auto open = [&]() {   // the next block that has any
-            while (at >= last && block < end) {
-                const uint16_t* offsets = o.lists.offsets + (size_t)block * o.lists.groups1 + 2 * group;
-                at = offsets[0];
-                last = offsets[2];
-                if (at < last) break;
-                block += ROWS_WARPS;
-            }
-        };
-        const auto fetch = [&]() {
-            next.in = false;
-            if (block >= end) return false;
-            next.in = at + lane < last;
-            const size_t i = block * block_entries + at + lane;
-            const uint32_t bits = next.in ? o.lists.bits[i] : 0u;
-            next.w = next.in && !(o.residual & bits) ? -o.lists.weight[i] : 0.0f;   // (bits & 1: the second of two places)
-            next.run = next.in ? (bits & (pg::ENTRY_PLACES - 1)) >> 4 : 0xFFFFFFFFu;   // half, column
-            next.product = next.in ? o.logits[i].x : 0.0f;
-            at += 32;
-            if (at >= last) {
-                block += ROWS_WARPS;
-                open();
-            }
-            return true;
-        };
-        open();
-        bool more = fetch();
-        while (more) {
-            now = next;
-            more = fetch();
-            float g = now.w, ga = now.w != 0.0f ? now.w * now.product : 0.0f;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t other = __shfl_up_sync(0xffffffffu, now.run, d);
-                if (!__any_sync(0xffffffffu, now.in && (int)lane >= d && other == now.run)) break;   // (nor further apart)
-                const float u = __shfl_up_sync(0xffffffffu, g, d), v = __shfl_up_sync(0xffffffffu, ga, d);
-                if ((int)lane >= d && other == now.run) {
-                    g += u;
-                    ga += v;
-                }
-            }
-            const uint32_t right = __shfl_down_sync(0xffffffffu, now.run, 1);
-            const bool ends = now.in && (lane == 31 || right != now.run);
-#pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {   // (a column may end a run of either)
-                if (ends && now.run >> 6 == half) {
-                    sums[warp][0][now.run & 63u] += g;
-                    sums[warp][1][now.run & 63u] += ga;
-                }
-                __syncwarp();
-            }
-        }
-        __syncthreads();
-        if (threadIdx.x < 2 * GROUP_COLUMNS) {
-            const uint32_t which = threadIdx.x / GROUP_COLUMNS, c = threadIdx.x % GROUP_COLUMNS;
-            float all = 0.0f;
-#pragma unroll
-            for (uint32_t w = 0; w < ROWS_WARPS; ++w) all += sums[w][which][c];
-            o.column_sums[((size_t)stretch * 2 + which) * o.column_pitch + group * GROUP_COLUMNS + c] = all;
-        }
-        return;
-    }
-    __shared__ float tops[ROWS_WARPS], row_lse[2][BLOCK_ROWS];
+    __shared__ float tops[ROWS_WARPS], row_target[BLOCK_ROWS];
+    __shared__ float2 target_more[BLOCK_ROWS];
+    __shared__ RowSums::Lse row_lse[BLOCK_ROWS];
     // the power of two of g * scale
     float largest = o.scale_max ? 0.0f : 1.0f;
     if (o.scale_max)
@@ -347,53 +347,35 @@ entries_rows_kernel(const EntryRows o) {
     }
     const uint32_t first = blockIdx.x * BLOCK_ROWS;
     if (first >= rows) return;
-    const bool two = t.second != 0.0f;
-    // two rows to a warp; a row's sixteen lanes: a quarter of the columns, every fourth slot
-    const uint32_t r = warp * 2 + (lane & 1), row = first + r, part_lane = lane >> 1, quarter = part_lane & 3;
-    const uint32_t m = row / pg::BM, m_tiles = (rows + pg::BM - 1) / pg::BM, whole_rows = m_tiles * pg::BM;   // (32 rows: of one tile)
-    float top = -INFINITY, sum = 0.0f, sum2 = 0.0f;
-    const auto add = [&](float u, float s, float s2) {
-        if (u > top) {
-            sum = sum * exp2f(top - u) + s;
-            if (two) sum2 = sum2 * exp2f((top - u) * t.second) + s2;
-            top = u;
-        } else if (s != 0.0f) {   // (NaN too)
-            sum += s * exp2f(u - top);
-            if (two) sum2 += s2 * exp2f((u - top) * t.second);
-        }
-    };
-    for (uint32_t begin = 0, piece = 0; begin < o.n_tiles; begin += o.piece_tiles, ++piece) {
-        const uint32_t width = min(o.piece_tiles, o.n_tiles - begin);
-        const pg::Share share = pg::share_of(m_tiles * width, o.pairs);
-        const uint32_t slots = share.owner(m * width + width - 1) - share.owner(m * width) + 1;
-        const size_t at = piece * o.part_piece + row;
-#pragma unroll 4
-        for (uint32_t i = part_lane >> 2; i < slots; i += 4) {
-            const size_t from = at + (size_t)(i * 4 + quarter) * whole_rows;
-            const float2 p = o.part[from];
-            add(p.x, p.y, two ? o.part2[from] : 0.0f);
-        }
-    }
+    // two rows to a warp, sixteen lanes to a row
+    const uint32_t r = warp * 2 + (lane & 1), row = first + r, part_lane = lane >> 1;   // (32 rows: of one tile)
+    RowSums sums_of;
+    sums_of.parts(o, rows, row, part_lane);
 #pragma unroll
     for (int k = 8; k > 0; k >>= 1) {   // (within a row's lanes, in a fixed order)
-        const float u = __shfl_xor_sync(0xffffffffu, top, 2 * k), s = __shfl_xor_sync(0xffffffffu, sum, 2 * k);
-        const float s2 = __shfl_xor_sync(0xffffffffu, sum2, 2 * k);
-        const float a = top, b = sum, b2 = sum2;
+        const RowSums mine = sums_of;
+        RowSums other;
+        other.top = __shfl_xor_sync(0xffffffffu, mine.top, 2 * k);
+        other.sum = __shfl_xor_sync(0xffffffffu, mine.sum, 2 * k);
+        other.sum2 = __shfl_xor_sync(0xffffffffu, mine.sum2, 2 * k);
         const bool mine_first = !(part_lane & k);
-        top = mine_first ? a : u;
-        sum = mine_first ? b : s;
-        sum2 = mine_first ? b2 : s2;
-        add(mine_first ? u : a, mine_first ? s : b, mine_first ? s2 : b2);
+        sums_of = mine_first ? mine : other;
+        if (mine_first) sums_of.add(o, other.top, other.sum, other.sum2);
+        else sums_of.add(o, mine.top, mine.sum, mine.sum2);
     }
     const bool in = row < rows;
+    const float target = in ? o.target_logit[row] : 0.0f;
+    const float2 logs = sums_of.logs(o, target);
     float off = 0.0f;   // sum of w * (top - z)
     if (in) {
+        const uint32_t target_place = o.lists.target[row];
 #pragma unroll 4
         for (uint32_t k = part_lane; k < t.K1; k += 16) {
             const uint32_t i = o.lists.place[(size_t)row * t.K1 + k];
             if (i == NO_PLACE) continue;
             const float w = o.lists.weight[blockIdx.x * block_entries + i];
-            if (w != 0.0f) off += w * (top - o.logits[blockIdx.x * block_entries + i].y);
+            const float z = i == target_place ? target : o.logits[blockIdx.x * block_entries + i].y;
+            if (w != 0.0f) off += w * (sums_of.top - z);
         }
     }
 #pragma unroll
@@ -401,25 +383,25 @@ entries_rows_kernel(const EntryRows o) {
     if (in && part_lane == 0) {
         const float constant = o.lists.constant[row];
         const bool has = constant == constant;
-        const float soft = has ? t.alpha * t.temperature : 0.0f, soft2 = soft * t.temperature;   // of the gradient and of the loss
-        const float more = log2f(sum);
-        float loss, lse = top + more, second = 0.0f;
-        if (two) {
-            const float more2 = log2f(sum2);
-            loss = t.hard * more + soft2 * more2;
-            lse -= log2f(t.hard);
-            second = top * t.second + more2 - log2f(soft);   // (no entries: infinity, whose exp is 0)
+        const float soft = has ? t.alpha * t.temperature * t.temperature : 0.0f;   // of the loss
+        const RowSums::Lse lse = sums_of.lse(o, logs, has);
+        float loss;
+        if (t.second != 0.0f) {
+            loss = t.hard * logs.x + soft * logs.y;
         } else {
-            loss = (t.hard + soft2) * more;
-            if (t.hard + soft == 0.0f) loss = 0.0f;
-            lse -= log2f(t.hard + soft);
+            loss = t.hard + soft != 0.0f ? (t.hard + soft) * logs.x : 0.0f;
             off /= t.first;
         }
         if (!(o.residual & row)) o.row_loss[o.list[row]] = (loss + off) * LN2 + (has ? constant : 0.0f);
-        o.lse2[row] = lse;
-        row_lse[0][r] = lse;
-        if (two) o.second_lse2[row] = second;
-        row_lse[1][r] = second;
+        o.lse2[row] = lse.first;
+        if (t.second != 0.0f) o.second_lse2[row] = lse.second;
+        row_lse[r] = lse;
+        row_target[r] = target;
+        // for the sums over the columns: GRAD has the probability and the product that were cut off
+        const size_t i = blockIdx.x * block_entries + o.lists.target[row];
+        const float2 cut = o.logits[i];
+        const float w = o.lists.weight[i], p = lse.probability(o, target), p_cut = lse.probability(o, cut.y);
+        target_more[r] = make_float2(p - p_cut - w, (p - w) * o.target_acc[row] - p_cut * cut.x);
     }
     __syncthreads();
     const float times = exp2f((float)power);
@@ -431,14 +413,105 @@ entries_rows_kernel(const EntryRows o) {
     for (uint32_t j = threadIdx.x; j < n; j += ROWS_THREADS) {
         const size_t i = blockIdx.x * block_entries + j;
         const uint32_t bits = o.lists.bits[i], column = o.lists.column[i], of = pg::entry_row(bits);
-        const float w = o.lists.weight[i], z = o.logits[i].y;
-        float g = pg::exp2_fast(z - row_lse[0][of]);
-        if (two) g += pg::exp2_fast(fmaf(z, t.second, -row_lse[1][of]));
-        g = (g - w) * times * pg::half_at(o.scale, column, 1.0f);
+        const float w = o.lists.weight[i];
+        const float2 logit = o.logits[i];
+        const bool is_target = bits & pg::ENTRY_TARGET;
+        const float z = is_target ? row_target[of] : logit.y;
+        o.logits[i] = (w == 0.0f && !is_target) || (o.residual & bits) ? make_float2(0.0f, 0.0f)
+                      : is_target                                  ? target_more[of]
+                                                                   : make_float2(-w, -w * logit.x);
+        const float g = (row_lse[of].probability(o, z) - w) * times * pg::half_at(o.scale, column, 1.0f);
         uint32_t g16 = to_bits(g);
         if (o.residual & bits) g16 = to_bits(g - (o.bf16 ? __uint_as_float(g16 << 16) : __half2float(__ushort_as_half((uint16_t)g16))));
         o.lists.column[i] = bits | g16 << 16;
     }
+}
+
+// The sums over the columns of what their entries add, four words of entries on their way (one, whose
+// targets' parts are looked up by row: 42 us instead of 24): a CTA has 64 columns and a stretch of blocks, and sums over runs of one column in a
+// word of 32 entries, then over the words and blocks of a warp, then over the warps.  It needs nothing of GRAD, which has waited for
+// entries_rows, or this would not have been launched: it begins on the SMs that GRAD leaves first, and waits for GRAD at its end, so that
+// whoever waits for this kernel has waited for both.
+__global__ void __launch_bounds__(COLUMNS_THREADS)
+entries_columns_kernel(const EntryRows o) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = *o.counted;
+    const size_t block_entries = (size_t)BLOCK_ROWS * o.teacher.K1;
+    __shared__ float sums[COLUMNS_WARPS][2][GROUP_COLUMNS];
+    const uint32_t group = blockIdx.x / o.stretches, stretch = blockIdx.x % o.stretches;
+    for (uint32_t i = lane; i < 2 * GROUP_COLUMNS; i += 32) sums[warp][0][i] = 0.0f;
+    __syncwarp();
+    const uint32_t end = min((stretch + 1) * o.stretch, (rows + BLOCK_ROWS - 1) / BLOCK_ROWS);
+    // block by block, words of 32 entries, the next four of them on their way
+    uint32_t block = stretch * o.stretch + warp, at = 0, last = 0;
+    struct {
+        uint32_t words, bits[WORDS];
+        float2 g[WORDS];   // and times the product
+    } now, next;
+    const auto open = [&]() {   // the next block that has any
+        while (at >= last && block < end) {
+            const uint16_t* offsets = o.lists.offsets + (size_t)block * o.lists.groups1 + 2 * group;
+            at = offsets[0];
+            last = offsets[2];
+            if (at < last) break;
+            block += COLUMNS_WARPS;
+        }
+    };
+    const auto fetch = [&]() {
+        next.words = 0;
+        if (block >= end) return;
+        const size_t i = block * block_entries + at + lane;
+#pragma unroll
+        for (uint32_t k = 0; k < WORDS; ++k) {
+            const bool in = at + k * 32 + lane < last;
+            next.bits[k] = in ? o.lists.bits[i + k * 32] : pg::NO_ENTRY;
+            next.g[k] = in ? o.logits[i + k * 32] : make_float2(0.0f, 0.0f);
+        }
+        next.words = min(WORDS, (last - at + 31) / 32);
+        at += WORDS * 32;
+        if (at >= last) {
+            block += COLUMNS_WARPS;
+            open();
+        }
+    };
+    open();
+    fetch();
+    while (next.words) {
+        now = next;
+        fetch();
+#pragma unroll
+        for (uint32_t k = 0; k < WORDS; ++k) {
+            if (k >= now.words) break;
+            const bool in = now.bits[k] != pg::NO_ENTRY;
+            const uint32_t run = in ? (now.bits[k] & (pg::ENTRY_PLACES - 1)) >> 4 : pg::NO_ENTRY;   // half, column
+            float2 g = now.g[k];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const bool same = __shfl_up_sync(0xffffffffu, run, d) == run && (int)lane >= d;
+                if (!__any_sync(0xffffffffu, in && same)) break;   // (nor further apart)
+                const float2 u = make_float2(__shfl_up_sync(0xffffffffu, g.x, d), __shfl_up_sync(0xffffffffu, g.y, d));
+                if (same) g = make_float2(g.x + u.x, g.y + u.y);
+            }
+            const uint32_t right = __shfl_down_sync(0xffffffffu, run, 1);
+            const bool ends = in && (lane == 31 || right != run);
+#pragma unroll
+            for (uint32_t half = 0; half < 2; ++half) {   // (a column may end a run of either)
+                if (ends && run >> 6 == half) {
+                    sums[warp][0][run & 63u] += g.x;
+                    sums[warp][1][run & 63u] += g.y;
+                }
+                __syncwarp();
+            }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 2 * GROUP_COLUMNS) {
+        const uint32_t which = threadIdx.x / GROUP_COLUMNS, c = threadIdx.x % GROUP_COLUMNS;
+        float all = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < COLUMNS_WARPS; ++w) all += sums[w][which][c];
+        o.column_sums[((size_t)stretch * 2 + which) * o.column_pitch + group * GROUP_COLUMNS + c] = all;
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace

@@ -148,8 +148,8 @@ struct Share {
 __host__ __device__ inline Share share_of(uint32_t total, uint32_t pairs) { return Share{total, total < pairs ? total : pairs}; }
 
 // An entry's place in its 32 rows and 64 columns, 0 .. 2^11 in the order of the list: the second sixteen rows last, then by
-// columns.  ENTRY_DEAD: an earlier one of the list has the same place and stands for both.
-constexpr uint32_t ENTRY_PLACES = 2048, ENTRY_DEAD = ENTRY_PLACES, NO_ENTRY = 0xFFFFFFFFu;
+// columns.  ENTRY_DEAD: an earlier one of the list has the same place and stands for both.  ENTRY_TARGET: its column is the row's target.
+constexpr uint32_t ENTRY_PLACES = 2048, ENTRY_DEAD = ENTRY_PLACES, ENTRY_TARGET = 2 * ENTRY_PLACES, NO_ENTRY = 0xFFFFFFFFu;
 __host__ __device__ inline uint32_t entry_bits(uint32_t row, uint32_t column) { return (row & 16u) << 6 | (column & 63u) << 4 | (row & 15u); }
 __device__ __forceinline__ uint32_t entry_row(uint32_t bits) { return (bits >> 6 & 16u) | (bits & 15u); }
 __device__ __forceinline__ uint32_t entry_column(uint32_t bits) { return bits >> 4 & 63u; }
@@ -673,7 +673,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     top = -INFINITY;
                     sum = sum2 = 0.0f;
                     const uint32_t row = m_now * BM + rank * 128 + quarter * 32 + lane;
-                    if (!ENTRIES) target = row < M ? p.target[row] : -1;
+                    target = row < M ? p.target[row] : -1;
                 }
                 __syncwarp();
                 ahead.keep(columns, lane, log2e);
@@ -716,7 +716,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                         }
                     }
                     const int32_t hit = target - (int32_t)(n0 + c * 16);
-                    const bool hits = !ENTRIES && __any_sync(0xffffffffu, hit >= 0 && hit < 16);   // of the warp's rows
+                    const bool hits = __any_sync(0xffffffffu, hit >= 0 && hit < 16);   // of the warp's rows
                     uint64_t z[8];
                     float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
