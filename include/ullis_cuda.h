@@ -506,8 +506,8 @@ ULLIS_CUDA_API int32_t ullis_cuda_embed(ullis_cuda_runtime* rt, void* cuda_strea
                                         size_t rows, size_t channels, size_t vocab, int32_t dtype, void* y);
 /* Its gradient (src/model.rs:2980-2987): g [vocab, channels] f32 = scale * the sum of
  * gy [rows, channels] (dtype) over the rows with that token, zero for tokens that none
- * has; rows of ignore_id and of tokens outside the vocabulary count for nothing, and gy
- * is not read there.  Tokens are sorted on the device; sums are f32, a token's rows in
+ * has; rows of ignore_id and of tokens outside the vocabulary count for nothing, whatever
+ * gy holds there.  Tokens are sorted on the device; sums are f32, a token's rows in
  * rising order in pieces that depend on the sizes and on where its rows lie among the
  * sorted ones alone, so that a call gives the same result every time. */
 ULLIS_CUDA_API int32_t ullis_cuda_embed_grad_workspace(const ullis_cuda_runtime* rt, int32_t dtype, size_t rows,

@@ -226,6 +226,19 @@ def test_gradient_of_many_chunks(cuda_rt, rows, vocab, kind):
     check_grad(cuda_rt.embed_grad(tokens, gy, vocab), tokens, gy, vocab)
 
 
+@pytest.mark.parametrize("rows", [196_608, 196_609, 212_993, 262_144, 262_145, 600_001, (1 << 20) + 3])
+@pytest.mark.parametrize("vocab,kind", [(3000, "words"), (1 << 20, "even"), (5, "same")])
+def test_gradient_of_chunks_that_are_merged(cuda_rt, rows, vocab, kind):
+    """Four to seven merges, the last runs with and without a partner; from one chunk fewer, which is not merged, on."""
+    g = torch.Generator("cuda").manual_seed(rows)
+    tokens = draw_tokens(rows, vocab, kind, g)
+    tokens[::977] = IGNORED
+    gy = torch.randn(rows, 4, generator=g, device="cuda").half()
+    got = cuda_rt.embed_grad(tokens, gy, vocab)
+    check_grad(got, tokens, gy, vocab)
+    assert torch.equal(got, cuda_rt.embed_grad(tokens, gy, vocab))
+
+
 def test_past_32_bits_of_elements(cuda_rt):
     """Tables, gradients and rows beyond 2^32 elements."""
     vocab, d = 8_400_000, 512                                  # 4.3e9
@@ -281,7 +294,7 @@ def test_the_library_refuses(cuda_rt):
     for bad in (dict(dtype=9), dict(scale=float("inf")), dict(tokens=None), dict(x=None), dict(g=None), dict(w=None), dict(w=work.data_ptr() + 4),
                 dict(g=out.data_ptr() + 2)):
         assert grad(**bad) == cuda.ERR_ARG, bad
-    for bad in (dict(stride=8), dict(size=need.value - 1), dict(vocab=0), dict(c=0)):
+    for bad in (dict(stride=8), dict(size=need.value - 1), dict(vocab=0), dict(c=0), dict(rows=1 << 31)):
         assert grad(**bad) == cuda.ERR_SHAPE, bad
     torch.cuda.synchronize()
     assert (out == 77).all()

@@ -9,6 +9,7 @@
 // 177 MB), 131072 x 512 bf16 73.
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "block_sort.cuh"
 #include "device_ops.hpp"
@@ -372,6 +373,31 @@ embed_rank_kernel(const uint32_t* __restrict__ chunk_token, const uint32_t* __re
     }
 }
 
+// Many chunks, whose searches in one another would grow with the square of the rows, are merged instead: runs of `run` sorted elements,
+// two and two, an element's place being its own in its run and what a search in the other gives (of tokens that are the same those of
+// the first run come first).  Neighbours search in neighbouring places.
+__global__ void __launch_bounds__(THREADS)
+embed_merge_kernel(const uint32_t* __restrict__ from_token, const uint32_t* __restrict__ from_row, uint32_t rows, uint32_t run,
+                   uint32_t* __restrict__ to_token, uint32_t* __restrict__ to_row, float* __restrict__ g, size_t zeros) {
+    chain_entry();
+    const uint32_t merge_ctas = (rows + THREADS - 1) / THREADS;
+    if (blockIdx.x >= merge_ctas) {
+        write_zeros(g, zeros, (size_t)(blockIdx.x - merge_ctas) * THREADS + threadIdx.x, (size_t)(gridDim.x - merge_ctas) * THREADS);
+        return;
+    }
+    const uint32_t i = blockIdx.x * THREADS + threadIdx.x;
+    if (i >= rows) return;
+    const uint32_t token = from_token[i], row = from_row[i];
+    const uint32_t own = i / run * run, other = own ^ run;   // (run: a power of two)
+    uint32_t at = i;
+    if (other < rows) {
+        const uint32_t n = min(run, rows - other), before = below(from_token + other, n, token, other < own);
+        at = min(own, other) + (i - own) + before;
+    }
+    to_token[at] = token;
+    to_row[at] = row;
+}
+
 struct GradSums {
     const uint32_t *token, *row;   // sorted
     const void* gy;
@@ -533,8 +559,11 @@ embed_join_kernel(const GradSums o, uint32_t tiles) {
     }
 }
 
+// Chunks that are ranked by searches in all others, not merged.  us of a call, 64 channels and 50021 tokens, ranked / merged: 8 chunks 47 / 52,
+// 12 61 / 65, 16 82 / 75, 32 183 / 129, 64 557 / 265, 256 6664 / 1046.
+constexpr uint32_t MOST_RANKED = 12;
 struct GradPlan {
-    bool few;
+    bool few, merged;   // merged: run by run
     uint32_t bits, chunks, places, blocks;
     size_t tiles, samples, chunk_token, chunk_row, token, row, head, tail, bytes;
 };
@@ -551,6 +580,7 @@ GradPlan grad_plan(const ullis_cuda_runtime* rt, size_t rows, size_t C) {
     p.places = 32;
     while (p.places > 4 && ceil_div(rows, p.places) * p.blocks < (size_t)rt->sm_count * 16) p.places /= 2;
     p.tiles = ceil_div(rows, p.places);
+    p.merged = p.chunks > MOST_RANKED;
     size_t at = 0;
     const auto add = [&](size_t n) {
         const size_t here = at;
@@ -586,6 +616,8 @@ void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, 
     uint32_t *token = reinterpret_cast<uint32_t*>(ws + p.token), *row = reinterpret_cast<uint32_t*>(ws + p.row);
     uint32_t *chunk_token = p.chunks > 1 ? reinterpret_cast<uint32_t*>(ws + p.chunk_token) : token;
     uint32_t *chunk_row = p.chunks > 1 ? reinterpret_cast<uint32_t*>(ws + p.chunk_row) : row;
+    uint32_t merges = 0;   // to and fro
+    while (p.merged && (size_t)1 << (p.bits + merges) < rows) ++merges;
     uint32_t* samples = reinterpret_cast<uint32_t*>(ws + p.samples);
     const size_t elements = vocab * C;
     const size_t zeros = p.chunks > 1 ? 0 : elements;   // beside the sort if it is the only launch before the sums
@@ -595,7 +627,16 @@ void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, 
     const auto sort = narrow ? embed_sort_kernel<uint32_t> : embed_sort_kernel<uint64_t>;
     s.chain_cluster("embed_sort", sort, sort_ctas + (unsigned)ceil_div(zero_ctas(zeros), ctas) * ctas, SORT_THREADS, 0, ctas, tokens, ignore_id,
                     (uint32_t)rows, (uint32_t)vocab, p.bits, sort_ctas, chunk_token, chunk_row, samples, g, zeros);
-    if (p.chunks > 1) {
+    for (uint32_t k = 0; k < merges; ++k) {
+        if (k > 0) {
+            std::swap(token, chunk_token);
+            std::swap(row, chunk_row);
+        }
+        const size_t now = k + 1 == merges ? elements : 0;
+        s.chain("embed_merge", embed_merge_kernel, (unsigned)(ceil_div(rows, THREADS) + zero_ctas(now)), THREADS, 0,
+                static_cast<const uint32_t*>(chunk_token), static_cast<const uint32_t*>(chunk_row), (uint32_t)rows, 1u << (p.bits + k), token, row, g, now);
+    }
+    if (p.chunks > 1 && !p.merged) {
         const size_t held = std::min<size_t>(SAMPLES_HELD, ((size_t)p.chunks << p.bits) / WINDOW) * 4;
         if (held > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(embed_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)held));
         s.chain("embed_rank", embed_rank_kernel, (unsigned)(ceil_div(rows, THREADS) + zero_ctas(elements - zeros)), THREADS, held,
