@@ -39,6 +39,12 @@ struct Stream {   // where a call's kernels go
         ULLIS_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
         launched(what);
     }
+    // A kernel's limit of dynamic shared memory belongs to the device, whichever handle sets it, and a launch above it is refused: every
+    // call says the most that the kernel ever asks for, so that calls of another thread's handle in between change nothing.
+    template <typename... P>
+    void allow_shared(void (*kernel)(P...), size_t most) const {
+        ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    }
     void launched(const char* what) const {
         if (stream == rt->stream) { rt->launched(what); return; }   // (timing marks are events on that stream)
         ++rt->launches;

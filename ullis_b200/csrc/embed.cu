@@ -638,7 +638,7 @@ void embed_grad_as(const Stream& s, const uint32_t* tokens, uint32_t ignore_id, 
     }
     if (p.chunks > 1 && !p.merged) {
         const size_t held = std::min<size_t>(SAMPLES_HELD, ((size_t)p.chunks << p.bits) / WINDOW) * 4;
-        if (held > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(embed_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)held));
+        if (held > 48 * 1024) s.allow_shared(embed_rank_kernel, SAMPLES_HELD * 4);
         s.chain("embed_rank", embed_rank_kernel, (unsigned)(ceil_div(rows, THREADS) + zero_ctas(elements - zeros)), THREADS, held,
                 static_cast<const uint32_t*>(chunk_token), static_cast<const uint32_t*>(chunk_row), static_cast<const uint32_t*>(samples),
                 (uint32_t)rows, p.chunks, token, row, g + zeros, elements - zeros);

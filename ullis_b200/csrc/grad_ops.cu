@@ -692,7 +692,7 @@ void launch_entries_list_of(const Stream& s, const Teacher& t, size_t blocks, co
                             const EntryLists& lists) {
     const auto kernel = entries_list_kernel<T, Key, E>;
     const size_t smem = E * LIST_THREADS * sizeof(Key) + BLOCK_ROWS * t.K * 4;
-    if (smem > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 48 * 1024) s.allow_shared(kernel, E * LIST_THREADS * sizeof(Key) + BLOCK_ROWS * DISTILL_MOST * 4);
     s.chain("entries_list", kernel, (unsigned)blocks, LIST_THREADS, smem, t, target, list, counted, lists);
 }
 template <typename T>

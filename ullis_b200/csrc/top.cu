@@ -325,7 +325,7 @@ template <typename T, uint32_t CAP>
 void launch(const Stream& s, const Top& o) {
     const uint32_t warps = std::max(4u, o.warps);   // of a CTA: few, since they end together
     const size_t smem = warps * CAP * 8;
-    if (smem > 48 * 1024) ULLIS_CUDA_CHECK(cudaFuncSetAttribute(top_kernel<T, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 48 * 1024) s.allow_shared(top_kernel<T, CAP>, MOST_WARPS * CAP * 8);
     s.chain("top_logits", top_kernel<T, CAP>, (unsigned)ceil_div(o.rows, warps / o.warps), warps * 32, smem, o);
 }
 template <typename T>
