@@ -237,7 +237,7 @@ entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const i
 // Between the products.  A CTA has a block of 32 rows: log2 sum exp of its rows out of their parts (sixteen lanes to a row) and their
 // targets' logits, less the logarithm of the softmax's share so that GRAD's exp has it as a factor; the losses; and of every entry the
 // 16-bit g * scale * 2^k that GRAD puts in its place, and what it adds to GRAD's sums over its column: -w and -w * product, and at the
-// target the difference that rounding makes to the probability and the product too.
+// target g less the probability that GRAD has there, and the same of the product.
 struct EntryRows {
     Teacher teacher;
     EntryLists lists;
@@ -293,16 +293,36 @@ struct RowSums {
             }
         }
     }
-    // log2 of both sums over all columns, less `top` (times the second's factor).  Where the target is the largest, from what the others add
-    // to its 1, which a sum with it has lost where a row is sure.
-    __device__ float2 logs(const EntryRows& o, float target) {
+    // log2 of both sums over all columns, less `top` (times the second's factor), and `p`, the target's probabilities: each as itself, or
+    // where it is above a half less 1 (with the sign set, of 0 too).  Where the target is the largest, from what the others add to its 1,
+    // which a sum with it has lost where a row is sure.
+    __device__ float2 logs(const EntryRows& o, float target, float2* p) {
         const float second = o.teacher.second;
+        float hit = 1.0f, hit2 = 1.0f, log, log2 = 0.0f;   // (target's and others' parts of a sum)
         if (target >= top) {
-            const float others = sum * exp2f(top - target), others2 = sum2 * exp2f((top - target) * second);
+            sum = sum * exp2f(top - target) + (target - target);   // (NaN where that is infinite)
+            sum2 *= exp2f((top - target) * second);
             top = target;
-            return make_float2(log1pf(others) * pg::LOG2E, second != 0.0f ? log1pf(others2) * pg::LOG2E : 0.0f);
+            log = log1pf(sum) * pg::LOG2E;
+            if (second != 0.0f) log2 = log1pf(sum2) * pg::LOG2E;
+        } else {
+            hit = exp2f(target - top);
+            hit2 = exp2f((target - top) * second);
+            log = log2f(sum + hit);
+            if (second != 0.0f) log2 = log2f(sum2 + hit2);
         }
-        return make_float2(log2f(sum + exp2f(target - top)), second != 0.0f ? log2f(sum2 + exp2f((target - top) * second)) : 0.0f);
+        const auto share = [](float hit, float others) { return (hit > others ? -others : hit) / (hit + others); };
+        p->x = share(hit, sum);
+        p->y = second != 0.0f ? share(hit2, sum2) : p->x;
+        return make_float2(log, log2);
+    }
+    // The target's g.  p: of `logs`; w: its weight, hard and the teacher's; others: the weights of the row's other entries, which add up to what
+    // the teacher's is short of its share.  A sure row's is the difference of what student and teacher leave to other columns.
+    static __device__ float target_g(const Teacher& t, float2 p, bool has, float w, float others) {
+        const float soft = has ? t.alpha * t.temperature : 0.0f;
+        const float of_label = t.hard * (signbit(p.x) ? p.x : p.x - 1.0f);
+        const float of_teacher = fmaf(soft, p.y, signbit(p.y) ? others : t.hard - w);
+        return t.hard > 0.0f ? of_label + of_teacher : of_teacher;
     }
     // ... and with the shares taken off, what GRAD takes from a logit (times the second's factor) before its exp
     struct Lse {
@@ -327,8 +347,10 @@ entries_rows_kernel(const EntryRows o) {
     const Teacher& t = o.teacher;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = *o.counted;
     const size_t block_entries = (size_t)BLOCK_ROWS * t.K1;
-    __shared__ float tops[ROWS_WARPS], row_target[BLOCK_ROWS];
-    __shared__ float2 target_more[BLOCK_ROWS];
+    __shared__ float tops[ROWS_WARPS];
+    // Of a row's target: g, and what it adds to GRAD's sums.
+    __shared__ float row_g[BLOCK_ROWS];
+    __shared__ float2 row_more[BLOCK_ROWS];
     __shared__ RowSums::Lse row_lse[BLOCK_ROWS];
     // the power of two of g * scale
     float largest = o.scale_max ? 0.0f : 1.0f;
@@ -365,8 +387,9 @@ entries_rows_kernel(const EntryRows o) {
     }
     const bool in = row < rows;
     const float target = in ? o.target_logit[row] : 0.0f;
-    const float2 logs = sums_of.logs(o, target);
-    float off = 0.0f;   // sum of w * (top - z)
+    float2 p_target;
+    const float2 logs = sums_of.logs(o, target, &p_target);
+    float off = 0.0f, others = 0.0f;   // sums of w * (top - z), and of w without the target's
     if (in) {
         const uint32_t target_place = o.lists.target[row];
 #pragma unroll 4
@@ -376,10 +399,14 @@ entries_rows_kernel(const EntryRows o) {
             const float w = o.lists.weight[blockIdx.x * block_entries + i];
             const float z = i == target_place ? target : o.logits[blockIdx.x * block_entries + i].y;
             if (w != 0.0f) off += w * (sums_of.top - z);
+            if (i != target_place) others += w;
         }
     }
 #pragma unroll
-    for (int k = 8; k > 0; k >>= 1) off += __shfl_xor_sync(0xffffffffu, off, 2 * k);
+    for (int k = 8; k > 0; k >>= 1) {
+        off += __shfl_xor_sync(0xffffffffu, off, 2 * k);
+        others += __shfl_xor_sync(0xffffffffu, others, 2 * k);
+    }
     if (in && part_lane == 0) {
         const float constant = o.lists.constant[row];
         const bool has = constant == constant;
@@ -396,12 +423,12 @@ entries_rows_kernel(const EntryRows o) {
         o.lse2[row] = lse.first;
         if (t.second != 0.0f) o.second_lse2[row] = lse.second;
         row_lse[r] = lse;
-        row_target[r] = target;
-        // for the sums over the columns: GRAD has the probability and the product that were cut off
         const size_t i = blockIdx.x * block_entries + o.lists.target[row];
+        const float g = RowSums::target_g(t, p_target, has, o.lists.weight[i], others);
         const float2 cut = o.logits[i];
-        const float w = o.lists.weight[i], p = lse.probability(o, target), p_cut = lse.probability(o, cut.y);
-        target_more[r] = make_float2(p - p_cut - w, (p - w) * o.target_acc[row] - p_cut * cut.x);
+        const float p_cut = lse.probability(o, cut.y);
+        row_g[r] = g;
+        row_more[r] = make_float2(g - p_cut, g * o.target_acc[row] - p_cut * cut.x);
     }
     __syncthreads();
     const float times = exp2f((float)power);
@@ -416,11 +443,10 @@ entries_rows_kernel(const EntryRows o) {
         const float w = o.lists.weight[i];
         const float2 logit = o.logits[i];
         const bool is_target = bits & pg::ENTRY_TARGET;
-        const float z = is_target ? row_target[of] : logit.y;
         o.logits[i] = (w == 0.0f && !is_target) || (o.residual & bits) ? make_float2(0.0f, 0.0f)
-                      : is_target                                  ? target_more[of]
+                      : is_target                                  ? row_more[of]
                                                                    : make_float2(-w, -w * logit.x);
-        const float g = (row_lse[of].probability(o, z) - w) * times * pg::half_at(o.scale, column, 1.0f);
+        const float g = (is_target ? row_g[of] : row_lse[of].probability(o, logit.y) - w) * times * pg::half_at(o.scale, column, 1.0f);
         uint32_t g16 = to_bits(g);
         if (o.residual & bits) g16 = to_bits(g - (o.bf16 ? __uint_as_float(g16 << 16) : __half2float(__ushort_as_half((uint16_t)g16))));
         o.lists.column[i] = bits | g16 << 16;
