@@ -573,8 +573,10 @@ ULLIS_CUDA_API int32_t ullis_cuda_head_ce_grad(ullis_cuda_runtime* rt, void* cud
  * no gradient; negative ids' logits are not looked at.  alpha in 0 .. 1, temperature in
  * 1/128 .. 128.  Arguments, outputs and limits otherwise as for ullis_cuda_head_ce_grad;
  * the target whose logit is added with rounding is the label, without labels the entry
- * of the largest logit.  Losses are sums of terms none of which is negative but alpha *
- * T^2 * sum p * log p. */
+ * of the largest logit.  Its g keeps its digits on rows that are sure, in every output,
+ * as ullis_cuda_head_ce_grad's does; that of another entry is the f32 difference of its
+ * two parts, the sums of which over the rows come from f32 sums of each part.  Losses are
+ * sums of terms none of which is negative but alpha * T^2 * sum p * log p. */
 ULLIS_CUDA_API int32_t ullis_cuda_head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels,
                                                               size_t vocab, size_t top, int32_t has_labels,
                                                               int32_t copies_weight, size_t* bytes);

@@ -96,3 +96,41 @@ def test_gradients_of_sure_rows(cuda_rt, rows, dtype, case):
         value = value * loss_scale
         off = (off + 2 * U * terms * size) * loss_scale + half * value.abs() + lowest + 4 * U * value.abs()
         assert ((x.double() - value).abs() <= off).all()
+
+
+@pytest.mark.parametrize("case", CASES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [100, 128, 129, 600])
+def test_sums_over_sure_rows(cuda_rt, rows, dtype, case):
+    s, after = sure(rows, dtype, 5, **CASES[case])
+    loss_scale = 65536.0 if dtype == "f16" else 1.0   # FP16 gradients of this size need one
+    got = call(cuda_rt, s, loss_scale=loss_scale)
+    a, g, sizes = gradient(s, after)
+    # what is summed over the rows: U a row, and the sums' own additions
+    for x, times in ((got.bias, torch.ones_like(a)), (got.scale, a)):
+        value = (g * times).sum(0) * loss_scale
+        off = (OFF + U * (32 + rows)) * (sizes * times.abs()).sum(0) * loss_scale
+        assert ((x.double() - value).abs() <= off).all()
+
+
+@pytest.mark.parametrize("rows", [4, 260])
+def test_by_pieces_of_the_vocabulary(cuda_rt, rows):
+    """Sure of a token in the last piece of a vocabulary of more than 2^20 columns: its bias is 30 above the others'.  The sums of the others'
+    exp are off by (80 + 2^20 / 256) * 2^-24 and their logits, below 50 in units of ln 2, by 4 * 2^-24 * 50 each: below 2^-11 in all."""
+    vocab, token, d = (1 << 20) + 300, (1 << 20) + 17, 8
+    g = torch.Generator("cuda").manual_seed(rows)
+    hidden = torch.randn(rows, d, generator=g, device="cuda").half()
+    weight = (0.1 * torch.randn(vocab, d, generator=g, device="cuda")).half()
+    bias = torch.zeros(vocab, device="cuda").half()
+    bias[token] = 30.0
+    z = hidden.double() @ weight.double().t() + bias.double()
+    for alpha, temperature in ((0.0, 1.0), (0.5, 1.0), (1.0, 1.0)):
+        s = dict(hidden=hidden, weight=weight, scale=None, bias=bias, labels=torch.full((rows,), token, dtype=torch.int32, device="cuda"), time=rows,
+                 top_ids=torch.tensor([[token, 5]], dtype=torch.int32, device="cuda").repeat(rows, 1), alpha=alpha, temperature=temperature,
+                 top_logits=torch.tensor([[0.0, -math.inf]], device="cuda").repeat(rows, 1))
+        got = call(cuda_rt, s)
+        rest = torch.exp(z - z[:, token:token + 1])
+        rest[:, token] = 0.0
+        value = -(rest.sum(1) / (1.0 + rest.sum(1)))[:-1].sum()
+        assert abs(got.bias[token].double() - value) <= 2.0 ** -11 * -value and value > -1e-6 * rows
+        del rest

@@ -17,6 +17,7 @@
 // bits, 5.6 for the rows' sums and 4.7 for the columns': reads and writes of what they name, bound by their latency.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include <cudaTypedefs.h>
 
@@ -81,8 +82,9 @@ template <int EPI, int ACCS, bool BF16>
 void launch_form(const Stream& s, const char* what, const pg::Maps& maps, const pg::Params& p, uint32_t pairs) {
     const auto kernel = pg::pair_gemm_kernel<EPI, ACCS, BF16>;
     const size_t smem = pg::smem_bytes(EPI, ACCS);
-    static_assert(pg::FORMS * 4 <= 64, "");
-    const uint64_t flag = 1ull << (EPI * 4 + (ACCS - 1) * 2 + BF16);
+    constexpr int form = (ACCS - 1) * 2 * pg::FORMS + EPI * 2 + BF16;
+    static_assert(form < 64, "");
+    const uint64_t flag = 1ull << form;
     if (!(s.rt->pair_gemms_ready & flag)) {
         ULLIS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         s.rt->pair_gemms_ready |= flag;
@@ -676,7 +678,7 @@ size_t head_ce_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t 
 bool head_copies_weight(const void* dense, size_t channels) { return !dense || channels % 8 != 0 || !aligned(dense, 16); }
 
 // A distilled row's gradient is a handful of terms, whose roundings to 16 bits do not average out over few rows.  Up to 128 rows, which
-// with two places each are one tile of the products all the same, g * scale goes in as the sum of two 16-bit numbers (GRAD, Params::residual):
+// with two places each are one tile of the products all the same, g * scale goes in as the sum of two 16-bit numbers (pair_gemm.cuh, TWICE):
 // its rounding is then far below that of what leaves.  (32 x 256 x 8192, FP16, 16 entries: g_hidden off by 2.1e-4 in norm instead of 3.2e-4;
 // 57 us so 60.)
 constexpr size_t RESIDUAL_ROWS = 128;
@@ -737,7 +739,7 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         teacher.hard = h.labels ? (float)(1.0 - (double)d->alpha) : 0.0f;
         teacher.temperature = d->alpha > 0.0f ? d->temperature : 1.0f;
         two = teacher.hard > 0.0f && teacher.temperature != 1.0f;
-        squarings = two && teacher.temperature == 2.0f ? 1 : two && teacher.temperature == 4.0f ? 2 : 0;
+        squarings = !two ? 0 : teacher.temperature == 2.0f ? 1 : teacher.temperature == 4.0f ? 2 : 0;
         teacher.first = two ? 1.0f : 1.0f / teacher.temperature;
         teacher.second = two ? 1.0f / teacher.temperature : 0.0f;
         lists.bits = reinterpret_cast<uint32_t*>(ws + p.entry_bits);
@@ -820,11 +822,10 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         q.second_factor = teacher.second;
         q.row_part2 = reinterpret_cast<float*>(ws + p.row_part2);
         q.second_lse2 = reinterpret_cast<float*>(ws + p.second_lse2);
-        q.residual = twice;
         const auto list_kernel = d->dtype == F32 ? launch_entries_list<float> : d->dtype == F16 ? launch_entries_list<__half> : launch_entries_list<__nv_bfloat16>;
         list_kernel(s, teacher, p.blocks, o.target, list, counted, lists);
-        if (squarings == 1) launch<8, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
-        else if (squarings == 2) launch<10, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+        if (squarings == 1) launch<pg::LSE_ENTRIES_SQUARE, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
+        else if (squarings == 2) launch<pg::LSE_ENTRIES_FOURTH, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
         else if (two) launch<pg::LSE_ENTRIES_2, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
         else launch<pg::LSE_ENTRIES, 1>(s, "head_lse", hidden, weight, bf16, q, p.pairs);
     } else {
@@ -900,11 +901,17 @@ void head_grad(const Stream& s, const HeadGrad& h, const Distill* d, void* works
         wp.data = static_cast<const uint16_t*>(w16) + v0 * weight.stride;
         wp.rows = width;
         const CUtensorMap grad_map = map_of(grad, rows, p.piece, p.piece, 16, bf16);
-        if (squarings == 1) launch<9, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
-        else if (squarings == 2) launch<11, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
-        else if (two) launch<pg::GRAD_ENTRIES_2, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
-        else if (d) launch<pg::GRAD_ENTRIES, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
-        else launch<pg::GRAD, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map);
+        const auto launch_grad = [&](auto form) { launch<decltype(form)::value, 1>(s, "head_grad", hidden, wp, bf16, g, p.pairs, &grad_map); };
+        const auto launch_entries = [&](auto more) {
+            constexpr int TWICE = decltype(more)::value;
+            if (squarings == 1) launch_grad(std::integral_constant<int, pg::GRAD_ENTRIES_SQUARE + TWICE>{});
+            else if (squarings == 2) launch_grad(std::integral_constant<int, pg::GRAD_ENTRIES_FOURTH + TWICE>{});
+            else if (two) launch_grad(std::integral_constant<int, pg::GRAD_ENTRIES_2 + TWICE>{});
+            else launch_grad(std::integral_constant<int, pg::GRAD_ENTRIES + TWICE>{});
+        };
+        if (!d) launch_grad(std::integral_constant<int, pg::GRAD>{});
+        else if (twice) launch_entries(std::integral_constant<int, pg::TWICE>{});
+        else launch_entries(std::integral_constant<int, 0>{});
         if (d && columns && piece == 0)
             s.chain("entries_columns", entries_columns_kernel, (unsigned)(p.groups * p.stretches), COLUMNS_THREADS, 0, e);
         // What follows reads g and nothing of one another: few rows leave room for all three at once.

@@ -44,13 +44,20 @@
 namespace ullis {
 namespace pg {
 
-enum { LSE = 0, GRAD = 1, STORE = 2, SUM = 3, LSE_ENTRIES = 4, GRAD_ENTRIES = 5, LSE_ENTRIES_2 = 6, GRAD_ENTRIES_2 = 7, FORMS = 12 };
+enum {   // (the numbers of LSE with entries are even)
+    LSE = 0, GRAD = 1, STORE = 2, SUM = 3,
+    LSE_ENTRIES = 4, GRAD_ENTRIES, LSE_ENTRIES_2, GRAD_ENTRIES_2, LSE_ENTRIES_SQUARE, GRAD_ENTRIES_SQUARE, LSE_ENTRIES_FOURTH, GRAD_ENTRIES_FOURTH,
+    TWICE = 8, FORMS = GRAD_ENTRIES_FOURTH + TWICE + 1   // GRAD_ENTRIES .. + TWICE
+};
+__host__ __device__ constexpr bool is_twice(int epi) { return epi >= GRAD_ENTRIES + TWICE; }
 __host__ __device__ constexpr int kind_of(int epi) { return epi >= LSE_ENTRIES ? epi & 1 : epi; }   // LSE, GRAD, STORE or SUM
 __host__ __device__ constexpr bool has_entries(int epi) { return epi >= LSE_ENTRIES; }
-__host__ __device__ constexpr bool has_two(int epi) { return epi >= LSE_ENTRIES_2; }
-// 8, 9: .._ENTRIES_2 at a second temperature of 2; 10, 11: of 4.  The exp of the first softmax is the second's squared once or twice:
+__host__ __device__ constexpr bool has_two(int epi) { return epi - (is_twice(epi) ? TWICE : 0) >= LSE_ENTRIES_2; }
+// .._SQUARE, .._FOURTH: .._ENTRIES_2 at a second temperature of 2 or 4.  The exp of the first softmax is the second's squared once or twice:
 // half the exps.  16384 x 512 x 8192 in FP16: LSE 134 us so 117, GRAD 167 so 151.
-__host__ __device__ constexpr int squarings(int epi) { return epi >= 8 ? (epi - 6) / 2 : 0; }
+__host__ __device__ constexpr int squarings(int epi) { return has_two(epi) ? (epi - (is_twice(epi) ? TWICE : 0) - LSE_ENTRIES_2) / 2 : 0; }
+// + TWICE: rows 2 m and 2 m + 1 are the same; the second has what rounding to 16 bits takes from the first's g, and is in no sum over the
+// columns.  (A form of its own: a branch in the others cost their loop registers, 157 us so 171.)
 
 constexpr uint32_t BM = 256, BN = 256, BK = 64;         // of a pair, per accumulator
 constexpr uint32_t OPERAND_BYTES = 128 * BK * 2;        // one CTA's 128 rows of A, or of one accumulator's B
@@ -92,15 +99,14 @@ struct Params {
     const float* target_g;     // GRAD: [M] its probability - 1
     const float* factor;       // GRAD: 2^k ; STORE: alpha
     // .._ENTRIES: entries of block b of 32 rows and group n of 64 columns of the vocabulary: those of its first sixteen rows at
-    // b * block_entries + [offsets[b * groups1 + 2 n], offsets[.. + 1]), the others up to offsets[.. + 2]
+    // b * block_entries + [offsets[b * groups1 + 2 n], offsets[.. + 1]), the others up to offsets[.. + 2].  GRAD: with OFFSET_SURE among the
+    // first (or second) of these the sums over the columns leave out the targets of these sixteen rows
     const uint16_t* offsets;
     uint32_t groups1, block_entries;
     const uint32_t* entries;   // LSE: entry_bits; GRAD: with the 16-bit g * scale * 2^k above them
     float2* entry_logits;      // LSE: the entry's product, and its logit as the epilogues have it
     float column_factor;       // 1 / the temperature that the epilogues' logits are at: of the first (only) softmax, with squarings of the second
     float second_factor;       // .._2: 1 / the temperature of the second
-    uint32_t residual;         // GRAD: rows 2 m and 2 m + 1 are the same; the second has what rounding to 16 bits takes from the first's g, and
-                               // is in no sum over the columns
     float* row_part2;          // .._2: LSE: the second sums beside row_part's
     const float* second_lse2;  // .._2: GRAD: as lse2
     uint32_t pitch;            // GRAD: of col_part, whole tiles
@@ -150,6 +156,7 @@ __host__ __device__ inline Share share_of(uint32_t total, uint32_t pairs) { retu
 // An entry's place in its 32 rows and 64 columns, 0 .. 2^11 in the order of the list: the second sixteen rows last, then by
 // columns.  ENTRY_DEAD: an earlier one of the list has the same place and stands for both.  ENTRY_TARGET: its column is the row's target.
 constexpr uint32_t ENTRY_PLACES = 2048, ENTRY_DEAD = ENTRY_PLACES, ENTRY_TARGET = 2 * ENTRY_PLACES, NO_ENTRY = 0xFFFFFFFFu;
+constexpr uint32_t OFFSET_SURE = 0x8000u;   // beside an offset (of at most 32 * 257)
 __host__ __device__ inline uint32_t entry_bits(uint32_t row, uint32_t column) { return (row & 16u) << 6 | (column & 63u) << 4 | (row & 15u); }
 __device__ __forceinline__ uint32_t entry_row(uint32_t bits) { return (bits >> 6 & 16u) | (bits & 15u); }
 __device__ __forceinline__ uint32_t entry_column(uint32_t bits) { return bits >> 4 & 63u; }
@@ -401,17 +408,18 @@ struct Columns {
 };
 // The entries of a warp's 32 rows and 64 columns: where they lie (on its way a tile ahead) and the first of them.
 struct Entries {
-    uint32_t first, middle, end;
+    uint32_t offsets[3];   // as they lie there
     __device__ void find(const Params& p, uint32_t row, uint32_t column, uint32_t M) {
-        first = middle = end = 0;
+        offsets[0] = offsets[1] = offsets[2] = 0;
         if (row < M) {
             const uint16_t* at = p.offsets + (size_t)(row / 32) * p.groups1 + column / 64 * 2;
-            first = at[0];
-            middle = at[1];
-            end = at[2];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) offsets[i] = at[i];
         }
     }
-    __device__ const uint32_t* list(const Params& p, uint32_t row) const { return p.entries + (size_t)(row / 32) * p.block_entries + first; }
+    __device__ uint32_t at(int i) const { return offsets[i] & (OFFSET_SURE - 1); }
+    __device__ uint32_t sure() const { return offsets[0] >> 15 | offsets[1] >> 14; }   // a bit for sixteen rows
+    __device__ const uint32_t* list(const Params& p, uint32_t row) const { return p.entries + (size_t)(row / 32) * p.block_entries + at(0); }
 };
 constexpr int ENTRIES_HELD = 2;   // LSE: words of 32 entries that are fetched before the accumulator is there
 // The others, in groups of words that are on their way together.
@@ -662,7 +670,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                     const uint32_t row = work.m * BM + rank * 128 + quarter * 32;
                     list = entries.list(p, row);
                     logits = p.entry_logits + (list - p.entries);
-                    n_entries = entries.end - entries.first;
+                    n_entries = entries.at(2) - entries.at(0);
 #pragma unroll
                     for (int b = 0; b < ENTRIES_HELD; ++b) held[b] = b * 32 + lane < n_entries ? list[b * 32 + lane] : NO_ENTRY;
                 }
@@ -835,11 +843,12 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             while (more) {
                 const uint32_t n0 = work.n * BN + group * 64, m0 = work.m * BM + rank * 128 + quarter * 32;
                 const uint32_t* list = nullptr;
-                uint32_t n_half[2] = {0, 0};
+                uint32_t n_half[2] = {0, 0}, sure = 0;
                 if (ENTRIES) {
                     list = entries.list(p, m0);
-                    n_half[0] = entries.middle - entries.first;
-                    n_half[1] = entries.end - entries.middle;
+                    n_half[0] = entries.at(1) - entries.at(0);
+                    n_half[1] = entries.at(2) - entries.at(1);
+                    sure = entries.sure();
                 }
                 // ENTRIES: the entries of a half on their way to shared memory, while its logits are worked on
                 const auto bring = [&](int h) {
@@ -861,7 +870,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 const float* rows = row_smem + turn * TURN;
                 turn ^= 1;
                 const uint32_t first = p.n_first + n0;
-                const bool any = ENTRIES ? p.residual != 0 : __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
+                const bool any = ENTRIES ? sure != 0 : __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
                 more = work.next();
                 if (more) {
                     fetch(turn);
@@ -873,9 +882,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 // 16 rows at a time, one copy of the code for both: with two the registers ran out.  TARGETS: the target of one of the
                 // warp's rows lies in its columns.  Its product and its g are the row's: lse2 is a number of the size of the logits, off
                 // by 2e-6 where those are 36, and a model that is sure leaves a g of that size.
-                // (ENTRIES: with a residual)
+                // ENTRIES: of sure rows (entries_rows_kernel) it is in the sums over the columns with the entries, and here its exp is 0.
                 const auto half = [&](int h, auto special) {
-                    constexpr bool TARGETS = decltype(special)::value && !ENTRIES, RESIDUAL = decltype(special)::value && ENTRIES;
+                    constexpr bool TARGETS = decltype(special)::value;
+                    const bool second = is_twice(EPI) && (r0 & 1);   // of a row's two places
                     uint32_t r[2][8];   // 16 columns are on their way while 16 are worked on
                     tmem_ld_16x16(taddr + ((h * 16) << 16), r[0]);
                     uint64_t l[2], l2[2];
@@ -891,8 +901,8 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             if (SQUARINGS > 0) lse2 = m0 + row < M ? exp2_fast(lse2 - lse) : 0.0f;
                             l2[i] = two(lse2, lse2);
                         }
-                        if (TARGETS)
-                            at[i] = m0 + row < M ? reinterpret_cast<const uint32_t*>(rows)[96 + row] - first - q2 : 0x80000000u;
+                        if (TARGETS && ENTRIES) at[i] = m0 + row < M && (sure >> h & 1u) ? (uint32_t)p.target[m0 + row] - first - q2 : 0x80000000u;
+                        else if (TARGETS) at[i] = m0 + row < M ? reinterpret_cast<const uint32_t*>(rows)[96 + row] - first - q2 : 0x80000000u;
                     }
                     const uint32_t to = blocks_at + h * STAGING_BYTES;
                     if (lane == 0) tma_store_read<1>();   // the store before the last has read this half
@@ -912,7 +922,12 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 uint64_t a = (uint64_t)now[u * 4 + i * 2 + 1] << 32 | now[u * 4 + i * 2];
-                                const uint64_t z = fma2(a, s, b);
+                                uint64_t z = fma2(a, s, b);
+                                const bool x = TARGETS && at[i] == (uint32_t)(j + u) * 8, y = TARGETS && at[i] == (uint32_t)(j + u) * 8 + 1;
+                                if (TARGETS && ENTRIES) {
+                                    const float2 zv = of_two(z);
+                                    z = two(x ? -INFINITY : zv.x, y ? -INFINITY : zv.y);
+                                }
                                 const float2 e = of_two(add2(z, l[i]));
                                 uint64_t g = two(exp2_fast(e.x), exp2_fast(e.y));
                                 if constexpr (SQUARINGS > 0) {
@@ -924,19 +939,18 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                                     const float2 e2 = of_two(fma2(z, two(p.second_factor, p.second_factor), l2[i]));
                                     g = add2(g, two(exp2_fast(e2.x), exp2_fast(e2.y)));
                                 }
-                                if (TARGETS) {
+                                if (TARGETS && !ENTRIES) {
                                     const uint32_t row = h * 16 + i * 8 + r0;
-                                    const bool x = at[i] == (uint32_t)(j + u) * 8, y = at[i] == (uint32_t)(j + u) * 8 + 1;
                                     const float2 av = of_two(a), gv = of_two(g);
                                     a = two(x ? rows[32 + row] : av.x, y ? rows[32 + row] : av.y);
                                     g = two(x ? rows[64 + row] : gv.x, y ? rows[64 + row] : gv.y);
                                 }
-                                const uint64_t counts = RESIDUAL && (r0 & 1) ? 0 : g;
+                                const uint64_t counts = second ? 0 : g;
                                 g_sum[j + u] = add2(g_sum[j + u], counts);
                                 ga_sum[j + u] = fma2(counts, a, ga_sum[j + u]);
                                 const float2 o = of_two(mul2(g, k));
                                 w[u * 2 + i] = pack16<BF16>(o.x, o.y);
-                                if (RESIDUAL && (r0 & 1)) {
+                                if (second) {
                                     const float2 r = unpack16<BF16>(w[u * 2 + i]);
                                     w[u * 2 + i] = pack16<BF16>(o.x - r.x, o.y - r.y);
                                 }
@@ -969,8 +983,8 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 };
 #pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
-                    if (any) half(h, std::true_type{});
-                    else half(h, std::false_type{});
+                    if (any || is_twice(EPI)) half(h, std::true_type{});
+                    else half(h, std::bool_constant<is_twice(EPI)>{});
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
