@@ -144,44 +144,41 @@ Cut cut_of(size_t M, size_t N, size_t K, uint32_t pairs, bool two) {
 size_t partial_bytes(size_t M, size_t N, const Cut& c) { return c.splits > 1 ? c.splits * M * N * 4 : 0; }
 
 // The sum of `splits` arrays [M][N], in their order, times alpha as 16 bits or f32; with `accum` added to it, or left there where
-// `out` is null.  Of the M rows the first *counted, if given, and row m goes to row out_rows[m] of `out`.  twice: of `out` a row is the sum of
-// two that follow on one another.
-template <typename T>
+// `out` is null.  Of the M rows the first *counted, if given, and row m goes to row out_rows[m] of `out`.  TWICE: of `out` a row is the sum of
+// two that follow on one another.  (A form of its own: as an argument it took 1 us of the 19 of a weight gradient of 2048 x 512 x 2048.)
+template <typename T, bool TWICE>
 __global__ void __launch_bounds__(THREADS)
 combine_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t M, uint32_t N, const float* __restrict__ factor, float* __restrict__ accum,
-               uint32_t accum_read, T* __restrict__ out, const uint32_t* __restrict__ counted, const int32_t* __restrict__ out_rows, uint32_t twice) {
+               uint32_t accum_read, T* __restrict__ out, const uint32_t* __restrict__ counted, const int32_t* __restrict__ out_rows) {
     chain_entry();
     const size_t n = (size_t)M * N, i = ((size_t)blockIdx.x * THREADS + threadIdx.x) * 4;
-    const size_t end = (counted ? min((size_t)*counted, (size_t)M) * N : n) >> twice;
+    const size_t end = (counted ? min((size_t)*counted, (size_t)M) * N : n) >> TWICE;
     if (i >= end) return;
     const float alpha = factor ? *factor : 1.0f;
     const bool whole = N % 4 == 0;   // four elements of one row, each of the arrays on 16 bytes
-    uint32_t row = (uint32_t)(i / N), c = (uint32_t)(i - (size_t)row * N);
     float v[4] = {};
-    const uint32_t arrays = splits + (accum && accum_read);
-    if (whole && twice) {
-        const size_t at = i + (size_t)row * N;   // rows 2 row and 2 row + 1
+    if (whole) {
+        const size_t at = TWICE ? i + i / N * N : i;   // TWICE: rows 2 m and 2 m + 1
 #pragma unroll 8
-        for (uint32_t k = 0; k < arrays; ++k) {
+        for (uint32_t k = 0; k < splits + (accum && accum_read); ++k) {
             const float* from = (k < splits ? partial + k * n : accum) + at;
-            const float4 t = *reinterpret_cast<const float4*>(from), u = *reinterpret_cast<const float4*>(from + N);
-            v[0] += t.x + u.x; v[1] += t.y + u.y; v[2] += t.z + u.z; v[3] += t.w + u.w;
-        }
-    } else if (whole) {
-#pragma unroll 8
-        for (uint32_t k = 0; k < arrays; ++k) {
-            const float4 t = *reinterpret_cast<const float4*>((k < splits ? partial + k * n : accum) + i);
+            float4 t = *reinterpret_cast<const float4*>(from);
+            if (TWICE) {
+                const float4 u = *reinterpret_cast<const float4*>(from + N);
+                t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
+            }
             v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
         }
     } else {
-        for (uint32_t k = 0; k < arrays; ++k)
+        for (uint32_t k = 0; k < splits + (accum && accum_read); ++k)
             for (int e = 0; e < 4; ++e)
-                for (uint32_t t = 0; t <= twice && i + e < end; ++t)
-                    v[e] += (k < splits ? partial + k * n : accum)[i + e + ((i + e) / N * twice + t) * N];
+                for (uint32_t t = 0; t <= TWICE && i + e < end; ++t)
+                    v[e] += (k < splits ? partial + k * n : accum)[i + e + (TWICE ? ((i + e) / N + t) * N : 0)];
     }
+    uint32_t row = (uint32_t)(i / N), c = (uint32_t)(i - (size_t)row * N);
     for (int e = 0; e < 4; ++e) {
         if (i + e >= end) break;
-        if (out) out[(size_t)(out_rows ? out_rows[row << twice] : (int32_t)row) * N + c] = tape::from_float<T>(v[e] * alpha);
+        if (out) out[(size_t)(out_rows ? out_rows[row << TWICE] : (int32_t)row) * N + c] = tape::from_float<T>(v[e] * alpha);
         else accum[i + e] = v[e];
         if (++c == N) { c = 0; ++row; }
     }
@@ -198,7 +195,7 @@ struct Output {
     bool count_k;
     const int32_t* rows;       // where its rows go
     bool beside;               // pair_gemm.cuh
-    bool twice;                // combine_kernel, where `out` is written
+    bool twice;                // combine_kernel's TWICE, where `out` is written
 };
 // A product, alpha * (a . b + accum) ...
 void product(const Stream& s, const char* what, const Operand& a, const Operand& b, bool bf16, size_t M, size_t N, size_t K, const Cut& cut,
@@ -228,11 +225,12 @@ void combine(const Stream& s, bool bf16, size_t M, size_t N, const Cut& cut, con
     const unsigned grid = (unsigned)ceil_div(M * N, 4 * THREADS);
     const auto launch = [&](auto kernel, auto* out) {
         s.chain("combine", kernel, grid, THREADS, 0, static_cast<const float*>(o.partial), cut.splits, (uint32_t)M, (uint32_t)N, o.factor, o.accum,
-                (uint32_t)o.accum_read, out, o.count_k ? nullptr : o.counted, o.rows, (uint32_t)(o.twice && o.out));
+                (uint32_t)o.accum_read, out, o.count_k ? nullptr : o.counted, o.rows);
     };
-    if (o.f32) launch(combine_kernel<float>, static_cast<float*>(o.out));
-    else if (bf16) launch(combine_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(o.out));
-    else launch(combine_kernel<__half>, static_cast<__half*>(o.out));
+    const bool twice = o.twice && o.out;
+    if (o.f32) launch(combine_kernel<float, false>, static_cast<float*>(o.out));
+    else if (bf16) launch(twice ? combine_kernel<__nv_bfloat16, true> : combine_kernel<__nv_bfloat16, false>, static_cast<__nv_bfloat16*>(o.out));
+    else launch(twice ? combine_kernel<__half, true> : combine_kernel<__half, false>, static_cast<__half*>(o.out));
 }
 
 // ------------------------------------------------------------------------------------------------ operands of the head
@@ -1240,8 +1238,8 @@ void tape_weight_grad(const Stream& s, int dtype, const uint8_t* codes, const ui
     const uint32_t pairs = (uint32_t)std::min<size_t>(pairs_of(s.rt), ceil_div(out, 256) * ceil_div(in, 256) * p.cut.splits);
     launch<pg::SUM, 1>(s, "tape_weight_grad", a, b, bf16, q, pairs, &in_parts);
     if (p.cut.splits > 1)
-        s.chain("combine", combine_kernel<float>, (unsigned)ceil_div(out * in, 4 * THREADS), THREADS, 0, static_cast<const float*>(q.partial), p.cut.splits,
-                (uint32_t)out, (uint32_t)in, nullptr, nullptr, 0u, g, nullptr, nullptr, 0u);
+        s.chain("combine", combine_kernel<float, false>, (unsigned)ceil_div(out * in, 4 * THREADS), THREADS, 0, static_cast<const float*>(q.partial), p.cut.splits,
+                (uint32_t)out, (uint32_t)in, nullptr, nullptr, 0u, g, nullptr, nullptr);
 }
 
 }  // namespace dev
