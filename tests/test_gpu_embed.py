@@ -304,3 +304,16 @@ def test_the_library_refuses(cuda_rt):
                                    (4, 16, 16, cuda.OK)):
         assert lib.ullis_cuda_top_logits(h, stream, 0, t.data_ptr(), stride, 8, vocab, k, ids.data_ptr(), top.data_ptr()) == code
     assert lib.ullis_cuda_top_logits(h, stream, 0, t.data_ptr(), 16, 8, 16, 4, None, top.data_ptr()) == cuda.ERR_ARG
+
+
+@pytest.mark.parametrize("shape", [(), (1,), (1, 1)])
+def test_a_single_token(cuda_rt, shape):
+    """A token of no dimensions has a row of one, and its gradient is taken as it comes."""
+    table = torch.randn(9, 40, device="cuda")
+    tokens = torch.full(shape, 4, dtype=torch.int32, device="cuda")
+    y = cuda_rt.embed(table, tokens)
+    assert y.shape == (*shape, 40) and torch.equal(y.reshape(40), table[4])
+    g = cuda_rt.embed_grad(tokens, y, 9, scale=2.0)
+    assert torch.equal(g[4], 2.0 * table[4]) and not g[:4].any() and not g[5:].any()
+    with pytest.raises(cuda.UllisCudaError):
+        cuda_rt.embed_grad(tokens, y.reshape(2, 20), 9)

@@ -293,8 +293,10 @@ class DeviceOps:
         """Gradient of `embed`'s table, float32 [vocab, channels]: scale * the sum of gy [*tokens.shape, channels] (float32, float16,
         bfloat16) over the rows of each token.  `ignore_id` and ids outside the table add nothing."""
         torch = _torch()
-        rows, channels, stride = self._matrix(gy, "gy", _DTYPES)
         self._ids(tokens, "tokens")
+        if tokens.dim() == 0 and isinstance(gy, torch.Tensor) and gy.dim() == 1:
+            gy = gy[None]                  # of a token without dimensions, whose row `embed` gives without them too
+        rows, channels, stride = self._matrix(gy, "gy", _DTYPES)
         if tokens.numel() != rows:
             _shape_error("tokens", tokens.shape, gy.shape[:-1])
         vocab, ignore = int(vocab), _id32(ignore_id)
