@@ -4,9 +4,10 @@
 //
 // Both read and write what they name once: the lookup is bound by memory, the gradient of many rows by memory and the steps of its sort.
 // The gradient's sums have a fixed order, with no atomics: the rows of a token in rising order, in pieces where there are many.
-// Lookup of 16384 x 512 from FP16 into f32 8.6 us (42 MB, 4.9 TB/s).  Gradient, in a graph: 512 x 256 into 8192 rows 8.5 us, 16384 x 512 f32 27
-// (sort 15, sums 8, parts 7 with their launches; 50 MB), 76550 x 500 bf16 into 50021 rows 66 (sort 14, searches 17, sums 27, parts 9;
-// 177 MB), 131072 x 512 bf16 73.
+// In a graph, us: lookup of 16384 x 512 from FP16 into f32 9.5 where the outputs leave L2 (42 MB, 4.4 TB/s; call by call 8.5, the host's, as
+// a lookup of 512 x 256 whose kernel takes 2), of 131072 rows 56 (277 MB, 4.9 TB/s).  Gradient of 512 x 256 into 8192 rows 7 to 8.5,
+// 16384 x 512 f32 27 (sort 15, sums 8, parts 7 with their launches; 50 MB), 76550 x 500 bf16 into 50021 rows 66 (sort 14, searches 17,
+// sums 27, parts 9; 177 MB), 131072 x 512 bf16 73.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -142,6 +143,9 @@ __device__ __forceinline__ uint32_t below(const uint32_t* list, uint32_t n, uint
 // different SMs: it writes zeros, lists the rows whose token is one of them, sorts
 // the list (a handful: a rank per entry by comparison with all others), and sums run by run with all of its threads: a group of
 // threads per row of gy, the groups' sums added in their order.
+// us in a graph, into 8192 rows of 256 FP16 channels, so / by the sort below: 512 rows 7.0 / 10.9, 1024 8.8 / 11.6, 1536 10.8 / 12.5, 2048
+// 13.0 / 12.7.  Where one token has all rows one CTA ranks and sums them: 256 rows 11 / 11, 512 23 / 13, 1024 62 / 15 (512 f32 channels
+// 115 / 16).
 constexpr uint32_t FEW = 1024;
 
 template <typename T, int N>
@@ -246,7 +250,8 @@ embed_grad_few_kernel(const uint32_t* __restrict__ tokens, uint32_t ignore_id, c
 // Tokens are sorted by chunks, each by a cluster; with more chunks than one an element's place among all is its place in its chunk and
 // what searches in the others give.  Beside the last of these launches other CTAs write the table's zeros, which costs little there
 // (zeros for the rows alone that no chunk has, found by the same searches: 76550 x 500 into 50021 rows 108 us instead of 82).  Then warps
-// sum runs of rows in that order, a fixed number of places each whatever the tokens are: a run that ends in another warp's places leaves a part of its sum, and a last launch adds those.
+// sum runs of rows in that order, a fixed number of places each whatever the tokens are: a run that ends in another warp's places leaves a
+// part of its sum, and a last launch adds those.
 constexpr uint32_t SORT_EACH = 8, SORT_THREADS = 256, SORT_CTA = SORT_EACH * SORT_THREADS;   // keys to a thread, of a CTA
 constexpr uint32_t MOST_CTAS = 8;   // of a cluster
 constexpr uint32_t WINDOW = 8;      // of sorted tokens, the last of which are kept apart
@@ -406,9 +411,9 @@ struct GradSums {
     float scale;
     float *g, *head, *tail;        // parts of sums that began before a warp's places, and that go on behind them: [warp][C]
 };
-// A warp has `places` (a power of two, at most 32) places of the sorted order and 256 channels, a lane BLOCKS times N of them.  Bound by memory's
-// latency and by instructions (45 to a row): rows are read without tests, the runs' ends are bits of a word, eight rows are on their way at once
-// (16384 x 512 f32 8 us, 76550 x 500 bf16 27).
+// A warp has `places` (a power of two, at most 32) places of the sorted order and 256 channels, a lane BLOCKS times N of them.  Bound by
+// memory's latency and by instructions (45 to a row): rows are read without tests, the runs' ends are bits of a word, eight rows are on
+// their way at once (16384 x 512 f32 8 us, 76550 x 500 bf16 27).
 template <typename T, int N, int BLOCKS, bool WIDE>
 __global__ void __launch_bounds__(THREADS)
 embed_sums_kernel(const GradSums o) {

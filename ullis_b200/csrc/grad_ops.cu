@@ -545,7 +545,8 @@ head_rows_kernel(const HeadRows o) {
     o.row_loss[o.list[row]] = loss;
 }
 
-// The columns' sums of a piece out of their parts, and of `stretches` that the entries add, times loss_scale.  32 columns to a CTA, a warp to each of a slot's eight parts.
+// The columns' sums of a piece out of their parts, and of `stretches` that the entries add, times loss_scale.  32 columns to a CTA, a warp
+// to each of a slot's eight parts.
 __global__ void __launch_bounds__(256)
 head_columns_kernel(const float* __restrict__ part, uint32_t pitch, const uint32_t* __restrict__ counted, uint32_t n_tiles, uint32_t pairs,
                     uint32_t columns, float loss_scale, const float* __restrict__ more, size_t more_pitch, uint32_t stretches,
@@ -678,7 +679,9 @@ bool head_copies_weight(const void* dense, size_t channels) { return !dense || c
 // A distilled row's gradient is a handful of terms, whose roundings to 16 bits do not average out over few rows.  Up to 128 rows, which
 // with two places each are one tile of the products all the same, g * scale goes in as the sum of two 16-bit numbers (pair_gemm.cuh, TWICE):
 // its rounding is then far below that of what leaves.  (32 x 256 x 8192, FP16, 16 entries: g_hidden off by 2.1e-4 in norm instead of 3.2e-4;
-// 57 us so 60.)
+// 57 us so 60.)  From 129 rows on g * scale is rounded once, as head_ce_grad's: gradients are off by 3.0e-4 in norm in FP16 and 2.4e-3 in
+// bf16, of which the rounding of what leaves is 2.1e-4 and 1.7e-3.  Two places would cost 5 % of a call of 192 rows, 12 to 25 % of one of
+// 512; in large calls every product has twice the rows.
 constexpr size_t RESIDUAL_ROWS = 128;
 size_t head_distill_grad_workspace(const ullis_cuda_runtime* rt, size_t rows, size_t channels, size_t vocab, size_t top, bool labels,
                                    bool copies_weight) {

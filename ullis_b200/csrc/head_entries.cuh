@@ -14,9 +14,10 @@
 //
 // The rows that count are taken 32 at a time, and their entries sorted by groups of 64 columns and within them by entry_bits: what an
 // epilogue warp has of a tile then lies in a row, and entries of one column beside one another.  Sums go by that order: a call gives the
-// same result every time.  What this costs beside the products, us with 64 entries in each of 16384 rows: states 7, lists 39,
-// entries_rows 22, entries_columns 24 (some of it behind GRAD), and 15 more in GRAD, whose pairs with the first columns have hundreds of entries
-// to a tile (a teacher's favourites).  All four kernels are bound by instructions (40 to 70 % of the slots) and the latency between them.
+// same result every time.  What this costs, us with 64 entries in each of 16384 rows: states 7, lists 39, entries_rows 22 and
+// entries_columns 24 warm and one after the other, 80 of a call, where entries_columns begins behind GRAD; and 15 more in GRAD, whose
+// pairs with the first columns have hundreds of entries to a tile (a teacher's favourites).  All four kernels are bound by instructions
+// (40 to 70 % of the slots) and the latency between them.
 #pragma once
 #include "block_sort.cuh"
 #include "pair_gemm.cuh"
@@ -240,7 +241,7 @@ entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const i
 // target g less the probability that GRAD has there, and the same of the product.  Where a student is sure of its target, its g is the
 // small difference of what it and the teacher leave to other columns, which a sum with a probability of 1 in it would lose: from 63 / 64 of
 // the softmaxes' share on GRAD leaves it out of its sums (sixteen rows and a group of columns at a time), and the entry adds its whole g.
-// (16384 x 512 x 8192, 64 entries: GRAD 157 us, with half of the rows sure 171; with every target left out 180 to 196 in four forms.)
+// (16384 x 512 x 8192, 64 entries: GRAD 155 us, with half of the rows sure 172; with every target left out 179 to 205 in five forms.)
 struct EntryRows {
     Teacher teacher;
     EntryLists lists;

@@ -31,8 +31,8 @@
 // time.  The products of such a call take the pipe 113 thousand cycles, a loop without an epilogue 148 (the same without the loads of
 // A: neither L2 nor the ring bounds it), LSE 177, GRAD 211: there it is the exp and the sums of the 16 epilogue warps, 36 and 45 %
 // of the issue slots; a STORE has 64 tiles for 74 pairs.
-// With entries (64 to a row) LSE takes 115 and GRAD 136 us at one temperature, 117 and 151 at two of which the second is 2; spread evenly over the
-// columns the entries cost GRAD nothing.
+// With entries (64 to a row) LSE takes 115 and GRAD 136 us at one temperature, 117 and 155 at two of which the second is 2 (172 where half
+// of the rows are sure of their targets); spread evenly over the columns the entries cost GRAD nothing.
 // Every wait is bounded and reports through the status words, as in tc_gemm_ws2.cuh.
 #pragma once
 #include <cuda_bf16.h>
@@ -54,10 +54,10 @@ __host__ __device__ constexpr int kind_of(int epi) { return epi >= LSE_ENTRIES ?
 __host__ __device__ constexpr bool has_entries(int epi) { return epi >= LSE_ENTRIES; }
 __host__ __device__ constexpr bool has_two(int epi) { return epi - (is_twice(epi) ? TWICE : 0) >= LSE_ENTRIES_2; }
 // .._SQUARE, .._FOURTH: .._ENTRIES_2 at a second temperature of 2 or 4.  The exp of the first softmax is the second's squared once or twice:
-// half the exps.  16384 x 512 x 8192 in FP16: LSE 134 us so 117, GRAD 167 so 151.
+// half the exps.  16384 x 512 x 8192 in FP16: LSE 134 us so 117, GRAD 167 so 151 (before it left sure targets out).
 __host__ __device__ constexpr int squarings(int epi) { return has_two(epi) ? (epi - (is_twice(epi) ? TWICE : 0) - LSE_ENTRIES_2) / 2 : 0; }
 // + TWICE: rows 2 m and 2 m + 1 are the same; the second has what rounding to 16 bits takes from the first's g, and is in no sum over the
-// columns.  (A form of its own: a branch in the others cost their loop registers, 157 us so 171.)
+// columns.  (A form of its own: a branch in the others cost their loop registers, 155 us so 170.)
 
 constexpr uint32_t BM = 256, BN = 256, BK = 64;         // of a pair, per accumulator
 constexpr uint32_t OPERAND_BYTES = 128 * BK * 2;        // one CTA's 128 rows of A, or of one accumulator's B

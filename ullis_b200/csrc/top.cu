@@ -10,8 +10,10 @@
 // of the bounds that each finds for its share of the k holds for all of them, and the first goes through what the others have kept.
 //
 // Bound by memory on long rows and by instructions on short ones: 4096 x 131072 bf16, k = 64 195 us (1.07 GB, 5.5 TB/s); 16384 x 8192 f32 132 us
-// (537 MB, 4.1 TB/s; some 5000 warp instructions to a row, a fifth of them for reading it by count, the others for what is kept).  Tried and slower there: tiles of 2 or 8 chunks (155, 127 but 220 on the long rows), a sample of 8 or 32 (139), a buffer of
-// 384 keys (149), the next tiles prefetched into L2 (127, long rows 214).  k = 128 and 256 keep two and four times as much: 250, 476 us.
+// (537 MB, 4.1 TB/s; some 5000 warp instructions to a row, a fifth of them for reading it by count, the others for what is kept).
+// Tried and slower there: tiles of 2 or 8 chunks (155, 127 but 220 on the long rows), a sample of 8 or 32 (139), a buffer of 384 keys
+// (149), the next tiles prefetched into L2 (127, long rows 214).  k = 128 and 256 take 250 and 476 us there: they keep two and four times
+// as much, and the bound begins at the k-th of 512 chunk maxima whatever k is.
 #include <algorithm>
 
 #include "block_sort.cuh"
@@ -346,7 +348,7 @@ void top_logits(const Stream& s, int dtype, Rows logits, size_t rows, size_t voc
     o.k = (uint32_t)k;
     o.ids = ids;
     o.out = out;
-    // Warps enough for every SM, of four tiles each at least.  us with up to 8 / 16: 1 x 131072 f32, k = 64 28.6 / 22.0, k = 256 51 / 38;
+    // Warps enough for every SM, of two tiles each at least.  us with up to 8 / 16: 1 x 131072 f32, k = 64 28.6 / 22.0, k = 256 51 / 38;
     // 32 x 131072 bf16 32 / 26.
     const size_t tiles = ceil_div(vocab * size_of(dtype), TILE * 32 * 16);
     o.warps = 1;
