@@ -240,8 +240,9 @@ entries_list_kernel(const Teacher t, const int32_t* __restrict__ target, const i
 // 16-bit g * scale * 2^k that GRAD puts in its place, and what it adds to GRAD's sums over its column: -w and -w * product, and at the
 // target g less the probability that GRAD has there, and the same of the product.  Where a student is sure of its target, its g is the
 // small difference of what it and the teacher leave to other columns, which a sum with a probability of 1 in it would lose: from 63 / 64 of
-// the softmaxes' share on GRAD leaves it out of its sums (sixteen rows and a group of columns at a time), and the entry adds its whole g.
-// (16384 x 512 x 8192, 64 entries: GRAD 155 us, with half of the rows sure 172; with every target left out 179 to 205 in five forms.)
+// the softmaxes' share on GRAD leaves it out of its sums (32 rows and a group of columns at a time), and the entry adds its whole g.
+// (16384 x 512 x 8192, 64 entries: GRAD at two temperatures 152 us, with half of the rows sure 163, at one 146 and 150; without any of this
+// 151 and 140.  With every target left out it took 17 to 33 % more, in five forms.)
 struct EntryRows {
     Teacher teacher;
     EntryLists lists;
@@ -438,11 +439,11 @@ entries_rows_kernel(const EntryRows o) {
         const float p_cut = lse.probability(o, cut.y);
         row_target[r] = make_float2(g, g * o.target_acc[row]);
         row_cut[r] = make_float2(p_cut, p_cut * cut.x);
-        row_at[r] = (o.lists.column[i] / GROUP_COLUMNS * 2 + r / 16) | (RowSums::sure(t, p_target, has) ? SURE : 0u);
+        row_at[r] = o.lists.column[i] / GROUP_COLUMNS * 2 | (RowSums::sure(t, p_target, has) ? SURE : 0u);
     }
     __syncthreads();
     const uint32_t n = o.lists.offsets[(size_t)blockIdx.x * o.lists.groups1 + o.lists.groups1 - 1];
-    // the rows whose targets GRAD leaves out: with a sure one of the same sixteen rows and group
+    // the rows whose targets GRAD leaves out: with a sure one in the same group of columns
     const uint32_t row_there = first + lane < rows ? row_at[lane] : 0u, all_sure = __ballot_sync(0xffffffffu, row_there & SURE);
     uint32_t left_out = 0;
     if (all_sure) {

@@ -31,8 +31,8 @@
 // time.  The products of such a call take the pipe 113 thousand cycles, a loop without an epilogue 148 (the same without the loads of
 // A: neither L2 nor the ring bounds it), LSE 177, GRAD 211: there it is the exp and the sums of the 16 epilogue warps, 36 and 45 %
 // of the issue slots; a STORE has 64 tiles for 74 pairs.
-// With entries (64 to a row) LSE takes 115 and GRAD 136 us at one temperature, 117 and 155 at two of which the second is 2 (172 where half
-// of the rows are sure of their targets); spread evenly over the columns the entries cost GRAD nothing.
+// With entries (64 to a row) LSE takes 115 and GRAD 142 us at one temperature, 117 and 152 at two of which the second is 2 (4 and 11 more
+// where half of the rows are sure of their targets); spread evenly over the columns the entries cost GRAD nothing.
 // Every wait is bounded and reports through the status words, as in tc_gemm_ws2.cuh.
 #pragma once
 #include <cuda_bf16.h>
@@ -99,8 +99,8 @@ struct Params {
     const float* target_g;     // GRAD: [M] its probability - 1
     const float* factor;       // GRAD: 2^k ; STORE: alpha
     // .._ENTRIES: entries of block b of 32 rows and group n of 64 columns of the vocabulary: those of its first sixteen rows at
-    // b * block_entries + [offsets[b * groups1 + 2 n], offsets[.. + 1]), the others up to offsets[.. + 2].  GRAD: with OFFSET_SURE among the
-    // first (or second) of these the sums over the columns leave out the targets of these sixteen rows
+    // b * block_entries + [offsets[b * groups1 + 2 n], offsets[.. + 1]), the others up to offsets[.. + 2].  GRAD: with OFFSET_SURE beside the
+    // first of these the sums over the columns leave out the targets of these rows and columns
     const uint16_t* offsets;
     uint32_t groups1, block_entries;
     const uint32_t* entries;   // LSE: entry_bits; GRAD: with the 16-bit g * scale * 2^k above them
@@ -418,7 +418,7 @@ struct Entries {
         }
     }
     __device__ uint32_t at(int i) const { return offsets[i] & (OFFSET_SURE - 1); }
-    __device__ uint32_t sure() const { return offsets[0] >> 15 | offsets[1] >> 14; }   // a bit for sixteen rows
+    __device__ bool sure() const { return offsets[0] & OFFSET_SURE; }
     __device__ const uint32_t* list(const Params& p, uint32_t row) const { return p.entries + (size_t)(row / 32) * p.block_entries + at(0); }
 };
 constexpr int ENTRIES_HELD = 2;   // LSE: words of 32 entries that are fetched before the accumulator is there
@@ -824,6 +824,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 float* to = row_smem + turn * TURN + lane;
                 copy_word(to, p.lse2 + (in ? row : 0), in);
                 if (ENTRIES) {
+                    if (!TWO) copy_word(to + 32, p.target + (in ? row : 0), in);   // (with two they are fetched where they are looked at)
                     if (TWO) copy_word(to + 32, p.second_lse2 + (in ? row : 0), in);
                     return;
                 }
@@ -843,12 +844,11 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
             while (more) {
                 const uint32_t n0 = work.n * BN + group * 64, m0 = work.m * BM + rank * 128 + quarter * 32;
                 const uint32_t* list = nullptr;
-                uint32_t n_half[2] = {0, 0}, sure = 0;
+                uint32_t n_half[2] = {0, 0};
                 if (ENTRIES) {
                     list = entries.list(p, m0);
                     n_half[0] = entries.at(1) - entries.at(0);
                     n_half[1] = entries.at(2) - entries.at(1);
-                    sure = entries.sure();
                 }
                 // ENTRIES: the entries of a half on their way to shared memory, while its logits are worked on
                 const auto bring = [&](int h) {
@@ -870,7 +870,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 const float* rows = row_smem + turn * TURN;
                 turn ^= 1;
                 const uint32_t first = p.n_first + n0;
-                const bool any = ENTRIES ? sure != 0 : __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
+                const bool any = ENTRIES ? entries.sure() : __any_sync(0xffffffffu, m0 + lane < M && reinterpret_cast<const uint32_t*>(rows)[96 + lane] - first < 64u);
                 more = work.next();
                 if (more) {
                     fetch(turn);
@@ -882,7 +882,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                 // 16 rows at a time, one copy of the code for both: with two the registers ran out.  TARGETS: the target of one of the
                 // warp's rows lies in its columns.  Its product and its g are the row's: lse2 is a number of the size of the logits, off
                 // by 2e-6 where those are 36, and a model that is sure leaves a g of that size.
-                // ENTRIES: of sure rows (entries_rows_kernel) it is in the sums over the columns with the entries, and here its exp is 0.
+                // ENTRIES: beside those of sure rows (entries_rows_kernel) it is in the sums over the columns with the entries, and here its exp is 0.
                 const auto half = [&](int h, auto special) {
                     constexpr bool TARGETS = decltype(special)::value;
                     const bool second = is_twice(EPI) && (r0 & 1);   // of a row's two places
@@ -901,8 +901,12 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
                             if (SQUARINGS > 0) lse2 = m0 + row < M ? exp2_fast(lse2 - lse) : 0.0f;
                             l2[i] = two(lse2, lse2);
                         }
-                        if (TARGETS && ENTRIES) at[i] = m0 + row < M && (sure >> h & 1u) ? (uint32_t)p.target[m0 + row] - first - q2 : 0x80000000u;
-                        else if (TARGETS) at[i] = m0 + row < M ? reinterpret_cast<const uint32_t*>(rows)[96 + row] - first - q2 : 0x80000000u;
+                        if (TARGETS && ENTRIES)
+                            at[i] = m0 + row < M && (any || !is_twice(EPI))
+                                        ? (TWO ? (uint32_t)p.target[m0 + row] : reinterpret_cast<const uint32_t*>(rows)[32 + row]) - first - q2
+                                        : 0x80000000u;
+                        else if (TARGETS)
+                            at[i] = m0 + row < M ? reinterpret_cast<const uint32_t*>(rows)[96 + row] - first - q2 : 0x80000000u;
                     }
                     const uint32_t to = blocks_at + h * STAGING_BYTES;
                     if (lane == 0) tma_store_read<1>();   // the store before the last has read this half
